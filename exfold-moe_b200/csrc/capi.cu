@@ -8,9 +8,11 @@
 #include <unordered_map>
 
 #include "exf_common.cuh"
+#include "exf_gated.h"
 #include "exf_kernels.h"
 #include "exf_launch.h"
 #include "exf_moe.h"
+#include "exf_mxfp4.h"
 
 namespace exf {
 
@@ -499,6 +501,103 @@ EXF_API int exf_decode_fused_experts(const void* x, const float* w, const int32_
                  nullptr, nullptr, coeff, loss, out_w, out_ids, nullptr};
   MoeArgs a{x, out_w, out_ids, batch, top_k, w13, w2, experts, hidden, inter, y, status};
   return cuda_status(launch_decode_moe_experts(d, a, workspace, (cudaStream_t)stream), name);
+}
+
+// ---- microscaled 4-bit floating point ----------------------------------------------------------
+EXF_API int exf_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t cols,
+                               int64_t row_stride, uint8_t* codes, uint8_t* scales,
+                               exf_stream_t stream) {
+  const char* name = "exf_mxfp4_quantize";
+  EXF_REQUIRE(good_wdtype(dtype), "%s: dtype must be EXF_F32, EXF_BF16 or EXF_F16", name);
+  EXF_REQUIRE(rows >= 0 && cols >= 0 && cols < ((int64_t)1 << 40) && rows < ((int64_t)1 << 40),
+              "%s: bad shape", name);
+  EXF_REQUIRE(rows <= 1 || row_stride >= cols, "%s: row_stride is below cols", name);
+  if (rows == 0 || cols == 0) return EXF_OK;
+  EXF_REQUIRE(x && codes && scales, "%s: null pointer", name);
+  EXF_REQUIRE(aligned16(codes), "%s: codes must be 16-byte aligned", name);
+  EXF_REQUIRE(reinterpret_cast<uintptr_t>(x) % (dtype == EXF_F32 ? 4 : 2) == 0,
+              "%s: x is not aligned to its elements", name);
+  return cuda_status(
+      launch_mxfp4_quantize(x, dtype, rows, cols, row_stride, codes, scales, (cudaStream_t)stream),
+      name);
+}
+
+EXF_API int exf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows,
+                                 int64_t cols, void* out, int dtype, exf_stream_t stream) {
+  const char* name = "exf_mxfp4_dequantize";
+  EXF_REQUIRE(good_wdtype(dtype), "%s: dtype must be EXF_F32, EXF_BF16 or EXF_F16", name);
+  EXF_REQUIRE(rows >= 0 && cols >= 0 && cols < ((int64_t)1 << 40) && rows < ((int64_t)1 << 40),
+              "%s: bad shape", name);
+  if (rows == 0 || cols == 0) return EXF_OK;
+  EXF_REQUIRE(codes && scales && out, "%s: null pointer", name);
+  EXF_REQUIRE(aligned16(codes), "%s: codes must be 16-byte aligned", name);
+  EXF_REQUIRE(reinterpret_cast<uintptr_t>(out) % (dtype == EXF_F32 ? 4 : 2) == 0,
+              "%s: out is not aligned to its elements", name);
+  return cuda_status(
+      launch_mxfp4_dequantize(codes, scales, rows, cols, out, dtype, (cudaStream_t)stream), name);
+}
+
+// ---- gated feed-forward block --------------------------------------------------------------------
+static int gated_checks(const char* name, int dtype, int64_t tokens, int hidden, int inter,
+                        int activation) {
+  if (dtype != EXF_BF16 && dtype != EXF_F16)
+    return fail(EXF_ERR_UNSUPPORTED, "%s: dtype must be EXF_BF16 or EXF_F16", name);
+  EXF_REQUIRE(activation == EXF_SILU || activation == EXF_GELU_TANH, "%s: unknown activation %d",
+              name, activation);
+  EXF_REQUIRE(tokens >= 0 && hidden >= 1 && inter >= 1, "%s: bad shape", name);
+  if (hidden % 8 != 0 || inter % 8 != 0)
+    return fail(EXF_ERR_UNSUPPORTED, "%s: hidden and intermediate must be multiples of 8", name);
+  if (tokens >= ((int64_t)1 << 30) || hidden >= (1 << 29) || inter >= (1 << 29) ||
+      ((tokens + 127) / 128) * (((int64_t)inter + 31) / 32) >= ((int64_t)1 << 31) ||
+      ((tokens + 127) / 128) * (((int64_t)hidden + 31) / 32) >= ((int64_t)1 << 31) ||
+      (((int64_t)inter + 63) / 64) * (((int64_t)hidden + 31) / 32) >= ((int64_t)1 << 31))
+    return fail(EXF_ERR_UNSUPPORTED, "%s: shape too large", name);
+  return EXF_OK;
+}
+
+EXF_API int exf_gated_mlp(const void* x, const void* w13, int dtype, int64_t tokens, int hidden,
+                          int inter, int activation, void* h, float* pre, int32_t* status,
+                          exf_stream_t stream) {
+  const char* name = "exf_gated_mlp";
+  const int rc = gated_checks(name, dtype, tokens, hidden, inter, activation);
+  if (rc != EXF_OK) return rc;
+  if (tokens == 0) return EXF_OK;
+  EXF_REQUIRE(x && w13 && h, "%s: null pointer", name);
+  EXF_REQUIRE(aligned16(x) && aligned16(w13) && aligned16(h) && aligned16(pre),
+              "%s: tensors must be 16-byte aligned", name);
+  GatedArgs a{x, w13, dtype == EXF_BF16, tokens, hidden, inter, activation, status};
+  return cuda_status(launch_gated_forward(a, h, pre, (cudaStream_t)stream), name);
+}
+
+EXF_API int64_t exf_gated_mlp_backward_workspace_bytes(int64_t tokens, int inter) {
+  if (tokens < 0 || inter < 1) return -1;
+  return tokens * 2 * inter * 2;
+}
+
+EXF_API int exf_gated_mlp_backward(const void* dh, const float* pre, const void* x,
+                                   const void* w13, int dtype, int64_t tokens, int hidden,
+                                   int inter, int activation, void* dx, void* dw13,
+                                   void* workspace, int64_t workspace_bytes, int32_t* status,
+                                   exf_stream_t stream) {
+  const char* name = "exf_gated_mlp_backward";
+  const int rc = gated_checks(name, dtype, tokens, hidden, inter, activation);
+  if (rc != EXF_OK) return rc;
+  if (!dx && !dw13) return EXF_OK;
+  if (tokens == 0) {
+    if (!dw13) return EXF_OK;
+    return cuda_status(
+        cudaMemsetAsync(dw13, 0, (size_t)inter * 2 * hidden * 2, (cudaStream_t)stream), name);
+  }
+  EXF_REQUIRE(dh && pre && workspace && (w13 || !dx) && (x || !dw13), "%s: null pointer", name);
+  EXF_REQUIRE(aligned16(dh) && aligned16(pre) && aligned16(x) && aligned16(w13) &&
+                  aligned16(dx) && aligned16(dw13) && aligned16(workspace),
+              "%s: tensors must be 16-byte aligned", name);
+  const int64_t need = exf_gated_mlp_backward_workspace_bytes(tokens, inter);
+  EXF_REQUIRE(workspace_bytes >= need, "%s: workspace of %lld bytes required", name,
+              (long long)need);
+  GatedArgs a{x, w13, dtype == EXF_BF16, tokens, hidden, inter, activation, status};
+  return cuda_status(
+      launch_gated_backward(a, dh, pre, workspace, dx, dw13, (cudaStream_t)stream), name);
 }
 
 // moe_align without any device allocation: the chunk-count table lives in the library's fixed

@@ -1,0 +1,427 @@
+// The gated feed-forward block h = act(x Wg^T) * (x Wu^T) and its gradients (sm_100a: tcgen05 +
+// TMA), bf16 or fp16 operands, fp32 accumulation.
+//
+//   forward   G = x Wg^T, U = x Wu^T                 one GEMM over W13 = [Wg; Wu]
+//             h = act(G) * U                         its epilogue
+//   backward  dG = dh * U * act'(G), dU = dh * act(G) elementwise, from G and U kept in fp32
+//             dx = [dG dU] W13                       reduction over the 2 * inter columns
+//             dW13 = [dG dU]^T x                     reduction over the tokens
+//   act(g) = g s(c(g)) with the logistic s: c(g) = g (silu) or 2 sqrt(2 / pi) (g + 0.044715 g^3)
+//   (the tanh form of gelu); act'(g) = s + g s (1 - s) c'(g).
+//
+// Every product is D[m][n] = sum_k A[m][k] B[n][k] on tcgen05.mma (M = 128, K = 16), both operands
+// in 128-byte-swizzled shared memory loaded by TMA.  The forward reads both operands along k
+// (K-major tiles).  The gradients need W13, x and [dG dU] along their other axis: those tiles are
+// loaded as they lie in memory, 64 m or n values by 64 k rows, and the MMA reads them MN-major, so
+// nothing is transposed in memory.  Sizes that are no multiple of a tile are filled with zeros by
+// TMA and masked on the store.
+//
+// G and U are kept in fp32 because the gradients already round twice (dG / dU to the operand type
+// for the tensor cores, and the result): rounding G and U too would add as much again.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <mutex>
+
+#include "exf_common.cuh"
+#include "exf_gated.h"
+#include "exf_launch.h"
+#include "exf_tc.cuh"
+
+namespace exf {
+using namespace tc;
+
+constexpr int kGatedThreads = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+constexpr int kGBM = 128;
+constexpr int kGBK = 64;            // 16-bit elements of a 128-byte row
+
+enum GatedKind { kForward = 0, kGradX = 1, kGradW = 2 };
+
+struct GatedGemm {
+  int m, n, k;       // n: inter (forward) or hidden
+  int m_tiles, n_tiles;
+  int kblocks;
+  int activation;
+  void* out;         // [m][n]
+  float* pre;        // forward: [m][2 * n] or null
+  int32_t* status;
+};
+
+// ---- activation -----------------------------------------------------------------------------
+template <int ACT>
+__device__ __forceinline__ float gate_sigmoid(float g) {
+  float c = g;
+  if (ACT == kGeluTanh) c = 1.5957691216057308f * fmaf(0.044715f * g, g * g, g);
+  return __fdividef(1.0f, 1.0f + __expf(-c));  // exp overflows to inf: the quotient is 0
+}
+template <int ACT>
+__device__ __forceinline__ float gate_slope(float g, float s) {
+  float dc = 1.0f;
+  if (ACT == kGeluTanh) {
+    // s (1 - s) is 0 long before |g| = 100, and the clamp keeps 0 * inf away
+    const float b = fminf(fmaxf(g, -100.0f), 100.0f);
+    dc = 1.5957691216057308f * fmaf(0.134145f * b, b, 1.0f);
+    return fmaf(b * s * (1.0f - s), dc, s);
+  }
+  return fmaf(g * s, 1.0f - s, s);
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if (BF16) return pack_bf16(a, b);
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <bool BF16>
+__device__ __forceinline__ void store_16b(void* base, int64_t at, const float* v) {
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at) =
+      make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]),
+                 pack2<BF16>(v[6], v[7]));
+}
+
+// ---- the GEMM ---------------------------------------------------------------------------------
+template <int NT>
+struct GatedCfg {
+  static constexpr int kATile = kGBM * kGBK * 2;
+  static constexpr int kBTile = NT * kGBK * 2;
+  static constexpr int kStage = kATile + kBTile;
+  static constexpr int kStages = (196 * 1024) / kStage;
+  static constexpr int kTmem = 2 * NT;
+};
+template <int NT>
+struct GatedSmem {
+  alignas(1024) uint8_t tiles[GatedCfg<NT>::kStages][GatedCfg<NT>::kStage];
+  alignas(8) uint64_t full[GatedCfg<NT>::kStages];
+  alignas(8) uint64_t empty[GatedCfg<NT>::kStages];
+  alignas(8) uint64_t acc_full[2];
+  alignas(8) uint64_t acc_empty[2];
+  alignas(8) uint64_t drain;
+  uint32_t tmem_base;
+  int failed;
+};
+template <int NT>
+constexpr size_t gated_smem_bytes() { return sizeof(GatedSmem<NT>) + 1024; }
+
+// Shared-memory matrix descriptor of an MN-major tile: 64 mn values (128 bytes, swizzled) a row, 64
+// k rows a box; 8-row groups along k 1024 bytes apart (SBO), boxes along mn 8192 bytes apart (LBO).
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(8192 >> 4) << 16) |
+         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+template <int KIND, int NT, bool BF16>
+__global__ void __launch_bounds__(kGatedThreads, 1)
+    gated_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
+                      const __grid_constant__ CUtensorMap map_b, const GatedGemm p) {
+  using C = GatedCfg<NT>;
+  constexpr bool kAMn = KIND == kGradW, kBMn = KIND != kForward;
+  constexpr uint32_t kIdesc = idesc_f16(kGBM, NT, BF16) | (kAMn ? 1u << 15 : 0u) |
+                              (kBMn ? 1u << 16 : 0u);
+  extern __shared__ uint8_t smem_raw[];
+  GatedSmem<NT>& sm = *reinterpret_cast<GatedSmem<NT>*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm.acc_full[b], 1);
+      mbar_init(&sm.acc_empty[b], 4);
+    }
+    mbar_init(&sm.drain, 1);
+    sm.failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc(&sm.tmem_base, C::kTmem);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  const int ntiles = p.m_tiles * p.n_tiles;
+  const uint32_t tmem = sm.tmem_base;
+  volatile int* failed = &sm.failed;
+
+  if (warp == 0) {
+    // ---- TMA producer
+    if (lane == 0) {
+      uint32_t g = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
+        const int mt = t / p.n_tiles, nt = t - mt * p.n_tiles;
+        for (int kb = 0; kb < p.kblocks; ++kb, ++g) {
+          const int s = g % C::kStages;
+          ok = mbar_wait(&sm.empty[s], ((g / C::kStages) & 1) ^ 1, failed);
+          if (!ok) break;
+          uint8_t* a = sm.tiles[s];
+          uint8_t* b = a + C::kATile;
+          uint64_t* bar = &sm.full[s];
+          mbar_expect_tx(bar, C::kStage);
+          if (kAMn) {
+            tma_load_2d(a, &map_a, bar, mt * kGBM, kb * kGBK);
+            tma_load_2d(a + 8192, &map_a, bar, mt * kGBM + 64, kb * kGBK);
+          } else {
+            tma_load_2d(a, &map_a, bar, kb * kGBK, mt * kGBM);
+          }
+          if (kBMn) {
+#pragma unroll
+            for (int j = 0; j < NT / 64; ++j)
+              tma_load_2d(b + j * 8192, &map_b, bar, nt * NT + 64 * j, kb * kGBK);
+          } else {  // gate rows, then up rows
+            tma_load_2d(b, &map_b, bar, kb * kGBK, nt * (NT / 2));
+            tma_load_2d(b + C::kBTile / 2, &map_b, bar, kb * kGBK, p.n + nt * (NT / 2));
+          }
+        }
+      }
+      for (uint32_t j = g > C::kStages ? g - C::kStages : 0; j < g; ++j)
+        mbar_wait_drain(&sm.full[j % C::kStages], (j / C::kStages) & 1);
+    }
+  } else if (warp == 1) {
+    // ---- MMA issuer: tile i accumulates into TMEM columns [NT (i & 1), +NT)
+    if (lane == 0) {
+      uint32_t g = 0;
+      int i = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++i) {
+        const int b = i & 1;
+        ok = mbar_wait(&sm.acc_empty[b], ((i >> 1) & 1) ^ 1, failed);
+        if (!ok) break;
+        fence_after_sync();
+        const uint32_t acc = tmem + static_cast<uint32_t>(b * NT);
+        for (int kb = 0; kb < p.kblocks; ++kb, ++g) {
+          const int s = g % C::kStages;
+          ok = mbar_wait(&sm.full[s], (g / C::kStages) & 1, failed);
+          if (!ok) break;
+          fence_after_sync();
+          const uint32_t a = smem_addr(sm.tiles[s]);
+          const uint32_t bb = a + C::kATile;
+#pragma unroll
+          for (int k = 0; k < kGBK / 16; ++k)
+            mma_kind_f16(acc, kAMn ? smem_desc_mn(a + k * 2048) : smem_desc(a + k * 32),
+                         kBMn ? smem_desc_mn(bb + k * 2048) : smem_desc(bb + k * 32), kIdesc,
+                         (kb > 0 || k > 0) ? 1u : 0u);
+          mma_commit(&sm.empty[s]);
+        }
+        if (!ok) break;
+        mma_commit(&sm.acc_full[b]);
+      }
+      mma_commit(&sm.drain);
+      mbar_wait_drain(&sm.drain, 0);
+    }
+  } else {
+    // ---- epilogue: one output row per thread
+    const int q = warp & 3;
+    int i = 0;
+    for (int t = blockIdx.x; t < ntiles; t += gridDim.x, ++i) {
+      const int mt = t / p.n_tiles, nt = t - mt * p.n_tiles;
+      const int b = i & 1;
+      const bool ok = mbar_wait(&sm.acc_full[b], (i >> 1) & 1, failed);
+      fence_after_sync();
+      if (!ok || *failed) break;
+      const int row = mt * kGBM + q * 32 + lane;
+      const uint32_t taddr = tmem + static_cast<uint32_t>(b * NT) + ((uint32_t)(q * 32) << 16);
+      if (KIND == kForward) {
+#pragma unroll 1
+        for (int c = 0; c < NT / 2; c += 32) {
+          float gt[32], up[32];
+          __syncwarp();
+          tmem_load32(taddr + c, gt);
+          tmem_load32(taddr + NT / 2 + c, up);
+          const int col = nt * (NT / 2) + c;
+          if (row < p.m) {
+            if (p.pre) {
+              float* pg = p.pre + (int64_t)row * 2 * p.n + col;
+#pragma unroll
+              for (int j = 0; j < 32; j += 4)
+                if (col + j < p.n) {
+                  *reinterpret_cast<float4*>(pg + j) =
+                      make_float4(gt[j], gt[j + 1], gt[j + 2], gt[j + 3]);
+                  *reinterpret_cast<float4*>(pg + p.n + j) =
+                      make_float4(up[j], up[j + 1], up[j + 2], up[j + 3]);
+                }
+            }
+            if (p.activation == kSilu) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) gt[j] = gt[j] * gate_sigmoid<kSilu>(gt[j]) * up[j];
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                gt[j] = gt[j] * gate_sigmoid<kGeluTanh>(gt[j]) * up[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+              if (col + j < p.n) store_16b<BF16>(p.out, (int64_t)row * p.n + col + j, gt + j);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < NT; c += 32) {
+          float v[32];
+          __syncwarp();
+          tmem_load32(taddr + c, v);
+          const int col = nt * NT + c;
+          if (row < p.m) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+              if (col + j < p.n) store_16b<BF16>(p.out, (int64_t)row * p.n + col + j, v + j);
+          }
+        }
+      }
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.acc_empty[b]);
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    fence_after_sync();
+    tmem_free(tmem, C::kTmem);
+  }
+  if (threadIdx.x == 0 && sm.failed && p.status) atomicExch(p.status, 1);
+}
+
+// ---- the elementwise part of backward -----------------------------------------------------------
+// both [tokens][2 * inter] = (dh * U * act'(G), dh * act(G)); 8 columns a thread.
+template <bool BF16, int ACT>
+__global__ void __launch_bounds__(256)
+    gated_slope_kernel(const uint16_t* dh, const float* pre, int64_t tokens, int inter,
+                       uint16_t* both) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int vec = inter / 8;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < tokens * vec;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t t = i / vec;
+    const int c = (int)(i - t * vec) * 8;
+    const float4* gp = reinterpret_cast<const float4*>(pre + t * 2 * inter + c);
+    const float4* up = reinterpret_cast<const float4*>(pre + t * 2 * inter + inter + c);
+    const float4 g0 = gp[0], g1 = gp[1], u0 = up[0], u1 = up[1];
+    const uint4 d = *reinterpret_cast<const uint4*>(dh + t * inter + c);
+    const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+    const float u[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+    const uint32_t dw[4] = {d.x, d.y, d.z, d.w};
+    float dg[8], du[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 e = unpack2<BF16>(dw[j >> 1]);
+      const float dv = (j & 1) ? e.y : e.x;
+      const float s = gate_sigmoid<ACT>(g[j]);
+      dg[j] = dv * u[j] * gate_slope<ACT>(g[j], s);
+      du[j] = dv * (g[j] * s);
+    }
+    store_16b<BF16>(both, t * 2 * inter + c, dg);
+    store_16b<BF16>(both, t * 2 * inter + inter + c, du);
+  }
+}
+
+// ---- host side ---------------------------------------------------------------------------------
+template <int KIND, int NT, bool BF16>
+static cudaError_t launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, GatedGemm p,
+                               cudaStream_t s) {
+  auto* kern = gated_gemm_kernel<KIND, NT, BF16>;
+  static std::mutex mu;
+  static bool done[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!done[dev]) {
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)gated_smem_bytes<NT>());
+      if (e != cudaSuccess) return e;
+      done[dev] = true;
+    }
+  }
+  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+  const int sms = sm_count();
+  const unsigned grid = (unsigned)(sms > 0 && tiles > sms ? sms : tiles);
+  return launch_pdl(kern, grid, kGatedThreads, gated_smem_bytes<NT>(), s, ma, mb, p);
+}
+
+static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+template <int NT, bool BF16>
+static cudaError_t forward_nt(const GatedArgs& a, void* h, float* pre, cudaStream_t s) {
+  constexpr auto dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, a.x, a.tokens, a.hidden, kGBM, dt) ||
+      !make_map(&mb, a.w13, 2 * (int64_t)a.inter, a.hidden, NT / 2, dt))
+    return cudaErrorInvalidValue;
+  GatedGemm p{(int)a.tokens, a.inter, a.hidden, ceil_div(a.tokens, kGBM),
+              ceil_div(a.inter, NT / 2), ceil_div(a.hidden, kGBK), a.activation, h, pre, a.status};
+  return launch_gemm<kForward, NT, BF16>(ma, mb, p, s);
+}
+
+template <bool BF16>
+static cudaError_t forward_t(const GatedArgs& a, void* h, float* pre, cudaStream_t s) {
+  return forward_nt<256, BF16>(a, h, pre, s);
+}
+
+template <int NT, bool BF16>
+static cudaError_t grad_x(const GatedArgs& a, const void* both, void* dx, cudaStream_t s) {
+  constexpr auto dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, both, a.tokens, 2 * (int64_t)a.inter, kGBM, dt) ||
+      !make_map(&mb, a.w13, 2 * (int64_t)a.inter, a.hidden, kGBK, dt))
+    return cudaErrorInvalidValue;
+  GatedGemm p{(int)a.tokens, a.hidden, 2 * a.inter, ceil_div(a.tokens, kGBM),
+              ceil_div(a.hidden, NT), ceil_div(2 * (int64_t)a.inter, kGBK), a.activation, dx,
+              nullptr, a.status};
+  return launch_gemm<kGradX, NT, BF16>(ma, mb, p, s);
+}
+
+template <int NT, bool BF16>
+static cudaError_t grad_w(const GatedArgs& a, const void* both, void* dw13, cudaStream_t s) {
+  constexpr auto dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, both, a.tokens, 2 * (int64_t)a.inter, kGBK, dt) ||
+      !make_map(&mb, a.x, a.tokens, a.hidden, kGBK, dt))
+    return cudaErrorInvalidValue;
+  GatedGemm p{2 * a.inter, a.hidden, (int)a.tokens, ceil_div(2 * (int64_t)a.inter, kGBM),
+              ceil_div(a.hidden, NT), ceil_div(a.tokens, kGBK), a.activation, dw13, nullptr,
+              a.status};
+  return launch_gemm<kGradW, NT, BF16>(ma, mb, p, s);
+}
+
+template <bool BF16>
+static cudaError_t backward_t(const GatedArgs& a, const void* dh, const float* pre, void* both,
+                              void* dx, void* dw13, cudaStream_t s) {
+  const int64_t work = a.tokens * (a.inter / 8);
+  int64_t blocks = (work + 255) / 256;
+  const int lim = 8 * sm_count();
+  if (lim > 0 && blocks > lim) blocks = lim;
+  auto* slope = a.activation == kSilu ? gated_slope_kernel<BF16, kSilu>
+                                      : gated_slope_kernel<BF16, kGeluTanh>;
+  cudaError_t e = launch_pdl(slope, (unsigned)blocks, 256, 0, s, static_cast<const uint16_t*>(dh),
+                             pre, a.tokens, a.inter, static_cast<uint16_t*>(both));
+  if (e == cudaSuccess && dx) e = grad_x<256, BF16>(a, both, dx, s);
+  if (e == cudaSuccess && dw13) e = grad_w<256, BF16>(a, both, dw13, s);
+  return e;
+}
+
+cudaError_t launch_gated_forward(const GatedArgs& a, void* h, float* pre, cudaStream_t s) {
+  return a.bf16 ? forward_t<true>(a, h, pre, s) : forward_t<false>(a, h, pre, s);
+}
+
+cudaError_t launch_gated_backward(const GatedArgs& a, const void* dh, const float* pre,
+                                  void* dboth, void* dx, void* dw13, cudaStream_t s) {
+  return a.bf16 ? backward_t<true>(a, dh, pre, dboth, dx, dw13, s)
+                : backward_t<false>(a, dh, pre, dboth, dx, dw13, s);
+}
+
+}  // namespace exf

@@ -698,25 +698,6 @@ static cudaError_t allow_gemm_smem() {
   return cudaSuccess;
 }
 
-// Launch as a programmatic dependent of the previous kernel in the stream (the kernel calls
-// griddepcontrol.wait before reading anything that kernel wrote).
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_pdl(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem,
-                              cudaStream_t s, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(block);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
-  return e != cudaSuccess ? e : cudaGetLastError();
-}
-
 // One CTA per SM (192 KB of pipeline stages and all 512 TMEM columns), never more than tiles.
 static unsigned persistent_tiles(const ExpertGemmParams& p) {
   const int64_t tiles = (int64_t)p.m_blocks * p.n_tiles;

@@ -19,6 +19,7 @@ EXF_F32, EXF_BF16, EXF_F16 = 0, 1, 2
 EXF_I32, EXF_I64 = 0, 1
 EXF_SOFTMAX, EXF_SIGMOID, EXF_SQRTSOFTPLUS = 0, 1, 2
 EXF_QWEN3, EXF_DSV4 = 0, 1
+EXF_SILU, EXF_GELU_TANH = 0, 1
 
 _vp, _i, _i64, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 
@@ -62,6 +63,12 @@ SIGNATURES = {
     "exf_decode_fused_experts_workspace_bytes": (_i64, [_i64, _i, _i, _i, _i]),
     "exf_decode_fused_experts": (_i, [_vp, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp,
                                       _i, _i, _vp, _vp, _vp, _vp, _i64, _vp, _vp]),
+    "exf_mxfp4_quantize": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "exf_mxfp4_dequantize": (_i, [_vp, _vp, _i64, _i64, _vp, _i, _vp]),
+    "exf_gated_mlp": (_i, [_vp, _vp, _i, _i64, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "exf_gated_mlp_backward_workspace_bytes": (_i64, [_i64, _i]),
+    "exf_gated_mlp_backward": (_i, [_vp, _vp, _vp, _vp, _i, _i64, _i, _i, _i, _vp, _vp, _vp, _i64,
+                                    _vp, _vp]),
 }
 
 _lock = threading.Lock()

@@ -17,6 +17,7 @@ from . import _lib as L
 _WDT = {torch.float32: L.EXF_F32, torch.bfloat16: L.EXF_BF16, torch.float16: L.EXF_F16}
 _IDT = {torch.int32: L.EXF_I32, torch.int64: L.EXF_I64}
 _SCORING = {"softmax": L.EXF_SOFTMAX, "sigmoid": L.EXF_SIGMOID, "sqrtsoftplus": L.EXF_SQRTSOFTPLUS}
+_ACTIVATION = {"silu": L.EXF_SILU, "gelu_tanh": L.EXF_GELU_TANH}
 _VARIANT = {"qwen3": L.EXF_QWEN3, "dsv4": L.EXF_DSV4}
 
 
@@ -376,3 +377,128 @@ def fused_experts(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor,
                                       y.data_ptr(), ws.data_ptr(), ws_bytes, _ptr(status),
                                       _stream(dev)))
     return y
+
+
+# ---- microscaled 4-bit floating point -----------------------------------------------------------
+def quantize_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """MXFP4 form of x [..., cols] (fp32, bf16 or fp16): codes uint8 [..., 16 * blocks] and scales
+    uint8 [..., blocks], blocks = ceil(cols / 32).
+
+    A block of 32 values along the last dimension shares the power of two 2^(scale - 127), the
+    largest at which its largest magnitude is at least 4; a value is the nearest of +-{0, 0.5, 1,
+    1.5, 2, 3, 4, 6} times it (ties to the even code, saturating at 6), two codes a byte, the even
+    column in the low half.  A block holding an infinity or a NaN reads back as NaN.
+    """
+    dev = _require_cuda(x)
+    if x.dtype not in _WDT:
+        raise TypeError("quantize_mxfp4 needs a float32, bfloat16 or float16 tensor")
+    if x.dim() == 0:
+        raise ValueError("quantize_mxfp4 needs at least one dimension")
+    cols = x.shape[-1]
+    blocks = (cols + 31) // 32
+    # rows at a constant distance are read where they lie
+    if not (x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= cols):
+        x = x.contiguous()
+    stride = x.stride(0) if x.dim() == 2 and x.shape[0] > 1 else cols
+    codes = torch.empty((*x.shape[:-1], 16 * blocks), dtype=torch.uint8, device=dev)
+    scales = torch.empty((*x.shape[:-1], blocks), dtype=torch.uint8, device=dev)
+    if x.numel() > 0:
+        with torch.cuda.device(dev):
+            L.check(L.lib().exf_mxfp4_quantize(x.data_ptr(), _WDT[x.dtype], x.numel() // cols,
+                                               cols, stride, codes.data_ptr(), scales.data_ptr(),
+                                               _stream(dev)))
+    return codes, scales
+
+
+def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, cols: int | None = None,
+                     dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values of quantize_mxfp4's codes and scales as dtype [..., cols] (default: every column
+    of the blocks)."""
+    dev = _require_cuda(codes, scales)
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise TypeError("dequantize_mxfp4 needs uint8 codes and scales")
+    if dtype not in _WDT:
+        raise TypeError("dequantize_mxfp4 gives float32, bfloat16 or float16")
+    if codes.dim() == 0 or codes.shape != (*scales.shape[:-1], 16 * scales.shape[-1]):
+        raise ValueError(f"codes {tuple(codes.shape)} do not match scales {tuple(scales.shape)}: "
+                         "16 bytes a block")
+    blocks = scales.shape[-1]
+    cols = 32 * blocks if cols is None else int(cols)
+    if cols < 0 or (cols + 31) // 32 != blocks:
+        raise ValueError(f"{cols} columns do not take {blocks} blocks of 32")
+    codes, scales = _aligned(codes), scales.contiguous()
+    out = torch.empty((*scales.shape[:-1], cols), dtype=dtype, device=dev)
+    if out.numel() > 0:
+        with torch.cuda.device(dev):
+            L.check(L.lib().exf_mxfp4_dequantize(codes.data_ptr(), scales.data_ptr(),
+                                                 out.numel() // cols, cols, out.data_ptr(),
+                                                 _WDT[dtype], _stream(dev)))
+    return out
+
+
+# ---- gated feed-forward block ---------------------------------------------------------------------
+def _gated_forward(x, w13, activation, status, keep):
+    """(h, pre): pre fp32 [tokens, 2 * inter] for the backward pass if `keep`, else None."""
+    tokens, hidden = x.shape
+    inter = w13.shape[0] // 2
+    h = torch.empty((tokens, inter), dtype=x.dtype, device=x.device)
+    pre = torch.empty((tokens, 2 * inter), dtype=torch.float32, device=x.device) if keep else None
+    with torch.cuda.device(x.device):
+        L.check(L.lib().exf_gated_mlp(x.data_ptr(), w13.data_ptr(), _WDT[x.dtype], tokens, hidden,
+                                      inter, activation, h.data_ptr(), _ptr(pre), _ptr(status),
+                                      _stream(x.device)))
+    return h, pre
+
+
+class _GatedMlp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w13, activation, status):
+        h, pre = _gated_forward(x, w13, activation, status, True)
+        ctx.save_for_backward(x, w13, pre)
+        ctx.activation, ctx.status = activation, status
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        x, w13, pre = ctx.saved_tensors
+        dh = _aligned(dh.to(x.dtype))
+        tokens, hidden = x.shape
+        inter = w13.shape[0] // 2
+        dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
+        dw13 = torch.empty_like(w13) if ctx.needs_input_grad[1] else None
+        ws_bytes = int(L.lib().exf_gated_mlp_backward_workspace_bytes(tokens, inter))
+        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=x.device)
+        with torch.cuda.device(x.device):
+            L.check(L.lib().exf_gated_mlp_backward(
+                dh.data_ptr(), pre.data_ptr(), x.data_ptr(), w13.data_ptr(), _WDT[x.dtype], tokens,
+                hidden, inter, ctx.activation, _ptr(dx), _ptr(dw13), ws.data_ptr(), ws_bytes,
+                _ptr(ctx.status), _stream(x.device)))
+        return dx, dw13, None, None
+
+
+def gated_mlp(x: torch.Tensor, w13: torch.Tensor, activation: str = "silu",
+              status: torch.Tensor | None = None) -> torch.Tensor:
+    """h = act(x Wg^T) * (x Wu^T): both projections, the activation and the product in one launch.
+
+    x [..., H] and w13 [2I, H] (gate rows, then up rows, as an expert of `fused_experts`) bf16 or
+    fp16; h [..., I].  activation "silu" or "gelu_tanh".  H and I are multiples of 8.
+    Differentiable in x and w13 (once): a forward pass that autograd records keeps both
+    projections in fp32 (8 bytes per token and intermediate feature) for the backward pass.
+    `status` (int32 [1] on the device) is set to 1 if a pipeline wait timed out.
+    """
+    _require_cuda(x, w13, status)
+    if x.dtype not in (torch.bfloat16, torch.float16) or w13.dtype != x.dtype:
+        raise TypeError("gated_mlp needs x and w13 both bfloat16 or both float16")
+    if activation not in _ACTIVATION:
+        raise ValueError(f"activation must be one of {sorted(_ACTIVATION)}, got {activation!r}")
+    if x.dim() < 1 or w13.dim() != 2 or w13.shape[0] % 2 or w13.shape[1] != x.shape[-1]:
+        raise ValueError(f"x {tuple(x.shape)} and w13 {tuple(w13.shape)} must be [..., H] and "
+                         "[2I, H]")
+    rows, w = _aligned(x.reshape(-1, x.shape[-1])), _aligned(w13)
+    act = _ACTIVATION[activation]
+    if torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad):
+        h = _GatedMlp.apply(rows, w, act, status)
+    else:
+        h, _ = _gated_forward(rows, w, act, status, False)
+    return h.view(*x.shape[:-1], h.shape[1])

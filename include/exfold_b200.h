@@ -256,6 +256,45 @@ EXF_API int exf_decode_fused_experts(const void* x, const float* w, const int32_
                                      void* y, void* workspace, int64_t workspace_bytes,
                                      int32_t* status, exf_stream_t stream);
 
+/* Microscaled 4-bit floating point (MXFP4: e2m1 values, one E8M0 scale per 32).  These entry points
+ * and the gated feed-forward block below have no counterpart in the reference.
+ *
+ * exf_mxfp4_quantize: x [rows][cols] (dtype EXF_F32, EXF_BF16 or EXF_F16; rows row_stride elements
+ * apart) -> codes [rows][ceil(cols / 32)][16] and scales [rows][ceil(cols / 32)].  A block of 32
+ * consecutive columns with the largest magnitude a has the exponent e = max(floor(log2 a) - 2,
+ * -127) and the scale byte e + 127; a value's code is its sign (bit 3) and the index of the
+ * nearest of {0, 0.5, 1, 1.5, 2, 3, 4, 6} to |x| 2^-e, ties to the even index, saturating at 6;
+ * column 2 i is in the low half of byte i.  A block with an infinity or NaN gets the scale byte
+ * 255 and codes 0.  Columns past the last fill up its block as zeros.
+ * exf_mxfp4_dequantize: the values code * 2^(scale - 127), rounded to dtype, in out [rows][cols]
+ * (scale byte 255: NaN).  codes 16-byte aligned. */
+EXF_API int exf_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t cols,
+                               int64_t row_stride, uint8_t* codes, uint8_t* scales,
+                               exf_stream_t stream);
+EXF_API int exf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows,
+                                 int64_t cols, void* out, int dtype, exf_stream_t stream);
+
+/* Gated feed-forward block (a layer's shared expert, or a dense layer's first half) and its
+ * gradients on the tcgen05 tensor cores: h = act(x Wg^T) * (x Wu^T).
+ * x [tokens][hidden], w13 [2*inter][hidden] (rows [0, inter) gate, rows [inter, 2*inter) up),
+ * h [tokens][inter], all of dtype (EXF_BF16 or EXF_F16), sums in fp32.  pre fp32
+ * [tokens][2*inter] receives x W13^T for the backward pass, or is NULL.
+ * exf_gated_mlp_backward: from dh [tokens][inter] and pre, dx [tokens][hidden] and dw13
+ * [2*inter][hidden] (either may be NULL); the gradients of the two projections are rounded to
+ * dtype before the products.  workspace: exf_gated_mlp_backward_workspace_bytes().  No tokens: dw13
+ * is zeroed.  hidden and inter multiples of 8; every tensor 16-byte aligned.  status as in
+ * exf_fused_experts. */
+enum exf_activation { EXF_SILU = 0, EXF_GELU_TANH = 1 };
+EXF_API int exf_gated_mlp(const void* x, const void* w13, int dtype, int64_t tokens, int hidden,
+                          int inter, int activation, void* h, float* pre, int32_t* status,
+                          exf_stream_t stream);
+EXF_API int64_t exf_gated_mlp_backward_workspace_bytes(int64_t tokens, int inter);
+EXF_API int exf_gated_mlp_backward(const void* dh, const float* pre, const void* x,
+                                   const void* w13, int dtype, int64_t tokens, int hidden,
+                                   int inter, int activation, void* dx, void* dw13,
+                                   void* workspace, int64_t workspace_bytes, int32_t* status,
+                                   exf_stream_t stream);
+
 /* Calibration statistics (offline): the GPU form of PairwiseScalarStats
  * (exfold/qwen3/calibration.py:9-140), which builds the [E][E] coefficient / loss tables and the
  * expert norms that the folds above read.
