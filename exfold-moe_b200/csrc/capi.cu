@@ -13,6 +13,7 @@
 #include "exf_launch.h"
 #include "exf_moe.h"
 #include "exf_mxfp4.h"
+#include "exf_mxmoe.h"
 
 namespace exf {
 
@@ -535,6 +536,49 @@ EXF_API int exf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, in
               "%s: out is not aligned to its elements", name);
   return cuda_status(
       launch_mxfp4_dequantize(codes, scales, rows, cols, out, dtype, (cudaStream_t)stream), name);
+}
+
+EXF_API int64_t exf_fused_experts_mxfp4_workspace_bytes(int64_t tokens, int top_k, int experts,
+                                                        int hidden, int inter) {
+  if (tokens < 0 || top_k < 1 || experts < 1 || hidden < 1 || inter < 1) return -1;
+  return mx_workspace(tokens, top_k, experts, hidden, inter, nullptr).bytes;
+}
+
+EXF_API int exf_fused_experts_mxfp4(const void* x, const float* topk_w, const int32_t* topk_ids,
+                                    int64_t tokens, int top_k, const uint8_t* w13,
+                                    const uint8_t* s13, const uint8_t* w2, const uint8_t* s2,
+                                    int experts, int hidden, int inter, void* y, void* workspace,
+                                    int64_t workspace_bytes, int32_t* status,
+                                    exf_stream_t stream) {
+  const char* name = "exf_fused_experts_mxfp4";
+  EXF_REQUIRE(tokens >= 0 && top_k >= 1 && hidden >= 1 && inter >= 1 && tokens < (1 << 30),
+              "%s: bad shape", name);
+  EXF_REQUIRE(tokens * top_k + (int64_t)experts * 127 < ((int64_t)1 << 30),
+              "%s: bad routing shape (routes plus block padding must stay below 2^30)", name);
+  if (top_k > 8) return fail(EXF_ERR_UNSUPPORTED, "%s: top_k must be at most 8, got %d", name, top_k);
+  if (experts < 1 || experts > align_max_experts())
+    return fail(EXF_ERR_UNSUPPORTED, "%s: experts must be in [1, %d]", name, align_max_experts());
+  if (hidden % 256 != 0 || inter % 128 != 0)
+    return fail(EXF_ERR_UNSUPPORTED,
+                "%s: hidden must be a multiple of 256 and intermediate a multiple of 128", name);
+  if ((int64_t)experts * 2 * inter >= ((int64_t)1 << 31) ||
+      (int64_t)experts * hidden >= ((int64_t)1 << 31))
+    return fail(EXF_ERR_UNSUPPORTED, "%s: shape too large", name);
+  if (tokens == 0) return EXF_OK;
+  EXF_REQUIRE(x && topk_w && topk_ids && w13 && s13 && w2 && s2 && y && workspace,
+              "%s: null pointer", name);
+  EXF_REQUIRE(aligned16(x) && aligned16(y) && aligned16(s13) && aligned16(s2),
+              "%s: tensors must be 16-byte aligned", name);
+  EXF_REQUIRE(reinterpret_cast<uintptr_t>(w13) % 32 == 0 &&
+                  reinterpret_cast<uintptr_t>(w2) % 32 == 0 &&
+                  reinterpret_cast<uintptr_t>(workspace) % 32 == 0,
+              "%s: weight codes and the workspace must be 32-byte aligned", name);
+  const MxWorkspace ws = mx_workspace(tokens, top_k, experts, hidden, inter, workspace);
+  EXF_REQUIRE(workspace_bytes >= ws.bytes, "%s: workspace of %lld bytes required", name,
+              (long long)ws.bytes);
+  MxArgs a{x,       topk_w, topk_ids, tokens, top_k, w13, s13, w2, s2,
+           experts, hidden, inter,    y,      status};
+  return cuda_status(launch_mx_experts(a, ws, (cudaStream_t)stream), name);
 }
 
 // ---- gated feed-forward block --------------------------------------------------------------------

@@ -1,0 +1,73 @@
+// Expert layer with MXFP4 weights: parameter blocks and host entries (internal).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "exf_kernels.h"
+
+namespace exf {
+
+struct MxRoutes {               // moe_align's result
+  const int32_t* num_post_pad;
+  const int32_t* expert_ids;    // [blocks]
+  const int32_t* sorted_ids;    // [capacity]
+};
+
+struct MxLayerParams {
+  MxRoutes routes;
+  int experts;
+  int numel;                    // routes = tokens * top_k
+  int hidden;
+  int inter;
+  int m_blocks;                 // route blocks of the capacity
+  int* status;                  // set to 1 if a pipeline wait timed out (may be null)
+  const uint8_t* s13;           // weight scales in tiles (see MxArgs)
+  const uint8_t* s2;
+  const uint8_t* xs;            // scales of the split token rows
+  uint8_t* hq;                  // GEMM-1 output, two-term form [blocks][2 BT][inter]
+  uint8_t* hs;                  // its scales [blocks][inter / 128][512]
+  const float* route_w;
+  float* out;                   // GEMM-2 output [numel][hidden]
+  int32_t* sync;                // [0] next tile; [1 + b] GEMM-1 epilogue warps done with block b
+};
+
+struct MxArgs {
+  const void* x;                // bf16 [tokens][hidden]
+  const float* topk_w;          // [tokens][top_k]
+  const int32_t* topk_ids;
+  int64_t tokens;
+  int top_k;
+  const uint8_t* w13;           // codes [experts][2 * inter][hidden / 2]
+  const uint8_t* s13;           // scales [experts][2 * inter / 128][hidden / 128][512]
+  const uint8_t* w2;            // codes [experts][hidden][inter / 2]
+  const uint8_t* s2;            // scales [experts][hidden / 128][inter / 128][512]
+  int experts;
+  int hidden;
+  int inter;
+  void* y;                      // bf16 [tokens][hidden]
+  int* status;
+};
+
+struct MxWorkspace {
+  int block;                    // routes of a block
+  int64_t capacity;
+  int32_t* sorted_ids;
+  int32_t* expert_ids;
+  int32_t* num_post_pad;
+  void* align_ws;
+  uint8_t* xq;                  // two-term token rows [blocks][2 * block][hidden]
+  uint8_t* xs;                  // [blocks][hidden / 128][512]
+  uint8_t* hq;
+  uint8_t* hs;
+  float* out;
+  int32_t* sync;
+  int sync_ints;
+  int64_t bytes;
+};
+
+// Carves the workspace at `base` (null: sizes only).
+MxWorkspace mx_workspace(int64_t tokens, int top_k, int experts, int hidden, int inter, void* base);
+cudaError_t launch_mx_experts(const MxArgs& a, const MxWorkspace& w, cudaStream_t s);
+
+}  // namespace exf

@@ -353,15 +353,6 @@ __device__ __forceinline__ LayerTile layer_tile(int t, int blocks, int n1, int n
   return r;
 }
 
-__device__ __forceinline__ int ld_acquire_gpu(const int32_t* p) {
-  int v;
-  asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ void red_release_gpu_add(int32_t* p, int v) {
-  asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
-}
-
 template <int BT>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     expert_layer_t_kernel(const __grid_constant__ CUtensorMap map_w13,

@@ -8,6 +8,7 @@ int64 natively; other dtypes are converted on the way in and back on the way out
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -26,7 +27,16 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 
 def _stream(device: torch.device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    # the raw handle: a torch.cuda.Stream object for it would cost 2 us a call
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(device.index))
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """Makes `device` current for a launch (nothing to do, and nothing spent, where it is)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _require_cuda(*tensors: torch.Tensor | None) -> torch.device:
@@ -56,9 +66,9 @@ def _logits_in(t: torch.Tensor) -> torch.Tensor:
     return _aligned(t)
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
+def _aligned(t: torch.Tensor, to: int = 16) -> torch.Tensor:
     t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t if t.data_ptr() % to == 0 else t.clone()
 
 
 def _weights_in(w: torch.Tensor) -> torch.Tensor:
@@ -403,7 +413,7 @@ def quantize_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     codes = torch.empty((*x.shape[:-1], 16 * blocks), dtype=torch.uint8, device=dev)
     scales = torch.empty((*x.shape[:-1], blocks), dtype=torch.uint8, device=dev)
     if x.numel() > 0:
-        with torch.cuda.device(dev):
+        with _on(dev):
             L.check(L.lib().exf_mxfp4_quantize(x.data_ptr(), _WDT[x.dtype], x.numel() // cols,
                                                cols, stride, codes.data_ptr(), scales.data_ptr(),
                                                _stream(dev)))
@@ -429,11 +439,75 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, cols: int | None
     codes, scales = _aligned(codes), scales.contiguous()
     out = torch.empty((*scales.shape[:-1], cols), dtype=dtype, device=dev)
     if out.numel() > 0:
-        with torch.cuda.device(dev):
+        with _on(dev):
             L.check(L.lib().exf_mxfp4_dequantize(codes.data_ptr(), scales.data_ptr(),
                                                  out.numel() // cols, cols, out.data_ptr(),
                                                  _WDT[dtype], _stream(dev)))
     return out
+
+
+def tile_mxfp4_scales(scales: torch.Tensor) -> torch.Tensor:
+    """The scales [experts, rows, blocks] of expert weights in the layout `fused_experts_mxfp4` reads,
+    [experts, rows / 128, blocks / 4, 512]: tiles of 128 rows x 4 blocks, row r of a tile at byte
+    16 * (r % 32) + 4 * (r // 32).  Done once, when the weights are loaded."""
+    if scales.dtype != torch.uint8:
+        raise TypeError("tile_mxfp4_scales needs uint8 scales")
+    if scales.dim() != 3 or scales.shape[1] % 128 or scales.shape[2] % 4:
+        raise ValueError(f"scales {tuple(scales.shape)} must be [experts, rows, blocks], rows a "
+                         "multiple of 128 and blocks of 4")
+    e, rows, blocks = scales.shape
+    return (scales.reshape(e, rows // 128, 4, 32, blocks // 4, 4).permute(0, 1, 4, 3, 2, 5)
+            .reshape(e, rows // 128, blocks // 4, 512).contiguous())
+
+
+def fused_experts_mxfp4(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor,
+                        w13: torch.Tensor, s13: torch.Tensor, w2: torch.Tensor, s2: torch.Tensor,
+                        status: torch.Tensor | None = None) -> torch.Tensor:
+    """`fused_experts` with MXFP4 weights: y = sum_j topk_w[:, j] * W2[e] (silu(W1[e] x) *
+    (W3[e] x)), e = topk_ids[:, j]; ids outside [0, E) contribute nothing.
+
+    x bf16 [T, H].  w13 uint8 [E, 2I, H / 2] (gate rows then up rows) and w2 uint8 [E, H, I / 2] are
+    `quantize_mxfp4`'s codes, s13 and s2 its scales after `tile_mxfp4_scales`.  Activations keep
+    bf16 precision (two 8-bit terms each); sums are fp32.  H is a multiple of 256, I of 128,
+    top_k <= 8.  `status` as in `fused_experts`.
+    """
+    dev = _require_cuda(x, topk_w, topk_ids, w13, s13, w2, s2, status)
+    if x.dtype != torch.bfloat16:
+        raise TypeError("fused_experts_mxfp4 needs bfloat16 activations")
+    if any(t.dtype != torch.uint8 for t in (w13, s13, w2, s2)):
+        raise TypeError("fused_experts_mxfp4 needs uint8 codes and scales")
+    if x.dim() != 2 or topk_ids.dim() != 2 or w13.dim() != 3:
+        raise ValueError("x must be [T, H], topk_ids [T, top_k] and w13 [E, 2I, H / 2]")
+    tokens, hidden = x.shape
+    experts, two_i, _ = w13.shape
+    inter, top_k = two_i // 2, topk_ids.shape[1]
+    if topk_ids.shape[0] != tokens or topk_w.shape != topk_ids.shape:
+        raise ValueError(f"routes {tuple(topk_w.shape)}, {tuple(topk_ids.shape)} do not match "
+                         f"{tokens} tokens")
+    if two_i % 2 or hidden % 256 or inter % 128:
+        raise NotImplementedError("fused_experts_mxfp4: hidden must be a multiple of 256 and "
+                                  "intermediate a multiple of 128")
+    for t, shape, what in ((w13, (experts, two_i, hidden // 2), "w13"),
+                           (s13, (experts, two_i // 128, hidden // 128, 512), "s13"),
+                           (w2, (experts, hidden, inter // 2), "w2"),
+                           (s2, (experts, hidden // 128, inter // 128, 512), "s2")):
+        if t.shape != shape:
+            raise ValueError(f"{what} {tuple(t.shape)} must be {shape}")
+    x, w13, s13, w2, s2 = (_aligned(t, 32) for t in (x, w13, s13, w2, s2))
+    ids = topk_ids.to(torch.int32).contiguous()
+    wts = topk_w.float().contiguous()
+    y = torch.empty_like(x)
+    if tokens == 0:
+        return y
+    ws_bytes = int(L.lib().exf_fused_experts_mxfp4_workspace_bytes(tokens, top_k, experts, hidden,
+                                                                   inter))
+    ws = torch.empty(max(ws_bytes, 32), dtype=torch.uint8, device=dev)
+    with _on(dev):
+        L.check(L.lib().exf_fused_experts_mxfp4(
+            x.data_ptr(), wts.data_ptr(), ids.data_ptr(), tokens, top_k, w13.data_ptr(),
+            s13.data_ptr(), w2.data_ptr(), s2.data_ptr(), experts, hidden, inter, y.data_ptr(),
+            ws.data_ptr(), ws_bytes, _ptr(status), _stream(dev)))
+    return y
 
 
 # ---- gated feed-forward block ---------------------------------------------------------------------
@@ -443,7 +517,7 @@ def _gated_forward(x, w13, activation, status, keep):
     inter = w13.shape[0] // 2
     h = torch.empty((tokens, inter), dtype=x.dtype, device=x.device)
     pre = torch.empty((tokens, 2 * inter), dtype=torch.float32, device=x.device) if keep else None
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         L.check(L.lib().exf_gated_mlp(x.data_ptr(), w13.data_ptr(), _WDT[x.dtype], tokens, hidden,
                                       inter, activation, h.data_ptr(), _ptr(pre), _ptr(status),
                                       _stream(x.device)))
@@ -469,7 +543,7 @@ class _GatedMlp(torch.autograd.Function):
         dw13 = torch.empty_like(w13) if ctx.needs_input_grad[1] else None
         ws_bytes = int(L.lib().exf_gated_mlp_backward_workspace_bytes(tokens, inter))
         ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=x.device)
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             L.check(L.lib().exf_gated_mlp_backward(
                 dh.data_ptr(), pre.data_ptr(), x.data_ptr(), w13.data_ptr(), _WDT[x.dtype], tokens,
                 hidden, inter, ctx.activation, _ptr(dx), _ptr(dw13), ws.data_ptr(), ws_bytes,
@@ -492,7 +566,8 @@ def gated_mlp(x: torch.Tensor, w13: torch.Tensor, activation: str = "silu",
         raise TypeError("gated_mlp needs x and w13 both bfloat16 or both float16")
     if activation not in _ACTIVATION:
         raise ValueError(f"activation must be one of {sorted(_ACTIVATION)}, got {activation!r}")
-    if x.dim() < 1 or w13.dim() != 2 or w13.shape[0] % 2 or w13.shape[1] != x.shape[-1]:
+    if (x.dim() < 1 or w13.dim() != 2 or w13.shape[0] % 2 or w13.shape[1] != x.shape[-1]
+            or w13.numel() == 0):
         raise ValueError(f"x {tuple(x.shape)} and w13 {tuple(w13.shape)} must be [..., H] and "
                          "[2I, H]")
     rows, w = _aligned(x.reshape(-1, x.shape[-1])), _aligned(w13)

@@ -274,6 +274,27 @@ EXF_API int exf_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t c
 EXF_API int exf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows,
                                  int64_t cols, void* out, int dtype, exf_stream_t stream);
 
+/* exf_fused_experts with MXFP4 weights and bf16 activations: y[t] = sum_j w[t,j] * W2[e]
+ * (silu(W1[e] x[t]) * (W3[e] x[t])), e = ids[t,j].  w13 [experts][2*inter][hidden / 2] and w2
+ * [experts][hidden][inter / 2]: codes as exf_mxfp4_quantize writes them (blocks along hidden and
+ * inter), 32-byte aligned.  s13 [experts][2*inter / 128][hidden / 128][512] and s2
+ * [experts][hidden / 128][inter / 128][512]: their scales in tiles of 128 rows x 4 blocks, the byte
+ * of row r, block b of a tile at 16 * (r % 32) + 4 * (r / 32) + b (laid out once, when the weights
+ * are loaded).  The tensor cores multiply the codes as they are; an activation enters as the sum of
+ * two e4m3 terms, exact for bf16 values above 2^-13 of the largest in their block of 32, else within
+ * 2^-22 of that; the intermediate activation is rounded to within 2^-9 of its value and 2^-22 of
+ * its block's largest.  The sums, over a token's routes too, are fp32.  A token that
+ * holds an infinity or a NaN gives NaN.  workspace: exf_fused_experts_mxfp4_workspace_bytes(),
+ * 32-byte aligned; other arguments and limits as exf_fused_experts. */
+EXF_API int64_t exf_fused_experts_mxfp4_workspace_bytes(int64_t tokens, int top_k, int experts,
+                                                        int hidden, int inter);
+EXF_API int exf_fused_experts_mxfp4(const void* x, const float* topk_w, const int32_t* topk_ids,
+                                    int64_t tokens, int top_k, const uint8_t* w13,
+                                    const uint8_t* s13, const uint8_t* w2, const uint8_t* s2,
+                                    int experts, int hidden, int inter, void* y, void* workspace,
+                                    int64_t workspace_bytes, int32_t* status,
+                                    exf_stream_t stream);
+
 /* Gated feed-forward block (a layer's shared expert, or a dense layer's first half) and its
  * gradients on the tcgen05 tensor cores: h = act(x Wg^T) * (x Wu^T).
  * x [tokens][hidden], w13 [2*inter][hidden] (rows [0, inter) gate, rows [inter, 2*inter) up),
