@@ -28,7 +28,7 @@
 namespace exf {
 using namespace tc;
 
-constexpr int kMxLayerThreads = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+constexpr int kMxLayerThreads = 256;  // warps 0, 6, 7 TMA, warp 1 MMA, warps 2-5 epilogue
 constexpr int kMxK = 128;             // k values of a stage: 4 MMA steps, one scale word
 
 // ---- the two-term form ------------------------------------------------------------------------
@@ -54,10 +54,14 @@ __device__ __forceinline__ void split2(float a, float b, float inv, uint32_t& hi
   lo = __nv_cvt_float2_to_fp8x2(make_float2((v.x - f.x) * 32.0f, (v.y - f.y) * 32.0f),
                                 __NV_SATFINITE, __NV_E4M3);
 }
-// byte of row n, block kb of a [tile][k / 128][512] scale table
-__device__ __forceinline__ int64_t scale_at(int64_t tile, int kblocks, int kb, int n) {
-  return (tile * kblocks + (kb >> 2)) * 512 + (n & 31) * 16 + (n >> 5) * 4 + (kb & 3);
+// Scales of a route block's rows [0, 2 BT): tables [k / 128][512], one per 128 rows.  Byte of row n,
+// scale block kb, in the tables of the route block's first one.
+__device__ __forceinline__ int64_t scale_at(int64_t table, int kblocks, int kb, int n) {
+  return ((table + (n >> 7)) * kblocks + (kb >> 2)) * 512 + (n & 31) * 16 + ((n >> 5) & 3) * 4 +
+         (kb & 3);
 }
+// tables of a route block
+__host__ __device__ constexpr int scale_tables(int bt) { return bt > 64 ? 2 : 1; }
 
 // ---- split: token rows in route order ------------------------------------------------------------
 // For every real slot m (block m / BT, row r = m % BT): rows r and BT + r of the block in xq hold
@@ -101,8 +105,9 @@ __global__ void __launch_bounds__(256) mx_split_kernel(const __nv_bfloat16* x, M
     *reinterpret_cast<uint2*>(q + (int64_t)bt * hidden) =
         make_uint2(lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
     if ((c & 3) == 0) {
-      xs[scale_at(blk, hidden / kMxK, c >> 2, n)] = (uint8_t)sb;
-      xs[scale_at(blk, hidden / kMxK, c >> 2, bt + n)] = (uint8_t)split_lo_byte(sb);
+      const int64_t table = blk * scale_tables(bt);
+      xs[scale_at(table, hidden / kMxK, c >> 2, n)] = (uint8_t)sb;
+      xs[scale_at(table, hidden / kMxK, c >> 2, bt + n)] = (uint8_t)split_lo_byte(sb);
     }
   }
 }
@@ -115,9 +120,14 @@ __global__ void __launch_bounds__(256) mx_split_kernel(const __nv_bfloat16* x, M
 //     (a warp's 32 features are one scale block);
 //   GEMM-2 tile (block, f): rows [256 f, +256) of W2[e], K = I; out[route][256 f + i] = w_route D.
 // One persistent launch: warp 0 takes tiles from a counter (every GEMM-1 tile, then the GEMM-2
-// tiles) and, before the first load of a GEMM-2 tile, waits until the epilogue warps of the block's
-// GEMM-1 tiles have counted themselves off.  A GEMM-1 tile waits only for earlier tiles of its own
-// CTA and was handed out before every GEMM-2 tile, so the wait ends; it is bounded all the same.
+// tiles) and passes them on through a ring.  Three warps load: the first weight tile, the second,
+// and the token tile, each with its scales (one thread issuing every copy of a stage held the
+// weight stream at 4.0 TB/s: a row of packed codes is a 64-byte request; alone, 16-byte padded
+// tiles stream at 5.3 TB/s from one issuing thread and at 6.6 from two).  The warp that loads
+// tokens waits, before the first load of a GEMM-2 tile, until the epilogue warps of the block's
+// GEMM-1 tiles have counted themselves off; the weights of such a tile do not wait.  A GEMM-1 tile
+// waits only for earlier tiles of its own CTA and was handed out before every GEMM-2 tile, so the
+// wait ends; it is bounded all the same.
 template <int BT>
 struct MxCfg {
   static constexpr int kN = 2 * BT;
@@ -125,12 +135,13 @@ struct MxCfg {
   static constexpr int kTTile = kN * kMxK;
   static constexpr int kScales = 3 * 512;                // two weight tiles, one token tile
   static constexpr int kTiles = 2 * kWTile + kTTile;
-  static constexpr int kTxBytes = kWTile + kTTile + kScales;  // weights count packed
+  static constexpr int kWTx = kWTile / 2 + 512;          // a copy of codes counts them packed
+  static constexpr int kTTx = kTTile + 512;
   static constexpr int kStages = (210 * 1024) / (kTiles + kScales);
   static constexpr int kAccCols = 2 * kN;
   static constexpr int kAccs = kAccCols * 2 + 64 <= 512 ? 2 : 1;
   static constexpr int kScaleCol = kAccs * kAccCols;     // 4 sets of 16 columns
-  static constexpr int kTmemCols = kScaleCol + 64 <= 128 ? 128 : kScaleCol + 64 <= 256 ? 256 : 512;
+  static constexpr int kTmemCols = 512;
   static constexpr int kRing = 8;
 };
 template <int BT>
@@ -150,8 +161,7 @@ struct MxSmem {
 };
 template <int BT>
 constexpr size_t mx_smem_bytes() { return sizeof(MxSmem<BT>) + 1024; }
-static_assert(mx_smem_bytes<16>() <= 232448 && mx_smem_bytes<32>() <= 232448 &&
-                  mx_smem_bytes<64>() <= 232448,
+static_assert(mx_smem_bytes<32>() <= 232448 && mx_smem_bytes<64>() <= 232448,
               "expert layer shared memory");
 
 struct MxTile {
@@ -167,6 +177,19 @@ __device__ __forceinline__ MxTile mx_tile(int t, int blocks, int n1, int n2) {
   r.blk = t / n;
   r.ft = t - r.blk * n;
   return r;
+}
+
+// After a time-out (else every load has been consumed): copies still in flight land before shared
+// memory is released.  The other loading warps may never arrive on a stage, so that its barrier
+// does not complete: the wait is bounded.
+template <int STAGES>
+__device__ __forceinline__ void drain_loads(uint64_t* full, uint32_t g) {
+  for (uint32_t j = g > STAGES ? g - STAGES : 0; j < g; ++j) {
+    for (int i = 0; i < 4096; ++i) {
+      if (mbar_try_wait(&full[j % STAGES], (j / STAGES) & 1)) break;
+      __nanosleep(256);
+    }
+  }
 }
 
 template <int BT>
@@ -186,7 +209,7 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.full[s], 3);  // one arrival per loading warp
       mbar_init(&sm.empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -195,7 +218,7 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
     }
     for (int j = 0; j < kRing; ++j) {
       mbar_init(&sm.ring_full[j], 1);
-      mbar_init(&sm.ring_empty[j], 5);  // the MMA thread and the four epilogue warps
+      mbar_init(&sm.ring_empty[j], 7);  // two loading warps, the MMA thread, four epilogue warps
     }
     mbar_init(&sm.drain, 1);
     sm.failed = 0;
@@ -220,66 +243,79 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
     return (e >= 0 && e < p.experts) ? e : -1;
   };
 
-  if (warp == 0) {
-    // ---- scheduler + producer (one thread)
+  uint32_t issued = 0;  // stages this thread has loaded into
+  if (warp == 0 || warp >= 6) {
+    // ---- loads: warp 0 (which also hands out the tiles) and warp 6 a weight tile each, warp 7 the
+    // token tile; one thread each
     if (lane == 0) {
       uint32_t g = 0;
       bool ok = true;
-      int t = atomicAdd(p.sync, 1);
+      int t = warp == 0 ? atomicAdd(p.sync, 1) : 0;
       for (int j = 0; ok; ++j) {
-        const int tile = t < total ? t : -1;
         const int slot = j % kRing;
-        ok = mbar_wait(&sm.ring_empty[slot], ((j / kRing) & 1) ^ 1, failed);
-        if (!ok) break;
-        sm.ring[slot] = tile;
-        mbar_arrive(&sm.ring_full[slot]);
+        int tile;
+        if (warp == 0) {
+          tile = t < total ? t : -1;
+          ok = mbar_wait(&sm.ring_empty[slot], ((j / kRing) & 1) ^ 1, failed);
+          if (!ok) break;
+          sm.ring[slot] = tile;
+          mbar_arrive(&sm.ring_full[slot]);
+          if (tile >= 0) t = atomicAdd(p.sync, 1);  // its latency overlaps this tile's loads
+        } else {
+          ok = mbar_wait(&sm.ring_full[slot], (j / kRing) & 1, failed);
+          if (!ok) break;
+          tile = sm.ring[slot];
+          mbar_arrive(&sm.ring_empty[slot]);
+        }
         if (tile < 0) break;
-        t = atomicAdd(p.sync, 1);
         const MxTile lt = mx_tile(tile, blocks, n1, n2);
         const int expert = expert_of(lt);
         if (expert < 0) continue;
-        if (lt.down) {
-          const int32_t* flag = p.sync + 1 + lt.blk;
-          uint32_t it = 0;
-          while (ld_acquire_gpu(flag) < 4 * n1) {
-            if (*failed || ++it >= kWaitLimit) {
-              *failed = 1;
-              ok = false;
-              break;
-            }
-            __nanosleep(128);
-          }
-          if (!ok) break;
-          asm volatile("fence.proxy.async.global;" ::: "memory");
-        }
         const int kblocks = (lt.down ? p.inter : p.hidden) / kMxK;
-        const CUtensorMap* mw = lt.down ? &map_w2 : &map_w13;
-        const CUtensorMap* mt = lt.down ? &map_hq : &map_xq;
-        // both weight tiles: gate and up rows of W13[e], or 256 rows of W2[e]
-        const int row0 =
-            lt.down ? expert * p.hidden + lt.ft * 256 : expert * 2 * p.inter + lt.ft * 128;
-        const int row1 = lt.down ? row0 + 128 : row0 + p.inter;
-        const uint8_t* ws = lt.down ? p.s2 : p.s13;
-        const uint8_t* ws0 = ws + (int64_t)(row0 / 128) * kblocks * 512;
-        const uint8_t* ws1 = ws + (int64_t)(row1 / 128) * kblocks * 512;
-        const uint8_t* ts = (lt.down ? p.hs : p.xs) + (int64_t)lt.blk * kblocks * 512;
-        for (int kb = 0; kb < kblocks; ++kb, ++g) {
-          const int s = g % kStages;
-          ok = mbar_wait(&sm.empty[s], ((g / kStages) & 1) ^ 1, failed);
-          if (!ok) break;
-          uint8_t* st = sm.tiles[s];
-          uint64_t* bar = &sm.full[s];
-          mbar_expect_tx(bar, C::kTxBytes);
-          tma_load_2d(st, mw, bar, kb * kMxK, row0);
-          tma_load_2d(st + C::kWTile, mw, bar, kb * kMxK, row1);
-          tma_load_2d(st + 2 * C::kWTile, mt, bar, kb * kMxK, lt.blk * C::kN);
-          bulk_load(sm.scales[s], ws0 + kb * 512, 512, bar);
-          bulk_load(sm.scales[s] + 512, ws1 + kb * 512, 512, bar);
-          bulk_load(sm.scales[s] + 1024, ts + kb * 512, 512, bar);
+        if (warp == 7) {
+          if (lt.down) {
+            const int32_t* flag = p.sync + 1 + lt.blk;
+            uint32_t it = 0;
+            while (ld_acquire_gpu(flag) < 4 * n1) {
+              if (*failed || ++it >= kWaitLimit) {
+                *failed = 1;
+                ok = false;
+                break;
+              }
+              __nanosleep(64);
+            }
+            if (!ok) break;
+            asm volatile("fence.proxy.async.global;" ::: "memory");
+          }
+          const CUtensorMap* map = lt.down ? &map_hq : &map_xq;
+          const uint8_t* sc = (lt.down ? p.hs : p.xs) + (int64_t)lt.blk * kblocks * 512;
+          for (int kb = 0; kb < kblocks; ++kb, ++g) {
+            const int s = g % kStages;
+            ok = mbar_wait(&sm.empty[s], ((g / kStages) & 1) ^ 1, failed);
+            if (!ok) break;
+            mbar_expect_tx(&sm.full[s], C::kTTx);
+            tma_load_2d(sm.tiles[s] + 2 * C::kWTile, map, &sm.full[s], kb * kMxK, lt.blk * C::kN);
+            bulk_load(sm.scales[s] + 1024, sc + kb * 512, 512, &sm.full[s]);
+          }
+        } else {
+          // gate (warp 0) and up (warp 6) rows of W13[e], or the halves of 256 rows of W2[e]
+          const int half = warp == 0 ? 0 : 1;
+          const int row = lt.down
+                              ? expert * p.hidden + lt.ft * 256 + half * 128
+                              : expert * 2 * p.inter + lt.ft * 128 + half * p.inter;
+          const CUtensorMap* map = lt.down ? &map_w2 : &map_w13;
+          const uint8_t* sc = (lt.down ? p.s2 : p.s13) + (int64_t)(row / 128) * kblocks * 512;
+          for (int kb = 0; kb < kblocks; ++kb, ++g) {
+            const int s = g % kStages;
+            ok = mbar_wait(&sm.empty[s], ((g / kStages) & 1) ^ 1, failed);
+            if (!ok) break;
+            mbar_expect_tx(&sm.full[s], C::kWTx);
+            tma_load_2d(sm.tiles[s] + half * C::kWTile, map, &sm.full[s], kb * kMxK, row);
+            bulk_load(sm.scales[s] + half * 512, sc + kb * 512, 512, &sm.full[s]);
+          }
         }
       }
-      for (uint32_t j = g > kStages ? g - kStages : 0; j < g; ++j)
-        mbar_wait_drain(&sm.full[j % kStages], (j / kStages) & 1);
+      issued = g;
     }
   } else if (warp == 1) {
     // ---- MMA issuer; scale sets rotate over 4 groups of 16 TMEM columns
@@ -420,7 +456,245 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
     fence_after_sync();
     tmem_free(tmem, C::kTmemCols);
   }
-  if (threadIdx.x == 0 && sm.failed && p.status) atomicExch(p.status, 1);
+  if (sm.failed) {
+    drain_loads<kStages>(sm.full, issued);
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, 1);
+  }
+}
+
+// ---- prefill ------------------------------------------------------------------------------------
+// Experts with many routes: 128 routes on the M side (hi rows, then lo rows of a route block, both
+// added into one accumulator), 256 weight rows on the N side, so that the MMA (128 x 256 x 32, 128
+// cycles) is not held up by its operand reads and the epilogue has a row a thread.
+//   GEMM-1 tile: gate rows [128 f, +128) and up rows of W13[e]; GEMM-2 tile: 256 rows of W2[e].
+// The accumulator takes 256 TMEM columns and the scales 64, which leaves no room for a second one:
+// 8 epilogue warps copy it to registers at once and give it back before they compute, so the
+// tensor cores wait for the copy only.  A persistent launch per GEMM, tiles of one route block side
+// by side (its rows and the expert's weights are reused from L2).
+constexpr int kMxGemmThreads = 384;  // warps 0, 2, 3 TMA, warp 1 MMA, warps 4-11 epilogue
+constexpr int kMxGemmStages = 3;
+struct MxGemmSmem {
+  // a stage: 128 hi rows, 128 lo rows, 256 rows of padded codes
+  alignas(1024) uint8_t tiles[kMxGemmStages][4 * 128 * kMxK];
+  alignas(128) uint8_t scales[kMxGemmStages][4 * 512];
+  alignas(8) uint64_t full[kMxGemmStages];
+  alignas(8) uint64_t empty[kMxGemmStages];
+  alignas(8) uint64_t acc_full;
+  alignas(8) uint64_t acc_empty;
+  alignas(8) uint64_t drain;
+  uint32_t tmem_base;
+  int failed;
+};
+constexpr size_t mx_gemm_smem_bytes() { return sizeof(MxGemmSmem) + 1024; }
+static_assert(mx_gemm_smem_bytes() <= 232448, "prefill expert GEMM shared memory");
+
+template <bool DOWN>
+__global__ void __launch_bounds__(kMxGemmThreads, 1)
+    mx_gemm_kernel(const __grid_constant__ CUtensorMap map_w,
+                   const __grid_constant__ CUtensorMap map_t, const MxLayerParams p) {
+  constexpr int kTile = 128 * kMxK;
+  extern __shared__ uint8_t smem_raw[];
+  MxGemmSmem& sm = *reinterpret_cast<MxGemmSmem*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kMxGemmStages; ++s) {
+      mbar_init(&sm.full[s], 3);
+      mbar_init(&sm.empty[s], 1);
+    }
+    mbar_init(&sm.acc_full, 1);
+    mbar_init(&sm.acc_empty, 8);
+    mbar_init(&sm.drain, 1);
+    sm.failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc(&sm.tmem_base, 512);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  const int post = *p.routes.num_post_pad;
+  const int blocks = (post + 127) / 128 < p.m_blocks ? (post + 127) / 128 : p.m_blocks;
+  const int n_tiles = DOWN ? p.hidden / 256 : p.inter / 128;
+  const int kblocks = (DOWN ? p.inter : p.hidden) / kMxK;
+  const int total = blocks * n_tiles;
+  const uint32_t tmem = sm.tmem_base;
+  volatile int* failed = &sm.failed;
+  auto expert_of = [&](int blk) {
+    const int e = p.routes.expert_ids[blk];
+    return (e >= 0 && e < p.experts) ? e : -1;
+  };
+
+  uint32_t issued = 0;
+  if (warp == 0 || warp == 2 || warp == 3) {
+    // ---- loads: warp 0 the hi and lo rows, warps 2 and 3 a weight tile each
+    if (lane == 0) {
+      uint32_t g = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        const int blk = t / n_tiles, ft = t - blk * n_tiles;
+        const int expert = expert_of(blk);
+        if (expert < 0) continue;
+        const int half = warp - 2;
+        const int row = DOWN ? expert * p.hidden + ft * 256 + half * 128
+                             : expert * 2 * p.inter + ft * 128 + half * p.inter;
+        const uint8_t* sc =
+            warp == 0 ? (DOWN ? p.hs : p.xs) + (int64_t)blk * 2 * kblocks * 512
+                      : (DOWN ? p.s2 : p.s13) + (int64_t)(row / 128) * kblocks * 512;
+        for (int kb = 0; kb < kblocks; ++kb, ++g) {
+          const int s = g % kMxGemmStages;
+          ok = mbar_wait(&sm.empty[s], ((g / kMxGemmStages) & 1) ^ 1, failed);
+          if (!ok) break;
+          uint64_t* bar = &sm.full[s];
+          if (warp == 0) {
+            mbar_expect_tx(bar, 2 * kTile + 1024);
+            tma_load_2d(sm.tiles[s], &map_t, bar, kb * kMxK, blk * 256);
+            bulk_load(sm.scales[s], sc + kb * 512, 512, bar);
+            bulk_load(sm.scales[s] + 512, sc + (kblocks + kb) * 512, 512, bar);
+          } else {
+            mbar_expect_tx(bar, kTile / 2 + 512);
+            tma_load_2d(sm.tiles[s] + (2 + half) * kTile, &map_w, bar, kb * kMxK, row);
+            bulk_load(sm.scales[s] + 1024 + half * 512, sc + kb * 512, 512, bar);
+          }
+        }
+      }
+      issued = g;
+    }
+  } else if (warp == 1) {
+    // ---- MMA issuer
+    if (lane == 0) {
+      uint32_t g = 0;
+      int i = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        if (expert_of(t / n_tiles) < 0) continue;
+        ok = mbar_wait(&sm.acc_empty, (i & 1) ^ 1, failed);
+        if (!ok) break;
+        fence_after_sync();
+        for (int kb = 0; kb < kblocks; ++kb, ++g) {
+          const int s = g % kMxGemmStages;
+          ok = mbar_wait(&sm.full[s], (g / kMxGemmStages) & 1, failed);
+          if (!ok) break;
+          fence_after_sync();
+          const uint32_t a = smem_addr(sm.tiles[s]);
+          const uint32_t b = a + 2 * kTile;
+          const uint32_t sc = smem_addr(sm.scales[s]);
+          const uint32_t sf = tmem + 256 + (g & 3) * 16;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) tmem_copy_scales(sf + 4 * j, sc + 512 * j);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t id = idesc_mx(128, 256, kMxE4M3, kMxE2M1, k);
+            mma_mx(tmem, smem_desc(a + k * 32), smem_desc(b + k * 32), id, sf, sf + 8,
+                   (kb > 0 || k > 0) ? 1u : 0u);
+            mma_mx(tmem, smem_desc(a + kTile + k * 32), smem_desc(b + k * 32), id, sf + 4, sf + 8,
+                   1u);
+          }
+          mma_commit(&sm.empty[s]);
+        }
+        if (!ok) break;
+        mma_commit(&sm.acc_full);
+        ++i;
+      }
+      mma_commit(&sm.drain);
+      mbar_wait_drain(&sm.drain, 0);
+    }
+  } else {
+    // ---- epilogue: warp w has TMEM lanes 32 (w % 4) .. +31 and half the columns; a row a thread
+    const int q = warp & 3;
+    const int hf = (warp - 4) >> 2;
+    int i = 0;
+    for (int t = blockIdx.x; t < total; t += gridDim.x) {
+      const int blk = t / n_tiles, ft = t - blk * n_tiles;
+      if (expert_of(blk) < 0) continue;
+      const int r = q * 32 + lane;
+      const int route = p.routes.sorted_ids[blk * 128 + r];
+      const bool real = route < p.numel;
+      const bool ok = mbar_wait(&sm.acc_full, i & 1, failed);
+      fence_after_sync();
+      if (!__all_sync(0xffffffffu, ok && !*failed)) break;
+      const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
+      // columns [64 hf, +64) and [128 + 64 hf, +64): 64 features' gate and up, or two runs of 64
+      // output columns
+      uint32_t v[8][16];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        tmem_load16(taddr + 64 * hf + 16 * j, v[j]);
+        tmem_load16(taddr + 128 + 64 * hf + 16 * j, v[4 + j]);
+      }
+      tmem_wait();
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.acc_empty);
+      ++i;
+      if (DOWN) {
+        if (real) {
+          const float wr = p.route_w[route];
+          float* o = p.out + (int64_t)route * p.hidden + ft * 256 + 64 * hf;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int c = 0; c < 16; c += 4)
+              *reinterpret_cast<float4*>(o + (j >> 2) * 128 + (j & 3) * 16 + c) = make_float4(
+                  __uint_as_float(v[j][c]) * wr, __uint_as_float(v[j][c + 1]) * wr,
+                  __uint_as_float(v[j][c + 2]) * wr, __uint_as_float(v[j][c + 3]) * wr);
+        }
+      } else if (real) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {  // two scale blocks of 32 features
+          uint32_t top = 0;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const float gt = __uint_as_float(v[2 * b + j][c]);
+              const float h = gt / (1.0f + __expf(-gt)) * __uint_as_float(v[4 + 2 * b + j][c]);
+              v[2 * b + j][c] = __float_as_uint(h);
+              top = max(top, __float_as_uint(h) & 0x7fffffffu);
+            }
+          const uint32_t sb = split_scale(top);
+          const float inv = split_inverse(sb);
+          const int feat = ft * 128 + 64 * hf + 32 * b;
+          uint8_t* hi_row = p.hq + ((int64_t)blk * 256 + r) * p.inter + feat;
+          uint8_t* lo_row = hi_row + (int64_t)128 * p.inter;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t h0, l0, h1, l1;
+              split2(__uint_as_float(v[2 * b + j][4 * c]),
+                     __uint_as_float(v[2 * b + j][4 * c + 1]), inv, h0, l0);
+              split2(__uint_as_float(v[2 * b + j][4 * c + 2]),
+                     __uint_as_float(v[2 * b + j][4 * c + 3]), inv, h1, l1);
+              hi[c] = h0 | h1 << 16;
+              lo[c] = l0 | l1 << 16;
+            }
+            reinterpret_cast<uint4*>(hi_row)[j] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            reinterpret_cast<uint4*>(lo_row)[j] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          }
+          p.hs[scale_at(2 * blk, p.inter / kMxK, feat / 32, r)] = (uint8_t)sb;
+          p.hs[scale_at(2 * blk, p.inter / kMxK, feat / 32, 128 + r)] =
+              (uint8_t)split_lo_byte(sb);
+        }
+      }
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    fence_after_sync();
+    tmem_free(tmem, 512);
+  }
+  if (sm.failed) {
+    drain_loads<kMxGemmStages>(sm.full, issued);
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, 1);
+  }
 }
 
 // ---- combine ---------------------------------------------------------------------------------------
@@ -459,9 +733,11 @@ __global__ void __launch_bounds__(256, 4)
 }
 
 // ---- host side ---------------------------------------------------------------------------------
-// The route block: the smallest of 16, 32 and 64 that holds the average expert's routes.
+// The route block, which also picks the kernels: 32 or 64 routes on the N side (decode) while the
+// average expert's routes fit with room for the fuller ones (an expert's second block reads its
+// weights again), else 128 on the M side (prefill).
 static int mx_block(int64_t numel, int experts) {
-  return numel <= (int64_t)experts * 16 ? 16 : numel <= (int64_t)experts * 32 ? 32 : 64;
+  return numel <= (int64_t)experts * 18 ? 32 : numel <= (int64_t)experts * 44 ? 64 : 128;
 }
 
 static int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
@@ -488,9 +764,10 @@ MxWorkspace mx_workspace(int64_t tokens, int top_k, int experts, int hidden, int
   const int64_t align_bytes = align_workspace_bytes(numel, experts);
   w.align_ws = take(align_bytes > 0 ? align_bytes : 4);
   w.xq = take(2 * cap * hidden);
-  w.xs = take(blocks * (hidden / kMxK) * 512);
+  const int tables = scale_tables(w.block);
+  w.xs = take(blocks * tables * (hidden / kMxK) * 512);
   w.hq = take(2 * cap * inter);
-  w.hs = take(blocks * (inter / kMxK) * 512);
+  w.hs = take(blocks * tables * (inter / kMxK) * 512);
   w.out = reinterpret_cast<float*>(take(numel * hidden * 4));
   w.sync_ints = (int)(1 + blocks);
   w.sync = reinterpret_cast<int32_t*>(take(w.sync_ints * 4));
@@ -498,38 +775,28 @@ MxWorkspace mx_workspace(int64_t tokens, int top_k, int experts, int hidden, int
   return w;
 }
 
-template <int BT>
-static cudaError_t launch_mx_layer(const MxArgs& a, const MxWorkspace& w, cudaStream_t s) {
-  auto* kern = mx_layer_kernel<BT>;
-  static std::mutex mu;
-  static bool done[64] = {};
+// Raises a kernel's shared-memory limit once per device.
+template <typename K>
+static cudaError_t allow_smem(K* kern, size_t bytes, std::mutex& mu, bool (&done)[64]) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (!done[dev]) {
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)mx_smem_bytes<BT>());
-      if (e != cudaSuccess) return e;
-      done[dev] = true;
-    }
-  }
-  const int64_t blocks = w.capacity / BT;
-  CUtensorMap m13, mx, m2, mh;
-  if (!make_map_4bit(&m13, a.w13, (uint64_t)a.experts * 2 * a.inter, a.hidden, 128) ||
-      !make_map_8bit(&mx, w.xq, blocks * 2 * BT, a.hidden, 2 * BT) ||
-      !make_map_4bit(&m2, a.w2, (uint64_t)a.experts * a.hidden, a.inter, 128) ||
-      !make_map_8bit(&mh, w.hq, blocks * 2 * BT, a.inter, 2 * BT))
-    return cudaErrorInvalidValue;
+  std::lock_guard<std::mutex> lock(mu);
+  if (done[dev]) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  done[dev] = e == cudaSuccess;
+  return e;
+}
+
+static MxLayerParams layer_params(const MxArgs& a, const MxWorkspace& w) {
   MxLayerParams p{};
   p.routes = {w.num_post_pad, w.expert_ids, w.sorted_ids};
   p.experts = a.experts;
   p.numel = (int)(a.tokens * a.top_k);
   p.hidden = a.hidden;
   p.inter = a.inter;
-  p.m_blocks = (int)blocks;
+  p.m_blocks = (int)(w.capacity / w.block);
   p.status = a.status;
   p.s13 = a.s13;
   p.s2 = a.s2;
@@ -539,9 +806,45 @@ static cudaError_t launch_mx_layer(const MxArgs& a, const MxWorkspace& w, cudaSt
   p.route_w = a.topk_w;
   p.out = w.out;
   p.sync = w.sync;
+  return p;
+}
+
+template <int BT>
+static cudaError_t launch_mx_layer(const MxArgs& a, const MxWorkspace& w, cudaStream_t s) {
+  auto* kern = mx_layer_kernel<BT>;
+  static std::mutex mu;
+  static bool done[64] = {};
+  const cudaError_t e = allow_smem(kern, mx_smem_bytes<BT>(), mu, done);
+  if (e != cudaSuccess) return e;
+  const int64_t rows = w.capacity / BT * 2 * BT;
+  CUtensorMap m13, mx, m2, mh;
+  if (!make_map_4bit(&m13, a.w13, (uint64_t)a.experts * 2 * a.inter, a.hidden, 128) ||
+      !make_map_8bit(&mx, w.xq, rows, a.hidden, 2 * BT) ||
+      !make_map_4bit(&m2, a.w2, (uint64_t)a.experts * a.hidden, a.inter, 128) ||
+      !make_map_8bit(&mh, w.hq, rows, a.inter, 2 * BT))
+    return cudaErrorInvalidValue;
   const int sms = sm_count();
   return launch_pdl(kern, sms > 0 ? (unsigned)sms : 1u, kMxLayerThreads, mx_smem_bytes<BT>(), s,
-                    m13, mx, m2, mh, p);
+                    m13, mx, m2, mh, layer_params(a, w));
+}
+
+template <bool DOWN>
+static cudaError_t launch_mx_gemm(const MxArgs& a, const MxWorkspace& w, cudaStream_t s) {
+  auto* kern = mx_gemm_kernel<DOWN>;
+  static std::mutex mu;
+  static bool done[64] = {};
+  const cudaError_t e = allow_smem(kern, mx_gemm_smem_bytes(), mu, done);
+  if (e != cudaSuccess) return e;
+  CUtensorMap mw, mt;
+  const int k = DOWN ? a.inter : a.hidden;
+  if (!make_map_4bit(&mw, DOWN ? a.w2 : a.w13,
+                     (uint64_t)a.experts * (DOWN ? a.hidden : 2 * a.inter), k, 128) ||
+      !make_map_8bit(&mt, DOWN ? w.hq : w.xq, 2 * w.capacity, k, 256))
+    return cudaErrorInvalidValue;
+  const int64_t tiles = w.capacity / 128 * (DOWN ? a.hidden / 256 : a.inter / 128);
+  const int sms = sm_count();
+  return launch_pdl(kern, (unsigned)(sms > 0 && tiles > sms ? sms : tiles), kMxGemmThreads,
+                    mx_gemm_smem_bytes(), s, mw, mt, layer_params(a, w));
 }
 
 static unsigned stream_grid(int64_t threads) {
@@ -562,9 +865,12 @@ cudaError_t launch_mx_experts(const MxArgs& a, const MxWorkspace& w, cudaStream_
                  static_cast<const __nv_bfloat16*>(a.x), routes, w.capacity, (int)numel, a.top_k,
                  a.hidden, w.block, w.xq, w.xs, w.sync, w.sync_ints);
   if (e != cudaSuccess) return e;
-  e = w.block == 16   ? launch_mx_layer<16>(a, w, s)
-      : w.block == 32 ? launch_mx_layer<32>(a, w, s)
-                      : launch_mx_layer<64>(a, w, s);
+  if (w.block == 128) {
+    e = launch_mx_gemm<false>(a, w, s);
+    if (e == cudaSuccess) e = launch_mx_gemm<true>(a, w, s);
+  } else {
+    e = w.block == 32 ? launch_mx_layer<32>(a, w, s) : launch_mx_layer<64>(a, w, s);
+  }
   if (e != cudaSuccess) return e;
   return launch_pdl(mx_combine_kernel, stream_grid(a.tokens * (a.hidden / 4)), 256, 0, s,
                     static_cast<const float*>(w.out), a.topk_ids, a.experts, a.tokens, a.top_k,
