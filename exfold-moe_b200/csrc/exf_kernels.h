@@ -110,6 +110,8 @@ struct AlignParams {
   int32_t* num_post_pad;
   int32_t* table;  // [chunks][experts]
   int64_t chunks;
+  int32_t* slots;  // the slot of each route, -1 for one of no expert (more than
+                   // align_gather_max_numel() routes; may be null)
 };
 
 cudaError_t launch_router(int experts, int scoring, int fold, const RouterParams& p, cudaStream_t s);
@@ -151,6 +153,11 @@ cudaError_t launch_align(int id_dtype, const AlignParams& p, cudaStream_t s);
 int64_t align_gather_max_numel();
 cudaError_t launch_align_gather(const AlignParams& p, const void* x, int top_k, int hidden,
                                 void* xs, int32_t* zero, int zero_n, cudaStream_t s);
+// The same with the token rows in the two-term form of the MXFP4 expert layer (exf_mx.cuh): xq and
+// their scales xs; p.block_size is that layer's route block, hidden a multiple of 256.
+cudaError_t launch_align_split(const AlignParams& p, const void* x, int top_k, int hidden,
+                               uint8_t* xq, uint8_t* xs, int32_t* zero, int zero_n,
+                               cudaStream_t s);
 cudaError_t launch_calib_update(int out_dtype, int id_dtype, const void* out, const void* ids,
                                 int64_t tokens, int K, int H, int E, double* dot, double* tsq,
                                 double* ssq, double* nsum, double* ncnt, cudaStream_t s);

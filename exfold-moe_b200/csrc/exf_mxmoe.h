@@ -25,8 +25,8 @@ struct MxLayerParams {
   const uint8_t* s13;           // weight scales in tiles (see MxArgs)
   const uint8_t* s2;
   const uint8_t* xs;            // scales of the split token rows
-  uint8_t* hq;                  // GEMM-1 output, two-term form [blocks][2 BT][inter]
-  uint8_t* hs;                  // its scales [blocks][inter / 128][512]
+  uint8_t* hq;                  // GEMM-1 output in the same form
+  uint8_t* hs;
   const float* route_w;
   float* out;                   // GEMM-2 output [numel][hidden]
   int32_t* sync;                // [0] next tile; [1 + b] GEMM-1 epilogue warps done with block b
@@ -56,8 +56,9 @@ struct MxWorkspace {
   int32_t* expert_ids;
   int32_t* num_post_pad;
   void* align_ws;
-  uint8_t* xq;                  // two-term token rows [blocks][2 * block][hidden]
-  uint8_t* xs;                  // [blocks][hidden / 128][512]
+  int32_t* slots;               // slot of each route (more routes than one align launch takes)
+  uint8_t* xq;                  // two-term token rows [blocks][2 * block][hidden] (exf_mx.cuh)
+  uint8_t* xs;                  // their scales [blocks][tables][hidden / 128][512]
   uint8_t* hq;
   uint8_t* hs;
   float* out;

@@ -11,6 +11,7 @@
 #include "exf_common.cuh"
 #include "exf_kernels.h"
 #include "exf_launch.h"
+#include "exf_mx.cuh"
 
 namespace exf {
 
@@ -70,10 +71,11 @@ __device__ __forceinline__ int scatter_round(int64_t r, int e, int E, AlignSmem&
 // Stable scatter of routes [start, end): base[e] holds the next slot of expert e.
 template <typename IT>
 __device__ void stable_scatter(const IT* ids, int64_t start, int64_t end, int E, AlignSmem& sm,
-                               int32_t* sorted_ids) {
+                               int32_t* sorted_ids, int32_t* slots) {
   for (int64_t s0 = start; s0 < end; s0 += kAlignThreads) {
     const int64_t r = s0 + threadIdx.x;
-    scatter_round(r, expert_of(ids, r, end, E), E, sm, sorted_ids);
+    const int slot = scatter_round(r, expert_of(ids, r, end, E), E, sm, sorted_ids);
+    if (slots && r < end) slots[r] = slot;
   }
 }
 
@@ -179,17 +181,33 @@ __global__ void __launch_bounds__(kAlignThreads, 1) align_small_kernel(const Ali
     if (j < rounds) scatter_round((int64_t)j * kAlignThreads + tid, ex[j], p.experts, sm, p.sorted_ids);
 }
 
+// What the fused kernel below does with the token row of a placed route, 16-byte vector c at a
+// time (the row's vectors on neighbouring lanes): copies it to its slot, or writes its two-term form.
+struct CopyRows {
+  uint4* xs;
+  int row_vecs;
+  __device__ __forceinline__ void operator()(int slot, int c, uint4 v) const {
+    xs[(int64_t)slot * row_vecs + c] = v;
+  }
+};
+struct SplitRows {
+  MxRows rows;
+  __device__ __forceinline__ void operator()(int slot, int c, uint4 v) const {
+    put8(rows, slot, c, split8(v));
+  }
+};
+
 // moe_align fused with the gather of token rows (numel <= kAlignSmall, the expert layer at
 // decode): every CTA counts all routes (they are few; an L2-resident read) and places only its
 // own slice [s0, s0 + slice) of consecutive routes, at the slots the one-CTA kernel gives them
 // (routes of an expert in earlier slices come first, then the slice's own in flat order); then
-// it copies the token row of each route it placed: xs[slot] = x[route / top_k] (16-byte
-// vectors).  Padding, tail and block names are split over the CTAs.  CTA 0 also zeroes
-// zero[0, zero_n) (the expert layer kernel's tile counters).
-template <typename IT>
+// it hands `put` the token row of each route it placed.  Padding, tail and block names are split
+// over the CTAs.  CTA 0 also zeroes zero[0, zero_n) (the expert layer kernel's tile counters).
+// A warp stays in one row: row_vecs is a multiple of 32 where `put` needs its lanes together.
+template <typename IT, typename Put>
 __global__ void __launch_bounds__(kAlignThreads, 1)
     align_gather_kernel(const AlignParams p, const uint4* __restrict__ x, int top_k, int row_vecs,
-                        uint4* __restrict__ xs, int slice, int32_t* zero, int zero_n) {
+                        const Put put, int slice, int32_t* zero, int zero_n) {
   __shared__ AlignSmem sm;
   __shared__ int slot_of[kAlignThreads];
   const IT* ids = static_cast<const IT*>(p.ids);
@@ -226,7 +244,7 @@ __global__ void __launch_bounds__(kAlignThreads, 1)
       const int k = i / row_vecs;
       const int c = i - k * row_vecs;
       const int slot = slot_of[k];
-      if (slot >= 0) xs[(int64_t)slot * row_vecs + c] = x[(r0 + k) / top_k * row_vecs + c];
+      if (slot >= 0) put(slot, c, x[(r0 + k) / top_k * row_vecs + c]);
     }
     __syncthreads();  // slot_of is rewritten by the next round
   }
@@ -302,7 +320,7 @@ __global__ void __launch_bounds__(kAlignThreads, 1) align_scatter_kernel(const A
   __syncthreads();
   const int64_t start = (int64_t)blockIdx.x * kAlignChunk;
   const int64_t end = min(start + kAlignChunk, p.numel);
-  stable_scatter(ids, start, end, p.experts, sm, p.sorted_ids);
+  stable_scatter(ids, start, end, p.experts, sm, p.sorted_ids, p.slots);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -347,27 +365,31 @@ cudaError_t launch_align(int id_dtype, const AlignParams& p, cudaStream_t s) {
 
 int64_t align_gather_max_numel() { return kAlignSmall; }
 
-cudaError_t launch_align_gather(const AlignParams& p, const void* x, int top_k, int hidden,
-                                void* xs, int32_t* zero, int zero_n, cudaStream_t s) {
+template <typename Put>
+static cudaError_t launch_align_put(const AlignParams& p, const void* x, int top_k, int hidden,
+                                    const Put& put, int32_t* zero, int zero_n, cudaStream_t s) {
   if (p.numel < 1 || p.numel > kAlignSmall || hidden % 8 != 0) return cudaErrorInvalidValue;
   // slices of at least 16 routes, one CTA each, at most one CTA per SM
   const int sms = sm_count() > 0 ? sm_count() : 1;
   int64_t slice = (p.numel + sms - 1) / sms;
   if (slice < 16) slice = 16;
   const unsigned grid = (unsigned)((p.numel + slice - 1) / slice);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kAlignThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e =
-      cudaLaunchKernelEx(&cfg, align_gather_kernel<int32_t>, p, static_cast<const uint4*>(x),
-                         top_k, hidden / 8, static_cast<uint4*>(xs), (int)slice, zero, zero_n);
-  return e != cudaSuccess ? e : cudaGetLastError();
+  return launch_pdl(align_gather_kernel<int32_t, Put>, grid, kAlignThreads, 0, s, p,
+                    static_cast<const uint4*>(x), top_k, hidden / 8, put, (int)slice, zero, zero_n);
+}
+
+cudaError_t launch_align_gather(const AlignParams& p, const void* x, int top_k, int hidden,
+                                void* xs, int32_t* zero, int zero_n, cudaStream_t s) {
+  return launch_align_put(p, x, top_k, hidden, CopyRows{static_cast<uint4*>(xs), hidden / 8}, zero,
+                          zero_n, s);
+}
+
+cudaError_t launch_align_split(const AlignParams& p, const void* x, int top_k, int hidden,
+                               uint8_t* xq, uint8_t* xs, int32_t* zero, int zero_n,
+                               cudaStream_t s) {
+  if (hidden % 256 != 0) return cudaErrorInvalidValue;
+  return launch_align_put(p, x, top_k, hidden, SplitRows{{xq, xs, hidden, p.block_size}}, zero,
+                          zero_n, s);
 }
 
 }  // namespace exf

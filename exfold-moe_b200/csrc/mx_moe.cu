@@ -3,166 +3,104 @@
 //
 // The weights go to the tensor cores as they are: TMA pads 16 packed codes to 16 bytes, and
 // tcgen05.mma kind::mxf8f6f4 takes e2m1 codes with their E8M0 scales (one per row and 32 k) against
-// 8-bit activations.  An activation is the sum of two e4m3 terms with scales 2^-5 apart: over a
-// block of 32 with the largest magnitude in [2^m, 2^(m+1)) and s = 2^(m-7),
-//   hi = e4m3(v / s),  lo = e4m3(32 (v / s - hi)),  v = s hi + (s / 32) lo.
-// hi keeps 4 significant bits and the remainder, below 2^-4 of v, keeps 4 more: a bf16 activation
-// (8 bits) is represented exactly unless it is smaller than 2^-13 of its block's largest, where
-// the error stays below 2^-22 of that; the fp32 intermediate h is rounded by at most 2^-9 of its
-// value (as bf16 would).  hi and lo are the two halves of the N side, so the weights are read once for
-// both, and the epilogue adds the two accumulators.  The products are exact, the sums fp32.
+// 8-bit activations, which enter as the sum of two e4m3 terms (exf_mx.cuh).  The products are exact,
+// the sums fp32.
 //
-// Launches: moe_align -> split (token rows into hi / lo rows in route order) -> the layer (both
-// GEMMs, persistent) -> combine (each token's routes summed in fp32, in order).
+// Launches: moe_align and the token rows' two-term form in route order (one launch up to 8192
+// routes) -> the layer (decode: both GEMMs in one persistent launch; prefill: a launch each) ->
+// combine (each token's routes summed in fp32, in order).
 #include <cuda.h>
 #include <cuda_bf16.h>
-#include <cuda_fp8.h>
 
 #include <mutex>
 
 #include "exf_common.cuh"
 #include "exf_launch.h"
+#include "exf_mx.cuh"
 #include "exf_mxmoe.h"
 #include "exf_tc.cuh"
 
 namespace exf {
 using namespace tc;
 
-constexpr int kMxLayerThreads = 256;  // warps 0, 6, 7 TMA, warp 1 MMA, warps 2-5 epilogue
-constexpr int kMxK = 128;             // k values of a stage: 4 MMA steps, one scale word
+constexpr int kMxLayerThreads = 384;  // warps 0, 2, 3 TMA, warp 1 MMA, warps 4-11 epilogue
 
-// ---- the two-term form ------------------------------------------------------------------------
-// scale byte of a block from the bits of its largest magnitude: s = 2^(byte - 127); at least 5, so
-// that lo's byte (5 less) exists; 255 (NaN) if the block holds an infinity or NaN
-__device__ __forceinline__ uint32_t split_scale(uint32_t top_bits) {
-  const int e = (int)(top_bits >> 23) - 7;
-  return top_bits >= 0x7f800000u ? 255u : (uint32_t)(e > 5 ? e : 5);
-}
-__device__ __forceinline__ float split_inverse(uint32_t byte) {
-  return __uint_as_float((254u - (byte == 255u ? 127u : byte)) << 23);
-}
-__device__ __forceinline__ uint32_t split_lo_byte(uint32_t byte) {
-  return byte == 255u ? 255u : byte - 5u;
-}
-// two values -> hi and lo terms, the first in the low byte
-__device__ __forceinline__ void split2(float a, float b, float inv, uint32_t& hi, uint32_t& lo) {
-  const float2 v = make_float2(a * inv, b * inv);
-  const __nv_fp8x2_storage_t h = __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
-  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(h, __NV_E4M3);
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
-  hi = h;
-  lo = __nv_cvt_float2_to_fp8x2(make_float2((v.x - f.x) * 32.0f, (v.y - f.y) * 32.0f),
-                                __NV_SATFINITE, __NV_E4M3);
-}
-// Scales of a route block's rows [0, 2 BT): tables [k / 128][512], one per 128 rows.  Byte of row n,
-// scale block kb, in the tables of the route block's first one.
-__device__ __forceinline__ int64_t scale_at(int64_t table, int kblocks, int kb, int n) {
-  return ((table + (n >> 7)) * kblocks + (kb >> 2)) * 512 + (n & 31) * 16 + ((n >> 5) & 3) * 4 +
-         (kb & 3);
-}
-// tables of a route block
-__host__ __device__ constexpr int scale_tables(int bt) { return bt > 64 ? 2 : 1; }
-
-// ---- split: token rows in route order ------------------------------------------------------------
-// For every real slot m (block m / BT, row r = m % BT): rows r and BT + r of the block in xq hold
-// the hi and lo terms of x[token], xs their scales.  4 lanes share a block of 32.  Padding rows
-// keep whatever the workspace holds: a row feeds its own accumulator column only, and a padding
-// column is never stored.  Also zeroes the layer's counters.
-__global__ void __launch_bounds__(256) mx_split_kernel(const __nv_bfloat16* x, MxRoutes r,
-                                                       int64_t rows, int numel, int top_k,
-                                                       int hidden, int bt, uint8_t* xq, uint8_t* xs,
+// ---- token rows in route order (more than align_gather_max_numel() routes) -----------------------
+// A warp takes a token: its row is split once and written to the slots of its routes.
+__global__ void __launch_bounds__(256) mx_split_kernel(const __nv_bfloat16* x, const int32_t* slots,
+                                                       int64_t tokens, int top_k, MxRows rows,
                                                        int32_t* zero, int zero_n) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < zero_n; i += gridDim.x * blockDim.x)
     zero[i] = 0;
-  const int vec = hidden / 8;  // a multiple of 32: a warp stays in one row
-  const int64_t used = *r.num_post_pad < rows ? *r.num_post_pad : rows;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < used * vec;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t m = i / vec;
-    const int c = (int)(i - m * vec);
-    const int route = r.sorted_ids[m];
-    if (route >= numel) continue;
-    const uint4 v = reinterpret_cast<const uint4*>(x + (int64_t)(route / top_k) * hidden)[c];
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      top = max(top, max((w[j] << 16) & 0x7fff0000u, w[j] & 0x7fff0000u));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t sb = split_scale(top);
-    const float inv = split_inverse(sb);
-    uint32_t hi[4], lo[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      split2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u), inv, hi[j], lo[j]);
-    const int64_t blk = m / bt;
-    const int n = (int)(m - blk * bt);
-    uint8_t* q = xq + (blk * 2 * bt + n) * hidden + 8 * c;
-    *reinterpret_cast<uint2*>(q) = make_uint2(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16);
-    *reinterpret_cast<uint2*>(q + (int64_t)bt * hidden) =
-        make_uint2(lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
-    if ((c & 3) == 0) {
-      const int64_t table = blk * scale_tables(bt);
-      xs[scale_at(table, hidden / kMxK, c >> 2, n)] = (uint8_t)sb;
-      xs[scale_at(table, hidden / kMxK, c >> 2, bt + n)] = (uint8_t)split_lo_byte(sb);
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = (int64_t)gridDim.x * (blockDim.x / 32);
+  for (int64_t t = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); t < tokens;
+       t += warps) {
+    const int mine = lane < top_k ? slots[t * top_k + lane] : -1;
+    if (__ballot_sync(0xffffffffu, mine >= 0) == 0) continue;
+    const uint4* row = reinterpret_cast<const uint4*>(x + t * rows.hidden);
+#pragma unroll 2
+    for (int c = lane; c < rows.hidden / 8; c += 32) {
+      const MxTerms v = split8(row[c]);
+      for (int j = 0; j < top_k; ++j) {
+        const int slot = __shfl_sync(0xffffffffu, mine, j);
+        if (slot >= 0) put8(rows, slot, c, v);
+      }
     }
   }
 }
 
-// ---- the layer ------------------------------------------------------------------------------------
-// As the bf16 decode layer: a tile is 256 weight rows of one expert (two 128-row MMA tiles on the M
-// side) times a block of BT of its routes (N = 2 BT: hi rows, lo rows).
+// ---- decode ---------------------------------------------------------------------------------------
+// A tile is a block of 64 routes (hi and lo rows: the 128 rows of the M side) times 256 weight rows of
+// one expert (the N side).  With the weights on the N side an MMA (128 x 256 x 32) takes 128 cycles for
+// 256 rows and hides the scales' copies to TMEM; on the M side it took 64 cycles for 128 rows
+// whatever the number of routes, and the copies came on top (763 cycles a stage against 525), which
+// held the weight stream at the copy peak's edge.
 //   GEMM-1 tile (block, f): gate rows [128 f, +128) and up rows [I + 128 f, +128) of W13[e], K = H;
-//     the epilogue forms h = silu(gate) * up, a lane per feature, and writes its two-term form
-//     (a warp's 32 features are one scale block);
+//     the epilogue forms h = silu(gate) * up and writes its two-term form;
 //   GEMM-2 tile (block, f): rows [256 f, +256) of W2[e], K = I; out[route][256 f + i] = w_route D.
 // One persistent launch: warp 0 takes tiles from a counter (every GEMM-1 tile, then the GEMM-2
-// tiles) and passes them on through a ring.  Three warps load: the first weight tile, the second,
-// and the token tile, each with its scales (one thread issuing every copy of a stage held the
-// weight stream at 4.0 TB/s: a row of packed codes is a 64-byte request; alone, 16-byte padded
-// tiles stream at 5.3 TB/s from one issuing thread and at 6.6 from two).  The warp that loads
-// tokens waits, before the first load of a GEMM-2 tile, until the epilogue warps of the block's
-// GEMM-1 tiles have counted themselves off; the weights of such a tile do not wait.  A GEMM-1 tile
-// waits only for earlier tiles of its own CTA and was handed out before every GEMM-2 tile, so the
-// wait ends; it is bounded all the same.
-template <int BT>
+// tiles) and passes them on through a ring.  Three warps load: the first 128 weight rows, the
+// second, and the token rows, each with its scales (a row of packed codes is a 64-byte request:
+// padded tiles stream at 5.3 TB/s from one issuing thread and at 6.6 from two).  The warp that
+// loads tokens waits, before the first load of a GEMM-2 tile, until the epilogue warps of the
+// block's GEMM-1 tiles have counted themselves off; the weights of such a tile do not wait.  A
+// GEMM-1 tile waits only for earlier tiles of its own CTA and was handed out before every GEMM-2
+// tile, so the wait ends; it is bounded all the same.
+//
+// The accumulator (256 TMEM columns) leaves room for the scales but not for a second one: 8
+// epilogue warps sum its two terms into registers and give it back before they compute (computing
+// from it, the epilogue was exposed and took 40 % of the layer).  Scales are loaded for 4 stages at a
+// time, 2 KB a copy: a copy a stage cost as much of the TMA unit as a third of a weight tile.
 struct MxCfg {
-  static constexpr int kN = 2 * BT;
+  static constexpr int kTTile = 128 * kMxK;
   static constexpr int kWTile = 128 * kMxK;              // padded codes of 128 rows
-  static constexpr int kTTile = kN * kMxK;
-  static constexpr int kScales = 3 * 512;                // two weight tiles, one token tile
-  static constexpr int kTiles = 2 * kWTile + kTTile;
-  static constexpr int kWTx = kWTile / 2 + 512;          // a copy of codes counts them packed
-  static constexpr int kTTx = kTTile + 512;
-  static constexpr int kStages = (210 * 1024) / (kTiles + kScales);
-  static constexpr int kAccCols = 2 * kN;
-  static constexpr int kAccs = kAccCols * 2 + 64 <= 512 ? 2 : 1;
-  static constexpr int kScaleCol = kAccs * kAccCols;     // 4 sets of 16 columns
-  static constexpr int kTmemCols = 512;
+  static constexpr int kStages = 4;
+  static constexpr int kScaleRun = 4;                    // stages a copy of scales serves
+  static constexpr int kScaleBytes = kScaleRun * 512;
   static constexpr int kRing = 8;
 };
-template <int BT>
 struct MxSmem {
-  alignas(1024) uint8_t tiles[MxCfg<BT>::kStages][MxCfg<BT>::kTiles];
-  alignas(128) uint8_t scales[MxCfg<BT>::kStages][MxCfg<BT>::kScales];
-  alignas(8) uint64_t full[MxCfg<BT>::kStages];
-  alignas(8) uint64_t empty[MxCfg<BT>::kStages];
-  alignas(8) uint64_t acc_full[2];
-  alignas(8) uint64_t acc_empty[2];
-  alignas(8) uint64_t ring_full[MxCfg<BT>::kRing];
-  alignas(8) uint64_t ring_empty[MxCfg<BT>::kRing];
+  alignas(1024) uint8_t tiles[MxCfg::kStages][MxCfg::kTTile + 2 * MxCfg::kWTile];
+  // Slots of scales (token rows, first and second weight rows).  A tile takes the next slot every
+  // kScaleRun stages; as many slots as stages, so that the slot a load overwrites belongs to
+  // stages already released (the loads between cover a stage each, at least).
+  alignas(128) uint8_t scales[MxCfg::kStages][3][MxCfg::kScaleBytes];
+  alignas(8) uint64_t full[MxCfg::kStages];
+  alignas(8) uint64_t empty[MxCfg::kStages];
+  alignas(8) uint64_t acc_full;
+  alignas(8) uint64_t acc_empty;
+  alignas(8) uint64_t ring_full[MxCfg::kRing];
+  alignas(8) uint64_t ring_empty[MxCfg::kRing];
   alignas(8) uint64_t drain;
-  int ring[MxCfg<BT>::kRing];
+  int ring[MxCfg::kRing];
   uint32_t tmem_base;
   int failed;
 };
-template <int BT>
-constexpr size_t mx_smem_bytes() { return sizeof(MxSmem<BT>) + 1024; }
-static_assert(mx_smem_bytes<32>() <= 232448 && mx_smem_bytes<64>() <= 232448,
-              "expert layer shared memory");
+constexpr size_t mx_smem_bytes() { return sizeof(MxSmem) + 1024; }
+static_assert(mx_smem_bytes() <= 232448, "decode expert layer shared memory");
 
 struct MxTile {
   bool down;
@@ -179,6 +117,11 @@ __device__ __forceinline__ MxTile mx_tile(int t, int blocks, int n1, int n2) {
   return r;
 }
 
+// bytes of scales from k block kb on that one copy brings
+__device__ __forceinline__ int scale_run(int kblocks, int kb) {
+  return 512 * (kblocks - kb < MxCfg::kScaleRun ? kblocks - kb : MxCfg::kScaleRun);
+}
+
 // After a time-out (else every load has been consumed): copies still in flight land before shared
 // memory is released.  The other loading warps may never arrive on a stage, so that its barrier
 // does not complete: the wait is bounded.
@@ -192,17 +135,36 @@ __device__ __forceinline__ void drain_loads(uint64_t* full, uint32_t g) {
   }
 }
 
-template <int BT>
+// silu(g) * u; exp overflows to inf, where the quotient is 0
+__device__ __forceinline__ float silu_up(float g, float u) {
+  return __fdividef(g, 1.0f + __expf(-g)) * u;
+}
+
+// Four lanes hold the 16-bit pairs w[0..3] of a row's four groups; lane j of them gets the four
+// lanes' pairs of group j, in lane order: 8 consecutive bytes of the row.
+__device__ __forceinline__ uint2 gather_pairs(const uint32_t (&w)[4], int j) {
+  const bool odd = j & 1, high = j & 2;
+  uint32_t send = odd ? __byte_perm(w[0], w[2], 0x5410) : __byte_perm(w[1], w[3], 0x5410);
+  const uint32_t keep = odd ? __byte_perm(w[1], w[3], 0x5410) : __byte_perm(w[0], w[2], 0x5410);
+  const uint32_t got = __shfl_xor_sync(0xffffffffu, send, 1);
+  // pairs of the groups j % 2 and j % 2 + 2 from this lane and its neighbour, even lane first
+  const uint32_t lo = odd ? __byte_perm(got, keep, 0x5410) : __byte_perm(keep, got, 0x5410);
+  const uint32_t hi = odd ? __byte_perm(got, keep, 0x7632) : __byte_perm(keep, got, 0x7632);
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, high ? lo : hi, 2);
+  return high ? make_uint2(other, hi) : make_uint2(lo, other);
+}
+
 __global__ void __launch_bounds__(kMxLayerThreads, 1)
     mx_layer_kernel(const __grid_constant__ CUtensorMap map_w13,
                     const __grid_constant__ CUtensorMap map_xq,
                     const __grid_constant__ CUtensorMap map_w2,
                     const __grid_constant__ CUtensorMap map_hq, const MxLayerParams p) {
-  using C = MxCfg<BT>;
+  using C = MxCfg;
   constexpr int kStages = C::kStages;
   constexpr int kRing = C::kRing;
+  constexpr int BT = kMxDecodeBlock;
   extern __shared__ uint8_t smem_raw[];
-  MxSmem<BT>& sm = *reinterpret_cast<MxSmem<BT>*>(
+  MxSmem& sm = *reinterpret_cast<MxSmem*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -212,19 +174,17 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
       mbar_init(&sm.full[s], 3);  // one arrival per loading warp
       mbar_init(&sm.empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&sm.acc_full[b], 1);
-      mbar_init(&sm.acc_empty[b], 4);
-    }
+    mbar_init(&sm.acc_full, 1);
+    mbar_init(&sm.acc_empty, 8);
     for (int j = 0; j < kRing; ++j) {
       mbar_init(&sm.ring_full[j], 1);
-      mbar_init(&sm.ring_empty[j], 7);  // two loading warps, the MMA thread, four epilogue warps
+      mbar_init(&sm.ring_empty[j], 11);  // two loading warps, the MMA thread, 8 epilogue warps
     }
     mbar_init(&sm.drain, 1);
     sm.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) tmem_alloc(&sm.tmem_base, C::kTmemCols);
+  if (warp == 1) tmem_alloc(&sm.tmem_base, 512);
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
@@ -242,13 +202,30 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
     const int e = p.routes.expert_ids[lt.blk];
     return (e >= 0 && e < p.experts) ? e : -1;
   };
+  // real routes of a block (they come first), by a whole warp
+  auto real_of = [&](int blk) {
+    const int32_t* ids = p.routes.sorted_ids + (int64_t)blk * BT;
+    return __popc(__ballot_sync(0xffffffffu, ids[lane] < p.numel)) +
+           __popc(__ballot_sync(0xffffffffu, ids[32 + lane] < p.numel));
+  };
+  // the next tile from the ring for a whole warp: its number, -1 at the end, -2 after a time-out
+  auto next_tile = [&](int j) {
+    const int slot = j % kRing;
+    int tile = -2;
+    if (lane == 0 && mbar_wait(&sm.ring_full[slot], (j / kRing) & 1, failed)) {
+      tile = sm.ring[slot];
+      mbar_arrive(&sm.ring_empty[slot]);
+    }
+    return __shfl_sync(0xffffffffu, tile, 0);
+  };
 
   uint32_t issued = 0;  // stages this thread has loaded into
-  if (warp == 0 || warp >= 6) {
-    // ---- loads: warp 0 (which also hands out the tiles) and warp 6 a weight tile each, warp 7 the
-    // token tile; one thread each
+  if (warp == 0 || warp == 2) {
+    // ---- weight loads, one thread each: gate (warp 0) and up (warp 2) rows of W13[e], or the
+    // halves of 256 rows of W2[e]; warp 0 also hands out the tiles
     if (lane == 0) {
-      uint32_t g = 0;
+      const int half = warp == 0 ? 0 : 1;
+      uint32_t g = 0, run = 0;  // stages and runs of scales loaded
       bool ok = true;
       int t = warp == 0 ? atomicAdd(p.sync, 1) : 0;
       for (int j = 0; ok; ++j) {
@@ -272,55 +249,73 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
         const int expert = expert_of(lt);
         if (expert < 0) continue;
         const int kblocks = (lt.down ? p.inter : p.hidden) / kMxK;
-        if (warp == 7) {
-          if (lt.down) {
-            const int32_t* flag = p.sync + 1 + lt.blk;
-            uint32_t it = 0;
-            while (ld_acquire_gpu(flag) < 4 * n1) {
-              if (*failed || ++it >= kWaitLimit) {
-                *failed = 1;
-                ok = false;
-                break;
-              }
-              __nanosleep(64);
-            }
-            if (!ok) break;
-            asm volatile("fence.proxy.async.global;" ::: "memory");
-          }
-          const CUtensorMap* map = lt.down ? &map_hq : &map_xq;
-          const uint8_t* sc = (lt.down ? p.hs : p.xs) + (int64_t)lt.blk * kblocks * 512;
-          for (int kb = 0; kb < kblocks; ++kb, ++g) {
-            const int s = g % kStages;
-            ok = mbar_wait(&sm.empty[s], ((g / kStages) & 1) ^ 1, failed);
-            if (!ok) break;
-            mbar_expect_tx(&sm.full[s], C::kTTx);
-            tma_load_2d(sm.tiles[s] + 2 * C::kWTile, map, &sm.full[s], kb * kMxK, lt.blk * C::kN);
-            bulk_load(sm.scales[s] + 1024, sc + kb * 512, 512, &sm.full[s]);
-          }
-        } else {
-          // gate (warp 0) and up (warp 6) rows of W13[e], or the halves of 256 rows of W2[e]
-          const int half = warp == 0 ? 0 : 1;
-          const int row = lt.down
-                              ? expert * p.hidden + lt.ft * 256 + half * 128
-                              : expert * 2 * p.inter + lt.ft * 128 + half * p.inter;
-          const CUtensorMap* map = lt.down ? &map_w2 : &map_w13;
-          const uint8_t* sc = (lt.down ? p.s2 : p.s13) + (int64_t)(row / 128) * kblocks * 512;
-          for (int kb = 0; kb < kblocks; ++kb, ++g) {
-            const int s = g % kStages;
-            ok = mbar_wait(&sm.empty[s], ((g / kStages) & 1) ^ 1, failed);
-            if (!ok) break;
-            mbar_expect_tx(&sm.full[s], C::kWTx);
-            tma_load_2d(sm.tiles[s] + half * C::kWTile, map, &sm.full[s], kb * kMxK, row);
-            bulk_load(sm.scales[s] + half * 512, sc + kb * 512, 512, &sm.full[s]);
-          }
+        const int row = lt.down ? expert * p.hidden + lt.ft * 256 + half * 128
+                                : expert * 2 * p.inter + lt.ft * 128 + half * p.inter;
+        const CUtensorMap* map = lt.down ? &map_w2 : &map_w13;
+        const uint8_t* sc = (lt.down ? p.s2 : p.s13) + (int64_t)(row / 128) * kblocks * 512;
+        for (int kb = 0; kb < kblocks; ++kb, ++g) {
+          const int s = g % kStages;
+          ok = mbar_wait(&sm.empty[s], ((g / kStages) & 1) ^ 1, failed);
+          if (!ok) break;
+          const int sb = kb % C::kScaleRun == 0 ? scale_run(kblocks, kb) : 0;
+          mbar_expect_tx(&sm.full[s], C::kWTile / 2 + sb);  // codes count as they lie in memory
+          tma_load_2d(sm.tiles[s] + C::kTTile + half * C::kWTile, map, &sm.full[s], kb * kMxK, row);
+          if (sb) bulk_load(sm.scales[run++ % kStages][1 + half], sc + kb * 512, sb, &sm.full[s]);
         }
       }
       issued = g;
     }
+  } else if (warp == 3) {
+    // ---- token loads: the quarters of the block that hold routes, a lane each
+    uint32_t g = 0, run = 0;
+    bool ok = true;
+    for (int j = 0; ok; ++j) {
+      const int tile = next_tile(j);
+      if (tile < 0) break;
+      const MxTile lt = mx_tile(tile, blocks, n1, n2);
+      if (expert_of(lt) < 0) continue;
+      const int quarters = (real_of(lt.blk) + 15) >> 4;
+      if (lt.down) {
+        const int32_t* flag = p.sync + 1 + lt.blk;
+        uint32_t it = 0;
+        while (ld_acquire_gpu(flag) < 8 * n1) {
+          if (*failed || ++it >= kWaitLimit) {
+            *failed = 1;
+            ok = false;
+            break;
+          }
+          __nanosleep(32);
+        }
+        if (!__all_sync(0xffffffffu, ok)) break;
+        asm volatile("fence.proxy.async.global;" ::: "memory");
+      }
+      const int kblocks = (lt.down ? p.inter : p.hidden) / kMxK;
+      const CUtensorMap* map = lt.down ? &map_hq : &map_xq;
+      const uint8_t* sc = (lt.down ? p.hs : p.xs) + (int64_t)lt.blk * kblocks * 512;
+      for (int kb = 0; kb < kblocks; ++kb, ++g) {
+        const int s = g % kStages;
+        ok = mbar_wait(&sm.empty[s], ((g / kStages) & 1) ^ 1, failed);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        const int sb = kb % C::kScaleRun == 0 ? scale_run(kblocks, kb) : 0;
+        if (lane == 0) mbar_expect_tx(&sm.full[s], quarters * 32 * kMxK + sb);
+        __syncwarp();
+        if (lane < quarters)
+          tma_load_2d(sm.tiles[s] + lane * 32 * kMxK, map, &sm.full[s], kb * kMxK,
+                      lt.blk * 128 + 32 * lane);
+        if (sb) {
+          if (lane == 31) bulk_load(sm.scales[run % kStages][0], sc + kb * 512, sb, &sm.full[s]);
+          ++run;
+        }
+      }
+    }
+    issued = g;
   } else if (warp == 1) {
-    // ---- MMA issuer; scale sets rotate over 4 groups of 16 TMEM columns
+    // ---- MMA issuer; scale sets rotate over 4 groups of 16 TMEM columns from 256 on
     if (lane == 0) {
-      uint32_t g = 0;
+      uint32_t g = 0, run = 0;
       int i = 0;
       bool ok = true;
       for (int j = 0; ok; ++j) {
@@ -333,113 +328,131 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
         const MxTile lt = mx_tile(tile, blocks, n1, n2);
         if (expert_of(lt) < 0) continue;
         const int kblocks = (lt.down ? p.inter : p.hidden) / kMxK;
-        const int b = i % C::kAccs;
-        ok = mbar_wait(&sm.acc_empty[b], ((i / C::kAccs) & 1) ^ 1, failed);
+        ok = mbar_wait(&sm.acc_empty, (i & 1) ^ 1, failed);
         if (!ok) break;
         fence_after_sync();
-        const uint32_t acc = tmem + static_cast<uint32_t>(b * C::kAccCols);
         for (int kb = 0; kb < kblocks; ++kb, ++g) {
           const int s = g % kStages;
           ok = mbar_wait(&sm.full[s], (g / kStages) & 1, failed);
           if (!ok) break;
           fence_after_sync();
-          const uint32_t w_base = smem_addr(sm.tiles[s]);
-          const uint32_t t_base = w_base + 2 * C::kWTile;
-          const uint32_t sc = smem_addr(sm.scales[s]);
-          const uint32_t sf = tmem + C::kScaleCol + (g & 3) * 16;
+          const uint32_t a = smem_addr(sm.tiles[s]);
+          const uint32_t b = a + C::kTTile;
+          if (kb % C::kScaleRun == 0) ++run;
+          const uint32_t sc =
+              smem_addr(sm.scales[(run - 1) % kStages][0]) + (kb % C::kScaleRun) * 512;
+          const uint32_t sf = tmem + 256 + (g & 3) * 16;
           tmem_copy_scales(sf, sc);
-          tmem_copy_scales(sf + 4, sc + 512);
-          tmem_copy_scales(sf + 8, sc + 1024);
+          tmem_copy_scales(sf + 8, sc + C::kScaleBytes);
+          tmem_copy_scales(sf + 12, sc + 2 * C::kScaleBytes);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t on = (kb > 0 || k > 0) ? 1u : 0u;
-            const uint32_t id = idesc_mx(128, C::kN, kMxE2M1, kMxE4M3, k);
-            mma_mx(acc, smem_desc(w_base + k * 32), smem_desc(t_base + k * 32), id, sf, sf + 8,
-                   on);
-            mma_mx(acc + C::kN, smem_desc(w_base + C::kWTile + k * 32),
-                   smem_desc(t_base + k * 32), id, sf + 4, sf + 8, on);
-          }
+          for (int k = 0; k < 4; ++k)
+            mma_mx(tmem, smem_desc(a + k * 32), smem_desc(b + k * 32),
+                   idesc_mx(128, 256, kMxE4M3, kMxE2M1, k), sf, sf + 8,
+                   (kb > 0 || k > 0) ? 1u : 0u);
           mma_commit(&sm.empty[s]);
         }
         if (!ok) break;
-        mma_commit(&sm.acc_full[b]);
+        mma_commit(&sm.acc_full);
         ++i;
       }
       mma_commit(&sm.drain);
       mbar_wait_drain(&sm.drain, 0);
     }
   } else {
-    // ---- epilogue: warp q owns TMEM lanes 32 q .. +31, i.e. 32 weight rows of each M tile;
-    // columns are routes (hi, then lo), 16 at a time
-    const int q = warp & 3;
+    // ---- epilogue: a warp has the 16 routes of quarter q (hi in TMEM lanes 32 q .. +15, lo in the
+    // next 16) and half the columns: gate and up of features [64 hf, +64), or output columns
+    // [64 hf, +64) and [128 + 64 hf, +64).  Read as 16 x 32 fragments, a lane has routes l / 4 and
+    // l / 4 + 8 and two neighbouring columns of every 8, both terms at the same place.
+    const int q = warp & 3, hf = (warp - 4) >> 2;
+    const int quad = lane & 3;
     int i = 0;
     for (int j = 0;; ++j) {
-      const int slot = j % kRing;
-      int tile = -2;
-      if (lane == 0 && mbar_wait(&sm.ring_full[slot], (j / kRing) & 1, failed)) {
-        tile = sm.ring[slot];
-        mbar_arrive(&sm.ring_empty[slot]);
-      }
-      tile = __shfl_sync(0xffffffffu, tile, 0);
+      const int tile = next_tile(j);
       if (tile < 0) break;
       const MxTile lt = mx_tile(tile, blocks, n1, n2);
       if (expert_of(lt) < 0) continue;
-      const int b = i % C::kAccs;
-      const bool ok = mbar_wait(&sm.acc_full[b], (i / C::kAccs) & 1, failed);
+      int r[2], route[2];
+      float wr[2];
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        r[z] = 16 * q + (lane >> 2) + 8 * z;
+        route[z] = p.routes.sorted_ids[lt.blk * BT + r[z]];
+        wr[z] = lt.down && route[z] < p.numel ? p.route_w[route[z]] : 0.0f;
+      }
+      const bool on[2] = {route[0] < p.numel, route[1] < p.numel};
+      const bool any = __any_sync(0xffffffffu, on[0]);  // routes fill their quarter from place 0
+      const bool any8 = __any_sync(0xffffffffu, on[1]);
+      const bool ok = mbar_wait(&sm.acc_full, i & 1, failed);
       fence_after_sync();
       if (!__all_sync(0xffffffffu, ok && !*failed)) break;
-      const uint32_t taddr =
-          tmem + static_cast<uint32_t>(b * C::kAccCols) + ((uint32_t)(q * 32) << 16);
-#pragma unroll 1
-      for (int c = 0; c < BT; c += 16) {
-        const int route_l =
-            lane < 16 ? p.routes.sorted_ids[lt.blk * BT + c + lane] : p.numel;
-        const uint32_t real = __ballot_sync(0xffffffffu, route_l < p.numel);
-        if (real == 0) continue;
-        uint32_t a0[16], a1[16], b0[16], b1[16];
-        tmem_load16(taddr + c, a0);
-        tmem_load16(taddr + BT + c, a1);
-        tmem_load16(taddr + C::kN + c, b0);
-        tmem_load16(taddr + C::kN + BT + c, b1);
-        tmem_wait();
-        if (!lt.down) {
-          const int feat = lt.ft * 128 + q * 32 + lane;
-          uint8_t* hq = p.hq + ((int64_t)lt.blk * C::kN + c) * p.inter + feat;
+      float v[4][16];  // runs of 32 columns
+      if (any) {
+        const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            if (!((real >> r) & 1)) continue;
-            const float gt = __uint_as_float(a0[r]) + __uint_as_float(a1[r]);
-            const float up = __uint_as_float(b0[r]) + __uint_as_float(b1[r]);
-            const float h = gt / (1.0f + __expf(-gt)) * up;
-            const uint32_t top =
-                __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
-            const uint32_t sb = split_scale(top);
-            uint32_t hi, lo;
-            split2(h, 0.0f, split_inverse(sb), hi, lo);
-            hq[(int64_t)r * p.inter] = (uint8_t)hi;
-            hq[(int64_t)(BT + r) * p.inter] = (uint8_t)lo;
-            if (lane < 2)
-              p.hs[scale_at(lt.blk, p.inter / kMxK, lt.ft * 4 + q, c + r + (lane ? BT : 0))] =
-                  (uint8_t)(lane ? split_lo_byte(sb) : sb);
-          }
-        } else {
-          const int feat = lt.ft * 256 + q * 32 + lane;
-          const float w_l = route_l < p.numel ? p.route_w[route_l] : 0.0f;
+        for (int b = 0; b < 4; ++b) {
+          const uint32_t col = 128 * (b >> 1) + 64 * hf + 32 * (b & 1);
+          uint32_t hi[16], lo[16];
+          tmem_load_16x32(lanes + col, hi);
+          tmem_load_16x32(lanes + (16u << 16) + col, lo);
+          tmem_wait();
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int route = __shfl_sync(0xffffffffu, route_l, r);
-            const float wr = __shfl_sync(0xffffffffu, w_l, r);
-            if (!((real >> r) & 1)) continue;
-            float* o = p.out + (int64_t)route * p.hidden + feat;
-            o[0] = (__uint_as_float(a0[r]) + __uint_as_float(a1[r])) * wr;
-            o[128] = (__uint_as_float(b0[r]) + __uint_as_float(b1[r])) * wr;
-          }
+          for (int n = 0; n < 16; ++n) v[b][n] = __uint_as_float(hi[n]) + __uint_as_float(lo[n]);
         }
       }
       fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.acc_empty[b]);
+      if (lane == 0) mbar_arrive(&sm.acc_empty);
       ++i;
+      if (any && !lt.down) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {  // scale blocks of 32 features
+          const int feat = lt.ft * 128 + 64 * hf + 32 * b;
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            if (z == 1 && !any8) break;
+            float h[8];
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int n = 4 * (e >> 1) + 2 * z + (e & 1);
+              h[e] = silu_up(v[b][n], v[2 + b][n]);
+              top = max(top, __float_as_uint(h[e]) & 0x7fffffffu);
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const uint32_t sb = split_scale(top);
+            const float inv = split_inverse(sb);
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split2(h[2 * e], h[2 * e + 1], inv, hi[e], lo[e]);
+            const uint2 hv = gather_pairs(hi, quad), lv = gather_pairs(lo, quad);
+            if (on[z]) {
+              const int n = mx_row(BT, r[z]);
+              uint8_t* at = p.hq + ((int64_t)lt.blk * 128 + n) * p.inter + feat + 8 * quad;
+              *reinterpret_cast<uint2*>(at) = hv;
+              *reinterpret_cast<uint2*>(at + (int64_t)mx_lo(BT) * p.inter) = lv;
+              if (quad < 2)
+                p.hs[scale_at(lt.blk, p.inter / kMxK, feat >> 5, quad ? n + mx_lo(BT) : n)] =
+                    (uint8_t)(quad ? split_lo_byte(sb) : sb);
+            }
+          }
+        }
+      } else if (any) {
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          if (!on[z]) continue;
+          float* o = p.out + (int64_t)route[z] * p.hidden + lt.ft * 256 + 64 * hf + 2 * quad;
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int n = 4 * e + 2 * z;
+              *reinterpret_cast<float2*>(o + 128 * (b >> 1) + 32 * (b & 1) + 8 * e) =
+                  make_float2(v[b][n] * wr[z], v[b][n + 1] * wr[z]);
+            }
+        }
+      }
       if (!lt.down) {
         // visible to the TMA loads of the block's GEMM-2 tiles, in any CTA; then count the warp off
         asm volatile("fence.proxy.async.global;" ::: "memory");
@@ -454,7 +467,7 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
   if (warp == 1) {
     __syncwarp();
     fence_after_sync();
-    tmem_free(tmem, C::kTmemCols);
+    tmem_free(tmem, 512);
   }
   if (sm.failed) {
     drain_loads<kStages>(sm.full, issued);
@@ -487,6 +500,17 @@ struct MxGemmSmem {
 };
 constexpr size_t mx_gemm_smem_bytes() { return sizeof(MxGemmSmem) + 1024; }
 static_assert(mx_gemm_smem_bytes() <= 232448, "prefill expert GEMM shared memory");
+
+// 8 values times w, a whole 32-byte sector in one store (two 16-byte stores of a row a thread each
+// cost L2 a partial write)
+__device__ __forceinline__ void store_sector(float* at, const uint32_t* v, float w) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at),
+               "f"(__uint_as_float(v[0]) * w), "f"(__uint_as_float(v[1]) * w),
+               "f"(__uint_as_float(v[2]) * w), "f"(__uint_as_float(v[3]) * w),
+               "f"(__uint_as_float(v[4]) * w), "f"(__uint_as_float(v[5]) * w),
+               "f"(__uint_as_float(v[6]) * w), "f"(__uint_as_float(v[7]) * w)
+               : "memory");
+}
 
 template <bool DOWN>
 __global__ void __launch_bounds__(kMxGemmThreads, 1)
@@ -638,10 +662,8 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
 #pragma unroll
           for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int c = 0; c < 16; c += 4)
-              *reinterpret_cast<float4*>(o + (j >> 2) * 128 + (j & 3) * 16 + c) = make_float4(
-                  __uint_as_float(v[j][c]) * wr, __uint_as_float(v[j][c + 1]) * wr,
-                  __uint_as_float(v[j][c + 2]) * wr, __uint_as_float(v[j][c + 3]) * wr);
+            for (int c = 0; c < 16; c += 8)
+              store_sector(o + (j >> 2) * 128 + (j & 3) * 16 + c, &v[j][c], wr);
         }
       } else if (real) {
 #pragma unroll
@@ -651,8 +673,8 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
           for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int c = 0; c < 16; ++c) {
-              const float gt = __uint_as_float(v[2 * b + j][c]);
-              const float h = gt / (1.0f + __expf(-gt)) * __uint_as_float(v[4 + 2 * b + j][c]);
+              const float h = silu_up(__uint_as_float(v[2 * b + j][c]),
+                                      __uint_as_float(v[4 + 2 * b + j][c]));
               v[2 * b + j][c] = __float_as_uint(h);
               top = max(top, __float_as_uint(h) & 0x7fffffffu);
             }
@@ -733,11 +755,10 @@ __global__ void __launch_bounds__(256, 4)
 }
 
 // ---- host side ---------------------------------------------------------------------------------
-// The route block, which also picks the kernels: 32 or 64 routes on the N side (decode) while the
-// average expert's routes fit with room for the fuller ones (an expert's second block reads its
-// weights again), else 128 on the M side (prefill).
+// The route block, which also picks the kernels: 64 routes while the average expert's fit with
+// room for the fuller ones (an expert's second block reads its weights again), else 128.
 static int mx_block(int64_t numel, int experts) {
-  return numel <= (int64_t)experts * 18 ? 32 : numel <= (int64_t)experts * 44 ? 64 : 128;
+  return numel <= (int64_t)experts * 44 ? kMxDecodeBlock : kMxPrefillBlock;
 }
 
 static int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
@@ -763,6 +784,7 @@ MxWorkspace mx_workspace(int64_t tokens, int top_k, int experts, int hidden, int
   w.num_post_pad = reinterpret_cast<int32_t*>(take(4));
   const int64_t align_bytes = align_workspace_bytes(numel, experts);
   w.align_ws = take(align_bytes > 0 ? align_bytes : 4);
+  w.slots = reinterpret_cast<int32_t*>(take(numel > align_gather_max_numel() ? numel * 4 : 4));
   w.xq = take(2 * cap * hidden);
   const int tables = scale_tables(w.block);
   w.xs = take(blocks * tables * (hidden / kMxK) * 512);
@@ -809,23 +831,20 @@ static MxLayerParams layer_params(const MxArgs& a, const MxWorkspace& w) {
   return p;
 }
 
-template <int BT>
 static cudaError_t launch_mx_layer(const MxArgs& a, const MxWorkspace& w, cudaStream_t s) {
-  auto* kern = mx_layer_kernel<BT>;
   static std::mutex mu;
   static bool done[64] = {};
-  const cudaError_t e = allow_smem(kern, mx_smem_bytes<BT>(), mu, done);
+  const cudaError_t e = allow_smem(mx_layer_kernel, mx_smem_bytes(), mu, done);
   if (e != cudaSuccess) return e;
-  const int64_t rows = w.capacity / BT * 2 * BT;
   CUtensorMap m13, mx, m2, mh;
   if (!make_map_4bit(&m13, a.w13, (uint64_t)a.experts * 2 * a.inter, a.hidden, 128) ||
-      !make_map_8bit(&mx, w.xq, rows, a.hidden, 2 * BT) ||
+      !make_map_8bit(&mx, w.xq, 2 * w.capacity, a.hidden, 32) ||
       !make_map_4bit(&m2, a.w2, (uint64_t)a.experts * a.hidden, a.inter, 128) ||
-      !make_map_8bit(&mh, w.hq, rows, a.inter, 2 * BT))
+      !make_map_8bit(&mh, w.hq, 2 * w.capacity, a.inter, 32))
     return cudaErrorInvalidValue;
   const int sms = sm_count();
-  return launch_pdl(kern, sms > 0 ? (unsigned)sms : 1u, kMxLayerThreads, mx_smem_bytes<BT>(), s,
-                    m13, mx, m2, mh, layer_params(a, w));
+  return launch_pdl(mx_layer_kernel, sms > 0 ? (unsigned)sms : 1u, kMxLayerThreads,
+                    mx_smem_bytes(), s, m13, mx, m2, mh, layer_params(a, w));
 }
 
 template <bool DOWN>
@@ -858,18 +877,24 @@ cudaError_t launch_mx_experts(const MxArgs& a, const MxWorkspace& w, cudaStream_
   const int64_t numel = a.tokens * a.top_k;
   AlignParams ap{a.topk_ids, numel, a.experts, w.block, w.capacity, w.sorted_ids, w.expert_ids,
                  w.num_post_pad, static_cast<int32_t*>(w.align_ws), 0};
-  cudaError_t e = launch_align(EXF_I32, ap, s);
+  cudaError_t e;
+  if (numel <= align_gather_max_numel()) {
+    e = launch_align_split(ap, a.x, a.top_k, a.hidden, w.xq, w.xs, w.sync, w.sync_ints, s);
+  } else {
+    ap.slots = w.slots;
+    e = launch_align(EXF_I32, ap, s);
+    if (e == cudaSuccess)
+      e = launch_pdl(mx_split_kernel, stream_grid(a.tokens * 32), 256, 0, s,
+                     static_cast<const __nv_bfloat16*>(a.x),
+                     static_cast<const int32_t*>(w.slots), a.tokens, a.top_k,
+                     MxRows{w.xq, w.xs, a.hidden, w.block}, w.sync, w.sync_ints);
+  }
   if (e != cudaSuccess) return e;
-  const MxRoutes routes{w.num_post_pad, w.expert_ids, w.sorted_ids};
-  e = launch_pdl(mx_split_kernel, stream_grid(w.capacity * (a.hidden / 8)), 256, 0, s,
-                 static_cast<const __nv_bfloat16*>(a.x), routes, w.capacity, (int)numel, a.top_k,
-                 a.hidden, w.block, w.xq, w.xs, w.sync, w.sync_ints);
-  if (e != cudaSuccess) return e;
-  if (w.block == 128) {
+  if (w.block == kMxPrefillBlock) {
     e = launch_mx_gemm<false>(a, w, s);
     if (e == cudaSuccess) e = launch_mx_gemm<true>(a, w, s);
   } else {
-    e = w.block == 32 ? launch_mx_layer<32>(a, w, s) : launch_mx_layer<64>(a, w, s);
+    e = launch_mx_layer(a, w, s);
   }
   if (e != cudaSuccess) return e;
   return launch_pdl(mx_combine_kernel, stream_grid(a.tokens * (a.hidden / 4)), 256, 0, s,
