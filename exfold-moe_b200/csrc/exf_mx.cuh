@@ -17,8 +17,7 @@
 namespace exf {
 
 constexpr int kMxK = 128;          // k values of a scale table: 4 MMA steps, one 32-bit scale word
-constexpr int kMxDecodeBlock = 64;   // routes of a block, decode
-constexpr int kMxPrefillBlock = 128; // and prefill
+constexpr int kMxPrefillBlock = 128; // routes of a block at prefill; 16, 32 or 64 at decode
 
 // scale byte of a block from the bits of its largest magnitude: s = 2^(byte - 127); at least 5, so
 // that lo's byte (5 less) exists; 255 (NaN) if the block holds an infinity or NaN
@@ -44,8 +43,8 @@ __device__ __forceinline__ void split2(float a, float b, float inv, uint32_t& hi
 }
 
 // Rows of a route block (of the two-term tensor and of the MMA's M side alike).  A block of 128: the
-// hi rows, then the lo rows, an MMA tile each.  A block of 64 is one tile: each 32-row quarter (the
-// TMEM lanes of an epilogue warp) holds the hi rows of 16 routes, then their lo rows.
+// hi rows, then the lo rows, an MMA tile each.  A smaller one is (part of) one tile: each 32-row
+// quarter (the TMEM lanes of an epilogue warp) holds the hi rows of 16 routes, then their lo rows.
 __device__ __forceinline__ int mx_row(int block, int r) {
   return block == kMxPrefillBlock ? r : 32 * (r >> 4) + (r & 15);
 }

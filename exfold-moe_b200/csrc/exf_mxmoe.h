@@ -22,7 +22,9 @@ struct MxLayerParams {
   int inter;
   int m_blocks;                 // route blocks of the capacity
   int* status;                  // set to 1 if a pipeline wait timed out (may be null)
-  const uint8_t* s13;           // weight scales in tiles (see MxArgs)
+  const uint8_t* w13;           // weights and their scales (see MxArgs)
+  const uint8_t* s13;
+  const uint8_t* w2;
   const uint8_t* s2;
   const uint8_t* xs;            // scales of the split token rows
   uint8_t* hq;                  // GEMM-1 output in the same form

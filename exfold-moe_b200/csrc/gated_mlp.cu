@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   GatedSmem<NT>& sm = *reinterpret_cast<GatedSmem<NT>*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  const int warp = threadIdx.x >> 5;
+  const int warp = uniform(threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -150,23 +150,23 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   const int ntiles = p.m_tiles * p.n_tiles;
-  const uint32_t tmem = sm.tmem_base;
+  const uint32_t tmem = uniform(sm.tmem_base);
   volatile int* failed = &sm.failed;
 
   if (warp == 0) {
     // ---- TMA producer
-    if (lane == 0) {
-      uint32_t g = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
-        const int mt = t / p.n_tiles, nt = t - mt * p.n_tiles;
-        for (int kb = 0; kb < p.kblocks; ++kb, ++g) {
-          const int s = g % C::kStages;
-          ok = mbar_wait(&sm.empty[s], ((g / C::kStages) & 1) ^ 1, failed);
-          if (!ok) break;
-          uint8_t* a = sm.tiles[s];
-          uint8_t* b = a + C::kATile;
-          uint64_t* bar = &sm.full[s];
+    uint32_t g = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
+      const int mt = t / p.n_tiles, nt = t - mt * p.n_tiles;
+      for (int kb = 0; kb < p.kblocks; ++kb, ++g) {
+        const int s = g % C::kStages;
+        ok = warp_wait(&sm.empty[s], ((g / C::kStages) & 1) ^ 1, failed);
+        if (!ok) break;
+        uint8_t* a = sm.tiles[s];
+        uint8_t* b = a + C::kATile;
+        uint64_t* bar = &sm.full[s];
+        if (elect_one()) {
           mbar_expect_tx(bar, C::kStage);
           if (kAMn) {
             tma_load_2d(a, &map_a, bar, mt * kGBM, kb * kGBK);
@@ -184,41 +184,43 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
           }
         }
       }
-      for (uint32_t j = g > C::kStages ? g - C::kStages : 0; j < g; ++j)
-        mbar_wait_drain(&sm.full[j % C::kStages], (j / C::kStages) & 1);
     }
+    for (uint32_t j = g > C::kStages ? g - C::kStages : 0; j < g; ++j)
+      mbar_wait_drain(&sm.full[j % C::kStages], (j / C::kStages) & 1);
   } else if (warp == 1) {
     // ---- MMA issuer: tile i accumulates into TMEM columns [NT (i & 1), +NT)
-    if (lane == 0) {
-      uint32_t g = 0;
-      int i = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++i) {
-        const int b = i & 1;
-        ok = mbar_wait(&sm.acc_empty[b], ((i >> 1) & 1) ^ 1, failed);
+    uint32_t g = 0;
+    int i = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++i) {
+      const int b = i & 1;
+      ok = warp_wait(&sm.acc_empty[b], ((i >> 1) & 1) ^ 1, failed);
+      if (!ok) break;
+      fence_after_sync();
+      const uint32_t acc = tmem + static_cast<uint32_t>(b * NT);
+      for (int kb = 0; kb < p.kblocks; ++kb, ++g) {
+        const int s = g % C::kStages;
+        ok = warp_wait(&sm.full[s], (g / C::kStages) & 1, failed);
         if (!ok) break;
         fence_after_sync();
-        const uint32_t acc = tmem + static_cast<uint32_t>(b * NT);
-        for (int kb = 0; kb < p.kblocks; ++kb, ++g) {
-          const int s = g % C::kStages;
-          ok = mbar_wait(&sm.full[s], (g / C::kStages) & 1, failed);
-          if (!ok) break;
-          fence_after_sync();
-          const uint32_t a = smem_addr(sm.tiles[s]);
-          const uint32_t bb = a + C::kATile;
+        // a K step of 16 is 32 bytes further on K-major, 16 rows of 128 bytes MN-major (the
+        // descriptors count 16 bytes)
+        const uint32_t base = smem_addr(sm.tiles[s]);
+        const uint64_t da = kAMn ? smem_desc_mn(base) : smem_desc(base);
+        const uint64_t db = kBMn ? smem_desc_mn(base + C::kATile) : smem_desc(base + C::kATile);
+        if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < kGBK / 16; ++k)
-            mma_kind_f16(acc, kAMn ? smem_desc_mn(a + k * 2048) : smem_desc(a + k * 32),
-                         kBMn ? smem_desc_mn(bb + k * 2048) : smem_desc(bb + k * 32), kIdesc,
+            mma_kind_f16(acc, da + k * (kAMn ? 128 : 2), db + k * (kBMn ? 128 : 2), kIdesc,
                          (kb > 0 || k > 0) ? 1u : 0u);
           mma_commit(&sm.empty[s]);
         }
-        if (!ok) break;
-        mma_commit(&sm.acc_full[b]);
       }
-      mma_commit(&sm.drain);
-      mbar_wait_drain(&sm.drain, 0);
+      if (!ok) break;
+      if (elect_one()) mma_commit(&sm.acc_full[b]);
     }
+    if (elect_one()) mma_commit(&sm.drain);
+    mbar_wait_drain(&sm.drain, 0);
   } else {
     // ---- epilogue: one output row per thread
     const int q = warp & 3;
@@ -226,9 +228,8 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
     for (int t = blockIdx.x; t < ntiles; t += gridDim.x, ++i) {
       const int mt = t / p.n_tiles, nt = t - mt * p.n_tiles;
       const int b = i & 1;
-      const bool ok = mbar_wait(&sm.acc_full[b], (i >> 1) & 1, failed);
+      if (!warp_wait(&sm.acc_full[b], (i >> 1) & 1, failed)) break;
       fence_after_sync();
-      if (!ok || *failed) break;
       const int row = mt * kGBM + q * 32 + lane;
       const uint32_t taddr = tmem + static_cast<uint32_t>(b * NT) + ((uint32_t)(q * 32) << 16);
       if (KIND == kForward) {

@@ -23,7 +23,7 @@
 namespace exf {
 using namespace tc;
 
-constexpr int kMxLayerThreads = 384;  // warps 0, 2, 3 TMA, warp 1 MMA, warps 4-11 epilogue
+constexpr int kMxLayerThreads = 416;  // warps 0, 2, 3 TMA, 1 MMA, 4-11 epilogue, 12 schedule
 
 // ---- token rows in route order (more than align_gather_max_numel() routes) -----------------------
 // A warp takes a token: its row is split once and written to the slots of its routes.
@@ -53,73 +53,80 @@ __global__ void __launch_bounds__(256) mx_split_kernel(const __nv_bfloat16* x, c
 }
 
 // ---- decode ---------------------------------------------------------------------------------------
-// A tile is a block of 64 routes (hi and lo rows: the 128 rows of the M side) times 256 weight rows of
-// one expert (the N side).  With the weights on the N side an MMA (128 x 256 x 32) takes 128 cycles for
-// 256 rows and hides the scales' copies to TMEM; on the M side it took 64 cycles for 128 rows
-// whatever the number of routes, and the copies came on top (763 cycles a stage against 525), which
-// held the weight stream at the copy peak's edge.
+// A tile is 256 weight rows of one expert (two MMA tiles of 128 rows on the M side) times a block of
+// BT = 16, 32 or 64 of its routes (the N side: 2 BT hi and lo rows).
 //   GEMM-1 tile (block, f): gate rows [128 f, +128) and up rows [I + 128 f, +128) of W13[e], K = H;
 //     the epilogue forms h = silu(gate) * up and writes its two-term form;
 //   GEMM-2 tile (block, f): rows [256 f, +256) of W2[e], K = I; out[route][256 f + i] = w_route D.
-// One persistent launch: warp 0 takes tiles from a counter (every GEMM-1 tile, then the GEMM-2
-// tiles) and passes them on through a ring.  Three warps load: the first 128 weight rows, the
+// One persistent launch: a scheduler warp takes tiles from a counter (every GEMM-1 tile, then the
+// GEMM-2 tiles) and passes them on through a ring.  Three warps load: the first 128 weight rows, the
 // second, and the token rows, each with its scales (a row of packed codes is a 64-byte request:
 // padded tiles stream at 5.3 TB/s from one issuing thread and at 6.6 from two).  The warp that
 // loads tokens waits, before the first load of a GEMM-2 tile, until the epilogue warps of the
 // block's GEMM-1 tiles have counted themselves off; the weights of such a tile do not wait.  A
-// GEMM-1 tile waits only for earlier tiles of its own CTA and was handed out before every GEMM-2
-// tile, so the wait ends; it is bounded all the same.
+// GEMM-1 tile waits only for earlier GEMM-1 tiles of its own CTA and was handed out before every
+// GEMM-2 tile, so the wait ends; it is bounded all the same.
 //
-// The accumulator (256 TMEM columns) leaves room for the scales but not for a second one: 8
-// epilogue warps sum its two terms into registers and give it back before they compute (computing
-// from it, the epilogue was exposed and took 40 % of the layer).  Scales are loaded for 4 stages at a
-// time, 2 KB a copy: a copy a stage cost as much of the TMA unit as a third of a weight tile.
+// Scales are loaded for several stages at a time: a copy a stage cost as much of the TMA unit as a
+// third of a weight tile.  8 epilogue warps sum the two terms into registers and give the
+// accumulator back before they compute; up to 32 routes there are two.
+//
+// What bounds the layer is the bytes in flight: padded, a stage's 17 KB of codes and scales take
+// 32 KB of shared memory, so the smaller token tiles of 16 and 32 routes buy a stage.
+template <int BT>
 struct MxCfg {
-  static constexpr int kTTile = 128 * kMxK;
+  static constexpr int kN = 2 * BT;
+  static constexpr int kTTile = kN * kMxK;
   static constexpr int kWTile = 128 * kMxK;              // padded codes of 128 rows
-  static constexpr int kStages = 4;
-  static constexpr int kScaleRun = 4;                    // stages a copy of scales serves
+  static constexpr int kStages = BT == 64 ? 4 : 5;
+  static constexpr int kScaleRun = BT == 32 ? 2 : 4;     // stages a copy of scales serves
   static constexpr int kScaleBytes = kScaleRun * 512;
-  static constexpr int kRing = 8;
+  static constexpr int kRing = 4;                        // tiles handed out ahead
+  static constexpr int kAccCols = 2 * kN;
+  static constexpr int kAccs = BT == 64 ? 1 : 2;
+  static constexpr int kScaleCol = kAccs * kAccCols;     // 4 sets of 16 columns
+  static constexpr int kTmemCols = kScaleCol + 64 <= 256 ? 256 : 512;
 };
+struct MxTile {
+  int kind;      // kGate, kDown, or kEnd: no more tiles
+  int blk, ft;
+  int expert;
+  int quarters;  // 32-row quarters of the block that hold routes
+};
+enum { kEnd = -1, kGate = 0, kDown = 1 };
+template <int BT>
 struct MxSmem {
-  alignas(1024) uint8_t tiles[MxCfg::kStages][MxCfg::kTTile + 2 * MxCfg::kWTile];
-  // Slots of scales (token rows, first and second weight rows).  A tile takes the next slot every
-  // kScaleRun stages; as many slots as stages, so that the slot a load overwrites belongs to
-  // stages already released (the loads between cover a stage each, at least).
-  alignas(128) uint8_t scales[MxCfg::kStages][3][MxCfg::kScaleBytes];
-  alignas(8) uint64_t full[MxCfg::kStages];
-  alignas(8) uint64_t empty[MxCfg::kStages];
-  alignas(8) uint64_t acc_full;
-  alignas(8) uint64_t acc_empty;
-  alignas(8) uint64_t ring_full[MxCfg::kRing];
-  alignas(8) uint64_t ring_empty[MxCfg::kRing];
+  using C = MxCfg<BT>;
+  // a stage: 256 rows of codes, token rows
+  alignas(1024) uint8_t tiles[C::kStages][2 * C::kWTile + C::kTTile];
+  // Slots of scales (token rows, first and second weight rows), taken in turn by the runs.  As many
+  // as stages: that many runs later, every stage that used a slot's scales has been released.
+  alignas(128) uint8_t scales[C::kStages][3][C::kScaleBytes];
+  alignas(8) uint64_t full[C::kStages];
+  alignas(8) uint64_t empty[C::kStages];
+  alignas(8) uint64_t acc_full[2];
+  alignas(8) uint64_t acc_empty[2];
+  alignas(8) uint64_t ring_full[C::kRing];
+  alignas(8) uint64_t ring_empty[C::kRing];
   alignas(8) uint64_t drain;
-  int ring[MxCfg::kRing];
+  MxTile ring[C::kRing];
   uint32_t tmem_base;
   int failed;
 };
-constexpr size_t mx_smem_bytes() { return sizeof(MxSmem) + 1024; }
-static_assert(mx_smem_bytes() <= 232448, "decode expert layer shared memory");
+template <int BT>
+constexpr size_t mx_smem_bytes() { return sizeof(MxSmem<BT>) + 1024; }
+static_assert(mx_smem_bytes<16>() <= 232448 && mx_smem_bytes<32>() <= 232448 &&
+                  mx_smem_bytes<64>() <= 232448,
+              "decode expert layer shared memory");
 
-struct MxTile {
-  bool down;
-  int blk;
-  int ft;
+// The scales that come with k block kb of a tile: those of R blocks with every R-th.  First block
+// and bytes (0: none).
+struct ScaleRun {
+  int kb, bytes;
 };
-__device__ __forceinline__ MxTile mx_tile(int t, int blocks, int n1, int n2) {
-  MxTile r;
-  r.down = t >= blocks * n1;
-  if (r.down) t -= blocks * n1;
-  const int n = r.down ? n2 : n1;
-  r.blk = t / n;
-  r.ft = t - r.blk * n;
-  return r;
-}
-
-// bytes of scales from k block kb on that one copy brings
-__device__ __forceinline__ int scale_run(int kblocks, int kb) {
-  return 512 * (kblocks - kb < MxCfg::kScaleRun ? kblocks - kb : MxCfg::kScaleRun);
+template <int R>
+__device__ __forceinline__ ScaleRun scale_run(int kblocks, int kb) {
+  return {kb, kb % R ? 0 : 512 * (kblocks - kb < R ? kblocks - kb : R)};
 }
 
 // After a time-out (else every load has been consumed): copies still in flight land before shared
@@ -140,33 +147,28 @@ __device__ __forceinline__ float silu_up(float g, float u) {
   return __fdividef(g, 1.0f + __expf(-g)) * u;
 }
 
-// Four lanes hold the 16-bit pairs w[0..3] of a row's four groups; lane j of them gets the four
-// lanes' pairs of group j, in lane order: 8 consecutive bytes of the row.
-__device__ __forceinline__ uint2 gather_pairs(const uint32_t (&w)[4], int j) {
-  const bool odd = j & 1, high = j & 2;
-  uint32_t send = odd ? __byte_perm(w[0], w[2], 0x5410) : __byte_perm(w[1], w[3], 0x5410);
-  const uint32_t keep = odd ? __byte_perm(w[1], w[3], 0x5410) : __byte_perm(w[0], w[2], 0x5410);
-  const uint32_t got = __shfl_xor_sync(0xffffffffu, send, 1);
-  // pairs of the groups j % 2 and j % 2 + 2 from this lane and its neighbour, even lane first
-  const uint32_t lo = odd ? __byte_perm(got, keep, 0x5410) : __byte_perm(keep, got, 0x5410);
-  const uint32_t hi = odd ? __byte_perm(got, keep, 0x7632) : __byte_perm(keep, got, 0x7632);
-  const uint32_t other = __shfl_xor_sync(0xffffffffu, high ? lo : hi, 2);
-  return high ? make_uint2(other, hi) : make_uint2(lo, other);
+// N consecutive fp32 columns of this thread's TMEM lane, N = 8 or 16
+template <int N>
+__device__ __forceinline__ void tmem_load_cols(uint32_t taddr, uint32_t (&r)[N]) {
+  if constexpr (N == 8)
+    tmem_load8(taddr, r);
+  else
+    tmem_load16(taddr, r);
 }
 
+template <int BT>
 __global__ void __launch_bounds__(kMxLayerThreads, 1)
     mx_layer_kernel(const __grid_constant__ CUtensorMap map_w13,
                     const __grid_constant__ CUtensorMap map_xq,
                     const __grid_constant__ CUtensorMap map_w2,
                     const __grid_constant__ CUtensorMap map_hq, const MxLayerParams p) {
-  using C = MxCfg;
+  using C = MxCfg<BT>;
   constexpr int kStages = C::kStages;
   constexpr int kRing = C::kRing;
-  constexpr int BT = kMxDecodeBlock;
   extern __shared__ uint8_t smem_raw[];
-  MxSmem& sm = *reinterpret_cast<MxSmem*>(
+  MxSmem<BT>& sm = *reinterpret_cast<MxSmem<BT>*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  const int warp = threadIdx.x >> 5;
+  const int warp = uniform(threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -174,17 +176,25 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
       mbar_init(&sm.full[s], 3);  // one arrival per loading warp
       mbar_init(&sm.empty[s], 1);
     }
-    mbar_init(&sm.acc_full, 1);
-    mbar_init(&sm.acc_empty, 8);
+    for (int b = 0; b < C::kAccs; ++b) {
+      mbar_init(&sm.acc_full[b], 1);
+      mbar_init(&sm.acc_empty[b], 8);
+    }
     for (int j = 0; j < kRing; ++j) {
       mbar_init(&sm.ring_full[j], 1);
-      mbar_init(&sm.ring_empty[j], 11);  // two loading warps, the MMA thread, 8 epilogue warps
+      mbar_init(&sm.ring_empty[j], 12);  // three loading warps, the MMA thread, 8 epilogue warps
     }
     mbar_init(&sm.drain, 1);
     sm.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) tmem_alloc(&sm.tmem_base, 512);
+  if (threadIdx.x == 32) {
+    prefetch_map(&map_w13);
+    prefetch_map(&map_xq);
+    prefetch_map(&map_w2);
+    prefetch_map(&map_hq);
+  }
+  if (warp == 1) tmem_alloc(&sm.tmem_base, C::kTmemCols);
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
@@ -196,264 +206,237 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
   const int n1 = p.inter / 128;
   const int n2 = p.hidden / 256;
   const int total = blocks * (n1 + n2);
-  const uint32_t tmem = sm.tmem_base;
+  const uint32_t tmem = uniform(sm.tmem_base);
   volatile int* failed = &sm.failed;
-  auto expert_of = [&](const MxTile& lt) {
-    const int e = p.routes.expert_ids[lt.blk];
-    return (e >= 0 && e < p.experts) ? e : -1;
-  };
-  // real routes of a block (they come first), by a whole warp
-  auto real_of = [&](int blk) {
-    const int32_t* ids = p.routes.sorted_ids + (int64_t)blk * BT;
-    return __popc(__ballot_sync(0xffffffffu, ids[lane] < p.numel)) +
-           __popc(__ballot_sync(0xffffffffu, ids[32 + lane] < p.numel));
-  };
-  // the next tile from the ring for a whole warp: its number, -1 at the end, -2 after a time-out
-  auto next_tile = [&](int j) {
+  // the next tile from the ring, for a whole warp
+  auto next_tile = [&](int j, MxTile& lt) {
     const int slot = j % kRing;
-    int tile = -2;
-    if (lane == 0 && mbar_wait(&sm.ring_full[slot], (j / kRing) & 1, failed)) {
-      tile = sm.ring[slot];
-      mbar_arrive(&sm.ring_empty[slot]);
-    }
-    return __shfl_sync(0xffffffffu, tile, 0);
+    if (!warp_wait(&sm.ring_full[slot], (j / kRing) & 1, failed)) return false;
+    const MxTile& t = sm.ring[slot];
+    lt = {uniform(t.kind), uniform(t.blk), uniform(t.ft), uniform(t.expert), uniform(t.quarters)};
+    if (lane == 0) mbar_arrive(&sm.ring_empty[slot]);
+    return lt.kind != kEnd;
   };
 
   uint32_t issued = 0;  // stages this thread has loaded into
-  if (warp == 0 || warp == 2) {
-    // ---- weight loads, one thread each: gate (warp 0) and up (warp 2) rows of W13[e], or the
-    // halves of 256 rows of W2[e]; warp 0 also hands out the tiles
-    if (lane == 0) {
-      const int half = warp == 0 ? 0 : 1;
-      uint32_t g = 0, run = 0;  // stages and runs of scales loaded
-      bool ok = true;
-      int t = warp == 0 ? atomicAdd(p.sync, 1) : 0;
-      for (int j = 0; ok; ++j) {
-        const int slot = j % kRing;
-        int tile;
-        if (warp == 0) {
-          tile = t < total ? t : -1;
-          ok = mbar_wait(&sm.ring_empty[slot], ((j / kRing) & 1) ^ 1, failed);
-          if (!ok) break;
-          sm.ring[slot] = tile;
-          mbar_arrive(&sm.ring_full[slot]);
-          if (tile >= 0) t = atomicAdd(p.sync, 1);  // its latency overlaps this tile's loads
-        } else {
-          ok = mbar_wait(&sm.ring_full[slot], (j / kRing) & 1, failed);
-          if (!ok) break;
-          tile = sm.ring[slot];
-          mbar_arrive(&sm.ring_empty[slot]);
-        }
-        if (tile < 0) break;
-        const MxTile lt = mx_tile(tile, blocks, n1, n2);
-        const int expert = expert_of(lt);
-        if (expert < 0) continue;
-        const int kblocks = (lt.down ? p.inter : p.hidden) / kMxK;
-        const int row = lt.down ? expert * p.hidden + lt.ft * 256 + half * 128
-                                : expert * 2 * p.inter + lt.ft * 128 + half * p.inter;
-        const CUtensorMap* map = lt.down ? &map_w2 : &map_w13;
-        const uint8_t* sc = (lt.down ? p.s2 : p.s13) + (int64_t)(row / 128) * kblocks * 512;
-        for (int kb = 0; kb < kblocks; ++kb, ++g) {
-          const int s = g % kStages;
-          ok = mbar_wait(&sm.empty[s], ((g / kStages) & 1) ^ 1, failed);
-          if (!ok) break;
-          const int sb = kb % C::kScaleRun == 0 ? scale_run(kblocks, kb) : 0;
-          mbar_expect_tx(&sm.full[s], C::kWTile / 2 + sb);  // codes count as they lie in memory
-          tma_load_2d(sm.tiles[s] + C::kTTile + half * C::kWTile, map, &sm.full[s], kb * kMxK, row);
-          if (sb) bulk_load(sm.scales[run++ % kStages][1 + half], sc + kb * 512, sb, &sm.full[s]);
+  if (warp == 12) {
+    // ---- scheduler: takes tiles from the counter and looks up what the other roles need to know of
+    // them (each of them doing so for itself lost a memory latency or two at every tile)
+    for (int j = 0;; ++j) {
+      int t = lane == 0 ? atomicAdd(p.sync, 1) : 0;
+      t = __shfl_sync(0xffffffffu, t, 0);
+      MxTile lt{kEnd, 0, 0, 0, 0};
+      if (t < total) {
+        lt.kind = t < blocks * n1 ? kGate : kDown;
+        if (lt.kind == kDown) t -= blocks * n1;
+        const int n = lt.kind == kDown ? n2 : n1;
+        lt.blk = t / n;
+        lt.ft = t - lt.blk * n;
+        lt.expert = p.routes.expert_ids[lt.blk];
+        const int32_t* ids = p.routes.sorted_ids + (int64_t)lt.blk * BT;
+        int real = __popc(__ballot_sync(0xffffffffu, lane < BT && ids[lane] < p.numel));
+        if (BT == 64) real += __popc(__ballot_sync(0xffffffffu, ids[32 + lane] < p.numel));
+        lt.quarters = (real + 15) >> 4;
+        if (lt.expert < 0 || lt.expert >= p.experts) {
+          --j;
+          continue;
         }
       }
-      issued = g;
+      const int slot = j % kRing;
+      if (!warp_wait(&sm.ring_empty[slot], ((j / kRing) & 1) ^ 1, failed)) break;
+      if (lane == 0) {
+        sm.ring[slot] = lt;
+        mbar_arrive(&sm.ring_full[slot]);
+      }
+      if (lt.kind == kEnd) break;
     }
-  } else if (warp == 3) {
-    // ---- token loads: the quarters of the block that hold routes, a lane each
-    uint32_t g = 0, run = 0;
+  } else if (warp == 0 || warp == 2) {
+    // ---- weight loads: gate (warp 0) and up (warp 2) rows of W13[e], or the halves of 256 rows of
+    // W2[e]
+    const int half = warp == 0 ? 0 : 1;
+    uint32_t g = 0, run = 0;  // stages and runs of scales loaded
     bool ok = true;
-    for (int j = 0; ok; ++j) {
-      const int tile = next_tile(j);
-      if (tile < 0) break;
-      const MxTile lt = mx_tile(tile, blocks, n1, n2);
-      if (expert_of(lt) < 0) continue;
-      const int quarters = (real_of(lt.blk) + 15) >> 4;
-      if (lt.down) {
-        const int32_t* flag = p.sync + 1 + lt.blk;
-        uint32_t it = 0;
-        while (ld_acquire_gpu(flag) < 8 * n1) {
-          if (*failed || ++it >= kWaitLimit) {
-            *failed = 1;
-            ok = false;
-            break;
-          }
-          __nanosleep(32);
-        }
-        if (!__all_sync(0xffffffffu, ok)) break;
-        asm volatile("fence.proxy.async.global;" ::: "memory");
-      }
-      const int kblocks = (lt.down ? p.inter : p.hidden) / kMxK;
-      const CUtensorMap* map = lt.down ? &map_hq : &map_xq;
-      const uint8_t* sc = (lt.down ? p.hs : p.xs) + (int64_t)lt.blk * kblocks * 512;
+    MxTile lt;
+    for (int j = 0; ok && next_tile(j, lt); ++j) {
+      const bool down = lt.kind == kDown;
+      const int kblocks = (down ? p.inter : p.hidden) / kMxK;
+      const int row = down ? lt.expert * p.hidden + lt.ft * 256 + half * 128
+                           : lt.expert * 2 * p.inter + lt.ft * 128 + half * p.inter;
+      const CUtensorMap* map = down ? &map_w2 : &map_w13;
+      const uint8_t* sc = (down ? p.s2 : p.s13) + (int64_t)(row / 128) * kblocks * 512;
       for (int kb = 0; kb < kblocks; ++kb, ++g) {
         const int s = g % kStages;
-        ok = mbar_wait(&sm.empty[s], ((g / kStages) & 1) ^ 1, failed);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
+        ok = warp_wait(&sm.empty[s], ((g / kStages) & 1) ^ 1, failed);
+        if (!ok) break;
+        const ScaleRun sr = scale_run<C::kScaleRun>(kblocks, kb);
+        if (elect_one()) {
+          mbar_expect_tx(&sm.full[s], C::kWTile / 2 + sr.bytes);  // codes count as in memory
+          tma_load_2d(sm.tiles[s] + half * C::kWTile, map, &sm.full[s], kb * kMxK, row);
+          if (sr.bytes)
+            bulk_load(sm.scales[run % kStages][1 + half], sc + sr.kb * 512, sr.bytes,
+                      &sm.full[s]);
         }
-        const int sb = kb % C::kScaleRun == 0 ? scale_run(kblocks, kb) : 0;
-        if (lane == 0) mbar_expect_tx(&sm.full[s], quarters * 32 * kMxK + sb);
-        __syncwarp();
-        if (lane < quarters)
-          tma_load_2d(sm.tiles[s] + lane * 32 * kMxK, map, &sm.full[s], kb * kMxK,
-                      lt.blk * 128 + 32 * lane);
-        if (sb) {
-          if (lane == 31) bulk_load(sm.scales[run % kStages][0], sc + kb * 512, sb, &sm.full[s]);
-          ++run;
+        if (sr.bytes) ++run;
+      }
+    }
+    issued = g;
+  } else if (warp == 3) {
+    // ---- token loads: the quarters of the block that hold routes
+    uint32_t g = 0, run = 0;
+    bool ok = true;
+    MxTile lt;
+    for (int j = 0; ok && next_tile(j, lt); ++j) {
+      const bool down = lt.kind == kDown;
+      if (down) {
+        const int32_t* flag = p.sync + 1 + lt.blk;
+        for (uint32_t it = 0; ok && !__all_sync(0xffffffffu, ld_acquire_gpu(flag) >= 8 * n1);) {
+          ok = !__any_sync(0xffffffffu, *failed || ++it >= kWaitLimit);
+          if (!ok) *failed = 1;
+          __nanosleep(32);
         }
+        if (!ok) break;
+        asm volatile("fence.proxy.async.global;" ::: "memory");
+      }
+      const int kblocks = (down ? p.inter : p.hidden) / kMxK;
+      const CUtensorMap* map = down ? &map_hq : &map_xq;
+      const uint8_t* sc = (down ? p.hs : p.xs) + (int64_t)lt.blk * kblocks * 512;
+      for (int kb = 0; kb < kblocks; ++kb, ++g) {
+        const int s = g % kStages;
+        ok = warp_wait(&sm.empty[s], ((g / kStages) & 1) ^ 1, failed);
+        if (!ok) break;
+        const ScaleRun sr = scale_run<C::kScaleRun>(kblocks, kb);
+        if (elect_one()) {
+          mbar_expect_tx(&sm.full[s], lt.quarters * 32 * kMxK + sr.bytes);
+          for (int q = 0; q < lt.quarters; ++q)
+            tma_load_2d(sm.tiles[s] + 2 * C::kWTile + q * 32 * kMxK, map, &sm.full[s],
+                        kb * kMxK, lt.blk * 2 * BT + 32 * q);
+          if (sr.bytes)
+            bulk_load(sm.scales[run % kStages][0], sc + sr.kb * 512, sr.bytes, &sm.full[s]);
+        }
+        if (sr.bytes) ++run;
       }
     }
     issued = g;
   } else if (warp == 1) {
-    // ---- MMA issuer; scale sets rotate over 4 groups of 16 TMEM columns from 256 on
-    if (lane == 0) {
-      uint32_t g = 0, run = 0;
-      int i = 0;
-      bool ok = true;
-      for (int j = 0; ok; ++j) {
-        const int slot = j % kRing;
-        ok = mbar_wait(&sm.ring_full[slot], (j / kRing) & 1, failed);
-        if (!ok) break;
-        const int tile = sm.ring[slot];
-        mbar_arrive(&sm.ring_empty[slot]);
-        if (tile < 0) break;
-        const MxTile lt = mx_tile(tile, blocks, n1, n2);
-        if (expert_of(lt) < 0) continue;
-        const int kblocks = (lt.down ? p.inter : p.hidden) / kMxK;
-        ok = mbar_wait(&sm.acc_empty, (i & 1) ^ 1, failed);
+    // ---- MMA issuer; scale sets rotate over 4 groups of 16 TMEM columns
+    uint32_t g = 0, run = 0;
+    int i = 0;
+    bool ok = true;
+    MxTile lt;
+    for (int j = 0; ok && next_tile(j, lt); ++j) {
+      const int kblocks = (lt.kind == kDown ? p.inter : p.hidden) / kMxK;
+      const int b = i % C::kAccs;
+      ok = warp_wait(&sm.acc_empty[b], ((i / C::kAccs) & 1) ^ 1, failed);
+      if (!ok) break;
+      fence_after_sync();
+      const uint32_t acc = tmem + static_cast<uint32_t>(b * C::kAccCols);
+      for (int kb = 0; kb < kblocks; ++kb, ++g) {
+        const int s = g % kStages;
+        ok = warp_wait(&sm.full[s], (g / kStages) & 1, failed);
         if (!ok) break;
         fence_after_sync();
-        for (int kb = 0; kb < kblocks; ++kb, ++g) {
-          const int s = g % kStages;
-          ok = mbar_wait(&sm.full[s], (g / kStages) & 1, failed);
-          if (!ok) break;
-          fence_after_sync();
-          const uint32_t a = smem_addr(sm.tiles[s]);
-          const uint32_t b = a + C::kTTile;
-          if (kb % C::kScaleRun == 0) ++run;
-          const uint32_t sc =
-              smem_addr(sm.scales[(run - 1) % kStages][0]) + (kb % C::kScaleRun) * 512;
-          const uint32_t sf = tmem + 256 + (g & 3) * 16;
-          tmem_copy_scales(sf, sc);
-          tmem_copy_scales(sf + 8, sc + C::kScaleBytes);
-          tmem_copy_scales(sf + 12, sc + 2 * C::kScaleBytes);
+        const uint64_t w0 = smem_desc(smem_addr(sm.tiles[s]));
+        const uint64_t w1 = w0 + C::kWTile / 16, t0 = w0 + 2 * C::kWTile / 16;
+        if (kb % C::kScaleRun == 0) ++run;
+        const uint32_t sc =
+            smem_addr(sm.scales[(run - 1) % kStages][0]) + (kb % C::kScaleRun) * 512;
+        const uint32_t sf = tmem + C::kScaleCol + (g & 3) * 16;
+        if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_mx(tmem, smem_desc(a + k * 32), smem_desc(b + k * 32),
-                   idesc_mx(128, 256, kMxE4M3, kMxE2M1, k), sf, sf + 8,
-                   (kb > 0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < 3; ++k) tmem_copy_scales(sf + 4 * k, sc + k * C::kScaleBytes);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // a K step is 32 bytes further on: 2 in the descriptor
+            const uint32_t on = (kb > 0 || k > 0) ? 1u : 0u;
+            const uint32_t id = idesc_mx(128, C::kN, kMxE2M1, kMxE4M3, k);
+            mma_mx(acc, w0 + 2 * k, t0 + 2 * k, id, sf + 4, sf, on);
+            mma_mx(acc + C::kN, w1 + 2 * k, t0 + 2 * k, id, sf + 8, sf, on);
+          }
           mma_commit(&sm.empty[s]);
         }
-        if (!ok) break;
-        mma_commit(&sm.acc_full);
-        ++i;
       }
-      mma_commit(&sm.drain);
-      mbar_wait_drain(&sm.drain, 0);
+      if (!ok) break;
+      if (elect_one()) mma_commit(&sm.acc_full[b]);
+      ++i;
     }
+    if (elect_one()) mma_commit(&sm.drain);
+    mbar_wait_drain(&sm.drain, 0);
   } else {
-    // ---- epilogue: a warp has the 16 routes of quarter q (hi in TMEM lanes 32 q .. +15, lo in the
-    // next 16) and half the columns: gate and up of features [64 hf, +64), or output columns
-    // [64 hf, +64) and [128 + 64 hf, +64).  Read as 16 x 32 fragments, a lane has routes l / 4 and
-    // l / 4 + 8 and two neighbouring columns of every 8, both terms at the same place.
+    // ---- epilogue: a warp has 32 weight rows of each MMA tile (TMEM lanes 32 q .. +31) and half of
+    // the block's routes, in chunks of 16 (of 8 where a block has 16); in the columns of 16 routes
+    // the hi rows come first, then the lo rows
+    constexpr int kChunk = BT == 16 ? 8 : 16;
+    constexpr int kChunks = BT / 2 / kChunk;
     const int q = warp & 3, hf = (warp - 4) >> 2;
-    const int quad = lane & 3;
     int i = 0;
-    for (int j = 0;; ++j) {
-      const int tile = next_tile(j);
-      if (tile < 0) break;
-      const MxTile lt = mx_tile(tile, blocks, n1, n2);
-      if (expert_of(lt) < 0) continue;
-      int r[2], route[2];
-      float wr[2];
-#pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        r[z] = 16 * q + (lane >> 2) + 8 * z;
-        route[z] = p.routes.sorted_ids[lt.blk * BT + r[z]];
-        wr[z] = lt.down && route[z] < p.numel ? p.route_w[route[z]] : 0.0f;
-      }
-      const bool on[2] = {route[0] < p.numel, route[1] < p.numel};
-      const bool any = __any_sync(0xffffffffu, on[0]);  // routes fill their quarter from place 0
-      const bool any8 = __any_sync(0xffffffffu, on[1]);
-      const bool ok = mbar_wait(&sm.acc_full, i & 1, failed);
+    MxTile lt;
+    for (int j = 0; next_tile(j, lt); ++j) {
+      const bool down = lt.kind == kDown;
+      // lane l looks after route l of the warp's half
+      const int r0 = hf * (BT / 2);
+      const int route_l = lane < BT / 2 ? p.routes.sorted_ids[lt.blk * BT + r0 + lane] : p.numel;
+      const float w_l = down && route_l < p.numel ? p.route_w[route_l] : 0.0f;
+      const int real = __popc(__ballot_sync(0xffffffffu, route_l < p.numel));  // they come first
+      const int b = i % C::kAccs;
+      if (!warp_wait(&sm.acc_full[b], (i / C::kAccs) & 1, failed)) break;
       fence_after_sync();
-      if (!__all_sync(0xffffffffu, ok && !*failed)) break;
-      float v[4][16];  // runs of 32 columns
-      if (any) {
-        const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
+      float v0[kChunks][kChunk], v1[kChunks][kChunk];  // gate and up, or rows r and r + 128
+      const uint32_t taddr =
+          tmem + static_cast<uint32_t>(b * C::kAccCols) + ((uint32_t)(q * 32) << 16);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const uint32_t col = 128 * (b >> 1) + 64 * hf + 32 * (b & 1);
-          uint32_t hi[16], lo[16];
-          tmem_load_16x32(lanes + col, hi);
-          tmem_load_16x32(lanes + (16u << 16) + col, lo);
-          tmem_wait();
+      for (int c = 0; c < kChunks; ++c) {
+        if (c * kChunk >= real) break;
+        const int r = r0 + c * kChunk;
+        const uint32_t col = taddr + 32 * (r >> 4) + (r & 15);
+        uint32_t a0[kChunk], a1[kChunk], b0[kChunk], b1[kChunk];
+        tmem_load_cols<kChunk>(col, a0);
+        tmem_load_cols<kChunk>(col + 16, a1);
+        tmem_load_cols<kChunk>(col + C::kN, b0);
+        tmem_load_cols<kChunk>(col + C::kN + 16, b1);
+        tmem_wait();
 #pragma unroll
-          for (int n = 0; n < 16; ++n) v[b][n] = __uint_as_float(hi[n]) + __uint_as_float(lo[n]);
+        for (int n = 0; n < kChunk; ++n) {
+          v0[c][n] = __uint_as_float(a0[n]) + __uint_as_float(a1[n]);
+          v1[c][n] = __uint_as_float(b0[n]) + __uint_as_float(b1[n]);
         }
       }
       fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.acc_empty);
+      if (lane == 0) mbar_arrive(&sm.acc_empty[b]);
       ++i;
-      if (any && !lt.down) {
+      if (!down) {
+        const int feat = lt.ft * 128 + q * 32 + lane;  // the warp's features: one scale block
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {  // scale blocks of 32 features
-          const int feat = lt.ft * 128 + 64 * hf + 32 * b;
+        for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            if (z == 1 && !any8) break;
-            float h[8];
-            uint32_t top = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int n = 4 * (e >> 1) + 2 * z + (e & 1);
-              h[e] = silu_up(v[b][n], v[2 + b][n]);
-              top = max(top, __float_as_uint(h[e]) & 0x7fffffffu);
-            }
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const uint32_t sb = split_scale(top);
-            const float inv = split_inverse(sb);
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) split2(h[2 * e], h[2 * e + 1], inv, hi[e], lo[e]);
-            const uint2 hv = gather_pairs(hi, quad), lv = gather_pairs(lo, quad);
-            if (on[z]) {
-              const int n = mx_row(BT, r[z]);
-              uint8_t* at = p.hq + ((int64_t)lt.blk * 128 + n) * p.inter + feat + 8 * quad;
-              *reinterpret_cast<uint2*>(at) = hv;
-              *reinterpret_cast<uint2*>(at + (int64_t)mx_lo(BT) * p.inter) = lv;
-              if (quad < 2)
-                p.hs[scale_at(lt.blk, p.inter / kMxK, feat >> 5, quad ? n + mx_lo(BT) : n)] =
-                    (uint8_t)(quad ? split_lo_byte(sb) : sb);
-            }
+          for (int n = 0; n < kChunk; ++n) {
+            if (c * kChunk + n >= real) break;
+            const float h = silu_up(v0[c][n], v1[c][n]);
+            const uint32_t sb = split_scale(
+                __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu));
+            uint32_t hi, lo;
+            split2(h, 0.0f, split_inverse(sb), hi, lo);
+            const int row = mx_row(BT, r0 + c * kChunk + n);
+            uint8_t* at = p.hq + ((int64_t)lt.blk * C::kN + row) * p.inter + feat;
+            at[0] = (uint8_t)hi;
+            at[(int64_t)mx_lo(BT) * p.inter] = (uint8_t)lo;
+            if (lane < 2)
+              p.hs[scale_at(lt.blk, p.inter / kMxK, feat >> 5, lane ? row + mx_lo(BT) : row)] =
+                  (uint8_t)(lane ? split_lo_byte(sb) : sb);
           }
-        }
-      } else if (any) {
+      } else {
+        float* o = p.out + lt.ft * 256 + q * 32 + lane;
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          if (!on[z]) continue;
-          float* o = p.out + (int64_t)route[z] * p.hidden + lt.ft * 256 + 64 * hf + 2 * quad;
+        for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int n = 4 * e + 2 * z;
-              *reinterpret_cast<float2*>(o + 128 * (b >> 1) + 32 * (b & 1) + 8 * e) =
-                  make_float2(v[b][n] * wr[z], v[b][n + 1] * wr[z]);
-            }
-        }
+          for (int n = 0; n < kChunk; ++n) {
+            if (c * kChunk + n >= real) break;
+            const int64_t route = __shfl_sync(0xffffffffu, route_l, c * kChunk + n);
+            const float wr = __shfl_sync(0xffffffffu, w_l, c * kChunk + n);
+            o[route * p.hidden] = v0[c][n] * wr;
+            o[route * p.hidden + 128] = v1[c][n] * wr;
+          }
       }
-      if (!lt.down) {
+      if (!down) {
         // visible to the TMA loads of the block's GEMM-2 tiles, in any CTA; then count the warp off
         asm volatile("fence.proxy.async.global;" ::: "memory");
         __threadfence();
@@ -467,7 +450,7 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
   if (warp == 1) {
     __syncwarp();
     fence_after_sync();
-    tmem_free(tmem, 512);
+    tmem_free(tmem, C::kTmemCols);
   }
   if (sm.failed) {
     drain_loads<kStages>(sm.full, issued);
@@ -520,7 +503,7 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   MxGemmSmem& sm = *reinterpret_cast<MxGemmSmem*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  const int warp = threadIdx.x >> 5;
+  const int warp = uniform(threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -546,39 +529,39 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
   const int n_tiles = DOWN ? p.hidden / 256 : p.inter / 128;
   const int kblocks = (DOWN ? p.inter : p.hidden) / kMxK;
   const int total = blocks * n_tiles;
-  const uint32_t tmem = sm.tmem_base;
+  const uint32_t tmem = uniform(sm.tmem_base);
   volatile int* failed = &sm.failed;
   auto expert_of = [&](int blk) {
     const int e = p.routes.expert_ids[blk];
-    return (e >= 0 && e < p.experts) ? e : -1;
+    return uniform((e >= 0 && e < p.experts) ? e : -1);
   };
 
   uint32_t issued = 0;
   if (warp == 0 || warp == 2 || warp == 3) {
     // ---- loads: warp 0 the hi and lo rows, warps 2 and 3 a weight tile each
-    if (lane == 0) {
-      uint32_t g = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-        const int blk = t / n_tiles, ft = t - blk * n_tiles;
-        const int expert = expert_of(blk);
-        if (expert < 0) continue;
-        const int half = warp - 2;
-        const int row = DOWN ? expert * p.hidden + ft * 256 + half * 128
-                             : expert * 2 * p.inter + ft * 128 + half * p.inter;
-        const uint8_t* sc =
-            warp == 0 ? (DOWN ? p.hs : p.xs) + (int64_t)blk * 2 * kblocks * 512
-                      : (DOWN ? p.s2 : p.s13) + (int64_t)(row / 128) * kblocks * 512;
-        for (int kb = 0; kb < kblocks; ++kb, ++g) {
-          const int s = g % kMxGemmStages;
-          ok = mbar_wait(&sm.empty[s], ((g / kMxGemmStages) & 1) ^ 1, failed);
-          if (!ok) break;
-          uint64_t* bar = &sm.full[s];
+    uint32_t g = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      const int blk = t / n_tiles, ft = t - blk * n_tiles;
+      const int expert = expert_of(blk);
+      if (expert < 0) continue;
+      const int half = warp - 2;
+      const int row = DOWN ? expert * p.hidden + ft * 256 + half * 128
+                           : expert * 2 * p.inter + ft * 128 + half * p.inter;
+      const uint8_t* sc = warp == 0
+                              ? (DOWN ? p.hs : p.xs) + (int64_t)blk * 2 * kblocks * 512
+                              : (DOWN ? p.s2 : p.s13) + (int64_t)(row / 128) * kblocks * 512;
+      for (int kb = 0; kb < kblocks; ++kb, ++g) {
+        const int s = g % kMxGemmStages;
+        ok = warp_wait(&sm.empty[s], ((g / kMxGemmStages) & 1) ^ 1, failed);
+        if (!ok) break;
+        uint64_t* bar = &sm.full[s];
+        if (elect_one()) {
           if (warp == 0) {
             mbar_expect_tx(bar, 2 * kTile + 1024);
             tma_load_2d(sm.tiles[s], &map_t, bar, kb * kMxK, blk * 256);
             bulk_load(sm.scales[s], sc + kb * 512, 512, bar);
-            bulk_load(sm.scales[s] + 512, sc + (kblocks + kb) * 512, 512, bar);
+            bulk_load(sm.scales[s] + 512, sc + (int64_t)(kblocks + kb) * 512, 512, bar);
           } else {
             mbar_expect_tx(bar, kTile / 2 + 512);
             tma_load_2d(sm.tiles[s] + (2 + half) * kTile, &map_w, bar, kb * kMxK, row);
@@ -586,47 +569,45 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
           }
         }
       }
-      issued = g;
     }
+    issued = g;
   } else if (warp == 1) {
     // ---- MMA issuer
-    if (lane == 0) {
-      uint32_t g = 0;
-      int i = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-        if (expert_of(t / n_tiles) < 0) continue;
-        ok = mbar_wait(&sm.acc_empty, (i & 1) ^ 1, failed);
+    uint32_t g = 0;
+    int i = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      if (expert_of(t / n_tiles) < 0) continue;
+      ok = warp_wait(&sm.acc_empty, (i & 1) ^ 1, failed);
+      if (!ok) break;
+      fence_after_sync();
+      for (int kb = 0; kb < kblocks; ++kb, ++g) {
+        const int s = g % kMxGemmStages;
+        ok = warp_wait(&sm.full[s], (g / kMxGemmStages) & 1, failed);
         if (!ok) break;
         fence_after_sync();
-        for (int kb = 0; kb < kblocks; ++kb, ++g) {
-          const int s = g % kMxGemmStages;
-          ok = mbar_wait(&sm.full[s], (g / kMxGemmStages) & 1, failed);
-          if (!ok) break;
-          fence_after_sync();
-          const uint32_t a = smem_addr(sm.tiles[s]);
-          const uint32_t b = a + 2 * kTile;
-          const uint32_t sc = smem_addr(sm.scales[s]);
-          const uint32_t sf = tmem + 256 + (g & 3) * 16;
+        const uint64_t hi = smem_desc(smem_addr(sm.tiles[s]));
+        const uint64_t lo = hi + kTile / 16, w = hi + 2 * kTile / 16;
+        const uint32_t sc = smem_addr(sm.scales[s]);
+        const uint32_t sf = tmem + 256 + (g & 3) * 16;
+        if (elect_one()) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) tmem_copy_scales(sf + 4 * j, sc + 512 * j);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t id = idesc_mx(128, 256, kMxE4M3, kMxE2M1, k);
-            mma_mx(tmem, smem_desc(a + k * 32), smem_desc(b + k * 32), id, sf, sf + 8,
-                   (kb > 0 || k > 0) ? 1u : 0u);
-            mma_mx(tmem, smem_desc(a + kTile + k * 32), smem_desc(b + k * 32), id, sf + 4, sf + 8,
-                   1u);
+            mma_mx(tmem, hi + 2 * k, w + 2 * k, id, sf, sf + 8, (kb > 0 || k > 0) ? 1u : 0u);
+            mma_mx(tmem, lo + 2 * k, w + 2 * k, id, sf + 4, sf + 8, 1u);
           }
           mma_commit(&sm.empty[s]);
         }
-        if (!ok) break;
-        mma_commit(&sm.acc_full);
-        ++i;
       }
-      mma_commit(&sm.drain);
-      mbar_wait_drain(&sm.drain, 0);
+      if (!ok) break;
+      if (elect_one()) mma_commit(&sm.acc_full);
+      ++i;
     }
+    if (elect_one()) mma_commit(&sm.drain);
+    mbar_wait_drain(&sm.drain, 0);
   } else {
     // ---- epilogue: warp w has TMEM lanes 32 (w % 4) .. +31 and half the columns; a row a thread
     const int q = warp & 3;
@@ -638,9 +619,8 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
       const int r = q * 32 + lane;
       const int route = p.routes.sorted_ids[blk * 128 + r];
       const bool real = route < p.numel;
-      const bool ok = mbar_wait(&sm.acc_full, i & 1, failed);
+      if (!warp_wait(&sm.acc_full, i & 1, failed)) break;
       fence_after_sync();
-      if (!__all_sync(0xffffffffu, ok && !*failed)) break;
       const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
       // columns [64 hf, +64) and [128 + 64 hf, +64): 64 features' gate and up, or two runs of 64
       // output columns
@@ -755,10 +735,14 @@ __global__ void __launch_bounds__(256, 4)
 }
 
 // ---- host side ---------------------------------------------------------------------------------
-// The route block, which also picks the kernels: 64 routes while the average expert's fit with
-// room for the fuller ones (an expert's second block reads its weights again), else 128.
+// The route block, which also picks the kernels: 16, 32 or 64 routes (decode) while the average
+// expert's fit with room for the fuller ones (an expert's second block reads its weights again),
+// else 128 (prefill).
 static int mx_block(int64_t numel, int experts) {
-  return numel <= (int64_t)experts * 44 ? kMxDecodeBlock : kMxPrefillBlock;
+  return numel <= (int64_t)experts * 5    ? 16
+         : numel <= (int64_t)experts * 18 ? 32
+         : numel <= (int64_t)experts * 44 ? 64
+                                          : kMxPrefillBlock;
 }
 
 static int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
@@ -820,7 +804,9 @@ static MxLayerParams layer_params(const MxArgs& a, const MxWorkspace& w) {
   p.inter = a.inter;
   p.m_blocks = (int)(w.capacity / w.block);
   p.status = a.status;
+  p.w13 = a.w13;
   p.s13 = a.s13;
+  p.w2 = a.w2;
   p.s2 = a.s2;
   p.xs = w.xs;
   p.hq = w.hq;
@@ -831,10 +817,12 @@ static MxLayerParams layer_params(const MxArgs& a, const MxWorkspace& w) {
   return p;
 }
 
+template <int BT>
 static cudaError_t launch_mx_layer(const MxArgs& a, const MxWorkspace& w, cudaStream_t s) {
+  auto* kern = mx_layer_kernel<BT>;
   static std::mutex mu;
   static bool done[64] = {};
-  const cudaError_t e = allow_smem(mx_layer_kernel, mx_smem_bytes(), mu, done);
+  const cudaError_t e = allow_smem(kern, mx_smem_bytes<BT>(), mu, done);
   if (e != cudaSuccess) return e;
   CUtensorMap m13, mx, m2, mh;
   if (!make_map_4bit(&m13, a.w13, (uint64_t)a.experts * 2 * a.inter, a.hidden, 128) ||
@@ -843,8 +831,8 @@ static cudaError_t launch_mx_layer(const MxArgs& a, const MxWorkspace& w, cudaSt
       !make_map_8bit(&mh, w.hq, 2 * w.capacity, a.inter, 32))
     return cudaErrorInvalidValue;
   const int sms = sm_count();
-  return launch_pdl(mx_layer_kernel, sms > 0 ? (unsigned)sms : 1u, kMxLayerThreads,
-                    mx_smem_bytes(), s, m13, mx, m2, mh, layer_params(a, w));
+  return launch_pdl(kern, sms > 0 ? (unsigned)sms : 1u, kMxLayerThreads, mx_smem_bytes<BT>(), s,
+                    m13, mx, m2, mh, layer_params(a, w));
 }
 
 template <bool DOWN>
@@ -894,7 +882,9 @@ cudaError_t launch_mx_experts(const MxArgs& a, const MxWorkspace& w, cudaStream_
     e = launch_mx_gemm<false>(a, w, s);
     if (e == cudaSuccess) e = launch_mx_gemm<true>(a, w, s);
   } else {
-    e = launch_mx_layer(a, w, s);
+    e = w.block == 16   ? launch_mx_layer<16>(a, w, s)
+        : w.block == 32 ? launch_mx_layer<32>(a, w, s)
+                        : launch_mx_layer<64>(a, w, s);
   }
   if (e != cudaSuccess) return e;
   return launch_pdl(mx_combine_kernel, stream_grid(a.tokens * (a.hidden / 4)), 256, 0, s,
