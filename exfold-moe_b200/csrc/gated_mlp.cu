@@ -92,7 +92,7 @@ struct GatedCfg {
   static constexpr int kBTile = NT * kGBK * 2;
   static constexpr int kStage = kATile + kBTile;
   static constexpr int kStages = (196 * 1024) / kStage;
-  static constexpr int kTmem = 2 * NT;
+  static constexpr int kTmem = 2 * NT;                 // two accumulators, a power of two
 };
 template <int NT>
 struct GatedSmem {
@@ -294,6 +294,67 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
   if (threadIdx.x == 0 && sm.failed && p.status) atomicExch(p.status, 1);
 }
 
+// ---- a few tokens ------------------------------------------------------------------------------
+// Up to 8 tokens: a warp computes one feature (a gate and an up row against every token) with fp32
+// FMAs, so that every SM streams weights; an MMA tile would be 1/16 full and 128 features wide.
+// Bound by the weights' latency and bytes.  TT: tokens rounded up to a power of two.
+constexpr int kFewTokens = 8;
+constexpr int kFewWarps = 4;
+
+template <bool BF16, int TT>
+__global__ void __launch_bounds__(32 * kFewWarps)
+    gated_few_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ w13, int tokens,
+                     int hidden, int inter, int activation, uint16_t* h, float* pre) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int f = blockIdx.x * kFewWarps + (threadIdx.x >> 5);
+  if (f >= inter) return;
+  const uint4* wg = reinterpret_cast<const uint4*>(w13 + (int64_t)f * hidden);
+  const uint4* wu = reinterpret_cast<const uint4*>(w13 + (int64_t)(inter + f) * hidden);
+  const int vecs = hidden / 8;
+  float g[TT] = {}, u[TT] = {};
+#pragma unroll 4
+  for (int c = lane; c < vecs; c += 32) {
+    const uint4 a = __ldg(wg + c), b = __ldg(wu + c);
+    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      // (rows past the last token read it again; their sums are not stored)
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(
+                                x + (int64_t)(t < tokens ? t : tokens - 1) * hidden) + c);
+      const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 xv = unpack2<BF16>(vw[j]), av = unpack2<BF16>(aw[j]),
+                     bv = unpack2<BF16>(bw[j]);
+        g[t] = fmaf(xv.x, av.x, g[t]);
+        g[t] = fmaf(xv.y, av.y, g[t]);
+        u[t] = fmaf(xv.x, bv.x, u[t]);
+        u[t] = fmaf(xv.y, bv.y, u[t]);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+      g[t] += __shfl_xor_sync(0xffffffffu, g[t], d);
+      u[t] += __shfl_xor_sync(0xffffffffu, u[t], d);
+    }
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    if (lane != t || t >= tokens) continue;
+    const float s = activation == kSilu ? gate_sigmoid<kSilu>(g[t]) : gate_sigmoid<kGeluTanh>(g[t]);
+    const uint32_t v = pack2<BF16>(g[t] * s * u[t], 0.0f);
+    h[(int64_t)t * inter + f] = (uint16_t)v;
+    if (pre) {
+      pre[(int64_t)t * 2 * inter + f] = g[t];
+      pre[(int64_t)t * 2 * inter + inter + f] = u[t];
+    }
+  }
+}
+
 // ---- the elementwise part of backward -----------------------------------------------------------
 // both [tokens][2 * inter] = (dh * U * act'(G), dh * act(G)); 8 columns a thread.
 template <bool BF16, int ACT>
@@ -368,9 +429,35 @@ static cudaError_t forward_nt(const GatedArgs& a, void* h, float* pre, cudaStrea
   return launch_gemm<kForward, NT, BF16>(ma, mb, p, s);
 }
 
+// The N tile: 256, halved while the tiles leave more than half of the SMs idle (a narrower tile reads
+// its A rows again for fewer columns, and starts as many more CTAs).
+static int pick_nt(int64_t m, int64_t n256) {  // n256: N tiles of 256 columns, in 64ths
+  const int64_t m_tiles = (m + kGBM - 1) / kGBM;
+  const int sms = sm_count();
+  if (m_tiles * ((n256 + 63) / 64) * 2 > sms) return 256;
+  return m_tiles * ((n256 + 31) / 32) * 2 > sms ? 128 : 64;
+}
+
+template <bool BF16, int TT>
+static cudaError_t forward_few(const GatedArgs& a, void* h, float* pre, cudaStream_t s) {
+  return launch_pdl(gated_few_kernel<BF16, TT>, (unsigned)ceil_div(a.inter, kFewWarps),
+                    32 * kFewWarps, 0, s, static_cast<const uint16_t*>(a.x),
+                    static_cast<const uint16_t*>(a.w13), (int)a.tokens, a.hidden, a.inter,
+                    a.activation, static_cast<uint16_t*>(h), pre);
+}
+
 template <bool BF16>
 static cudaError_t forward_t(const GatedArgs& a, void* h, float* pre, cudaStream_t s) {
-  return forward_nt<256, BF16>(a, h, pre, s);
+  if (a.tokens <= kFewTokens)
+    return a.tokens == 1   ? forward_few<BF16, 1>(a, h, pre, s)
+           : a.tokens == 2 ? forward_few<BF16, 2>(a, h, pre, s)
+           : a.tokens <= 4 ? forward_few<BF16, 4>(a, h, pre, s)
+                           : forward_few<BF16, 8>(a, h, pre, s);
+  switch (pick_nt(a.tokens, ceil_div(a.inter, 2))) {
+    case 256: return forward_nt<256, BF16>(a, h, pre, s);
+    case 128: return forward_nt<128, BF16>(a, h, pre, s);
+    default: return forward_nt<64, BF16>(a, h, pre, s);
+  }
 }
 
 template <int NT, bool BF16>
@@ -410,8 +497,16 @@ static cudaError_t backward_t(const GatedArgs& a, const void* dh, const float* p
                                       : gated_slope_kernel<BF16, kGeluTanh>;
   cudaError_t e = launch_pdl(slope, (unsigned)blocks, 256, 0, s, static_cast<const uint16_t*>(dh),
                              pre, a.tokens, a.inter, static_cast<uint16_t*>(both));
-  if (e == cudaSuccess && dx) e = grad_x<256, BF16>(a, both, dx, s);
-  if (e == cudaSuccess && dw13) e = grad_w<256, BF16>(a, both, dw13, s);
+  if (e == cudaSuccess && dx) switch (pick_nt(a.tokens, ceil_div(a.hidden, 4))) {
+      case 256: e = grad_x<256, BF16>(a, both, dx, s); break;
+      case 128: e = grad_x<128, BF16>(a, both, dx, s); break;
+      default: e = grad_x<64, BF16>(a, both, dx, s);
+    }
+  if (e == cudaSuccess && dw13) switch (pick_nt(2 * (int64_t)a.inter, ceil_div(a.hidden, 4))) {
+      case 256: e = grad_w<256, BF16>(a, both, dw13, s); break;
+      case 128: e = grad_w<128, BF16>(a, both, dw13, s); break;
+      default: e = grad_w<64, BF16>(a, both, dw13, s);
+    }
   return e;
 }
 
