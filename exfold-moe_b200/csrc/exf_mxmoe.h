@@ -30,7 +30,8 @@ struct MxLayerParams {
   uint8_t* hq;                  // GEMM-1 output in the same form
   uint8_t* hs;
   const float* route_w;
-  float* out;                   // GEMM-2 output [numel][hidden]
+  float* out;                   // GEMM-2 output [numel][hidden]; prefill: 16-bit multiples of
+  uint8_t* out_scale;           // the powers in [numel][hidden / 32]
   int32_t* sync;                // [0] next tile; [1 + b] GEMM-1 epilogue warps done with block b
 };
 
@@ -64,6 +65,7 @@ struct MxWorkspace {
   uint8_t* hq;
   uint8_t* hs;
   float* out;
+  uint8_t* out_scale;
   int32_t* sync;
   int sync_ints;
   int64_t bytes;

@@ -484,14 +484,25 @@ struct MxGemmSmem {
 constexpr size_t mx_gemm_smem_bytes() { return sizeof(MxGemmSmem) + 1024; }
 static_assert(mx_gemm_smem_bytes() <= 232448, "prefill expert GEMM shared memory");
 
-// 8 values times w, a whole 32-byte sector in one store (two 16-byte stores of a row a thread each
-// cost L2 a partial write)
-__device__ __forceinline__ void store_sector(float* at, const uint32_t* v, float w) {
-  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at),
-               "f"(__uint_as_float(v[0]) * w), "f"(__uint_as_float(v[1]) * w),
-               "f"(__uint_as_float(v[2]) * w), "f"(__uint_as_float(v[3]) * w),
-               "f"(__uint_as_float(v[4]) * w), "f"(__uint_as_float(v[5]) * w),
-               "f"(__uint_as_float(v[6]) * w), "f"(__uint_as_float(v[7]) * w)
+// The route outputs at prefill, 16-bit: 32 columns share 2^(byte - 127), above their largest
+// magnitude; a value is a signed 16-bit multiple of 2^(byte - 142), within 2^-16 of that power
+// (bf16 route outputs would add as much error as the result's own rounding, fp32 ones held GEMM-2
+// and the combine to the memory's speed).  Byte 255: NaN.
+__device__ __forceinline__ uint32_t half_scale(uint32_t top_bits) {
+  const uint32_t e = (top_bits >> 23) + 1;
+  return top_bits >= 0x7f800000u ? 255u : (e < 16 ? 16u : e);
+}
+// 16 values -> 16 multiples, one 32-byte sector
+__device__ __forceinline__ void store_halves(int16_t* at, const uint32_t* v, float w, float inv) {
+  uint32_t o[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int a = max(min(__float2int_rn(__uint_as_float(v[2 * j]) * w * inv), 32767), -32767);
+    const int b = max(min(__float2int_rn(__uint_as_float(v[2 * j + 1]) * w * inv), 32767), -32767);
+    o[j] = __byte_perm(a, b, 0x5410);
+  }
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(o[0]),
+               "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
                : "memory");
 }
 
@@ -638,12 +649,23 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
       if (DOWN) {
         if (real) {
           const float wr = p.route_w[route];
-          float* o = p.out + (int64_t)route * p.hidden + ft * 256 + 64 * hf;
+          const int64_t at = (int64_t)route * p.hidden + ft * 256 + 64 * hf;
+          int16_t* o = reinterpret_cast<int16_t*>(p.out);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+          for (int b = 0; b < 4; ++b) {  // runs of 32 columns
+            uint32_t top = 0;
 #pragma unroll
-            for (int c = 0; c < 16; c += 8)
-              store_sector(o + (j >> 2) * 128 + (j & 3) * 16 + c, &v[j][c], wr);
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int c = 0; c < 16; ++c)
+                top = max(top, __float_as_uint(__uint_as_float(v[2 * b + j][c]) * wr) & 0x7fffffffu);
+            const uint32_t sb = half_scale(top);
+            const float inv = __uint_as_float((269u - (sb == 255u ? 142u : sb)) << 23);
+            const int64_t col = at + 128 * (b >> 1) + 32 * (b & 1);
+            store_halves(o + col, v[2 * b], wr, inv);
+            store_halves(o + col + 16, v[2 * b + 1], wr, inv);
+            p.out_scale[col / 32] = (uint8_t)sb;
+          }
         }
       } else if (real) {
 #pragma unroll
@@ -701,7 +723,48 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
 
 // ---- combine ---------------------------------------------------------------------------------------
 // y[t] = sum_j out[t * top_k + j] in fp32, in route order; routes out of range were never placed.
-// The route outputs are fp32: rounding each to bf16 would add as much error as the result's own.
+// The 16-bit form of the route outputs (prefill): 8 columns a thread.
+__global__ void __launch_bounds__(256)
+    mx_combine16_kernel(const int16_t* __restrict__ out, const uint8_t* __restrict__ out_scale,
+                        const int32_t* __restrict__ ids, int experts, int64_t tokens, int top_k,
+                        int hidden, __nv_bfloat16* y) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int vec = hidden / 8;
+  const uint4* out4 = reinterpret_cast<const uint4*>(out);
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < tokens * vec;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t t = i / vec;
+    const int c = (int)(i - t * vec);
+    uint4 v[8];
+    float s[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int e = j < top_k ? __ldg(ids + t * top_k + j) : -1;
+      v[j] = make_uint4(0, 0, 0, 0);
+      s[j] = 0.0f;
+      if (e >= 0 && e < experts) {
+        v[j] = __ldg(out4 + (t * top_k + j) * vec + c);
+        const uint32_t b = __ldg(out_scale + (t * top_k + j) * (vec / 4) + (c >> 2));
+        s[j] = __uint_as_float(b == 255u ? 0x7fffffffu : (b - 15u) << 23);
+      }
+    }
+    float acc[8] = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        acc[2 * k] = fmaf((float)(int16_t)(w[k] & 0xffff), s[j], acc[2 * k]);
+        acc[2 * k + 1] = fmaf((float)((int32_t)w[k] >> 16), s[j], acc[2 * k + 1]);
+      }
+    }
+    reinterpret_cast<uint4*>(y)[i] = make_uint4(pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3]),
+                                                pack_bf16(acc[4], acc[5]), pack_bf16(acc[6], acc[7]));
+  }
+}
+
+// fp32 route outputs (decode).
 __global__ void __launch_bounds__(256, 4)
     mx_combine_kernel(const float* __restrict__ out, const int32_t* __restrict__ ids, int experts,
                       int64_t tokens, int top_k, int hidden, __nv_bfloat16* y) {
@@ -774,7 +837,9 @@ MxWorkspace mx_workspace(int64_t tokens, int top_k, int experts, int hidden, int
   w.xs = take(blocks * tables * (hidden / kMxK) * 512);
   w.hq = take(2 * cap * inter);
   w.hs = take(blocks * tables * (inter / kMxK) * 512);
-  w.out = reinterpret_cast<float*>(take(numel * hidden * 4));
+  // fp32, or 16-bit with a scale byte per 32 columns
+  w.out = reinterpret_cast<float*>(take(numel * hidden * (w.block == kMxPrefillBlock ? 2 : 4)));
+  w.out_scale = take(w.block == kMxPrefillBlock ? numel * (hidden / 32) : 4);
   w.sync_ints = (int)(1 + blocks);
   w.sync = reinterpret_cast<int32_t*>(take(w.sync_ints * 4));
   w.bytes = off;
@@ -813,6 +878,7 @@ static MxLayerParams layer_params(const MxArgs& a, const MxWorkspace& w) {
   p.hs = w.hs;
   p.route_w = a.topk_w;
   p.out = w.out;
+  p.out_scale = w.out_scale;
   p.sync = w.sync;
   return p;
 }
@@ -881,6 +947,11 @@ cudaError_t launch_mx_experts(const MxArgs& a, const MxWorkspace& w, cudaStream_
   if (w.block == kMxPrefillBlock) {
     e = launch_mx_gemm<false>(a, w, s);
     if (e == cudaSuccess) e = launch_mx_gemm<true>(a, w, s);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(mx_combine16_kernel, stream_grid(a.tokens * (a.hidden / 8)), 256, 0, s,
+                      reinterpret_cast<const int16_t*>(w.out),
+                      static_cast<const uint8_t*>(w.out_scale), a.topk_ids, a.experts, a.tokens,
+                      a.top_k, a.hidden, static_cast<__nv_bfloat16*>(a.y));
   } else {
     e = w.block == 16   ? launch_mx_layer<16>(a, w, s)
         : w.block == 32 ? launch_mx_layer<32>(a, w, s)

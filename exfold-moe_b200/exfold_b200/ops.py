@@ -410,12 +410,14 @@ def quantize_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if not (x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= cols):
         x = x.contiguous()
     stride = x.stride(0) if x.dim() == 2 and x.shape[0] > 1 else cols
-    codes = torch.empty((*x.shape[:-1], 16 * blocks), dtype=torch.uint8, device=dev)
-    scales = torch.empty((*x.shape[:-1], blocks), dtype=torch.uint8, device=dev)
-    if x.numel() > 0:
+    lead = x.shape[:-1]
+    codes = torch.empty(*lead, 16 * blocks, dtype=torch.uint8, device=dev)
+    scales = torch.empty(*lead, blocks, dtype=torch.uint8, device=dev)
+    n = x.numel()
+    if n > 0:
         with _on(dev):
-            L.check(L.lib().exf_mxfp4_quantize(x.data_ptr(), _WDT[x.dtype], x.numel() // cols,
-                                               cols, stride, codes.data_ptr(), scales.data_ptr(),
+            L.check(L.lib().exf_mxfp4_quantize(x.data_ptr(), _WDT[x.dtype], n // cols, cols,
+                                               stride, codes.data_ptr(), scales.data_ptr(),
                                                _stream(dev)))
     return codes, scales
 
@@ -429,20 +431,21 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, cols: int | None
         raise TypeError("dequantize_mxfp4 needs uint8 codes and scales")
     if dtype not in _WDT:
         raise TypeError("dequantize_mxfp4 gives float32, bfloat16 or float16")
-    if codes.dim() == 0 or codes.shape != (*scales.shape[:-1], 16 * scales.shape[-1]):
+    lead, blocks = scales.shape[:-1], scales.shape[-1] if scales.dim() else 0
+    if codes.dim() == 0 or codes.shape[:-1] != lead or codes.shape[-1] != 16 * blocks:
         raise ValueError(f"codes {tuple(codes.shape)} do not match scales {tuple(scales.shape)}: "
                          "16 bytes a block")
-    blocks = scales.shape[-1]
     cols = 32 * blocks if cols is None else int(cols)
     if cols < 0 or (cols + 31) // 32 != blocks:
         raise ValueError(f"{cols} columns do not take {blocks} blocks of 32")
     codes, scales = _aligned(codes), scales.contiguous()
-    out = torch.empty((*scales.shape[:-1], cols), dtype=dtype, device=dev)
-    if out.numel() > 0:
+    out = torch.empty(*lead, cols, dtype=dtype, device=dev)
+    n = out.numel()
+    if n > 0:
         with _on(dev):
-            L.check(L.lib().exf_mxfp4_dequantize(codes.data_ptr(), scales.data_ptr(),
-                                                 out.numel() // cols, cols, out.data_ptr(),
-                                                 _WDT[dtype], _stream(dev)))
+            L.check(L.lib().exf_mxfp4_dequantize(codes.data_ptr(), scales.data_ptr(), n // cols,
+                                                 cols, out.data_ptr(), _WDT[dtype],
+                                                 _stream(dev)))
     return out
 
 
@@ -487,12 +490,13 @@ def fused_experts_mxfp4(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.T
     if two_i % 2 or hidden % 256 or inter % 128:
         raise NotImplementedError("fused_experts_mxfp4: hidden must be a multiple of 256 and "
                                   "intermediate a multiple of 128")
-    for t, shape, what in ((w13, (experts, two_i, hidden // 2), "w13"),
-                           (s13, (experts, two_i // 128, hidden // 128, 512), "s13"),
-                           (w2, (experts, hidden, inter // 2), "w2"),
-                           (s2, (experts, hidden // 128, inter // 128, 512), "s2")):
+    for t, shape in ((w13, (experts, two_i, hidden // 2)),
+                     (s13, (experts, two_i // 128, hidden // 128, 512)),
+                     (w2, (experts, hidden, inter // 2)),
+                     (s2, (experts, hidden // 128, inter // 128, 512))):
         if t.shape != shape:
-            raise ValueError(f"{what} {tuple(t.shape)} must be {shape}")
+            raise ValueError(f"weights of {experts} experts, hidden {hidden} and intermediate "
+                             f"{inter}: a tensor {tuple(t.shape)} must be {shape}")
     x, w13, s13, w2, s2 = (_aligned(t, 32) for t in (x, w13, s13, w2, s2))
     ids = topk_ids.to(torch.int32).contiguous()
     wts = topk_w.float().contiguous()
@@ -515,12 +519,13 @@ def _gated_forward(x, w13, activation, status, keep):
     """(h, pre): pre fp32 [tokens, 2 * inter] for the backward pass if `keep`, else None."""
     tokens, hidden = x.shape
     inter = w13.shape[0] // 2
-    h = torch.empty((tokens, inter), dtype=x.dtype, device=x.device)
-    pre = torch.empty((tokens, 2 * inter), dtype=torch.float32, device=x.device) if keep else None
-    with _on(x.device):
+    dev = x.device
+    h = torch.empty(tokens, inter, dtype=x.dtype, device=dev)
+    pre = torch.empty(tokens, 2 * inter, dtype=torch.float32, device=dev) if keep else None
+    with _on(dev):
         L.check(L.lib().exf_gated_mlp(x.data_ptr(), w13.data_ptr(), _WDT[x.dtype], tokens, hidden,
                                       inter, activation, h.data_ptr(), _ptr(pre), _ptr(status),
-                                      _stream(x.device)))
+                                      _stream(dev)))
     return h, pre
 
 
@@ -542,7 +547,7 @@ class _GatedMlp(torch.autograd.Function):
         dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
         dw13 = torch.empty_like(w13) if ctx.needs_input_grad[1] else None
         ws_bytes = int(L.lib().exf_gated_mlp_backward_workspace_bytes(tokens, inter))
-        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=x.device)
+        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=x.device)  # [dG dU]
         with _on(x.device):
             L.check(L.lib().exf_gated_mlp_backward(
                 dh.data_ptr(), pre.data_ptr(), x.data_ptr(), w13.data_ptr(), _WDT[x.dtype], tokens,
@@ -570,10 +575,11 @@ def gated_mlp(x: torch.Tensor, w13: torch.Tensor, activation: str = "silu",
             or w13.numel() == 0):
         raise ValueError(f"x {tuple(x.shape)} and w13 {tuple(w13.shape)} must be [..., H] and "
                          "[2I, H]")
-    rows, w = _aligned(x.reshape(-1, x.shape[-1])), _aligned(w13)
+    flat = x.dim() == 2
+    rows, w = _aligned(x if flat else x.reshape(-1, x.shape[-1])), _aligned(w13)
     act = _ACTIVATION[activation]
     if torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad):
         h = _GatedMlp.apply(rows, w, act, status)
     else:
         h, _ = _gated_forward(rows, w, act, status, False)
-    return h.view(*x.shape[:-1], h.shape[1])
+    return h if flat else h.view(*x.shape[:-1], h.shape[1])
