@@ -484,23 +484,22 @@ struct MxGemmSmem {
 constexpr size_t mx_gemm_smem_bytes() { return sizeof(MxGemmSmem) + 1024; }
 static_assert(mx_gemm_smem_bytes() <= 232448, "prefill expert GEMM shared memory");
 
-// The route outputs at prefill, 16-bit: 32 columns share 2^(byte - 127), above their largest
-// magnitude; a value is a signed 16-bit multiple of 2^(byte - 142), within 2^-16 of that power
-// (bf16 route outputs would add as much error as the result's own rounding, fp32 ones held GEMM-2
-// and the combine to the memory's speed).  Byte 255: NaN.
+// The route outputs at prefill, 16-bit: 32 columns share u = 2^(byte - 127), the largest magnitude
+// being in [2^13 u, 2^14 u); a value is a signed 16-bit multiple of u, within 2^-14 of that magnitude.
+// (bf16 route outputs would add as much error as the result's own rounding, fp32 ones twice the
+// traffic.)  Byte 255: NaN.
 __device__ __forceinline__ uint32_t half_scale(uint32_t top_bits) {
-  const uint32_t e = (top_bits >> 23) + 1;
-  return top_bits >= 0x7f800000u ? 255u : (e < 16 ? 16u : e);
+  const uint32_t e = top_bits >> 23;
+  return top_bits >= 0x7f800000u ? 255u : (e < 14 ? 1u : e - 13u);
 }
-// 16 values -> 16 multiples, one 32-byte sector
-__device__ __forceinline__ void store_halves(int16_t* at, const uint32_t* v, float w, float inv) {
+// 16 values times w -> 16 multiples, one 32-byte sector.  Adding 1.5 2^23 rounds to an integer, whose
+// low 16 bits are its two's complement.
+__device__ __forceinline__ void store_halves(int16_t* at, const uint32_t* v, float w) {
   uint32_t o[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int a = max(min(__float2int_rn(__uint_as_float(v[2 * j]) * w * inv), 32767), -32767);
-    const int b = max(min(__float2int_rn(__uint_as_float(v[2 * j + 1]) * w * inv), 32767), -32767);
-    o[j] = __byte_perm(a, b, 0x5410);
-  }
+  for (int j = 0; j < 8; ++j)
+    o[j] = __byte_perm(__float_as_uint(fmaf(__uint_as_float(v[2 * j]), w, 12582912.0f)),
+                       __float_as_uint(fmaf(__uint_as_float(v[2 * j + 1]), w, 12582912.0f)), 0x5410);
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(o[0]),
                "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
                : "memory");
@@ -633,13 +632,12 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
       if (!warp_wait(&sm.acc_full, i & 1, failed)) break;
       fence_after_sync();
       const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
-      // columns [64 hf, +64) and [128 + 64 hf, +64): 64 features' gate and up, or two runs of 64
-      // output columns
+      // 64 features' gate and up: columns [64 hf, +64) and [128 + 64 hf, +64); or 128 output columns
       uint32_t v[8][16];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        tmem_load16(taddr + 64 * hf + 16 * j, v[j]);
-        tmem_load16(taddr + 128 + 64 * hf + 16 * j, v[4 + j]);
+        tmem_load16(taddr + (DOWN ? 128 : 64) * hf + 16 * j, v[j]);
+        tmem_load16(taddr + (DOWN ? 64 + 128 * hf : 128 + 64 * hf) + 16 * j, v[4 + j]);
       }
       tmem_wait();
       fence_before_sync();
@@ -649,25 +647,27 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
       if (DOWN) {
         if (real) {
           const float wr = p.route_w[route];
-          const int64_t at = (int64_t)route * p.hidden + ft * 256 + 64 * hf;
+          const int64_t at = (int64_t)route * p.hidden + ft * 256 + 128 * hf;
           int16_t* o = reinterpret_cast<int16_t*>(p.out);
+          uint32_t bytes = 0;
 #pragma unroll
           for (int b = 0; b < 4; ++b) {  // runs of 32 columns
             uint32_t top = 0;
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-              for (int c = 0; c < 16; ++c)
-                top = max(top, __float_as_uint(__uint_as_float(v[2 * b + j][c]) * wr) & 0x7fffffffu);
-            const uint32_t sb = half_scale(top);
-            const float inv = __uint_as_float((269u - (sb == 255u ? 142u : sb)) << 23);
-            const int64_t col = at + 128 * (b >> 1) + 32 * (b & 1);
-            store_halves(o + col, v[2 * b], wr, inv);
-            store_halves(o + col + 16, v[2 * b + 1], wr, inv);
-            p.out_scale[col / 32] = (uint8_t)sb;
+              for (int c = 0; c < 16; ++c) top = max(top, v[2 * b + j][c] & 0x7fffffffu);
+            const uint32_t sb =
+                half_scale(__float_as_uint(__uint_as_float(top) * wr) & 0x7fffffffu);
+            const float w = wr * __uint_as_float((254u - (sb == 255u ? 127u : sb)) << 23);
+            store_halves(o + at + 32 * b, v[2 * b], w);
+            store_halves(o + at + 32 * b + 16, v[2 * b + 1], w);
+            bytes |= sb << (8 * b);
           }
+          *reinterpret_cast<uint32_t*>(p.out_scale + at / 32) = bytes;
         }
       } else if (real) {
+        uint32_t hi_bytes = 0, lo_bytes = 0;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {  // two scale blocks of 32 features
           uint32_t top = 0;
@@ -701,10 +701,15 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
             reinterpret_cast<uint4*>(hi_row)[j] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             reinterpret_cast<uint4*>(lo_row)[j] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           }
-          p.hs[scale_at(2 * blk, p.inter / kMxK, feat / 32, r)] = (uint8_t)sb;
-          p.hs[scale_at(2 * blk, p.inter / kMxK, feat / 32, 128 + r)] =
-              (uint8_t)split_lo_byte(sb);
+          hi_bytes |= sb << (8 * b);
+          lo_bytes |= split_lo_byte(sb) << (8 * b);
         }
+        // the two blocks' scales are neighbouring bytes
+        const int kb = ft * 4 + 2 * hf;
+        *reinterpret_cast<uint16_t*>(p.hs + scale_at(2 * blk, p.inter / kMxK, kb, r)) =
+            (uint16_t)hi_bytes;
+        *reinterpret_cast<uint16_t*>(p.hs + scale_at(2 * blk, p.inter / kMxK, kb, 128 + r)) =
+            (uint16_t)lo_bytes;
       }
     }
   }
@@ -746,7 +751,7 @@ __global__ void __launch_bounds__(256)
       if (e >= 0 && e < experts) {
         v[j] = __ldg(out4 + (t * top_k + j) * vec + c);
         const uint32_t b = __ldg(out_scale + (t * top_k + j) * (vec / 4) + (c >> 2));
-        s[j] = __uint_as_float(b == 255u ? 0x7fffffffu : (b - 15u) << 23);
+        s[j] = __uint_as_float(b == 255u ? 0x7fffffffu : b << 23);
       }
     }
     float acc[8] = {};
