@@ -60,10 +60,11 @@ __host__ __device__ constexpr int scale_tables(int block) {
   return block == kMxPrefillBlock ? 2 : 1;
 }
 
-// 8 bf16 values (vector c of a row) in the two-term form; the 4 lanes of a block of 32 together
+// 8 bf16 values (vector c of a row, c = the lane modulo 32) in the two-term form; the 4 lanes of a block
+// of 32 together.  scales, lo_scales: the terms' scale bytes of the half warp's 4 blocks.
 struct MxTerms {
   uint2 hi, lo;
-  uint32_t scale;
+  uint32_t scales, lo_scales;
 };
 __device__ __forceinline__ MxTerms split8(uint4 v) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -74,8 +75,15 @@ __device__ __forceinline__ MxTerms split8(uint4 v) {
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
   MxTerms t;
-  t.scale = split_scale(top);
-  const float inv = split_inverse(t.scale);
+  const uint32_t scale = split_scale(top);
+  const float inv = split_inverse(scale);
+  t.scales = t.lo_scales = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t b = __shfl_sync(0xffffffffu, scale, (threadIdx.x & 16) + 4 * j);
+    t.scales |= b << (8 * j);
+    t.lo_scales |= split_lo_byte(b) << (8 * j);
+  }
   uint32_t hi[4], lo[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -84,24 +92,29 @@ __device__ __forceinline__ MxTerms split8(uint4 v) {
   t.lo = make_uint2(lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
   return t;
 }
-// writes vector c of the token row of slot `slot`
 struct MxRows {
   uint8_t* xq;   // [blocks][2 * block][hidden]
   uint8_t* xs;   // [blocks][tables][hidden / 128][512]
   int hidden;
   int block;
 };
-__device__ __forceinline__ void put8(const MxRows& o, int64_t slot, int c, const MxTerms& t) {
-  const int64_t blk = slot / o.block;
-  const int n = mx_row(o.block, (int)(slot - blk * o.block));
-  uint8_t* hi = o.xq + (blk * 2 * o.block + n) * o.hidden + 8 * c;
+// the hi row of a slot
+__device__ __forceinline__ int mx_slot_row(int block, int slot) {
+  const int blk = slot / block;
+  return blk * 2 * block + mx_row(block, slot - blk * block);
+}
+// writes vector c of a token to the slot with that hi row
+__device__ __forceinline__ void put8(const MxRows& o, int row, int c, const MxTerms& t) {
+  uint8_t* hi = o.xq + (int64_t)row * o.hidden + 8 * c;
   *reinterpret_cast<uint2*>(hi) = t.hi;
-  *reinterpret_cast<uint2*>(hi + (int64_t)mx_lo(o.block) * o.hidden) = t.lo;
-  if ((c & 3) < 2) {
+  *reinterpret_cast<uint2*>(hi + mx_lo(o.block) * o.hidden) = t.lo;
+  if ((c & 15) < 2) {  // a word of 4 blocks' scales: hi's, lo's
     const bool lo = c & 1;
-    o.xs[scale_at(blk * scale_tables(o.block), o.hidden / kMxK, c >> 2,
-                  lo ? n + mx_lo(o.block) : n)] =
-        (uint8_t)(lo ? split_lo_byte(t.scale) : t.scale);
+    const int blk = row / (2 * o.block);
+    const int n = row - blk * 2 * o.block + (lo ? mx_lo(o.block) : 0);
+    *reinterpret_cast<uint32_t*>(o.xs + scale_at((int64_t)blk * scale_tables(o.block),
+                                                 o.hidden / kMxK, (c >> 4) * 4, n)) =
+        lo ? t.lo_scales : t.scales;
   }
 }
 

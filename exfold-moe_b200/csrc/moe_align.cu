@@ -193,7 +193,7 @@ struct CopyRows {
 struct SplitRows {
   MxRows rows;
   __device__ __forceinline__ void operator()(int slot, int c, uint4 v) const {
-    put8(rows, slot, c, split8(v));
+    put8(rows, mx_slot_row(rows.block, slot), c, split8(v));
   }
 };
 

@@ -26,7 +26,7 @@ using namespace tc;
 constexpr int kMxLayerThreads = 416;  // warps 0, 2, 3 TMA, 1 MMA, 4-11 epilogue, 12 schedule
 
 // ---- token rows in route order (more than align_gather_max_numel() routes) -----------------------
-// A warp takes a token: its row is split once and written to the slots of its routes.
+// A warp takes 1024 columns of a token: they are split once and written to the slots of its routes.
 __global__ void __launch_bounds__(256) mx_split_kernel(const __nv_bfloat16* x, const int32_t* slots,
                                                        int64_t tokens, int top_k, MxRows rows,
                                                        int32_t* zero, int zero_n) {
@@ -35,18 +35,29 @@ __global__ void __launch_bounds__(256) mx_split_kernel(const __nv_bfloat16* x, c
   for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < zero_n; i += gridDim.x * blockDim.x)
     zero[i] = 0;
   const int lane = threadIdx.x & 31;
+  const int vecs = rows.hidden / 8;          // a multiple of 32
+  const int pieces = (vecs + 127) / 128;
   const int64_t warps = (int64_t)gridDim.x * (blockDim.x / 32);
-  for (int64_t t = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); t < tokens;
-       t += warps) {
-    const int mine = lane < top_k ? slots[t * top_k + lane] : -1;
+  for (int64_t u = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5);
+       u < tokens * pieces; u += warps) {
+    const int64_t t = u / pieces;
+    const int c0 = (int)(u - t * pieces) * 128;
+    int mine = lane < top_k ? slots[t * top_k + lane] : -1;
+    if (mine >= 0) mine = mx_slot_row(rows.block, mine);
     if (__ballot_sync(0xffffffffu, mine >= 0) == 0) continue;
     const uint4* row = reinterpret_cast<const uint4*>(x + t * rows.hidden);
-#pragma unroll 2
-    for (int c = lane; c < rows.hidden / 8; c += 32) {
-      const MxTerms v = split8(row[c]);
-      for (int j = 0; j < top_k; ++j) {
-        const int slot = __shfl_sync(0xffffffffu, mine, j);
-        if (slot >= 0) put8(rows, slot, c, v);
+    uint4 raw[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      raw[j] = c0 + 32 * j < vecs ? __ldg(row + c0 + 32 * j + lane) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = c0 + 32 * j + lane;
+      if (c0 + 32 * j >= vecs) break;
+      const MxTerms v = split8(raw[j]);
+      for (int r = 0; r < top_k; ++r) {
+        const int to = __shfl_sync(0xffffffffu, mine, r);
+        if (to >= 0) put8(rows, to, c, v);
       }
     }
   }
@@ -728,44 +739,56 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
 
 // ---- combine ---------------------------------------------------------------------------------------
 // y[t] = sum_j out[t * top_k + j] in fp32, in route order; routes out of range were never placed.
-// The 16-bit form of the route outputs (prefill): 8 columns a thread.
+// The 16-bit form of the route outputs (prefill).
 __global__ void __launch_bounds__(256)
     mx_combine16_kernel(const int16_t* __restrict__ out, const uint8_t* __restrict__ out_scale,
                         const int32_t* __restrict__ ids, int experts, int64_t tokens, int top_k,
                         int hidden, __nv_bfloat16* y) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int vec = hidden / 8;
+  // a warp takes 1024 columns of a token, 256 at a time, the loads of all its routes together
+  const int lane = threadIdx.x & 31;
+  const int vecs = hidden / 8;  // a multiple of 32
+  const int pieces = (vecs + 127) / 128;
   const uint4* out4 = reinterpret_cast<const uint4*>(out);
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < tokens * vec;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t t = i / vec;
-    const int c = (int)(i - t * vec);
-    uint4 v[8];
-    float s[8];
+  const int64_t warps = (int64_t)gridDim.x * (blockDim.x / 32);
+  for (int64_t u = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5);
+       u < tokens * pieces; u += warps) {
+    const int64_t t = u / pieces;
+    const int c0 = (int)(u - t * pieces) * 128;
+    const int e = lane < top_k ? ids[t * top_k + lane] : -1;
+    const uint32_t use = __ballot_sync(0xffffffffu, e >= 0 && e < experts);
+    for (int c1 = c0; c1 < c0 + 128 && c1 < vecs; c1 += 32) {
+      const int c = c1 + lane;
+      uint4 v[8];
+      uint32_t b[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int e = j < top_k ? __ldg(ids + t * top_k + j) : -1;
-      v[j] = make_uint4(0, 0, 0, 0);
-      s[j] = 0.0f;
-      if (e >= 0 && e < experts) {
-        v[j] = __ldg(out4 + (t * top_k + j) * vec + c);
-        const uint32_t b = __ldg(out_scale + (t * top_k + j) * (vec / 4) + (c >> 2));
-        s[j] = __uint_as_float(b == 255u ? 0x7fffffffu : b << 23);
+      for (int j = 0; j < 8; ++j) {
+        if ((use >> j) & 1) {
+          v[j] = __ldg(out4 + (t * top_k + j) * vecs + c);
+          b[j] = __ldg(out_scale + (t * top_k + j) * (vecs / 4) + (c >> 2));
+        }
       }
-    }
-    float acc[8] = {};
+      float acc[8] = {};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+      for (int j = 0; j < 8; ++j) {
+        if (!((use >> j) & 1)) continue;
+        const float s = __uint_as_float(b[j] == 255u ? 0x7fffffffu : b[j] << 23);
+        const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        acc[2 * k] = fmaf((float)(int16_t)(w[k] & 0xffff), s[j], acc[2 * k]);
-        acc[2 * k + 1] = fmaf((float)((int32_t)w[k] >> 16), s[j], acc[2 * k + 1]);
+        for (int k = 0; k < 4; ++k) {
+          // a signed 16-bit q, its sign bit flipped, in the low bits of 2^23: 2^23 + 2^15 + q
+          const uint32_t f = w[k] ^ 0x80008000u;
+          acc[2 * k] = fmaf(__uint_as_float(__byte_perm(f, 0x4b000000u, 0x7610)) - 8421376.0f, s,
+                            acc[2 * k]);
+          acc[2 * k + 1] = fmaf(__uint_as_float(__byte_perm(f, 0x4b000000u, 0x7632)) - 8421376.0f,
+                                s, acc[2 * k + 1]);
+        }
       }
+      reinterpret_cast<uint4*>(y)[t * vecs + c] =
+          make_uint4(pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3]),
+                     pack_bf16(acc[4], acc[5]), pack_bf16(acc[6], acc[7]));
     }
-    reinterpret_cast<uint4*>(y)[i] = make_uint4(pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3]),
-                                                pack_bf16(acc[4], acc[5]), pack_bf16(acc[6], acc[7]));
   }
 }
 
@@ -943,7 +966,8 @@ cudaError_t launch_mx_experts(const MxArgs& a, const MxWorkspace& w, cudaStream_
     ap.slots = w.slots;
     e = launch_align(EXF_I32, ap, s);
     if (e == cudaSuccess)
-      e = launch_pdl(mx_split_kernel, stream_grid(a.tokens * 32), 256, 0, s,
+      e = launch_pdl(mx_split_kernel, stream_grid(a.tokens * 32 * ((a.hidden + 1023) / 1024)), 256,
+                     0, s,
                      static_cast<const __nv_bfloat16*>(a.x),
                      static_cast<const int32_t*>(w.slots), a.tokens, a.top_k,
                      MxRows{w.xq, w.xs, a.hidden, w.block}, w.sync, w.sync_ints);
@@ -953,7 +977,8 @@ cudaError_t launch_mx_experts(const MxArgs& a, const MxWorkspace& w, cudaStream_
     e = launch_mx_gemm<false>(a, w, s);
     if (e == cudaSuccess) e = launch_mx_gemm<true>(a, w, s);
     if (e != cudaSuccess) return e;
-    return launch_pdl(mx_combine16_kernel, stream_grid(a.tokens * (a.hidden / 8)), 256, 0, s,
+    return launch_pdl(mx_combine16_kernel,
+                      stream_grid(a.tokens * 32 * ((a.hidden + 1023) / 1024)), 256, 0, s,
                       reinterpret_cast<const int16_t*>(w.out),
                       static_cast<const uint8_t*>(w.out_scale), a.topk_ids, a.experts, a.tokens,
                       a.top_k, a.hidden, static_cast<__nv_bfloat16*>(a.y));
