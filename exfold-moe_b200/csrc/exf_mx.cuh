@@ -17,7 +17,7 @@
 namespace exf {
 
 constexpr int kMxK = 128;          // k values of a scale table: 4 MMA steps, one 32-bit scale word
-constexpr int kMxPrefillBlock = 128; // routes of a block at prefill; 16, 32 or 64 at decode
+constexpr int kMxPrefillBlock = 128; // routes of a block at prefill; 16 or 32 at decode
 
 // scale byte of a block from the bits of its largest magnitude: s = 2^(byte - 127); at least 5, so
 // that lo's byte (5 less) exists; 255 (NaN) if the block holds an infinity or NaN

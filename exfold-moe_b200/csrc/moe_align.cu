@@ -224,11 +224,17 @@ __global__ void __launch_bounds__(kAlignThreads, 1)
     sm.base[e] = 0;
   }
   __syncthreads();
-  for (int64_t r = tid; r < p.numel; r += kAlignThreads) {
-    const int e = expert_of(ids, r, p.numel, E);
-    if (e >= 0) {
-      atomicAdd(&sm.count[e], 1);
-      if (r < s0) atomicAdd(&sm.base[e], 1);  // routes of e placed by earlier slices
+  constexpr int kBatch = 4;  // loads in flight together, here and below
+  for (int64_t r0 = tid; r0 < p.numel; r0 += kBatch * kAlignThreads) {
+    int ex[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) ex[b] = expert_of(ids, r0 + b * kAlignThreads, p.numel, E);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      if (ex[b] < 0) continue;
+      atomicAdd(&sm.count[ex[b]], 1);
+      // routes of the expert placed by earlier slices
+      if (r0 + b * kAlignThreads < s0) atomicAdd(&sm.base[ex[b]], 1);
     }
   }
   __syncthreads();
@@ -240,11 +246,20 @@ __global__ void __launch_bounds__(kAlignThreads, 1)
     slot_of[tid] = scatter_round(r0 + tid, expert_of(ids, r0 + tid, s1, E), E, sm, p.sorted_ids);
     __syncthreads();
     const int n = s1 - r0 < kAlignThreads ? (int)(s1 - r0) : kAlignThreads;
-    for (int i = tid; i < n * row_vecs; i += kAlignThreads) {
-      const int k = i / row_vecs;
-      const int c = i - k * row_vecs;
-      const int slot = slot_of[k];
-      if (slot >= 0) put(slot, c, x[(r0 + k) / top_k * row_vecs + c]);
+    for (int i0 = tid; i0 < n * row_vecs; i0 += kBatch * kAlignThreads) {
+      int slot[kBatch], c[kBatch];
+      uint4 v[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int i = i0 + b * kAlignThreads;
+        const int k = i / row_vecs;
+        c[b] = i - k * row_vecs;
+        slot[b] = i < n * row_vecs ? slot_of[k] : -1;
+        if (slot[b] >= 0) v[b] = x[(r0 + k) / top_k * row_vecs + c[b]];
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b)
+        if (slot[b] >= 0) put(slot[b], c[b], v[b]);
     }
     __syncthreads();  // slot_of is rewritten by the next round
   }

@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(256) mx_split_kernel(const __nv_bfloat16* x, c
 
 // ---- decode ---------------------------------------------------------------------------------------
 // A tile is 256 weight rows of one expert (two MMA tiles of 128 rows on the M side) times a block of
-// BT = 16, 32 or 64 of its routes (the N side: 2 BT hi and lo rows).
+// BT = 16 or 32 of its routes (the N side: 2 BT hi and lo rows).
 //   GEMM-1 tile (block, f): gate rows [128 f, +128) and up rows [I + 128 f, +128) of W13[e], K = H;
 //     the epilogue forms h = silu(gate) * up and writes its two-term form;
 //   GEMM-2 tile (block, f): rows [256 f, +256) of W2[e], K = I; out[route][256 f + i] = w_route D.
@@ -80,22 +80,21 @@ __global__ void __launch_bounds__(256) mx_split_kernel(const __nv_bfloat16* x, c
 //
 // Scales are loaded for several stages at a time: a copy a stage cost as much of the TMA unit as a
 // third of a weight tile.  8 epilogue warps sum the two terms into registers and give the
-// accumulator back before they compute; up to 32 routes there are two.
+// accumulator back before they compute; there are two accumulators.
 //
 // What bounds the layer is the bytes in flight: padded, a stage's 17 KB of codes and scales take
-// 32 KB of shared memory, so the smaller token tiles of 16 and 32 routes buy a stage.
+// 32 KB of shared memory, and four stages instead of five cost 4 %.
 template <int BT>
 struct MxCfg {
   static constexpr int kN = 2 * BT;
   static constexpr int kTTile = kN * kMxK;
   static constexpr int kWTile = 128 * kMxK;              // padded codes of 128 rows
-  static constexpr int kStages = BT == 64 ? 4 : 5;
+  static constexpr int kStages = 5;
   static constexpr int kScaleRun = BT == 32 ? 2 : 4;     // stages a copy of scales serves
   static constexpr int kScaleBytes = kScaleRun * 512;
   static constexpr int kRing = 4;                        // tiles handed out ahead
   static constexpr int kAccCols = 2 * kN;
-  static constexpr int kAccs = BT == 64 ? 1 : 2;
-  static constexpr int kScaleCol = kAccs * kAccCols;     // 4 sets of 16 columns
+  static constexpr int kScaleCol = 2 * kAccCols;         // 4 sets of 16 columns
   static constexpr int kTmemCols = kScaleCol + 64 <= 256 ? 256 : 512;
 };
 struct MxTile {
@@ -126,8 +125,7 @@ struct MxSmem {
 };
 template <int BT>
 constexpr size_t mx_smem_bytes() { return sizeof(MxSmem<BT>) + 1024; }
-static_assert(mx_smem_bytes<16>() <= 232448 && mx_smem_bytes<32>() <= 232448 &&
-                  mx_smem_bytes<64>() <= 232448,
+static_assert(mx_smem_bytes<16>() <= 232448 && mx_smem_bytes<32>() <= 232448,
               "decode expert layer shared memory");
 
 // The scales that come with k block kb of a tile: those of R blocks with every R-th.  First block
@@ -187,7 +185,7 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
       mbar_init(&sm.full[s], 3);  // one arrival per loading warp
       mbar_init(&sm.empty[s], 1);
     }
-    for (int b = 0; b < C::kAccs; ++b) {
+    for (int b = 0; b < 2; ++b) {
       mbar_init(&sm.acc_full[b], 1);
       mbar_init(&sm.acc_empty[b], 8);
     }
@@ -245,8 +243,7 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
         lt.ft = t - lt.blk * n;
         lt.expert = p.routes.expert_ids[lt.blk];
         const int32_t* ids = p.routes.sorted_ids + (int64_t)lt.blk * BT;
-        int real = __popc(__ballot_sync(0xffffffffu, lane < BT && ids[lane] < p.numel));
-        if (BT == 64) real += __popc(__ballot_sync(0xffffffffu, ids[32 + lane] < p.numel));
+        const int real = __popc(__ballot_sync(0xffffffffu, lane < BT && ids[lane] < p.numel));
         lt.quarters = (real + 15) >> 4;
         if (lt.expert < 0 || lt.expert >= p.experts) {
           --j;
@@ -336,8 +333,8 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
     MxTile lt;
     for (int j = 0; ok && next_tile(j, lt); ++j) {
       const int kblocks = (lt.kind == kDown ? p.inter : p.hidden) / kMxK;
-      const int b = i % C::kAccs;
-      ok = warp_wait(&sm.acc_empty[b], ((i / C::kAccs) & 1) ^ 1, failed);
+      const int b = i % 2;
+      ok = warp_wait(&sm.acc_empty[b], ((i / 2) & 1) ^ 1, failed);
       if (!ok) break;
       fence_after_sync();
       const uint32_t acc = tmem + static_cast<uint32_t>(b * C::kAccCols);
@@ -373,41 +370,35 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
     mbar_wait_drain(&sm.drain, 0);
   } else {
     // ---- epilogue: a warp has 32 weight rows of each MMA tile (TMEM lanes 32 q .. +31) and half of
-    // the block's routes, in chunks of 16 (of 8 where a block has 16); in the columns of 16 routes
-    // the hi rows come first, then the lo rows
-    constexpr int kChunk = BT == 16 ? 8 : 16;
-    constexpr int kChunks = BT / 2 / kChunk;
+    // the block's routes; in the columns of 16 routes the hi rows come first, then the lo rows
+    constexpr int kHalf = BT / 2;
     const int q = warp & 3, hf = (warp - 4) >> 2;
     int i = 0;
     MxTile lt;
     for (int j = 0; next_tile(j, lt); ++j) {
       const bool down = lt.kind == kDown;
       // lane l looks after route l of the warp's half
-      const int r0 = hf * (BT / 2);
-      const int route_l = lane < BT / 2 ? p.routes.sorted_ids[lt.blk * BT + r0 + lane] : p.numel;
+      const int r0 = hf * kHalf;
+      const int route_l = lane < kHalf ? p.routes.sorted_ids[lt.blk * BT + r0 + lane] : p.numel;
       const float w_l = down && route_l < p.numel ? p.route_w[route_l] : 0.0f;
       const int real = __popc(__ballot_sync(0xffffffffu, route_l < p.numel));  // they come first
-      const int b = i % C::kAccs;
-      if (!warp_wait(&sm.acc_full[b], (i / C::kAccs) & 1, failed)) break;
+      const int b = i % 2;
+      if (!warp_wait(&sm.acc_full[b], (i / 2) & 1, failed)) break;
       fence_after_sync();
-      float v0[kChunks][kChunk], v1[kChunks][kChunk];  // gate and up, or rows r and r + 128
-      const uint32_t taddr =
-          tmem + static_cast<uint32_t>(b * C::kAccCols) + ((uint32_t)(q * 32) << 16);
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        if (c * kChunk >= real) break;
-        const int r = r0 + c * kChunk;
-        const uint32_t col = taddr + 32 * (r >> 4) + (r & 15);
-        uint32_t a0[kChunk], a1[kChunk], b0[kChunk], b1[kChunk];
-        tmem_load_cols<kChunk>(col, a0);
-        tmem_load_cols<kChunk>(col + 16, a1);
-        tmem_load_cols<kChunk>(col + C::kN, b0);
-        tmem_load_cols<kChunk>(col + C::kN + 16, b1);
+      float v0[kHalf], v1[kHalf];  // gate and up, or rows r and r + 128
+      if (real > 0) {
+        const uint32_t col = tmem + static_cast<uint32_t>(b * C::kAccCols) +
+                             ((uint32_t)(q * 32) << 16) + 32 * (r0 >> 4) + (r0 & 15);
+        uint32_t a0[kHalf], a1[kHalf], b0[kHalf], b1[kHalf];
+        tmem_load_cols<kHalf>(col, a0);
+        tmem_load_cols<kHalf>(col + 16, a1);
+        tmem_load_cols<kHalf>(col + C::kN, b0);
+        tmem_load_cols<kHalf>(col + C::kN + 16, b1);
         tmem_wait();
 #pragma unroll
-        for (int n = 0; n < kChunk; ++n) {
-          v0[c][n] = __uint_as_float(a0[n]) + __uint_as_float(a1[n]);
-          v1[c][n] = __uint_as_float(b0[n]) + __uint_as_float(b1[n]);
+        for (int n = 0; n < kHalf; ++n) {
+          v0[n] = __uint_as_float(a0[n]) + __uint_as_float(a1[n]);
+          v1[n] = __uint_as_float(b0[n]) + __uint_as_float(b1[n]);
         }
       }
       fence_before_sync();
@@ -417,35 +408,31 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
       if (!down) {
         const int feat = lt.ft * 128 + q * 32 + lane;  // the warp's features: one scale block
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-          for (int n = 0; n < kChunk; ++n) {
-            if (c * kChunk + n >= real) break;
-            const float h = silu_up(v0[c][n], v1[c][n]);
-            const uint32_t sb = split_scale(
-                __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu));
-            uint32_t hi, lo;
-            split2(h, 0.0f, split_inverse(sb), hi, lo);
-            const int row = mx_row(BT, r0 + c * kChunk + n);
-            uint8_t* at = p.hq + ((int64_t)lt.blk * C::kN + row) * p.inter + feat;
-            at[0] = (uint8_t)hi;
-            at[(int64_t)mx_lo(BT) * p.inter] = (uint8_t)lo;
-            if (lane < 2)
-              p.hs[scale_at(lt.blk, p.inter / kMxK, feat >> 5, lane ? row + mx_lo(BT) : row)] =
-                  (uint8_t)(lane ? split_lo_byte(sb) : sb);
-          }
+        for (int n = 0; n < kHalf; ++n) {
+          if (n >= real) break;
+          const float h = silu_up(v0[n], v1[n]);
+          const uint32_t sb =
+              split_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu));
+          uint32_t hi, lo;
+          split2(h, 0.0f, split_inverse(sb), hi, lo);
+          const int row = mx_row(BT, r0 + n);
+          uint8_t* at = p.hq + ((int64_t)lt.blk * C::kN + row) * p.inter + feat;
+          at[0] = (uint8_t)hi;
+          at[(int64_t)mx_lo(BT) * p.inter] = (uint8_t)lo;
+          if (lane < 2)
+            p.hs[scale_at(lt.blk, p.inter / kMxK, feat >> 5, lane ? row + mx_lo(BT) : row)] =
+                (uint8_t)(lane ? split_lo_byte(sb) : sb);
+        }
       } else {
         float* o = p.out + lt.ft * 256 + q * 32 + lane;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-          for (int n = 0; n < kChunk; ++n) {
-            if (c * kChunk + n >= real) break;
-            const int64_t route = __shfl_sync(0xffffffffu, route_l, c * kChunk + n);
-            const float wr = __shfl_sync(0xffffffffu, w_l, c * kChunk + n);
-            o[route * p.hidden] = v0[c][n] * wr;
-            o[route * p.hidden + 128] = v1[c][n] * wr;
-          }
+        for (int n = 0; n < kHalf; ++n) {
+          if (n >= real) break;
+          const int64_t route = __shfl_sync(0xffffffffu, route_l, n);
+          const float wr = __shfl_sync(0xffffffffu, w_l, n);
+          o[route * p.hidden] = v0[n] * wr;
+          o[route * p.hidden + 128] = v1[n] * wr;
+        }
       }
       if (!down) {
         // visible to the TMA loads of the block's GEMM-2 tiles, in any CTA; then count the warp off
@@ -569,6 +556,9 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
       const int half = warp - 2;
       const int row = DOWN ? expert * p.hidden + ft * 256 + half * 128
                            : expert * 2 * p.inter + ft * 128 + half * p.inter;
+      // quarters of 32 routes that hold any (routes fill their block from its first row)
+      const int first = p.routes.sorted_ids[blk * 128 + 32 * (lane & 3)];
+      const int quarters = __popc(__ballot_sync(0xffffffffu, lane < 4 && first < p.numel));
       const uint8_t* sc = warp == 0
                               ? (DOWN ? p.hs : p.xs) + (int64_t)blk * 2 * kblocks * 512
                               : (DOWN ? p.s2 : p.s13) + (int64_t)(row / 128) * kblocks * 512;
@@ -579,8 +569,13 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
         uint64_t* bar = &sm.full[s];
         if (elect_one()) {
           if (warp == 0) {
-            mbar_expect_tx(bar, 2 * kTile + 1024);
-            tma_load_2d(sm.tiles[s], &map_t, bar, kb * kMxK, blk * 256);
+            mbar_expect_tx(bar, quarters * (2 * kTile / 4) + 1024);
+            for (int q = 0; q < quarters; ++q) {
+              tma_load_2d(sm.tiles[s] + q * (kTile / 4), &map_t, bar, kb * kMxK,
+                          blk * 256 + 32 * q);
+              tma_load_2d(sm.tiles[s] + kTile + q * (kTile / 4), &map_t, bar, kb * kMxK,
+                          blk * 256 + 128 + 32 * q);
+            }
             bulk_load(sm.scales[s], sc + kb * 512, 512, bar);
             bulk_load(sm.scales[s] + 512, sc + (int64_t)(kblocks + kb) * 512, 512, bar);
           } else {
@@ -792,47 +787,56 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// fp32 route outputs (decode).
-__global__ void __launch_bounds__(256, 4)
+// fp32 route outputs (decode): a warp takes 256 columns of a token.
+__global__ void __launch_bounds__(256)
     mx_combine_kernel(const float* __restrict__ out, const int32_t* __restrict__ ids, int experts,
                       int64_t tokens, int top_k, int hidden, __nv_bfloat16* y) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int vec = hidden / 4;
-  const float4* out4 = reinterpret_cast<const float4*>(out);
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < tokens * vec;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t t = i / vec;
-    const int c = (int)(i - t * vec);
-    float4 v[8];
-    bool use[8];
+  const int lane = threadIdx.x & 31;
+  const int pieces = hidden / 256;
+  const int64_t warps = (int64_t)gridDim.x * (blockDim.x / 32);
+  for (int64_t u = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5);
+       u < tokens * pieces; u += warps) {
+    const int64_t t = u / pieces;
+    const int c = (int)(u - t * pieces) * 256 + 4 * lane;
+    const int e = lane < top_k ? ids[t * top_k + lane] : -1;
+    const uint32_t use = __ballot_sync(0xffffffffu, e >= 0 && e < experts);
+    float4 v[8][2];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int e = j < top_k ? __ldg(ids + t * top_k + j) : -1;
-      use[j] = e >= 0 && e < experts;
-      if (use[j]) v[j] = __ldg(out4 + (t * top_k + j) * vec + c);
+      if (!((use >> j) & 1)) continue;
+      const float* o = out + (t * top_k + j) * hidden + c;
+      v[j][0] = __ldg(reinterpret_cast<const float4*>(o));
+      v[j][1] = __ldg(reinterpret_cast<const float4*>(o + 128));
     }
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float4 acc[2] = {};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (!use[j]) continue;
-      acc.x += v[j].x;
-      acc.y += v[j].y;
-      acc.z += v[j].z;
-      acc.w += v[j].w;
+      if (!((use >> j) & 1)) continue;
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        acc[z].x += v[j][z].x;
+        acc[z].y += v[j][z].y;
+        acc[z].z += v[j][z].z;
+        acc[z].w += v[j][z].w;
+      }
     }
-    reinterpret_cast<uint2*>(y)[i] = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
+#pragma unroll
+    for (int z = 0; z < 2; ++z)
+      *reinterpret_cast<uint2*>(y + t * hidden + c + 128 * z) =
+          make_uint2(pack_bf16(acc[z].x, acc[z].y), pack_bf16(acc[z].z, acc[z].w));
   }
 }
 
 // ---- host side ---------------------------------------------------------------------------------
-// The route block, which also picks the kernels: 16, 32 or 64 routes (decode) while the average
-// expert's fit with room for the fuller ones (an expert's second block reads its weights again),
-// else 128 (prefill).
+// The route block, which also picks the kernels, by the average expert's routes: 16, 32 (decode) or
+// 128 (prefill).  An expert's second block reads its weights again, from L2.  128 experts of 2048 x
+// 768, us with blocks of 16 / 32 / 128: 84 / 86 / 127 at 2 routes an expert, 96 / 98 / 139 at 12,
+// 129 / 108 / 143 at 20, - / 156 / 162 at 39, - / 168 / 168 at 47.
 static int mx_block(int64_t numel, int experts) {
-  return numel <= (int64_t)experts * 5    ? 16
-         : numel <= (int64_t)experts * 18 ? 32
-         : numel <= (int64_t)experts * 44 ? 64
+  return numel <= (int64_t)experts * 12   ? 16
+         : numel <= (int64_t)experts * 44 ? 32
                                           : kMxPrefillBlock;
 }
 
@@ -940,7 +944,7 @@ static cudaError_t launch_mx_gemm(const MxArgs& a, const MxWorkspace& w, cudaStr
   const int k = DOWN ? a.inter : a.hidden;
   if (!make_map_4bit(&mw, DOWN ? a.w2 : a.w13,
                      (uint64_t)a.experts * (DOWN ? a.hidden : 2 * a.inter), k, 128) ||
-      !make_map_8bit(&mt, DOWN ? w.hq : w.xq, 2 * w.capacity, k, 256))
+      !make_map_8bit(&mt, DOWN ? w.hq : w.xq, 2 * w.capacity, k, 32))
     return cudaErrorInvalidValue;
   const int64_t tiles = w.capacity / 128 * (DOWN ? a.hidden / 256 : a.inter / 128);
   const int sms = sm_count();
@@ -983,12 +987,10 @@ cudaError_t launch_mx_experts(const MxArgs& a, const MxWorkspace& w, cudaStream_
                       static_cast<const uint8_t*>(w.out_scale), a.topk_ids, a.experts, a.tokens,
                       a.top_k, a.hidden, static_cast<__nv_bfloat16*>(a.y));
   } else {
-    e = w.block == 16   ? launch_mx_layer<16>(a, w, s)
-        : w.block == 32 ? launch_mx_layer<32>(a, w, s)
-                        : launch_mx_layer<64>(a, w, s);
+    e = w.block == 16 ? launch_mx_layer<16>(a, w, s) : launch_mx_layer<32>(a, w, s);
   }
   if (e != cudaSuccess) return e;
-  return launch_pdl(mx_combine_kernel, stream_grid(a.tokens * (a.hidden / 4)), 256, 0, s,
+  return launch_pdl(mx_combine_kernel, stream_grid(a.tokens * (a.hidden / 8)), 256, 0, s,
                     static_cast<const float*>(w.out), a.topk_ids, a.experts, a.tokens, a.top_k,
                     a.hidden, static_cast<__nv_bfloat16*>(a.y));
 }
