@@ -599,23 +599,35 @@ static int gated_checks(const char* name, int dtype, int64_t tokens, int hidden,
   return EXF_OK;
 }
 
+EXF_API int64_t exf_gated_mlp_workspace_bytes(int64_t tokens, int hidden, int inter) {
+  if (tokens < 0 || hidden < 1 || inter < 1) return -1;
+  return gated_forward_workspace(tokens, hidden, inter);
+}
+
 EXF_API int exf_gated_mlp(const void* x, const void* w13, int dtype, int64_t tokens, int hidden,
-                          int inter, int activation, void* h, float* pre, int32_t* status,
-                          exf_stream_t stream) {
+                          int inter, int activation, void* h, float* pre, void* workspace,
+                          int64_t workspace_bytes, int32_t* status, exf_stream_t stream) {
   const char* name = "exf_gated_mlp";
   const int rc = gated_checks(name, dtype, tokens, hidden, inter, activation);
   if (rc != EXF_OK) return rc;
   if (tokens == 0) return EXF_OK;
   EXF_REQUIRE(x && w13 && h, "%s: null pointer", name);
-  EXF_REQUIRE(aligned16(x) && aligned16(w13) && aligned16(h) && aligned16(pre),
+  EXF_REQUIRE(aligned16(x) && aligned16(w13) && aligned16(h) && aligned16(pre) &&
+                  aligned16(workspace),
               "%s: tensors must be 16-byte aligned", name);
+  EXF_REQUIRE(reinterpret_cast<uintptr_t>(pre) % 32 == 0 &&
+                  reinterpret_cast<uintptr_t>(workspace) % 32 == 0,
+              "%s: pre and the workspace must be 32-byte aligned", name);
+  const int64_t need = gated_forward_workspace(tokens, hidden, inter);
+  EXF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
+              "%s: workspace of %lld bytes required", name, (long long)need);
   GatedArgs a{x, w13, dtype == EXF_BF16, tokens, hidden, inter, activation, status};
-  return cuda_status(launch_gated_forward(a, h, pre, (cudaStream_t)stream), name);
+  return cuda_status(launch_gated_forward(a, h, pre, workspace, (cudaStream_t)stream), name);
 }
 
-EXF_API int64_t exf_gated_mlp_backward_workspace_bytes(int64_t tokens, int inter) {
-  if (tokens < 0 || inter < 1) return -1;
-  return tokens * 2 * inter * 2;
+EXF_API int64_t exf_gated_mlp_backward_workspace_bytes(int64_t tokens, int hidden, int inter) {
+  if (tokens < 0 || hidden < 1 || inter < 1) return -1;
+  return gated_backward_workspace(tokens, hidden, inter);
 }
 
 EXF_API int exf_gated_mlp_backward(const void* dh, const float* pre, const void* x,
@@ -636,7 +648,9 @@ EXF_API int exf_gated_mlp_backward(const void* dh, const float* pre, const void*
   EXF_REQUIRE(aligned16(dh) && aligned16(pre) && aligned16(x) && aligned16(w13) &&
                   aligned16(dx) && aligned16(dw13) && aligned16(workspace),
               "%s: tensors must be 16-byte aligned", name);
-  const int64_t need = exf_gated_mlp_backward_workspace_bytes(tokens, inter);
+  EXF_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 32 == 0,
+              "%s: the workspace must be 32-byte aligned", name);
+  const int64_t need = exf_gated_mlp_backward_workspace_bytes(tokens, hidden, inter);
   EXF_REQUIRE(workspace_bytes >= need, "%s: workspace of %lld bytes required", name,
               (long long)need);
   GatedArgs a{x, w13, dtype == EXF_BF16, tokens, hidden, inter, activation, status};

@@ -20,9 +20,12 @@ struct GatedArgs {
 };
 
 // h [tokens][inter]; pre fp32 [tokens][2 * inter] or null: gate and up projections for backward
-cudaError_t launch_gated_forward(const GatedArgs& a, void* h, float* pre, cudaStream_t s);
-// dx [tokens][hidden] or null, dw13 [2 * inter][hidden] or null; dboth [tokens][2 * inter] scratch
+int64_t gated_forward_workspace(int64_t tokens, int hidden, int inter);
+cudaError_t launch_gated_forward(const GatedArgs& a, void* h, float* pre, void* workspace,
+                                 cudaStream_t s);
+// dx [tokens][hidden] or null, dw13 [2 * inter][hidden] or null
+int64_t gated_backward_workspace(int64_t tokens, int hidden, int inter);
 cudaError_t launch_gated_backward(const GatedArgs& a, const void* dh, const float* pre,
-                                  void* dboth, void* dx, void* dw13, cudaStream_t s);
+                                  void* workspace, void* dx, void* dw13, cudaStream_t s);
 
 }  // namespace exf

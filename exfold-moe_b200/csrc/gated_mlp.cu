@@ -46,6 +46,9 @@ struct GatedGemm {
   void* out;         // [m][n]
   float* pre;        // forward: [m][2 * n] or null
   int32_t* status;
+  int splits;        // the reduction is split over this many tiles, whose fp32 sums go to
+  float* part;       // [splits][m][n] (forward: [splits][m][2 * n]) when there are several
+  bool wide;         // rows of out are 32-byte aligned
 };
 
 // ---- activation -----------------------------------------------------------------------------
@@ -83,6 +86,32 @@ __device__ __forceinline__ void store_16b(void* base, int64_t at, const float* v
   *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at) =
       make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]),
                  pack2<BF16>(v[6], v[7]));
+}
+
+// 16 results, 32 bytes: one store of a whole sector where `wide` says that rows keep its alignment
+// (a row a thread, two 16-byte stores cost L2 a partial write each), the last 8 columns only if n1
+template <bool BF16>
+__device__ __forceinline__ void store_32b(void* base, int64_t at, const float* v, bool wide,
+                                          bool n1) {
+  if (wide && n1) {
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = pack2<BF16>(v[2 * j], v[2 * j + 1]);
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(
+                     static_cast<uint16_t*>(base) + at),
+                 "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]),
+                 "r"(w[7])
+                 : "memory");
+  } else {
+    store_16b<BF16>(base, at, v);
+    if (n1) store_16b<BF16>(base, at + 8, v + 8);
+  }
+}
+// 8 fp32 sums, 32-byte aligned
+__device__ __forceinline__ void store_sums(float* at, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "f"(v[0]),
+               "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
 }
 
 // ---- the GEMM ---------------------------------------------------------------------------------
@@ -149,7 +178,22 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  const int ntiles = p.m_tiles * p.n_tiles;
+  const int mn_tiles = p.m_tiles * p.n_tiles;
+  const int ntiles = mn_tiles * p.splits;
+  // tile t: reduction part, M tile, N tile; k blocks [kb0, kb1)
+  struct Tile {
+    int part, mt, nt, kb0, kb1;
+  };
+  auto tile_of = [&](int t) {
+    Tile r;
+    r.part = t / mn_tiles;
+    t -= r.part * mn_tiles;
+    r.mt = t / p.n_tiles;
+    r.nt = t - r.mt * p.n_tiles;
+    r.kb0 = (int)((int64_t)p.kblocks * r.part / p.splits);
+    r.kb1 = (int)((int64_t)p.kblocks * (r.part + 1) / p.splits);
+    return r;
+  };
   const uint32_t tmem = uniform(sm.tmem_base);
   volatile int* failed = &sm.failed;
 
@@ -158,8 +202,9 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
     uint32_t g = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
-      const int mt = t / p.n_tiles, nt = t - mt * p.n_tiles;
-      for (int kb = 0; kb < p.kblocks; ++kb, ++g) {
+      const Tile tl = tile_of(t);
+      const int mt = tl.mt, nt = tl.nt;
+      for (int kb = tl.kb0; kb < tl.kb1; ++kb, ++g) {
         const int s = g % C::kStages;
         ok = warp_wait(&sm.empty[s], ((g / C::kStages) & 1) ^ 1, failed);
         if (!ok) break;
@@ -198,7 +243,8 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
       if (!ok) break;
       fence_after_sync();
       const uint32_t acc = tmem + static_cast<uint32_t>(b * NT);
-      for (int kb = 0; kb < p.kblocks; ++kb, ++g) {
+      const Tile tl = tile_of(t);
+      for (int kb = tl.kb0; kb < tl.kb1; ++kb, ++g) {
         const int s = g % C::kStages;
         ok = warp_wait(&sm.full[s], (g / C::kStages) & 1, failed);
         if (!ok) break;
@@ -212,7 +258,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
 #pragma unroll
           for (int k = 0; k < kGBK / 16; ++k)
             mma_kind_f16(acc, da + k * (kAMn ? 128 : 2), db + k * (kBMn ? 128 : 2), kIdesc,
-                         (kb > 0 || k > 0) ? 1u : 0u);
+                         (kb > tl.kb0 || k > 0) ? 1u : 0u);
           mma_commit(&sm.empty[s]);
         }
       }
@@ -226,13 +272,30 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
     const int q = warp & 3;
     int i = 0;
     for (int t = blockIdx.x; t < ntiles; t += gridDim.x, ++i) {
-      const int mt = t / p.n_tiles, nt = t - mt * p.n_tiles;
+      const Tile tl = tile_of(t);
+      const int mt = tl.mt, nt = tl.nt;
       const int b = i & 1;
       if (!warp_wait(&sm.acc_full[b], (i >> 1) & 1, failed)) break;
       fence_after_sync();
       const int row = mt * kGBM + q * 32 + lane;
       const uint32_t taddr = tmem + static_cast<uint32_t>(b * NT) + ((uint32_t)(q * 32) << 16);
-      if (KIND == kForward) {
+      if (p.splits > 1) {  // fp32 sums of this part of the reduction
+        constexpr int kRuns = KIND == kForward ? 2 : 1;  // gate and up columns
+        float* at = p.part + ((int64_t)tl.part * p.m + row) * kRuns * p.n;
+#pragma unroll 1
+        for (int c = 0; c < NT; c += 32) {
+          float v[32];
+          __syncwarp();
+          tmem_load32(taddr + c, v);
+          const int run = c / (NT / kRuns);
+          const int col = nt * (NT / kRuns) + c % (NT / kRuns);
+          if (row < p.m) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+              if (col + j < p.n) store_sums(at + run * p.n + col + j, v + j);
+          }
+        }
+      } else if (KIND == kForward) {
 #pragma unroll 1
         for (int c = 0; c < NT / 2; c += 32) {
           float gt[32], up[32];
@@ -244,12 +307,10 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
             if (p.pre) {
               float* pg = p.pre + (int64_t)row * 2 * p.n + col;
 #pragma unroll
-              for (int j = 0; j < 32; j += 4)
+              for (int j = 0; j < 32; j += 8)
                 if (col + j < p.n) {
-                  *reinterpret_cast<float4*>(pg + j) =
-                      make_float4(gt[j], gt[j + 1], gt[j + 2], gt[j + 3]);
-                  *reinterpret_cast<float4*>(pg + p.n + j) =
-                      make_float4(up[j], up[j + 1], up[j + 2], up[j + 3]);
+                  store_sums(pg + j, gt + j);
+                  store_sums(pg + p.n + j, up + j);
                 }
             }
             if (p.activation == kSilu) {
@@ -261,8 +322,10 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
                 gt[j] = gt[j] * gate_sigmoid<kGeluTanh>(gt[j]) * up[j];
             }
 #pragma unroll
-            for (int j = 0; j < 32; j += 8)
-              if (col + j < p.n) store_16b<BF16>(p.out, (int64_t)row * p.n + col + j, gt + j);
+            for (int j = 0; j < 32; j += 16)
+              if (col + j < p.n)
+                store_32b<BF16>(p.out, (int64_t)row * p.n + col + j, gt + j, p.wide,
+                                col + j + 8 < p.n);
           }
         }
       } else {
@@ -274,8 +337,10 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
           const int col = nt * NT + c;
           if (row < p.m) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 8)
-              if (col + j < p.n) store_16b<BF16>(p.out, (int64_t)row * p.n + col + j, v + j);
+            for (int j = 0; j < 32; j += 16)
+              if (col + j < p.n)
+                store_32b<BF16>(p.out, (int64_t)row * p.n + col + j, v + j, p.wide,
+                                col + j + 8 < p.n);
           }
         }
       }
@@ -294,11 +359,66 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
   if (threadIdx.x == 0 && sm.failed && p.status) atomicExch(p.status, 1);
 }
 
+// ---- joining a split reduction --------------------------------------------------------------------
+// out [m][n] from the parts' sums, added in order; forward: h and pre from the gate and up sums.  8
+// columns a thread.
+template <int KIND, bool BF16>
+__global__ void __launch_bounds__(256)
+    gated_join_kernel(const float* part, int splits, int64_t m, int n, int activation, void* out,
+                      float* pre) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr int kRuns = KIND == kForward ? 2 : 1;
+  const int vec = n / 8;
+  const int64_t stride = m * kRuns * n;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < m * vec;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = i / vec;
+    const int c = (int)(i - row * vec) * 8;
+    float v[kRuns][8] = {};
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s)
+#pragma unroll
+      for (int r = 0; r < kRuns; ++r) {
+        const float4* at =
+            reinterpret_cast<const float4*>(part + s * stride + (row * kRuns + r) * n + c);
+        const float4 a = __ldg(at), b = __ldg(at + 1);
+        v[r][0] += a.x;
+        v[r][1] += a.y;
+        v[r][2] += a.z;
+        v[r][3] += a.w;
+        v[r][4] += b.x;
+        v[r][5] += b.y;
+        v[r][6] += b.z;
+        v[r][7] += b.w;
+      }
+    if (KIND == kForward) {
+      float(&u)[8] = v[kRuns - 1];
+      if (pre) {
+#pragma unroll
+        for (int r = 0; r < kRuns; ++r) {
+          float4* at = reinterpret_cast<float4*>(pre + (row * kRuns + r) * n + c);
+          at[0] = make_float4(v[r][0], v[r][1], v[r][2], v[r][3]);
+          at[1] = make_float4(v[r][4], v[r][5], v[r][6], v[r][7]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[0][j] *= (activation == kSilu ? gate_sigmoid<kSilu>(v[0][j])
+                                        : gate_sigmoid<kGeluTanh>(v[0][j])) *
+                   u[j];
+    }
+    store_16b<BF16>(out, row * n + c, v[0]);
+  }
+}
+
 // ---- a few tokens ------------------------------------------------------------------------------
-// Up to 8 tokens: a warp computes one feature (a gate and an up row against every token) with fp32
-// FMAs, so that every SM streams weights; an MMA tile would be 1/16 full and 128 features wide.
-// Bound by the weights' latency and bytes.  TT: tokens rounded up to a power of two.
-constexpr int kFewTokens = 8;
+// Up to 4 tokens: a warp computes one feature (a gate and an up row against every token) with fp32
+// FMAs, so that every SM streams weights; an MMA tile would be 1/32 full and 64 features wide.  us of
+// this kernel and of the tiles with a split reduction: 6 / 10 (512 x 256), 12 / 14 (2048 x 768) and
+// 18 / 18 (4096 x 2048) up to 4 tokens, 31 / 18 at 8 (4096 x 2048).  Bound by the weights' latency and
+// bytes.  TT: tokens rounded up to a power of two.
+constexpr int kFewTokens = 4;
 constexpr int kFewWarps = 4;
 
 template <bool BF16, int TT>
@@ -314,7 +434,7 @@ __global__ void __launch_bounds__(32 * kFewWarps)
   const uint4* wu = reinterpret_cast<const uint4*>(w13 + (int64_t)(inter + f) * hidden);
   const int vecs = hidden / 8;
   float g[TT] = {}, u[TT] = {};
-#pragma unroll 4
+#pragma unroll(TT <= 2 ? 8 : 4)
   for (int c = lane; c < vecs; c += 32) {
     const uint4 a = __ldg(wg + c), b = __ldg(wu + c);
     const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
@@ -409,7 +529,7 @@ static cudaError_t launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, Gat
       done[dev] = true;
     }
   }
-  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles * p.splits;
   const int sms = sm_count();
   const unsigned grid = (unsigned)(sms > 0 && tiles > sms ? sms : tiles);
   return launch_pdl(kern, grid, kGatedThreads, gated_smem_bytes<NT>(), s, ma, mb, p);
@@ -417,25 +537,68 @@ static cudaError_t launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, Gat
 
 static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-template <int NT, bool BF16>
-static cudaError_t forward_nt(const GatedArgs& a, void* h, float* pre, cudaStream_t s) {
-  constexpr auto dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUtensorMap ma, mb;
-  if (!make_map(&ma, a.x, a.tokens, a.hidden, kGBM, dt) ||
-      !make_map(&mb, a.w13, 2 * (int64_t)a.inter, a.hidden, NT / 2, dt))
-    return cudaErrorInvalidValue;
-  GatedGemm p{(int)a.tokens, a.inter, a.hidden, ceil_div(a.tokens, kGBM),
-              ceil_div(a.inter, NT / 2), ceil_div(a.hidden, kGBK), a.activation, h, pre, a.status};
-  return launch_gemm<kForward, NT, BF16>(ma, mb, p, s);
+static unsigned stream_grid(int64_t threads) {
+  int64_t blocks = (threads + 255) / 256;
+  const int lim = 8 * sm_count();
+  if (lim > 0 && blocks > lim) blocks = lim;
+  return (unsigned)(blocks > 0 ? blocks : 1);
 }
 
-// The N tile: 256, halved while the tiles leave more than half of the SMs idle (a narrower tile reads
-// its A rows again for fewer columns, and starts as many more CTAs).
-static int pick_nt(int64_t m, int64_t n256) {  // n256: N tiles of 256 columns, in 64ths
-  const int64_t m_tiles = (m + kGBM - 1) / kGBM;
-  const int sms = sm_count();
-  if (m_tiles * ((n256 + 63) / 64) * 2 > sms) return 256;
-  return m_tiles * ((n256 + 31) / 32) * 2 > sms ? 128 : 64;
+// The N tile and the parts of the reduction of a GEMM [m][n] over k.  Tiles of 256 columns (forward:
+// 128 gate and 128 up) while they fill more than half of the SMs; else narrower ones, and where the
+// reduction is long it is split, at least 8 k blocks a part, until the SMs are full (9 tokens, 4096 x
+// 2048: 31 us with 64 whole tiles of 64 columns, 18 with 32 x 4 of 128; 333 tokens, 1000 x 712: 14 and
+// 16).
+struct GatedPlan {
+  int nt, splits;
+};
+static GatedPlan plan(int kind, int64_t m, int64_t n, int64_t k) {
+  const int sms = sm_count() > 0 ? sm_count() : 1;
+  const int kblocks = ceil_div(k, kGBK);
+  auto tiles = [&](int nt) {
+    return (int64_t)ceil_div(m, kGBM) * ceil_div(n, kind == kForward ? nt / 2 : nt);
+  };
+  if (tiles(256) * 2 > sms) return {256, 1};
+  if (kblocks < 32) return {tiles(128) * 2 > sms ? 128 : 64, 1};
+  int64_t s = sms / tiles(128);
+  if (s > kblocks / 8) s = kblocks / 8;
+  return {128, (int)(s > 1 ? s : 1)};
+}
+static int64_t part_bytes(int kind, int64_t m, int64_t n, int64_t k) {
+  const GatedPlan pl = plan(kind, m, n, k);
+  return pl.splits > 1 ? pl.splits * m * n * (kind == kForward ? 8 : 4) : 0;
+}
+
+template <int KIND, int NT, bool BF16>
+static cudaError_t run_gemm(const void* a, int64_t a_rows, int64_t a_cols, const void* b,
+                            int64_t b_rows, int64_t b_cols, GatedGemm p, cudaStream_t s) {
+  constexpr auto dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, a, a_rows, a_cols, KIND == kGradW ? kGBK : kGBM, dt) ||
+      !make_map(&mb, b, b_rows, b_cols, KIND == kForward ? NT / 2 : kGBK, dt))
+    return cudaErrorInvalidValue;
+  p.m_tiles = ceil_div(p.m, kGBM);
+  p.n_tiles = ceil_div(p.n, KIND == kForward ? NT / 2 : NT);
+  p.kblocks = ceil_div(p.k, kGBK);
+  p.wide = p.n % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 32 == 0;
+  cudaError_t e = launch_gemm<KIND, NT, BF16>(ma, mb, p, s);
+  if (e != cudaSuccess || p.splits == 1) return e;
+  return launch_pdl(gated_join_kernel<KIND, BF16>, stream_grid((int64_t)p.m * (p.n / 8)), 256, 0, s,
+                    static_cast<const float*>(p.part), p.splits, (int64_t)p.m, p.n, p.activation,
+                    p.out, p.pre);
+}
+
+// One product: its A and B tensors as they lie in memory, m, n, k and outputs in p.
+template <int KIND, bool BF16>
+static cudaError_t product(const void* a, int64_t a_rows, int64_t a_cols, const void* b,
+                           int64_t b_rows, int64_t b_cols, GatedGemm p, cudaStream_t s) {
+  const GatedPlan pl = plan(KIND, p.m, p.n, p.k);
+  p.splits = pl.splits;
+  switch (pl.nt) {
+    case 256: return run_gemm<KIND, 256, BF16>(a, a_rows, a_cols, b, b_rows, b_cols, p, s);
+    case 128: return run_gemm<KIND, 128, BF16>(a, a_rows, a_cols, b, b_rows, b_cols, p, s);
+    default: return run_gemm<KIND, 64, BF16>(a, a_rows, a_cols, b, b_rows, b_cols, p, s);
+  }
 }
 
 template <bool BF16, int TT>
@@ -447,77 +610,80 @@ static cudaError_t forward_few(const GatedArgs& a, void* h, float* pre, cudaStre
 }
 
 template <bool BF16>
-static cudaError_t forward_t(const GatedArgs& a, void* h, float* pre, cudaStream_t s) {
+static cudaError_t forward_t(const GatedArgs& a, void* h, float* pre, float* part,
+                             cudaStream_t s) {
   if (a.tokens <= kFewTokens)
     return a.tokens == 1   ? forward_few<BF16, 1>(a, h, pre, s)
            : a.tokens == 2 ? forward_few<BF16, 2>(a, h, pre, s)
-           : a.tokens <= 4 ? forward_few<BF16, 4>(a, h, pre, s)
-                           : forward_few<BF16, 8>(a, h, pre, s);
-  switch (pick_nt(a.tokens, ceil_div(a.inter, 2))) {
-    case 256: return forward_nt<256, BF16>(a, h, pre, s);
-    case 128: return forward_nt<128, BF16>(a, h, pre, s);
-    default: return forward_nt<64, BF16>(a, h, pre, s);
-  }
-}
-
-template <int NT, bool BF16>
-static cudaError_t grad_x(const GatedArgs& a, const void* both, void* dx, cudaStream_t s) {
-  constexpr auto dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUtensorMap ma, mb;
-  if (!make_map(&ma, both, a.tokens, 2 * (int64_t)a.inter, kGBM, dt) ||
-      !make_map(&mb, a.w13, 2 * (int64_t)a.inter, a.hidden, kGBK, dt))
-    return cudaErrorInvalidValue;
-  GatedGemm p{(int)a.tokens, a.hidden, 2 * a.inter, ceil_div(a.tokens, kGBM),
-              ceil_div(a.hidden, NT), ceil_div(2 * (int64_t)a.inter, kGBK), a.activation, dx,
-              nullptr, a.status};
-  return launch_gemm<kGradX, NT, BF16>(ma, mb, p, s);
-}
-
-template <int NT, bool BF16>
-static cudaError_t grad_w(const GatedArgs& a, const void* both, void* dw13, cudaStream_t s) {
-  constexpr auto dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUtensorMap ma, mb;
-  if (!make_map(&ma, both, a.tokens, 2 * (int64_t)a.inter, kGBK, dt) ||
-      !make_map(&mb, a.x, a.tokens, a.hidden, kGBK, dt))
-    return cudaErrorInvalidValue;
-  GatedGemm p{2 * a.inter, a.hidden, (int)a.tokens, ceil_div(2 * (int64_t)a.inter, kGBM),
-              ceil_div(a.hidden, NT), ceil_div(a.tokens, kGBK), a.activation, dw13, nullptr,
-              a.status};
-  return launch_gemm<kGradW, NT, BF16>(ma, mb, p, s);
+                           : forward_few<BF16, 4>(a, h, pre, s);
+  GatedGemm p{};
+  p.m = (int)a.tokens;
+  p.n = a.inter;
+  p.k = a.hidden;
+  p.activation = a.activation;
+  p.out = h;
+  p.pre = pre;
+  p.status = a.status;
+  p.part = part;
+  return product<kForward, BF16>(a.x, a.tokens, a.hidden, a.w13, 2 * (int64_t)a.inter, a.hidden, p,
+                                 s);
 }
 
 template <bool BF16>
 static cudaError_t backward_t(const GatedArgs& a, const void* dh, const float* pre, void* both,
-                              void* dx, void* dw13, cudaStream_t s) {
-  const int64_t work = a.tokens * (a.inter / 8);
-  int64_t blocks = (work + 255) / 256;
-  const int lim = 8 * sm_count();
-  if (lim > 0 && blocks > lim) blocks = lim;
+                              float* part, void* dx, void* dw13, cudaStream_t s) {
   auto* slope = a.activation == kSilu ? gated_slope_kernel<BF16, kSilu>
                                       : gated_slope_kernel<BF16, kGeluTanh>;
-  cudaError_t e = launch_pdl(slope, (unsigned)blocks, 256, 0, s, static_cast<const uint16_t*>(dh),
-                             pre, a.tokens, a.inter, static_cast<uint16_t*>(both));
-  if (e == cudaSuccess && dx) switch (pick_nt(a.tokens, ceil_div(a.hidden, 4))) {
-      case 256: e = grad_x<256, BF16>(a, both, dx, s); break;
-      case 128: e = grad_x<128, BF16>(a, both, dx, s); break;
-      default: e = grad_x<64, BF16>(a, both, dx, s);
-    }
-  if (e == cudaSuccess && dw13) switch (pick_nt(2 * (int64_t)a.inter, ceil_div(a.hidden, 4))) {
-      case 256: e = grad_w<256, BF16>(a, both, dw13, s); break;
-      case 128: e = grad_w<128, BF16>(a, both, dw13, s); break;
-      default: e = grad_w<64, BF16>(a, both, dw13, s);
-    }
+  cudaError_t e = launch_pdl(slope, stream_grid(a.tokens * (a.inter / 8)), 256, 0, s,
+                             static_cast<const uint16_t*>(dh), pre, a.tokens, a.inter,
+                             static_cast<uint16_t*>(both));
+  const int64_t wide = 2 * (int64_t)a.inter;
+  GatedGemm p{};
+  p.activation = a.activation;
+  p.status = a.status;
+  p.part = part;
+  p.n = a.hidden;
+  if (e == cudaSuccess && dx) {
+    p.m = (int)a.tokens;
+    p.k = (int)wide;
+    p.out = dx;
+    e = product<kGradX, BF16>(both, a.tokens, wide, a.w13, wide, a.hidden, p, s);
+  }
+  if (e == cudaSuccess && dw13) {
+    p.m = (int)wide;
+    p.k = (int)a.tokens;
+    p.out = dw13;
+    e = product<kGradW, BF16>(both, a.tokens, wide, a.x, a.tokens, a.hidden, p, s);
+  }
   return e;
 }
 
-cudaError_t launch_gated_forward(const GatedArgs& a, void* h, float* pre, cudaStream_t s) {
-  return a.bf16 ? forward_t<true>(a, h, pre, s) : forward_t<false>(a, h, pre, s);
+int64_t gated_forward_workspace(int64_t tokens, int hidden, int inter) {
+  return tokens <= kFewTokens ? 0 : part_bytes(kForward, tokens, inter, hidden);
+}
+
+static int64_t both_bytes(int64_t tokens, int inter) {
+  return (tokens * 2 * inter * 2 + 255) / 256 * 256;
+}
+int64_t gated_backward_workspace(int64_t tokens, int hidden, int inter) {
+  const int64_t x = part_bytes(kGradX, tokens, hidden, 2 * (int64_t)inter);
+  const int64_t w = part_bytes(kGradW, 2 * (int64_t)inter, hidden, tokens);
+  return both_bytes(tokens, inter) + (x > w ? x : w);
+}
+
+cudaError_t launch_gated_forward(const GatedArgs& a, void* h, float* pre, void* workspace,
+                                 cudaStream_t s) {
+  return a.bf16 ? forward_t<true>(a, h, pre, static_cast<float*>(workspace), s)
+                : forward_t<false>(a, h, pre, static_cast<float*>(workspace), s);
 }
 
 cudaError_t launch_gated_backward(const GatedArgs& a, const void* dh, const float* pre,
-                                  void* dboth, void* dx, void* dw13, cudaStream_t s) {
-  return a.bf16 ? backward_t<true>(a, dh, pre, dboth, dx, dw13, s)
-                : backward_t<false>(a, dh, pre, dboth, dx, dw13, s);
+                                  void* workspace, void* dx, void* dw13, cudaStream_t s) {
+  // [dG dU], then the parts of a split reduction (dx's, then dW13's)
+  float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
+                                         both_bytes(a.tokens, a.inter));
+  return a.bf16 ? backward_t<true>(a, dh, pre, workspace, part, dx, dw13, s)
+                : backward_t<false>(a, dh, pre, workspace, part, dx, dw13, s);
 }
 
 }  // namespace exf

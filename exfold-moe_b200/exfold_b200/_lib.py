@@ -68,8 +68,9 @@ SIGNATURES = {
     "exf_fused_experts_mxfp4_workspace_bytes": (_i64, [_i64, _i, _i, _i, _i]),
     "exf_fused_experts_mxfp4": (_i, [_vp, _vp, _vp, _i64, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _vp,
                                      _vp, _i64, _vp, _vp]),
-    "exf_gated_mlp": (_i, [_vp, _vp, _i, _i64, _i, _i, _i, _vp, _vp, _vp, _vp]),
-    "exf_gated_mlp_backward_workspace_bytes": (_i64, [_i64, _i]),
+    "exf_gated_mlp_workspace_bytes": (_i64, [_i64, _i, _i]),
+    "exf_gated_mlp": (_i, [_vp, _vp, _i, _i64, _i, _i, _i, _vp, _vp, _vp, _i64, _vp, _vp]),
+    "exf_gated_mlp_backward_workspace_bytes": (_i64, [_i64, _i, _i]),
     "exf_gated_mlp_backward": (_i, [_vp, _vp, _vp, _vp, _i, _i64, _i, _i, _i, _vp, _vp, _vp, _i64,
                                     _vp, _vp]),
 }

@@ -523,9 +523,11 @@ def _gated_forward(x, w13, activation, status, keep):
     h = torch.empty(tokens, inter, dtype=x.dtype, device=dev)
     pre = torch.empty(tokens, 2 * inter, dtype=torch.float32, device=dev) if keep else None
     with _on(dev):
+        ws_bytes = L.lib().exf_gated_mlp_workspace_bytes(tokens, hidden, inter)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
         L.check(L.lib().exf_gated_mlp(x.data_ptr(), w13.data_ptr(), _WDT[x.dtype], tokens, hidden,
-                                      inter, activation, h.data_ptr(), _ptr(pre), _ptr(status),
-                                      _stream(dev)))
+                                      inter, activation, h.data_ptr(), _ptr(pre), _ptr(ws),
+                                      ws_bytes, _ptr(status), _stream(dev)))
     return h, pre
 
 
@@ -546,9 +548,9 @@ class _GatedMlp(torch.autograd.Function):
         inter = w13.shape[0] // 2
         dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
         dw13 = torch.empty_like(w13) if ctx.needs_input_grad[1] else None
-        ws_bytes = int(L.lib().exf_gated_mlp_backward_workspace_bytes(tokens, inter))
-        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=x.device)  # [dG dU]
         with _on(x.device):
+            ws_bytes = L.lib().exf_gated_mlp_backward_workspace_bytes(tokens, hidden, inter)
+            ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=x.device)
             L.check(L.lib().exf_gated_mlp_backward(
                 dh.data_ptr(), pre.data_ptr(), x.data_ptr(), w13.data_ptr(), _WDT[x.dtype], tokens,
                 hidden, inter, ctx.activation, _ptr(dx), _ptr(dw13), ws.data_ptr(), ws_bytes,

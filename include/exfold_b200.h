@@ -302,14 +302,15 @@ EXF_API int exf_fused_experts_mxfp4(const void* x, const float* topk_w, const in
  * [tokens][2*inter] receives x W13^T for the backward pass, or is NULL.
  * exf_gated_mlp_backward: from dh [tokens][inter] and pre, dx [tokens][hidden] and dw13
  * [2*inter][hidden] (either may be NULL); the gradients of the two projections are rounded to
- * dtype before the products.  workspace: exf_gated_mlp_backward_workspace_bytes().  No tokens: dw13
- * is zeroed.  hidden and inter multiples of 8; every tensor 16-byte aligned.  status as in
- * exf_fused_experts. */
+ * dtype before the products.  workspace: exf_gated_mlp_workspace_bytes() (may be NULL when that is 0)
+ * and exf_gated_mlp_backward_workspace_bytes(), for the current device.  No tokens: dw13 is zeroed.  hidden and inter multiples of 8; every tensor 16-byte aligned, pre and the workspaces 32-byte.
+ * status as in exf_fused_experts. */
 enum exf_activation { EXF_SILU = 0, EXF_GELU_TANH = 1 };
+EXF_API int64_t exf_gated_mlp_workspace_bytes(int64_t tokens, int hidden, int inter);
 EXF_API int exf_gated_mlp(const void* x, const void* w13, int dtype, int64_t tokens, int hidden,
-                          int inter, int activation, void* h, float* pre, int32_t* status,
-                          exf_stream_t stream);
-EXF_API int64_t exf_gated_mlp_backward_workspace_bytes(int64_t tokens, int inter);
+                          int inter, int activation, void* h, float* pre, void* workspace,
+                          int64_t workspace_bytes, int32_t* status, exf_stream_t stream);
+EXF_API int64_t exf_gated_mlp_backward_workspace_bytes(int64_t tokens, int hidden, int inter);
 EXF_API int exf_gated_mlp_backward(const void* dh, const float* pre, const void* x,
                                    const void* w13, int dtype, int64_t tokens, int hidden,
                                    int inter, int activation, void* dx, void* dw13,
