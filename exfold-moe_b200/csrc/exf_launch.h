@@ -4,12 +4,28 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
+
 namespace exf {
 
 // Blocks that fill every SM of the current device at the kernel's occupancy (cached per
 // device and kernel); 0 if the query fails.
 int persistent_grid(const void* kernel, int threads, size_t dynamic_smem);
 int sm_count();
+
+// Raises a kernel's shared-memory limit once per device.
+template <typename K>
+static cudaError_t allow_smem(K* kern, size_t bytes, std::mutex& mu, bool (&done)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> lock(mu);
+  if (done[dev]) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  done[dev] = e == cudaSuccess;
+  return e;
+}
 
 // Launch as a programmatic dependent of the previous kernel in the stream (the kernel calls
 // griddepcontrol.wait before reading anything that kernel wrote).

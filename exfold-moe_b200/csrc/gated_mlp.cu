@@ -144,6 +144,78 @@ __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr) {
          ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
+// The epilogue of a tile: row `row` of D, columns from TMEM address taddr on (NT of them, a thread a
+// row); every lane of the warp takes part in the TMEM loads.
+template <int KIND, int NT, bool BF16>
+__device__ __forceinline__ void write_tile(const GatedGemm& p, uint32_t taddr, int row, int nt,
+                                           int part) {
+        if (p.splits > 1) {  // fp32 sums of this part of the reduction
+          constexpr int kRuns = KIND == kForward ? 2 : 1;  // gate and up columns
+          float* at = p.part + ((int64_t)part * p.m + row) * kRuns * p.n;
+  #pragma unroll 1
+          for (int c = 0; c < NT; c += 32) {
+            float v[32];
+            __syncwarp();
+            tmem_load32(taddr + c, v);
+            const int run = c / (NT / kRuns);
+            const int col = nt * (NT / kRuns) + c % (NT / kRuns);
+            if (row < p.m) {
+  #pragma unroll
+              for (int j = 0; j < 32; j += 8)
+                if (col + j < p.n) store_sums(at + run * p.n + col + j, v + j);
+            }
+          }
+        } else if (KIND == kForward) {
+  #pragma unroll 1
+          for (int c = 0; c < NT / 2; c += 32) {
+            float gt[32], up[32];
+            __syncwarp();
+            tmem_load32(taddr + c, gt);
+            tmem_load32(taddr + NT / 2 + c, up);
+            const int col = nt * (NT / 2) + c;
+            if (row < p.m) {
+              if (p.pre) {
+                float* pg = p.pre + (int64_t)row * 2 * p.n + col;
+  #pragma unroll
+                for (int j = 0; j < 32; j += 8)
+                  if (col + j < p.n) {
+                    store_sums(pg + j, gt + j);
+                    store_sums(pg + p.n + j, up + j);
+                  }
+              }
+              if (p.activation == kSilu) {
+  #pragma unroll
+                for (int j = 0; j < 32; ++j) gt[j] = gt[j] * gate_sigmoid<kSilu>(gt[j]) * up[j];
+              } else {
+  #pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  gt[j] = gt[j] * gate_sigmoid<kGeluTanh>(gt[j]) * up[j];
+              }
+  #pragma unroll
+              for (int j = 0; j < 32; j += 16)
+                if (col + j < p.n)
+                  store_32b<BF16>(p.out, (int64_t)row * p.n + col + j, gt + j, p.wide,
+                                  col + j + 8 < p.n);
+            }
+          }
+        } else {
+  #pragma unroll 1
+          for (int c = 0; c < NT; c += 32) {
+            float v[32];
+            __syncwarp();
+            tmem_load32(taddr + c, v);
+            const int col = nt * NT + c;
+            if (row < p.m) {
+  #pragma unroll
+              for (int j = 0; j < 32; j += 16)
+                if (col + j < p.n)
+                  store_32b<BF16>(p.out, (int64_t)row * p.n + col + j, v + j, p.wide,
+                                  col + j + 8 < p.n);
+            }
+          }
+        }
+}
+
 template <int KIND, int NT, bool BF16>
 __global__ void __launch_bounds__(kGatedThreads, 1)
     gated_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
@@ -279,71 +351,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
       fence_after_sync();
       const int row = mt * kGBM + q * 32 + lane;
       const uint32_t taddr = tmem + static_cast<uint32_t>(b * NT) + ((uint32_t)(q * 32) << 16);
-      if (p.splits > 1) {  // fp32 sums of this part of the reduction
-        constexpr int kRuns = KIND == kForward ? 2 : 1;  // gate and up columns
-        float* at = p.part + ((int64_t)tl.part * p.m + row) * kRuns * p.n;
-#pragma unroll 1
-        for (int c = 0; c < NT; c += 32) {
-          float v[32];
-          __syncwarp();
-          tmem_load32(taddr + c, v);
-          const int run = c / (NT / kRuns);
-          const int col = nt * (NT / kRuns) + c % (NT / kRuns);
-          if (row < p.m) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 8)
-              if (col + j < p.n) store_sums(at + run * p.n + col + j, v + j);
-          }
-        }
-      } else if (KIND == kForward) {
-#pragma unroll 1
-        for (int c = 0; c < NT / 2; c += 32) {
-          float gt[32], up[32];
-          __syncwarp();
-          tmem_load32(taddr + c, gt);
-          tmem_load32(taddr + NT / 2 + c, up);
-          const int col = nt * (NT / 2) + c;
-          if (row < p.m) {
-            if (p.pre) {
-              float* pg = p.pre + (int64_t)row * 2 * p.n + col;
-#pragma unroll
-              for (int j = 0; j < 32; j += 8)
-                if (col + j < p.n) {
-                  store_sums(pg + j, gt + j);
-                  store_sums(pg + p.n + j, up + j);
-                }
-            }
-            if (p.activation == kSilu) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) gt[j] = gt[j] * gate_sigmoid<kSilu>(gt[j]) * up[j];
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                gt[j] = gt[j] * gate_sigmoid<kGeluTanh>(gt[j]) * up[j];
-            }
-#pragma unroll
-            for (int j = 0; j < 32; j += 16)
-              if (col + j < p.n)
-                store_32b<BF16>(p.out, (int64_t)row * p.n + col + j, gt + j, p.wide,
-                                col + j + 8 < p.n);
-          }
-        }
-      } else {
-#pragma unroll 1
-        for (int c = 0; c < NT; c += 32) {
-          float v[32];
-          __syncwarp();
-          tmem_load32(taddr + c, v);
-          const int col = nt * NT + c;
-          if (row < p.m) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 16)
-              if (col + j < p.n)
-                store_32b<BF16>(p.out, (int64_t)row * p.n + col + j, v + j, p.wide,
-                                col + j + 8 < p.n);
-          }
-        }
-      }
+      write_tile<KIND, NT, BF16>(p, taddr, row, nt, tl.part);
       fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.acc_empty[b]);
@@ -415,8 +423,8 @@ __global__ void __launch_bounds__(256)
 // ---- a few tokens ------------------------------------------------------------------------------
 // Up to 4 tokens: a warp computes one feature (a gate and an up row against every token) with fp32
 // FMAs, so that every SM streams weights; an MMA tile would be 1/32 full and 64 features wide.  us of
-// this kernel and of the tiles with a split reduction: 6 / 10 (512 x 256), 12 / 14 (2048 x 768) and
-// 18 / 18 (4096 x 2048) up to 4 tokens, 31 / 18 at 8 (4096 x 2048).  Bound by the weights' latency and
+// this kernel and of the tiles with a split reduction: 8 / 10 (512 x 256), 12 / 14 (2048 x 768) and
+// 18 / 20 (4096 x 2048) up to 4 tokens, 31 / 20 at 8 (4096 x 2048).  Bound by the weights' latency and
 // bytes.  TT: tokens rounded up to a power of two.
 constexpr int kFewTokens = 4;
 constexpr int kFewWarps = 4;
@@ -475,6 +483,212 @@ __global__ void __launch_bounds__(32 * kFewWarps)
   }
 }
 
+// ---- the GEMM on pairs of SMs -------------------------------------------------------------------
+// Large products: a cluster of two CTAs computes a tile of 256 x 256 with tcgen05.mma cta_group::2.
+// Each CTA loads 128 rows of A and 128 of B into its own shared memory (32 KB a stage instead of 48)
+// and holds 128 rows of D in its TMEM; the MMA, issued by the leader (rank 0), reads both CTAs'
+// operands.  A third less traffic from L2 and into shared memory also buys clock under the power
+// limit.  Pairs / single SMs, us: 8192 tokens, 4096 x 2048, forward 171 / 188 (1.61 PFLOP/s, 0.97 of the
+// measured bf16 burst rate), with gradients 600 / 652; 2048 tokens 53 / 59; 8192 tokens, 256 x 2048
+// (the epilogue bounds it) 33 / 29.
+// Barriers: `full` of the leader counts both CTAs' copies; `empty` and `acc_full` of each CTA are
+// signalled by the leader's commits; `acc_empty` of the leader collects both CTAs' epilogue warps.
+constexpr int kPairStages = 6;
+struct PairSmem {
+  alignas(1024) uint8_t tiles[kPairStages][32768];
+  alignas(8) uint64_t full[kPairStages];
+  alignas(8) uint64_t empty[kPairStages];
+  alignas(8) uint64_t acc_full[2];
+  alignas(8) uint64_t acc_empty[2];
+  alignas(8) uint64_t drain;
+  uint32_t tmem_base;
+  int failed;
+};
+constexpr size_t pair_smem_bytes() { return sizeof(PairSmem) + 1024; }
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+// the address of a shared object in the leader's CTA
+__device__ __forceinline__ uint32_t leader_addr(const void* p) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(p)));
+  return a;
+}
+// a copy into this CTA's shared memory that completes on a barrier of the pair
+__device__ __forceinline__ void pair_load_2d(void* dst, const CUtensorMap* map, uint32_t bar, int c0,
+                                             int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                         uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+// arrives on the barrier at this offset in both CTAs once the MMAs issued so far have completed
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;" ::"r"(smem_addr(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+template <int KIND, bool BF16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
+    gated_pair_kernel(const __grid_constant__ CUtensorMap map_a,
+                      const __grid_constant__ CUtensorMap map_b, const GatedGemm p) {
+  constexpr bool kAMn = KIND == kGradW, kBMn = KIND != kForward;
+  constexpr uint32_t kIdesc =
+      idesc_f16(256, 256, BF16) | (kAMn ? 1u << 15 : 0u) | (kBMn ? 1u << 16 : 0u);
+  constexpr int S = kPairStages;
+  extern __shared__ uint8_t smem_raw[];
+  PairSmem& sm = *reinterpret_cast<PairSmem*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = uniform(threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const int rank = blockIdx.x & 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm.acc_full[b], 1);
+      mbar_init(&sm.acc_empty[b], 8);
+    }
+    mbar_init(&sm.drain, 1);
+    sm.failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_addr(&sm.tmem_base)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  fence_before_sync();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are initialised
+  fence_after_sync();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  const int ntiles = p.m_tiles * p.n_tiles;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const uint32_t tmem = uniform(sm.tmem_base);
+  volatile int* failed = &sm.failed;
+
+  if (warp == 0) {
+    // ---- TMA producer of this CTA's halves
+    uint32_t g = 0;
+    bool ok = true;
+    for (int t = first; t < ntiles && ok; t += step) {
+      const int mt = t / p.n_tiles, nt = t - mt * p.n_tiles;
+      const int row = mt * 256 + rank * 128;
+      for (int kb = 0; kb < p.kblocks; ++kb, ++g) {
+        const int s = g % S;
+        ok = warp_wait(&sm.empty[s], ((g / S) & 1) ^ 1, failed);
+        if (!ok) break;
+        uint8_t* a = sm.tiles[s];
+        uint8_t* b = a + 16384;
+        const uint32_t bar = leader_addr(&sm.full[s]);
+        if (elect_one()) {
+          if (rank == 0) mbar_expect_tx(&sm.full[s], 65536);  // both CTAs' copies
+          if (kAMn) {
+            pair_load_2d(a, &map_a, bar, row, kb * kGBK);
+            pair_load_2d(a + 8192, &map_a, bar, row + 64, kb * kGBK);
+          } else {
+            pair_load_2d(a, &map_a, bar, kb * kGBK, row);
+          }
+          if (kBMn) {
+            pair_load_2d(b, &map_b, bar, nt * 256 + rank * 128, kb * kGBK);
+            pair_load_2d(b + 8192, &map_b, bar, nt * 256 + rank * 128 + 64, kb * kGBK);
+          } else {  // the leader has the gate rows, its peer the up rows
+            pair_load_2d(b, &map_b, bar, kb * kGBK, rank * p.n + nt * 128);
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---- MMA issuer, in the leader
+    if (rank == 0) {
+      uint32_t g = 0;
+      int i = 0;
+      bool ok = true;
+      for (int t = first; t < ntiles && ok; t += step, ++i) {
+        const int b = i & 1;
+        ok = warp_wait(&sm.acc_empty[b], ((i >> 1) & 1) ^ 1, failed);
+        if (!ok) break;
+        fence_after_sync();
+        const uint32_t acc = tmem + static_cast<uint32_t>(b * 256);
+        for (int kb = 0; kb < p.kblocks; ++kb, ++g) {
+          const int s = g % S;
+          ok = warp_wait(&sm.full[s], (g / S) & 1, failed);
+          if (!ok) break;
+          fence_after_sync();
+          const uint32_t base = smem_addr(sm.tiles[s]);
+          const uint64_t da = kAMn ? smem_desc_mn(base) : smem_desc(base);
+          const uint64_t db = kBMn ? smem_desc_mn(base + 16384) : smem_desc(base + 16384);
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < kGBK / 16; ++k)
+              pair_mma(acc, da + k * (kAMn ? 128 : 2), db + k * (kBMn ? 128 : 2), kIdesc,
+                       (kb > 0 || k > 0) ? 1u : 0u);
+            pair_commit(&sm.empty[s]);
+          }
+        }
+        if (!ok) break;
+        if (elect_one()) pair_commit(&sm.acc_full[b]);
+      }
+      if (elect_one()) pair_commit(&sm.drain);
+      mbar_wait_drain(&sm.drain, 0);
+    }
+  } else {
+    // ---- epilogue of this CTA's 128 rows
+    const int q = warp & 3;
+    int i = 0;
+    for (int t = first; t < ntiles; t += step, ++i) {
+      const int mt = t / p.n_tiles, nt = t - mt * p.n_tiles;
+      const int b = i & 1;
+      if (!warp_wait(&sm.acc_full[b], (i >> 1) & 1, failed)) break;
+      fence_after_sync();
+      write_tile<KIND, 256, BF16>(
+          p, tmem + static_cast<uint32_t>(b * 256) + ((uint32_t)(q * 32) << 16),
+          mt * 256 + rank * 128 + q * 32 + lane, nt, 0);
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                         leader_addr(&sm.acc_empty[b]))
+                     : "memory");
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  // neither CTA leaves while the other may still read its operands or signal its barriers; after a
+  // time-out, copies still in flight land first (a load started has at most its memory's latency left)
+  if (sm.failed) {
+    for (int j = 0; j < 256; ++j) __nanosleep(1000);
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, 1);
+  }
+  cluster_sync();
+  if (warp == 1) {
+    __syncwarp();
+    fence_after_sync();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
 // ---- the elementwise part of backward -----------------------------------------------------------
 // both [tokens][2 * inter] = (dh * U * act'(G), dh * act(G)); 8 columns a thread.
 template <bool BF16, int ACT>
@@ -516,19 +730,8 @@ static cudaError_t launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, Gat
   auto* kern = gated_gemm_kernel<KIND, NT, BF16>;
   static std::mutex mu;
   static bool done[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  const cudaError_t e = allow_smem(kern, gated_smem_bytes<NT>(), mu, done);
   if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (!done[dev]) {
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)gated_smem_bytes<NT>());
-      if (e != cudaSuccess) return e;
-      done[dev] = true;
-    }
-  }
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles * p.splits;
   const int sms = sm_count();
   const unsigned grid = (unsigned)(sms > 0 && tiles > sms ? sms : tiles);
@@ -548,9 +751,10 @@ static unsigned stream_grid(int64_t threads) {
 // 128 gate and 128 up) while they fill more than half of the SMs; else narrower ones, and where the
 // reduction is long it is split, at least 8 k blocks a part, until the SMs are full (9 tokens, 4096 x
 // 2048: 31 us with 64 whole tiles of 64 columns, 18 with 32 x 4 of 128; 333 tokens, 1000 x 712: 14 and
-// 16).
+// 16).  Pairs of SMs where their tiles fill the card and the reduction outlasts the epilogue.
 struct GatedPlan {
   int nt, splits;
+  bool pair;  // tiles of 256 x 256 on pairs of SMs
 };
 static GatedPlan plan(int kind, int64_t m, int64_t n, int64_t k) {
   const int sms = sm_count() > 0 ? sm_count() : 1;
@@ -558,11 +762,12 @@ static GatedPlan plan(int kind, int64_t m, int64_t n, int64_t k) {
   auto tiles = [&](int nt) {
     return (int64_t)ceil_div(m, kGBM) * ceil_div(n, kind == kForward ? nt / 2 : nt);
   };
-  if (tiles(256) * 2 > sms) return {256, 1};
-  if (kblocks < 32) return {tiles(128) * 2 > sms ? 128 : 64, 1};
+  if (m >= 1024 && kblocks >= 12 && tiles(256) >= sms) return {256, 1, true};
+  if (tiles(256) * 2 > sms) return {256, 1, false};
+  if (kblocks < 32) return {tiles(128) * 2 > sms ? 128 : 64, 1, false};
   int64_t s = sms / tiles(128);
   if (s > kblocks / 8) s = kblocks / 8;
-  return {128, (int)(s > 1 ? s : 1)};
+  return {128, (int)(s > 1 ? s : 1), false};
 }
 static int64_t part_bytes(int kind, int64_t m, int64_t n, int64_t k) {
   const GatedPlan pl = plan(kind, m, n, k);
@@ -588,12 +793,36 @@ static cudaError_t run_gemm(const void* a, int64_t a_rows, int64_t a_cols, const
                     p.out, p.pre);
 }
 
+template <int KIND, bool BF16>
+static cudaError_t run_pair(const void* a, int64_t a_rows, int64_t a_cols, const void* b,
+                            int64_t b_rows, int64_t b_cols, GatedGemm p, cudaStream_t s) {
+  constexpr auto dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  auto* kern = gated_pair_kernel<KIND, BF16>;
+  static std::mutex mu;
+  static bool done[64] = {};
+  const cudaError_t e = allow_smem(kern, pair_smem_bytes(), mu, done);
+  if (e != cudaSuccess) return e;
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, a, a_rows, a_cols, KIND == kGradW ? kGBK : 128, dt) ||
+      !make_map(&mb, b, b_rows, b_cols, KIND == kForward ? 128 : kGBK, dt))
+    return cudaErrorInvalidValue;
+  p.m_tiles = ceil_div(p.m, 256);
+  p.n_tiles = ceil_div(p.n, KIND == kForward ? 128 : 256);
+  p.kblocks = ceil_div(p.k, kGBK);
+  p.wide = p.n % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 32 == 0;
+  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+  const int64_t pairs = sm_count() > 1 ? sm_count() / 2 : 1;
+  return launch_pdl(kern, (unsigned)(2 * (tiles < pairs ? tiles : pairs)), kGatedThreads,
+                    pair_smem_bytes(), s, ma, mb, p);
+}
+
 // One product: its A and B tensors as they lie in memory, m, n, k and outputs in p.
 template <int KIND, bool BF16>
 static cudaError_t product(const void* a, int64_t a_rows, int64_t a_cols, const void* b,
                            int64_t b_rows, int64_t b_cols, GatedGemm p, cudaStream_t s) {
   const GatedPlan pl = plan(KIND, p.m, p.n, p.k);
   p.splits = pl.splits;
+  if (pl.pair) return run_pair<KIND, BF16>(a, a_rows, a_cols, b, b_rows, b_cols, p, s);
   switch (pl.nt) {
     case 256: return run_gemm<KIND, 256, BF16>(a, a_rows, a_cols, b, b_rows, b_cols, p, s);
     case 128: return run_gemm<KIND, 128, BF16>(a, a_rows, a_cols, b, b_rows, b_cols, p, s);

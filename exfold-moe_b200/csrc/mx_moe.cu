@@ -878,20 +878,6 @@ MxWorkspace mx_workspace(int64_t tokens, int top_k, int experts, int hidden, int
   return w;
 }
 
-// Raises a kernel's shared-memory limit once per device.
-template <typename K>
-static cudaError_t allow_smem(K* kern, size_t bytes, std::mutex& mu, bool (&done)[64]) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  std::lock_guard<std::mutex> lock(mu);
-  if (done[dev]) return cudaSuccess;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  done[dev] = e == cudaSuccess;
-  return e;
-}
-
 static MxLayerParams layer_params(const MxArgs& a, const MxWorkspace& w) {
   MxLayerParams p{};
   p.routes = {w.num_post_pad, w.expert_ids, w.sorted_ids};

@@ -81,7 +81,11 @@ def status():
 
 SHAPES = [(1, 8, 8), (1, 2048, 768), (2, 64, 24), (3, 1000, 712), (5, 72, 40), (8, 512, 256),
           (9, 128, 136), (17, 264, 200), (64, 2048, 768), (127, 320, 128), (128, 64, 128),
-          (129, 4096, 264), (333, 1000, 712), (700, 136, 1032), (1500, 640, 520)]
+          (129, 4096, 264), (333, 1000, 712), (700, 136, 1032), (1500, 640, 520),
+          # split reductions: of the forward pass, dx and dW
+          (20, 4104, 72), (9, 2048, 2056), (2200, 72, 40), (4100, 264, 136),
+          # pairs of SMs: the forward pass, dx and dW, rows past the last pair tile
+          (1100, 776, 2184), (1100, 4360, 392), (1057, 2312, 1032)]
 
 
 @pytest.mark.parametrize("activation", ["silu", "gelu_tanh"])
