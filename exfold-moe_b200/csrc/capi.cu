@@ -561,7 +561,8 @@ EXF_API int exf_fused_experts_mxfp4(const void* x, const float* topk_w, const in
   if (hidden % 256 != 0 || inter % 128 != 0)
     return fail(EXF_ERR_UNSUPPORTED,
                 "%s: hidden must be a multiple of 256 and intermediate a multiple of 128", name);
-  if ((int64_t)experts * 2 * inter >= ((int64_t)1 << 31) ||
+  if (hidden >= (1 << 23) || inter >= (1 << 23) ||
+      (int64_t)experts * 2 * inter >= ((int64_t)1 << 31) ||
       (int64_t)experts * hidden >= ((int64_t)1 << 31))
     return fail(EXF_ERR_UNSUPPORTED, "%s: shape too large", name);
   if (tokens == 0) return EXF_OK;
@@ -591,7 +592,8 @@ static int gated_checks(const char* name, int dtype, int64_t tokens, int hidden,
   EXF_REQUIRE(tokens >= 0 && hidden >= 1 && inter >= 1, "%s: bad shape", name);
   if (hidden % 8 != 0 || inter % 8 != 0)
     return fail(EXF_ERR_UNSUPPORTED, "%s: hidden and intermediate must be multiples of 8", name);
-  if (tokens >= ((int64_t)1 << 30) || hidden >= (1 << 29) || inter >= (1 << 29) ||
+  // (a reduction of 2^24 stays far inside the kernels' bounded waits)
+  if (tokens >= (1 << 24) || hidden >= (1 << 23) || inter >= (1 << 23) ||
       ((tokens + 127) / 128) * (((int64_t)inter + 31) / 32) >= ((int64_t)1 << 31) ||
       ((tokens + 127) / 128) * (((int64_t)hidden + 31) / 32) >= ((int64_t)1 << 31) ||
       (((int64_t)inter + 63) / 64) * (((int64_t)hidden + 31) / 32) >= ((int64_t)1 << 31))

@@ -389,6 +389,14 @@ def fused_experts(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor,
     return y
 
 
+def _status_ptr(status: torch.Tensor | None) -> int | None:
+    if status is None:
+        return None
+    if status.dtype != torch.int32 or status.numel() < 1:
+        raise TypeError("status must be an int32 tensor of one element")
+    return status.data_ptr()
+
+
 # ---- microscaled 4-bit floating point -----------------------------------------------------------
 def quantize_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """MXFP4 form of x [..., cols] (fp32, bf16 or fp16): codes uint8 [..., 16 * blocks] and scales
@@ -498,6 +506,8 @@ def fused_experts_mxfp4(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.T
             raise ValueError(f"weights of {experts} experts, hidden {hidden} and intermediate "
                              f"{inter}: a tensor {tuple(t.shape)} must be {shape}")
     x, w13, s13, w2, s2 = (_aligned(t, 32) for t in (x, w13, s13, w2, s2))
+    if topk_ids.dtype != torch.int32:  # ids past int32 stay out of range
+        topk_ids = topk_ids.clamp(-1, experts)
     ids = topk_ids.to(torch.int32).contiguous()
     wts = topk_w.float().contiguous()
     y = torch.empty_like(x)
@@ -510,7 +520,7 @@ def fused_experts_mxfp4(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.T
         L.check(L.lib().exf_fused_experts_mxfp4(
             x.data_ptr(), wts.data_ptr(), ids.data_ptr(), tokens, top_k, w13.data_ptr(),
             s13.data_ptr(), w2.data_ptr(), s2.data_ptr(), experts, hidden, inter, y.data_ptr(),
-            ws.data_ptr(), ws_bytes, _ptr(status), _stream(dev)))
+            ws.data_ptr(), ws_bytes, _status_ptr(status), _stream(dev)))
     return y
 
 
@@ -527,7 +537,7 @@ def _gated_forward(x, w13, activation, status, keep):
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
         L.check(L.lib().exf_gated_mlp(x.data_ptr(), w13.data_ptr(), _WDT[x.dtype], tokens, hidden,
                                       inter, activation, h.data_ptr(), _ptr(pre), _ptr(ws),
-                                      ws_bytes, _ptr(status), _stream(dev)))
+                                      ws_bytes, _status_ptr(status), _stream(dev)))
     return h, pre
 
 
@@ -554,7 +564,7 @@ class _GatedMlp(torch.autograd.Function):
             L.check(L.lib().exf_gated_mlp_backward(
                 dh.data_ptr(), pre.data_ptr(), x.data_ptr(), w13.data_ptr(), _WDT[x.dtype], tokens,
                 hidden, inter, ctx.activation, _ptr(dx), _ptr(dw13), ws.data_ptr(), ws_bytes,
-                _ptr(ctx.status), _stream(x.device)))
+                _status_ptr(ctx.status), _stream(x.device)))
         return dx, dw13, None, None
 
 

@@ -6,7 +6,9 @@ fp32 chains):
   |dG| <= (e_x + t |x|) |W|^T =: a (the same for U); the logistic function within r = 2^-19;
   |dh| <= 1.13 a |U| + (|act| + 1.13 a) a + 2 r |h|, then its two-term form: 2^-9 |h| plus
   2^-22 of the largest |h| of its block of 32;
-  |dy| <= sum_j w_j (|dh| + t |h|) |W2|^T + 9 * 2^-24 sum_j |w_j o_j| + u |y|.
+  |dy| <= sum_j w_j (|dh| + t |h|) |W2|^T + 9 * 2^-24 sum_j |w_j o_j| + u |y|, and 2^-14 of the largest
+  |w_j o_j| of its 32 columns where route outputs are held in 16 bits (multiples of a power of two u
+  with that largest in [2^13 u, 2^14 u), so within u / 2; never below u = 2^-126).
 """
 
 from __future__ import annotations
@@ -73,6 +75,8 @@ def formula(x, tw, ids, w13, w2):
         w = tw[at, slot].unsqueeze(1)
         y.index_add_(0, at, w * o)
         bound.index_add_(0, at, w.abs() * (eo + 9 * 2.0 ** -24 * (o.abs() + eo)))
+        if ids.numel() > 44 * w13.shape[0]:
+            bound.index_add_(0, at, 2.0 ** -14 * block_max(w.abs() * (o.abs() + eo)) + 2.0 ** -127)
     return y, bound * (1 + 2.0 ** -8) + 2.0 ** -9 * y.abs() + 2.0 ** -134
 
 
@@ -134,6 +138,24 @@ def test_masked_routes_and_tokens():
     assert torch.count_nonzero(y) == 0
 
 
+def test_prefill_values_far_apart():
+    """The 16-bit route outputs: expert outputs from 2^-100 to 2^100, empty and NaN ones."""
+    tw, ids = routing(700, 4, 2, seed=30)
+    p13, p2 = weights(4, 256, 128, seed=31)
+    x = tokens_of(700, 256, seed=32)
+    size = torch.exp2(torch.arange(700, device=DEV) % 100 - 50.0).unsqueeze(1)
+    x = (x.float() * size).bfloat16()
+    x[5] = 0.0
+    tw[6] = 0.0
+    y = run(x, tw, ids, p13, p2)
+    near(y, *formula(x, tw, ids, p13[2], p2[2]))
+    tw[7, 0], tw[8, 1] = math.nan, math.inf
+    got = run(x, tw, ids, p13, p2)
+    keep = [i for i in range(700) if i not in (7, 8)]
+    assert torch.equal(got[keep], y[keep])
+    assert not bool(torch.isfinite(got[7:9]).any())
+
+
 def test_values_far_apart_and_not_finite():
     """Blocks of zeros, of the smallest and of large values; a token with an infinity or NaN gives
     NaN and leaves the others as they are."""
@@ -182,7 +204,6 @@ def test_unaligned_and_strided_inputs():
     tw, ids = routing(20, 8, 4, seed=10)
     p13, p2 = weights(8, 256, 128, seed=11)
     x = tokens_of(20, 256, seed=12)
-    want = run(x, tw, ids, p13, p2)
     wide = torch.zeros(20, 261, dtype=torch.bfloat16, device=DEV)
     wide[:, 5:] = x
 
@@ -191,8 +212,13 @@ def test_unaligned_and_strided_inputs():
         flat[n:] = t.reshape(-1)
         return flat[n:].view(t.shape)
 
+    far = ids.long()
+    far[3, 1] += 1 << 32  # out of range, although its low 32 bits are an expert
+    masked = ids.clone()
+    masked[3, 1] = -1
+    want = run(x, tw, masked, p13, p2)
     got = ops.fused_experts_mxfp4(
-        wide[:, 5:], tw.double(), ids.long(), shifted(p13[0], 1),
+        wide[:, 5:], tw.double(), far, shifted(p13[0], 1),
         shifted(ops.tile_mxfp4_scales(p13[1]), 3), shifted(p2[0], 16),
         shifted(ops.tile_mxfp4_scales(p2[1]), 8))
     assert torch.equal(got, want)

@@ -49,6 +49,9 @@ def test_gated():
         ops.gated_mlp(x[:, :60], w[:, :60])
     with pytest.raises(NotImplementedError):
         ops.gated_mlp(x, w[:24 - 4])
+    for status in (torch.zeros(1, device=DEV), torch.zeros(0, dtype=torch.int32, device=DEV)):
+        with pytest.raises(TypeError):
+            ops.gated_mlp(x, w, status=status)
 
 
 def test_experts():

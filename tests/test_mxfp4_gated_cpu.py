@@ -79,7 +79,9 @@ def test_gated_refusals():
     refused(gated(inter=4), L.EXF_ERR_UNSUPPORTED, "multiples of 8")
     refused(gated(hidden=0), L.EXF_ERR_INVALID, "shape")
     refused(gated(tokens=-1), L.EXF_ERR_INVALID, "shape")
-    refused(gated(tokens=1 << 31), L.EXF_ERR_UNSUPPORTED, "large")
+    refused(gated(tokens=1 << 24), L.EXF_ERR_UNSUPPORTED, "large")
+    refused(gated(hidden=1 << 23), L.EXF_ERR_UNSUPPORTED, "large")
+    refused(gated(pre=ctypes.c_void_p(80)), L.EXF_ERR_INVALID, "32-byte")
     refused(gated(x=None), L.EXF_ERR_INVALID, "null")
     refused(gated(x=ODD), L.EXF_ERR_INVALID, "aligned")
     refused(gated(pre=ODD), L.EXF_ERR_INVALID, "aligned")
