@@ -380,14 +380,15 @@ cudaError_t launch_align(int id_dtype, const AlignParams& p, cudaStream_t s) {
 
 int64_t align_gather_max_numel() { return kAlignSmall; }
 
+// Slices of at least `least` routes, one CTA each, at most one CTA per SM.
 template <typename Put>
 static cudaError_t launch_align_put(const AlignParams& p, const void* x, int top_k, int hidden,
-                                    const Put& put, int32_t* zero, int zero_n, cudaStream_t s) {
+                                    const Put& put, int least, int32_t* zero, int zero_n,
+                                    cudaStream_t s) {
   if (p.numel < 1 || p.numel > kAlignSmall || hidden % 8 != 0) return cudaErrorInvalidValue;
-  // slices of at least 16 routes, one CTA each, at most one CTA per SM
   const int sms = sm_count() > 0 ? sm_count() : 1;
   int64_t slice = (p.numel + sms - 1) / sms;
-  if (slice < 16) slice = 16;
+  if (slice < least) slice = least;
   const unsigned grid = (unsigned)((p.numel + slice - 1) / slice);
   return launch_pdl(align_gather_kernel<int32_t, Put>, grid, kAlignThreads, 0, s, p,
                     static_cast<const uint4*>(x), top_k, hidden / 8, put, (int)slice, zero, zero_n);
@@ -395,15 +396,16 @@ static cudaError_t launch_align_put(const AlignParams& p, const void* x, int top
 
 cudaError_t launch_align_gather(const AlignParams& p, const void* x, int top_k, int hidden,
                                 void* xs, int32_t* zero, int zero_n, cudaStream_t s) {
-  return launch_align_put(p, x, top_k, hidden, CopyRows{static_cast<uint4*>(xs), hidden / 8}, zero,
-                          zero_n, s);
+  return launch_align_put(p, x, top_k, hidden, CopyRows{static_cast<uint4*>(xs), hidden / 8}, 16,
+                          zero, zero_n, s);
 }
 
 cudaError_t launch_align_split(const AlignParams& p, const void* x, int top_k, int hidden,
                                uint8_t* xq, uint8_t* xs, int32_t* zero, int zero_n,
                                cudaStream_t s) {
   if (hidden % 256 != 0) return cudaErrorInvalidValue;
-  return launch_align_put(p, x, top_k, hidden, SplitRows{{xq, xs, hidden, p.block_size}}, zero,
+  // (one token x top-8: 25.1 us for the layer with slices of 16 routes, 22.5 with slices of one)
+  return launch_align_put(p, x, top_k, hidden, SplitRows{{xq, xs, hidden, p.block_size}}, 1, zero,
                           zero_n, s);
 }
 
