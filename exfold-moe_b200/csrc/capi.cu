@@ -531,9 +531,8 @@ EXF_API int exf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, in
               "%s: bad shape", name);
   if (rows == 0 || cols == 0) return EXF_OK;
   EXF_REQUIRE(codes && scales && out, "%s: null pointer", name);
-  EXF_REQUIRE(aligned16(codes), "%s: codes must be 16-byte aligned", name);
-  EXF_REQUIRE(reinterpret_cast<uintptr_t>(out) % (dtype == EXF_F32 ? 4 : 2) == 0,
-              "%s: out is not aligned to its elements", name);
+  EXF_REQUIRE(aligned16(codes) && aligned16(out), "%s: codes and out must be 16-byte aligned",
+              name);
   return cuda_status(
       launch_mxfp4_dequantize(codes, scales, rows, cols, out, dtype, (cudaStream_t)stream), name);
 }

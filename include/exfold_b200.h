@@ -267,7 +267,7 @@ EXF_API int exf_decode_fused_experts(const void* x, const float* w, const int32_
  * column 2 i is in the low half of byte i.  A block with an infinity or NaN gets the scale byte
  * 255 and codes 0.  Columns past the last fill up its block as zeros.
  * exf_mxfp4_dequantize: the values code * 2^(scale - 127), rounded to dtype, in out [rows][cols]
- * (scale byte 255: NaN).  codes 16-byte aligned. */
+ * (scale byte 255: NaN).  codes and out 16-byte aligned. */
 EXF_API int exf_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t cols,
                                int64_t row_stride, uint8_t* codes, uint8_t* scales,
                                exf_stream_t stream);
