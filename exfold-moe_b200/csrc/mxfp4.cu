@@ -13,7 +13,7 @@
 // 16-byte vector divides are read through aligned vectors shifted into place, and written in the
 // pieces that share aligned places of the result.  403 M bf16 values (196608 x 2048): 155 us to quantise,
 // 185 to read back (6.6 and 5.5 TB/s; four fifths of the latter's bytes are writes); with 2044
-// columns 298 and 352, bound by the shifting and the row arithmetic.
+// columns 309 and 283, bound by the shifting and the row arithmetic.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -102,78 +102,89 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
   return __uint_as_float(byte == 255u ? 0x7fffffffu : byte == 0u ? 0x00400000u : byte << 23);
 }
 
+// One vector, element by element, of what lies in [lo, hi); the rest zero.
+template <typename T>
+__device__ __noinline__ uint4 load_edge(const char* a, const T* lo, const T* hi) {
+  uint32_t e[4] = {0, 0, 0, 0};
+  constexpr int kPer = 16 / (int)sizeof(T);
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const T* t = reinterpret_cast<const T*>(a) + j;
+    if (t < lo || t >= hi) continue;
+    if (sizeof(T) == 4)
+      e[j] = *reinterpret_cast<const uint32_t*>(t);
+    else
+      e[j / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(t) << (16 * (j & 1));
+  }
+  return make_uint4(e[0], e[1], e[2], e[3]);
+}
+
 // The 8 (n < 8: the first n) values at p, which need not be aligned to 16 bytes, the rest zero:
-// aligned vectors shifted into place; [lo, hi) is the memory that may be read.
+// aligned vectors shifted into place.  [lo, hi) is the memory that may be read; the vectors at its
+// ends are read element by element.
 template <typename T>
 __device__ __forceinline__ void load8_any(const T* p, int n, const T* lo, const T* hi, Vec8<T>& v) {
   constexpr int W = Vec8<T>::kWords;
-  if (n <= 0) {
-#pragma unroll
-    for (int i = 0; i < W; ++i) v.w[i] = 0;
-    return;
-  }
   const uint32_t sh = reinterpret_cast<uintptr_t>(p) & 15u;
-  if (sh == 0 && n == 8) {
-    load8(p, v);
-    return;
-  }
   const char* at = reinterpret_cast<const char*>(p) - sh;
-  const int need = (int)sh + n * (int)sizeof(T);
   uint32_t w[W + 4];
+  if (p - lo >= 8 && hi - p >= 16) {
 #pragma unroll
-  for (int k = 0; k < W / 4 + 1; ++k) {
-    uint4 q = make_uint4(0, 0, 0, 0);
-    if (16 * k < need) {
-      const char* a = at + 16 * k;
-      if (a >= reinterpret_cast<const char*>(lo) && a + 16 <= reinterpret_cast<const char*>(hi)) {
-        q = __ldg(reinterpret_cast<const uint4*>(a));
-      } else {  // the first or last vector of the tensor: element by element
-        uint32_t e[4] = {0, 0, 0, 0};
-        constexpr int kPer = 16 / (int)sizeof(T);
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const T* t = reinterpret_cast<const T*>(a) + j;
-          if (t < lo || t >= hi) continue;
-          if (sizeof(T) == 4)
-            e[j] = *reinterpret_cast<const uint32_t*>(t);
-          else
-            e[j / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(t) << (16 * (j & 1));
-        }
-        q = make_uint4(e[0], e[1], e[2], e[3]);
-      }
+    for (int k = 0; k < W / 4 + 1; ++k) {
+      uint4 q = make_uint4(0, 0, 0, 0);
+      if (k < W / 4 || sh) q = __ldg(reinterpret_cast<const uint4*>(at) + k);
+      w[4 * k] = q.x;
+      w[4 * k + 1] = q.y;
+      w[4 * k + 2] = q.z;
+      w[4 * k + 3] = q.w;
     }
-    w[4 * k] = q.x;
-    w[4 * k + 1] = q.y;
-    w[4 * k + 2] = q.z;
-    w[4 * k + 3] = q.w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < W / 4 + 1; ++k) {
+      uint4 q = make_uint4(0, 0, 0, 0);
+      if (16 * k < (int)sh + n * (int)sizeof(T)) q = load_edge(at + 16 * k, lo, hi);
+      w[4 * k] = q.x;
+      w[4 * k + 1] = q.y;
+      w[4 * k + 2] = q.z;
+      w[4 * k + 3] = q.w;
+    }
+  }
+  if (sh) {
+#pragma unroll
+    for (int d = 1; d <= 2; d *= 2)  // whole words: 1, then 2
+      if ((sh >> 2) & d) {
+#pragma unroll
+        for (int i = 0; i + d < W + 4; ++i) w[i] = w[i + d];
+      }
+    if (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (sh & 2u) * 8);
+    }
   }
 #pragma unroll
-  for (int d = 1; d <= 2; d *= 2)  // whole words: 1, then 2
-    if ((sh >> 2) & d) {
+  for (int i = 0; i < W; ++i) v.w[i] = w[i];
+  if (n < 8) {  // the values past the n-th
 #pragma unroll
-      for (int i = 0; i + d < W + 4; ++i) w[i] = w[i + d];
-    }
-#pragma unroll
-  for (int i = 0; i < W; ++i) {
-    v.w[i] = sizeof(T) == 4 ? w[i] : __funnelshift_r(w[i], w[i + 1], (sh & 2u) * 8);
-    // values past the n-th
-    if (sizeof(T) == 4) {
-      if (i >= n) v.w[i] = 0;
-    } else if (2 * i + 1 >= n) {
-      v.w[i] = 2 * i >= n ? 0u : v.w[i] & 0xffffu;
+    for (int i = 0; i < W; ++i) {
+      if (sizeof(T) == 4) {
+        if (i >= n) v.w[i] = 0;
+      } else if (2 * i + 1 >= n) {
+        v.w[i] = 2 * i >= n ? 0u : v.w[i] & 0xffffu;
+      }
     }
   }
 }
 
 // FLAT: cols a multiple of 32, rows contiguous, x 16-byte aligned: the matrix is one run of rows *
-// cols values.  Otherwise every 4 lanes find the row of their block.
-template <typename T, bool FLAT>
+// cols values.  Otherwise every 4 lanes find the row of their block.  I: the type of a block's number
+// (a 64-bit division costs several times a 32-bit one).
+template <typename T, bool FLAT, typename I>
 __global__ void __launch_bounds__(kMxThreads)
     mxfp4_quantize_kernel(const T* x, int64_t rows, int64_t cols, int64_t row_stride,
                           uint8_t* codes, uint8_t* scales) {
   const int lane = threadIdx.x & 31;
-  const int64_t blocks = (cols + 31) / 32;       // of one row
-  const int64_t total = rows * blocks;
+  const I blocks = (I)((cols + 31) / 32);        // of one row
+  const int64_t total = rows * (int64_t)blocks;
   const int64_t strips = (total + 8 * kUnits - 1) / (8 * kUnits);
   const int64_t warps = (int64_t)gridDim.x * (kMxThreads / 32);
   const T* hi = x + (rows - 1) * row_stride + cols;
@@ -191,11 +202,15 @@ __global__ void __launch_bounds__(kMxThreads)
 #pragma unroll
           for (int j = 0; j < Vec8<T>::kWords; ++j) v[i].w[j] = 0;
       } else {
-        // (a 64-bit division costs several times a 32-bit one)
-        const int64_t row = total <= 0xffffffffll ? (uint32_t)q / (uint32_t)blocks : q / blocks;
-        const int64_t c = (q - row * blocks) * 32 + 8 * (lane & 3);
-        const int n = q >= total || c >= cols ? 0 : cols - c < 8 ? (int)(cols - c) : 8;
-        load8_any(x + row * row_stride + c, n, x, hi, v[i]);
+        const I row = (I)q / blocks;
+        const int64_t c = (int64_t)((I)q - row * blocks) * 32 + 8 * (lane & 3);
+        if (q < total && c < cols) {
+          load8_any(x + (int64_t)row * row_stride + c, cols - c < 8 ? (int)(cols - c) : 8, x, hi,
+                    v[i]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < Vec8<T>::kWords; ++j) v[i].w[j] = 0;
+        }
       }
     }
 #pragma unroll
@@ -321,42 +336,45 @@ __global__ void __launch_bounds__(kMxThreads)
 }
 
 // Any cols: a thread takes the values of a row that share 8 aligned places of the result (the row's
-// first and last may be fewer): a codes word and its neighbour shifted into place, two scales.
-template <typename T>
+// first and last may be fewer): a codes word and its neighbour shifted into place, two scales.  I: the
+// type of values' numbers.
+template <typename T, typename I>
 __global__ void __launch_bounds__(kMxThreads)
     mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                            int64_t rows, int64_t cols, T* out) {
-  const int64_t blocks = (cols + 31) / 32;
-  const int64_t per_row = (cols + 14) / 8;
-  const int64_t total = rows * per_row;
+                            int64_t rows, int64_t cols64, T* out) {
+  const I cols = (I)cols64;
+  const I blocks = (cols + 31) / 32;
+  const I per_row = (cols + 14) / 8;
+  const int64_t total = rows * (int64_t)per_row;
   const int64_t stride = (int64_t)gridDim.x * kMxThreads;
   const uint32_t* words = reinterpret_cast<const uint32_t*>(codes);
   for (int64_t g0 = (int64_t)blockIdx.x * kMxThreads + threadIdx.x; g0 < total;
        g0 += kUnits * stride) {
     uint32_t q[kUnits], sb[kUnits];
-    int64_t at[kUnits];
+    I at[kUnits];
     int n[kUnits], in[kUnits];  // values, and how many of them are of the first block
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
       const int64_t g = g0 + i * stride;
       n[i] = 0;
       if (g >= total) continue;
-      // (a 64-bit division costs several times a 32-bit one)
-      const int64_t row = total <= 0xffffffffll ? (uint32_t)g / (uint32_t)per_row : g / per_row;
-      const int64_t c0 = (g - row * per_row) * 8 - ((row * cols) & 7);
-      const int64_t c = c0 > 0 ? c0 : 0, end = c0 + 8 < cols ? c0 + 8 : cols;
+      const I row = (I)g / per_row;
+      const I k8 = ((I)g - row * per_row) * 8;
+      const I before = (row * cols) & 7;  // places of the first 8 that belong to earlier rows
+      const I c = k8 > before ? k8 - before : 0;
+      const I end = k8 + 8 - before < cols ? k8 + 8 - before : cols;
       if (c >= end) continue;
       n[i] = (int)(end - c);
       in[i] = 32 - (int)(c & 31);
       at[i] = row * cols + c;
-      const uint32_t* w = words + row * blocks * 4 + (c >> 3);
+      const I w = row * blocks * 4 + (c >> 3);
       const int k = (int)c & 7;
-      q[i] = __ldg(w);
+      q[i] = __ldg(words + w);
       // (the neighbour is of this row where the values reach into it)
-      if (k + n[i] > 8) q[i] = __funnelshift_r(q[i], __ldg(w + 1), 4 * k);
+      if (k + n[i] > 8) q[i] = __funnelshift_r(q[i], __ldg(words + w + 1), 4 * k);
       else q[i] >>= 4 * k;
-      const uint8_t* s = scales + row * blocks;
-      sb[i] = __ldg(s + (c >> 5)) | (uint32_t)__ldg(s + ((end - 1) >> 5)) << 8;
+      const I s = row * blocks;
+      sb[i] = __ldg(scales + s + (c >> 5)) | (uint32_t)__ldg(scales + s + ((end - 1) >> 5)) << 8;
     }
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
@@ -377,6 +395,8 @@ static unsigned mx_grid(const void* kernel, int64_t warps) {
   const int64_t most = persistent_grid(kernel, kMxThreads, 0);
   return (unsigned)(most > 0 && need > most ? most : need);
 }
+// every number of a value, padding and a grid's overshoot included, fits 32 bits
+static bool narrow(int64_t rows, int64_t cols) { return rows * (cols + 64) < ((int64_t)1 << 31); }
 static bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <typename T>
@@ -385,7 +405,9 @@ static cudaError_t quantize_t(const void* xv, int64_t rows, int64_t cols, int64_
   const T* x = static_cast<const T*>(xv);
   if (rows == 1) stride = cols;
   const bool flat = cols % 32 == 0 && stride == cols && al16(x);
-  auto* k = flat ? mxfp4_quantize_kernel<T, true> : mxfp4_quantize_kernel<T, false>;
+  auto* k = flat              ? mxfp4_quantize_kernel<T, true, int64_t>
+            : narrow(rows, cols) ? mxfp4_quantize_kernel<T, false, uint32_t>
+                                 : mxfp4_quantize_kernel<T, false, int64_t>;
   const int64_t strips = (rows * ((cols + 31) / 32) + 8 * kUnits - 1) / (8 * kUnits);
   k<<<mx_grid((const void*)k, strips), kMxThreads, 0, s>>>(x, rows, cols, stride, codes, scales);
   return cudaGetLastError();
@@ -402,7 +424,8 @@ static cudaError_t dequantize_t(const uint8_t* codes, const uint8_t* scales, int
         reinterpret_cast<const uint2*>(codes), scales, halves,
         (reinterpret_cast<uintptr_t>(out) & 31u) == 0, out);
   } else {
-    auto* k = mxfp4_dequantize_kernel<T>;
+    auto* k = narrow(rows, cols) ? mxfp4_dequantize_kernel<T, uint32_t>
+                                 : mxfp4_dequantize_kernel<T, int64_t>;
     const int64_t groups = rows * ((cols + 14) / 8);
     k<<<mx_grid((const void*)k, (groups + 32 * kUnits - 1) / (32 * kUnits)), kMxThreads, 0, s>>>(
         codes, scales, rows, cols, out);

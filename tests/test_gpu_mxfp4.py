@@ -123,6 +123,20 @@ def test_rows_far_apart_in_memory():
     del base, big
 
 
+def test_more_values_than_32_bits_number():
+    """2.15e9 values in odd rows: the last rows as on their own."""
+    rows, cols = 40000, 53701
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=DEV)
+    for r in range(0, rows, 4000):
+        x[r:r + 4000] = torch.randn(4000, cols, device=DEV, dtype=torch.bfloat16)
+    codes, scales = ops.quantize_mxfp4(x)
+    back = ops.dequantize_mxfp4(codes, scales, cols=cols)
+    for part in (slice(0, 3), slice(19998, 20003), slice(rows - 3, rows)):
+        c, s = ops.quantize_mxfp4(x[part].clone())
+        assert torch.equal(codes[part], c) and torch.equal(scales[part], s)
+        assert torch.equal(back[part], ops.dequantize_mxfp4(c, s, cols=cols))
+
+
 def test_empty():
     codes, scales = ops.quantize_mxfp4(torch.empty(0, 64, device=DEV))
     assert codes.shape == (0, 32) and scales.shape == (0, 2)
