@@ -483,9 +483,10 @@ def fused_experts_mxfp4(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.T
     top_k <= 8.  `status` as in `fused_experts`.
     """
     dev = _require_cuda(x, topk_w, topk_ids, w13, s13, w2, s2, status)
-    if x.dtype != torch.bfloat16:
+    if x.dtype is not torch.bfloat16:
         raise TypeError("fused_experts_mxfp4 needs bfloat16 activations")
-    if any(t.dtype != torch.uint8 for t in (w13, s13, w2, s2)):
+    u8 = torch.uint8
+    if not (w13.dtype is u8 and s13.dtype is u8 and w2.dtype is u8 and s2.dtype is u8):
         raise TypeError("fused_experts_mxfp4 needs uint8 codes and scales")
     if x.dim() != 2 or topk_ids.dim() != 2 or w13.dim() != 3:
         raise ValueError("x must be [T, H], topk_ids [T, top_k] and w13 [E, 2I, H / 2]")
@@ -498,26 +499,28 @@ def fused_experts_mxfp4(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.T
     if two_i % 2 or hidden % 256 or inter % 128:
         raise NotImplementedError("fused_experts_mxfp4: hidden must be a multiple of 256 and "
                                   "intermediate a multiple of 128")
-    for t, shape in ((w13, (experts, two_i, hidden // 2)),
-                     (s13, (experts, two_i // 128, hidden // 128, 512)),
-                     (w2, (experts, hidden, inter // 2)),
-                     (s2, (experts, hidden // 128, inter // 128, 512))):
-        if t.shape != shape:
-            raise ValueError(f"weights of {experts} experts, hidden {hidden} and intermediate "
-                             f"{inter}: a tensor {tuple(t.shape)} must be {shape}")
-    x, w13, s13, w2, s2 = (_aligned(t, 32) for t in (x, w13, s13, w2, s2))
-    if topk_ids.dtype != torch.int32:  # ids past int32 stay out of range
-        topk_ids = topk_ids.clamp(-1, experts)
-    ids = topk_ids.to(torch.int32).contiguous()
-    wts = topk_w.float().contiguous()
+    if (w13.shape != (experts, two_i, hidden // 2)
+            or s13.shape != (experts, two_i // 128, hidden // 128, 512)
+            or w2.shape != (experts, hidden, inter // 2)
+            or s2.shape != (experts, hidden // 128, inter // 128, 512)):
+        raise ValueError(
+            f"for {experts} experts, hidden {hidden} and intermediate {inter}, w13, s13, w2 and s2 "
+            f"are {tuple(w13.shape)}, {tuple(s13.shape)}, {tuple(w2.shape)}, {tuple(s2.shape)}")
+    x, w13, s13 = _aligned(x), _aligned(w13, 32), _aligned(s13)
+    w2, s2 = _aligned(w2, 32), _aligned(s2)
+    if topk_ids.dtype is not torch.int32:  # ids past int32 stay out of range
+        topk_ids = topk_ids.clamp(-1, experts).to(torch.int32)
+    if topk_w.dtype is not torch.float32:
+        topk_w = topk_w.float()
+    ids, wts = topk_ids.contiguous(), topk_w.contiguous()
     y = torch.empty_like(x)
     if tokens == 0:
         return y
-    ws_bytes = int(L.lib().exf_fused_experts_mxfp4_workspace_bytes(tokens, top_k, experts, hidden,
-                                                                   inter))
-    ws = torch.empty(max(ws_bytes, 32), dtype=torch.uint8, device=dev)
+    lib = L.lib()
+    ws_bytes = lib.exf_fused_experts_mxfp4_workspace_bytes(tokens, top_k, experts, hidden, inter)
+    ws = torch.empty(ws_bytes if ws_bytes > 32 else 32, dtype=u8, device=dev)
     with _on(dev):
-        L.check(L.lib().exf_fused_experts_mxfp4(
+        L.check(lib.exf_fused_experts_mxfp4(
             x.data_ptr(), wts.data_ptr(), ids.data_ptr(), tokens, top_k, w13.data_ptr(),
             s13.data_ptr(), w2.data_ptr(), s2.data_ptr(), experts, hidden, inter, y.data_ptr(),
             ws.data_ptr(), ws_bytes, _status_ptr(status), _stream(dev)))
@@ -541,6 +544,29 @@ def _gated_forward(x, w13, activation, status, keep):
     return h, pre
 
 
+def _gated_backward(ctx, dh):
+    x, w13, pre = ctx.saved_tensors
+    dtype, dev = x.dtype, x.device
+    dh = _aligned(dh if dh.dtype is dtype else dh.to(dtype))
+    tokens, hidden = x.shape
+    inter = w13.shape[0] // 2
+    want_x, want_w, _, _ = ctx.needs_input_grad
+    dx = torch.empty_like(x) if want_x else None
+    dw13 = torch.empty_like(w13) if want_w else None
+    lib = L.lib()
+    with _on(dev):
+        ws_bytes = lib.exf_gated_mlp_backward_workspace_bytes(tokens, hidden, inter)
+        ws = torch.empty(ws_bytes if ws_bytes > 32 else 32, dtype=torch.uint8, device=dev)
+        L.check(lib.exf_gated_mlp_backward(
+            dh.data_ptr(), pre.data_ptr(), x.data_ptr(), w13.data_ptr(), _WDT[dtype], tokens,
+            hidden, inter, ctx.activation, _ptr(dx), _ptr(dw13), ws.data_ptr(), ws_bytes,
+            _status_ptr(ctx.status), _stream(dev)))
+    return dx, dw13, None, None
+
+
+_gated_backward_once = torch.autograd.function.once_differentiable(_gated_backward)
+
+
 class _GatedMlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w13, activation, status):
@@ -550,22 +576,9 @@ class _GatedMlp(torch.autograd.Function):
         return h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
-        x, w13, pre = ctx.saved_tensors
-        dh = _aligned(dh.to(x.dtype))
-        tokens, hidden = x.shape
-        inter = w13.shape[0] // 2
-        dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
-        dw13 = torch.empty_like(w13) if ctx.needs_input_grad[1] else None
-        with _on(x.device):
-            ws_bytes = L.lib().exf_gated_mlp_backward_workspace_bytes(tokens, hidden, inter)
-            ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=x.device)
-            L.check(L.lib().exf_gated_mlp_backward(
-                dh.data_ptr(), pre.data_ptr(), x.data_ptr(), w13.data_ptr(), _WDT[x.dtype], tokens,
-                hidden, inter, ctx.activation, _ptr(dx), _ptr(dw13), ws.data_ptr(), ws_bytes,
-                _status_ptr(ctx.status), _stream(x.device)))
-        return dx, dw13, None, None
+        # recorded itself (create_graph): its gradients raise when they are differentiated
+        return (_gated_backward_once if torch.is_grad_enabled() else _gated_backward)(ctx, dh)
 
 
 def gated_mlp(x: torch.Tensor, w13: torch.Tensor, activation: str = "silu",
