@@ -78,20 +78,18 @@ __global__ void __launch_bounds__(256) mx_split_kernel(const __nv_bfloat16* x, c
 // GEMM-1 tile waits only for earlier GEMM-1 tiles of its own CTA and was handed out before every
 // GEMM-2 tile, so the wait ends; it is bounded all the same.
 //
-// Scales are loaded for several stages at a time: a copy a stage cost as much of the TMA unit as a
-// third of a weight tile.  8 epilogue warps sum the two terms into registers and give the
-// accumulator back before they compute; there are two accumulators.
+// 8 epilogue warps sum the two terms into registers and give the accumulator back before they
+// compute; there are two accumulators.
 //
 // What bounds the layer is the bytes in flight: padded, a stage's 17 KB of codes and scales take
-// 32 KB of shared memory, and four stages instead of five cost 4 %.
+// 32 KB of shared memory and its token rows 4 or 8.  us of a 742 MB layer with blocks of 16: 149 with
+// four stages, 141 with five, 139 with six.
 template <int BT>
 struct MxCfg {
   static constexpr int kN = 2 * BT;
   static constexpr int kTTile = kN * kMxK;
   static constexpr int kWTile = 128 * kMxK;              // padded codes of 128 rows
-  static constexpr int kStages = 5;
-  static constexpr int kScaleRun = BT == 32 ? 2 : 4;     // stages a copy of scales serves
-  static constexpr int kScaleBytes = kScaleRun * 512;
+  static constexpr int kStages = BT == 16 ? 6 : 5;
   static constexpr int kRing = 4;                        // tiles handed out ahead
   static constexpr int kAccCols = 2 * kN;
   static constexpr int kScaleCol = 2 * kAccCols;         // 4 sets of 16 columns
@@ -109,9 +107,7 @@ struct MxSmem {
   using C = MxCfg<BT>;
   // a stage: 256 rows of codes, token rows
   alignas(1024) uint8_t tiles[C::kStages][2 * C::kWTile + C::kTTile];
-  // Slots of scales (token rows, first and second weight rows), taken in turn by the runs.  As many
-  // as stages: that many runs later, every stage that used a slot's scales has been released.
-  alignas(128) uint8_t scales[C::kStages][3][C::kScaleBytes];
+  alignas(128) uint8_t scales[C::kStages][3][512];  // token rows, first and second weight rows
   alignas(8) uint64_t full[C::kStages];
   alignas(8) uint64_t empty[C::kStages];
   alignas(8) uint64_t acc_full[2];
@@ -127,16 +123,6 @@ template <int BT>
 constexpr size_t mx_smem_bytes() { return sizeof(MxSmem<BT>) + 1024; }
 static_assert(mx_smem_bytes<16>() <= 232448 && mx_smem_bytes<32>() <= 232448,
               "decode expert layer shared memory");
-
-// The scales that come with k block kb of a tile: those of R blocks with every R-th.  First block
-// and bytes (0: none).
-struct ScaleRun {
-  int kb, bytes;
-};
-template <int R>
-__device__ __forceinline__ ScaleRun scale_run(int kblocks, int kb) {
-  return {kb, kb % R ? 0 : 512 * (kblocks - kb < R ? kblocks - kb : R)};
-}
 
 // After a time-out (else every load has been consumed): copies still in flight land before shared
 // memory is released.  The other loading warps may never arrive on a stage, so that its barrier
@@ -262,7 +248,7 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
     // ---- weight loads: gate (warp 0) and up (warp 2) rows of W13[e], or the halves of 256 rows of
     // W2[e]
     const int half = warp == 0 ? 0 : 1;
-    uint32_t g = 0, run = 0;  // stages and runs of scales loaded
+    uint32_t g = 0;
     bool ok = true;
     MxTile lt;
     for (int j = 0; ok && next_tile(j, lt); ++j) {
@@ -276,21 +262,17 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
         const int s = g % kStages;
         ok = warp_wait(&sm.empty[s], ((g / kStages) & 1) ^ 1, failed);
         if (!ok) break;
-        const ScaleRun sr = scale_run<C::kScaleRun>(kblocks, kb);
         if (elect_one()) {
-          mbar_expect_tx(&sm.full[s], C::kWTile / 2 + sr.bytes);  // codes count as in memory
+          mbar_expect_tx(&sm.full[s], C::kWTile / 2 + 512);  // codes count as they lie in memory
           tma_load_2d(sm.tiles[s] + half * C::kWTile, map, &sm.full[s], kb * kMxK, row);
-          if (sr.bytes)
-            bulk_load(sm.scales[run % kStages][1 + half], sc + sr.kb * 512, sr.bytes,
-                      &sm.full[s]);
+          bulk_load(sm.scales[s][1 + half], sc + kb * 512, 512, &sm.full[s]);
         }
-        if (sr.bytes) ++run;
       }
     }
     issued = g;
   } else if (warp == 3) {
     // ---- token loads: the quarters of the block that hold routes
-    uint32_t g = 0, run = 0;
+    uint32_t g = 0;
     bool ok = true;
     MxTile lt;
     for (int j = 0; ok && next_tile(j, lt); ++j) {
@@ -312,22 +294,19 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
         const int s = g % kStages;
         ok = warp_wait(&sm.empty[s], ((g / kStages) & 1) ^ 1, failed);
         if (!ok) break;
-        const ScaleRun sr = scale_run<C::kScaleRun>(kblocks, kb);
         if (elect_one()) {
-          mbar_expect_tx(&sm.full[s], lt.quarters * 32 * kMxK + sr.bytes);
+          mbar_expect_tx(&sm.full[s], lt.quarters * 32 * kMxK + 512);
           for (int q = 0; q < lt.quarters; ++q)
             tma_load_2d(sm.tiles[s] + 2 * C::kWTile + q * 32 * kMxK, map, &sm.full[s],
                         kb * kMxK, lt.blk * 2 * BT + 32 * q);
-          if (sr.bytes)
-            bulk_load(sm.scales[run % kStages][0], sc + sr.kb * 512, sr.bytes, &sm.full[s]);
+          bulk_load(sm.scales[s][0], sc + kb * 512, 512, &sm.full[s]);
         }
-        if (sr.bytes) ++run;
       }
     }
     issued = g;
   } else if (warp == 1) {
     // ---- MMA issuer; scale sets rotate over 4 groups of 16 TMEM columns
-    uint32_t g = 0, run = 0;
+    uint32_t g = 0;
     int i = 0;
     bool ok = true;
     MxTile lt;
@@ -345,13 +324,11 @@ __global__ void __launch_bounds__(kMxLayerThreads, 1)
         fence_after_sync();
         const uint64_t w0 = smem_desc(smem_addr(sm.tiles[s]));
         const uint64_t w1 = w0 + C::kWTile / 16, t0 = w0 + 2 * C::kWTile / 16;
-        if (kb % C::kScaleRun == 0) ++run;
-        const uint32_t sc =
-            smem_addr(sm.scales[(run - 1) % kStages][0]) + (kb % C::kScaleRun) * 512;
+        const uint32_t sc = smem_addr(sm.scales[s][0]);
         const uint32_t sf = tmem + C::kScaleCol + (g & 3) * 16;
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 3; ++k) tmem_copy_scales(sf + 4 * k, sc + k * C::kScaleBytes);
+          for (int k = 0; k < 3; ++k) tmem_copy_scales(sf + 4 * k, sc + k * 512);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {  // a K step is 32 bytes further on: 2 in the descriptor
             const uint32_t on = (kb > 0 || k > 0) ? 1u : 0u;
