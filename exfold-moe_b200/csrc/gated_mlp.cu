@@ -17,7 +17,10 @@
 // TMA and masked on the store.
 //
 // G and U are kept in fp32 because the gradients already round twice (dG / dU to the operand type
-// for the tensor cores, and the result): rounding G and U too would add as much again.
+// for the tensor cores, and the result): rounding G and U too would add as much again.  Over many
+// values the two roundings make sqrt(2) of one; over few (up to 65536 tokens x inter) a few large ones
+// can weigh more, and there, where it costs nothing, dG and dU go in as the sum of two terms of the
+// operand type, the reduction running over both.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -46,6 +49,8 @@ struct GatedGemm {
   void* out;         // [m][n]
   float* pre;        // forward: [m][2 * n] or null
   int32_t* status;
+  int k_term;        // k blocks of one term of A; the second term's rows lie term_rows further on,
+  int term_rows;     // and take B's k blocks again
   int splits;        // the reduction is split over this many tiles, whose fp32 sums go to
   float* part;       // [splits][m][n] (forward: [splits][m][2 * n]) when there are several
   bool wide;         // rows of out are 32-byte aligned
@@ -283,21 +288,24 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
         uint8_t* a = sm.tiles[s];
         uint8_t* b = a + C::kATile;
         uint64_t* bar = &sm.full[s];
+        // (in a term's last k block B's rows or columns past the end are zeros, whatever A has there)
+        const int term = KIND != kForward && kb >= p.k_term ? p.term_rows : 0;
+        const int k0 = (kb - (term ? p.k_term : 0)) * kGBK;
         if (elect_one()) {
           mbar_expect_tx(bar, C::kStage);
           if (kAMn) {
-            tma_load_2d(a, &map_a, bar, mt * kGBM, kb * kGBK);
-            tma_load_2d(a + 8192, &map_a, bar, mt * kGBM + 64, kb * kGBK);
+            tma_load_2d(a, &map_a, bar, mt * kGBM, term + k0);
+            tma_load_2d(a + 8192, &map_a, bar, mt * kGBM + 64, term + k0);
           } else {
-            tma_load_2d(a, &map_a, bar, kb * kGBK, mt * kGBM);
+            tma_load_2d(a, &map_a, bar, k0, term + mt * kGBM);
           }
           if (kBMn) {
 #pragma unroll
             for (int j = 0; j < NT / 64; ++j)
-              tma_load_2d(b + j * 8192, &map_b, bar, nt * NT + 64 * j, kb * kGBK);
+              tma_load_2d(b + j * 8192, &map_b, bar, nt * NT + 64 * j, k0);
           } else {  // gate rows, then up rows
-            tma_load_2d(b, &map_b, bar, kb * kGBK, nt * (NT / 2));
-            tma_load_2d(b + C::kBTile / 2, &map_b, bar, kb * kGBK, p.n + nt * (NT / 2));
+            tma_load_2d(b, &map_b, bar, k0, nt * (NT / 2));
+            tma_load_2d(b + C::kBTile / 2, &map_b, bar, k0, p.n + nt * (NT / 2));
           }
         }
       }
@@ -689,11 +697,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
   }
 }
 
+// what rounding v to the operand type leaves; 0 where it overflows to an infinity or is one
+template <bool BF16>
+__device__ __forceinline__ float remainder_of(float v) {
+  const float2 r = unpack2<BF16>(pack2<BF16>(v, 0.0f));
+  return fabsf(r.x) < __int_as_float(0x7f800000) ? v - r.x : 0.0f;
+}
+
 // ---- the elementwise part of backward -----------------------------------------------------------
-// both [tokens][2 * inter] = (dh * U * act'(G), dh * act(G)); 8 columns a thread.
+// both [tokens][2 * inter] = (dh * U * act'(G), dh * act(G)); with a second term, the remainders in the
+// same form behind it.  8 columns a thread.
 template <bool BF16, int ACT>
 __global__ void __launch_bounds__(256)
-    gated_slope_kernel(const uint16_t* dh, const float* pre, int64_t tokens, int inter,
+    gated_slope_kernel(const uint16_t* dh, const float* pre, int64_t tokens, int inter, int terms,
                        uint16_t* both) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -720,6 +736,15 @@ __global__ void __launch_bounds__(256)
     }
     store_16b<BF16>(both, t * 2 * inter + c, dg);
     store_16b<BF16>(both, t * 2 * inter + inter + c, du);
+    if (terms == 2) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        dg[j] = remainder_of<BF16>(dg[j]);
+        du[j] = remainder_of<BF16>(du[j]);
+      }
+      store_16b<BF16>(both, (tokens + t) * 2 * inter + c, dg);
+      store_16b<BF16>(both, (tokens + t) * 2 * inter + inter + c, du);
+    }
   }
 }
 
@@ -756,35 +781,37 @@ struct GatedPlan {
   int nt, splits;
   bool pair;  // tiles of 256 x 256 on pairs of SMs
 };
-static GatedPlan plan(int kind, int64_t m, int64_t n, int64_t k) {
+static GatedPlan plan(int kind, int64_t m, int64_t n, int64_t k, int terms) {
   const int sms = sm_count() > 0 ? sm_count() : 1;
-  const int kblocks = ceil_div(k, kGBK);
+  const int kblocks = terms * ceil_div(k, kGBK);
   auto tiles = [&](int nt) {
     return (int64_t)ceil_div(m, kGBM) * ceil_div(n, kind == kForward ? nt / 2 : nt);
   };
-  if (m >= 1024 && kblocks >= 12 && tiles(256) >= sms) return {256, 1, true};
+  if (terms == 1 && m >= 1024 && kblocks >= 12 && tiles(256) >= sms) return {256, 1, true};
   if (tiles(256) * 2 > sms) return {256, 1, false};
   if (kblocks < 32) return {tiles(128) * 2 > sms ? 128 : 64, 1, false};
   int64_t s = sms / tiles(128);
   if (s > kblocks / 8) s = kblocks / 8;
   return {128, (int)(s > 1 ? s : 1), false};
 }
-static int64_t part_bytes(int kind, int64_t m, int64_t n, int64_t k) {
-  const GatedPlan pl = plan(kind, m, n, k);
+static int64_t part_bytes(int kind, int64_t m, int64_t n, int64_t k, int terms) {
+  const GatedPlan pl = plan(kind, m, n, k, terms);
   return pl.splits > 1 ? pl.splits * m * n * (kind == kForward ? 8 : 4) : 0;
 }
 
 template <int KIND, int NT, bool BF16>
 static cudaError_t run_gemm(const void* a, int64_t a_rows, int64_t a_cols, const void* b,
-                            int64_t b_rows, int64_t b_cols, GatedGemm p, cudaStream_t s) {
+                            int64_t b_rows, int64_t b_cols, int terms, GatedGemm p,
+                            cudaStream_t s) {
   constexpr auto dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap ma, mb;
-  if (!make_map(&ma, a, a_rows, a_cols, KIND == kGradW ? kGBK : kGBM, dt) ||
+  if (!make_map(&ma, a, terms * a_rows, a_cols, KIND == kGradW ? kGBK : kGBM, dt) ||
       !make_map(&mb, b, b_rows, b_cols, KIND == kForward ? NT / 2 : kGBK, dt))
     return cudaErrorInvalidValue;
   p.m_tiles = ceil_div(p.m, kGBM);
   p.n_tiles = ceil_div(p.n, KIND == kForward ? NT / 2 : NT);
-  p.kblocks = ceil_div(p.k, kGBK);
+  p.k_term = ceil_div(p.k, kGBK);
+  p.kblocks = terms * p.k_term;
   p.wide = p.n % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 32 == 0;
   cudaError_t e = launch_gemm<KIND, NT, BF16>(ma, mb, p, s);
   if (e != cudaSuccess || p.splits == 1) return e;
@@ -816,17 +843,20 @@ static cudaError_t run_pair(const void* a, int64_t a_rows, int64_t a_cols, const
                     pair_smem_bytes(), s, ma, mb, p);
 }
 
-// One product: its A and B tensors as they lie in memory, m, n, k and outputs in p.
+// One product: its A (`terms` of them, one behind the other) and B tensors as they lie in memory, m, n,
+// k and outputs in p.
 template <int KIND, bool BF16>
 static cudaError_t product(const void* a, int64_t a_rows, int64_t a_cols, const void* b,
-                           int64_t b_rows, int64_t b_cols, GatedGemm p, cudaStream_t s) {
-  const GatedPlan pl = plan(KIND, p.m, p.n, p.k);
+                           int64_t b_rows, int64_t b_cols, int terms, GatedGemm p,
+                           cudaStream_t s) {
+  const GatedPlan pl = plan(KIND, p.m, p.n, p.k, terms);
   p.splits = pl.splits;
+  p.term_rows = (int)a_rows;
   if (pl.pair) return run_pair<KIND, BF16>(a, a_rows, a_cols, b, b_rows, b_cols, p, s);
   switch (pl.nt) {
-    case 256: return run_gemm<KIND, 256, BF16>(a, a_rows, a_cols, b, b_rows, b_cols, p, s);
-    case 128: return run_gemm<KIND, 128, BF16>(a, a_rows, a_cols, b, b_rows, b_cols, p, s);
-    default: return run_gemm<KIND, 64, BF16>(a, a_rows, a_cols, b, b_rows, b_cols, p, s);
+    case 256: return run_gemm<KIND, 256, BF16>(a, a_rows, a_cols, b, b_rows, b_cols, terms, p, s);
+    case 128: return run_gemm<KIND, 128, BF16>(a, a_rows, a_cols, b, b_rows, b_cols, terms, p, s);
+    default: return run_gemm<KIND, 64, BF16>(a, a_rows, a_cols, b, b_rows, b_cols, terms, p, s);
   }
 }
 
@@ -854,17 +884,20 @@ static cudaError_t forward_t(const GatedArgs& a, void* h, float* pre, float* par
   p.pre = pre;
   p.status = a.status;
   p.part = part;
-  return product<kForward, BF16>(a.x, a.tokens, a.hidden, a.w13, 2 * (int64_t)a.inter, a.hidden, p,
-                                 s);
+  return product<kForward, BF16>(a.x, a.tokens, a.hidden, a.w13, 2 * (int64_t)a.inter, a.hidden, 1,
+                                 p, s);
 }
+
+static int gradient_terms(int64_t tokens, int inter) { return tokens * inter <= 65536 ? 2 : 1; }
 
 template <bool BF16>
 static cudaError_t backward_t(const GatedArgs& a, const void* dh, const float* pre, void* both,
                               float* part, void* dx, void* dw13, cudaStream_t s) {
+  const int terms = gradient_terms(a.tokens, a.inter);
   auto* slope = a.activation == kSilu ? gated_slope_kernel<BF16, kSilu>
                                       : gated_slope_kernel<BF16, kGeluTanh>;
   cudaError_t e = launch_pdl(slope, stream_grid(a.tokens * (a.inter / 8)), 256, 0, s,
-                             static_cast<const uint16_t*>(dh), pre, a.tokens, a.inter,
+                             static_cast<const uint16_t*>(dh), pre, a.tokens, a.inter, terms,
                              static_cast<uint16_t*>(both));
   const int64_t wide = 2 * (int64_t)a.inter;
   GatedGemm p{};
@@ -876,27 +909,28 @@ static cudaError_t backward_t(const GatedArgs& a, const void* dh, const float* p
     p.m = (int)a.tokens;
     p.k = (int)wide;
     p.out = dx;
-    e = product<kGradX, BF16>(both, a.tokens, wide, a.w13, wide, a.hidden, p, s);
+    e = product<kGradX, BF16>(both, a.tokens, wide, a.w13, wide, a.hidden, terms, p, s);
   }
   if (e == cudaSuccess && dw13) {
     p.m = (int)wide;
     p.k = (int)a.tokens;
     p.out = dw13;
-    e = product<kGradW, BF16>(both, a.tokens, wide, a.x, a.tokens, a.hidden, p, s);
+    e = product<kGradW, BF16>(both, a.tokens, wide, a.x, a.tokens, a.hidden, terms, p, s);
   }
   return e;
 }
 
 int64_t gated_forward_workspace(int64_t tokens, int hidden, int inter) {
-  return tokens <= kFewTokens ? 0 : part_bytes(kForward, tokens, inter, hidden);
+  return tokens <= kFewTokens ? 0 : part_bytes(kForward, tokens, inter, hidden, 1);
 }
 
 static int64_t both_bytes(int64_t tokens, int inter) {
-  return (tokens * 2 * inter * 2 + 255) / 256 * 256;
+  return (gradient_terms(tokens, inter) * tokens * 2 * inter * 2 + 255) / 256 * 256;
 }
 int64_t gated_backward_workspace(int64_t tokens, int hidden, int inter) {
-  const int64_t x = part_bytes(kGradX, tokens, hidden, 2 * (int64_t)inter);
-  const int64_t w = part_bytes(kGradW, 2 * (int64_t)inter, hidden, tokens);
+  const int terms = gradient_terms(tokens, inter);
+  const int64_t x = part_bytes(kGradX, tokens, hidden, 2 * (int64_t)inter, terms);
+  const int64_t w = part_bytes(kGradW, 2 * (int64_t)inter, hidden, tokens, terms);
   return both_bytes(tokens, inter) + (x > w ? x : w);
 }
 
