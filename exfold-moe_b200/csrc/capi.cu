@@ -510,7 +510,8 @@ EXF_API int exf_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t c
                                exf_stream_t stream) {
   const char* name = "exf_mxfp4_quantize";
   EXF_REQUIRE(good_wdtype(dtype), "%s: dtype must be EXF_F32, EXF_BF16 or EXF_F16", name);
-  EXF_REQUIRE(rows >= 0 && cols >= 0 && cols < ((int64_t)1 << 40) && rows < ((int64_t)1 << 40),
+  EXF_REQUIRE(rows >= 0 && cols >= 0 && cols < ((int64_t)1 << 40) &&
+                  rows <= ((int64_t)1 << 50) / (cols + 64),
               "%s: bad shape", name);
   EXF_REQUIRE(rows <= 1 || row_stride >= cols, "%s: row_stride is below cols", name);
   if (rows == 0 || cols == 0) return EXF_OK;
@@ -527,7 +528,8 @@ EXF_API int exf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, in
                                  int64_t cols, void* out, int dtype, exf_stream_t stream) {
   const char* name = "exf_mxfp4_dequantize";
   EXF_REQUIRE(good_wdtype(dtype), "%s: dtype must be EXF_F32, EXF_BF16 or EXF_F16", name);
-  EXF_REQUIRE(rows >= 0 && cols >= 0 && cols < ((int64_t)1 << 40) && rows < ((int64_t)1 << 40),
+  EXF_REQUIRE(rows >= 0 && cols >= 0 && cols < ((int64_t)1 << 40) &&
+                  rows <= ((int64_t)1 << 50) / (cols + 64),
               "%s: bad shape", name);
   if (rows == 0 || cols == 0) return EXF_OK;
   EXF_REQUIRE(codes && scales && out, "%s: null pointer", name);

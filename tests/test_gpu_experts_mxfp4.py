@@ -290,3 +290,27 @@ def test_moe_block_with_shared_expert(tokens):
     es = (eh + inter * 2.0 ** -23 * (h.abs() + eh)) @ shared2.double().abs().t()
     es = es * (1 + 2.0 ** -8) + 2.0 ** -9 * s.abs()
     near(y, want + s, (bound + es) * (1 + 2.0 ** -8) + 2.0 ** -9 * (want + s).abs())
+
+
+def test_calls_at_once_on_two_streams():
+    """A decode and a prefill call in flight together, many times."""
+    sets = []
+    for k, (tokens, experts, top_k) in enumerate([(60, 16, 4), (900, 8, 4)]):
+        tw, ids = routing(tokens, experts, top_k, seed=40 + k)
+        p13, p2 = weights(experts, 512, 384, seed=42 + k)
+        x = tokens_of(tokens, 512, seed=44 + k)
+        t13, t2 = ops.tile_mxfp4_scales(p13[1]), ops.tile_mxfp4_scales(p2[1])
+
+        def call(x=x, tw=tw, ids=ids, w13=p13[0], t13=t13, w2=p2[0], t2=t2):
+            return ops.fused_experts_mxfp4(x, tw, ids, w13, t13, w2, t2)
+
+        sets.append((call, call(), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for call, _, stream in sets:
+            with torch.cuda.stream(stream):
+                got.append(call())
+    torch.cuda.synchronize()
+    for i, y in enumerate(got):
+        assert torch.equal(y, sets[i % 2][1])

@@ -81,7 +81,8 @@ def status():
     return torch.zeros(1, dtype=torch.int32, device=DEV)
 
 
-SHAPES = [(1, 8, 8), (1, 2048, 768), (2, 64, 24), (3, 1000, 712), (5, 72, 40), (8, 512, 256),
+SHAPES = [(1, 8, 8), (1, 2048, 768), (2, 64, 24), (3, 1000, 712), (4, 264, 8), (5, 8, 8),
+          (5, 72, 40), (6, 24, 1000), (8, 512, 256), (150, 8, 16),
           (9, 128, 136), (17, 264, 200), (64, 2048, 768), (127, 320, 128), (128, 64, 128),
           (129, 4096, 264), (333, 1000, 712), (700, 136, 1032), (1500, 640, 520),
           # split reductions: of the forward pass, dx and dW
@@ -192,6 +193,8 @@ def test_views_dimensions_and_broadcast_gradients():
     want = ops.gated_mlp(x, w)
     assert torch.equal(ops.gated_mlp(wide[:, 3:], w), want)
     assert torch.equal(ops.gated_mlp(x.view(3, 20, 128), w), want.view(3, 20, 64))
+    assert torch.equal(ops.gated_mlp(x[7], w), ops.gated_mlp(x[7:8], w)[0])
+    assert ops.gated_mlp(x.view(3, 20, 128)[:0], w).shape == (0, 20, 64)
     assert torch.equal(ops.gated_mlp(x.t().contiguous().t(), w.t().contiguous().t()), want)
     # an input shared by every row: its gradient is the rows' sum, in the input's type
     one = x[:1].clone().requires_grad_(True)
@@ -255,3 +258,28 @@ def test_gradients_of_few_values_are_rounded_once(dtype):
     for got, e in ((xr.grad, want[1]), (wr.grad, want[2])):
         once = (e.to(dtype).double() - e).norm()
         assert float((got.double() - e).norm()) <= 1.1 * float(once)
+
+
+def test_calls_at_once_on_two_streams():
+    """Products of different sizes and the two kinds of gradients in flight together, many times."""
+    sets = []
+    for k, (tokens, hidden, inter) in enumerate([(1100, 776, 2184), (300, 512, 384)]):
+        x, w, dh = inputs(tokens, hidden, inter, torch.bfloat16, seed=30 + k)
+        x.requires_grad_(True)
+        w.requires_grad_(True)
+
+        def step(x=x, w=w, dh=dh):
+            h = ops.gated_mlp(x, w)
+            return (h.detach(), *torch.autograd.grad(h, (x, w), dh))
+
+        sets.append((step, step(), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(8):
+        for step, _, stream in sets:
+            with torch.cuda.stream(stream):
+                got.append(step())
+    torch.cuda.synchronize()
+    for i, outs in enumerate(got):
+        for a, b in zip(outs, sets[i % 2][1]):
+            assert torch.equal(a, b)

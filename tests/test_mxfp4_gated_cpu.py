@@ -30,6 +30,7 @@ def test_quantize_refusals():
     refused(call(q, FAKE, 3, 4, 32, 32, FAKE, FAKE, None), L.EXF_ERR_INVALID, "dtype")
     refused(call(q, FAKE, 0, -1, 32, 32, FAKE, FAKE, None), L.EXF_ERR_INVALID, "shape")
     refused(call(q, FAKE, 0, 4, 32, 31, FAKE, FAKE, None), L.EXF_ERR_INVALID, "row_stride")
+    refused(call(q, FAKE, 0, 1 << 39, 1 << 39, 1 << 39, FAKE, FAKE, None), L.EXF_ERR_INVALID, "shape")
     refused(call(q, None, 0, 4, 32, 32, FAKE, FAKE, None), L.EXF_ERR_INVALID, "null")
     refused(call(q, FAKE, 0, 4, 32, 32, ODD, FAKE, None), L.EXF_ERR_INVALID, "aligned")
     refused(call(q, ctypes.c_void_p(66), 0, 4, 32, 32, FAKE, FAKE, None), L.EXF_ERR_INVALID,
