@@ -30,11 +30,11 @@ static cudaError_t allow_smem(K* kern, size_t bytes, std::mutex& mu, bool (&done
 // Launch as a programmatic dependent of the previous kernel in the stream (the kernel calls
 // griddepcontrol.wait before reading anything that kernel wrote).
 template <typename... KArgs, typename... Args>
-static cudaError_t launch_pdl(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem,
+static cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
                               cudaStream_t s, Args... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(block);
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];

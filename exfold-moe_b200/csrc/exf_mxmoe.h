@@ -53,7 +53,7 @@ struct MxArgs {
 };
 
 struct MxWorkspace {
-  int block;                    // routes of a block
+  int block;                    // routes of a block (with few routes there is only out: h fp32)
   int64_t capacity;
   int32_t* sorted_ids;
   int32_t* expert_ids;
@@ -73,6 +73,9 @@ struct MxWorkspace {
 
 // Carves the workspace at `base` (null: sizes only).
 MxWorkspace mx_workspace(int64_t tokens, int top_k, int experts, int hidden, int inter, void* base);
+// Layers of few routes (mx_few): h [tokens * top_k][inter] is scratch.
+bool mx_few(int64_t routes, int hidden, int inter);
+cudaError_t launch_mx_few(const MxArgs& a, float* h, cudaStream_t s);
 cudaError_t launch_mx_experts(const MxArgs& a, const MxWorkspace& w, cudaStream_t s);
 
 }  // namespace exf

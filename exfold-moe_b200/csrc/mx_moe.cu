@@ -6,9 +6,10 @@
 // 8-bit activations, which enter as the sum of two e4m3 terms (exf_mx.cuh).  The products are exact,
 // the sums fp32.
 //
-// Launches: moe_align and the token rows' two-term form in route order (one launch up to 8192
-// routes) -> the layer (decode: both GEMMs in one persistent launch; prefill: a launch each) ->
-// combine (each token's routes summed in fp32, in order).
+// A few routes take kernels of their own (mx_few.cu).  Else the launches are: moe_align and the token
+// rows' two-term form in route order (one launch up to 8192 routes) -> the layer (decode: both GEMMs
+// in one persistent launch; prefill: a launch each) -> combine (each token's routes summed in fp32,
+// in order).
 #include <cuda.h>
 #include <cuda_bf16.h>
 
@@ -462,10 +463,41 @@ static_assert(mx_gemm_smem_bytes() <= 232448, "prefill expert GEMM shared memory
 // The route outputs at prefill, 16-bit: 32 columns share u = 2^(byte - 127), the largest magnitude
 // being in [2^13 u, 2^14 u); a value is a signed 16-bit multiple of u, within 2^-14 of that magnitude.
 // (bf16 route outputs would add as much error as the result's own rounding, fp32 ones twice the
-// traffic.)  Byte 255: NaN.
+// traffic.)  Values that are not finite leave the other 31 as they are: they have multiples beyond
+// +-2^14, which no finite value reaches.
+constexpr int kHalfNan = -32768, kHalfInf = 32767;  // and -32767
 __device__ __forceinline__ uint32_t half_scale(uint32_t top_bits) {
   const uint32_t e = top_bits >> 23;
-  return top_bits >= 0x7f800000u ? 255u : (e < 14 ? 1u : e - 13u);
+  return e < 14 ? 1u : e - 13u;
+}
+// 32 columns with a value that is not finite; returns their byte
+__device__ __forceinline__ uint32_t store_not_finite(int16_t* at, const uint32_t* v0,
+                                                     const uint32_t* v1, float wr) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    const uint32_t x =
+        __float_as_uint(__uint_as_float(c < 16 ? v0[c] : v1[c - 16]) * wr) & 0x7fffffffu;
+    if (x < 0x7f800000u) top = max(top, x);
+  }
+  const uint32_t sb = half_scale(top);
+  const float inv = __uint_as_float((254u - sb) << 23);
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    const float x = __uint_as_float(c < 16 ? v0[c] : v1[c - 16]) * wr;
+    const int q = x != x                  ? kHalfNan
+                  : isinf(x)              ? (x > 0.0f ? kHalfInf : -kHalfInf)
+                                          : __float2int_rn(x * inv);
+    at[c] = (int16_t)q;
+  }
+  return sb;
+}
+// the value of a multiple
+__device__ __forceinline__ float half_value(int q, float s) {
+  return q == kHalfNan    ? __uint_as_float(0x7fffffffu)
+         : q == kHalfInf  ? __uint_as_float(0x7f800000u)
+         : q == -kHalfInf ? __uint_as_float(0xff800000u)
+                          : (float)q * s;
 }
 // 16 values times w -> 16 multiples, one 32-byte sector.  Adding 1.5 2^23 rounds to an integer, whose
 // low 16 bits are its two's complement.
@@ -640,11 +672,16 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
             for (int j = 0; j < 2; ++j)
 #pragma unroll
               for (int c = 0; c < 16; ++c) top = max(top, v[2 * b + j][c] & 0x7fffffffu);
-            const uint32_t sb =
-                half_scale(__float_as_uint(__uint_as_float(top) * wr) & 0x7fffffffu);
-            const float w = wr * __uint_as_float((254u - (sb == 255u ? 127u : sb)) << 23);
-            store_halves(o + at + 32 * b, v[2 * b], w);
-            store_halves(o + at + 32 * b + 16, v[2 * b + 1], w);
+            top = __float_as_uint(__uint_as_float(top) * wr) & 0x7fffffffu;
+            uint32_t sb;
+            if (top >= 0x7f800000u) {
+              sb = store_not_finite(o + at + 32 * b, v[2 * b], v[2 * b + 1], wr);
+            } else {
+              sb = half_scale(top);
+              const float w = wr * __uint_as_float((254u - sb) << 23);
+              store_halves(o + at + 32 * b, v[2 * b], w);
+              store_halves(o + at + 32 * b + 16, v[2 * b + 1], w);
+            }
             bytes |= sb << (8 * b);
           }
           *reinterpret_cast<uint32_t*>(p.out_scale + at / 32) = bytes;
@@ -745,8 +782,20 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if (!((use >> j) & 1)) continue;
-        const float s = __uint_as_float(b[j] == 255u ? 0x7fffffffu : b[j] << 23);
+        const float s = __uint_as_float(b[j] << 23);
         const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+        // multiples outside [-2^14, 2^14) differ in their two highest bits
+        uint32_t far = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) far |= w[k] ^ (w[k] << 1);
+        if (far & 0x80008000u) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            acc[2 * k] += half_value((int16_t)(w[k] & 0xffffu), s);
+            acc[2 * k + 1] += half_value((int32_t)w[k] >> 16, s);
+          }
+          continue;
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           // a signed 16-bit q, its sign bit flipped, in the low bits of 2^23: 2^23 + 2^15 + q
@@ -823,6 +872,11 @@ MxWorkspace mx_workspace(int64_t tokens, int top_k, int experts, int hidden, int
                          void* base) {
   MxWorkspace w{};
   const int64_t numel = tokens * top_k;
+  if (mx_few(numel, hidden, inter)) {
+    w.out = static_cast<float*>(base);
+    w.bytes = up256(numel * inter * 4);
+    return w;
+  }
   w.block = mx_block(numel, experts);
   int64_t cap = numel + (int64_t)experts * (w.block - 1);
   cap = (cap + w.block - 1) / w.block * w.block;
@@ -924,6 +978,7 @@ static unsigned stream_grid(int64_t threads) {
 
 cudaError_t launch_mx_experts(const MxArgs& a, const MxWorkspace& w, cudaStream_t s) {
   const int64_t numel = a.tokens * a.top_k;
+  if (mx_few(numel, a.hidden, a.inter)) return launch_mx_few(a, w.out, s);
   AlignParams ap{a.topk_ids, numel, a.experts, w.block, w.capacity, w.sorted_ids, w.expert_ids,
                  w.num_post_pad, static_cast<int32_t*>(w.align_ws), 0};
   cudaError_t e;

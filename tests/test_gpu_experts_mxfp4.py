@@ -120,7 +120,7 @@ def test_against_formula(tokens, experts, top_k, hidden, inter):
 def test_masked_routes_and_tokens():
     """Ids of -1 and >= experts contribute nothing, whatever their weight; a token without a valid
     route gives 0, and a padded batch's last rows too."""
-    for tokens, experts in ((40, 16), (900, 8)):
+    for tokens, experts in ((20, 16), (40, 16), (900, 8)):
         tw, ids = routing(tokens, experts, 4, seed=1)
         p13, p2 = weights(experts, 512, 256, seed=2)
         x = tokens_of(tokens, 512, seed=3)
@@ -156,12 +156,13 @@ def test_prefill_values_far_apart():
     assert not bool(torch.isfinite(got[7:9]).any())
 
 
-def test_values_far_apart_and_not_finite():
+@pytest.mark.parametrize("tokens", [48, 160, 400])  # the layer for a few routes, decode, prefill
+def test_values_far_apart_and_not_finite(tokens):
     """Blocks of zeros, of the smallest and of large values; a token with an infinity or NaN gives
     NaN and leaves the others as they are."""
-    tw, ids = routing(48, 8, 2, seed=4)
+    tw, ids = routing(tokens, 8, 2, seed=4)
     p13, p2 = weights(8, 256, 128, seed=5)
-    x = tokens_of(48, 256, seed=6)
+    x = tokens_of(tokens, 256, seed=6)
     x[0] = 0.0
     x[1, 32:64] = 0.0
     x[2] = 2.0 ** -133                      # bf16's smallest subnormal
@@ -174,28 +175,29 @@ def test_values_far_apart_and_not_finite():
     bad = x.clone()
     bad[7, 9], bad[8, 200], bad[9, 3] = math.inf, math.nan, -math.inf
     got = run(bad, tw, ids, p13, p2)
-    keep = [i for i in range(48) if i not in (7, 8, 9)]
+    keep = [i for i in range(tokens) if i not in (7, 8, 9)]
     assert torch.equal(got[keep], y[keep])
     assert bool(torch.isnan(got[7:10]).all())
 
 
-def test_scales_at_their_limits():
+@pytest.mark.parametrize("tokens,experts", [(30, 2), (150, 16), (150, 2)])
+def test_scales_at_their_limits(tokens, experts):
     """Every code against scales from 2^-127 up, and the NaN scale of one weight row."""
     g = torch.Generator(device=DEV).manual_seed(8)
-    w13 = torch.randint(0, 256, (2, 256, 128), generator=g, device=DEV).to(torch.uint8)
-    w2 = torch.randint(0, 256, (2, 256, 64), generator=g, device=DEV).to(torch.uint8)
-    s13 = torch.randint(110, 124, (2, 256, 8), generator=g, device=DEV).to(torch.uint8)
-    s2 = torch.randint(110, 124, (2, 256, 4), generator=g, device=DEV).to(torch.uint8)
+    w13 = torch.randint(0, 256, (experts, 256, 128), generator=g, device=DEV).to(torch.uint8)
+    w2 = torch.randint(0, 256, (experts, 256, 64), generator=g, device=DEV).to(torch.uint8)
+    s13 = torch.randint(110, 124, (experts, 256, 8), generator=g, device=DEV).to(torch.uint8)
+    s2 = torch.randint(110, 124, (experts, 256, 4), generator=g, device=DEV).to(torch.uint8)
     s13[0, :, 3], s2[1, 7] = 0, 0
     s2[0, 9, 2] = 255
     v13 = ops.dequantize_mxfp4(w13, s13, dtype=torch.float32).double()
     v2 = ops.dequantize_mxfp4(w2, s2, dtype=torch.float32).double()
-    x = tokens_of(30, 256, seed=9)
-    ids = torch.arange(30, device=DEV).remainder(2).int().unsqueeze(1)
-    tw = torch.ones(30, 1, device=DEV)
+    x = tokens_of(tokens, 256, seed=9)
+    ids = torch.arange(tokens, device=DEV).remainder(experts).int().unsqueeze(1)
+    tw = torch.ones(tokens, 1, device=DEV)
     y = run(x, tw, ids, (w13, s13), (w2, s2))
-    assert bool(torch.isnan(y[::2, 9]).all())
-    y[::2, 9] = 0.0
+    assert bool(torch.isnan(y[::experts, 9]).all())
+    y[::experts, 9] = 0.0
     v2[0, 9] = 0.0
     near(y, *formula(x, tw, ids, v13, v2))
 
@@ -256,6 +258,73 @@ def test_streams_and_graphs():
         assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("tokens,experts", [(20, 4), (160, 8), (400, 4)])
+def test_results_not_finite_stay_in_their_columns(tokens, experts):
+    """Columns of the down projection whose scale is NaN, and ones whose route outputs overflow: NaN or
+    an infinity there, everywhere else what the call gives without them."""
+    hidden, inter = 512, 128
+    tw, ids = routing(tokens, experts, 2, seed=70)
+    p13, p2 = weights(experts, hidden, inter, seed=71)
+    x = tokens_of(tokens, hidden, seed=72)
+    want, bound = formula(x, tw, ids, p13[2], p2[2])
+    near(run(x, tw, ids, p13, p2), want, bound)
+    codes, scales = p2[0].clone(), p2[1].clone()
+    scales[0, 9] = 255
+    scales[:, 300] = 254                    # sums near 2^127 * 6 * |h|: beyond fp32
+    codes[:, 300] = 0x77                    # 6
+    y = run(x, tw, ids, p13, (codes, scales))
+    first = (ids == 0).any(-1)
+    assert bool(torch.isnan(y[first, 9]).all())
+    assert bool(torch.isinf(y[:, 300]).any()) and not bool(torch.isfinite(y[:, 300]).all())
+    others = torch.ones(hidden, dtype=torch.bool, device=DEV)
+    others[[9, 300]] = False
+    near(y[:, others], want[:, others], bound[:, others])
+    rest = ~first
+    near(y[rest, 9], want[rest, 9], bound[rest, 9])
+
+
+@pytest.mark.parametrize("top_k", range(1, 9))
+def test_few_routes(top_k):
+    """One to 16 tokens, every number of routes a token, lengths of one to eleven groups of 128."""
+    for tokens, hidden, inter in ((1, 1408, 1408), (3, 256, 896), (16, 512, 128)):
+        hidden = hidden // 256 * 256
+        tw, ids = routing(tokens, 12, top_k, seed=50 + top_k)
+        if tokens == 3:
+            ids[1, 0], ids[2, top_k - 1] = -1, 12
+        p13, p2 = weights(12, hidden, inter, seed=51 + top_k)
+        x = tokens_of(tokens, hidden, seed=52 + top_k)
+        y = run(x, tw, ids, p13, p2)
+        near(y, *formula(x, tw, ids, p13[2], p2[2]))
+
+
+def test_few_routes_by_graph_between_other_calls():
+    """Calls of one token in a row on a stream, each reading what the one before it wrote, in a graph."""
+    p13, p2 = weights(8, 256, 128, seed=60)
+    tw, ids = routing(1, 8, 4, seed=61)
+    x = tokens_of(1, 256, seed=62)
+    t13, t2 = ops.tile_mxfp4_scales(p13[1]), ops.tile_mxfp4_scales(p2[1])
+
+    def chain():
+        y = x
+        for _ in range(12):
+            y = ops.fused_experts_mxfp4(y, tw, ids, p13[0], t13, p2[0], t2)
+            y = torch.tanh(y) + x
+        return y
+
+    want = x
+    for _ in range(12):
+        want = ops.fused_experts_mxfp4(want, tw, ids, p13[0], t13, p2[0], t2)
+        torch.cuda.synchronize()
+        want = torch.tanh(want) + x
+    assert torch.equal(chain(), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain()
+    for _ in range(3):
+        graph.replay()
+    assert torch.equal(got, want)
+
+
 def test_no_tokens():
     p13, p2 = weights(8, 256, 128, seed=18)
     x = torch.empty(0, 256, dtype=torch.bfloat16, device=DEV)
@@ -292,10 +361,10 @@ def test_moe_block_with_shared_expert(tokens):
     near(y, want + s, (bound + es) * (1 + 2.0 ** -8) + 2.0 ** -9 * (want + s).abs())
 
 
-def test_calls_at_once_on_two_streams():
-    """A decode and a prefill call in flight together, many times."""
+def test_calls_at_once_on_three_streams():
+    """A decode and a prefill call in flight together with one of a few routes, many times."""
     sets = []
-    for k, (tokens, experts, top_k) in enumerate([(60, 16, 4), (900, 8, 4)]):
+    for k, (tokens, experts, top_k) in enumerate([(60, 16, 4), (900, 8, 4), (2, 8, 4)]):
         tw, ids = routing(tokens, experts, top_k, seed=40 + k)
         p13, p2 = weights(experts, 512, 384, seed=42 + k)
         x = tokens_of(tokens, 512, seed=44 + k)
@@ -313,4 +382,4 @@ def test_calls_at_once_on_two_streams():
                 got.append(call())
     torch.cuda.synchronize()
     for i, y in enumerate(got):
-        assert torch.equal(y, sets[i % 2][1])
+        assert torch.equal(y, sets[i % 3][1])
