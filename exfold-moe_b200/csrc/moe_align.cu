@@ -404,7 +404,8 @@ cudaError_t launch_align_split(const AlignParams& p, const void* x, int top_k, i
                                uint8_t* xq, uint8_t* xs, int32_t* zero, int zero_n,
                                cudaStream_t s) {
   if (hidden % 256 != 0) return cudaErrorInvalidValue;
-  // (one token x top-8: 25.1 us for the layer with slices of 16 routes, 22.5 with slices of one)
+  // (5 tokens x top-8 of 128: 49.0 us for the layer with slices of 16 routes, 42.9 with slices of one;
+  // 32 tokens: 81.1 and 75.6)
   return launch_align_put(p, x, top_k, hidden, SplitRows{{xq, xs, hidden, p.block_size}}, 1, zero,
                           zero_n, s);
 }

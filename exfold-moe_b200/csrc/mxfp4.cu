@@ -12,8 +12,8 @@
 // loads first.  Reading back, a lane writes 16 values in whole 32-byte sectors.  Rows that no
 // 16-byte vector divides are read through aligned vectors shifted into place, and written in the
 // pieces that share aligned places of the result.  403 M bf16 values (196608 x 2048): 155 us to quantise,
-// 185 to read back (6.6 and 5.5 TB/s; four fifths of the latter's bytes are writes); with 2044
-// columns 309 and 283, bound by the shifting and the row arithmetic.
+// 185 to read back (6.6 and 5.5 TB/s; four fifths of the latter's bytes are writes, and a fill alone
+// runs at 3.9); with 2044 columns 309 and 283, bound by the shifting and the row arithmetic.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

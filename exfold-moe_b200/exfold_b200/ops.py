@@ -479,7 +479,7 @@ def fused_experts_mxfp4(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.T
 
     x bf16 [T, H].  w13 uint8 [E, 2I, H / 2] (gate rows then up rows) and w2 uint8 [E, H, I / 2] are
     `quantize_mxfp4`'s codes, s13 and s2 its scales after `tile_mxfp4_scales`.  Activations keep
-    bf16 precision (two 8-bit terms each); sums are fp32.  H is a multiple of 256, I of 128,
+    bf16 precision (two 8-bit terms each, or fp16 ones for a few routes); sums are fp32.  H is a multiple of 256, I of 128,
     top_k <= 8.  `status` as in `fused_experts`.
     """
     dev = _require_cuda(x, topk_w, topk_ids, w13, s13, w2, s2, status)

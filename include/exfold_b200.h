@@ -283,11 +283,13 @@ EXF_API int exf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, in
  * are loaded).  The tensor cores multiply the codes as they are; an activation enters as the sum of
  * two e4m3 terms, exact for bf16 values above 2^-13 of the largest in their block of 32, else within
  * 2^-22 of that; the intermediate activation is rounded to within 2^-9 of its value and 2^-22 of
- * its block's largest.  The sums are fp32; where the experts hold more than
- * 44 routes on average, a route's outputs are held to within 2^-14 of the largest of their 32 columns
- * before they are summed over the token.  A token that holds an infinity or a NaN gives
- * NaN.  workspace: exf_fused_experts_mxfp4_workspace_bytes(),
- * 32-byte aligned; other arguments and limits as exf_fused_experts. */
+ * its block's largest.  (A few routes, up to 128 with routes * hidden * inter <= 5 2^23, take fp16
+ * terms instead: activations within 2^-39 of their block's largest, intermediate ones within 2^-22.)
+ * The sums are fp32; where the experts hold more than 44 routes on average, a route's outputs are held
+ * to within 2^-14 of the largest finite one of their 32 columns before they are summed over the token.
+ * A token that holds an infinity or a NaN gives NaN.
+ * workspace: exf_fused_experts_mxfp4_workspace_bytes(), 32-byte aligned; other arguments and limits as
+ * exf_fused_experts. */
 EXF_API int64_t exf_fused_experts_mxfp4_workspace_bytes(int64_t tokens, int top_k, int experts,
                                                         int hidden, int inter);
 EXF_API int exf_fused_experts_mxfp4(const void* x, const float* topk_w, const int32_t* topk_ids,
