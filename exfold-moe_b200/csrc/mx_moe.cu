@@ -470,8 +470,9 @@ __device__ __forceinline__ uint32_t half_scale(uint32_t top_bits) {
   const uint32_t e = top_bits >> 23;
   return e < 14 ? 1u : e - 13u;
 }
-// 32 columns with a value that is not finite; returns their byte
-__device__ __forceinline__ uint32_t store_not_finite(int16_t* at, const uint32_t* v0,
+// 32 columns with a value that is not finite, or of which the largest before its weight is below
+// 2^-113 (the factor of store_halves would overflow); returns their byte
+__device__ __forceinline__ uint32_t store_by_value(int16_t* at, const uint32_t* v0,
                                                      const uint32_t* v1, float wr) {
   uint32_t top = 0;
 #pragma unroll
@@ -673,12 +674,11 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
 #pragma unroll
               for (int c = 0; c < 16; ++c) top = max(top, v[2 * b + j][c] & 0x7fffffffu);
             top = __float_as_uint(__uint_as_float(top) * wr) & 0x7fffffffu;
-            uint32_t sb;
-            if (top >= 0x7f800000u) {
-              sb = store_not_finite(o + at + 32 * b, v[2 * b], v[2 * b + 1], wr);
+            uint32_t sb = half_scale(top);
+            const float w = wr * __uint_as_float((254u - sb) << 23);
+            if (top >= 0x7f800000u || isinf(w)) {
+              sb = store_by_value(o + at + 32 * b, v[2 * b], v[2 * b + 1], wr);
             } else {
-              sb = half_scale(top);
-              const float w = wr * __uint_as_float((254u - sb) << 23);
               store_halves(o + at + 32 * b, v[2 * b], w);
               store_halves(o + at + 32 * b + 16, v[2 * b + 1], w);
             }

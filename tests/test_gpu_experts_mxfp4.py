@@ -156,6 +156,19 @@ def test_prefill_values_far_apart():
     assert not bool(torch.isfinite(got[7:9]).any())
 
 
+@pytest.mark.parametrize("tokens,experts", [(20, 4), (160, 8), (400, 4)])
+@pytest.mark.parametrize("size", [3.0, 2.0 ** 20, 2.0 ** 60])
+def test_tiny_outputs_and_large_weights(tokens, experts, size):
+    """Expert outputs about 2^-115 with routing weights of 3 and more (a two-term value is held to
+    2^-137: half a step of its second term's smallest)."""
+    tw, ids = routing(tokens, experts, 2, seed=33)
+    p13, p2 = weights(experts, 256, 128, seed=34)
+    x = (tokens_of(tokens, 256, seed=35).float() * 2.0 ** -60).bfloat16()
+    want, bound = formula(x, tw * size, ids, p13[2], p2[2])
+    floor = 2.0 ** -137 * size * p2[2].abs().sum(-1).amax()
+    near(run(x, tw * size, ids, p13, p2), want, bound + floor)
+
+
 @pytest.mark.parametrize("tokens", [48, 160, 400])  # the layer for a few routes, decode, prefill
 def test_values_far_apart_and_not_finite(tokens):
     """Blocks of zeros, of the smallest and of large values; a token with an infinity or NaN gives
