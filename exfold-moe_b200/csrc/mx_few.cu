@@ -14,7 +14,8 @@
 // took 18.4 us where these take 16.4 (one token, 128 experts of 2048 x 768, cold: 20 MB, 3 us of
 // the memory's time), and 88 where these take 75 for 8 tokens.  Moving the codes' bits into fp16
 // fields instead of the conversion: 22.5.  Three blocks an SM with one group of 128 in flight a warp
-// beat two blocks with twice the loads in flight at many routes (39 and 45 us for 32).
+// beat two blocks with twice the loads in flight at many routes (39 and 45 us for 32).  Persistent
+// blocks with a ring of asynchronous copies three and four groups deep: the same (4 tokens 36.8 us).
 // Activations are fp16 times a power of two per 32, with the largest in [2^14, 2^15): bf16 is exact
 // down to 2^-31 of the largest and off by at most 2^-39 of it below; h (fp32) is the sum of two such
 // terms, the second in columns 4 to 7, with error 2^-22.
