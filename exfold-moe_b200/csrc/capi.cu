@@ -584,6 +584,14 @@ EXF_API int exf_fused_experts_mxfp4(const void* x, const float* topk_w, const in
 }
 
 // ---- gated feed-forward block --------------------------------------------------------------------
+// (a reduction of 2^24 stays far inside the kernels' bounded waits)
+static bool gated_too_large(int64_t tokens, int hidden, int inter) {
+  return tokens >= (1 << 24) || hidden >= (1 << 23) || inter >= (1 << 23) ||
+         ((tokens + 127) / 128) * (((int64_t)inter + 31) / 32) >= ((int64_t)1 << 31) ||
+         ((tokens + 127) / 128) * (((int64_t)hidden + 31) / 32) >= ((int64_t)1 << 31) ||
+         (((int64_t)inter + 63) / 64) * (((int64_t)hidden + 31) / 32) >= ((int64_t)1 << 31);
+}
+
 static int gated_checks(const char* name, int dtype, int64_t tokens, int hidden, int inter,
                         int activation) {
   if (dtype != EXF_BF16 && dtype != EXF_F16)
@@ -593,17 +601,13 @@ static int gated_checks(const char* name, int dtype, int64_t tokens, int hidden,
   EXF_REQUIRE(tokens >= 0 && hidden >= 1 && inter >= 1, "%s: bad shape", name);
   if (hidden % 8 != 0 || inter % 8 != 0)
     return fail(EXF_ERR_UNSUPPORTED, "%s: hidden and intermediate must be multiples of 8", name);
-  // (a reduction of 2^24 stays far inside the kernels' bounded waits)
-  if (tokens >= (1 << 24) || hidden >= (1 << 23) || inter >= (1 << 23) ||
-      ((tokens + 127) / 128) * (((int64_t)inter + 31) / 32) >= ((int64_t)1 << 31) ||
-      ((tokens + 127) / 128) * (((int64_t)hidden + 31) / 32) >= ((int64_t)1 << 31) ||
-      (((int64_t)inter + 63) / 64) * (((int64_t)hidden + 31) / 32) >= ((int64_t)1 << 31))
+  if (gated_too_large(tokens, hidden, inter))
     return fail(EXF_ERR_UNSUPPORTED, "%s: shape too large", name);
   return EXF_OK;
 }
 
 EXF_API int64_t exf_gated_mlp_workspace_bytes(int64_t tokens, int hidden, int inter) {
-  if (tokens < 0 || hidden < 1 || inter < 1) return -1;
+  if (tokens < 0 || hidden < 1 || inter < 1 || gated_too_large(tokens, hidden, inter)) return -1;
   return gated_forward_workspace(tokens, hidden, inter);
 }
 
@@ -629,7 +633,7 @@ EXF_API int exf_gated_mlp(const void* x, const void* w13, int dtype, int64_t tok
 }
 
 EXF_API int64_t exf_gated_mlp_backward_workspace_bytes(int64_t tokens, int hidden, int inter) {
-  if (tokens < 0 || hidden < 1 || inter < 1) return -1;
+  if (tokens < 0 || hidden < 1 || inter < 1 || gated_too_large(tokens, hidden, inter)) return -1;
   return gated_backward_workspace(tokens, hidden, inter);
 }
 

@@ -763,7 +763,7 @@ static cudaError_t launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, Gat
   return launch_pdl(kern, grid, kGatedThreads, gated_smem_bytes<NT>(), s, ma, mb, p);
 }
 
-static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 static unsigned stream_grid(int64_t threads) {
   int64_t blocks = (threads + 255) / 256;
@@ -783,9 +783,9 @@ struct GatedPlan {
 };
 static GatedPlan plan(int kind, int64_t m, int64_t n, int64_t k, int terms) {
   const int sms = sm_count() > 0 ? sm_count() : 1;
-  const int kblocks = terms * ceil_div(k, kGBK);
+  const int64_t kblocks = terms * ceil_div(k, kGBK);
   auto tiles = [&](int nt) {
-    return (int64_t)ceil_div(m, kGBM) * ceil_div(n, kind == kForward ? nt / 2 : nt);
+    return ceil_div(m, kGBM) * ceil_div(n, kind == kForward ? nt / 2 : nt);
   };
   if (terms == 1 && m >= 1024 && kblocks >= 12 && tiles(256) >= sms) return {256, 1, true};
   if (tiles(256) * 2 > sms) return {256, 1, false};
@@ -808,9 +808,9 @@ static cudaError_t run_gemm(const void* a, int64_t a_rows, int64_t a_cols, const
   if (!make_map(&ma, a, terms * a_rows, a_cols, KIND == kGradW ? kGBK : kGBM, dt) ||
       !make_map(&mb, b, b_rows, b_cols, KIND == kForward ? NT / 2 : kGBK, dt))
     return cudaErrorInvalidValue;
-  p.m_tiles = ceil_div(p.m, kGBM);
-  p.n_tiles = ceil_div(p.n, KIND == kForward ? NT / 2 : NT);
-  p.k_term = ceil_div(p.k, kGBK);
+  p.m_tiles = (int)ceil_div(p.m, kGBM);
+  p.n_tiles = (int)ceil_div(p.n, KIND == kForward ? NT / 2 : NT);
+  p.k_term = (int)ceil_div(p.k, kGBK);
   p.kblocks = terms * p.k_term;
   p.wide = p.n % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 32 == 0;
   cudaError_t e = launch_gemm<KIND, NT, BF16>(ma, mb, p, s);
@@ -833,9 +833,9 @@ static cudaError_t run_pair(const void* a, int64_t a_rows, int64_t a_cols, const
   if (!make_map(&ma, a, a_rows, a_cols, KIND == kGradW ? kGBK : 128, dt) ||
       !make_map(&mb, b, b_rows, b_cols, KIND == kForward ? 128 : kGBK, dt))
     return cudaErrorInvalidValue;
-  p.m_tiles = ceil_div(p.m, 256);
-  p.n_tiles = ceil_div(p.n, KIND == kForward ? 128 : 256);
-  p.kblocks = ceil_div(p.k, kGBK);
+  p.m_tiles = (int)ceil_div(p.m, 256);
+  p.n_tiles = (int)ceil_div(p.n, KIND == kForward ? 128 : 256);
+  p.kblocks = (int)ceil_div(p.k, kGBK);
   p.wide = p.n % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 32 == 0;
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
   const int64_t pairs = sm_count() > 1 ? sm_count() / 2 : 1;
@@ -928,6 +928,7 @@ static int64_t both_bytes(int64_t tokens, int inter) {
   return (gradient_terms(tokens, inter) * tokens * 2 * inter * 2 + 255) / 256 * 256;
 }
 int64_t gated_backward_workspace(int64_t tokens, int hidden, int inter) {
+  if (tokens == 0) return 0;  // nothing is launched, and there are no tiles to plan with
   const int terms = gradient_terms(tokens, inter);
   const int64_t x = part_bytes(kGradX, tokens, hidden, 2 * (int64_t)inter, terms);
   const int64_t w = part_bytes(kGradW, 2 * (int64_t)inter, hidden, tokens, terms);
