@@ -471,6 +471,16 @@ def tile_mxfp4_scales(scales: torch.Tensor) -> torch.Tensor:
             .reshape(e, rows // 128, blocks // 4, 512).contiguous())
 
 
+def _expert_ids(ids: torch.Tensor, experts: int) -> torch.Tensor:
+    """Integer ids of any width as int32; what lies outside [0, experts) stays outside."""
+    if ids.dtype is torch.int32:
+        return ids
+    if ids.is_floating_point() or ids.is_complex() or ids.dtype is torch.bool:
+        raise TypeError(f"expert ids must be integers, got {ids.dtype}")
+    # (clamped in 64 bits: -1 is 255 in uint8, and experts may not fit the narrow types)
+    return ids.to(torch.int64).clamp(-1, experts).to(torch.int32)
+
+
 def fused_experts_mxfp4(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor,
                         w13: torch.Tensor, s13: torch.Tensor, w2: torch.Tensor, s2: torch.Tensor,
                         status: torch.Tensor | None = None) -> torch.Tensor:
@@ -478,9 +488,9 @@ def fused_experts_mxfp4(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.T
     (W3[e] x)), e = topk_ids[:, j]; ids outside [0, E) contribute nothing.
 
     x bf16 [T, H].  w13 uint8 [E, 2I, H / 2] (gate rows then up rows) and w2 uint8 [E, H, I / 2] are
-    `quantize_mxfp4`'s codes, s13 and s2 its scales after `tile_mxfp4_scales`.  Activations keep
-    bf16 precision (two 8-bit terms each, or fp16 ones for a few routes); sums are fp32.  H is a multiple of 256, I of 128,
-    top_k <= 8.  `status` as in `fused_experts`.
+    `quantize_mxfp4`'s codes, s13 and s2 its scales after `tile_mxfp4_scales`; topk_ids integers of
+    any width.  Activations keep bf16 precision (two 8-bit terms each, or fp16 ones for a few routes);
+    sums are fp32.  H is a multiple of 256, I of 128, top_k <= 8.  `status` as in `fused_experts`.
     """
     dev = _require_cuda(x, topk_w, topk_ids, w13, s13, w2, s2, status)
     if x.dtype is not torch.bfloat16:
@@ -508,8 +518,7 @@ def fused_experts_mxfp4(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.T
             f"are {tuple(w13.shape)}, {tuple(s13.shape)}, {tuple(w2.shape)}, {tuple(s2.shape)}")
     x, w13, s13 = _aligned(x), _aligned(w13, 32), _aligned(s13)
     w2, s2 = _aligned(w2, 32), _aligned(s2)
-    if topk_ids.dtype is not torch.int32:  # ids past int32 stay out of range
-        topk_ids = topk_ids.clamp(-1, experts).to(torch.int32)
+    topk_ids = _expert_ids(topk_ids, experts)
     if topk_w.dtype is not torch.float32:
         topk_w = topk_w.float()
     ids, wts = topk_ids.contiguous(), topk_w.contiguous()
