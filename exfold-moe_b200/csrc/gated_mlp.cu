@@ -21,6 +21,14 @@
 // values the two roundings make sqrt(2) of one; over few (up to 65536 tokens x inter) a few large ones
 // can weigh more, and there, where it costs nothing, dG and dU go in as the sum of two terms of the
 // operand type, the reduction running over both.
+//
+// fp16 holds 2^-14 to 2^16 at full precision, and dG, dU of a scaled loss or of a mean over many tokens
+// lie outside.  Their fp16 form is therefore multiplied by a power of two that brings the largest finite
+// one to [2^14, 2^15), and the product's row by its inverse in fp32: a power per token for dx, per
+// feature for dW13, so that a token far above the others takes nothing from them.  An element is then
+// off by 2^-11 of itself or 2^-39 of that largest.  It costs fp16 a pass that finds the largest and a
+// second form of dG and dU (8192 tokens, 4096 x 2048, forward and gradients: 627 -> 705 us; 777 tokens,
+// 1000 x 520: 115 -> 121); bf16 has fp32's range and needs none.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -54,6 +62,7 @@ struct GatedGemm {
   int splits;        // the reduction is split over this many tiles, whose fp32 sums go to
   float* part;       // [splits][m][n] (forward: [splits][m][2 * n]) when there are several
   bool wide;         // rows of out are 32-byte aligned
+  const uint32_t* top;  // fp16 gradients: the bits of the largest finite magnitude in each row of A
 };
 
 // ---- activation -----------------------------------------------------------------------------
@@ -117,6 +126,20 @@ __device__ __forceinline__ void store_sums(float* at, const float* v) {
   asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "f"(v[0]),
                "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
                : "memory");
+}
+
+// ---- the powers of two of fp16 gradients ----------------------------------------------------------
+// From the bits of a finite magnitude: the power that brings it to [2^14, 2^15) (at most 2^126, for 0 and
+// what is below 2^-112), and the inverse.
+__device__ __forceinline__ int top_power(uint32_t top) {
+  const int k = 14 + 127 - (int)(top >> 23);
+  return k < 126 ? k : 126;
+}
+__device__ __forceinline__ float scale_up(uint32_t top) {
+  return __uint_as_float((uint32_t)(127 + top_power(top)) << 23);
+}
+__device__ __forceinline__ float scale_back(uint32_t top) {
+  return __uint_as_float((uint32_t)(127 - top_power(top)) << 23);
 }
 
 // ---- the GEMM ---------------------------------------------------------------------------------
@@ -204,6 +227,7 @@ __device__ __forceinline__ void write_tile(const GatedGemm& p, uint32_t taddr, i
             }
           }
         } else {
+          const float back = !BF16 && row < p.m ? scale_back(p.top[row]) : 1.0f;
   #pragma unroll 1
           for (int c = 0; c < NT; c += 32) {
             float v[32];
@@ -211,6 +235,10 @@ __device__ __forceinline__ void write_tile(const GatedGemm& p, uint32_t taddr, i
             tmem_load32(taddr + c, v);
             const int col = nt * NT + c;
             if (row < p.m) {
+              if (!BF16) {
+  #pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] *= back;
+              }
   #pragma unroll
               for (int j = 0; j < 32; j += 16)
                 if (col + j < p.n)
@@ -381,7 +409,7 @@ __global__ void __launch_bounds__(kGatedThreads, 1)
 template <int KIND, bool BF16>
 __global__ void __launch_bounds__(256)
     gated_join_kernel(const float* part, int splits, int64_t m, int n, int activation, void* out,
-                      float* pre) {
+                      float* pre, const uint32_t* top) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int kRuns = KIND == kForward ? 2 : 1;
@@ -423,6 +451,10 @@ __global__ void __launch_bounds__(256)
         v[0][j] *= (activation == kSilu ? gate_sigmoid<kSilu>(v[0][j])
                                         : gate_sigmoid<kGeluTanh>(v[0][j])) *
                    u[j];
+    } else if (!BF16) {
+      const float back = scale_back(top[row]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[0][j] *= back;
     }
     store_16b<BF16>(out, row * n + c, v[0]);
   }
@@ -705,12 +737,104 @@ __device__ __forceinline__ float remainder_of(float v) {
 }
 
 // ---- the elementwise part of backward -----------------------------------------------------------
-// both [tokens][2 * inter] = (dh * U * act'(G), dh * act(G)); with a second term, the remainders in the
-// same form behind it.  8 columns a thread.
+// dG = dh * U * act'(G) and dU = dh * act(G) of 8 columns of a token
+template <bool BF16, int ACT>
+__device__ __forceinline__ void projection_grads(const uint16_t* dh, const float* pre, int64_t t,
+                                                 int inter, int c, float (&dg)[8], float (&du)[8]) {
+  const float4* gp = reinterpret_cast<const float4*>(pre + t * 2 * inter + c);
+  const float4* up = reinterpret_cast<const float4*>(pre + t * 2 * inter + inter + c);
+  const float4 g0 = gp[0], g1 = gp[1], u0 = up[0], u1 = up[1];
+  const uint4 d = *reinterpret_cast<const uint4*>(dh + t * inter + c);
+  const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+  const float u[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+  const uint32_t dw[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float2 e = unpack2<BF16>(dw[j >> 1]);
+    const float dv = (j & 1) ? e.y : e.x;
+    const float s = gate_sigmoid<ACT>(g[j]);
+    dg[j] = dv * u[j] * gate_slope<ACT>(g[j], s);
+    du[j] = dv * (g[j] * s);
+  }
+}
+
+// fp16: the bits of the largest finite |dG|, |dU| of each feature in top[0, 2 * inter) and of each token in
+// top[2 * inter, +tokens), which are 0 before.  A block takes 256 columns of 8 * rows tokens, a warp a
+// token at a time; maxima do not depend on the atomics' order.
+template <int ACT>
+__global__ void __launch_bounds__(256)
+    gated_top_kernel(const uint16_t* dh, const float* pre, int64_t tokens, int inter, int rows,
+                     uint32_t* top) {
+  __shared__ uint32_t part[8][2][256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int groups = (inter + 255) / 256;
+  const int64_t t0 = (int64_t)(blockIdx.x / groups) * rows * 8;
+  const int c0 = (int)(blockIdx.x % groups) * 256;
+  const int c = c0 + 8 * lane;
+  auto finite = [](float v) {
+    const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+    return b < 0x7f800000u ? b : 0u;
+  };
+  uint32_t of[2][8] = {};
+#pragma unroll 2
+  for (int i = 0; i < rows; ++i) {
+    const int64_t t = t0 + 8 * i + warp;
+    if (t >= tokens) break;
+    uint32_t m = 0;
+    if (c < inter) {
+      float dg[8], du[8];
+      projection_grads<false, ACT>(dh, pre, t, inter, c, dg, du);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t a = finite(dg[j]), b = finite(du[j]);
+        of[0][j] = max(of[0][j], a);
+        of[1][j] = max(of[1][j], b);
+        m = max(m, max(a, b));
+      }
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) atomicMax(top + 2 * inter + t, m);
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part[warp][r][8 * lane + j] = of[r][j];
+  __syncthreads();
+  const int at = c0 + (int)threadIdx.x;
+  if (at >= inter) return;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = max(m, part[w][r][threadIdx.x]);
+    atomicMax(top + r * inter + at, m);
+  }
+}
+
+// The 16-bit form of 8 columns of dG and dU, [tokens][2 * inter]; with a second term, the remainders in the
+// same form behind it.
+template <bool BF16>
+__device__ __forceinline__ void store_grads(uint16_t* both, int64_t tokens, int64_t t, int inter,
+                                            int c, int terms, float (&dg)[8], float (&du)[8]) {
+  store_16b<BF16>(both, t * 2 * inter + c, dg);
+  store_16b<BF16>(both, t * 2 * inter + inter + c, du);
+  if (terms == 2) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      dg[j] = remainder_of<BF16>(dg[j]);
+      du[j] = remainder_of<BF16>(du[j]);
+    }
+    store_16b<BF16>(both, (tokens + t) * 2 * inter + c, dg);
+    store_16b<BF16>(both, (tokens + t) * 2 * inter + inter + c, du);
+  }
+}
+
+// by_token = (dG, dU); 8 columns a thread.  fp16: times the tokens' powers of two, and by_feature the same
+// with the features' (either may be null).
 template <bool BF16, int ACT>
 __global__ void __launch_bounds__(256)
     gated_slope_kernel(const uint16_t* dh, const float* pre, int64_t tokens, int inter, int terms,
-                       uint16_t* both) {
+                       const uint32_t* top, uint16_t* by_token, uint16_t* by_feature) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int vec = inter / 8;
@@ -718,32 +842,36 @@ __global__ void __launch_bounds__(256)
        i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t t = i / vec;
     const int c = (int)(i - t * vec) * 8;
-    const float4* gp = reinterpret_cast<const float4*>(pre + t * 2 * inter + c);
-    const float4* up = reinterpret_cast<const float4*>(pre + t * 2 * inter + inter + c);
-    const float4 g0 = gp[0], g1 = gp[1], u0 = up[0], u1 = up[1];
-    const uint4 d = *reinterpret_cast<const uint4*>(dh + t * inter + c);
-    const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
-    const float u[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
-    const uint32_t dw[4] = {d.x, d.y, d.z, d.w};
     float dg[8], du[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float2 e = unpack2<BF16>(dw[j >> 1]);
-      const float dv = (j & 1) ? e.y : e.x;
-      const float s = gate_sigmoid<ACT>(g[j]);
-      dg[j] = dv * u[j] * gate_slope<ACT>(g[j], s);
-      du[j] = dv * (g[j] * s);
+    projection_grads<BF16, ACT>(dh, pre, t, inter, c, dg, du);
+    if (BF16) {
+      store_grads<BF16>(by_token, tokens, t, inter, c, terms, dg, du);
+      continue;
     }
-    store_16b<BF16>(both, t * 2 * inter + c, dg);
-    store_16b<BF16>(both, t * 2 * inter + inter + c, du);
-    if (terms == 2) {
+    float a[8], b[8];
+    if (by_token) {
+      const float up = scale_up(top[2 * inter + t]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        dg[j] = remainder_of<BF16>(dg[j]);
-        du[j] = remainder_of<BF16>(du[j]);
+        a[j] = dg[j] * up;
+        b[j] = du[j] * up;
       }
-      store_16b<BF16>(both, (tokens + t) * 2 * inter + c, dg);
-      store_16b<BF16>(both, (tokens + t) * 2 * inter + inter + c, du);
+      store_grads<BF16>(by_token, tokens, t, inter, c, terms, a, b);
+    }
+    if (by_feature) {
+      const uint4* tg = reinterpret_cast<const uint4*>(top + c);
+      const uint4* tu = reinterpret_cast<const uint4*>(top + inter + c);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 g = tg[h], u = tu[h];
+        const uint32_t gw[4] = {g.x, g.y, g.z, g.w}, uw[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          a[4 * h + j] = dg[4 * h + j] * scale_up(gw[j]);
+          b[4 * h + j] = du[4 * h + j] * scale_up(uw[j]);
+        }
+      }
+      store_grads<BF16>(by_feature, tokens, t, inter, c, terms, a, b);
     }
   }
 }
@@ -817,7 +945,7 @@ static cudaError_t run_gemm(const void* a, int64_t a_rows, int64_t a_cols, const
   if (e != cudaSuccess || p.splits == 1) return e;
   return launch_pdl(gated_join_kernel<KIND, BF16>, stream_grid((int64_t)p.m * (p.n / 8)), 256, 0, s,
                     static_cast<const float*>(p.part), p.splits, (int64_t)p.m, p.n, p.activation,
-                    p.out, p.pre);
+                    p.out, p.pre, p.top);
 }
 
 template <int KIND, bool BF16>
@@ -890,32 +1018,81 @@ static cudaError_t forward_t(const GatedArgs& a, void* h, float* pre, float* par
 
 static int gradient_terms(int64_t tokens, int inter) { return tokens * inter <= 65536 ? 2 : 1; }
 
+template <int ACT>
+static cudaError_t launch_top(const GatedArgs& a, const void* dh, const float* pre, uint32_t* top,
+                              cudaStream_t s) {
+  const cudaError_t e =
+      cudaMemsetAsync(top, 0, (size_t)(a.tokens + 2 * (int64_t)a.inter) * 4, s);
+  if (e != cudaSuccess) return e;
+  // 8 tokens a warp, fewer where the card would not fill
+  const int64_t groups = ceil_div(a.inter, 256);
+  int64_t rows = a.tokens * groups / (32 * (int64_t)(sm_count() > 0 ? sm_count() : 1));
+  rows = rows < 1 ? 1 : rows > 8 ? 8 : rows;
+  gated_top_kernel<ACT><<<(unsigned)(ceil_div(a.tokens, 8 * rows) * groups), 256, 0, s>>>(
+      static_cast<const uint16_t*>(dh), pre, a.tokens, a.inter, (int)rows, top);
+  return cudaGetLastError();
+}
+
+static int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
+static int64_t both_bytes(int64_t tokens, int inter) {
+  return up256(gradient_terms(tokens, inter) * tokens * 2 * inter * 2);
+}
+static int64_t top_bytes(int64_t tokens, int inter) {
+  return up256((tokens + 2 * (int64_t)inter) * 4);
+}
+// fp16: up to 16 MB a form, the two forms of [dG dU] lie side by side and are written at once; above,
+// the second takes the first's place, by an elementwise pass of its own.  Forward and gradients of 777
+// tokens, 1000 x 520: 121 us at once, 126 in two passes; 8192 tokens, 4096 x 2048: 678 and 706, which
+// would cost every caller 67 MB more workspace.
+static bool two_forms(int64_t tokens, int inter) { return both_bytes(tokens, inter) <= (16 << 20); }
+
 template <bool BF16>
-static cudaError_t backward_t(const GatedArgs& a, const void* dh, const float* pre, void* both,
-                              float* part, void* dx, void* dw13, cudaStream_t s) {
+static cudaError_t backward_t(const GatedArgs& a, const void* dh, const float* pre,
+                              uint8_t* workspace, void* dx, void* dw13, cudaStream_t s) {
   const int terms = gradient_terms(a.tokens, a.inter);
-  auto* slope = a.activation == kSilu ? gated_slope_kernel<BF16, kSilu>
-                                      : gated_slope_kernel<BF16, kGeluTanh>;
-  cudaError_t e = launch_pdl(slope, stream_grid(a.tokens * (a.inter / 8)), 256, 0, s,
-                             static_cast<const uint16_t*>(dh), pre, a.tokens, a.inter, terms,
-                             static_cast<uint16_t*>(both));
+  const bool silu = a.activation == kSilu;
   const int64_t wide = 2 * (int64_t)a.inter;
+  const int64_t form = both_bytes(a.tokens, a.inter);
+  // [dG dU]: by token for dx, by feature for dW13 (bf16: the same); the maxima (fp16); the parts of a
+  // split reduction (dx's, then dW13's)
+  const bool at_once = !BF16 && two_forms(a.tokens, a.inter);
+  uint16_t* by_token = reinterpret_cast<uint16_t*>(workspace);
+  uint16_t* by_feature = reinterpret_cast<uint16_t*>(workspace + (at_once ? form : 0));
+  uint8_t* at = workspace + (two_forms(a.tokens, a.inter) ? 2 : 1) * form;
+  uint32_t* top = reinterpret_cast<uint32_t*>(at);
   GatedGemm p{};
   p.activation = a.activation;
   p.status = a.status;
-  p.part = part;
+  p.part = reinterpret_cast<float*>(at + top_bytes(a.tokens, a.inter));
   p.n = a.hidden;
+  auto slope = [&](bool tokens, bool features) {
+    auto* kern = silu ? gated_slope_kernel<BF16, kSilu> : gated_slope_kernel<BF16, kGeluTanh>;
+    return launch_pdl(kern, stream_grid(a.tokens * (a.inter / 8)), 256, 0, s,
+                      static_cast<const uint16_t*>(dh), pre, a.tokens, a.inter, terms,
+                      static_cast<const uint32_t*>(top), tokens ? by_token : nullptr,
+                      features ? by_feature : nullptr);
+  };
+  cudaError_t e = cudaSuccess;
+  if (!BF16)
+    e = silu ? launch_top<kSilu>(a, dh, pre, top, s) : launch_top<kGeluTanh>(a, dh, pre, top, s);
+  if (e == cudaSuccess && (BF16 || at_once)) e = slope(BF16 || dx, !BF16 && dw13);
   if (e == cudaSuccess && dx) {
+    if (!BF16 && !at_once) e = slope(true, false);
+    if (e != cudaSuccess) return e;
     p.m = (int)a.tokens;
     p.k = (int)wide;
     p.out = dx;
-    e = product<kGradX, BF16>(both, a.tokens, wide, a.w13, wide, a.hidden, terms, p, s);
+    p.top = top + wide;
+    e = product<kGradX, BF16>(by_token, a.tokens, wide, a.w13, wide, a.hidden, terms, p, s);
   }
   if (e == cudaSuccess && dw13) {
+    if (!BF16 && !at_once) e = slope(false, true);
+    if (e != cudaSuccess) return e;
     p.m = (int)wide;
     p.k = (int)a.tokens;
     p.out = dw13;
-    e = product<kGradW, BF16>(both, a.tokens, wide, a.x, a.tokens, a.hidden, terms, p, s);
+    p.top = top;
+    e = product<kGradW, BF16>(by_feature, a.tokens, wide, a.x, a.tokens, a.hidden, terms, p, s);
   }
   return e;
 }
@@ -924,15 +1101,13 @@ int64_t gated_forward_workspace(int64_t tokens, int hidden, int inter) {
   return tokens <= kFewTokens ? 0 : part_bytes(kForward, tokens, inter, hidden, 1);
 }
 
-static int64_t both_bytes(int64_t tokens, int inter) {
-  return (gradient_terms(tokens, inter) * tokens * 2 * inter * 2 + 255) / 256 * 256;
-}
 int64_t gated_backward_workspace(int64_t tokens, int hidden, int inter) {
   if (tokens == 0) return 0;  // nothing is launched, and there are no tiles to plan with
   const int terms = gradient_terms(tokens, inter);
   const int64_t x = part_bytes(kGradX, tokens, hidden, 2 * (int64_t)inter, terms);
   const int64_t w = part_bytes(kGradW, 2 * (int64_t)inter, hidden, tokens, terms);
-  return both_bytes(tokens, inter) + (x > w ? x : w);
+  return (two_forms(tokens, inter) ? 2 : 1) * both_bytes(tokens, inter) +
+         top_bytes(tokens, inter) + (x > w ? x : w);
 }
 
 cudaError_t launch_gated_forward(const GatedArgs& a, void* h, float* pre, void* workspace,
@@ -943,11 +1118,9 @@ cudaError_t launch_gated_forward(const GatedArgs& a, void* h, float* pre, void* 
 
 cudaError_t launch_gated_backward(const GatedArgs& a, const void* dh, const float* pre,
                                   void* workspace, void* dx, void* dw13, cudaStream_t s) {
-  // [dG dU], then the parts of a split reduction (dx's, then dW13's)
-  float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
-                                         both_bytes(a.tokens, a.inter));
-  return a.bf16 ? backward_t<true>(a, dh, pre, workspace, part, dx, dw13, s)
-                : backward_t<false>(a, dh, pre, workspace, part, dx, dw13, s);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  return a.bf16 ? backward_t<true>(a, dh, pre, ws, dx, dw13, s)
+                : backward_t<false>(a, dh, pre, ws, dx, dw13, s);
 }
 
 }  // namespace exf

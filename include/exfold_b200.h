@@ -306,8 +306,12 @@ EXF_API int exf_fused_experts_mxfp4(const void* x, const float* topk_w, const in
  * [tokens][2*inter] receives x W13^T for the backward pass, or is NULL.
  * exf_gated_mlp_backward: from dh [tokens][inter] and pre, dx [tokens][hidden] and dw13
  * [2*inter][hidden] (either may be NULL); the gradients of the two projections are rounded to
- * dtype before the products (up to 65536 tokens x inter: to the sum of two terms of dtype).  workspace: exf_gated_mlp_workspace_bytes() (may be NULL when that is 0)
- * and exf_gated_mlp_backward_workspace_bytes(), for the current device.  No tokens: dw13 is zeroed.  hidden and inter multiples of 8; every tensor 16-byte aligned, pre and the workspaces 32-byte.
+ * dtype before the products (up to 65536 tokens x inter: to the sum of two terms of dtype), for
+ * EXF_F16 times a power of two per token (dx) or feature (dw13) that keeps them in its range.
+ * No tokens: dw13 is zeroed.  workspace: exf_gated_mlp_workspace_bytes() (may be NULL when that is
+ * 0) and exf_gated_mlp_backward_workspace_bytes(), for the current device (-1: a shape that the call
+ * refuses).  hidden and inter multiples of 8; every tensor 16-byte aligned, pre and the workspaces
+ * 32-byte.
  * status as in exf_fused_experts. */
 enum exf_activation { EXF_SILU = 0, EXF_GELU_TANH = 1 };
 EXF_API int64_t exf_gated_mlp_workspace_bytes(int64_t tokens, int hidden, int inter);
