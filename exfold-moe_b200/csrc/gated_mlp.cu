@@ -659,6 +659,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
         }
       }
     }
+    // the leader's last commits on this CTA's `empty` barriers arrive before it leaves
+    for (uint32_t j = g > S ? g - S : 0; j < g; ++j)
+      mbar_wait_drain(&sm.empty[j % S], (j / S) & 1);
   } else if (warp == 1) {
     // ---- MMA issuer, in the leader
     if (rank == 0) {
@@ -715,8 +718,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
   }
   fence_before_sync();
   __syncthreads();
-  // neither CTA leaves while the other may still read its operands or signal its barriers; after a
-  // time-out, copies still in flight land first (a load started has at most its memory's latency left)
+  // Neither CTA leaves while the other may still read its operands or signal its barriers: all of the
+  // leader's commits have arrived here too (`empty` and `acc_full` are waited for above, `drain` is the
+  // last), and the threads' own arrivals are ordered by the cluster's barrier.  After a time-out, copies
+  // still in flight land first (a load started has at most its memory's latency left).
+  if (warp == 1 && rank == 1) mbar_wait_drain(&sm.drain, 0);
   if (sm.failed) {
     for (int j = 0; j < 256; ++j) __nanosleep(1000);
     if (threadIdx.x == 0 && p.status) atomicExch(p.status, 1);

@@ -22,3 +22,27 @@ def test_no_tokens(hidden, inter, dtype):
     h.backward(torch.empty_like(h))
     assert x.grad.shape == (0, hidden)
     assert w.grad.shape == w.shape and torch.count_nonzero(w.grad) == 0
+
+
+@pytest.mark.parametrize("tokens,hidden,inter", [(1100, 776, 2184), (1057, 2312, 1032)])
+def test_pairs_of_sms_between_other_kernels(tokens, hidden, inter):
+    """Products on pairs of SMs, some pairs with a tile less than others, each followed at once by kernels
+    that take the same SMs' shared and tensor memory, many times: the same values every time."""
+    g = torch.Generator(device=DEV).manual_seed(tokens)
+    x = torch.randn(tokens, hidden, generator=g, device=DEV).bfloat16().requires_grad_(True)
+    w = (torch.randn(2 * inter, hidden, generator=g, device=DEV) / hidden ** 0.5).bfloat16()
+    w.requires_grad_(True)
+    dh = torch.randn(tokens, inter, generator=g, device=DEV).bfloat16()
+    small = torch.randn(300, 512, generator=g, device=DEV).bfloat16()
+    ws = torch.randn(768, 512, generator=g, device=DEV).bfloat16()
+
+    def step():
+        h = ops.gated_mlp(x, w)
+        s = ops.gated_mlp(small, ws)
+        return (h.detach(), s, *torch.autograd.grad(h, (x, w), dh), ops.gated_mlp(small, ws))
+
+    want = step()
+    torch.cuda.synchronize()
+    got = [step() for _ in range(30)]
+    for outs in got:
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
