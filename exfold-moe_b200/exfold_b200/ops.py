@@ -12,6 +12,7 @@ import contextlib
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -491,6 +492,7 @@ def fused_experts_mxfp4(x: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.T
     `quantize_mxfp4`'s codes, s13 and s2 its scales after `tile_mxfp4_scales`; topk_ids integers of
     any width.  Activations keep bf16 precision (two 8-bit terms each, or fp16 ones for a few routes);
     sums are fp32.  H is a multiple of 256, I of 128, top_k <= 8.  `status` as in `fused_experts`.
+    For inference: like `fused_experts`, the result carries no gradient.
     """
     dev = _require_cuda(x, topk_w, topk_ids, w13, s13, w2, s2, status)
     if x.dtype is not torch.bfloat16:
@@ -590,14 +592,21 @@ class _GatedMlp(torch.autograd.Function):
         return (_gated_backward_once if torch.is_grad_enabled() else _gated_backward)(ctx, dh)
 
 
+def _has_tangent(*tensors: torch.Tensor) -> bool:
+    """Whether one of them is a dual tensor of forward-mode differentiation."""
+    return (forward_ad._current_level >= 0
+            and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors))
+
+
 def gated_mlp(x: torch.Tensor, w13: torch.Tensor, activation: str = "silu",
               status: torch.Tensor | None = None) -> torch.Tensor:
     """h = act(x Wg^T) * (x Wu^T): both projections, the activation and the product in one launch.
 
     x [..., H] and w13 [2I, H] (gate rows, then up rows, as an expert of `fused_experts`) bf16 or
     fp16; h [..., I].  activation "silu" or "gelu_tanh".  H and I are multiples of 8.
-    Differentiable in x and w13 (once): a forward pass that autograd records keeps both
-    projections in fp32 (8 bytes per token and intermediate feature) for the backward pass.
+    Differentiable in x and w13 (once, in reverse mode; forward mode is refused): a forward pass that
+    autograd records keeps both projections in fp32 (8 bytes per token and intermediate feature) for
+    the backward pass.
     `status` (int32 [1] on the device) is set to 1 if a pipeline wait timed out.
     """
     _require_cuda(x, w13, status)
@@ -609,6 +618,8 @@ def gated_mlp(x: torch.Tensor, w13: torch.Tensor, activation: str = "silu",
             or w13.numel() == 0):
         raise ValueError(f"x {tuple(x.shape)} and w13 {tuple(w13.shape)} must be [..., H] and "
                          "[2I, H]")
+    if _has_tangent(x, w13):
+        raise NotImplementedError("gated_mlp has no forward-mode derivative")
     flat = x.dim() == 2
     rows, w = _aligned(x if flat else x.reshape(-1, x.shape[-1])), _aligned(w13)
     act = _ACTIVATION[activation]

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from exfold_b200 import ops
 
@@ -46,3 +47,20 @@ def test_pairs_of_sms_between_other_kernels(tokens, hidden, inter):
     got = [step() for _ in range(30)]
     for outs in got:
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(which, grad):
+    """A dual tensor is an error, not a result without its tangent; the other calls inside a dual level
+    are what they are outside."""
+    args = [torch.randn(4, 16, device=DEV).bfloat16(), torch.randn(16, 16, device=DEV).bfloat16()]
+    want = ops.gated_mlp(*args)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        assert torch.equal(ops.gated_mlp(*args), want)
+        dual = list(args)
+        dual[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError):
+            ops.gated_mlp(*dual)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(lambda a: ops.gated_mlp(a, args[1]), (args[0],), (torch.ones_like(args[0]),))
