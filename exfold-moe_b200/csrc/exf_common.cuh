@@ -92,6 +92,14 @@ __device__ __forceinline__ float approx_sigmoid(float x) {
   x = fminf(x, 88.0f);
   return __fdividef(1.0f, 1.0f + __expf(-x));
 }
+
+// 1 / (1 + e^-c) to a few units in the last place of e^c.  The exponential is taken of -|c|, so that the
+// divisor lies in [1, 2]: __fdividef gives 0 for one above 2^126, where the result (c in -88.7 to
+// -87.3) is still a normal number.
+__device__ __forceinline__ float logistic(float c) {
+  const float e = __expf(-fabsf(c));
+  return __fdividef(c < 0.0f ? e : 1.0f, 1.0f + e);
+}
 // sqrt(softplus(x)), the "sqrtsoftplus" router score: softplus(x) = max(x, 0) + log1p(exp(-|x|))
 // with exact_exp (NaN goes to its lower clamp), log1p(y) for 0 < y <= 1 as 2 atanh(u), u =
 // y / (2 + y) <= 1/3: 2u (1 + u^2/3 + ... + u^14/15) by Horner in u^2 with fused multiply-adds

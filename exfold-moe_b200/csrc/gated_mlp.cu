@@ -70,7 +70,7 @@ template <int ACT>
 __device__ __forceinline__ float gate_sigmoid(float g) {
   float c = g;
   if (ACT == kGeluTanh) c = 1.5957691216057308f * fmaf(0.044715f * g, g * g, g);
-  return __fdividef(1.0f, 1.0f + __expf(-c));  // exp overflows to inf: the quotient is 0
+  return logistic(c);
 }
 template <int ACT>
 __device__ __forceinline__ float gate_slope(float g, float s) {

@@ -24,6 +24,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "exf_common.cuh"
 #include "exf_launch.h"
 #include "exf_mx.cuh"
 #include "exf_mxmoe.h"
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 3)
       gate += part[w][i][n];
       up += part[w][i][8 + n];
     }
-    h[(int64_t)route * inter + f + threadIdx.x] = __fdividef(gate, 1.0f + __expf(-gate)) * up;
+    h[(int64_t)route * inter + f + threadIdx.x] = gate * logistic(gate) * up;
   }
 }
 

@@ -138,10 +138,7 @@ __device__ __forceinline__ void drain_loads(uint64_t* full, uint32_t g) {
   }
 }
 
-// silu(g) * u; exp overflows to inf, where the quotient is 0
-__device__ __forceinline__ float silu_up(float g, float u) {
-  return __fdividef(g, 1.0f + __expf(-g)) * u;
-}
+__device__ __forceinline__ float silu_up(float g, float u) { return g * logistic(g) * u; }
 
 // N consecutive fp32 columns of this thread's TMEM lane, N = 8 or 16
 template <int N>
