@@ -86,9 +86,10 @@ def inputs(tokens, hidden, inter, seed, x_size=1.0, w_size=1.0, dh_size=1.0):
             make(tokens, inter, dh_size))
 
 
-# tiles of each kind, split reductions of either gradient, pairs of SMs, two-term sizes
+# two-term sizes, tiles of each kind, split reductions of either gradient, pairs of SMs, and one whose two
+# forms of [dG dU] (over 16 MB each) take the same place one behind the other
 SHAPES = [(1, 64, 24), (2, 136, 192), (9, 128, 136), (20, 4104, 72), (333, 1000, 712), (2200, 72, 40),
-          (4100, 264, 136), (700, 136, 1032), (1100, 776, 2184)]
+          (4100, 264, 136), (700, 136, 1032), (1100, 776, 2184), (2300, 264, 2056)]
 
 
 @pytest.mark.parametrize("activation", ["silu", "gelu_tanh"])
@@ -156,9 +157,10 @@ def test_not_finite():
     assert not bool(torch.isfinite(gw[[3, 100, 139, 236]]).any())
 
 
+@pytest.mark.parametrize("tokens,hidden,inter", [(333, 1000, 712), (2300, 264, 2056)])
 @pytest.mark.parametrize("needs", [(True, False), (False, True)])
-def test_one_gradient_only(needs):
-    x, w, dh = inputs(333, 1000, 712, 7, dh_size=2.0 ** -10)
+def test_one_gradient_only(needs, tokens, hidden, inter):
+    x, w, dh = inputs(tokens, hidden, inter, 7, dh_size=2.0 ** -10)
     both = gradients(x, w, dh, "gelu_tanh")
     x.requires_grad_(needs[0])
     w.requires_grad_(needs[1])
