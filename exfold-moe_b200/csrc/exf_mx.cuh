@@ -5,7 +5,9 @@
 //   hi = e4m3(v / s),  lo = e4m3(32 (v / s - hi)),  v = s hi + (s / 32) lo.
 // hi keeps 4 significant bits and the remainder, below 2^-4 of v, keeps 4 more: a bf16 activation
 // (8 bits) is represented exactly unless it is smaller than 2^-13 of its block's largest, where the
-// error stays below 2^-22 of that; an fp32 value is rounded by at most 2^-9 of itself (as to bf16).
+// error stays below 2^-22 of that; an fp32 value is rounded by at most 2^-9 of itself (half as much as by
+// bf16).  s is at least 2^-122 (lo's scale byte is 5 below hi's), so that lo's smallest step is 2^-136:
+// in blocks whose largest is below 2^-115 either may be off by 2^-137 instead.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -19,8 +19,8 @@
 // G and U are kept in fp32 because the gradients already round twice (dG / dU to the operand type
 // for the tensor cores, and the result): rounding G and U too would add as much again.  Over many
 // values the two roundings make sqrt(2) of one; over few (up to 65536 tokens x inter) a few large ones
-// can weigh more, and there, where it costs nothing, dG and dU go in as the sum of two terms of the
-// operand type, the reduction running over both.
+// can weigh more, and there dG and dU go in as the sum of two terms of the operand type, the reduction
+// running over both (gradient_terms).
 //
 // fp16 holds 2^-14 to 2^16 at full precision, and dG, dU of a scaled loss or of a mean over many tokens
 // lie outside.  Their fp16 form is therefore multiplied by a power of two that brings the largest finite
@@ -1022,6 +1022,9 @@ static cudaError_t forward_t(const GatedArgs& a, void* h, float* pre, float* par
                                  p, s);
 }
 
+// Device time of a forward and backward step in us, bf16, with one term and two: 27 and 31 (32 tokens,
+// 2048 x 2048), 22 and 23 (64, 1024 x 1024) at the border, hidden behind a call's host time of over 100;
+// 26 and 35 (777, 1000 x 520), 55 and 75 (2048, 2048 x 1024) above it.
 static int gradient_terms(int64_t tokens, int inter) { return tokens * inter <= 65536 ? 2 : 1; }
 
 template <int ACT>

@@ -9,7 +9,8 @@
 // 16-byte load: the four lanes of a row hold four neighbouring blocks.  The activations of block b
 // stand in column b alone, with zeros in the other lanes' places, so that column b of the product is
 // block b's sum, which the powers of two of weights and activations then scale in fp32.
-// What bounds them is the warps' instructions (63 % of the issue slots at 32 routes): one conversion
+// What bounds them: from cold weights latency (one token: 39 and 19 % of the issue slots; 24 routes: 47
+// and 37), from weights in L2 the warps' instructions (32 routes to 8 experts: 63 and 55 %): one conversion
 // a pair of codes, then one matrix instruction for 256 weights; the same kernels with an FMA a weight
 // took 18.4 us where these take 16.4 (one token, 128 experts of 2048 x 768, cold: 20 MB, 3 us of
 // the memory's time), and 88 where these take 75 for 8 tokens.  Moving the codes' bits into fp16

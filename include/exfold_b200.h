@@ -159,8 +159,9 @@ EXF_API int exf_decode_apply(const int64_t* importance, const void* w, int w_dty
  * call number beside half a value (so a word that shows the current call is complete: no fence
  * or flag round trip), waits until every rank's words of this call have arrived, and sums the
  * vectors in rank order, then selects, builds the table and applies it to its own routes:
- * results equal exf_decode on the unsharded batch bit for bit.  Like a collective, every rank must make the same sequence of
- * calls on its buffer (same experts, world, budget and variant), each on one stream.
+ * results equal exf_decode on the unsharded batch bit for bit.  Like a collective, every rank must
+ * make the same sequence of calls on its buffer (same experts, world, budget and variant), each on
+ * one stream.
  * A wait is bounded by wait_ns (0: 2 s); when it runs out, *status (device int32, may be NULL)
  * is set to 1, the result uses this rank's importance only, and the buffers must be rebuilt.
  * Replaces exf_decode_importance + an all-reduce + exf_decode_apply. */
@@ -283,10 +284,11 @@ EXF_API int exf_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, in
  * are loaded).  The tensor cores multiply the codes as they are; an activation enters as the sum of
  * two e4m3 terms, exact for bf16 values above 2^-13 of the largest in their block of 32, else within
  * 2^-22 of that; the intermediate activation is rounded to within 2^-9 of its value and 2^-22 of
- * its block's largest.  (A few routes, up to 128 with routes * hidden * inter <= 5 2^23, take fp16
- * terms instead: activations within 2^-39 of their block's largest, intermediate ones within 2^-22.)
- * The sums are fp32; where the experts hold more than 44 routes on average, a route's outputs are held
- * to within 2^-14 of the largest finite one of their 32 columns before they are summed over the token.
+ * its block's largest; either within 2^-137 where that is more.  (A few routes, up to 128 with
+ * routes * hidden * inter <= 5 2^23, take fp16 terms instead: activations within 2^-39 of their
+ * block's largest, intermediate ones within 2^-22.)  The sums are fp32; where the experts hold more
+ * than 44 routes on average, a route's outputs are held to within 2^-14 of the largest finite one of
+ * their 32 columns (2^-127 at least) before they are summed over the token.
  * A token that holds an infinity or a NaN gives NaN.
  * workspace: exf_fused_experts_mxfp4_workspace_bytes(), 32-byte aligned; other arguments and limits as
  * exf_fused_experts. */
