@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(256)
       for (int r = 0; r < kRuns; ++r) {
         const float4* at =
             reinterpret_cast<const float4*>(part + s * stride + (row * kRuns + r) * n + c);
-        const float4 a = __ldg(at), b = __ldg(at + 1);
+        const float4 a = __ldcg(at), b = __ldcg(at + 1);
         v[r][0] += a.x;
         v[r][1] += a.y;
         v[r][2] += a.z;
@@ -471,7 +471,7 @@ constexpr int kFewWarps = 4;
 
 template <bool BF16, int TT>
 __global__ void __launch_bounds__(32 * kFewWarps)
-    gated_few_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ w13, int tokens,
+    gated_few_kernel(const uint16_t* x, const uint16_t* __restrict__ w13, int tokens,
                      int hidden, int inter, int activation, uint16_t* h, float* pre) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -489,8 +489,8 @@ __global__ void __launch_bounds__(32 * kFewWarps)
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
       // (rows past the last token read it again; their sums are not stored)
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(
-                                x + (int64_t)(t < tokens ? t : tokens - 1) * hidden) + c);
+      const uint4 v = *(reinterpret_cast<const uint4*>(
+                            x + (int64_t)(t < tokens ? t : tokens - 1) * hidden) + c);
       const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {

@@ -152,7 +152,7 @@ __device__ __forceinline__ float quad_sum(float v) {
 }
 
 __global__ void __launch_bounds__(32 * kFewWarps, 3)
-    mx_few_gate_kernel(const __nv_bfloat16* __restrict__ x, const int32_t* ids,
+    mx_few_gate_kernel(const __nv_bfloat16* x, const int32_t* ids,
                        const uint8_t* __restrict__ w13, const uint8_t* __restrict__ s13,
                        int experts, int top_k, int hidden, int inter, float* h) {
   constexpr int T = kFewTiles;
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 3)
   const int64_t up_scales = (int64_t)(inter / 128) * groups * 512;
   float acc[T][2] = {};
   for (int k = warp; k < groups; k += kFewWarps) {
-    const uint2 xv = __ldg(xr + 32 * k);
+    const uint2 xv = xr[32 * k];
     uint4 c[T][2];
     uint32_t s[T][2];
 #pragma unroll

@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(256) mx_split_kernel(const __nv_bfloat16* x, c
     uint4 raw[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      raw[j] = c0 + 32 * j < vecs ? __ldg(row + c0 + 32 * j + lane) : make_uint4(0, 0, 0, 0);
+      raw[j] = c0 + 32 * j < vecs ? __ldcg(row + c0 + 32 * j + lane) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = c0 + 32 * j + lane;
@@ -744,12 +744,13 @@ __global__ void __launch_bounds__(kMxGemmThreads, 1)
 }
 
 // ---- combine ---------------------------------------------------------------------------------------
-// y[t] = sum_j out[t * top_k + j] in fp32, in route order; routes out of range were never placed.
+// y[t] = sum_j out[t * top_k + j] in fp32, in route order; routes out of range were never placed.  (These
+// kernels may be resident while the one before still writes what they read after their wait: no load
+// through the read-only path, here and wherever a kernel reads a predecessor's results.)
 // The 16-bit form of the route outputs (prefill).
 __global__ void __launch_bounds__(256)
-    mx_combine16_kernel(const int16_t* __restrict__ out, const uint8_t* __restrict__ out_scale,
-                        const int32_t* __restrict__ ids, int experts, int64_t tokens, int top_k,
-                        int hidden, __nv_bfloat16* y) {
+    mx_combine16_kernel(const int16_t* out, const uint8_t* out_scale, const int32_t* ids, int experts,
+                        int64_t tokens, int top_k, int hidden, __nv_bfloat16* y) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // a warp takes 1024 columns of a token, 256 at a time, the loads of all its routes together
@@ -771,8 +772,8 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if ((use >> j) & 1) {
-          v[j] = __ldg(out4 + (t * top_k + j) * vecs + c);
-          b[j] = __ldg(out_scale + (t * top_k + j) * (vecs / 4) + (c >> 2));
+          v[j] = __ldcg(out4 + (t * top_k + j) * vecs + c);
+          b[j] = __ldcg(out_scale + (t * top_k + j) * (vecs / 4) + (c >> 2));
         }
       }
       float acc[8] = {};
@@ -812,8 +813,8 @@ __global__ void __launch_bounds__(256)
 
 // fp32 route outputs (decode): a warp takes 256 columns of a token.
 __global__ void __launch_bounds__(256)
-    mx_combine_kernel(const float* __restrict__ out, const int32_t* __restrict__ ids, int experts,
-                      int64_t tokens, int top_k, int hidden, __nv_bfloat16* y) {
+    mx_combine_kernel(const float* out, const int32_t* ids, int experts, int64_t tokens,
+                      int top_k, int hidden, __nv_bfloat16* y) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31;
@@ -830,8 +831,8 @@ __global__ void __launch_bounds__(256)
     for (int j = 0; j < 8; ++j) {
       if (!((use >> j) & 1)) continue;
       const float* o = out + (t * top_k + j) * hidden + c;
-      v[j][0] = __ldg(reinterpret_cast<const float4*>(o));
-      v[j][1] = __ldg(reinterpret_cast<const float4*>(o + 128));
+      v[j][0] = __ldcg(reinterpret_cast<const float4*>(o));
+      v[j][1] = __ldcg(reinterpret_cast<const float4*>(o + 128));
     }
     float4 acc[2] = {};
 #pragma unroll

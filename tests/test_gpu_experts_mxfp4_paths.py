@@ -116,3 +116,44 @@ def test_routes_on_a_few_experts(tokens, top_k):
     tw = torch.rand(tokens, top_k, generator=g, device=DEV)
     p13, p2 = weights(experts, hidden, inter, seed=tokens + 1)
     check(tokens_of(tokens, hidden, seed=tokens + 2), tw, ids, p13, p2)
+
+
+@pytest.mark.parametrize("tokens", [2, 40, 300, 800])  # a few routes, blocks of 16, 32, 128
+def test_calls_that_read_what_the_one_before_wrote(tokens):
+    """Router, experts, gated block and experts again with nothing between the launches, eagerly and by
+    graph, against the same calls with the device idle before each: a kernel is resident before its
+    predecessor has finished, and reads its results only after."""
+    hidden, inter, experts, top_k = 512, 256, 64, 4
+    p13, p2 = weights(experts, hidden, inter, seed=tokens)
+    t13, t2 = ops.tile_mxfp4_scales(p13[1]), ops.tile_mxfp4_scales(p2[1])
+    g = torch.Generator(device=DEV).manual_seed(tokens + 1)
+    w = (torch.randn(2 * hidden, hidden, generator=g, device=DEV) / hidden ** 0.5).bfloat16()
+    logits = torch.randn(tokens, experts, generator=g, device=DEV)
+    x = tokens_of(tokens, hidden, seed=tokens + 2)
+
+    def chain(between):
+        outs = []
+        y = x
+        for k in range(3):
+            tw, ids = ops.router_topk(logits, top_k, renormalize=k > 0)
+            between()
+            y = ops.fused_experts_mxfp4(y, tw, ids, p13[0], t13, p2[0], t2)
+            between()
+            outs.append(y)
+            y = ops.gated_mlp(y, w)
+            between()
+            outs.append(y)
+        return outs
+
+    want = chain(torch.cuda.synchronize)
+    assert torch.count_nonzero(want[0]) > 0
+    for _ in range(5):
+        for a, b in zip(chain(lambda: None), want):
+            assert torch.equal(a.nan_to_num(), b.nan_to_num())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain(lambda: None)
+    for _ in range(5):
+        graph.replay()
+    for a, b in zip(got, want):
+        assert torch.equal(a.nan_to_num(), b.nan_to_num())
