@@ -95,7 +95,7 @@ def test_experts(tokens, experts):
     act, _, rel = act64(g, "silu")
     want = act * 2.0 ** 20
     # prefill holds route outputs within 2^-14 of the largest (here all are equal), at least 2^-127
-    bound = ((rel + 2.0 ** -8 + 1.01 * 2.0 ** -9 + 2.0 ** -14) * want.abs() + (3 * g.abs() + 1) * 2.0 ** 20 * 2.0 ** -149
-             + 2.0 ** -126)
+    bound = ((rel + 2.0 ** -8 + 1.01 * 2.0 ** -9 + 2.0 ** -14) * want.abs()
+             + (3 * g.abs() + 1) * 2.0 ** 20 * 2.0 ** -149 + 2.0 ** -126)
     off = (y.double() - want.unsqueeze(1)).abs()
     assert bool((off <= bound.unsqueeze(1)).all()), float((off / bound.unsqueeze(1)).max())
