@@ -1,0 +1,338 @@
+// The balance loss of a router over groups of tokens, the experts' counts, and the logits' gradient
+// (sm_100a).
+//
+//   p_te  softmax over e, or sigmoid_te / sum_e sigmoid_te, of the tokens that the mask keeps (N of them)
+//   c_e   routes to expert e,   P_e = sum_t p_te
+//   loss = E / (k N^2) sum_e c_e P_e
+//   dlogit_te = dloss E / (k N^2) p_te (c_e - sum_i p_ti c_i)  [sigmoid: times 1 - sigmoid_te]
+//
+// The counts carry no gradient.  They enter the gradient less their mean (sum_e p = 1, so nothing changes),
+// which keeps the difference's bits when the experts are nearly even.  A row whose logits are all -inf has
+// p = 0.  A token's sums are fp32, P_e fp32 within a block and 64 bits over the blocks, in a fixed order.
+//
+// Bound by memory: the logits are read once forward; backward reads them again and writes the gradient.
+// A token lies on a few lanes of a warp (about 16 columns a lane), so that a warp takes several at a time
+// and a row's two reductions are a few shuffles; a lane keeps its columns, and adds them in registers.
+#include <mutex>
+
+#include "exf_balance.h"
+#include "exf_common.cuh"
+#include "exf_launch.h"
+#include "exf_norm.cuh"
+
+namespace exf {
+
+constexpr int kBalanceThreads = 256;
+
+// e^x within 2^-21: 2^t of the rounded product t = x log2(e), corrected by what the rounding left.
+__device__ __forceinline__ float exp_near(float x) {
+  x = x < -150.0f ? -150.0f : x;  // (0 below; -inf would make a NaN of the rest; NaN stays)
+  const float t = x * 1.44269502f;
+  const float rest = fmaf(x, 1.44269502f, -t) + x * 1.92596299e-8f;
+  float e;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return fmaf(e, rest * 0.693147182f, e);
+}
+
+// A row's scores on `lanes` neighbouring lanes, in place of its logits; SLOPE: 1 - sigmoid in `slope`.
+// Columns past the last hold -inf.
+template <int C, bool SIGMOID, bool SLOPE>
+__device__ __forceinline__ void scores(float (&x)[C], float (&slope)[SLOPE ? C : 1], int lanes) {
+  float m = x[0];
+#pragma unroll
+  for (int j = 1; j < C; ++j) m = fmaxf(m, x[j]);
+  for (int d = lanes / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  // sigmoid(x) is e^x to the last bit where the row's largest is below -30: that row is a softmax too
+  const bool soft = !SIGMOID || m < -30.0f;
+  const float shift = soft && m > -__int_as_float(0x7f800000) ? m : 0.0f;
+  float sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < C; ++j) {
+    if (SIGMOID) {
+      const float e = exp_near(soft ? x[j] - shift : -fabsf(x[j]));
+      const bool high = x[j] >= 0.0f;
+      if (SLOPE) slope[j] = soft ? 1.0f : (high ? e : 1.0f) / (1.0f + e);
+      x[j] = soft ? e : (high ? 1.0f : e) / (1.0f + e);
+    } else {
+      x[j] = exp_near(x[j] - shift);
+    }
+    sum += x[j];
+  }
+  for (int d = lanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int j = 0; j < C; ++j) x[j] *= inv;
+}
+
+// A lane's columns: unit u = lane + lanes * i of V columns each.
+template <typename T, int V, int NV>
+__device__ __forceinline__ void load_logits(const T* row, int l, int lanes, int units, bool there,
+                                            float (&x)[NV * V]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int u = l + lanes * i;
+    float e[V];
+    if (there && u < units) {
+      load_pack<T, V>(row + u * V, e);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) e[j] = -__int_as_float(0x7f800000);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[i * V + j] = e[j];
+  }
+}
+
+// Block b of a group takes tokens [T b / blocks, T (b + 1) / blocks): its sums of p, counts and number of
+// tokens.
+template <typename T, int V, int NV, bool SIGMOID>
+__global__ void __launch_bounds__(kBalanceThreads)
+    balance_sums_kernel(const BalanceArgs a, const void* ids, bool ids64, int lanes, float* psum,
+                        int32_t* pcount, int32_t* pvalid) {
+  extern __shared__ float shared[];  // [warps][experts] sums, [experts] counts
+  constexpr int kWarps = kBalanceThreads / 32;
+  const int e = a.experts, units = e / V;
+  int32_t* count = reinterpret_cast<int32_t*>(shared + kWarps * e);
+  __shared__ int valid;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  for (int i = threadIdx.x; i < e; i += kBalanceThreads) count[i] = 0;
+  if (threadIdx.x == 0) valid = 0;
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int group = blockIdx.y;
+  const int64_t t0 = a.tokens * blockIdx.x / gridDim.x, t1 = a.tokens * (blockIdx.x + 1) / gridDim.x;
+  const uint8_t* mask = a.mask ? a.mask + (int64_t)group * a.tokens : nullptr;
+
+  const int per_warp = 32 / lanes, lane = threadIdx.x & 31, l = lane % lanes;
+  const T* logits = static_cast<const T*>(a.logits) + (int64_t)group * a.tokens * e;
+  float acc[NV * V] = {};
+  int mine = 0;
+  for (int64_t base = t0 + (threadIdx.x >> 5) * per_warp; base < t1; base += kWarps * per_warp) {
+    const int64_t t = base + lane / lanes;
+    const bool there = t < t1 && !(mask && !mask[t]);
+    float x[NV * V], none[1];
+    load_logits<T, V, NV>(logits + (there ? t : t0) * e, l, lanes, units, there, x);
+    scores<NV * V, SIGMOID, false>(x, none, lanes);
+#pragma unroll
+    for (int j = 0; j < NV * V; ++j) acc[j] += x[j];
+    mine += there && l == 0;
+  }
+  // the lanes of a warp that share columns, then the warps
+#pragma unroll
+  for (int j = 0; j < NV * V; ++j)
+    for (int d = lanes; d < 32; d <<= 1) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], d);
+  if (lane < lanes) {
+#pragma unroll
+    for (int j = 0; j < NV * V; ++j) {
+      const int u = l + lanes * (j / V);
+      if (u < units) shared[(threadIdx.x >> 5) * e + u * V + j % V] = acc[j];
+    }
+  }
+  if (mine) atomicAdd(&valid, mine);
+  const int64_t at = (int64_t)group * a.tokens * a.top_k;
+  for (int64_t i = t0 * a.top_k + threadIdx.x; i < t1 * a.top_k; i += kBalanceThreads) {
+    if (mask && !mask[i / a.top_k]) continue;
+    const int64_t id = ids64 ? static_cast<const int64_t*>(ids)[at + i]
+                             : static_cast<const int32_t*>(ids)[at + i];
+    if (id >= 0 && id < e) atomicAdd(count + id, 1);
+  }
+  __syncthreads();
+  const int64_t slot = (int64_t)group * gridDim.x + blockIdx.x;
+  for (int c = threadIdx.x; c < e; c += kBalanceThreads) {
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) s += shared[w * e + c];
+    psum[slot * e + c] = s;
+    pcount[slot * e + c] = count[c];
+  }
+  if (threadIdx.x == 0) pvalid[slot] = valid;
+}
+
+// A block a group joins its blocks' sums: 64 columns at a time, 16 threads a column.
+__global__ void __launch_bounds__(1024)
+    balance_join_kernel(const float* psum, const int32_t* pcount, const int32_t* pvalid, int blocks,
+                        int experts, int top_k, float* loss, int32_t* counts, int32_t* valid) {
+  __shared__ double sums[16][64];
+  __shared__ int32_t routes[16][64];
+  __shared__ int tokens;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) tokens = 0;
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t base = (int64_t)blockIdx.x * blocks;
+  int n = 0;
+  for (int b = threadIdx.x; b < blocks; b += 1024) n += pvalid[base + b];
+  if (n) atomicAdd(&tokens, n);
+  const int x = threadIdx.x & 63, j = threadIdx.x >> 6;
+  double total = 0.0;
+  for (int c0 = 0; c0 < experts; c0 += 64) {
+    const int c = c0 + x;
+    double s = 0.0;
+    int32_t r = 0;
+    if (c < experts) {
+#pragma unroll 8
+      for (int b = j; b < blocks; b += 16) {
+        s += (double)__ldcg(psum + (base + b) * experts + c);
+        r += __ldcg(pcount + (base + b) * experts + c);
+      }
+    }
+    __syncthreads();
+    sums[j][x] = s;
+    routes[j][x] = r;
+    __syncthreads();
+    if (j == 0 && c < experts) {
+#pragma unroll
+      for (int i = 1; i < 16; ++i) {
+        s += sums[i][x];
+        r += routes[i][x];
+      }
+      counts[(int64_t)blockIdx.x * experts + c] = r;
+      total += s * (double)r;
+    }
+  }
+  __syncthreads();
+  if (j == 0) sums[0][x] = total;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int i = 0; i < 64; ++i) s += sums[0][i];
+    const double t = (double)tokens;
+    loss[blockIdx.x] = tokens ? (float)(s * experts / ((double)top_k * t * t)) : 0.0f;
+    valid[blockIdx.x] = tokens;
+  }
+}
+
+template <typename T, int V, int NV, bool SIGMOID>
+__global__ void __launch_bounds__(kBalanceThreads)
+    balance_backward_kernel(const BalanceArgs a, int lanes, const float* dloss, const int32_t* counts,
+                            const int32_t* valid, T* dlogits) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr int kWarps = kBalanceThreads / 32;
+  const int e = a.experts, units = e / V, group = blockIdx.y;
+  const uint8_t* mask = a.mask ? a.mask + (int64_t)group * a.tokens : nullptr;
+  const int per_warp = 32 / lanes, lane = threadIdx.x & 31, l = lane % lanes;
+  const T* logits = static_cast<const T*>(a.logits) + (int64_t)group * a.tokens * e;
+  T* out = dlogits + (int64_t)group * a.tokens * e;
+  const double n = (double)valid[group];
+  const float size = n > 0.0 ? (float)((double)dloss[group] * e / (a.top_k * n * n)) : 0.0f;
+  const int middle = (int)(n * a.top_k / e);
+  float c[NV * V];
+#pragma unroll
+  for (int j = 0; j < NV * V; ++j) {
+    const int u = l + lanes * (j / V);
+    c[j] = u < units ? (float)(counts[(int64_t)group * e + u * V + j % V] - middle) : 0.0f;
+  }
+  const int64_t first = ((int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * per_warp;
+  for (int64_t base = first; base < a.tokens; base += (int64_t)gridDim.x * kWarps * per_warp) {
+    const int64_t t = base + lane / lanes;
+    const bool in = t < a.tokens;
+    const bool there = in && !(mask && !mask[t]);
+    float x[NV * V], slope[SIGMOID ? NV * V : 1];
+    load_logits<T, V, NV>(logits + (there ? t : 0) * e, l, lanes, units, there, x);
+    scores<NV * V, SIGMOID, SIGMOID>(x, slope, lanes);
+    float dot = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV * V; ++j) dot = fmaf(x[j], c[j], dot);
+    for (int d = lanes / 2; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+    if (!in) continue;  // (the loop's condition is the warp's: no lane waits for another after it)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int u = l + lanes * i;
+      if (u < units) {
+        float d[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          d[j] = size * (x[i * V + j] * (c[i * V + j] - dot));
+          if (SIGMOID) d[j] *= slope[SIGMOID ? i * V + j : 0];
+          if (!there) d[j] = 0.0f;
+        }
+        store_pack<T, V>(out + t * e + u * V, d);
+      }
+    }
+  }
+}
+
+// ---- host side ----------------------------------------------------------------------------------
+// Blocks a group of the forward pass: all groups together two on an SM, at least 8 tokens a warp.
+static int64_t balance_blocks(int groups, int64_t tokens) {
+  const int64_t sms = sm_count() > 0 ? sm_count() : 1;
+  const int64_t most = (2 * sms + groups - 1) / groups;
+  const int64_t need = (tokens + 63) / 64;
+  return need < most ? need : most;
+}
+
+int64_t balance_workspace(int groups, int64_t tokens, int experts) {
+  return groups * balance_blocks(groups, tokens) * (8 * (int64_t)experts + 4);
+}
+
+// f(logits' type, V, NV, sigmoid) of the call's layout: vectors where rows allow them, 16 columns a lane,
+// 32 for more than 512 experts
+template <typename T, int V, typename F>
+static cudaError_t balance_v(const BalanceArgs& a, F f) {
+  const int units = a.experts / V;
+  int lanes = 1;
+  while (lanes < 32 && lanes * (16 / V) < units) lanes *= 2;
+  using std::integral_constant;
+  auto pick = [&](auto nv) {
+    constexpr int NV = decltype(nv)::value;
+    return a.sigmoid ? f(T(), integral_constant<int, V>(), nv, std::true_type(), lanes)
+                     : f(T(), integral_constant<int, V>(), nv, std::false_type(), lanes);
+    (void)NV;
+  };
+  return lanes * (16 / V) >= units ? pick(integral_constant<int, 16 / V>())
+                                   : pick(integral_constant<int, 32 / V>());
+}
+template <typename T, typename F>
+static cudaError_t balance_t(const BalanceArgs& a, const void* out, F f) {
+  constexpr int V = 16 / sizeof(T);
+  return a.experts % V == 0 && norm_aligned(a.logits) && norm_aligned(out)
+             ? balance_v<T, V>(a, f)
+             : balance_v<T, 1>(a, f);
+}
+template <typename F>
+static cudaError_t balance_dispatch(const BalanceArgs& a, const void* out, F f) {
+  if (a.dtype == EXF_F32) return balance_t<float>(a, out, f);
+  if (a.dtype == EXF_BF16) return balance_t<__nv_bfloat16>(a, out, f);
+  return balance_t<__half>(a, out, f);
+}
+
+cudaError_t launch_balance_loss(const BalanceArgs& a, const void* ids, bool ids64, void* workspace,
+                                float* loss, int32_t* counts, int32_t* valid, cudaStream_t s) {
+  const int64_t blocks = balance_blocks(a.groups, a.tokens);
+  float* psum = static_cast<float*>(workspace);
+  int32_t* pcount = reinterpret_cast<int32_t*>(psum + a.groups * blocks * a.experts);
+  int32_t* pvalid = pcount + a.groups * blocks * a.experts;
+  cudaError_t err = cudaSuccess;
+  if (blocks > 0)
+    err = balance_dispatch(a, nullptr, [&](auto t, auto v, auto nv, auto sigmoid, int lanes) {
+      return launch_pdl(
+          balance_sums_kernel<decltype(t), decltype(v)::value, decltype(nv)::value,
+                              decltype(sigmoid)::value>,
+          dim3((unsigned)blocks, a.groups), dim3(kBalanceThreads),
+          (kBalanceThreads / 32 + 1) * (size_t)a.experts * 4, s, a, ids, ids64, lanes, psum, pcount,
+          pvalid);
+    });
+  if (err != cudaSuccess) return err;
+  return launch_pdl(balance_join_kernel, dim3(a.groups), dim3(1024), 0, s,
+                    static_cast<const float*>(psum), static_cast<const int32_t*>(pcount),
+                    static_cast<const int32_t*>(pvalid), (int)blocks, a.experts, a.top_k, loss,
+                    counts, valid);
+}
+
+cudaError_t launch_balance_loss_backward(const BalanceArgs& a, const float* dloss,
+                                         const int32_t* counts, const int32_t* valid, void* dlogits,
+                                         cudaStream_t s) {
+  return balance_dispatch(a, dlogits, [&](auto t, auto v, auto nv, auto sigmoid, int lanes) {
+    const int64_t sms = sm_count() > 0 ? sm_count() : 1;
+    const int64_t most = (8 * sms + a.groups - 1) / a.groups;
+    const int64_t per_block = kBalanceThreads / lanes;
+    const int64_t need = (a.tokens + per_block - 1) / per_block;
+    return launch_pdl(balance_backward_kernel<decltype(t), decltype(v)::value, decltype(nv)::value,
+                                              decltype(sigmoid)::value>,
+                      dim3((unsigned)(need < most ? need : most), a.groups), dim3(kBalanceThreads),
+                      0, s, a, lanes, dloss, counts, valid, static_cast<decltype(t)*>(dlogits));
+  });
+}
+
+}  // namespace exf

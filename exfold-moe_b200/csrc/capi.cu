@@ -7,6 +7,7 @@
 #include <mutex>
 #include <unordered_map>
 
+#include "exf_balance.h"
 #include "exf_common.cuh"
 #include "exf_gated.h"
 #include "exf_kernels.h"
@@ -14,6 +15,7 @@
 #include "exf_moe.h"
 #include "exf_mxfp4.h"
 #include "exf_mxmoe.h"
+#include "exf_norm.h"
 
 namespace exf {
 
@@ -663,6 +665,184 @@ EXF_API int exf_gated_mlp_backward(const void* dh, const float* pre, const void*
   GatedArgs a{x, w13, dtype == EXF_BF16, tokens, hidden, inter, activation, status};
   return cuda_status(
       launch_gated_backward(a, dh, pre, workspace, dx, dw13, (cudaStream_t)stream), name);
+}
+
+// ---- root-mean-square norm ------------------------------------------------------------------------
+static int norm_checks(const char* name, int dtype, int weight_dtype, int64_t rows, int64_t cols,
+                       int64_t x_stride, float eps) {
+  EXF_REQUIRE(good_wdtype(dtype), "%s: dtype must be EXF_F32, EXF_BF16 or EXF_F16", name);
+  EXF_REQUIRE(weight_dtype == EXF_F32 || weight_dtype == dtype,
+              "%s: the weight's dtype must be EXF_F32 or dtype", name);
+  EXF_REQUIRE(rows >= 0 && cols >= 1, "%s: bad shape", name);
+  if (rows >= ((int64_t)1 << 31) || cols >= (1 << 24))
+    return fail(EXF_ERR_UNSUPPORTED, "%s: at most 2^31 - 1 rows and 2^24 - 1 columns", name);
+  EXF_REQUIRE(rows <= 1 || x_stride >= cols, "%s: row stride below the row's length", name);
+  EXF_REQUIRE(eps >= 0.0f, "%s: eps must not be negative", name);
+  return EXF_OK;
+}
+static bool aligned_to(const void* p, int dtype) {
+  return reinterpret_cast<uintptr_t>(p) % (dtype == EXF_F32 ? 4 : 2) == 0;
+}
+
+EXF_API int exf_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t r_stride,
+                         const void* weight, int dtype, int weight_dtype, int64_t rows, int64_t cols,
+                         float eps, void* sum, void* y, exf_stream_t stream) {
+  const char* name = "exf_rms_norm";
+  const int rc = norm_checks(name, dtype, weight_dtype, rows, cols, x_stride, eps);
+  if (rc != EXF_OK) return rc;
+  EXF_REQUIRE(!residual || rows <= 1 || r_stride >= cols, "%s: row stride below the row's length",
+              name);
+  if (rows == 0) return EXF_OK;
+  EXF_REQUIRE(x && weight && y && (!residual || sum), "%s: null pointer", name);
+  EXF_REQUIRE(aligned_to(x, dtype) && aligned_to(residual, dtype) && aligned_to(sum, dtype) &&
+                  aligned_to(y, dtype) && aligned_to(weight, weight_dtype),
+              "%s: a tensor is not aligned to its type", name);
+  NormArgs a{x,    x_stride, residual, r_stride, weight, dtype, weight_dtype == EXF_F32,
+             rows, (int)cols, eps,     sum};
+  return cuda_status(launch_rms_norm(a, y, (cudaStream_t)stream), name);
+}
+
+static int code_checks(const char* name, int code, int64_t cols, int group) {
+  EXF_REQUIRE(code == EXF_E4M3 || code == EXF_I8, "%s: code must be EXF_E4M3 or EXF_I8", name);
+  EXF_REQUIRE(group == 0 || group == 32 || group == 64 || group == 128,
+              "%s: group must be 0 (a row), 32, 64 or 128", name);
+  if (cols > (1 << 18))
+    return fail(EXF_ERR_UNSUPPORTED, "%s: at most 2^18 columns", name);
+  return EXF_OK;
+}
+
+EXF_API int exf_rms_norm_8bit(const void* x, int64_t x_stride, const void* residual,
+                              int64_t r_stride, const void* weight, int dtype, int weight_dtype,
+                              int64_t rows, int64_t cols, float eps, int code, int group, void* sum,
+                              void* codes, float* scales, exf_stream_t stream) {
+  const char* name = "exf_rms_norm_8bit";
+  int rc = norm_checks(name, dtype, weight_dtype, rows, cols, x_stride, eps);
+  if (rc == EXF_OK) rc = code_checks(name, code, cols, group);
+  if (rc != EXF_OK) return rc;
+  EXF_REQUIRE(!residual || rows <= 1 || r_stride >= cols, "%s: row stride below the row's length",
+              name);
+  if (rows == 0) return EXF_OK;
+  EXF_REQUIRE(x && weight && codes && scales && (!residual || sum), "%s: null pointer", name);
+  EXF_REQUIRE(aligned_to(x, dtype) && aligned_to(residual, dtype) && aligned_to(sum, dtype) &&
+                  aligned_to(scales, EXF_F32) && aligned_to(weight, weight_dtype),
+              "%s: a tensor is not aligned to its type", name);
+  NormArgs a{x,    x_stride, residual, r_stride, weight, dtype, weight_dtype == EXF_F32,
+             rows, (int)cols, eps,     sum};
+  return cuda_status(launch_rms_norm_8bit(a, code == EXF_I8, group, static_cast<uint8_t*>(codes),
+                                          scales, (cudaStream_t)stream),
+                     name);
+}
+
+EXF_API int exf_dequantize_8bit(const void* codes, int code, const float* scales, int64_t rows,
+                                int64_t cols, int group, void* out, int dtype,
+                                exf_stream_t stream) {
+  const char* name = "exf_dequantize_8bit";
+  EXF_REQUIRE(good_wdtype(dtype), "%s: dtype must be EXF_F32, EXF_BF16 or EXF_F16", name);
+  EXF_REQUIRE(rows >= 0 && cols >= 1 && rows < ((int64_t)1 << 31), "%s: bad shape", name);
+  const int rc = code_checks(name, code, cols, group);
+  if (rc != EXF_OK) return rc;
+  if (rows == 0) return EXF_OK;
+  EXF_REQUIRE(codes && scales && out, "%s: null pointer", name);
+  EXF_REQUIRE(reinterpret_cast<uintptr_t>(codes) % 8 == 0 && aligned16(out) &&
+                  aligned_to(scales, EXF_F32),
+              "%s: codes must be 8-byte and out 16-byte aligned", name);
+  return cuda_status(launch_dequantize_8bit(static_cast<const uint8_t*>(codes), code == EXF_I8,
+                                            scales, rows, (int)cols, group, out, dtype,
+                                            (cudaStream_t)stream),
+                     name);
+}
+
+EXF_API int64_t exf_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols) {
+  if (rows < 0 || cols < 1 || rows >= ((int64_t)1 << 31) || cols >= (1 << 24)) return -1;
+  return norm_backward_workspace(rows, (int)cols);
+}
+
+EXF_API int exf_rms_norm_backward(const void* dy, const void* dsum, const void* x, int64_t x_stride,
+                                  const void* weight, int dtype, int weight_dtype, int64_t rows,
+                                  int64_t cols, float eps, void* dx, void* dweight, void* workspace,
+                                  int64_t workspace_bytes, exf_stream_t stream) {
+  const char* name = "exf_rms_norm_backward";
+  const int rc = norm_checks(name, dtype, weight_dtype, rows, cols, x_stride, eps);
+  if (rc != EXF_OK) return rc;
+  if (!dx && !dweight) return EXF_OK;
+  if (rows == 0) {
+    if (!dweight) return EXF_OK;
+    return cuda_status(cudaMemsetAsync(dweight, 0, (size_t)cols * (weight_dtype == EXF_F32 ? 4 : 2),
+                                       (cudaStream_t)stream),
+                       name);
+  }
+  EXF_REQUIRE(dy && x && weight && (workspace || !dweight), "%s: null pointer", name);
+  EXF_REQUIRE(aligned_to(dy, dtype) && aligned_to(dsum, dtype) && aligned_to(x, dtype) &&
+                  aligned_to(dx, dtype) && aligned_to(weight, weight_dtype) &&
+                  aligned_to(dweight, weight_dtype) && aligned_to(workspace, EXF_F32),
+              "%s: a tensor is not aligned to its type", name);
+  const int64_t need = norm_backward_workspace(rows, (int)cols);
+  EXF_REQUIRE(!dweight || workspace_bytes >= need, "%s: workspace of %lld bytes required", name,
+              (long long)need);
+  NormArgs a{x,    x_stride,  nullptr, 0,      weight, dtype, weight_dtype == EXF_F32,
+             rows, (int)cols, eps,     nullptr};
+  return cuda_status(
+      launch_rms_norm_backward(a, dy, dsum, dx, dweight, workspace, (cudaStream_t)stream), name);
+}
+
+// ---- balance loss -----------------------------------------------------------------------------------
+static int balance_checks(const char* name, int dtype, int groups, int64_t tokens, int experts,
+                          int top_k, int scoring) {
+  EXF_REQUIRE(good_wdtype(dtype), "%s: logits must be EXF_F32, EXF_BF16 or EXF_F16", name);
+  EXF_REQUIRE(scoring == EXF_SOFTMAX || scoring == EXF_SIGMOID,
+              "%s: scoring must be EXF_SOFTMAX or EXF_SIGMOID", name);
+  EXF_REQUIRE(groups >= 0 && tokens >= 0 && experts >= 1 && top_k >= 1, "%s: bad shape", name);
+  if (experts > 1024 || groups > 65535)
+    return fail(EXF_ERR_UNSUPPORTED, "%s: at most 1024 experts and 65535 groups", name);
+  if (tokens >= ((int64_t)1 << 31) / top_k)
+    return fail(EXF_ERR_UNSUPPORTED, "%s: a group's routes must be below 2^31", name);
+  return EXF_OK;
+}
+
+EXF_API int64_t exf_balance_loss_workspace_bytes(int groups, int64_t tokens, int experts) {
+  if (groups < 0 || groups > 65535 || tokens < 0 || tokens >= ((int64_t)1 << 31) || experts < 1 ||
+      experts > 1024)
+    return -1;
+  return groups == 0 ? 0 : balance_workspace(groups, tokens, experts);
+}
+
+EXF_API int exf_balance_loss(const void* logits, int dtype, const void* ids, int id_dtype,
+                             const uint8_t* mask, int groups, int64_t tokens, int experts, int top_k,
+                             int scoring, float* loss, int32_t* counts, int32_t* valid,
+                             void* workspace, int64_t workspace_bytes, exf_stream_t stream) {
+  const char* name = "exf_balance_loss";
+  const int rc = balance_checks(name, dtype, groups, tokens, experts, top_k, scoring);
+  if (rc != EXF_OK) return rc;
+  EXF_REQUIRE(good_idtype(id_dtype), "%s: ids must be EXF_I32 or EXF_I64", name);
+  if (groups == 0) return EXF_OK;
+  EXF_REQUIRE(loss && counts && valid, "%s: null pointer", name);
+  EXF_REQUIRE(tokens == 0 || (logits && ids && workspace), "%s: null pointer", name);
+  EXF_REQUIRE(aligned_to(logits, dtype) && aligned_to(workspace, EXF_F32) &&
+                  reinterpret_cast<uintptr_t>(ids) % (id_dtype == EXF_I64 ? 8 : 4) == 0,
+              "%s: a tensor is not aligned to its type", name);
+  const int64_t need = balance_workspace(groups, tokens, experts);
+  EXF_REQUIRE(workspace_bytes >= need, "%s: workspace of %lld bytes required", name,
+              (long long)need);
+  BalanceArgs a{logits, dtype, mask, groups, tokens, experts, top_k, scoring == EXF_SIGMOID};
+  return cuda_status(launch_balance_loss(a, ids, id_dtype == EXF_I64, workspace, loss, counts, valid,
+                                         (cudaStream_t)stream),
+                     name);
+}
+
+EXF_API int exf_balance_loss_backward(const float* dloss, const void* logits, int dtype,
+                                      const uint8_t* mask, const int32_t* counts,
+                                      const int32_t* valid, int groups, int64_t tokens, int experts,
+                                      int top_k, int scoring, void* dlogits, exf_stream_t stream) {
+  const char* name = "exf_balance_loss_backward";
+  const int rc = balance_checks(name, dtype, groups, tokens, experts, top_k, scoring);
+  if (rc != EXF_OK) return rc;
+  if (groups == 0 || tokens == 0) return EXF_OK;
+  EXF_REQUIRE(dloss && logits && counts && valid && dlogits, "%s: null pointer", name);
+  EXF_REQUIRE(aligned_to(logits, dtype) && aligned_to(dlogits, dtype),
+              "%s: a tensor is not aligned to its type", name);
+  BalanceArgs a{logits, dtype, mask, groups, tokens, experts, top_k, scoring == EXF_SIGMOID};
+  return cuda_status(
+      launch_balance_loss_backward(a, dloss, counts, valid, dlogits, (cudaStream_t)stream), name);
 }
 
 // moe_align without any device allocation: the chunk-count table lives in the library's fixed

@@ -20,6 +20,7 @@ EXF_I32, EXF_I64 = 0, 1
 EXF_SOFTMAX, EXF_SIGMOID, EXF_SQRTSOFTPLUS = 0, 1, 2
 EXF_QWEN3, EXF_DSV4 = 0, 1
 EXF_SILU, EXF_GELU_TANH = 0, 1
+EXF_E4M3, EXF_I8 = 0, 1
 
 _vp, _i, _i64, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 
@@ -73,6 +74,18 @@ SIGNATURES = {
     "exf_gated_mlp_backward_workspace_bytes": (_i64, [_i64, _i, _i]),
     "exf_gated_mlp_backward": (_i, [_vp, _vp, _vp, _vp, _i, _i64, _i, _i, _i, _vp, _vp, _vp, _i64,
                                     _vp, _vp]),
+    "exf_rms_norm": (_i, [_vp, _i64, _vp, _i64, _vp, _i, _i, _i64, _i64, _f, _vp, _vp, _vp]),
+    "exf_rms_norm_8bit": (_i, [_vp, _i64, _vp, _i64, _vp, _i, _i, _i64, _i64, _f, _i, _i, _vp, _vp,
+                               _vp, _vp]),
+    "exf_dequantize_8bit": (_i, [_vp, _i, _vp, _i64, _i64, _i, _vp, _i, _vp]),
+    "exf_rms_norm_backward_workspace_bytes": (_i64, [_i64, _i64]),
+    "exf_rms_norm_backward": (_i, [_vp, _vp, _vp, _i64, _vp, _i, _i, _i64, _i64, _f, _vp, _vp, _vp,
+                                   _i64, _vp]),
+    "exf_balance_loss_workspace_bytes": (_i64, [_i, _i64, _i]),
+    "exf_balance_loss": (_i, [_vp, _i, _vp, _i, _vp, _i, _i64, _i, _i, _i, _vp, _vp, _vp, _vp, _i64,
+                              _vp]),
+    "exf_balance_loss_backward": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _i64, _i, _i, _i, _vp,
+                                       _vp]),
 }
 
 _lock = threading.Lock()

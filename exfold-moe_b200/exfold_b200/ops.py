@@ -628,3 +628,274 @@ def gated_mlp(x: torch.Tensor, w13: torch.Tensor, activation: str = "silu",
     else:
         h, _ = _gated_forward(rows, w, act, status, False)
     return h if flat else h.view(*x.shape[:-1], h.shape[1])
+
+
+# ---- root-mean-square norm ----------------------------------------------------------------------
+_CODE = {torch.float8_e4m3fn: L.EXF_E4M3, torch.int8: L.EXF_I8}
+
+
+def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """t [..., cols] as rows [n, cols] at a constant distance, where they lie if they do."""
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
+    if (t.stride(1) == 1 or cols == 1) and (t.shape[0] <= 1 or t.stride(0) >= cols):
+        return t
+    return t.contiguous()
+
+
+def _norm_in(name, x, weight, eps, residual):
+    """The checked inputs as (x rows, residual rows or None, weight)."""
+    _require_cuda(x, weight, residual)
+    if x.dtype not in _WDT:
+        raise TypeError(f"{name} needs a float32, bfloat16 or float16 input")
+    if weight.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"{name}: the weight must be float32 or of the input's type")
+    if residual is not None and residual.dtype != x.dtype:
+        raise TypeError(f"{name}: the residual must be of the input's type")
+    if x.dim() < 1 or weight.dim() != 1 or weight.shape[0] != x.shape[-1] or x.shape[-1] == 0:
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} must be [..., H] and "
+                         "[H]")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual {tuple(residual.shape)} must have x's shape {tuple(x.shape)}")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    cols = x.shape[-1]
+    return (_rows(x, cols), None if residual is None else _rows(residual, cols),
+            weight.contiguous())
+
+
+def _norm_forward(x, residual, weight, eps):
+    """(y, s) of rows; s is x without a residual."""
+    rows, cols = x.shape
+    dev = x.device
+    y = torch.empty(rows, cols, dtype=x.dtype, device=dev)
+    s = x if residual is None else torch.empty_like(y)
+    if rows > 0:
+        with _on(dev):
+            L.check(L.lib().exf_rms_norm(
+                x.data_ptr(), x.stride(0), _ptr(residual),
+                0 if residual is None else residual.stride(0), weight.data_ptr(), _WDT[x.dtype],
+                _WDT[weight.dtype], rows, cols, eps, s.data_ptr(), y.data_ptr(), _stream(dev)))
+    return y, s
+
+
+def _norm_backward(ctx, dy, ds):
+    x, weight = ctx.saved_tensors
+    rows, cols = x.shape
+    dev, dtype = x.device, x.dtype
+    want_x, want_r, want_w, _ = ctx.needs_input_grad
+    want_x = want_x or want_r
+    dx = torch.empty(rows, cols, dtype=dtype, device=dev) if want_x else None
+    dw = torch.empty_like(weight) if want_w else None
+    if dy is None:  # only s was used
+        dy = torch.zeros(rows, cols, dtype=dtype, device=dev)
+    dy = dy.contiguous()
+    ds = None if ds is None else ds.contiguous()
+    lib = L.lib()
+    with _on(dev):
+        ws = None
+        ws_bytes = lib.exf_rms_norm_backward_workspace_bytes(rows, cols) if want_w else 0
+        if ws_bytes > 0:
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        L.check(lib.exf_rms_norm_backward(
+            dy.data_ptr(), _ptr(ds), x.data_ptr(), x.stride(0), weight.data_ptr(), _WDT[dtype],
+            _WDT[weight.dtype], rows, cols, ctx.eps, _ptr(dx), _ptr(dw), _ptr(ws), ws_bytes,
+            _stream(dev)))
+    # (the gradient of the sum is that of both of its terms)
+    return dx if ctx.needs_input_grad[0] else None, dx if want_r else None, dw, None
+
+
+_norm_backward_once = torch.autograd.function.once_differentiable(_norm_backward)
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):
+        y, s = _norm_forward(x, residual, weight, eps)
+        ctx.save_for_backward(s, weight)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        return y if residual is None else (y, s)
+
+    @staticmethod
+    def backward(ctx, dy, ds=None):
+        # recorded itself (create_graph): its gradients raise when they are differentiated
+        return (_norm_backward_once if torch.is_grad_enabled() else _norm_backward)(ctx, dy, ds)
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+             residual: torch.Tensor | None = None):
+    """y = s * weight / sqrt(mean(s^2) + eps) over the last dimension, s = x, or (y, s) with s = x +
+    residual rounded to their type.
+
+    x and residual [..., H] fp32, bf16 or fp16 (rows at a constant distance are read where they lie),
+    weight [H] fp32 or of x's type; y and s [..., H] of x's type.  Sums are fp32.  Differentiable in
+    x, residual and weight (once, in reverse mode; forward mode is refused); nothing is kept for the
+    backward pass but s.
+    """
+    rows, res, w = _norm_in("rms_norm", x, weight, eps, residual)
+    if _has_tangent(x, weight, *(() if residual is None else (residual,))):
+        raise NotImplementedError("rms_norm has no forward-mode derivative")
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                    or (residual is not None and residual.requires_grad)):
+        out = _RmsNorm.apply(rows, res, w, float(eps))
+    else:
+        out = _norm_forward(rows, res, w, float(eps))
+        out = out[0] if residual is None else out
+    if residual is None:
+        return out.view(x.shape)
+    return out[0].view(x.shape), out[1].view(x.shape)
+
+
+def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+                  residual: torch.Tensor | None = None, dtype: torch.dtype = torch.float8_e4m3fn,
+                  group: int | None = 128):
+    """`rms_norm` with its output in 8 bits: (codes, scales), or (codes, scales, s) with a residual.
+
+    codes [..., H] of dtype float8_e4m3fn or int8, scales fp32 [..., ceil(H / group)]: a scale for each
+    group of 32, 64 or 128 columns, or [..., 1] for the row (group None).  A group's largest value has
+    the largest code (448, or 127); the others are rounded to the nearest, ties to even.  Values are
+    code * scale (`dequantize_8bit`).  A group with a value that is not finite reads back as NaN.  H up to
+    2^18.  For inference: the result carries no gradient.
+    """
+    rows, res, w = _norm_in("rms_norm_8bit", x, weight, eps, residual)
+    if dtype not in _CODE:
+        raise TypeError("rms_norm_8bit gives float8_e4m3fn or int8 codes")
+    if group not in (None, 32, 64, 128):
+        raise ValueError(f"group must be 32, 64, 128 or None (a row), got {group}")
+    n, cols = rows.shape
+    dev = rows.device
+    groups = 1 if group is None else -(-cols // group)
+    codes = torch.empty(n, cols, dtype=dtype, device=dev)
+    scales = torch.empty(n, groups, dtype=torch.float32, device=dev)
+    s = None if res is None else torch.empty(n, cols, dtype=x.dtype, device=dev)
+    if n > 0:
+        with _on(dev):
+            L.check(L.lib().exf_rms_norm_8bit(
+                rows.data_ptr(), rows.stride(0), _ptr(res), 0 if res is None else res.stride(0),
+                w.data_ptr(), _WDT[x.dtype], _WDT[w.dtype], n, cols, float(eps), _CODE[dtype],
+                group or 0, _ptr(s), codes.data_ptr(), scales.data_ptr(), _stream(dev)))
+    codes, scales = codes.view(x.shape), scales.view(*x.shape[:-1], groups)
+    return (codes, scales) if s is None else (codes, scales, s.view(x.shape))
+
+
+def dequantize_8bit(codes: torch.Tensor, scales: torch.Tensor, group: int | None = 128,
+                    dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values code * scale of `rms_norm_8bit`'s codes and scales, rounded to dtype."""
+    dev = _require_cuda(codes, scales)
+    if codes.dtype not in _CODE or scales.dtype != torch.float32:
+        raise TypeError("dequantize_8bit needs float8_e4m3fn or int8 codes and float32 scales")
+    if dtype not in _WDT:
+        raise TypeError("dequantize_8bit gives float32, bfloat16 or float16")
+    if group not in (None, 32, 64, 128):
+        raise ValueError(f"group must be 32, 64, 128 or None (a row), got {group}")
+    cols = codes.shape[-1] if codes.dim() else 0
+    groups = 1 if group is None else -(-cols // group)
+    if cols == 0 or scales.shape != (*codes.shape[:-1], groups):
+        raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} must be "
+                         "[..., H] and [..., groups]")
+    codes, scales = _aligned(codes, 8), scales.contiguous()
+    out = torch.empty(codes.shape, dtype=dtype, device=dev)
+    n = out.numel()
+    if n > 0:
+        with _on(dev):
+            L.check(L.lib().exf_dequantize_8bit(codes.data_ptr(), _CODE[codes.dtype],
+                                                scales.data_ptr(), n // cols, cols, group or 0,
+                                                out.data_ptr(), _WDT[dtype], _stream(dev)))
+    return out
+
+
+# ---- balance loss -------------------------------------------------------------------------------
+def _balance_forward(logits, ids, mask, scoring):
+    groups, tokens, experts = logits.shape
+    top_k = ids.shape[-1]
+    dev = logits.device
+    loss = torch.empty(groups, dtype=torch.float32, device=dev)
+    counts = torch.empty(groups, experts, dtype=torch.int32, device=dev)
+    valid = torch.empty(groups, dtype=torch.int32, device=dev)
+    lib = L.lib()
+    with _on(dev):
+        ws_bytes = lib.exf_balance_loss_workspace_bytes(groups, tokens, experts)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
+        L.check(lib.exf_balance_loss(
+            logits.data_ptr(), _WDT[logits.dtype], ids.data_ptr(), _IDT[ids.dtype], _ptr(mask),
+            groups, tokens, experts, top_k, scoring, loss.data_ptr(), counts.data_ptr(),
+            valid.data_ptr(), _ptr(ws), ws_bytes, _stream(dev)))
+    return loss, counts, valid
+
+
+def _balance_backward(ctx, dloss, _):
+    logits, mask, counts, valid = ctx.saved_tensors
+    groups, tokens, experts = logits.shape
+    dev = logits.device
+    dlogits = torch.empty_like(logits)
+    dloss = dloss.float().contiguous()
+    with _on(dev):
+        L.check(L.lib().exf_balance_loss_backward(
+            dloss.data_ptr(), logits.data_ptr(), _WDT[logits.dtype], _ptr(mask), counts.data_ptr(),
+            valid.data_ptr(), groups, tokens, experts, ctx.top_k, ctx.scoring, dlogits.data_ptr(),
+            _stream(dev)))
+    return dlogits, None, None, None
+
+
+_balance_backward_once = torch.autograd.function.once_differentiable(_balance_backward)
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, mask, scoring):
+        loss, counts, valid = _balance_forward(logits, ids, mask, scoring)
+        ctx.save_for_backward(logits, mask, counts, valid)
+        ctx.top_k, ctx.scoring = ids.shape[-1], scoring
+        ctx.mark_non_differentiable(counts)
+        return loss, counts
+
+    @staticmethod
+    def backward(ctx, dloss, dcounts):
+        # recorded itself (create_graph): its gradients raise when they are differentiated
+        return (_balance_backward_once if torch.is_grad_enabled()
+                else _balance_backward)(ctx, dloss, dcounts)
+
+
+def balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor, scoring: str = "softmax",
+                 mask: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The balance loss of a router and the experts' counts: (loss fp32 [...], counts int32 [..., E]).
+
+    logits [..., T, E] fp32, bf16 or fp16, topk_ids [..., T, k] integers of any width (a router's routes),
+    mask bool [..., T] or None.  Each leading index (a layer, a sequence) has a loss of its own:
+    with p the softmax of a token's logits (scoring "softmax") or its sigmoids divided by their sum
+    ("sigmoid"), N the tokens that mask keeps and counts_e the routes of those to expert e,
+      loss = E / (k N^2) * sum_e counts_e * sum_t p[t, e],
+    1 when both are even, 0 for N = 0.  What stands in left-out tokens does not matter; ids outside
+    [0, E) count nowhere.  Differentiable in logits (once, in reverse mode; forward mode is refused); the
+    counts carry no gradient.  E up to 1024.
+    """
+    _require_cuda(logits, topk_ids, mask)
+    if logits.dtype not in _WDT:
+        raise TypeError("balance_loss needs float32, bfloat16 or float16 logits")
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError(f"scoring must be softmax or sigmoid, got {scoring!r}")
+    if (logits.dim() < 2 or topk_ids.shape[:-1] != logits.shape[:-1] or logits.shape[-1] == 0
+            or topk_ids.shape[-1] == 0):
+        raise ValueError(f"logits {tuple(logits.shape)} and topk_ids {tuple(topk_ids.shape)} must be "
+                         "[..., T, E] and [..., T, k]")
+    if mask is not None and (mask.dtype != torch.bool or mask.shape != logits.shape[:-1]):
+        raise ValueError(f"mask must be bool {tuple(logits.shape[:-1])}, got {mask.dtype} "
+                         f"{tuple(mask.shape)}")
+    if _has_tangent(logits):
+        raise NotImplementedError("balance_loss has no forward-mode derivative")
+    *lead, tokens, experts = logits.shape
+    groups = 1
+    for n in lead:
+        groups *= n
+    x = logits.reshape(groups, tokens, experts).contiguous()
+    if topk_ids.dtype is not torch.int64:
+        topk_ids = _expert_ids(topk_ids, experts)
+    ids = topk_ids.reshape(groups, tokens, topk_ids.shape[-1]).contiguous()
+    m = None if mask is None else mask.contiguous()
+    code = _SCORING[scoring]
+    if torch.is_grad_enabled() and logits.requires_grad:
+        loss, counts = _BalanceLoss.apply(x, ids, m, code)
+    else:
+        loss, counts, _ = _balance_forward(x, ids, m, code)
+    return loss.view(lead), counts.view(*lead, experts)

@@ -327,6 +327,61 @@ EXF_API int exf_gated_mlp_backward(const void* dh, const float* pre, const void*
                                    void* workspace, int64_t workspace_bytes, int32_t* status,
                                    exf_stream_t stream);
 
+/* Root-mean-square norm of rows, with the residual's addition: s = x + residual rounded to dtype (x
+ * itself without a residual), y_j = s_j weight_j / sqrt(mean_i s_i^2 + eps), rounded once.  These entry
+ * points and the balance loss below have no counterpart in the reference.
+ * x, residual: [rows][cols] of dtype (EXF_F32, EXF_BF16 or EXF_F16), rows x_stride and r_stride elements
+ * apart; weight [cols] fp32 or of dtype; sum (s; required with a residual, else unused) and y contiguous,
+ * neither overlapping an input.  Any number of columns and any alignment of the type (rows on 16-byte
+ * boundaries are read as vectors).  Sums are fp32; a sum of squares outside fp32's range is taken in 64 bits.
+ * exf_rms_norm_8bit: the norm as 8-bit codes [rows][cols] and scales fp32 [rows][ceil(cols / group)],
+ * group 32, 64 or 128 columns, or 0 for the row.  With p_j = s_j weight_j and a group's largest |p| = top,
+ * a code is p_j M / top rounded to the nearest e4m3 value (EXF_E4M3, M = 448) or integer (EXF_I8, M =
+ * 127), ties to even, and the scale is top / (M sqrt(mean s^2 + eps)).  A group of zeros has scale 0; one
+ * with a product that is not finite in fp32 has codes 0 and a NaN scale.  cols up to 2^18.
+ * exf_dequantize_8bit: code * scale, rounded to dtype; codes 8-byte and out 16-byte aligned.
+ * exf_rms_norm_backward: from dy and dsum (the upstream gradient of s; may be NULL), both contiguous, and x
+ * (the normed rows: sum where there was a residual), dx [rows][cols] (the gradient of x and of the
+ * residual alike) and dweight [cols] of the weight's type; either may be NULL.  workspace (for dweight):
+ * exf_rms_norm_backward_workspace_bytes(), for the current device.  No rows: dweight is zeroed. */
+enum exf_code { EXF_E4M3 = 0, EXF_I8 = 1 };
+EXF_API int exf_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t r_stride,
+                         const void* weight, int dtype, int weight_dtype, int64_t rows, int64_t cols,
+                         float eps, void* sum, void* y, exf_stream_t stream);
+EXF_API int exf_rms_norm_8bit(const void* x, int64_t x_stride, const void* residual,
+                              int64_t r_stride, const void* weight, int dtype, int weight_dtype,
+                              int64_t rows, int64_t cols, float eps, int code, int group, void* sum,
+                              void* codes, float* scales, exf_stream_t stream);
+EXF_API int exf_dequantize_8bit(const void* codes, int code, const float* scales, int64_t rows,
+                                int64_t cols, int group, void* out, int dtype, exf_stream_t stream);
+EXF_API int64_t exf_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
+EXF_API int exf_rms_norm_backward(const void* dy, const void* dsum, const void* x, int64_t x_stride,
+                                  const void* weight, int dtype, int weight_dtype, int64_t rows,
+                                  int64_t cols, float eps, void* dx, void* dweight, void* workspace,
+                                  int64_t workspace_bytes, exf_stream_t stream);
+
+/* The balance loss of a router over groups of tokens (layers, or sequences), the experts' counts, and the
+ * logits' gradient.  For the N tokens of a group that mask keeps (mask [groups][tokens] bytes, 0: left out,
+ * its logits and ids not used; NULL: all), with p the softmax of a token's logits over the experts
+ * (EXF_SOFTMAX) or its sigmoids divided by their sum (EXF_SIGMOID):
+ *   counts_e = number of ids equal to e,  loss = experts / (top_k N^2) sum_e counts_e sum_t p_te
+ * (1 when routes and scores are even; 0 for N = 0).  logits [groups][tokens][experts] EXF_F32, EXF_BF16
+ * or EXF_F16; ids [groups][tokens][top_k] EXF_I32 or EXF_I64, what lies outside [0, experts) counts
+ * nowhere; loss fp32 [groups], counts int32 [groups][experts], valid int32 [groups] (N).  A token whose
+ * logits are all -infinity has p = 0.  exf_balance_loss_backward: dlogits of the logits' type from dloss
+ * fp32 [groups] and the forward pass's counts and valid (the counts carry no gradient); left-out tokens
+ * get zeros.  At most 1024 experts, 65535 groups, 2^31 - 1 routes a group.  Sums are joined in a fixed
+ * order.  workspace: exf_balance_loss_workspace_bytes(), for the current device. */
+EXF_API int64_t exf_balance_loss_workspace_bytes(int groups, int64_t tokens, int experts);
+EXF_API int exf_balance_loss(const void* logits, int dtype, const void* ids, int id_dtype,
+                             const uint8_t* mask, int groups, int64_t tokens, int experts, int top_k,
+                             int scoring, float* loss, int32_t* counts, int32_t* valid,
+                             void* workspace, int64_t workspace_bytes, exf_stream_t stream);
+EXF_API int exf_balance_loss_backward(const float* dloss, const void* logits, int dtype,
+                                      const uint8_t* mask, const int32_t* counts,
+                                      const int32_t* valid, int groups, int64_t tokens, int experts,
+                                      int top_k, int scoring, void* dlogits, exf_stream_t stream);
+
 /* Calibration statistics (offline): the GPU form of PairwiseScalarStats
  * (exfold/qwen3/calibration.py:9-140), which builds the [E][E] coefficient / loss tables and the
  * expert norms that the folds above read.
