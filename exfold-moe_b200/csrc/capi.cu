@@ -4,8 +4,9 @@
 #include <string.h>
 
 #include <atomic>
+#include <map>
 #include <mutex>
-#include <unordered_map>
+#include <tuple>
 
 #include "exf_balance.h"
 #include "exf_common.cuh"
@@ -23,7 +24,7 @@ namespace exf {
 
 // ---- launch helpers -----------------------------------------------------------------------
 static std::mutex g_grid_mu;
-static std::unordered_map<uint64_t, int> g_grid_cache;
+static std::map<std::tuple<const void*, int, size_t, int>, int> g_grid_cache;
 
 int sm_count() {
   int dev = 0;
@@ -36,7 +37,7 @@ int sm_count() {
 int persistent_grid(const void* kernel, int threads, size_t smem) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  const uint64_t key = (reinterpret_cast<uint64_t>(kernel) << 8) ^ (uint64_t)dev;
+  const auto key = std::make_tuple(kernel, threads, smem, dev);
   {
     std::lock_guard<std::mutex> lk(g_grid_mu);
     auto it = g_grid_cache.find(key);
@@ -706,8 +707,8 @@ static int code_checks(const char* name, int code, int64_t cols, int group) {
   EXF_REQUIRE(code == EXF_E4M3 || code == EXF_I8, "%s: code must be EXF_E4M3 or EXF_I8", name);
   EXF_REQUIRE(group == 0 || group == 32 || group == 64 || group == 128,
               "%s: group must be 0 (a row), 32, 64 or 128", name);
-  if (cols > (1 << 18))
-    return fail(EXF_ERR_UNSUPPORTED, "%s: at most 2^18 columns", name);
+  if (cols > (1 << 17))
+    return fail(EXF_ERR_UNSUPPORTED, "%s: at most 2^17 columns", name);
   return EXF_OK;
 }
 
@@ -743,9 +744,8 @@ EXF_API int exf_dequantize_8bit(const void* codes, int code, const float* scales
   if (rc != EXF_OK) return rc;
   if (rows == 0) return EXF_OK;
   EXF_REQUIRE(codes && scales && out, "%s: null pointer", name);
-  EXF_REQUIRE(reinterpret_cast<uintptr_t>(codes) % 8 == 0 && aligned16(out) &&
-                  aligned_to(scales, EXF_F32),
-              "%s: codes must be 8-byte and out 16-byte aligned", name);
+  EXF_REQUIRE(aligned16(codes) && aligned16(out) && aligned_to(scales, EXF_F32),
+              "%s: codes and out must be 16-byte aligned", name);
   return cuda_status(launch_dequantize_8bit(static_cast<const uint8_t*>(codes), code == EXF_I8,
                                             scales, rows, (int)cols, group, out, dtype,
                                             (cudaStream_t)stream),

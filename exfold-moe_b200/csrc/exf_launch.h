@@ -9,7 +9,7 @@
 namespace exf {
 
 // Blocks that fill every SM of the current device at the kernel's occupancy (cached per
-// device and kernel); 0 if the query fails.
+// device, kernel, block and shared memory); 0 if the query fails.
 int persistent_grid(const void* kernel, int threads, size_t dynamic_smem);
 int sm_count();
 

@@ -3,74 +3,146 @@
 #pragma once
 
 #include "exf_common.cuh"
+#include "exf_launch.h"
 #include "exf_norm.h"
+
+#include <string.h>
+
+#include <type_traits>
 
 namespace exf {
 
-// V elements of a row of type T, one access (V = 1, or 16 bytes where base and stride allow it)
+// V elements of type T as they lie in memory: one element, or 16 bytes (fp32 weights beside 16-bit values: 32).
+// Kept as words and taken apart where they are used: as elements, the compiler gives each 16-bit one a
+// register of its own.
 template <typename T, int V>
 struct Pack {
-  T v[V];
+  static constexpr int kWords = V * sizeof(T) > 4 ? V * sizeof(T) / 4 : 1;
+  static_assert(V == 1 || V == 2 || kWords % 4 == 0, "one element, two, or whole 16-byte vectors");
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[j]);
+    } else {
+      const uint32_t two = w[j >> 1];
+      if constexpr (std::is_same<T, __half>::value)
+        return __half2float(__ushort_as_half((unsigned short)(j & 1 ? two >> 16 : two & 0xffffu)));
+      else
+        return __uint_as_float(j & 1 ? two & 0xffff0000u : two << 16);
+    }
+  }
+  __device__ __forceinline__ void set(const float (&e)[V]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[j] = __float_as_uint(e[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; j += 2) {
+        const float hi = j + 1 < V ? e[j + 1 < V ? j + 1 : j] : 0.0f;
+        if constexpr (std::is_same<T, __half>::value) {
+          const __half2 h = __floats2half2_rn(e[j], hi);
+          memcpy(&w[j >> 1], &h, 4);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(e[j], hi);
+          memcpy(&w[j >> 1], &h, 4);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void read(const T* p) {
+    if constexpr (V == 1) {
+      if constexpr (sizeof(T) == 4)
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+      else
+        w[0] = *reinterpret_cast<const uint16_t*>(p);
+    } else if constexpr (kWords < 4) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 u = reinterpret_cast<const uint4*>(p)[i / 4];
+        w[i] = u.x;
+        w[i + 1] = u.y;
+        w[i + 2] = u.z;
+        w[i + 3] = u.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void write(T* p) const {
+    if constexpr (V == 1) {
+      if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<uint32_t*>(p) = w[0];
+      else
+        *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+    } else if constexpr (kWords < 4) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) reinterpret_cast<uint32_t*>(p)[i] = w[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4)
+        reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    }
+  }
+  // the words as if newly read: what was taken from them before is not kept for later
+  __device__ __forceinline__ void anew() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) asm volatile("" : "+r"(w[i]));
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
 };
 template <typename T, int V>
 __device__ __forceinline__ void load_pack(const T* p, float (&out)[V]) {
-  if constexpr (V == 1) {
-    out[0] = to_f32<T>(*p);
-  } else {
-    static_assert(V * sizeof(T) == 16, "one 16-byte vector");
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(&u);
+  Pack<T, V> k;
+  k.read(p);
 #pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = to_f32<T>(k.v[i]);
-  }
+  for (int i = 0; i < V; ++i) out[i] = k.get(i);
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_pack(T* p, const float (&in)[V]) {
-  if constexpr (V == 1) {
-    *p = from_f32<T>(in[0]);
-  } else {
-    Pack<T, V> k;
-#pragma unroll
-    for (int i = 0; i < V; ++i) k.v[i] = from_f32<T>(in[i]);
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&k);
-  }
+  Pack<T, V> k;
+  k.set(in);
+  k.write(p);
 }
-// V weights from column c on, fp32 or of type T (16-byte aligned where V > 1)
+// V weights from column c on as fp32, of type T or fp32 (16-byte aligned where V > 1)
 template <typename T, int V>
 __device__ __forceinline__ void load_weight(const void* w, bool f32, int c, float (&out)[V]) {
-  if (f32) {
-    const float* p = static_cast<const float*>(w) + c;
-    if constexpr (V == 1) {
-      out[0] = *p;
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; i += 4) {
-        const float4 q = *reinterpret_cast<const float4*>(p + i);
-        out[i] = q.x;
-        out[i + 1] = q.y;
-        out[i + 2] = q.z;
-        out[i + 3] = q.w;
-      }
-    }
-  } else {
+  if (f32)
+    load_pack<float, V>(static_cast<const float*>(w) + c, out);
+  else
     load_pack<T, V>(static_cast<const T*>(w) + c, out);
-  }
 }
 
 // x (+ residual), rounded to T: what the norm is taken of
 template <typename T, int V>
-__device__ __forceinline__ void load_sum(const T* x, const T* r, float (&out)[V]) {
-  load_pack<T, V>(x, out);
-  if (r) {
-    float b[V];
-    load_pack<T, V>(r, b);
+__device__ __forceinline__ Pack<T, V> rounded_sum(const Pack<T, V>& x, const Pack<T, V>& r) {
+  float e[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = to_f32<T>(from_f32<T>(out[i] + b[i]));
+  for (int i = 0; i < V; ++i) e[i] = x.get(i) + r.get(i);
+  Pack<T, V> k;
+  k.set(e);
+  return k;
+}
+template <typename T, int V>
+__device__ __forceinline__ void load_sum(const T* x, const T* r, float (&out)[V]) {
+  Pack<T, V> k;
+  k.read(x);
+  if (r) {
+    Pack<T, V> b;
+    b.read(r);
+    k = rounded_sum<T, V>(k, b);
   }
+#pragma unroll
+  for (int i = 0; i < V; ++i) out[i] = k.get(i);
 }
 
 // The sum over the G threads of a row (in a fixed order), for all of them.  G <= 32: lanes of a warp; else
-// the whole block, through 32 words of shared memory that a barrier frees for the next use.
+// the whole block, through 32 words of shared memory; the next use of the same words needs a barrier of
+// all threads in between (another row_sum over other words is one).
 template <typename A>
 __device__ __forceinline__ A row_sum(A v, int g, A* shared) {
   const int w = g < 32 ? g : 32;
@@ -81,26 +153,31 @@ __device__ __forceinline__ A row_sum(A v, int g, A* shared) {
   const int warps = g >> 5, lane = threadIdx.x & 31;
   v = lane < warps ? shared[lane] : A(0);
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  __syncthreads();
   return v;
 }
-template <typename A>
-__device__ __forceinline__ A row_max(A v, int g, A* shared) {
+__device__ __forceinline__ float2 row_sum2(float2 v, int g, float2* shared) {
+  auto add = [](float2 p, int d) {
+    p.x += __shfl_xor_sync(0xffffffffu, p.x, d);
+    p.y += __shfl_xor_sync(0xffffffffu, p.y, d);
+    return p;
+  };
   const int w = g < 32 ? g : 32;
-  for (int d = w / 2; d > 0; d >>= 1) {
-    const A o = __shfl_xor_sync(0xffffffffu, v, d);
-    v = o > v ? o : v;
-  }
+  for (int d = w / 2; d > 0; d >>= 1) v = add(v, d);
   if (g <= 32) return v;
   if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
   __syncthreads();
   const int warps = g >> 5, lane = threadIdx.x & 31;
-  v = lane < warps ? shared[lane] : A(0);
-  for (int d = 16; d > 0; d >>= 1) {
+  v = lane < warps ? shared[lane] : make_float2(0.0f, 0.0f);
+  for (int d = 16; d > 0; d >>= 1) v = add(v, d);
+  return v;
+}
+// the largest over `lanes` neighbouring lanes
+template <typename A>
+__device__ __forceinline__ A warp_max(A v, int lanes) {
+  for (int d = lanes / 2; d > 0; d >>= 1) {
     const A o = __shfl_xor_sync(0xffffffffu, v, d);
     v = o > v ? o : v;
   }
-  __syncthreads();
   return v;
 }
 
@@ -111,21 +188,127 @@ __device__ __forceinline__ bool out_of_range(float sum, float eps) {
   return !(sum < 3.0e38f) || (sum < 1.0e-28f && eps < 1.0e-26f);
 }
 
-// 1 / sqrt(mean square + eps) of a row from its threads' sums q; sum64 gives a thread's sum in 64 bits.  Every
-// thread of the block calls it.
-template <typename F>
-__device__ __forceinline__ float inverse_norm(float q, const NormArgs& a, int g, float* part,
-                                              double* part64, F sum64) {
+// A thread's sums of a row's squares, and of w dy s where dy is given, in 64 bits (read again from memory;
+// out of line, so that its registers cost the usual path nothing).
+template <typename T>
+__device__ __noinline__ double2 sums_64(const T* x, const T* r, const T* dy, const void* weight,
+                                        bool weight_f32, int cols, int t, int g) {
+  double2 d = make_double2(0.0, 0.0);
+  for (int c = t; c < cols; c += g) {
+    float s[1], e[1], w[1];
+    load_sum<T, 1>(x + c, r ? r + c : nullptr, s);
+    d.x = fma((double)s[0], (double)s[0], d.x);
+    if (dy) {
+      load_pack<T, 1>(dy + c, e);
+      load_weight<T, 1>(weight, weight_f32, c, w);
+      d.y = fma((double)e[0] * (double)w[0], (double)s[0], d.y);
+    }
+  }
+  return d;
+}
+
+// 1 / sqrt(mean square + eps) of a row from its threads' sums q; x, r: the row.  Every thread of the block
+// calls it.
+template <typename T>
+__device__ __forceinline__ float inverse_norm(float q, const NormArgs& a, int g, int t, const T* x,
+                                              const T* r, float* part, double* part64) {
   q = row_sum(q, g, part);
   float v = rsqrtf(q / (float)a.cols + a.eps);
   const bool again = out_of_range(q, a.eps);
   // (the same for the block where a row is a block; else the warp's other rows go along)
   if (g > 32 ? again : __any_sync(0xffffffffu, again)) {
-    const double d = row_sum(sum64(), g, part64);
-    if (again) v = (float)(1.0 / sqrt(d / a.cols + (double)a.eps));
+    const double2 d = sums_64<T>(x, r, nullptr, nullptr, false, a.cols, t, g);
+    const double sum = row_sum(d.x, g, part64);
+    if (g > 32) __syncthreads();
+    if (again) v = (float)(1.0 / sqrt(sum / a.cols + (double)a.eps));
   }
   return v;
 }
+
+// ---- rows in units -----------------------------------------------------------------------------------
+// A row is taken in units of V elements, a unit being one aligned access: 16 bytes where base, stride and
+// length allow it; else 4 bytes (two 16-bit elements, V = 2), rows that begin on an odd element having
+// units that begin one element earlier (shift 1); else one element.  Unit u holds the columns V u - shift
+// + [0, V); those outside the row are zeros, and are not written.
+template <int V>
+__device__ __forceinline__ int units_of(int cols, int shift) {
+  return V == 2 ? (cols + shift + 1) / 2 : cols / V;
+}
+template <typename T, int V>
+__device__ __forceinline__ void read_unit(Pack<T, V>& k, const T* row, int u, int cols, int shift) {
+  if constexpr (V == 2) {
+    const int c = 2 * u - shift;
+    if (c >= 0 && c + 1 < cols) {
+      k.read(row + c);
+    } else {
+      k.w[0] = c >= 0 ? *reinterpret_cast<const uint16_t*>(row + c) : 0u;
+      if (c + 1 < cols) k.w[0] |= (uint32_t)*reinterpret_cast<const uint16_t*>(row + c + 1) << 16;
+    }
+  } else {
+    k.read(row + u * V);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void write_unit(const Pack<T, V>& k, T* row, int u, int cols, int shift) {
+  if constexpr (V == 2) {
+    const int c = 2 * u - shift;
+    if (c >= 0 && c + 1 < cols) {
+      k.write(row + c);
+    } else {
+      if (c >= 0) *reinterpret_cast<uint16_t*>(row + c) = (uint16_t)k.w[0];
+      if (c + 1 < cols) *reinterpret_cast<uint16_t*>(row + c + 1) = (uint16_t)(k.w[0] >> 16);
+    }
+  } else {
+    k.write(row + u * V);
+  }
+}
+
+// The weights of a thread's units, kept from row to row; V = 2: for both shifts (fp32 ones are read again
+// each time: 32 registers else).
+template <typename W, int V, int NU>
+struct Weights {
+  static constexpr bool kKept = !(V == 2 && sizeof(W) == 4);
+  static constexpr int kShifts = V == 2 && kKept ? 2 : 1;
+  Pack<W, V> w[kShifts][kKept ? NU : 1];
+  __device__ __forceinline__ void init(const void* weight, int t, int g, int cols) {
+    if constexpr (kKept) {
+#pragma unroll
+      for (int h = 0; h < kShifts; ++h)
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+          w[h][i].clear();
+          const int u = t + g * i;
+          if (h == 0) {
+            if (u < units_of<V>(cols, 0))
+              read_unit<W, V>(w[h][i], static_cast<const W*>(weight), u, cols, 0);
+          } else {  // (the weights themselves do not move: columns 2 u - 1 and 2 u, one by one)
+            const uint16_t* p = static_cast<const uint16_t*>(weight) + 2 * u;
+            if (u > 0 && 2 * u - 1 < cols) w[h][i].w[0] = p[-1];
+            if (2 * u < cols) w[h][i].w[0] |= (uint32_t)p[0] << 16;
+          }
+        }
+    }
+  }
+  // those of unit u, the thread's i-th
+  __device__ __forceinline__ Pack<W, V> of(const void* weight, int i, int u, int cols, int shift) {
+    if constexpr (kShifts == 2) {
+      Pack<W, V> k = w[0][i];
+      k.w[0] = shift ? w[kShifts - 1][i].w[0] : k.w[0];
+      return k;
+    } else if constexpr (kKept) {
+      w[0][i].anew();
+      return w[0][i];
+    } else {
+      const W* p = static_cast<const W*>(weight);
+      const int c = 2 * u - shift;
+      Pack<W, V> k;
+      k.clear();
+      if (c >= 0 && c < cols) k.w[0] = *reinterpret_cast<const uint32_t*>(p + c);
+      if (c + 1 < cols) k.w[V - 1] = *reinterpret_cast<const uint32_t*>(p + c + 1);
+      return k;
+    }
+  }
+};
 
 // ---- layout, host side --------------------------------------------------------------------------------
 static inline bool norm_aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -137,14 +320,44 @@ static inline int norm_threads(int64_t units, int per, int least) {
   return g;
 }
 
-// Whether rows can be read and written as 16-byte vectors.
-template <typename T>
-static bool norm_vectors(const NormArgs& a) {
+// Blocks that fill the card once, at most one for each of `need`.
+static inline unsigned stay_grid(const void* kernel, int block, size_t smem, int64_t need) {
+  const int64_t most = persistent_grid(kernel, block, smem);
+  return (unsigned)(most > 0 && most < need ? most : need);
+}
+
+// The widest unit that every row of the call allows: 16 bytes, two 16-bit elements (base aligned to 4
+// bytes; rows of the inputs and the results then begin on odd elements together), or one element.
+enum NormUnit { kVector, kPair, kSingle };
+template <typename T, typename... P>
+static NormUnit norm_unit(const NormArgs& a, P... others) {
   constexpr int V = 16 / sizeof(T);
-  return a.cols % V == 0 &&
-         (a.rows == 1 || (a.x_stride % V == 0 && (!a.residual || a.r_stride % V == 0))) &&
-         norm_aligned(a.x) && norm_aligned(a.residual) && norm_aligned(a.weight) &&
-         norm_aligned(a.sum);
+  const void* all[] = {a.x, a.residual, a.sum, others...};
+  uintptr_t bits = 0;
+  for (const void* p : all) bits |= reinterpret_cast<uintptr_t>(p);
+  const int64_t xs = a.rows > 1 ? a.x_stride : a.cols;
+  const int64_t rs = a.rows > 1 && a.residual ? a.r_stride : a.cols;
+  if (a.cols % V == 0 && xs % V == 0 && rs % V == 0 && bits % 16 == 0 && norm_aligned(a.weight))
+    return kVector;
+  if (sizeof(T) == 2 && bits % 4 == 0 && (xs - a.cols) % 2 == 0 && (rs - a.cols) % 2 == 0 &&
+      (a.weight_f32 || reinterpret_cast<uintptr_t>(a.weight) % 4 == 0))
+    return kPair;
+  return kSingle;
+}
+
+// f(weight type, V) for the call's unit and weight
+template <typename T, typename F>
+static cudaError_t norm_dispatch(const NormArgs& a, NormUnit unit, F f) {
+  using std::integral_constant;
+  auto by_weight = [&](auto v) {
+    if constexpr (!std::is_same<T, float>::value)
+      if (!a.weight_f32) return f(T(), v);
+    return f(float(), v);
+  };
+  if (unit == kVector) return by_weight(integral_constant<int, 16 / sizeof(T)>());
+  if constexpr (sizeof(T) == 2)
+    if (unit == kPair) return by_weight(integral_constant<int, 2>());
+  return by_weight(integral_constant<int, 1>());
 }
 
 }  // namespace exf

@@ -19,239 +19,335 @@
 namespace exf {
 
 // ---- forward ------------------------------------------------------------------------------------
-// G threads a row, NV units of V elements a thread (unit u = thread + G * i); NV = 0: rows of any length,
-// read again after the reduction.
-template <typename T, int V, int NV>
-__global__ void __launch_bounds__(1024)
+// Blocks that stay: G threads a row, NU units of V elements a thread (unit u = thread + G * i).  The next
+// row's loads are issued before this row is reduced, so that memory stays busy through the reduction and
+// its barrier, and the weights stay in registers.  (A block a row, without either: 32768 x 4096 bf16 with a
+// residual 255 us.)  G <= 32: a block holds 128 / G rows, and nothing waits but lanes for lanes.
+template <typename T, typename W, int V, int NU, int THREADS>
+__global__ void __launch_bounds__(THREADS)
     rms_norm_kernel(const NormArgs a, int g, T* y) {
-  __shared__ float part[32];
-  __shared__ double part64[32];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int per_block = blockDim.x / g;
-  const int64_t row = (int64_t)blockIdx.x * per_block + threadIdx.x / g;
-  const int t = threadIdx.x % g;
-  const bool live = row < a.rows;
-  const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.x_stride;
-  const T* r = a.residual ? static_cast<const T*>(a.residual) + (live ? row : 0) * a.r_stride : nullptr;
-  T* sum_out = a.residual && live ? static_cast<T*>(a.sum) + row * a.cols : nullptr;
-  const int units = a.cols / V;
-
-  constexpr int N = NV > 0 ? NV : 1;
-  float s[N][V];
-  float q = 0.0f;
-  if constexpr (NV > 0) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int u = t + g * i;
-      if (u < units) {
-        load_sum<T, V>(x + u * V, r ? r + u * V : nullptr, s[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) s[i][j] = 0.0f;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) q = fmaf(s[i][j], s[i][j], q);
-  } else {
-    for (int u = t; u < units; u += g) {
-      load_sum<T, V>(x + u * V, r ? r + u * V : nullptr, s[0]);
-#pragma unroll
-      for (int j = 0; j < V; ++j) q = fmaf(s[0][j], s[0][j], q);
-    }
-  }
-  // up to two units' weights are on their way during the reduction
-  constexpr bool kEarly = NV == 1 || NV == 2 || V == 1 && NV == 4;
-  float w[N][V];
-  if constexpr (kEarly) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (t + g * i < units) load_weight<T, V>(a.weight, a.weight_f32, (t + g * i) * V, w[i]);
-  }
-  const float v = inverse_norm(q, a, g, part, part64, [&] {
-    double d = 0.0;
-    if constexpr (NV > 0) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) d = fma((double)s[i][j], (double)s[i][j], d);
-    } else {
-      for (int u = t; u < units; u += g) {
-        load_sum<T, V>(x + u * V, r ? r + u * V : nullptr, s[0]);
-#pragma unroll
-        for (int j = 0; j < V; ++j) d = fma((double)s[0][j], (double)s[0][j], d);
-      }
-    }
-    return d;
-  });
-  if (!live) return;
-  T* out = y + row * a.cols;
-  auto finish = [&](int u, float (&e)[V], float (&we)[V]) {
-    if (!kEarly) load_weight<T, V>(a.weight, a.weight_f32, u * V, we);
-    if (sum_out) store_pack<T, V>(sum_out + u * V, e);
-#pragma unroll
-    for (int j = 0; j < V; ++j) e[j] = e[j] * v * we[j];
-    store_pack<T, V>(out + u * V, e);
-  };
-  if constexpr (NV > 0) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (t + g * i < units) finish(t + g * i, s[i], w[kEarly ? i : 0]);
-  } else {
-    for (int u = t; u < units; u += g) {
-      load_sum<T, V>(x + u * V, r ? r + u * V : nullptr, s[0]);
-      finish(u, s[0], w[0]);
-    }
-  }
-}
-
-// ---- backward -----------------------------------------------------------------------------------
-// Blocks that stay: a thread keeps its columns from row to row and adds dw in registers; each block's sums
-// go to part [blocks][cols] and rms_norm_join_kernel adds them in order.  (NV = 0: the sums stay in part.)
-template <typename T, int V, int NV>
-__global__ void __launch_bounds__(1024)
-    rms_norm_backward_kernel(const NormArgs a, int g, const T* dy, const T* ds,
-                             T* dx, float* part_dw) {
   __shared__ float part[2][32];
   __shared__ double part64[32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int per_block = blockDim.x / g;
-  const int sub = threadIdx.x / g, t = threadIdx.x % g;
-  const int units = a.cols / V;
-  const float mean = 1.0f / (float)a.cols;
-  constexpr int N = NV > 0 ? NV : 1;
-  float acc[N][V];
+  const int t = threadIdx.x % g;
+  const T* x = static_cast<const T*>(a.x);
+  const T* r = static_cast<const T*>(a.residual);
+  T* sum = static_cast<T*>(a.sum);
+  const int64_t step = (int64_t)gridDim.x * per_block;
+  int64_t row = (int64_t)blockIdx.x * per_block + threadIdx.x / g;
+
+  Pack<T, V> nx[NU], nr[NU], s[NU];
+  Weights<W, V, NU> w;
+  auto shift_of = [&](int64_t at) { return V == 2 ? (int)at & a.cols & 1 : 0; };
+  auto fetch = [&](int64_t at) {
+    const int shift = shift_of(at), units = units_of<V>(a.cols, shift);
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) acc[i][j] = 0.0f;
-  bool first = true;
-  for (int64_t base = (int64_t)blockIdx.x * per_block; base < a.rows;
-       base += (int64_t)gridDim.x * per_block) {
-    const int64_t row = base + sub;
-    const bool live = row < a.rows;
-    const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.x_stride;
-    const T* up = dy + (live ? row : 0) * (int64_t)a.cols;
-    const T* side = ds ? ds + (live ? row : 0) * (int64_t)a.cols : nullptr;
-    float s[N][V], d[N][V];
-    float q = 0.0f, c = 0.0f;
-    auto take = [&](int u, float (&sv)[V], float (&dv)[V]) {
-      float w[V];
-      load_pack<T, V>(x + u * V, sv);
-      load_pack<T, V>(up + u * V, dv);
-      load_weight<T, V>(a.weight, a.weight_f32, u * V, w);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        q = fmaf(sv[j], sv[j], q);
-        c = fmaf(dv[j] * w[j], sv[j], c);
+    for (int i = 0; i < NU; ++i) {
+      const int u = t + g * i;
+      if (u < units && at < a.rows) {
+        read_unit<T, V>(nx[i], x + at * a.x_stride, u, a.cols, shift);
+        if (r) read_unit<T, V>(nr[i], r + at * a.r_stride, u, a.cols, shift);
+      } else {
+        nx[i].clear();
+        nr[i].clear();
       }
-    };
-    if constexpr (NV > 0) {
+    }
+  };
+  fetch(row);
+  w.init(a.weight, t, g, a.cols);
+  // every thread of a block (G <= 32: of a warp) takes as many turns
+  const int64_t first = (int64_t)blockIdx.x * per_block;
+  int b = 0;
+  for (int64_t base = first; base < a.rows; base += step, row += step, b ^= 1) {
+    float q = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (t + g * i < units) {
-          take(t + g * i, s[i], d[i]);
-        } else {
+    for (int i = 0; i < NU; ++i) {
+      s[i] = r ? rounded_sum<T, V>(nx[i], nr[i]) : nx[i];
 #pragma unroll
-          for (int j = 0; j < V; ++j) s[i][j] = d[i][j] = 0.0f;
+      for (int j = 0; j < V; ++j) q = fmaf(s[i].get(j), s[i].get(j), q);
+    }
+    const bool live = row < a.rows;
+    const int64_t at = row * a.cols;
+    const int shift = shift_of(row), units = units_of<V>(a.cols, shift);
+    fetch(row + step);
+    if (r && live) {
+#pragma unroll
+      for (int i = 0; i < NU; ++i)
+        if (t + g * i < units) write_unit<T, V>(s[i], sum + at, t + g * i, a.cols, shift);
+    }
+    const int64_t mine = live ? row : 0;
+    const float v = inverse_norm<T>(q, a, g, t, x + mine * a.x_stride,
+                                       r ? r + mine * a.r_stride : nullptr, part[b], part64);
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        const int u = t + g * i;
+        s[i].anew();
+        if (u < units) {
+          const Pack<W, V> k = w.of(a.weight, i, u, a.cols, shift);
+          float e[V];
+#pragma unroll
+          for (int j = 0; j < V; ++j) e[j] = s[i].get(j) * v * k.get(j);
+          Pack<T, V> o;
+          o.set(e);
+          write_unit<T, V>(o, y + at, u, a.cols, shift);
         }
       }
-    } else {
-      for (int u = t; u < units; u += g) take(u, s[0], d[0]);
     }
-    q = row_sum(q, g, part[0]);
-    c = row_sum(c, g, part[1]);
+  }
+}
+
+// Rows of any length, read again after the reduction; a block a row.
+template <typename T, int V>
+__global__ void __launch_bounds__(1024) rms_norm_long_kernel(const NormArgs a, T* y) {
+  __shared__ float part[32];
+  __shared__ double part64[32];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+  const T* r = a.residual ? static_cast<const T*>(a.residual) + row * a.r_stride : nullptr;
+  const int units = a.cols / V;
+  float s[V];
+  float q = 0.0f;
+#pragma unroll 4
+  for (int u = threadIdx.x; u < units; u += 1024) {
+    load_sum<T, V>(x + u * V, r ? r + u * V : nullptr, s);
+#pragma unroll
+    for (int j = 0; j < V; ++j) q = fmaf(s[j], s[j], q);
+  }
+  const float v = inverse_norm<T>(q, a, 1024, threadIdx.x, x, r, part, part64);
+#pragma unroll 4
+  for (int u = threadIdx.x; u < units; u += 1024) {
+    float w[V];
+    load_sum<T, V>(x + u * V, r ? r + u * V : nullptr, s);
+    load_weight<T, V>(a.weight, a.weight_f32, u * V, w);
+    if (r) store_pack<T, V>(static_cast<T*>(a.sum) + row * a.cols + u * V, s);
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = s[j] * v * w[j];
+    store_pack<T, V>(y + row * a.cols + u * V, s);
+  }
+}
+
+// ---- backward -----------------------------------------------------------------------------------
+// The same blocks and layout; a thread keeps its columns from row to row and adds dw in registers.  Each
+// block's sums go to part_dw [blocks][cols], and rms_norm_join_kernel adds them in order.
+template <typename T, typename W, int V, int NU, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+    rms_norm_backward_kernel(const NormArgs a, int g, const T* dy, const T* ds, T* dx,
+                             float* part_dw) {
+  __shared__ float2 part[2][32];
+  __shared__ double part64[32];
+  extern __shared__ float sums[];  // [per_block][cols] where a block has several rows
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int per_block = blockDim.x / g;
+  const int sub = threadIdx.x / g, t = threadIdx.x % g;
+  const float mean = 1.0f / (float)a.cols;
+  const T* x = static_cast<const T*>(a.x);
+  const int64_t step = (int64_t)gridDim.x * per_block;
+  const int64_t first = (int64_t)blockIdx.x * per_block;
+  int64_t row = first + sub;
+
+  Pack<T, V> nx[NU], ny[NU], nd[NU];
+  Weights<W, V, NU> w;
+  // V = 2: a third sum, so that the column before an odd row's unit has a place of its own
+  constexpr int A = V == 2 ? 3 : V;
+  float acc[NU][A];
+  auto shift_of = [&](int64_t at) { return V == 2 ? (int)at & a.cols & 1 : 0; };
+  auto fetch = [&](int64_t at) {
+    const int shift = shift_of(at), units = units_of<V>(a.cols, shift);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int u = t + g * i;
+      if (u < units && at < a.rows) {
+        read_unit<T, V>(nx[i], x + at * a.x_stride, u, a.cols, shift);
+        read_unit<T, V>(ny[i], dy + at * a.cols, u, a.cols, shift);
+        if (ds) read_unit<T, V>(nd[i], ds + at * a.cols, u, a.cols, shift);
+      } else {
+        nx[i].clear();
+        ny[i].clear();
+        nd[i].clear();
+      }
+    }
+  };
+  // (1024 threads have no registers for the row after this one)
+  constexpr bool kAhead = THREADS < 1024;
+  if (kAhead) fetch(row);
+  w.init(a.weight, t, g, a.cols);
+#pragma unroll
+  for (int i = 0; i < NU; ++i)
+#pragma unroll
+    for (int j = 0; j < A; ++j) acc[i][j] = 0.0f;
+  int b = 0;
+  for (int64_t base = first; base < a.rows; base += step, row += step, b ^= 1) {
+    Pack<T, V> s[NU], d[NU], o[NU];
+    float q = 0.0f, c = 0.0f;
+    if (!kAhead) fetch(row);
+    const int shift = shift_of(row), units = units_of<V>(a.cols, shift);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      s[i] = nx[i];
+      d[i] = ny[i];
+      o[i] = nd[i];
+      const Pack<W, V> k = w.of(a.weight, i, t + g * i, a.cols, shift);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float e = s[i].get(j);
+        q = fmaf(e, e, q);
+        c = fmaf(d[i].get(j) * k.get(j), e, c);
+      }
+    }
+    if (kAhead) fetch(row + step);
+    const float2 both = row_sum2(make_float2(q, c), g, part[b]);
+    q = both.x;
+    c = both.y;
     float v = rsqrtf(q * mean + a.eps);
     float k = c * mean * v;
     const bool again = out_of_range(q, a.eps) || !(fabsf(c) < 3.0e38f);
     if (g > 32 ? again : __any_sync(0xffffffffu, again)) {
-      double q64 = 0.0, c64 = 0.0;
-      for (int u = t; u < units; u += g) {
-        float e[V], o[V], w[V];
-        load_pack<T, V>(x + u * V, e);
-        load_pack<T, V>(up + u * V, o);
-        load_weight<T, V>(a.weight, a.weight_f32, u * V, w);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          q64 = fma((double)e[j], (double)e[j], q64);
-          c64 = fma((double)o[j] * (double)w[j], (double)e[j], c64);
-        }
-      }
-      q64 = row_sum(q64, g, part64);
-      c64 = row_sum(c64, g, part64);
+      const int64_t mine = row < a.rows ? row : 0;
+      const double2 d64 = sums_64<T>(x + mine * a.x_stride, nullptr, dy + mine * a.cols, a.weight,
+                                        std::is_same<W, float>::value, a.cols, t, g);
+      const double q64 = row_sum(d64.x, g, part64);
+      if (g > 32) __syncthreads();
+      const double c64 = row_sum(d64.y, g, part64);
+      if (g > 32) __syncthreads();
       if (again) {
         const double v64 = 1.0 / sqrt(q64 / a.cols + (double)a.eps);
         v = (float)v64;
         k = (float)(c64 / a.cols * v64);
       }
     }
-    auto give = [&](int u, const float (&sv)[V], const float (&dv)[V], float (&sum)[V], bool add) {
-      if (part_dw) {
+    if (row < a.rows) {
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        const int u = t + g * i;
+        s[i].anew();
+        d[i].anew();
+        const Pack<W, V> f = w.of(a.weight, i, u, a.cols, shift);
+        float e[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float e = dv[j] * (sv[j] * v);
-          sum[j] = add ? sum[j] + e : e;
-        }
-      }
-      if (dx) {
-        float w[V], o[V], e[V];
-        load_weight<T, V>(a.weight, a.weight_f32, u * V, w);
-        if (side) load_pack<T, V>(side + u * V, o);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          e[j] = v * fmaf(-(sv[j] * v), k, dv[j] * w[j]);
-          if (side) e[j] += o[j];
-        }
-        store_pack<T, V>(dx + row * a.cols + u * V, e);
-      }
-    };
-    if (live) {
-      if constexpr (NV > 0) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (t + g * i < units) give(t + g * i, s[i], d[i], acc[i], true);
-      } else {
-        for (int u = t; u < units; u += g) {
-          load_pack<T, V>(x + u * V, s[0]);
-          load_pack<T, V>(up + u * V, d[0]);
-          float* at = part_dw ? part_dw + (int64_t)blockIdx.x * a.cols + u * V : nullptr;
-          if (at && !first) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) acc[0][j] = at[j];
+          const float hat = s[i].get(j) * v, up = d[i].get(j);
+          if constexpr (V == 2) {  // acc: the columns 2 u - 1, 2 u and 2 u + 1
+            const float add = up * hat;
+            acc[i][j] += shift ? add : 0.0f;
+            acc[i][j + 1] += shift ? 0.0f : add;
+          } else {
+            acc[i][j] = fmaf(up, hat, acc[i][j]);
           }
-          give(u, s[0], d[0], acc[0], !first);
-          if (at) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) at[j] = acc[0][j];
-          }
+          e[j] = v * fmaf(-hat, k, up * f.get(j));
+          if (ds) e[j] += o[i].get(j);
+        }
+        if (dx && u < units) {
+          Pack<T, V> out;
+          out.set(e);
+          write_unit<T, V>(out, dx + row * a.cols, u, a.cols, shift);
         }
       }
     }
-    first = false;
   }
-  if (NV == 0 || !part_dw) return;
-  // the block's rows beside one another are added in order
-  extern __shared__ float sums[];  // [per_block][cols] where a block has several rows
+  if (!part_dw) return;
   float* to = part_dw + (int64_t)blockIdx.x * a.cols;
+  if constexpr (V == 2) {
+    // two threads share a column: one adds after the other; the rows of a block, one after another
+    float* at = per_block > 1 ? sums + sub * a.cols : to;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int u = t + g * i;
-    if (u < units) {
+    for (int i = 0; i < NU; ++i) {
+      const int c = 2 * (t + g * i);
+      if (c < a.cols) at[c] = acc[i][1];
+      if (c + 1 < a.cols) at[c + 1] = acc[i][2];
+    }
+    __syncthreads();
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        (per_block > 1 ? sums + sub * a.cols : to)[u * V + j] = acc[i][j];
+    for (int i = 0; i < NU; ++i) {
+      const int c = 2 * (t + g * i) - 1;
+      if (c > 0 && c < a.cols) at[c] += acc[i][0];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int u = t + g * i;
+      if (u < units_of<V>(a.cols, 0)) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          (per_block > 1 ? sums + sub * a.cols : to)[u * V + j] = acc[i][j];
+      }
     }
   }
+  // the block's rows beside one another are added in order
   if (per_block > 1) {
     __syncthreads();
     for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
       float e = 0.0f;
-      for (int b = 0; b < per_block; ++b) e += sums[b * a.cols + c];
+      for (int p = 0; p < per_block; ++p) e += sums[p * a.cols + c];
       to[c] = e;
     }
+  }
+}
+
+// Rows of any length, read again after the reduction; dw is added in part_dw itself, by the thread of its
+// column.
+template <typename T, int V>
+__global__ void __launch_bounds__(1024)
+    rms_norm_backward_long_kernel(const NormArgs a, const T* dy, const T* ds, T* dx,
+                                  float* part_dw) {
+  __shared__ float2 part[32];
+  __shared__ double part64[2][32];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int units = a.cols / V;
+  const float mean = 1.0f / (float)a.cols;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    const T* up = dy + row * a.cols;
+    float s[V], d[V], w[V];
+    float q = 0.0f, c = 0.0f;
+#pragma unroll 2
+    for (int u = threadIdx.x; u < units; u += 1024) {
+      load_pack<T, V>(x + u * V, s);
+      load_pack<T, V>(up + u * V, d);
+      load_weight<T, V>(a.weight, a.weight_f32, u * V, w);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        q = fmaf(s[j], s[j], q);
+        c = fmaf(d[j] * w[j], s[j], c);
+      }
+    }
+    const float2 both = row_sum2(make_float2(q, c), 1024, part);
+    q = both.x;
+    c = both.y;
+    float v = rsqrtf(q * mean + a.eps);
+    float k = c * mean * v;
+    if (out_of_range(q, a.eps) || !(fabsf(c) < 3.0e38f)) {
+      const double2 d64 = sums_64<T>(x, nullptr, up, a.weight, a.weight_f32, a.cols, threadIdx.x, 1024);
+      const double q64 = row_sum(d64.x, 1024, part64[0]);
+      const double c64 = row_sum(d64.y, 1024, part64[1]);
+      const double v64 = 1.0 / sqrt(q64 / a.cols + (double)a.eps);
+      v = (float)v64;
+      k = (float)(c64 / a.cols * v64);
+    }
+    float* to = part_dw ? part_dw + (int64_t)blockIdx.x * a.cols : nullptr;
+#pragma unroll 2
+    for (int u = threadIdx.x; u < units; u += 1024) {
+      float e[V], o[V];
+      load_pack<T, V>(x + u * V, s);
+      load_pack<T, V>(up + u * V, d);
+      load_weight<T, V>(a.weight, a.weight_f32, u * V, w);
+      if (ds) load_pack<T, V>(ds + row * a.cols + u * V, o);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float hat = s[j] * v;
+        e[j] = v * fmaf(-hat, k, d[j] * w[j]);
+        if (ds) e[j] += o[j];
+        if (to) to[u * V + j] = row == blockIdx.x ? d[j] * hat : fmaf(d[j], hat, to[u * V + j]);
+      }
+      if (dx) store_pack<T, V>(dx + row * a.cols + u * V, e);
+    }
+    __syncthreads();  // (the sums' shared memory is free for the next row)
   }
 }
 
@@ -278,36 +374,30 @@ __global__ void __launch_bounds__(512) rms_norm_join_kernel(const float* part, i
 }
 
 // ---- host side ----------------------------------------------------------------------------------
-template <typename T, int V>
+template <typename T, typename W, int V>
 static cudaError_t forward_v(const NormArgs& a, void* y, cudaStream_t s) {
-  const int64_t units = a.cols / V;
-  // few rows: a unit a thread, the shortest chain; else two (single elements: four), so that more loads
-  // are in flight a thread
-  const int per = a.rows < 296 ? 1 : V > 1 ? 2 : 4;
-  const int g = norm_threads(units, per, 8);
-  const int block = g <= 32 ? 128 : g;
-  const int per_block = block / g;
-  const int64_t grid = (a.rows + per_block - 1) / per_block;
-  const int need = (int)((units + g - 1) / g);
+  constexpr int NU = V > 2 ? 2 : 8;
+  const int64_t units = V == 2 ? a.cols / 2 + 1 : a.cols / V;
   auto* out = static_cast<T*>(y);
-  auto go = [&](auto* kern) {
-    return launch_pdl(kern, dim3((unsigned)grid), dim3(block), 0, s, a, g, out);
+  if (units > 1024 * NU)
+    return launch_pdl(rms_norm_long_kernel<T, V == 2 ? 1 : V>, dim3((unsigned)a.rows), dim3(1024), 0, s, a, out);
+  auto go = [&](auto* kern, int g, int block) {
+    const int64_t need = (a.rows + block / g - 1) / (block / g);
+    const unsigned grid = stay_grid(reinterpret_cast<const void*>(kern), block, 0, need);
+    return launch_pdl(kern, dim3(grid), dim3(block), 0, s, a, g, out);
   };
-  if (need <= 1) return go(rms_norm_kernel<T, V, 1>);
-  if (V > 1) {
-    if (need <= 2) return go(rms_norm_kernel<T, V, 2>);
-    if (need <= 4) return go(rms_norm_kernel<T, V, (V > 1 ? 4 : 1)>);
-  } else {
-    if (need <= 4) return go(rms_norm_kernel<T, V, 4>);
-    if (need <= 16) return go(rms_norm_kernel<T, V, (V > 1 ? 1 : 16)>);
-  }
-  return go(rms_norm_kernel<T, V, 0>);
+  // few rows: half as many units a thread, the shorter chain
+  const int g = norm_threads(units, a.rows <= 148 ? NU / 2 : NU, 8);
+  const int block = g <= 32 ? 128 : g;
+  if (block <= 256) return go(rms_norm_kernel<T, W, V, NU, 256>, g, block);
+  return go(rms_norm_kernel<T, W, V, NU, 1024>, g, block);
 }
 
 template <typename T>
 static cudaError_t forward_t(const NormArgs& a, void* y, cudaStream_t s) {
-  return norm_vectors<T>(a) && norm_aligned(y) ? forward_v<T, 16 / sizeof(T)>(a, y, s)
-                                               : forward_v<T, 1>(a, y, s);
+  return norm_dispatch<T>(a, norm_unit<T>(a, y), [&](auto w, auto v) {
+    return forward_v<T, decltype(w), decltype(v)::value>(a, y, s);
+  });
 }
 
 cudaError_t launch_rms_norm(const NormArgs& a, void* y, cudaStream_t s) {
@@ -316,61 +406,57 @@ cudaError_t launch_rms_norm(const NormArgs& a, void* y, cudaStream_t s) {
   return forward_t<__half>(a, y, s);
 }
 
-// Blocks of the backward pass: four on an SM at 256 threads; at most a row each.
-static int64_t backward_blocks(int64_t rows, int block, int per_block) {
-  const int64_t sms = sm_count() > 0 ? sm_count() : 1;
-  const int64_t most = sms * (block <= 256 ? 4 : block <= 512 ? 2 : 1);
-  const int64_t need = (rows + per_block - 1) / per_block;
-  return need < most ? need : most;
-}
+// The backward pass's blocks: at most four on an SM, so that their sums stay few.
+constexpr int kBackwardBlocks = 4;
 
 int64_t norm_backward_workspace(int64_t rows, int cols) {
-  const int64_t sms = sm_count() > 0 ? sm_count() : 1;
-  const int64_t blocks = rows < 4 * sms ? rows : 4 * sms;  // the most that any layout takes
-  return blocks * cols * (int64_t)sizeof(float);
+  const int64_t most = kBackwardBlocks * (int64_t)(sm_count() > 0 ? sm_count() : 1);
+  return (rows < most ? rows : most) * cols * (int64_t)sizeof(float);
 }
 
-template <typename T, int V>
+template <typename T, typename W, int V>
 static cudaError_t backward_v(const NormArgs& a, const void* dy, const void* ds, void* dx, void* dw,
                               float* part, cudaStream_t s) {
-  const int64_t units = a.cols / V;
-  const int g = norm_threads(units, V > 1 ? 2 : 4, 8);
-  const int block = g <= 32 ? 128 : g;
-  const int per_block = block / g;
-  const int64_t blocks = backward_blocks(a.rows, block, per_block);
-  const int need = (int)((units + g - 1) / g);
-  const size_t smem = per_block > 1 ? (size_t)per_block * a.cols * sizeof(float) : 0;
-  auto go = [&](auto* kern) {
-    return launch_pdl(kern, dim3((unsigned)blocks), dim3(block), smem, s, a, g,
-                      static_cast<const T*>(dy), static_cast<const T*>(ds), static_cast<T*>(dx),
-                      dw ? part : nullptr);
-  };
+  constexpr int NU = V > 2 ? 2 : 8;
+  const int64_t units = V == 2 ? a.cols / 2 + 1 : a.cols / V;
+  const int64_t sms = sm_count() > 0 ? sm_count() : 1;
+  auto* up = static_cast<const T*>(dy);
+  auto* side = static_cast<const T*>(ds);
+  auto* out = static_cast<T*>(dx);
+  float* sums = dw ? part : nullptr;
+  unsigned blocks;
   cudaError_t e;
-  if (need <= 1)
-    e = go(rms_norm_backward_kernel<T, V, 1>);
-  else if (V > 1 && need <= 2)
-    e = go(rms_norm_backward_kernel<T, V, 2>);
-  else if (V == 1 && need <= 4)
-    e = go(rms_norm_backward_kernel<T, V, (V > 1 ? 1 : 4)>);
-  else if (V == 1 && need <= 8)
-    e = go(rms_norm_backward_kernel<T, V, (V > 1 ? 1 : 8)>);
-  else
-    e = go(rms_norm_backward_kernel<T, V, 0>);
+  if (units > 1024 * NU) {
+    blocks = (unsigned)(a.rows < sms ? a.rows : sms);
+    e = launch_pdl(rms_norm_backward_long_kernel<T, V == 2 ? 1 : V>, dim3(blocks), dim3(1024), 0, s, a, up, side,
+                   out, sums);
+  } else {
+    const int g = norm_threads(units, NU, 8);
+    const int block = g <= 32 ? 128 : g;
+    const int per_block = block / g;
+    const size_t smem = per_block > 1 ? (size_t)per_block * a.cols * sizeof(float) : 0;
+    const int64_t need = (a.rows + per_block - 1) / per_block;
+    auto go = [&](auto* kern) {
+      blocks = stay_grid(reinterpret_cast<const void*>(kern), block, smem,
+                         need < kBackwardBlocks * sms ? need : kBackwardBlocks * sms);
+      return launch_pdl(kern, dim3(blocks), dim3(block), smem, s, a, g, up, side, out, sums);
+    };
+    e = block <= 256   ? go(rms_norm_backward_kernel<T, W, V, NU, 256>)
+        : block <= 512 ? go(rms_norm_backward_kernel<T, W, V, NU, 512>)
+                       : go(rms_norm_backward_kernel<T, W, V, NU, 1024>);
+  }
   if (e != cudaSuccess || !dw) return e;
   const dim3 grid((unsigned)((a.cols + 31) / 32));
-  if (a.weight_f32)
-    return launch_pdl(rms_norm_join_kernel<float>, grid, dim3(512), 0, s,
-                      static_cast<const float*>(part), (int)blocks, a.cols, static_cast<float*>(dw));
-  return launch_pdl(rms_norm_join_kernel<T>, grid, dim3(512), 0, s, static_cast<const float*>(part),
-                    (int)blocks, a.cols, static_cast<T*>(dw));
+  return launch_pdl(rms_norm_join_kernel<W>, grid, dim3(512), 0, s, static_cast<const float*>(part),
+                    (int)blocks, a.cols, static_cast<W*>(dw));
 }
 
 template <typename T>
 static cudaError_t backward_t(const NormArgs& a, const void* dy, const void* ds, void* dx, void* dw,
                               float* part, cudaStream_t s) {
-  return norm_vectors<T>(a) && norm_aligned(dy) && norm_aligned(ds) && norm_aligned(dx)
-             ? backward_v<T, 16 / sizeof(T)>(a, dy, ds, dx, dw, part, s)
-             : backward_v<T, 1>(a, dy, ds, dx, dw, part, s);
+  return norm_dispatch<T>(a, norm_unit<T>(a, dy, ds, dx), [&](auto w, auto v) {
+    return backward_v<T, decltype(w), decltype(v)::value>(a, dy, ds, dx, dw, part, s);
+  });
 }
 
 cudaError_t launch_rms_norm_backward(const NormArgs& a, const void* dy, const void* ds, void* dx,

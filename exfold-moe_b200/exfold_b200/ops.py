@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import math
 
 import torch
 from torch.autograd import forward_ad
@@ -643,14 +644,13 @@ def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
     return t.contiguous()
 
 
-def _norm_in(name, x, weight, eps, residual):
-    """The checked inputs as (x rows, residual rows or None, weight)."""
+def _norm_checks(name, x, weight, eps, residual):
     _require_cuda(x, weight, residual)
     if x.dtype not in _WDT:
         raise TypeError(f"{name} needs a float32, bfloat16 or float16 input")
-    if weight.dtype not in (x.dtype, torch.float32):
+    if weight.dtype is not x.dtype and weight.dtype is not torch.float32:
         raise TypeError(f"{name}: the weight must be float32 or of the input's type")
-    if residual is not None and residual.dtype != x.dtype:
+    if residual is not None and residual.dtype is not x.dtype:
         raise TypeError(f"{name}: the residual must be of the input's type")
     if x.dim() < 1 or weight.dim() != 1 or weight.shape[0] != x.shape[-1] or x.shape[-1] == 0:
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} must be [..., H] and "
@@ -659,63 +659,66 @@ def _norm_in(name, x, weight, eps, residual):
         raise ValueError(f"residual {tuple(residual.shape)} must have x's shape {tuple(x.shape)}")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    cols = x.shape[-1]
-    return (_rows(x, cols), None if residual is None else _rows(residual, cols),
-            weight.contiguous())
 
 
 def _norm_forward(x, residual, weight, eps):
-    """(y, s) of rows; s is x without a residual."""
-    rows, cols = x.shape
-    dev = x.device
-    y = torch.empty(rows, cols, dtype=x.dtype, device=dev)
-    s = x if residual is None else torch.empty_like(y)
-    if rows > 0:
+    """(y, s, x's rows); s is None without a residual."""
+    cols, dev = x.shape[-1], x.device
+    rows = _rows(x, cols)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    s, res, stride = None, None, 0
+    if residual is not None:
+        s, res = torch.empty_like(y), _rows(residual, cols)
+        stride = res.stride(0)
+    weight = weight.contiguous()
+    n = rows.shape[0]
+    if n > 0:
         with _on(dev):
             L.check(L.lib().exf_rms_norm(
-                x.data_ptr(), x.stride(0), _ptr(residual),
-                0 if residual is None else residual.stride(0), weight.data_ptr(), _WDT[x.dtype],
-                _WDT[weight.dtype], rows, cols, eps, s.data_ptr(), y.data_ptr(), _stream(dev)))
-    return y, s
+                rows.data_ptr(), rows.stride(0), _ptr(res), stride, weight.data_ptr(),
+                _WDT[x.dtype], _WDT[weight.dtype], n, cols, eps, _ptr(s), y.data_ptr(),
+                _stream(dev)))
+    return y, s, rows
 
 
 def _norm_backward(ctx, dy, ds):
     x, weight = ctx.saved_tensors
-    rows, cols = x.shape
-    dev, dtype = x.device, x.dtype
+    cols = weight.shape[0]
+    rows, weight = _rows(x, cols), weight.contiguous()
+    dev, dtype, n = x.device, x.dtype, rows.shape[0]
     want_x, want_r, want_w, _ = ctx.needs_input_grad
-    want_x = want_x or want_r
-    dx = torch.empty(rows, cols, dtype=dtype, device=dev) if want_x else None
+    dx = torch.empty(x.shape, dtype=dtype, device=dev) if want_x or want_r else None
     dw = torch.empty_like(weight) if want_w else None
-    if dy is None:  # only s was used
-        dy = torch.zeros(rows, cols, dtype=dtype, device=dev)
-    dy = dy.contiguous()
+    # (of s alone, where y was not used)
+    dy = torch.zeros(x.shape, dtype=dtype, device=dev) if dy is None else dy.contiguous()
     ds = None if ds is None else ds.contiguous()
     lib = L.lib()
     with _on(dev):
         ws = None
-        ws_bytes = lib.exf_rms_norm_backward_workspace_bytes(rows, cols) if want_w else 0
+        ws_bytes = lib.exf_rms_norm_backward_workspace_bytes(n, cols) if want_w else 0
         if ws_bytes > 0:
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         L.check(lib.exf_rms_norm_backward(
-            dy.data_ptr(), _ptr(ds), x.data_ptr(), x.stride(0), weight.data_ptr(), _WDT[dtype],
-            _WDT[weight.dtype], rows, cols, ctx.eps, _ptr(dx), _ptr(dw), _ptr(ws), ws_bytes,
-            _stream(dev)))
+            dy.data_ptr(), _ptr(ds), rows.data_ptr(), rows.stride(0), weight.data_ptr(),
+            _WDT[dtype], _WDT[weight.dtype], n, cols, ctx.eps, _ptr(dx), _ptr(dw), _ptr(ws),
+            ws_bytes, _stream(dev)))
     # (the gradient of the sum is that of both of its terms)
-    return dx if ctx.needs_input_grad[0] else None, dx if want_r else None, dw, None
+    return dx if want_x else None, dx if want_r else None, dw, None
 
 
 _norm_backward_once = torch.autograd.function.once_differentiable(_norm_backward)
 
 
 class _RmsNorm(torch.autograd.Function):
+    # (takes and gives the caller's shapes: a view outside would be another node of the graph)
     @staticmethod
     def forward(ctx, x, residual, weight, eps):
-        y, s = _norm_forward(x, residual, weight, eps)
-        ctx.save_for_backward(s, weight)
+        y, s, rows = _norm_forward(x, residual, weight, eps)
+        copied = rows.data_ptr() != x.data_ptr()
+        ctx.save_for_backward((rows if copied else x) if s is None else s, weight)
         ctx.eps = eps
         ctx.set_materialize_grads(False)
-        return y if residual is None else (y, s)
+        return y if s is None else (y, s)
 
     @staticmethod
     def backward(ctx, dy, ds=None):
@@ -733,18 +736,14 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     x, residual and weight (once, in reverse mode; forward mode is refused); nothing is kept for the
     backward pass but s.
     """
-    rows, res, w = _norm_in("rms_norm", x, weight, eps, residual)
+    _norm_checks("rms_norm", x, weight, eps, residual)
     if _has_tangent(x, weight, *(() if residual is None else (residual,))):
         raise NotImplementedError("rms_norm has no forward-mode derivative")
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                     or (residual is not None and residual.requires_grad)):
-        out = _RmsNorm.apply(rows, res, w, float(eps))
-    else:
-        out = _norm_forward(rows, res, w, float(eps))
-        out = out[0] if residual is None else out
-    if residual is None:
-        return out.view(x.shape)
-    return out[0].view(x.shape), out[1].view(x.shape)
+        return _RmsNorm.apply(x, residual, weight, float(eps))
+    y, s, _ = _norm_forward(x, residual, weight, float(eps))
+    return y if s is None else (y, s)
 
 
 def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -756,27 +755,30 @@ def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     group of 32, 64 or 128 columns, or [..., 1] for the row (group None).  A group's largest value has
     the largest code (448, or 127); the others are rounded to the nearest, ties to even.  Values are
     code * scale (`dequantize_8bit`).  A group with a value that is not finite reads back as NaN.  H up to
-    2^18.  For inference: the result carries no gradient.
+    2^17.  For inference: the result carries no gradient.
     """
-    rows, res, w = _norm_in("rms_norm_8bit", x, weight, eps, residual)
+    _norm_checks("rms_norm_8bit", x, weight, eps, residual)
     if dtype not in _CODE:
         raise TypeError("rms_norm_8bit gives float8_e4m3fn or int8 codes")
     if group not in (None, 32, 64, 128):
         raise ValueError(f"group must be 32, 64, 128 or None (a row), got {group}")
-    n, cols = rows.shape
-    dev = rows.device
+    cols, dev = x.shape[-1], x.device
+    rows, w = _rows(x, cols), weight.contiguous()
     groups = 1 if group is None else -(-cols // group)
-    codes = torch.empty(n, cols, dtype=dtype, device=dev)
-    scales = torch.empty(n, groups, dtype=torch.float32, device=dev)
-    s = None if res is None else torch.empty(n, cols, dtype=x.dtype, device=dev)
+    codes = torch.empty(x.shape, dtype=dtype, device=dev)
+    scales = torch.empty(*x.shape[:-1], groups, dtype=torch.float32, device=dev)
+    s, res, stride = None, None, 0
+    if residual is not None:
+        s, res = torch.empty(x.shape, dtype=x.dtype, device=dev), _rows(residual, cols)
+        stride = res.stride(0)
+    n = rows.shape[0]
     if n > 0:
         with _on(dev):
             L.check(L.lib().exf_rms_norm_8bit(
-                rows.data_ptr(), rows.stride(0), _ptr(res), 0 if res is None else res.stride(0),
-                w.data_ptr(), _WDT[x.dtype], _WDT[w.dtype], n, cols, float(eps), _CODE[dtype],
-                group or 0, _ptr(s), codes.data_ptr(), scales.data_ptr(), _stream(dev)))
-    codes, scales = codes.view(x.shape), scales.view(*x.shape[:-1], groups)
-    return (codes, scales) if s is None else (codes, scales, s.view(x.shape))
+                rows.data_ptr(), rows.stride(0), _ptr(res), stride, w.data_ptr(), _WDT[x.dtype],
+                _WDT[w.dtype], n, cols, float(eps), _CODE[dtype], group or 0, _ptr(s),
+                codes.data_ptr(), scales.data_ptr(), _stream(dev)))
+    return (codes, scales) if s is None else (codes, scales, s)
 
 
 def dequantize_8bit(codes: torch.Tensor, scales: torch.Tensor, group: int | None = 128,
@@ -794,7 +796,7 @@ def dequantize_8bit(codes: torch.Tensor, scales: torch.Tensor, group: int | None
     if cols == 0 or scales.shape != (*codes.shape[:-1], groups):
         raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} must be "
                          "[..., H] and [..., groups]")
-    codes, scales = _aligned(codes, 8), scales.contiguous()
+    codes, scales = _aligned(codes), scales.contiguous()
     out = torch.empty(codes.shape, dtype=dtype, device=dev)
     n = out.numel()
     if n > 0:
@@ -807,34 +809,35 @@ def dequantize_8bit(codes: torch.Tensor, scales: torch.Tensor, group: int | None
 
 # ---- balance loss -------------------------------------------------------------------------------
 def _balance_forward(logits, ids, mask, scoring):
-    groups, tokens, experts = logits.shape
-    top_k = ids.shape[-1]
+    """(loss, counts, valid) of contiguous inputs, in the logits' leading shape."""
+    *lead, tokens, experts = logits.shape
+    groups = math.prod(lead)
     dev = logits.device
-    loss = torch.empty(groups, dtype=torch.float32, device=dev)
-    counts = torch.empty(groups, experts, dtype=torch.int32, device=dev)
-    valid = torch.empty(groups, dtype=torch.int32, device=dev)
+    loss = torch.empty(lead, dtype=torch.float32, device=dev)
+    counts = torch.empty(*lead, experts, dtype=torch.int32, device=dev)
+    valid = torch.empty(lead, dtype=torch.int32, device=dev)
     lib = L.lib()
     with _on(dev):
         ws_bytes = lib.exf_balance_loss_workspace_bytes(groups, tokens, experts)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
         L.check(lib.exf_balance_loss(
             logits.data_ptr(), _WDT[logits.dtype], ids.data_ptr(), _IDT[ids.dtype], _ptr(mask),
-            groups, tokens, experts, top_k, scoring, loss.data_ptr(), counts.data_ptr(),
+            groups, tokens, experts, ids.shape[-1], scoring, loss.data_ptr(), counts.data_ptr(),
             valid.data_ptr(), _ptr(ws), ws_bytes, _stream(dev)))
     return loss, counts, valid
 
 
 def _balance_backward(ctx, dloss, _):
     logits, mask, counts, valid = ctx.saved_tensors
-    groups, tokens, experts = logits.shape
+    *lead, tokens, experts = logits.shape
     dev = logits.device
     dlogits = torch.empty_like(logits)
-    dloss = dloss.float().contiguous()
+    dloss = dloss.contiguous()
     with _on(dev):
         L.check(L.lib().exf_balance_loss_backward(
             dloss.data_ptr(), logits.data_ptr(), _WDT[logits.dtype], _ptr(mask), counts.data_ptr(),
-            valid.data_ptr(), groups, tokens, experts, ctx.top_k, ctx.scoring, dlogits.data_ptr(),
-            _stream(dev)))
+            valid.data_ptr(), math.prod(lead), tokens, experts, ctx.top_k, ctx.scoring,
+            dlogits.data_ptr(), _stream(dev)))
     return dlogits, None, None, None
 
 
@@ -844,6 +847,7 @@ _balance_backward_once = torch.autograd.function.once_differentiable(_balance_ba
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, mask, scoring):
+        logits = logits.contiguous()
         loss, counts, valid = _balance_forward(logits, ids, mask, scoring)
         ctx.save_for_backward(logits, mask, counts, valid)
         ctx.top_k, ctx.scoring = ids.shape[-1], scoring
@@ -884,18 +888,10 @@ def balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor, scoring: str = "s
                          f"{tuple(mask.shape)}")
     if _has_tangent(logits):
         raise NotImplementedError("balance_loss has no forward-mode derivative")
-    *lead, tokens, experts = logits.shape
-    groups = 1
-    for n in lead:
-        groups *= n
-    x = logits.reshape(groups, tokens, experts).contiguous()
     if topk_ids.dtype is not torch.int64:
-        topk_ids = _expert_ids(topk_ids, experts)
-    ids = topk_ids.reshape(groups, tokens, topk_ids.shape[-1]).contiguous()
+        topk_ids = _expert_ids(topk_ids, logits.shape[-1])
+    ids = topk_ids.contiguous()
     m = None if mask is None else mask.contiguous()
-    code = _SCORING[scoring]
     if torch.is_grad_enabled() and logits.requires_grad:
-        loss, counts = _BalanceLoss.apply(x, ids, m, code)
-    else:
-        loss, counts, _ = _balance_forward(x, ids, m, code)
-    return loss.view(lead), counts.view(*lead, experts)
+        return _BalanceLoss.apply(logits, ids, m, _SCORING[scoring])
+    return _balance_forward(logits.contiguous(), ids, m, _SCORING[scoring])[:2]
