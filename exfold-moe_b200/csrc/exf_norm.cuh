@@ -171,16 +171,6 @@ __device__ __forceinline__ float2 row_sum2(float2 v, int g, float2* shared) {
   for (int d = 16; d > 0; d >>= 1) v = add(v, d);
   return v;
 }
-// the largest over `lanes` neighbouring lanes
-template <typename A>
-__device__ __forceinline__ A warp_max(A v, int lanes) {
-  for (int d = lanes / 2; d > 0; d >>= 1) {
-    const A o = __shfl_xor_sync(0xffffffffu, v, d);
-    v = o > v ? o : v;
-  }
-  return v;
-}
-
 // Whether a sum of squares has left the range in which fp32 holds it to its last bits: it overflowed (or
 // holds an infinity or a NaN), or it is so small that its terms were cut off.  Then it is summed again in
 // 64 bits.  (Small sums count only where eps does not hide them.)
@@ -227,86 +217,43 @@ __device__ __forceinline__ float inverse_norm(float q, const NormArgs& a, int g,
 
 // ---- rows in units -----------------------------------------------------------------------------------
 // A row is taken in units of V elements, a unit being one aligned access: 16 bytes where base, stride and
-// length allow it; else 4 bytes (two 16-bit elements, V = 2), rows that begin on an odd element having
-// units that begin one element earlier (shift 1); else one element.  Unit u holds the columns V u - shift
-// + [0, V); those outside the row are zeros, and are not written.
+// length allow it; else 4 bytes (two 16-bit elements, V = 2), else one element.  Units of two: a row that
+// begins on an odd element has its units one element on (shift 1), and a row of odd length leaves one
+// element, its first (shift 1) or last, to thread 0 of the row.  Unit u holds the columns V u + shift +
+// [0, V).  A thread's rows all have one shift: the blocks' stride is even (even_grid).
 template <int V>
-__device__ __forceinline__ int units_of(int cols, int shift) {
-  return V == 2 ? (cols + shift + 1) / 2 : cols / V;
-}
-template <typename T, int V>
-__device__ __forceinline__ void read_unit(Pack<T, V>& k, const T* row, int u, int cols, int shift) {
-  if constexpr (V == 2) {
-    const int c = 2 * u - shift;
-    if (c >= 0 && c + 1 < cols) {
-      k.read(row + c);
-    } else {
-      k.w[0] = c >= 0 ? *reinterpret_cast<const uint16_t*>(row + c) : 0u;
-      if (c + 1 < cols) k.w[0] |= (uint32_t)*reinterpret_cast<const uint16_t*>(row + c + 1) << 16;
-    }
-  } else {
-    k.read(row + u * V);
+struct Units {
+  int count, shift, odd;  // odd: the column of the element left over, or -1
+  __device__ __forceinline__ Units(int64_t row, int cols) {
+    count = cols / V;
+    shift = V == 2 ? (int)row & cols & 1 : 0;
+    odd = V == 2 && (cols & 1) ? (shift ? 0 : cols - 1) : -1;
   }
-}
-template <typename T, int V>
-__device__ __forceinline__ void write_unit(const Pack<T, V>& k, T* row, int u, int cols, int shift) {
-  if constexpr (V == 2) {
-    const int c = 2 * u - shift;
-    if (c >= 0 && c + 1 < cols) {
-      k.write(row + c);
-    } else {
-      if (c >= 0) *reinterpret_cast<uint16_t*>(row + c) = (uint16_t)k.w[0];
-      if (c + 1 < cols) *reinterpret_cast<uint16_t*>(row + c + 1) = (uint16_t)(k.w[0] >> 16);
-    }
-  } else {
-    k.write(row + u * V);
-  }
-}
+  __device__ __forceinline__ int column(int u) const { return u * V + shift; }
+};
 
-// The weights of a thread's units, kept from row to row; V = 2: for both shifts (fp32 ones are read again
-// each time: 32 registers else).
+// A thread's weights, kept from row to row, and the element left over's.
 template <typename W, int V, int NU>
 struct Weights {
-  static constexpr bool kKept = !(V == 2 && sizeof(W) == 4);
-  static constexpr int kShifts = V == 2 && kKept ? 2 : 1;
-  Pack<W, V> w[kShifts][kKept ? NU : 1];
-  __device__ __forceinline__ void init(const void* weight, int t, int g, int cols) {
-    if constexpr (kKept) {
+  Pack<W, V> w[NU];
+  float single;
+  __device__ __forceinline__ void init(const void* weight, int t, int g, const Units<V>& n) {
+    const W* p = static_cast<const W*>(weight);
 #pragma unroll
-      for (int h = 0; h < kShifts; ++h)
-#pragma unroll
-        for (int i = 0; i < NU; ++i) {
-          w[h][i].clear();
-          const int u = t + g * i;
-          if (h == 0) {
-            if (u < units_of<V>(cols, 0))
-              read_unit<W, V>(w[h][i], static_cast<const W*>(weight), u, cols, 0);
-          } else {  // (the weights themselves do not move: columns 2 u - 1 and 2 u, one by one)
-            const uint16_t* p = static_cast<const uint16_t*>(weight) + 2 * u;
-            if (u > 0 && 2 * u - 1 < cols) w[h][i].w[0] = p[-1];
-            if (2 * u < cols) w[h][i].w[0] |= (uint32_t)p[0] << 16;
-          }
+    for (int i = 0; i < NU; ++i) {
+      const int u = t + g * i;
+      w[i].clear();
+      if (u < n.count) {
+        if constexpr (V == 2) {  // (the weights themselves do not move)
+          const float e[2] = {to_f32<W>(p[n.column(u)]), to_f32<W>(p[n.column(u) + 1])};
+          w[i].set(e);
+        } else {
+          w[i].read(p + u * V);
         }
+      }
     }
-  }
-  // those of unit u, the thread's i-th
-  __device__ __forceinline__ Pack<W, V> of(const void* weight, int i, int u, int cols, int shift) {
-    if constexpr (kShifts == 2) {
-      Pack<W, V> k = w[0][i];
-      k.w[0] = shift ? w[kShifts - 1][i].w[0] : k.w[0];
-      return k;
-    } else if constexpr (kKept) {
-      w[0][i].anew();
-      return w[0][i];
-    } else {
-      const W* p = static_cast<const W*>(weight);
-      const int c = 2 * u - shift;
-      Pack<W, V> k;
-      k.clear();
-      if (c >= 0 && c < cols) k.w[0] = *reinterpret_cast<const uint32_t*>(p + c);
-      if (c + 1 < cols) k.w[V - 1] = *reinterpret_cast<const uint32_t*>(p + c + 1);
-      return k;
-    }
+    single = 0.0f;
+    if (V == 2 && n.odd >= 0 && t == 0) single = to_f32<W>(p[n.odd]);
   }
 };
 
@@ -324,6 +271,11 @@ static inline int norm_threads(int64_t units, int per, int least) {
 static inline unsigned stay_grid(const void* kernel, int block, size_t smem, int64_t need) {
   const int64_t most = persistent_grid(kernel, block, smem);
   return (unsigned)(most > 0 && most < need ? most : need);
+}
+
+// The same for rows in units of two: an even stride between a block's rows.
+static inline unsigned even_grid(unsigned grid, int64_t need) {
+  return grid < need && grid > 1 ? grid & ~1u : grid;
 }
 
 // The widest unit that every row of the call allows: 16 bytes, two 16-bit elements (base aligned to 4

@@ -36,29 +36,36 @@ __global__ void __launch_bounds__(THREADS)
   const T* r = static_cast<const T*>(a.residual);
   T* sum = static_cast<T*>(a.sum);
   const int64_t step = (int64_t)gridDim.x * per_block;
-  int64_t row = (int64_t)blockIdx.x * per_block + threadIdx.x / g;
+  const int64_t first = (int64_t)blockIdx.x * per_block;
+  int64_t row = first + threadIdx.x / g;
+  const Units<V> n(row, a.cols);
+  const bool extra = V == 2 && n.odd >= 0 && t == 0;
 
   Pack<T, V> nx[NU], nr[NU], s[NU];
+  float nx1 = 0.0f, nr1 = 0.0f;
   Weights<W, V, NU> w;
-  auto shift_of = [&](int64_t at) { return V == 2 ? (int)at & a.cols & 1 : 0; };
   auto fetch = [&](int64_t at) {
-    const int shift = shift_of(at), units = units_of<V>(a.cols, shift);
+    const T* xr = x + at * a.x_stride + n.shift;
+    const T* rr = r + at * a.r_stride + n.shift;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       const int u = t + g * i;
-      if (u < units && at < a.rows) {
-        read_unit<T, V>(nx[i], x + at * a.x_stride, u, a.cols, shift);
-        if (r) read_unit<T, V>(nr[i], r + at * a.r_stride, u, a.cols, shift);
+      if (u < n.count && at < a.rows) {
+        nx[i].read(xr + u * V);
+        if (r) nr[i].read(rr + u * V);
       } else {
         nx[i].clear();
         nr[i].clear();
       }
     }
+    if (extra && at < a.rows) {
+      nx1 = to_f32<T>(xr[n.odd - n.shift]);
+      if (r) nr1 = to_f32<T>(rr[n.odd - n.shift]);
+    }
   };
   fetch(row);
-  w.init(a.weight, t, g, a.cols);
+  w.init(a.weight, t, g, n);
   // every thread of a block (G <= 32: of a warp) takes as many turns
-  const int64_t first = (int64_t)blockIdx.x * per_block;
   int b = 0;
   for (int64_t base = first; base < a.rows; base += step, row += step, b ^= 1) {
     float q = 0.0f;
@@ -68,33 +75,36 @@ __global__ void __launch_bounds__(THREADS)
 #pragma unroll
       for (int j = 0; j < V; ++j) q = fmaf(s[i].get(j), s[i].get(j), q);
     }
+    const float s1 = r ? to_f32<T>(from_f32<T>(nx1 + nr1)) : nx1;
+    if (V == 2) q = fmaf(s1, s1, q);
     const bool live = row < a.rows;
     const int64_t at = row * a.cols;
-    const int shift = shift_of(row), units = units_of<V>(a.cols, shift);
     fetch(row + step);
     if (r && live) {
+      T* to = sum + at + n.shift;
 #pragma unroll
       for (int i = 0; i < NU; ++i)
-        if (t + g * i < units) write_unit<T, V>(s[i], sum + at, t + g * i, a.cols, shift);
+        if (t + g * i < n.count) s[i].write(to + (t + g * i) * V);
+      if (extra) to[n.odd - n.shift] = from_f32<T>(s1);
     }
     const int64_t mine = live ? row : 0;
     const float v = inverse_norm<T>(q, a, g, t, x + mine * a.x_stride,
-                                       r ? r + mine * a.r_stride : nullptr, part[b], part64);
+                                    r ? r + mine * a.r_stride : nullptr, part[b], part64);
     if (live) {
+      T* to = y + at + n.shift;
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
         const int u = t + g * i;
         s[i].anew();
-        if (u < units) {
-          const Pack<W, V> k = w.of(a.weight, i, u, a.cols, shift);
+        w.w[i].anew();
+        if (u < n.count) {
           float e[V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) e[j] = s[i].get(j) * v * k.get(j);
-          Pack<T, V> o;
-          o.set(e);
-          write_unit<T, V>(o, y + at, u, a.cols, shift);
+          for (int j = 0; j < V; ++j) e[j] = s[i].get(j) * v * w.w[i].get(j);
+          store_pack<T, V>(to + u * V, e);
         }
       }
+      if (extra) to[n.odd - n.shift] = from_f32<T>(s1 * v * w.single);
     }
   }
 }
@@ -135,7 +145,7 @@ __global__ void __launch_bounds__(1024) rms_norm_long_kernel(const NormArgs a, T
 // The same blocks and layout; a thread keeps its columns from row to row and adds dw in registers.  Each
 // block's sums go to part_dw [blocks][cols], and rms_norm_join_kernel adds them in order.
 template <typename T, typename W, int V, int NU, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
     rms_norm_backward_kernel(const NormArgs a, int g, const T* dy, const T* ds, T* dx,
                              float* part_dw) {
   __shared__ float2 part[2][32];
@@ -150,55 +160,66 @@ __global__ void __launch_bounds__(THREADS)
   const int64_t step = (int64_t)gridDim.x * per_block;
   const int64_t first = (int64_t)blockIdx.x * per_block;
   int64_t row = first + sub;
+  const Units<V> n(row, a.cols);
+  const bool extra = V == 2 && n.odd >= 0 && t == 0;
 
   Pack<T, V> nx[NU], ny[NU], nd[NU];
+  float nx1 = 0.0f, ny1 = 0.0f, nd1 = 0.0f;
   Weights<W, V, NU> w;
-  // V = 2: a third sum, so that the column before an odd row's unit has a place of its own
-  constexpr int A = V == 2 ? 3 : V;
-  float acc[NU][A];
-  auto shift_of = [&](int64_t at) { return V == 2 ? (int)at & a.cols & 1 : 0; };
+  float acc[NU][V], acc1 = 0.0f;
   auto fetch = [&](int64_t at) {
-    const int shift = shift_of(at), units = units_of<V>(a.cols, shift);
+    const T* xr = x + at * a.x_stride + n.shift;
+    const T* yr = dy + at * a.cols + n.shift;
+    const T* dr = ds + at * a.cols + n.shift;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       const int u = t + g * i;
-      if (u < units && at < a.rows) {
-        read_unit<T, V>(nx[i], x + at * a.x_stride, u, a.cols, shift);
-        read_unit<T, V>(ny[i], dy + at * a.cols, u, a.cols, shift);
-        if (ds) read_unit<T, V>(nd[i], ds + at * a.cols, u, a.cols, shift);
+      if (u < n.count && at < a.rows) {
+        nx[i].read(xr + u * V);
+        ny[i].read(yr + u * V);
+        if (ds) nd[i].read(dr + u * V);
       } else {
         nx[i].clear();
         ny[i].clear();
         nd[i].clear();
       }
     }
+    if (extra && at < a.rows) {
+      nx1 = to_f32<T>(xr[n.odd - n.shift]);
+      ny1 = to_f32<T>(yr[n.odd - n.shift]);
+      if (ds) nd1 = to_f32<T>(dr[n.odd - n.shift]);
+    }
   };
   // (1024 threads have no registers for the row after this one)
   constexpr bool kAhead = THREADS < 1024;
   if (kAhead) fetch(row);
-  w.init(a.weight, t, g, a.cols);
+  w.init(a.weight, t, g, n);
 #pragma unroll
   for (int i = 0; i < NU; ++i)
 #pragma unroll
-    for (int j = 0; j < A; ++j) acc[i][j] = 0.0f;
+    for (int j = 0; j < V; ++j) acc[i][j] = 0.0f;
   int b = 0;
   for (int64_t base = first; base < a.rows; base += step, row += step, b ^= 1) {
     Pack<T, V> s[NU], d[NU], o[NU];
     float q = 0.0f, c = 0.0f;
     if (!kAhead) fetch(row);
-    const int shift = shift_of(row), units = units_of<V>(a.cols, shift);
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       s[i] = nx[i];
       d[i] = ny[i];
       o[i] = nd[i];
-      const Pack<W, V> k = w.of(a.weight, i, t + g * i, a.cols, shift);
+      w.w[i].anew();
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float e = s[i].get(j);
         q = fmaf(e, e, q);
-        c = fmaf(d[i].get(j) * k.get(j), e, c);
+        c = fmaf(d[i].get(j) * w.w[i].get(j), e, c);
       }
+    }
+    const float s1 = nx1, d1 = ny1, o1 = nd1;
+    if (extra) {
+      q = fmaf(s1, s1, q);
+      c = fmaf(d1 * w.single, s1, c);
     }
     if (kAhead) fetch(row + step);
     const float2 both = row_sum2(make_float2(q, c), g, part[b]);
@@ -210,7 +231,7 @@ __global__ void __launch_bounds__(THREADS)
     if (g > 32 ? again : __any_sync(0xffffffffu, again)) {
       const int64_t mine = row < a.rows ? row : 0;
       const double2 d64 = sums_64<T>(x + mine * a.x_stride, nullptr, dy + mine * a.cols, a.weight,
-                                        std::is_same<W, float>::value, a.cols, t, g);
+                                     std::is_same<W, float>::value, a.cols, t, g);
       const double q64 = row_sum(d64.x, g, part64);
       if (g > 32) __syncthreads();
       const double c64 = row_sum(d64.y, g, part64);
@@ -222,62 +243,44 @@ __global__ void __launch_bounds__(THREADS)
       }
     }
     if (row < a.rows) {
+      T* to = dx + row * a.cols + n.shift;
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
         const int u = t + g * i;
         s[i].anew();
         d[i].anew();
-        const Pack<W, V> f = w.of(a.weight, i, u, a.cols, shift);
+        w.w[i].anew();
         float e[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float hat = s[i].get(j) * v, up = d[i].get(j);
-          if constexpr (V == 2) {  // acc: the columns 2 u - 1, 2 u and 2 u + 1
-            const float add = up * hat;
-            acc[i][j] += shift ? add : 0.0f;
-            acc[i][j + 1] += shift ? 0.0f : add;
-          } else {
-            acc[i][j] = fmaf(up, hat, acc[i][j]);
-          }
-          e[j] = v * fmaf(-hat, k, up * f.get(j));
+          acc[i][j] = fmaf(up, hat, acc[i][j]);
+          e[j] = v * fmaf(-hat, k, up * w.w[i].get(j));
           if (ds) e[j] += o[i].get(j);
         }
-        if (dx && u < units) {
-          Pack<T, V> out;
-          out.set(e);
-          write_unit<T, V>(out, dx + row * a.cols, u, a.cols, shift);
-        }
+        if (dx && u < n.count) store_pack<T, V>(to + u * V, e);
+      }
+      if (extra) {
+        const float hat = s1 * v;
+        acc1 = fmaf(d1, hat, acc1);
+        float e = v * fmaf(-hat, k, d1 * w.single);
+        if (ds) e += o1;
+        if (dx) to[n.odd - n.shift] = from_f32<T>(e);
       }
     }
   }
   if (!part_dw) return;
   float* to = part_dw + (int64_t)blockIdx.x * a.cols;
-  if constexpr (V == 2) {
-    // two threads share a column: one adds after the other; the rows of a block, one after another
-    float* at = per_block > 1 ? sums + sub * a.cols : to;
+  float* mine = per_block > 1 ? sums + sub * a.cols : to;
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      const int c = 2 * (t + g * i);
-      if (c < a.cols) at[c] = acc[i][1];
-      if (c + 1 < a.cols) at[c + 1] = acc[i][2];
-    }
-    __syncthreads();
+  for (int i = 0; i < NU; ++i) {
+    const int u = t + g * i;
+    if (u < n.count) {
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      const int c = 2 * (t + g * i) - 1;
-      if (c > 0 && c < a.cols) at[c] += acc[i][0];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      const int u = t + g * i;
-      if (u < units_of<V>(a.cols, 0)) {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          (per_block > 1 ? sums + sub * a.cols : to)[u * V + j] = acc[i][j];
-      }
+      for (int j = 0; j < V; ++j) mine[n.column(u) + j] = acc[i][j];
     }
   }
+  if (extra) mine[n.odd] = acc1;
   // the block's rows beside one another are added in order
   if (per_block > 1) {
     __syncthreads();
@@ -377,13 +380,14 @@ __global__ void __launch_bounds__(512) rms_norm_join_kernel(const float* part, i
 template <typename T, typename W, int V>
 static cudaError_t forward_v(const NormArgs& a, void* y, cudaStream_t s) {
   constexpr int NU = V > 2 ? 2 : 8;
-  const int64_t units = V == 2 ? a.cols / 2 + 1 : a.cols / V;
+  const int64_t units = a.cols / V > 0 ? a.cols / V : 1;
   auto* out = static_cast<T*>(y);
   if (units > 1024 * NU)
     return launch_pdl(rms_norm_long_kernel<T, V == 2 ? 1 : V>, dim3((unsigned)a.rows), dim3(1024), 0, s, a, out);
   auto go = [&](auto* kern, int g, int block) {
     const int64_t need = (a.rows + block / g - 1) / (block / g);
-    const unsigned grid = stay_grid(reinterpret_cast<const void*>(kern), block, 0, need);
+    const unsigned grid =
+        even_grid(stay_grid(reinterpret_cast<const void*>(kern), block, 0, need), need);
     return launch_pdl(kern, dim3(grid), dim3(block), 0, s, a, g, out);
   };
   // few rows: half as many units a thread, the shorter chain
@@ -418,7 +422,7 @@ template <typename T, typename W, int V>
 static cudaError_t backward_v(const NormArgs& a, const void* dy, const void* ds, void* dx, void* dw,
                               float* part, cudaStream_t s) {
   constexpr int NU = V > 2 ? 2 : 8;
-  const int64_t units = V == 2 ? a.cols / 2 + 1 : a.cols / V;
+  const int64_t units = a.cols / V > 0 ? a.cols / V : 1;
   const int64_t sms = sm_count() > 0 ? sm_count() : 1;
   auto* up = static_cast<const T*>(dy);
   auto* side = static_cast<const T*>(ds);
@@ -439,6 +443,7 @@ static cudaError_t backward_v(const NormArgs& a, const void* dy, const void* ds,
     auto go = [&](auto* kern) {
       blocks = stay_grid(reinterpret_cast<const void*>(kern), block, smem,
                          need < kBackwardBlocks * sms ? need : kBackwardBlocks * sms);
+      blocks = even_grid(blocks, need);
       return launch_pdl(kern, dim3(blocks), dim3(block), smem, s, a, g, up, side, out, sums);
     };
     e = block <= 256   ? go(rms_norm_backward_kernel<T, W, V, NU, 256>)

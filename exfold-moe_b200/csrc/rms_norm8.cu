@@ -18,29 +18,39 @@
 namespace exf {
 
 // ---- the largest product of a group ----------------------------------------------------------------
-// Kept as an integer that compares as the magnitudes do, infinities and NaN above all.  Products of 16-bit
-// values are exact in fp32 (EXACT): the bits.  Others: the rounded product's bits and, below them, what the
-// rounding left, its order made that of unsigned integers.
+// Products of 16-bit values are exact in fp32 (EXACT): the value.  Others: an integer that compares as the
+// magnitudes do, the rounded product's bits and, below them, what the rounding left, its order made that of
+// unsigned integers.  Infinities and NaN come out above all.
 template <bool EXACT>
 struct Top;
 template <>
 struct Top<true> {
-  using Key = uint32_t;
-  static __device__ __forceinline__ Key of(float s, float w) {
-    return __float_as_uint(s * w) & 0x7fffffffu;
+  using Key = float;
+  using Shared = uint32_t;
+  static __device__ __forceinline__ Key of(float s, float w, float p) { return fabsf(p); }
+  static __device__ __forceinline__ Key larger(Key a, Key b) {
+    float c;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+    return c;
   }
-  static __device__ __forceinline__ float rounded(Key k) { return __uint_as_float(k); }
-  static __device__ __forceinline__ double value(Key k) { return (double)__uint_as_float(k); }
+  static __device__ __forceinline__ Shared shared(Key k) { return __float_as_uint(k); }
+  static __device__ __forceinline__ Key back(Shared k) { return __uint_as_float(k); }
+  static __device__ __forceinline__ float rounded(Key k) { return k; }
+  static __device__ __forceinline__ double value(Key k) { return (double)k; }
 };
 template <>
 struct Top<false> {
   using Key = unsigned long long;
-  static __device__ __forceinline__ Key of(float s, float w) {
-    const float a = fabsf(s), b = fabsf(w), p = a * b;
-    const uint32_t rest = __float_as_uint(fmaf(a, b, -p));
+  using Shared = unsigned long long;
+  static __device__ __forceinline__ Key of(float s, float w, float p) {
+    const float a = fabsf(p);
+    const uint32_t rest = __float_as_uint(fmaf(fabsf(s), fabsf(w), -a));
     const uint32_t order = rest ^ ((uint32_t)((int32_t)rest >> 31) | 0x80000000u);
-    return (Key)(__float_as_uint(p) & 0x7fffffffu) << 32 | order;
+    return (Key)__float_as_uint(a) << 32 | order;
   }
+  static __device__ __forceinline__ Key larger(Key a, Key b) { return a > b ? a : b; }
+  static __device__ __forceinline__ Shared shared(Key k) { return k; }
+  static __device__ __forceinline__ Key back(Shared k) { return k; }
   static __device__ __forceinline__ float rounded(Key k) { return __uint_as_float((uint32_t)(k >> 32)); }
   static __device__ __forceinline__ double value(Key k) {
     const uint32_t order = (uint32_t)k;
@@ -48,96 +58,104 @@ struct Top<false> {
     return k ? (double)rounded(k) + (double)__uint_as_float(rest) : 0.0;
   }
 };
+template <bool EXACT>
+__device__ __forceinline__ typename Top<EXACT>::Key top_over(typename Top<EXACT>::Key k, int lanes) {
+  for (int d = lanes / 2; d > 0; d >>= 1)
+    k = Top<EXACT>::larger(k, __shfl_xor_sync(0xffffffffu, k, d));
+  return k;
+}
 
 // ---- codes --------------------------------------------------------------------------------------------
 // A group's factors: quotients p M / top are taken with M / top a little too small and a little too large.
-// Where both give the same code it is the definition's (2^-21 to either side; the rounded top, the division
-// and the product are off by 4 steps of 2^-24 together).  Else, one value in 2^16, and for all values of a
-// group below 2^-100, the quotient is taken in 64 bits, where its distance from a border shows.
+// Where both give the same code it is the definition's (2^-20 to either side; the rounded top, the division
+// (2 units in the last place) and the products are off by 8 steps of 2^-24 together).  Else, one value in
+// 2^15, and for all values of a group whose top is far from 1, the quotient is taken in 64 bits, where its
+// distance from a border shows.
 struct Quantum {
   float low, high, scale;
   bool all;  // in 64 bits
 };
-__device__ __forceinline__ Quantum quantum_of(float top, float v, float most) {
+template <bool INT8>
+__device__ __forceinline__ Quantum quantum_of(float top, float v) {
   Quantum z;
-  const float m = top > 0.0f ? most / top : 0.0f;
-  z.low = m * (1.0f - 0x1p-21f);
-  z.high = m * (1.0f + 0x1p-21f);
-  z.scale = top * v / most;
-  z.all = top < 0x1p-100f && top > 0.0f;
-  if (!(top < __int_as_float(0x7f800000))) {
-    z.low = z.high = 0.0f;
-    z.scale = __int_as_float(0x7fc00000);
-  }
+  const float m = __fdividef(INT8 ? 127.0f : 448.0f, top);
+  z.low = m * (1.0f - 0x1p-20f);
+  z.high = m * (1.0f + 0x1p-20f);
+  z.scale = top * v * (1.0f / (INT8 ? 127.0f : 448.0f));
+  z.all = !(top > 0x1p-100f) || !(top < 0x1p100f);
   return z;
 }
-// the value of the code of p = s w, in 64 bits
-template <bool INT8>
-__device__ __noinline__ float code_64(float s, float w, double top) {
-  const double q = fabs((double)s * (double)w) * (INT8 ? 127.0 : 448.0) / top;
-  double unit = 1.0;
-  if (!INT8) {  // three bits behind the leading one, multiples of 2^-9 below 2^-6
-    int e = (int)((unsigned long long)__double_as_longlong(q) >> 52) - 1023;
-    e = e < -6 ? -6 : e;
-    unit = __longlong_as_double((long long)(e - 3 + 1023) << 52);
-  }
-  return copysignf((float)(rint(q / unit) * unit), s * w);
+// the scale of a group whose top is far from 1: NaN for one that is not finite
+__device__ __forceinline__ float top_scale(float top, const Quantum& z) {
+  return top < __int_as_float(0x7f800000) ? z.scale : __int_as_float(0x7fc00000);
 }
 __device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {  // a in the low byte
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
   return r;
 }
+// the distance of e4m3's values about q: three bits behind the leading one, multiples of 2^-9 below 2^-6
+__device__ __forceinline__ float unit_of(float q) {
+  const uint32_t e = __float_as_uint(q) >> 23;
+  return __uint_as_float(((e < 121u ? 121u : e) - 3u) << 23);
+}
+// The code of one value, in 64 bits, read again from memory; top is its group's.  (Out of line: its
+// registers cost the usual path nothing.)
+template <typename T, typename W, bool INT8>
+__device__ __noinline__ uint8_t code_64(const T* x, const T* r, const W* w, double top) {
+  if (!(top > 0.0) || !(top < 3.4028235677973366e38)) return 0;
+  float s[1];
+  load_sum<T, 1>(x, r, s);
+  const float f = to_f32<W>(*w), m = INT8 ? 127.0f : 448.0f;
+  const double p = fabs((double)s[0] * (double)f) * (double)m;
+  float c;
+  if (top > 0x1p-100 && top < 0x1p100) {
+    // the border beside the quotient, and the side of it on which p lies
+    const float q = __fdividef((float)p, (float)top);
+    float unit = 1.0f;
+    if (!INT8) unit = unit_of(q);
+    const float h = rintf(q / unit - 0.5f);
+    const double side = p - (double)((h + 0.5f) * unit) * top;
+    c = (h + (side > 0.0 || (side == 0.0 && ((int)h & 1)) ? 1.0f : 0.0f)) * unit;
+  } else {
+    const double q = p / top;
+    const double unit = INT8 ? 1.0 : (double)unit_of((float)q);
+    c = (float)(rint(q / unit) * unit);
+  }
+  c = copysignf(c, s[0] * f);
+  return (uint8_t)(INT8 ? (uint32_t)(int)c : e4m3_pair(c, 0.0f));
+}
 // The codes of up to four products, the first in the low byte.  Integers: rounded by adding 1.5 2^23, whose
 // low byte they become.
 template <bool INT8, int N>
-__device__ __forceinline__ uint32_t code_word(const float (&p)[N], float m) {
-  uint32_t b[4] = {0, 0, 0, 0};
+__device__ __forceinline__ uint32_t code_word(const float* p, float m) {
   if (INT8) {
+    uint32_t b[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < N; ++j) b[j] = __float_as_uint(fmaf(p[j], m, 12582912.0f));
-    uint32_t lo = b[0], hi = b[2];
-    if (N > 1) lo = __byte_perm(b[0], b[1], 0x0040);
-    if (N > 2) hi = __byte_perm(b[2], b[3], 0x0040);
-    return N > 2 ? __byte_perm(lo, hi, 0x5410) : N > 1 ? lo & 0xffffu : lo & 0xffu;
+    const uint32_t lo = N > 1 ? __byte_perm(b[0], b[1], 0x0040) : b[0];
+    if (N > 2) return __byte_perm(lo, __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    return N > 1 ? lo & 0xffffu : lo & 0xffu;
   }
-  uint32_t lo = e4m3_pair(p[0] * m, N > 1 ? p[N > 1 ? 1 : 0] * m : 0.0f), hi = 0;
-  if (N > 2) hi = e4m3_pair(p[N > 2 ? 2 : 0] * m, p[N > 2 ? 3 : 0] * m);
-  return lo | hi << 16;
-}
-template <bool INT8, bool EXACT, int N, typename S, typename W>
-__device__ __forceinline__ uint32_t codes_of(S s, W w, const Quantum& z,
-                                             typename Top<EXACT>::Key top) {
-  if (z.scale != z.scale) return 0;
-  float p[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) p[j] = s(j) * w(j);
-  uint32_t low = code_word<INT8, N>(p, z.low);
-  const uint32_t high = code_word<INT8, N>(p, z.high);
-  if (low != high || z.all) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (!z.all && ((low ^ high) >> (8 * j) & 255u) == 0) continue;
-      const float q = code_64<INT8>(s(j), w(j), Top<EXACT>::value(top));
-      const uint32_t c = (INT8 ? (uint32_t)(int)q : e4m3_pair(q, 0.0f)) & 255u;
-      low = (low & ~(255u << (8 * j))) | c << (8 * j);
-    }
-  }
-  return low;
+  if (N == 1) return e4m3_pair(p[0] * m, 0.0f) & 0xffu;
+  uint32_t lo = e4m3_pair(p[0] * m, p[N > 1 ? 1 : 0] * m);
+  if (N > 2) lo |= e4m3_pair(p[N > 2 ? 2 : 0] * m, p[N > 2 ? 3 : 0] * m) << 16;
+  return lo;
 }
 
 // ---- the kernel -----------------------------------------------------------------------------------------
 // Blocks that stay, as rms_norm_kernel's, with at least a warp a row.  The largest products are taken with
 // the loads' results; 32 columns lie on 32 / V neighbouring lanes.  Vectors: a group is 1 to 4 such runs, so
 // its lanes find its largest among them.  Else (V <= 2) a run's largest goes to the group's word in shared
-// memory (three sets of words: one is filled, one read, one zeroed), and where an odd row's units begin one
-// column early, the run's first element goes to its own group.  group 0: the row, reduced beside the sum
-// of squares.
+// memory (three sets of words: one is filled, one read, one zeroed), and where the units lie one column
+// on, the run's last element goes to its own group.  group 0: the row, reduced beside the sum of squares.
 template <typename T, typename W, int V, int NU, int THREADS, bool INT8>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
     rms_norm_8bit_kernel(const NormArgs a, int g, int group, uint8_t* codes, float* scales) {
   constexpr bool EXACT = sizeof(T) == 2 && sizeof(W) == 2;
-  using Key = typename Top<EXACT>::Key;
+  using K = Top<EXACT>;
+  using Key = typename K::Key;
+  using Shared = typename K::Shared;
   constexpr int kRun = 32 / V;
   __shared__ float part[2][32];
   __shared__ double part64[32];
@@ -149,34 +167,42 @@ __global__ void __launch_bounds__(THREADS)
   const int sub = threadIdx.x / g, t = threadIdx.x % g;
   const T* x = static_cast<const T*>(a.x);
   const T* r = static_cast<const T*>(a.residual);
+  const W* weight = static_cast<const W*>(a.weight);
   T* sum = static_cast<T*>(a.sum);
   const int64_t step = (int64_t)gridDim.x * per_block;
   const int64_t first = (int64_t)blockIdx.x * per_block;
   int64_t row = first + sub;
-  const int groups = group ? (a.cols + group - 1) / group : 1;
-  constexpr float kMost = INT8 ? 127.0f : 448.0f;
-  Key* tops = reinterpret_cast<Key*>(words) + (size_t)sub * 3 * groups;
+  const Units<V> n(row, a.cols);
+  const bool extra = V == 2 && n.odd >= 0 && t == 0;
+  const int shift = group == 32 ? 5 : group == 64 ? 6 : 7;  // columns to groups
+  const int groups = group ? (a.cols + group - 1) >> shift : 1;
+  Shared* tops = reinterpret_cast<Shared*>(words) + (size_t)sub * 3 * groups;
   const bool shared_tops = V <= 2 && group != 0;
 
-  Pack<T, V> nx[NU], nr[NU], s[NU];
+  Pack<T, V> nx[NU], nr[NU];
+  float nx1 = 0.0f, nr1 = 0.0f;
   Weights<W, V, NU> w;
-  auto shift_of = [&](int64_t at) { return V == 2 ? (int)at & a.cols & 1 : 0; };
   auto fetch = [&](int64_t at) {
-    const int shift = shift_of(at), units = units_of<V>(a.cols, shift);
+    const T* xr = x + at * a.x_stride + n.shift;
+    const T* rr = r + at * a.r_stride + n.shift;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       const int u = t + g * i;
-      if (u < units && at < a.rows) {
-        read_unit<T, V>(nx[i], x + at * a.x_stride, u, a.cols, shift);
-        if (r) read_unit<T, V>(nr[i], r + at * a.r_stride, u, a.cols, shift);
+      if (u < n.count && at < a.rows) {
+        nx[i].read(xr + u * V);
+        if (r) nr[i].read(rr + u * V);
       } else {
         nx[i].clear();
         nr[i].clear();
       }
     }
+    if (extra && at < a.rows) {
+      nx1 = to_f32<T>(xr[n.odd - n.shift]);
+      if (r) nr1 = to_f32<T>(rr[n.odd - n.shift]);
+    }
   };
   fetch(row);
-  w.init(a.weight, t, g, a.cols);
+  w.init(a.weight, t, g, n);
   if (shared_tops) {
     for (int i = t; i < groups; i += g) tops[i] = 0;
     if (g > 32)
@@ -188,116 +214,149 @@ __global__ void __launch_bounds__(THREADS)
   for (int64_t base = first; base < a.rows; base += step, row += step, b ^= 1) {
     const bool live = row < a.rows;
     const int64_t at = row * a.cols;
-    const int shift = shift_of(row), units = units_of<V>(a.cols, shift);
-    Key* here = tops + set * groups;
+    Shared* here = tops + set * groups;
     set = set == 2 ? 0 : set + 1;
     if (shared_tops)
       for (int i = t; i < groups; i += g) tops[set * groups + i] = 0;
     float q = 0.0f;
-    Key top[NU], all = 0;
+    Key top[NU], all = Key(0);
+    float p[NU][V];
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       const int u = t + g * i;
-      s[i] = r ? rounded_sum<T, V>(nx[i], nr[i]) : nx[i];
-      const Pack<W, V> k = w.of(a.weight, i, u, a.cols, shift);
-      Key one[V], most = 0;
+      const Pack<T, V> s = r ? rounded_sum<T, V>(nx[i], nr[i]) : nx[i];
+      if (r && live && u < n.count) s.write(sum + at + n.column(u));
+      w.w[i].anew();
+      Key most = Key(0), last = Key(0);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        q = fmaf(s[i].get(j), s[i].get(j), q);
-        one[j] = u < units ? Top<EXACT>::of(s[i].get(j), k.get(j)) : 0;
-        if (j > 0 || !shared_tops || !shift || t % kRun != 0)
-          most = one[j] > most ? one[j] : most;
+        const float e = s.get(j);
+        q = fmaf(e, e, q);
+        p[i][j] = e * w.w[i].get(j);
+        last = K::of(e, w.w[i].get(j), p[i][j]);
+        // (a run's last element one column on belongs to the group behind)
+        if (V == 2 && j == 1 && n.shift && t % kRun == kRun - 1) continue;
+        most = K::larger(most, last);
       }
       if (shared_tops) {
-#pragma unroll
-        for (int d = kRun / 2; d > 0; d >>= 1) {
-          const Key o = __shfl_xor_sync(0xffffffffu, most, d);
-          most = o > most ? o : most;
+        most = top_over<EXACT>(most, kRun);
+        const int c = n.column(u);
+        if (u < n.count) {
+          if (t % kRun == 0) atomicMax(here + (c >> shift), K::shared(most));
+          if (V == 2 && n.shift && t % kRun == kRun - 1)
+            atomicMax(here + ((c + 1) >> shift), K::shared(last));
         }
-        if (t % kRun == 0 && u < units) {
-          const int c = u * V;
-          if (c < a.cols) atomicMax(here + c / group, most);
-          if (shift && c > 0) atomicMax(here + (c - 1) / group, one[0]);
-        }
+      } else if (V == 2) {
+        most = K::larger(most, last);
       }
       top[i] = most;
-      all = most > all ? most : all;
+      all = K::larger(all, most);
+    }
+    float p1 = 0.0f;
+    if (extra) {
+      const float s1 = r ? to_f32<T>(from_f32<T>(nx1 + nr1)) : nx1;
+      q = fmaf(s1, s1, q);
+      p1 = s1 * w.single;
+      const Key k = K::of(s1, w.single, p1);
+      all = K::larger(all, k);
+      if (shared_tops) atomicMax(here + (n.odd >> shift), K::shared(k));
+      if (r && live) sum[at + n.odd] = from_f32<T>(s1);
     }
     fetch(row + step);
-    if (r && live) {
-#pragma unroll
-      for (int i = 0; i < NU; ++i)
-        if (t + g * i < units) write_unit<T, V>(s[i], sum + at, t + g * i, a.cols, shift);
-    }
     const int64_t mine = live ? row : 0;
+    const T* xr = x + mine * a.x_stride;
+    const T* rr = r ? r + mine * a.r_stride : nullptr;
     if (group == 0) {
       // (its barrier is the sum's: the partial maxima are written before it and read after it)
-      all = warp_max(all, g < 32 ? g : 32);
+      all = top_over<EXACT>(all, 32);
       if (g > 32 && (threadIdx.x & 31) == 0) part_top[b][threadIdx.x >> 5] = all;
     }
-    const float v = inverse_norm<T>(q, a, g, t, x + mine * a.x_stride,
-                                    r ? r + mine * a.r_stride : nullptr, part[b], part64);
+    const float v = inverse_norm<T>(q, a, g, t, xr, rr, part[b], part64);
     if (group == 0 && g > 32) {
       const int lane = threadIdx.x & 31;
-      all = warp_max(lane < (g >> 5) ? part_top[b][lane] : Key(0), 32);
+      all = top_over<EXACT>(lane < (g >> 5) ? part_top[b][lane] : Key(0), 32);
     }
     if (g <= 32 && shared_tops) __syncwarp();
     float* row_scales = scales + row * groups;
     uint8_t* out = codes + at;
+    Quantum z = quantum_of<INT8>(K::rounded(all), v);  // (of the row; of groups below)
+    if (group == 0 && live && t == 0) row_scales[0] = z.all ? top_scale(K::rounded(all), z) : z.scale;
+    uint32_t doubt = 0;  // elements (the one left over last) whose codes are taken again in 64 bits
+    auto word = [&](const float* e, auto count, int i) {
+      constexpr int N = decltype(count)::value;
+      const uint32_t low = code_word<INT8, N>(e, z.low), other = low ^ code_word<INT8, N>(e, z.high);
+      if (other || z.all) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (z.all || (other >> (8 * j) & 255u)) doubt |= 1u << (i + j);
+      }
+      return low;
+    };
+    using std::integral_constant;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      const int u = t + g * i;
-      s[i].anew();
+      const int u = t + g * i, c = n.column(u);
       if constexpr (V > 2) {
-        Key k = top[i];
-        if (group == 0) {
-          k = all;
-        } else {
-          for (int d = group / V / 2; d > 0; d >>= 1) {
-            const Key o = __shfl_xor_sync(0xffffffffu, k, d);
-            k = o > k ? o : k;
-          }
+        if (group != 0) {
+          top[i] = top_over<EXACT>(top[i], group / V);
+          z = quantum_of<INT8>(K::rounded(top[i]), v);
         }
-        if (u < units && live) {
-          const Quantum z = quantum_of(Top<EXACT>::rounded(k), v, kMost);
-          const Pack<W, V> e = w.of(a.weight, i, u, a.cols, shift);
-          const int c = u * V;
-          if (group == 0 ? c == 0 : c % group == 0) row_scales[group ? c / group : 0] = z.scale;
-          uint32_t word[V / 4];
-#pragma unroll
-          for (int h = 0; h < V / 4; ++h)
-            word[h] = codes_of<INT8, EXACT, 4>([&](int j) { return s[i].get(4 * h + j); },
-                                               [&](int j) { return e.get(4 * h + j); }, z, k);
+        if (u < n.count && live) {
+          if (group != 0 && (c & (group - 1)) == 0)
+            row_scales[c >> shift] = z.all ? top_scale(K::rounded(top[i]), z) : z.scale;
+          const integral_constant<int, 4> four;
           if constexpr (V == 8)
-            *reinterpret_cast<uint2*>(out + c) = make_uint2(word[0], word[V / 4 - 1]);
+            *reinterpret_cast<uint2*>(out + c) =
+                make_uint2(word(p[i], four, i * V), word(p[i] + (V > 4 ? 4 : 0), four, i * V + 4));
           else
-            *reinterpret_cast<uint32_t*>(out + c) = word[0];
+            *reinterpret_cast<uint32_t*>(out + c) = word(p[i], four, i * V);
         }
-      } else if (u < units && live) {
-        const Pack<W, V> e = w.of(a.weight, i, u, a.cols, shift);
-        const int c0 = u * V - shift;
-        uint32_t code[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int c = c0 + j;
-          code[j] = 0;
-          if (c >= 0 && c < a.cols) {
-            const Key k = group == 0 ? all : here[c / group];
-            const Quantum z = quantum_of(Top<EXACT>::rounded(k), v, kMost);
-            if (group == 0 ? c == 0 : c % group == 0) row_scales[group ? c / group : 0] = z.scale;
-            code[j] = codes_of<INT8, EXACT, 1>([&](int) { return s[i].get(j); },
-                                               [&](int) { return e.get(j); }, z, k);
-          }
+      } else if (u < n.count && live) {
+        const integral_constant<int, 1> one;
+        if (group != 0) {
+          const float k = K::rounded(K::back(here[c >> shift]));
+          z = quantum_of<INT8>(k, v);
+          if ((c & (group - 1)) == 0) row_scales[c >> shift] = z.all ? top_scale(k, z) : z.scale;
         }
-        // (an odd row's units begin on even places of the codes too)
-        if (V == 2 && c0 >= 0 && c0 + 1 < a.cols && reinterpret_cast<uintptr_t>(codes) % 2 == 0) {
-          *reinterpret_cast<uint16_t*>(out + c0) = (uint16_t)(code[0] | code[V - 1] << 8);
+        uint32_t code;
+        if (V == 2 && group != 0 && ((c + 1) & (group - 1)) == 0) {  // two groups
+          code = word(p[i], one, i * V);
+          const float k = K::rounded(K::back(here[(c + 1) >> shift]));
+          z = quantum_of<INT8>(k, v);
+          row_scales[(c + 1) >> shift] = z.all ? top_scale(k, z) : z.scale;
+          code |= word(p[i] + (V - 1), one, i * V + V - 1) << 8;
         } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (c0 + j >= 0 && c0 + j < a.cols) out[c0 + j] = (uint8_t)code[j];
+          code = word(p[i], integral_constant<int, V>(), i * V);
+        }
+        if (V == 2 && reinterpret_cast<uintptr_t>(codes) % 2 == 0) {
+          *reinterpret_cast<uint16_t*>(out + c) = (uint16_t)code;
+        } else {
+          out[c] = (uint8_t)code;
+          if (V == 2) out[c + 1] = (uint8_t)(code >> 8);
         }
       }
+    }
+    if (extra && live) {
+      if (group != 0) {
+        const float k = K::rounded(K::back(here[n.odd >> shift]));
+        z = quantum_of<INT8>(k, v);
+        if ((n.odd & (group - 1)) == 0)
+          row_scales[n.odd >> shift] = z.all ? top_scale(k, z) : z.scale;
+      }
+      out[n.odd] = (uint8_t)word(&p1, integral_constant<int, 1>(), NU * V);
+    }
+#pragma unroll 1
+    for (; doubt; doubt &= doubt - 1) {
+      const int j = __ffs(doubt) - 1, i = j / V;
+      const int c = i < NU ? n.column(t + g * i) + j % V : n.odd;
+      Key k = all;
+      if (V > 2 && group != 0) {
+#pragma unroll
+        for (int h = 0; h < NU; ++h) k = h == i ? top[h] : k;
+      } else if (V <= 2 && group != 0) {
+        k = K::back(here[c >> shift]);
+      }
+      out[c] = code_64<T, W, INT8>(xr + c, rr ? rr + c : nullptr, weight + c, K::value(k));
     }
   }
 }
@@ -308,11 +367,12 @@ template <typename T, typename W, bool INT8>
 __global__ void __launch_bounds__(1024)
     rms_norm_8bit_long_kernel(const NormArgs a, int group, uint8_t* codes, float* scales) {
   constexpr bool EXACT = sizeof(T) == 2 && sizeof(W) == 2;
-  using Key = typename Top<EXACT>::Key;
+  using K = Top<EXACT>;
+  using Key = typename K::Key;
   __shared__ float part[32];
   __shared__ double part64[32];
   extern __shared__ unsigned long long words[];
-  Key* tops = reinterpret_cast<Key*>(words);
+  auto* tops = reinterpret_cast<typename K::Shared*>(words);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t row = blockIdx.x;
@@ -323,39 +383,44 @@ __global__ void __launch_bounds__(1024)
   for (int i = threadIdx.x; i < groups; i += 1024) tops[i] = 0;
   __syncthreads();
   float q = 0.0f;
-  Key all = 0;
+  Key all = Key(0);
   for (int c0 = 0; c0 < a.cols; c0 += 1024) {  // a warp's 32 columns lie in one group
     const int c = c0 + threadIdx.x;
-    Key k = 0;
+    Key k = Key(0);
     if (c < a.cols) {
       float s[1];
       load_sum<T, 1>(x + c, r ? r + c : nullptr, s);
       if (r) store_pack<T, 1>(static_cast<T*>(a.sum) + row * a.cols + c, s);
       q = fmaf(s[0], s[0], q);
-      k = Top<EXACT>::of(s[0], to_f32<W>(w[c]));
+      const float e = to_f32<W>(w[c]);
+      k = K::of(s[0], e, s[0] * e);
     }
     if (group) {
-      k = warp_max(k, 32);
-      if ((threadIdx.x & 31) == 0 && c < a.cols) atomicMax(tops + c / group, k);
+      k = top_over<EXACT>(k, 32);
+      if ((threadIdx.x & 31) == 0 && c < a.cols) atomicMax(tops + c / group, K::shared(k));
     } else {
-      all = k > all ? k : all;
+      all = K::larger(all, k);
     }
   }
   if (!group) {
-    all = warp_max(all, 32);
-    if ((threadIdx.x & 31) == 0) atomicMax(tops, all);
+    all = top_over<EXACT>(all, 32);
+    if ((threadIdx.x & 31) == 0) atomicMax(tops, K::shared(all));
   }
   // (behind a barrier of its own: the maxima are complete)
   const float v = inverse_norm<T>(q, a, 1024, threadIdx.x, x, r, part, part64);
   for (int c = threadIdx.x; c < a.cols; c += 1024) {
     float s[1];
     load_sum<T, 1>(x + c, r ? r + c : nullptr, s);
-    const float e = to_f32<W>(w[c]);
-    const Key k = tops[group ? c / group : 0];
-    const Quantum z = quantum_of(Top<EXACT>::rounded(k), v, INT8 ? 127.0f : 448.0f);
-    if (group == 0 ? c == 0 : c % group == 0) scales[row * groups + (group ? c / group : 0)] = z.scale;
-    codes[row * a.cols + c] = (uint8_t)codes_of<INT8, EXACT, 1>(
-        [&](int) { return s[0]; }, [&](int) { return e; }, z, k);
+    const float p = s[0] * to_f32<W>(w[c]);
+    const Key k = K::back(tops[group ? c / group : 0]);
+    const Quantum z = quantum_of<INT8>(K::rounded(k), v);
+    if (group == 0 ? c == 0 : c % group == 0)
+      scales[row * groups + (group ? c / group : 0)] =
+          z.all ? top_scale(K::rounded(k), z) : z.scale;
+    uint32_t code = code_word<INT8, 1>(&p, z.low);
+    if (code != code_word<INT8, 1>(&p, z.high) || z.all)
+      code = code_64<T, W, INT8>(x + c, r ? r + c : nullptr, w + c, K::value(k));
+    codes[row * a.cols + c] = (uint8_t)code;
   }
 }
 
@@ -435,7 +500,7 @@ static cudaError_t quantize_v(const NormArgs& a, int group, uint8_t* codes, floa
                               cudaStream_t s) {
   constexpr int NU = V > 2 ? 2 : 8;
   const size_t key = sizeof(T) == 2 && sizeof(W) == 2 ? 4 : 8;
-  const int64_t units = V == 2 ? a.cols / 2 + 1 : a.cols / V;
+  const int64_t units = a.cols / V > 0 ? a.cols / V : 1;
   const int groups = group ? (a.cols + group - 1) / group : 1;
   if (units > 1024 * NU)
     return launch_pdl(rms_norm_8bit_long_kernel<T, W, INT8>, dim3((unsigned)a.rows), dim3(1024),
@@ -445,8 +510,9 @@ static cudaError_t quantize_v(const NormArgs& a, int group, uint8_t* codes, floa
   const int per_block = block / g;
   const size_t smem = V <= 2 && group ? per_block * 3 * groups * key : 0;
   auto go = [&](auto* kern) {
-    const unsigned grid = stay_grid(reinterpret_cast<const void*>(kern), block, smem,
-                                    (a.rows + per_block - 1) / per_block);
+    const int64_t need = (a.rows + per_block - 1) / per_block;
+    const unsigned grid =
+        even_grid(stay_grid(reinterpret_cast<const void*>(kern), block, smem, need), need);
     return launch_pdl(kern, dim3(grid), dim3(block), smem, s, a, g, group, codes, scales);
   };
   if (block <= 256) return go(rms_norm_8bit_kernel<T, W, V, NU, 256, INT8>);
