@@ -66,29 +66,29 @@ __device__ __forceinline__ void scores(float (&x)[C], float (&slope)[SLOPE ? C :
 
 // A lane's columns: unit u = lane + lanes * i of V columns each.
 template <typename T, int V, int NV>
-__device__ __forceinline__ void load_logits(const T* row, int l, int lanes, int units, bool there,
-                                            float (&x)[NV * V]) {
+__device__ __forceinline__ void fetch_logits(const T* row, int l, int lanes, int units, bool there,
+                                             Pack<T, V> (&k)[NV]) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int u = l + lanes * i;
-    float e[V];
-    if (there && u < units) {
-      load_pack<T, V>(row + u * V, e);
-    } else {
+  for (int i = 0; i < NV; ++i)
+    if (there && l + lanes * i < units) k[i].read(row + (l + lanes * i) * V);
+}
+template <typename T, int V, int NV>
+__device__ __forceinline__ void take_logits(const Pack<T, V> (&k)[NV], int l, int lanes, int units,
+                                            bool there, float (&x)[NV * V]) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) e[j] = -__int_as_float(0x7f800000);
-    }
+  for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < V; ++j) x[i * V + j] = e[j];
-  }
+    for (int j = 0; j < V; ++j)
+      x[i * V + j] =
+          there && l + lanes * i < units ? k[i].get(j) : -__int_as_float(0x7f800000);
 }
 
 // Block b of a group takes tokens [T b / blocks, T (b + 1) / blocks): its sums of p, counts and number of
 // tokens.
 template <typename T, int V, int NV, bool SIGMOID>
-__global__ void __launch_bounds__(kBalanceThreads)
+__global__ void __launch_bounds__(kBalanceThreads, NV * V <= 16 ? 4 : 2)
     balance_sums_kernel(const BalanceArgs a, const void* ids, bool ids64, int lanes, float* psum,
-                        int32_t* pcount, int32_t* pvalid) {
+                        int32_t* pcount, int32_t* pvalid, int32_t* ticket) {
   extern __shared__ float shared[];  // [warps][experts] sums, [experts] counts
   constexpr int kWarps = kBalanceThreads / 32;
   const int e = a.experts, units = e / V;
@@ -107,15 +107,21 @@ __global__ void __launch_bounds__(kBalanceThreads)
   const T* logits = static_cast<const T*>(a.logits) + (int64_t)group * a.tokens * e;
   float acc[NV * V] = {};
   int mine = 0;
-  for (int64_t base = t0 + (threadIdx.x >> 5) * per_warp; base < t1; base += kWarps * per_warp) {
-    const int64_t t = base + lane / lanes;
-    const bool there = t < t1 && !(mask && !mask[t]);
+  Pack<T, V> next[NV];
+  const int64_t first = t0 + (threadIdx.x >> 5) * per_warp + lane / lanes, step = kWarps * per_warp;
+  auto kept = [&](int64_t t) { return t < t1 && !(mask && !mask[t]); };
+  bool there = kept(first);
+  fetch_logits<T, V, NV>(logits + first * e, l, lanes, units, there, next);
+  for (int64_t t = first; t - lane / lanes < t1; t += step) {
     float x[NV * V], none[1];
-    load_logits<T, V, NV>(logits + (there ? t : t0) * e, l, lanes, units, there, x);
+    take_logits<T, V, NV>(next, l, lanes, units, there, x);
+    mine += there && l == 0;
+    // the next token's logits are on their way during this one's sums
+    there = kept(t + step);
+    fetch_logits<T, V, NV>(logits + (t + step) * e, l, lanes, units, there, next);
     scores<NV * V, SIGMOID, false>(x, none, lanes);
 #pragma unroll
     for (int j = 0; j < NV * V; ++j) acc[j] += x[j];
-    mine += there && l == 0;
   }
   // the lanes of a warp that share columns, then the warps
 #pragma unroll
@@ -145,60 +151,77 @@ __global__ void __launch_bounds__(kBalanceThreads)
     psum[slot * e + c] = s;
     pcount[slot * e + c] = count[c];
   }
-  if (threadIdx.x == 0) pvalid[slot] = valid;
+  if (threadIdx.x == 0) {
+    pvalid[slot] = valid;
+    if (blockIdx.x == 0) ticket[group] = 0;
+  }
 }
 
-// A block a group joins its blocks' sums: 64 columns at a time, 16 threads a column.
-__global__ void __launch_bounds__(1024)
+// The joined sums: a block takes 8 experts of a group (a sector of each block's sums), 32 threads an expert;
+// the last block of a group to finish adds the experts' products c_e P_e, in order.
+__global__ void __launch_bounds__(256)
     balance_join_kernel(const float* psum, const int32_t* pcount, const int32_t* pvalid, int blocks,
-                        int experts, int top_k, float* loss, int32_t* counts, int32_t* valid) {
-  __shared__ double sums[16][64];
-  __shared__ int32_t routes[16][64];
+                        int experts, int top_k, double* product, int32_t* ticket, float* loss,
+                        int32_t* counts, int32_t* valid) {
+  __shared__ double sums[8][8];
+  __shared__ int32_t routes[8][8];
   __shared__ int tokens;
+  __shared__ bool last;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (threadIdx.x == 0) tokens = 0;
-  __syncthreads();
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t base = (int64_t)blockIdx.x * blocks;
-  int n = 0;
-  for (int b = threadIdx.x; b < blocks; b += 1024) n += pvalid[base + b];
-  if (n) atomicAdd(&tokens, n);
-  const int x = threadIdx.x & 63, j = threadIdx.x >> 6;
-  double total = 0.0;
-  for (int c0 = 0; c0 < experts; c0 += 64) {
-    const int c = c0 + x;
-    double s = 0.0;
-    int32_t r = 0;
-    if (c < experts) {
+  const int group = blockIdx.y;
+  const int64_t base = (int64_t)group * blocks;
+  const int x = threadIdx.x & 7, c = blockIdx.x * 8 + x;
+  double s = 0.0;
+  int32_t r = 0;
+  if (c < experts) {
 #pragma unroll 8
-      for (int b = j; b < blocks; b += 16) {
-        s += (double)__ldcg(psum + (base + b) * experts + c);
-        r += __ldcg(pcount + (base + b) * experts + c);
-      }
+    for (int b = threadIdx.x >> 3; b < blocks; b += 32) {
+      s += (double)__ldcg(psum + (base + b) * experts + c);
+      r += __ldcg(pcount + (base + b) * experts + c);
     }
-    __syncthreads();
-    sums[j][x] = s;
-    routes[j][x] = r;
-    __syncthreads();
-    if (j == 0 && c < experts) {
+  }
 #pragma unroll
-      for (int i = 1; i < 16; ++i) {
-        s += sums[i][x];
-        r += routes[i][x];
-      }
-      counts[(int64_t)blockIdx.x * experts + c] = r;
-      total += s * (double)r;
+  for (int d = 8; d < 32; d <<= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, d);
+    r += __shfl_xor_sync(0xffffffffu, r, d);
+  }
+  if ((threadIdx.x & 31) < 8) {
+    sums[threadIdx.x >> 5][x] = s;
+    routes[threadIdx.x >> 5][x] = r;
+  }
+  __syncthreads();
+  if (threadIdx.x < 8) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      s += sums[i][x];
+      r += routes[i][x];
+    }
+    if (c < experts) counts[(int64_t)group * experts + c] = r;
+    double total = c < experts ? s * (double)r : 0.0;
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) total += __shfl_xor_sync(0xffu, total, d);
+    if (x == 0) {
+      product[(int64_t)group * gridDim.x + blockIdx.x] = total;
+      __threadfence();
+      last = atomicAdd(ticket + group, 1) == (int)gridDim.x - 1;
+      tokens = 0;
     }
   }
   __syncthreads();
-  if (j == 0) sums[0][x] = total;
+  if (!last) return;
+  int n = 0;
+  for (int b = threadIdx.x; b < blocks; b += 256) n += __ldcg(pvalid + base + b);
+  if (n) atomicAdd(&tokens, n);
   __syncthreads();
   if (threadIdx.x == 0) {
-    double s = 0.0;
-    for (int i = 0; i < 64; ++i) s += sums[0][i];
+    __threadfence();
+    double total = 0.0;
+    for (int i = 0; i < gridDim.x; ++i)
+      total += __ldcg(product + (int64_t)group * gridDim.x + i);
     const double t = (double)tokens;
-    loss[blockIdx.x] = tokens ? (float)(s * experts / ((double)top_k * t * t)) : 0.0f;
-    valid[blockIdx.x] = tokens;
+    loss[group] = tokens ? (float)(total * experts / ((double)top_k * t * t)) : 0.0f;
+    valid[group] = tokens;
   }
 }
 
@@ -228,8 +251,10 @@ __global__ void __launch_bounds__(kBalanceThreads)
     const int64_t t = base + lane / lanes;
     const bool in = t < a.tokens;
     const bool there = in && !(mask && !mask[t]);
+    Pack<T, V> k[NV];
     float x[NV * V], slope[SIGMOID ? NV * V : 1];
-    load_logits<T, V, NV>(logits + (there ? t : 0) * e, l, lanes, units, there, x);
+    fetch_logits<T, V, NV>(logits + t * e, l, lanes, units, there, k);
+    take_logits<T, V, NV>(k, l, lanes, units, there, x);
     scores<NV * V, SIGMOID, SIGMOID>(x, slope, lanes);
     float dot = 0.0f;
 #pragma unroll
@@ -254,16 +279,19 @@ __global__ void __launch_bounds__(kBalanceThreads)
 }
 
 // ---- host side ----------------------------------------------------------------------------------
-// Blocks a group of the forward pass: all groups together two on an SM, at least 8 tokens a warp.
+// Blocks a group of the forward pass: all groups together four on an SM, at least 8 tokens a warp.
 static int64_t balance_blocks(int groups, int64_t tokens) {
   const int64_t sms = sm_count() > 0 ? sm_count() : 1;
-  const int64_t most = (2 * sms + groups - 1) / groups;
+  const int64_t most = (4 * sms + groups - 1) / groups;
   const int64_t need = (tokens + 63) / 64;
   return need < most ? need : most;
 }
+static int join_blocks(int experts) { return (experts + 7) / 8; }
 
+// products, then the blocks' sums, counts and numbers of tokens, then the tickets
 int64_t balance_workspace(int groups, int64_t tokens, int experts) {
-  return groups * balance_blocks(groups, tokens) * (8 * (int64_t)experts + 4);
+  return groups * (8 * (int64_t)join_blocks(experts) + 4 +
+                   balance_blocks(groups, tokens) * (8 * (int64_t)experts + 4));
 }
 
 // f(logits' type, V, NV, sigmoid) of the call's layout: vectors where rows allow them, 16 columns a lane,
@@ -300,24 +328,32 @@ static cudaError_t balance_dispatch(const BalanceArgs& a, const void* out, F f) 
 cudaError_t launch_balance_loss(const BalanceArgs& a, const void* ids, bool ids64, void* workspace,
                                 float* loss, int32_t* counts, int32_t* valid, cudaStream_t s) {
   const int64_t blocks = balance_blocks(a.groups, a.tokens);
-  float* psum = static_cast<float*>(workspace);
+  if (blocks == 0) {  // no tokens
+    cudaError_t e = cudaMemsetAsync(loss, 0, a.groups * sizeof(float), s);
+    if (e == cudaSuccess) e = cudaMemsetAsync(valid, 0, a.groups * sizeof(int32_t), s);
+    if (e == cudaSuccess)
+      e = cudaMemsetAsync(counts, 0, (size_t)a.groups * a.experts * sizeof(int32_t), s);
+    return e;
+  }
+  double* product = static_cast<double*>(workspace);
+  float* psum = reinterpret_cast<float*>(product + (int64_t)a.groups * join_blocks(a.experts));
   int32_t* pcount = reinterpret_cast<int32_t*>(psum + a.groups * blocks * a.experts);
   int32_t* pvalid = pcount + a.groups * blocks * a.experts;
-  cudaError_t err = cudaSuccess;
-  if (blocks > 0)
-    err = balance_dispatch(a, nullptr, [&](auto t, auto v, auto nv, auto sigmoid, int lanes) {
-      return launch_pdl(
-          balance_sums_kernel<decltype(t), decltype(v)::value, decltype(nv)::value,
-                              decltype(sigmoid)::value>,
-          dim3((unsigned)blocks, a.groups), dim3(kBalanceThreads),
-          (kBalanceThreads / 32 + 1) * (size_t)a.experts * 4, s, a, ids, ids64, lanes, psum, pcount,
-          pvalid);
-    });
+  int32_t* ticket = pvalid + a.groups * blocks;
+  const cudaError_t err =
+      balance_dispatch(a, nullptr, [&](auto t, auto v, auto nv, auto sigmoid, int lanes) {
+        return launch_pdl(
+            balance_sums_kernel<decltype(t), decltype(v)::value, decltype(nv)::value,
+                                decltype(sigmoid)::value>,
+            dim3((unsigned)blocks, a.groups), dim3(kBalanceThreads),
+            (kBalanceThreads / 32 + 1) * (size_t)a.experts * 4, s, a, ids, ids64, lanes, psum, pcount,
+            pvalid, ticket);
+      });
   if (err != cudaSuccess) return err;
-  return launch_pdl(balance_join_kernel, dim3(a.groups), dim3(1024), 0, s,
+  return launch_pdl(balance_join_kernel, dim3(join_blocks(a.experts), a.groups), dim3(256), 0, s,
                     static_cast<const float*>(psum), static_cast<const int32_t*>(pcount),
-                    static_cast<const int32_t*>(pvalid), (int)blocks, a.experts, a.top_k, loss,
-                    counts, valid);
+                    static_cast<const int32_t*>(pvalid), (int)blocks, a.experts, a.top_k, product,
+                    ticket, loss, counts, valid);
 }
 
 cudaError_t launch_balance_loss_backward(const BalanceArgs& a, const float* dloss,

@@ -817,7 +817,7 @@ EXF_API int exf_balance_loss(const void* logits, int dtype, const void* ids, int
   if (groups == 0) return EXF_OK;
   EXF_REQUIRE(loss && counts && valid, "%s: null pointer", name);
   EXF_REQUIRE(tokens == 0 || (logits && ids && workspace), "%s: null pointer", name);
-  EXF_REQUIRE(aligned_to(logits, dtype) && aligned_to(workspace, EXF_F32) &&
+  EXF_REQUIRE(aligned_to(logits, dtype) && reinterpret_cast<uintptr_t>(workspace) % 8 == 0 &&
                   reinterpret_cast<uintptr_t>(ids) % (id_dtype == EXF_I64 ? 8 : 4) == 0,
               "%s: a tensor is not aligned to its type", name);
   const int64_t need = balance_workspace(groups, tokens, experts);

@@ -354,24 +354,27 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// dw [cols] from the blocks' sums: 32 columns a block, 16 threads a column.
+// dw [cols] from the blocks' sums: 8 columns (a sector of each row) a block, 64 threads a column, so that
+// short rows fill the card too.
 template <typename W>
 __global__ void __launch_bounds__(512) rms_norm_join_kernel(const float* part, int blocks, int cols,
                                                             W* dw) {
-  __shared__ float sums[16][33];
+  __shared__ float sums[16][8];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), j = threadIdx.x >> 5;
+  const int x = threadIdx.x & 7, c = blockIdx.x * 8 + x;
   float e = 0.0f;
   if (c < cols) {
 #pragma unroll 8
-    for (int b = j; b < blocks; b += 16) e += __ldcg(part + (int64_t)b * cols + c);
+    for (int b = threadIdx.x >> 3; b < blocks; b += 64) e += __ldcg(part + (int64_t)b * cols + c);
   }
-  sums[j][threadIdx.x & 31] = e;
+  e += __shfl_xor_sync(0xffffffffu, e, 8);
+  e += __shfl_xor_sync(0xffffffffu, e, 16);
+  if ((threadIdx.x & 31) < 8) sums[threadIdx.x >> 5][x] = e;
   __syncthreads();
-  if (j == 0 && c < cols) {
+  if (threadIdx.x < 8 && c < cols) {
 #pragma unroll
-    for (int i = 1; i < 16; ++i) e += sums[i][threadIdx.x];
+    for (int i = 1; i < 16; ++i) e += sums[i][x];
     dw[c] = from_f32<W>(e);
   }
 }
@@ -410,11 +413,13 @@ cudaError_t launch_rms_norm(const NormArgs& a, void* y, cudaStream_t s) {
   return forward_t<__half>(a, y, s);
 }
 
-// The backward pass's blocks: at most four on an SM, so that their sums stay few.
-constexpr int kBackwardBlocks = 4;
+// The backward pass's blocks: few on an SM, so that their sums stay few; more where the blocks are small.
+static int64_t backward_blocks(int cols) {
+  return (cols <= 1024 ? 8 : 4) * (int64_t)(sm_count() > 0 ? sm_count() : 1);
+}
 
 int64_t norm_backward_workspace(int64_t rows, int cols) {
-  const int64_t most = kBackwardBlocks * (int64_t)(sm_count() > 0 ? sm_count() : 1);
+  const int64_t most = backward_blocks(cols);
   return (rows < most ? rows : most) * cols * (int64_t)sizeof(float);
 }
 
@@ -441,8 +446,9 @@ static cudaError_t backward_v(const NormArgs& a, const void* dy, const void* ds,
     const size_t smem = per_block > 1 ? (size_t)per_block * a.cols * sizeof(float) : 0;
     const int64_t need = (a.rows + per_block - 1) / per_block;
     auto go = [&](auto* kern) {
+      const int64_t most = backward_blocks(a.cols);
       blocks = stay_grid(reinterpret_cast<const void*>(kern), block, smem,
-                         need < kBackwardBlocks * sms ? need : kBackwardBlocks * sms);
+                         need < most ? need : most);
       blocks = even_grid(blocks, need);
       return launch_pdl(kern, dim3(blocks), dim3(block), smem, s, a, g, up, side, out, sums);
     };
@@ -451,7 +457,7 @@ static cudaError_t backward_v(const NormArgs& a, const void* dy, const void* ds,
                        : go(rms_norm_backward_kernel<T, W, V, NU, 1024>);
   }
   if (e != cudaSuccess || !dw) return e;
-  const dim3 grid((unsigned)((a.cols + 31) / 32));
+  const dim3 grid((unsigned)((a.cols + 7) / 8));
   return launch_pdl(rms_norm_join_kernel<W>, grid, dim3(512), 0, s, static_cast<const float*>(part),
                     (int)blocks, a.cols, static_cast<W*>(dw));
 }

