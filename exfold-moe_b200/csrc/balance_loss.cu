@@ -51,8 +51,9 @@ __device__ __forceinline__ void scores(float (&x)[C], float (&slope)[SLOPE ? C :
     if (SIGMOID) {
       const float e = exp_near(soft ? x[j] - shift : -fabsf(x[j]));
       const bool high = x[j] >= 0.0f;
-      if (SLOPE) slope[j] = soft ? 1.0f : (high ? e : 1.0f) / (1.0f + e);
-      x[j] = soft ? e : (high ? 1.0f : e) / (1.0f + e);
+      const float r = __fdividef(1.0f, 1.0f + e);
+      if (SLOPE) slope[j] = soft ? 1.0f : high ? e * r : r;
+      x[j] = soft ? e : high ? r : e * r;
     } else {
       x[j] = exp_near(x[j] - shift);
     }

@@ -8,6 +8,7 @@
 #include <mutex>
 #include <tuple>
 
+#include "exf_adapters.h"
 #include "exf_balance.h"
 #include "exf_common.cuh"
 #include "exf_gated.h"
@@ -843,6 +844,52 @@ EXF_API int exf_balance_loss_backward(const float* dloss, const void* logits, in
   BalanceArgs a{logits, dtype, mask, groups, tokens, experts, top_k, scoring == EXF_SIGMOID};
   return cuda_status(
       launch_balance_loss_backward(a, dloss, counts, valid, dlogits, (cudaStream_t)stream), name);
+}
+
+// ---- projection with adapters ----------------------------------------------------------------------
+static bool adapted_too_large(int64_t tokens, int64_t inner, int64_t outer, int64_t adapters) {
+  return tokens >= (1 << 24) || inner >= (1 << 23) || outer >= (1 << 23) ||
+         adapters >= (1 << 24) ||
+         ((tokens + 127) / 128) * ((outer + 63) / 64) >= ((int64_t)1 << 31);
+}
+
+EXF_API int64_t exf_adapted_linear_workspace_bytes(int64_t tokens, int inner, int outer, int rank) {
+  if (tokens < 0 || inner < 1 || outer < 1 || rank < 1 || rank > 128 ||
+      adapted_too_large(tokens, inner, outer, 0))
+    return -1;
+  return adapters_workspace(tokens, inner, outer, rank);
+}
+
+EXF_API int exf_adapted_linear(const void* x, const void* w, const void* a, const void* b,
+                               const int32_t* ids, const float* scaling, int dtype, int64_t tokens,
+                               int inner, int outer, int adapters, int rank, void* y,
+                               void* workspace, int64_t workspace_bytes, int32_t* status,
+                               exf_stream_t stream) {
+  const char* name = "exf_adapted_linear";
+  if (dtype != EXF_BF16 && dtype != EXF_F16)
+    return fail(EXF_ERR_UNSUPPORTED, "%s: dtype must be EXF_BF16 or EXF_F16", name);
+  EXF_REQUIRE(tokens >= 0 && inner >= 1 && outer >= 1 && adapters >= 0 && rank >= 1,
+              "%s: bad shape", name);
+  if (inner % 8 != 0 || outer % 8 != 0 || rank % 8 != 0)
+    return fail(EXF_ERR_UNSUPPORTED, "%s: inner, outer and rank must be multiples of 8", name);
+  if (rank > 128) return fail(EXF_ERR_UNSUPPORTED, "%s: rank must be at most 128", name);
+  if (adapted_too_large(tokens, inner, outer, adapters))
+    return fail(EXF_ERR_UNSUPPORTED, "%s: shape too large", name);
+  if (tokens == 0) return EXF_OK;
+  EXF_REQUIRE(x && w && ids && y && workspace && (adapters == 0 || (a && b)), "%s: null pointer",
+              name);
+  EXF_REQUIRE(aligned16(x) && aligned16(w) && aligned16(a) && aligned16(b) && aligned16(y),
+              "%s: tensors must be 16-byte aligned", name);
+  EXF_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 32 == 0,
+              "%s: the workspace must be 32-byte aligned", name);
+  EXF_REQUIRE(reinterpret_cast<uintptr_t>(ids) % 4 == 0 && aligned_to(scaling, EXF_F32),
+              "%s: a tensor is not aligned to its type", name);
+  const int64_t need = adapters_workspace(tokens, inner, outer, rank);
+  EXF_REQUIRE(workspace_bytes >= need, "%s: workspace of %lld bytes required", name,
+              (long long)need);
+  AdapterArgs p{x,     w,     a,     b,        ids,  scaling, dtype == EXF_BF16,
+                tokens, inner, outer, adapters, rank, y,       status};
+  return cuda_status(launch_adapters(p, workspace, (cudaStream_t)stream), name);
 }
 
 // moe_align without any device allocation: the chunk-count table lives in the library's fixed

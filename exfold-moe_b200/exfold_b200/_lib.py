@@ -86,6 +86,9 @@ SIGNATURES = {
                               _vp]),
     "exf_balance_loss_backward": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _i64, _i, _i, _i, _vp,
                                        _vp]),
+    "exf_adapted_linear_workspace_bytes": (_i64, [_i64, _i, _i, _i]),
+    "exf_adapted_linear": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i64, _i, _i, _i, _i, _vp, _vp,
+                                _i64, _vp, _vp]),
 }
 
 _lock = threading.Lock()

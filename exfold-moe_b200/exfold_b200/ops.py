@@ -895,3 +895,50 @@ def balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor, scoring: str = "s
     if torch.is_grad_enabled() and logits.requires_grad:
         return _BalanceLoss.apply(logits, ids, m, _SCORING[scoring])
     return _balance_forward(logits.contiguous(), ids, m, _SCORING[scoring])[:2]
+
+
+# ---- projection with adapters -------------------------------------------------------------------
+def adapted_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+                   adapter_ids: torch.Tensor, scaling: torch.Tensor | None = None,
+                   status: torch.Tensor | None = None) -> torch.Tensor:
+    """y = x W^T + scaling[i] * (x A[i]^T) B[i]^T, i = adapter_ids of the token: a shared projection
+    with the low-rank adapters of many requests.
+
+    x [..., K] and w [N, K] (the shared expert's down projection, or its gate and up rows), a [R, rank, K]
+    and b [R, N, rank], all bf16 or all fp16; y [..., N].  adapter_ids [...] integers of any width, in any
+    order; tokens whose id lies outside [0, R) have no adapter.  scaling fp32 [R], or None for 1.  K, N
+    and rank are multiples of 8, rank at most 128.  Sums are fp32; y is rounded once.  `status` as in
+    `fused_experts`.  For inference: the result carries no gradient.
+    """
+    dev = _require_cuda(x, w, a, b, adapter_ids, scaling, status)
+    dtype = x.dtype
+    if dtype not in (torch.bfloat16, torch.float16) or not (w.dtype is dtype and a.dtype is dtype
+                                                            and b.dtype is dtype):
+        raise TypeError("adapted_linear needs x, w, a and b all bfloat16 or all float16")
+    if (x.dim() < 1 or w.dim() != 2 or a.dim() != 3 or b.dim() != 3 or w.shape[1] != x.shape[-1]
+            or a.shape[2] != w.shape[1] or b.shape != (a.shape[0], w.shape[0], a.shape[1])
+            or w.numel() == 0 or a.shape[1] == 0):
+        raise ValueError(f"x {tuple(x.shape)}, w {tuple(w.shape)}, a {tuple(a.shape)} and b "
+                         f"{tuple(b.shape)} must be [..., K], [N, K], [R, rank, K] and [R, N, rank]")
+    if adapter_ids.shape != x.shape[:-1]:
+        raise ValueError(f"adapter_ids {tuple(adapter_ids.shape)} must have x's leading shape "
+                         f"{tuple(x.shape[:-1])}")
+    if scaling is not None and scaling.shape != a.shape[:1]:
+        raise ValueError(f"scaling {tuple(scaling.shape)} must be [{a.shape[0]}]")
+    outer, inner = w.shape
+    adapters, rank = a.shape[:2]
+    rows, w, a, b = _aligned(x), _aligned(w), _aligned(a), _aligned(b)
+    ids = _expert_ids(adapter_ids, adapters).contiguous()
+    if scaling is not None:
+        scaling = _f32c(scaling)
+    y = torch.empty(*x.shape[:-1], outer, dtype=dtype, device=dev)
+    tokens = ids.numel()
+    lib = L.lib()
+    with _on(dev):
+        ws_bytes = lib.exf_adapted_linear_workspace_bytes(tokens, inner, outer, rank)
+        ws = torch.empty(ws_bytes if ws_bytes > 32 else 32, dtype=torch.uint8, device=dev)
+        L.check(lib.exf_adapted_linear(
+            rows.data_ptr(), w.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(),
+            _ptr(scaling), _WDT[dtype], tokens, inner, outer, adapters, rank, y.data_ptr(),
+            ws.data_ptr(), ws_bytes, _status_ptr(status), _stream(dev)))
+    return y

@@ -1,4 +1,4 @@
-"""Refusals of the norm and balance-loss entry points: bad arguments come back as errors before
+"""Refusals of the norm, balance-loss and adapter entry points: bad arguments come back as errors before
 anything touches the device."""
 
 from __future__ import annotations
@@ -132,3 +132,34 @@ def test_python_entry_points_refuse_cpu_tensors():
         ops.dequantize_8bit(x.to(torch.int8), torch.zeros(2, 1))
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.balance_loss(x, torch.zeros(2, 8, dtype=torch.int32))
+
+
+def adapted(x=FAKE, ids=FAKE, a=FAKE, dt=L.EXF_BF16, tokens=4, inner=64, outer=64, adapters=2, rank=8,
+            ws=FAKE, size=BIG):
+    return call("exf_adapted_linear", x, FAKE, a, FAKE, ids, None, dt, tokens, inner, outer, adapters,
+                rank, FAKE, ws, size, None, None)
+
+
+def test_adapted_linear_refusals():
+    refused(adapted(dt=L.EXF_F32), L.EXF_ERR_UNSUPPORTED, "dtype")
+    refused(adapted(inner=60), L.EXF_ERR_UNSUPPORTED, "multiples of 8")
+    refused(adapted(outer=4), L.EXF_ERR_UNSUPPORTED, "multiples of 8")
+    refused(adapted(rank=12), L.EXF_ERR_UNSUPPORTED, "multiples of 8")
+    refused(adapted(rank=136), L.EXF_ERR_UNSUPPORTED, "rank")
+    refused(adapted(rank=0), L.EXF_ERR_INVALID, "shape")
+    refused(adapted(tokens=-1), L.EXF_ERR_INVALID, "shape")
+    refused(adapted(tokens=1 << 24), L.EXF_ERR_UNSUPPORTED, "large")
+    refused(adapted(inner=1 << 23), L.EXF_ERR_UNSUPPORTED, "large")
+    refused(adapted(x=None), L.EXF_ERR_INVALID, "null")
+    refused(adapted(a=None), L.EXF_ERR_INVALID, "null")
+    refused(adapted(x=ODD), L.EXF_ERR_INVALID, "aligned")
+    refused(adapted(ids=ODD), L.EXF_ERR_INVALID, "aligned")
+    refused(adapted(ws=ctypes.c_void_p(80)), L.EXF_ERR_INVALID, "32-byte")
+    refused(adapted(size=3), L.EXF_ERR_INVALID, "workspace")
+    assert adapted(tokens=0, x=None, ws=None, size=0)[0] == 0
+    ws = L.lib().exf_adapted_linear_workspace_bytes
+    assert ws(4, 64, 64, 8) > 0 and ws(0, 64, 64, 8) == 0
+    assert ws(-1, 64, 64, 8) == -1 and ws(4, 64, 64, 129) == -1 and ws(4, 0, 64, 8) == -1
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.adapted_linear(x, x, x, x, torch.zeros(2, dtype=torch.int32))
