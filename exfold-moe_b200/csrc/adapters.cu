@@ -63,6 +63,17 @@ __device__ __forceinline__ void warp_mma(float (&d)[4], uint32_t a0, uint32_t a1
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// whether one of two 16-bit values is an infinity or a NaN
+template <bool BF16>
+__device__ __forceinline__ bool not_finite2(uint32_t w) {
+  constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+  return (w & kExp) == kExp || (w >> 16 & kExp) == kExp;
+}
+template <bool BF16>
+__device__ __forceinline__ bool not_finite(const uint4& v) {
+  return not_finite2<BF16>(v.x) || not_finite2<BF16>(v.y) || not_finite2<BF16>(v.z) ||
+         not_finite2<BF16>(v.w);
+}
 // 8 columns of 16 bits, or zeros
 __device__ __forceinline__ uint4 load8(const uint16_t* p, bool there) {
   return there ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
@@ -266,6 +277,9 @@ __global__ void __launch_bounds__(256)
 // 32 (64-byte swizzle) of their own, written by four warps while the main stages are multiplied, and are
 // taken in between them, spread over the tile: a sum's order is free, and nothing waits for loads that could
 // have been under way.  (The first tile takes them last: z may still be on its way.)
+// A tile's tokens meet all of its adapters, all but their own times 0, and 0 times an infinity is a NaN.  So
+// eight columns of B with one that is not finite go in as zeros, and the epilogue adds them to their own
+// adapter's tokens: one request's broken adapter does not reach another's.
 template <int NT>
 struct AdaptedCfg {
   static constexpr int kATile = kABM * kABK * 2;
@@ -289,6 +303,7 @@ struct AdaptedSmem {
   alignas(8) uint64_t drain;
   uint32_t tmem_base;
   int failed;
+  int broken[2];  // by accumulator: 1 + the last tile that left columns of B out
 };
 template <int NT>
 constexpr size_t adapted_smem_bytes() { return sizeof(AdaptedSmem<NT>) + 1024; }
@@ -306,6 +321,30 @@ struct AdaptedGemm {
   int m_tiles, n_tiles, kblocks, splits, parts;
   bool wide;  // y's rows are 32-byte aligned
 };
+
+// The columns of B that stages [q0, q1) of M tile mt left out, for 32 of a token's features.
+template <bool BF16>
+__device__ __noinline__ void add_broken(const AdaptedGemm& p, int token, int mt, int col, int q0, int q1,
+                                        float (&v)[32]) {
+  const int slot = p.l.place[token], rank = p.a.rank, width = 2 * rank;
+  if (slot == 255) return;
+  const int id = p.l.list[mt * 128 + slot];
+  for (int r0 = 0; r0 < rank; r0 += 8) {
+    const int q = (slot * width + r0) / 32;  // the stage of their first terms
+    if (q < q0 || q >= q1) continue;
+#pragma unroll 1
+    for (int j = 0; j < 32 && col + j < p.a.outer; ++j) {
+      const uint16_t* b =
+          static_cast<const uint16_t*>(p.a.b) + ((int64_t)id * p.a.outer + col + j) * rank + r0;
+      if (!not_finite<BF16>(load8(b, true))) continue;
+      for (int r = 0; r < 8; ++r) {
+        float z = 0.0f;
+        for (int k = 0; k < p.parts; ++k) z += p.l.z[((int64_t)k * p.a.tokens + token) * rank + r0 + r];
+        v[j] = fmaf(z, unpack2<BF16>(b[r]).x, v[j]);
+      }
+    }
+  }
+}
 
 template <int NT, bool BF16>
 __global__ void __launch_bounds__(kAdaptedThreads, 1)
@@ -334,6 +373,7 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
     }
     mbar_init(&sm.drain, 1);
     sm.failed = 0;
+    sm.broken[0] = sm.broken[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(&sm.tmem_base, C::kTmem);
@@ -463,6 +503,9 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
       fence_after_sync();
       const int row = tl.mt * kABM + q * 32 + lane;
       const uint32_t taddr = tmem + static_cast<uint32_t>(b * NT) + ((uint32_t)(q * 32) << 16);
+      const bool broken = *const_cast<volatile int*>(&sm.broken[b]) == t + 1;
+      int q0 = 0, q1 = 0;
+      extra_of(tl, q0, q1);  // (by whole warps)
 #pragma unroll 1
       for (int c = 0; c < NT; c += 32) {
         float v[32];
@@ -470,6 +513,7 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
         tmem_load32(taddr + c, v);
         const int col = tl.nt * NT + c;
         if (row < p.a.tokens) {
+          if (broken) add_broken<BF16>(p, row, tl.mt, col, q0, q1, v);
           if (p.splits > 1) {
             float* at = p.l.part + ((int64_t)tl.part * p.a.tokens + row) * outer + col;
 #pragma unroll
@@ -498,7 +542,8 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
     const int tokens = (int)p.a.tokens, rank = p.a.rank, outer = p.a.outer;
     uint32_t h = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
+    int i = 0;
+    for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++i) {
       const Tile tl = tile_of(t);
       int q0, q1;
       extra_of(tl, q0, q1);
@@ -517,6 +562,10 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
           const int col = tl.nt * NT + row0 + 32 * j;
           bv[j] = load8(static_cast<const uint16_t*>(p.a.b) + ((int64_t)id * outer + col) * rank + r0,
                         in && col < outer);
+          if (not_finite<BF16>(bv[j])) {
+            bv[j] = make_uint4(0, 0, 0, 0);
+            *const_cast<volatile int*>(&sm.broken[i & 1]) = t + 1;
+          }
         }
 #pragma unroll
         for (int j = 0; j < kABM / 32; ++j) {

@@ -146,6 +146,29 @@ def test_which_adapter(tokens):
             :tokens // 2])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("tokens,inner", [(8, 264), (50, 264), (50, 4096), (300, 264)])
+def test_one_requests_broken_adapter(tokens, inner, dtype):
+    """Infinities and NaN of an adapter's B reach its own tokens' features alone."""
+    x, w, a, b, _, s = inputs(tokens, inner, 136, 3, 24, dtype, tokens)
+    ids = torch.arange(tokens, device=DEV).int() % 4 - 1
+    want = check(x, w, a, b, ids, s)
+    broken = b.clone()
+    broken[1, 5, 3] = float("inf")
+    broken[1, 70, 23] = float("nan")
+    broken[1, 135, 8] = -float("inf")
+    y = ops.adapted_linear(x, w, a, broken, ids, scaling=s)
+    own = ids == 1
+    assert torch.equal(y[~own], want[~own])
+    good = torch.ones(136, dtype=torch.bool, device=DEV)
+    good[[5, 70, 135]] = False
+    assert torch.equal(y[own][:, good], want[own][:, good])
+    assert bool(y[own][:, 70].isnan().all())
+    z = (x[own].double() @ a[1].double().t())
+    assert torch.equal(y[own][:, 5], (z[:, 3] * float("inf")).to(dtype))
+    assert torch.equal(y[own][:, 135], (z[:, 8] * -float("inf")).to(dtype))
+
+
 def test_far_apart_terms():
     """Adapters that outweigh the projection: z keeps two terms' accuracy."""
     for dtype in (BF16, F16):
