@@ -6,7 +6,7 @@
 // instructions: x and the adapters in use are read once.  Then one GEMM over W whose reduction goes on over
 // z and B: a tile of 128 tokens lists its distinct adapters, and for each the reduction gains 2 rank columns,
 // z of that adapter's tokens (0 for the others) as the sum of two 16-bit terms (what one would round away is
-// in the other: 2^-16 of z in bf16) against B twice.  So the adapters' part costs matrix instructions on
+// in the other: 2^-16 of z in bf16), both against B.  So the adapters' part costs matrix instructions on
 // tiles that are there anyway, and y is written once, rounded once.  The GEMM starts on x and W while z is
 // still being computed.  Up to 16 tokens, where W's bytes are all that counts, a kernel of warp matrix
 // instructions reads W by every SM and adds z B in fp32.
@@ -25,15 +25,15 @@
 namespace exf {
 using namespace tc;
 
-constexpr int kFewAdapted = 16;     // tokens of the kernel without tiles
+constexpr int kFewAdapted = 16;       // tokens of the kernel without tiles
+constexpr int kDownTokens = 256;      // tokens of adapter_down_kernel
 constexpr int kAdaptedThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue, warps 6-9 adapters
 constexpr int kABM = 128;           // tokens of a tile
 constexpr int kABK = 64;            // columns of a stage: 128 bytes
 
 struct AdapterPlan {
-  int parts;        // z's reduction lies in this many parts, added where it is read
-  int block_tokens; // of adapter_down_kernel
-  int nt, splits;   // the GEMM's tile and the parts of its reduction
+  int parts;       // z's reduction lies in this many parts, added where it is read
+  int nt, splits;  // the GEMM's tile and the parts of its reduction
 };
 
 // What the kernels hand on: z [parts][tokens][rank]; for each tile of 128 tokens its number of distinct
@@ -74,22 +74,100 @@ __device__ __forceinline__ bool not_finite(const uint4& v) {
   return not_finite2<BF16>(v.x) || not_finite2<BF16>(v.y) || not_finite2<BF16>(v.z) ||
          not_finite2<BF16>(v.w);
 }
+// 8 values of a token's z, its parts added in order; every part's load is under way at once
+constexpr int kMostParts = 8;
+__device__ __forceinline__ void load_z(const AdapterLists& l, int parts, int64_t tokens, int token,
+                                       int rank, int r0, float (&z)[8]) {
+  float4 u[kMostParts][2];
+#pragma unroll
+  for (int k = 0; k < kMostParts; ++k) {
+    if (k < parts) {
+      const float4* at = reinterpret_cast<const float4*>(l.z + (k * tokens + token) * rank + r0);
+      u[k][0] = at[0];
+      u[k][1] = at[1];
+    } else {
+      u[k][0] = u[k][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) z[j] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kMostParts; ++k) {
+    z[0] += u[k][0].x;
+    z[1] += u[k][0].y;
+    z[2] += u[k][0].z;
+    z[3] += u[k][0].w;
+    z[4] += u[k][1].x;
+    z[5] += u[k][1].y;
+    z[6] += u[k][1].z;
+    z[7] += u[k][1].w;
+  }
+}
 // 8 columns of 16 bits, or zeros
 __device__ __forceinline__ uint4 load8(const uint16_t* p, bool there) {
   return there ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
 }
 
-// ---- z --------------------------------------------------------------------------------------------------
-// A block takes TB = 8 NB tokens and one part of the reduction, its 8 warps an eighth of that each; for each
-// distinct adapter among the tokens, 16 MB of its rows against all of them (a token keeps its own adapter's
-// column).  A lane loads 8 columns (16 bytes) of a row, and the instruction's 16 columns are taken as words
-// 0, 1 and then 2, 3 of each: the order of a sum is free as long as both operands have the same.  Blocks
-// before them (one for each tile of 128 tokens; none where no tiles follow) list the tiles' adapters.
-template <bool BF16, int MB, int NB>
+// ---- the adapters of a tile --------------------------------------------------------------------------------
+// The distinct adapters among 128 tokens in the order of their first token, and each token's place among them
+// (255: none), by the first 128 threads of a block that all call it.
+struct TileAdapters {
+  int id[128], list[128];
+  uint32_t first[4];
+  int count;
+};
+__device__ __forceinline__ int list_adapters(const AdapterArgs& p, int tile, TileAdapters& sm) {
+  const int t = tile * 128 + (int)threadIdx.x;
+  if (threadIdx.x < 128) {
+    const int i = t < p.tokens ? p.ids[t] : -1;
+    sm.id[threadIdx.x] = i >= 0 && i < p.adapters ? i : -1;
+  }
+  __syncthreads();
+  int lead = 0, mine = -1;
+  if (threadIdx.x < 128) {
+    mine = sm.id[threadIdx.x];
+    while (sm.id[lead] != mine) ++lead;
+    const uint32_t word = __ballot_sync(0xffffffffu, mine >= 0 && lead == (int)threadIdx.x);
+    if ((threadIdx.x & 31) == 0) sm.first[threadIdx.x >> 5] = word;
+  }
+  __syncthreads();
+  int place = 255;
+  if (threadIdx.x < 128) {
+    if (mine >= 0) {
+      place = __popc(sm.first[lead >> 5] & ((1u << (lead & 31)) - 1u));
+      for (int w = 0; w < lead >> 5; ++w) place += __popc(sm.first[w]);
+      if (lead == (int)threadIdx.x) sm.list[place] = mine;
+    }
+    if (threadIdx.x == 0) {
+      sm.count = 0;
+      for (int w = 0; w < 4; ++w) sm.count += __popc(sm.first[w]);
+    }
+  }
+  __syncthreads();
+  return place;
+}
+__device__ __forceinline__ void write_list(const AdapterArgs& p, const AdapterLists& l, int tile,
+                                           const TileAdapters& sm, int place) {
+  const int t = tile * 128 + (int)threadIdx.x;
+  if (threadIdx.x >= 128) return;
+  if (t < p.tokens) l.place[t] = (uint8_t)place;
+  if ((int)threadIdx.x < sm.count) l.list[tile * 128 + threadIdx.x] = sm.list[threadIdx.x];
+  if (threadIdx.x == 0) l.count[tile] = sm.count;
+}
+
+// ---- z of up to 256 tokens ----------------------------------------------------------------------------------
+// A block takes 8 tokens and one part of the reduction.  Its work is each distinct adapter's rows, 16 MB at a
+// time, against all 8 tokens (a token keeps its own adapter's column), in units of 32 columns, dealt out to
+// the 8 warps in equal runs: where every token has an adapter of its own, each warp streams one of them.  A
+// lane loads 8 columns (16 bytes) of a row, and the instruction's 16 columns are taken as words 0, 1 and then
+// 2, 3 of each: the order of a sum is free as long as both operands have the same.  (All warps on one
+// adapter after another: 64 tokens of 32 adapters, 2048 columns, rank 16: 10 us, a load's latency each.)
+// Blocks before them, one for each tile of 128 tokens that follows, list the tiles' adapters.
+template <bool BF16, int MB>
 __global__ void __launch_bounds__(256)
     adapter_down_kernel(const AdapterArgs p, const AdapterLists l, int list_blocks, int parts) {
-  constexpr int TB = 8 * NB, R = 16 * MB;
-  extern __shared__ float sums[];  // [8 warps][TB tokens][R ranks]
+  constexpr int TB = 8, R = 16 * MB;
+  __shared__ float sums[8][TB][R + 1];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // (only now: the GEMM reads x before it waits for this kernel)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -97,61 +175,44 @@ __global__ void __launch_bounds__(256)
   const int tokens = (int)p.tokens;
 
   if ((int)blockIdx.x < list_blocks) {
-    __shared__ int id[128], first[128];
-    const int t = blockIdx.x * 128 + threadIdx.x;
-    if (threadIdx.x < 128) {
-      const int i = t < tokens ? p.ids[t] : -1;
-      id[threadIdx.x] = i >= 0 && i < p.adapters ? i : -1;
-    }
-    __syncthreads();
-    int lead = 0;
-    if (threadIdx.x < 128) {
-      while (id[lead] != id[threadIdx.x]) ++lead;
-      first[threadIdx.x] = lead == (int)threadIdx.x && id[threadIdx.x] >= 0;
-    }
-    __syncthreads();
-    if (threadIdx.x < 128) {
-      int before = 0;
-      for (int j = 0; j < lead; ++j) before += first[j];
-      if (first[threadIdx.x]) l.list[blockIdx.x * 128 + before] = id[threadIdx.x];
-      if (t < tokens) l.place[t] = id[threadIdx.x] >= 0 ? (uint8_t)before : 255;
-      if (threadIdx.x == 127) {
-        int all = 0;
-        for (int j = 0; j < 128; ++j) all += first[j];
-        l.count[blockIdx.x] = all;
-      }
-    }
+    TileAdapters& sm = *reinterpret_cast<TileAdapters*>(&sums[0][0][0]);
+    const int place = list_adapters(p, blockIdx.x, sm);
+    write_list(p, l, blockIdx.x, sm, place);
     return;
   }
 
   const int block = blockIdx.x - list_blocks;
   const int part = block % parts, t0 = block / parts * TB;
-  // this warp's columns, in units of 32
-  const int units = (p.inner + 31) / 32, slices = parts * 8, slice = part * 8 + warp;
-  const int k0 = (int)((int64_t)units * slice / slices) * 32;
-  const int k1 = (int)((int64_t)units * (slice + 1) / slices) * 32;
+  const int all = (p.inner + 31) / 32;
+  const int u0 = all * part / parts, units = all * (part + 1) / parts - u0;
   int mine = lane < TB && t0 + lane < tokens ? p.ids[t0 + lane] : -1;
   if (mine < 0 || mine >= p.adapters) mine = -1;
   const uint32_t same = __match_any_sync(0xffffffffu, mine);
   const uint32_t leaders = __ballot_sync(0xffffffffu, mine >= 0 && __ffs(same) - 1 == lane);
+  const int items = __popc(leaders) * units;
+  const int i0 = items * warp / 8, i1 = items * (warp + 1) / 8;  // this warp's
+  const int first = units ? i0 / units : 0, last = units ? (i1 + units - 1) / units : 0;
 
   const uint16_t* x = static_cast<const uint16_t*>(p.x);
   const int g = lane >> 2, c = lane & 3;
-  float* own = sums + warp * TB * R;
   for (int r0 = 0; r0 < p.rank; r0 += R) {
-    for (uint32_t left = leaders; left; left &= left - 1) {
+    for (int i = lane; i < TB * (R + 1); i += 32) (&sums[warp][0][0])[i] = 0.0f;
+    __syncwarp();
+    uint32_t left = leaders;
+    for (int n = 0; n < last; ++n, left &= left - 1) {
+      if (n < first) continue;
       const int lead = __ffs(left) - 1;
       const int id = __shfl_sync(0xffffffffu, mine, lead);
       const uint32_t members = __shfl_sync(0xffffffffu, same, lead);
       const uint16_t* a = static_cast<const uint16_t*>(p.a) + ((int64_t)id * p.rank + r0) * p.inner;
-      float d[MB][NB][4] = {};
-#pragma unroll 2
-      for (int k = k0 + 8 * c; k < k1 + 8 * c; k += 32) {
+      const int b0 = n == first ? i0 - n * units : 0, b1 = n == last - 1 ? i1 - n * units : units;
+      float d[MB][4] = {};
+#pragma unroll(MB == 4 ? 2 : 4)
+      for (int u = b0; u < b1; ++u) {
+        const int k = (u0 + u) * 32 + 8 * c;
         const bool in = k < p.inner;
-        uint4 xv[NB], av[MB][2];
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-          xv[n] = load8(x + (int64_t)(t0 + 8 * n + g) * p.inner + k, in && t0 + 8 * n + g < tokens);
+        uint4 av[MB][2];
+        const uint4 xv = load8(x + (int64_t)(t0 + g) * p.inner + k, in && t0 + g < tokens);
 #pragma unroll
         for (int m = 0; m < MB; ++m)
 #pragma unroll
@@ -159,43 +220,197 @@ __global__ void __launch_bounds__(256)
             av[m][h] = load8(a + (int64_t)(16 * m + 8 * h + g) * p.inner + k,
                              in && r0 + 16 * m + 8 * h + g < p.rank);
 #pragma unroll
-        for (int m = 0; m < MB; ++m)
-#pragma unroll
-          for (int n = 0; n < NB; ++n) {
-            warp_mma<BF16>(d[m][n], av[m][0].x, av[m][1].x, av[m][0].y, av[m][1].y, xv[n].x, xv[n].y);
-            warp_mma<BF16>(d[m][n], av[m][0].z, av[m][1].z, av[m][0].w, av[m][1].w, xv[n].z, xv[n].w);
-          }
+        for (int m = 0; m < MB; ++m) {
+          warp_mma<BF16>(d[m], av[m][0].x, av[m][1].x, av[m][0].y, av[m][1].y, xv.x, xv.y);
+          warp_mma<BF16>(d[m], av[m][0].z, av[m][1].z, av[m][0].w, av[m][1].w, xv.z, xv.w);
+        }
       }
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
+      for (int j = 0; j < 2; ++j) {
+        const int t = 2 * c + j;
+        if (members >> t & 1) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int t = 8 * n + 2 * c + j;
-          if (members >> t & 1) {
-#pragma unroll
-            for (int m = 0; m < MB; ++m) {
-              own[t * R + 16 * m + g] = d[m][n][j];
-              own[t * R + 16 * m + 8 + g] = d[m][n][2 + j];
-            }
+          for (int m = 0; m < MB; ++m) {
+            sums[warp][t][16 * m + g] = d[m][j];
+            sums[warp][t][16 * m + 8 + g] = d[m][2 + j];
           }
         }
+      }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < TB * R; i += 256) {
-      const int t = i / R, r = r0 + i % R;
-      if (t0 + t < tokens && r < p.rank) {
+      const int t = i / R, r = i % R;
+      if (t0 + t < tokens && r0 + r < p.rank) {
         const int id = p.ids[t0 + t];
-        float z = 0.0f;
         if (id >= 0 && id < p.adapters) {
+          float z = 0.0f;
 #pragma unroll
-          for (int w = 0; w < 8; ++w) z += sums[w * TB * R + i];
+          for (int w = 0; w < 8; ++w) z += sums[w][t][r];
           if (p.scaling) z *= p.scaling[id];
+          l.z[((int64_t)part * tokens + t0 + t) * p.rank + r0 + r] = z;
         }
-        l.z[((int64_t)part * tokens + t0 + t) * p.rank + r] = z;
       }
     }
     __syncthreads();
   }
+}
+
+// ---- z of more tokens -----------------------------------------------------------------------------------------
+// Tiles of 128 tokens on tcgen05: a block takes one part of the reduction of a tile, lists the tile's adapters
+// (for the GEMM too), and multiplies the tile by each one's rows (RN of them, from its first on; those past
+// its rank are another's, and not used); a token's thread keeps its own adapter's.  (Warp matrix
+// instructions, 32 tokens a block: 8192 tokens, 2048 columns, rank 64: 38 us.)
+template <int RN>
+struct DownSmem {
+  static constexpr int kStage = kABM * kABK * 2 + RN * kABK * 2;
+  static constexpr int kStages = 6;
+  alignas(1024) uint8_t tiles[kStages][kStage];
+  alignas(8) uint64_t full[kStages];
+  alignas(8) uint64_t empty[kStages];
+  alignas(8) uint64_t acc_full[2];
+  alignas(8) uint64_t acc_empty[2];
+  alignas(8) uint64_t drain;
+  TileAdapters tile;
+  uint32_t tmem_base;
+  int failed;
+};
+template <int RN, bool BF16>
+__global__ void __launch_bounds__(192, 1)
+    adapter_down_tile_kernel(const __grid_constant__ CUtensorMap map_x,
+                             const __grid_constant__ CUtensorMap map_a, const AdapterArgs p,
+                             const AdapterLists l, int parts) {
+  using S = DownSmem<RN>;
+  constexpr int kStages = S::kStages;
+  constexpr int kColumns = 2 * RN < 32 ? 32 : 2 * RN;
+  constexpr uint32_t kIdesc = idesc_f16(kABM, RN, BF16);
+  extern __shared__ uint8_t smem_raw[];
+  S& sm = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                ~static_cast<uintptr_t>(1023));
+  const int warp = uniform(threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm.acc_full[b], 1);
+      mbar_init(&sm.acc_empty[b], 4);
+    }
+    mbar_init(&sm.drain, 1);
+    sm.failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc(&sm.tmem_base, kColumns);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // (only now: the GEMM reads x before it waits for this kernel)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int mt = blockIdx.x / parts, part = blockIdx.x % parts;
+  const int place = list_adapters(p, mt, sm.tile);
+  if (part == 0) write_list(p, l, mt, sm.tile, place);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+
+  const int slots = uniform(sm.tile.count);
+  const int kblocks = (p.inner + kABK - 1) / kABK;
+  const int kb0 = (int)((int64_t)kblocks * part / parts);
+  const int n = (int)((int64_t)kblocks * (part + 1) / parts) - kb0;
+  const uint32_t tmem = uniform(sm.tmem_base);
+  volatile int* failed = &sm.failed;
+  if (warp == 0) {
+    uint32_t g = 0;
+    bool ok = true;
+    for (int i = 0; i < slots && ok; ++i) {
+      const int row = uniform(sm.tile.list[i]) * p.rank;
+      for (int k = 0; k < n; ++k, ++g) {
+        const int s = g % kStages;
+        ok = warp_wait(&sm.empty[s], ((g / kStages) & 1) ^ 1, failed);
+        if (!ok) break;
+        if (elect_one()) {
+          mbar_expect_tx(&sm.full[s], S::kStage);
+          tma_load_2d(sm.tiles[s], &map_x, &sm.full[s], (kb0 + k) * kABK, mt * kABM);
+          tma_load_2d(sm.tiles[s] + kABM * kABK * 2, &map_a, &sm.full[s], (kb0 + k) * kABK, row);
+        }
+      }
+    }
+    for (uint32_t j = g > kStages ? g - kStages : 0; j < g; ++j)
+      mbar_wait_drain(&sm.full[j % kStages], (j / kStages) & 1);
+  } else if (warp == 1) {
+    uint32_t g = 0;
+    bool ok = true;
+    for (int i = 0; i < slots && ok; ++i) {
+      const int b = i & 1;
+      ok = warp_wait(&sm.acc_empty[b], ((i >> 1) & 1) ^ 1, failed);
+      if (!ok) break;
+      fence_after_sync();
+      const uint32_t acc = tmem + static_cast<uint32_t>(b * RN);
+      for (int k = 0; k < n; ++k, ++g) {
+        const int s = g % kStages;
+        ok = warp_wait(&sm.full[s], (g / kStages) & 1, failed);
+        if (!ok) break;
+        fence_after_sync();
+        const uint32_t base = smem_addr(sm.tiles[s]);
+        const uint64_t da = smem_desc(base), db = smem_desc(base + kABM * kABK * 2);
+        if (elect_one()) {
+#pragma unroll
+          for (int e = 0; e < kABK / 16; ++e)
+            mma_kind_f16(acc, da + 2 * e, db + 2 * e, kIdesc, k > 0 || e > 0 ? 1u : 0u);
+          mma_commit(&sm.empty[s]);
+        }
+      }
+      if (!ok) break;
+      if (elect_one()) mma_commit(&sm.acc_full[b]);
+    }
+    if (slots > 0) {
+      if (elect_one()) mma_commit(&sm.drain);
+      mbar_wait_drain(&sm.drain, 0);
+    }
+  } else {
+    const int q = warp & 3;
+    const int token = mt * kABM + q * 32 + lane;
+    const int id = token < p.tokens ? sm.tile.id[q * 32 + lane] : -1;
+    const float scale = id >= 0 && p.scaling ? p.scaling[id] : 1.0f;
+    float* to = l.z + ((int64_t)part * p.tokens + token) * p.rank;
+    for (int i = 0; i < slots; ++i) {
+      const int b = i & 1;
+      if (!warp_wait(&sm.acc_full[b], (i >> 1) & 1, failed)) break;
+      fence_after_sync();
+      const bool mine = id >= 0 && id == sm.tile.list[i];
+      if (__any_sync(0xffffffffu, mine)) {
+        const uint32_t taddr = tmem + static_cast<uint32_t>(b * RN) + ((uint32_t)(q * 32) << 16);
+#pragma unroll 1
+        for (int c = 0; c < RN; c += 16) {
+          uint32_t v[16];
+          __syncwarp();
+          tmem_load16(taddr + c, v);
+          tmem_wait();
+          if (mine) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 8)
+              if (c + j < p.rank) {
+                float e[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) e[r] = __uint_as_float(v[j + r]) * scale;
+                *reinterpret_cast<float4*>(to + c + j) = make_float4(e[0], e[1], e[2], e[3]);
+                *reinterpret_cast<float4*>(to + c + j + 4) = make_float4(e[4], e[5], e[6], e[7]);
+              }
+          }
+        }
+      }
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.acc_empty[b]);
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    fence_after_sync();
+    tmem_free(tmem, kColumns);
+  }
+  if (threadIdx.x == 0 && sm.failed && p.status) atomicExch(p.status, 1);
 }
 
 // ---- a few tokens -----------------------------------------------------------------------------------------
@@ -246,19 +461,8 @@ __global__ void __launch_bounds__(256)
       const uint16_t* b = static_cast<const uint16_t*>(p.b) + ((int64_t)id * p.outer + n) * p.rank;
       for (int r = 0; r < p.rank; r += 8) {
         const uint4 v = load8(b + r, true);
-        float z[8] = {};
-        for (int q = 0; q < parts; ++q) {
-          const float4* at = reinterpret_cast<const float4*>(l.z + ((int64_t)q * tokens + t) * p.rank + r);
-          const float4 u0 = at[0], u1 = at[1];
-          z[0] += u0.x;
-          z[1] += u0.y;
-          z[2] += u0.z;
-          z[3] += u0.w;
-          z[4] += u1.x;
-          z[5] += u1.y;
-          z[6] += u1.z;
-          z[7] += u1.w;
-        }
+        float z[8];
+        load_z(l, parts, tokens, t, p.rank, r, z);
         const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -273,10 +477,11 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---- tiles ----------------------------------------------------------------------------------------------
-// Stages of 64 columns of x and W come by TMA (128-byte swizzle).  The adapters' columns come in stages of
-// 32 (64-byte swizzle) of their own, written by four warps while the main stages are multiplied, and are
-// taken in between them, spread over the tile: a sum's order is free, and nothing waits for loads that could
-// have been under way.  (The first tile takes them last: z may still be on its way.)
+// Stages of 64 columns of x and W come by TMA (128-byte swizzle).  The adapters come in stages of their own,
+// 16 ranks of one adapter: z's two terms (zeros for other adapters' tokens) and B, each 16 columns (32-byte
+// swizzle), two products with one B.  Four warps write them, the next stage's loads under way while one
+// waits for its place, and they are taken in between the main stages, spread over the tile: a sum's order
+// is free.  (The first tile takes them last: z may still be on its way.)
 // A tile's tokens meet all of its adapters, all but their own times 0, and 0 times an infinity is a NaN.  So
 // eight columns of B with one that is not finite go in as zeros, and the epilogue adds them to their own
 // adapter's tokens: one request's broken adapter does not reach another's.
@@ -285,9 +490,9 @@ struct AdaptedCfg {
   static constexpr int kATile = kABM * kABK * 2;
   static constexpr int kBTile = NT * kABK * 2;
   static constexpr int kStage = kATile + kBTile;
-  static constexpr int kExtra = (kABM + NT) * 64;
-  static constexpr int kExtras = NT == 256 ? 1 : 2;
-  static constexpr int kStages = (220 * 1024 - kExtras * kExtra) / kStage;
+  static constexpr int kExtra = (2 * kABM + NT) * 32;
+  static constexpr int kExtras = NT == 256 ? 2 : 4;
+  static constexpr int kStages = (224 * 1024 - kExtras * kExtra) / kStage;
   static constexpr int kTmem = 2 * NT;  // two accumulators, a power of two
 };
 template <int NT>
@@ -308,11 +513,11 @@ struct AdaptedSmem {
 template <int NT>
 constexpr size_t adapted_smem_bytes() { return sizeof(AdaptedSmem<NT>) + 1024; }
 
-// Shared-memory matrix descriptor: K-major tile with 64-byte rows, 64-byte swizzle (16-byte piece j of row m
-// at piece j ^ (m / 2 % 4)); 8-row groups 512 bytes apart.
-__device__ __forceinline__ uint64_t smem_desc_64(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(512 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)4 << 61);
+// Shared-memory matrix descriptor: K-major tile with 32-byte rows, 32-byte swizzle (16-byte piece j of row m
+// at piece j ^ (m / 4 % 2)); 8-row groups 256 bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_32(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(256 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)6 << 61);
 }
 
 struct AdaptedGemm {
@@ -326,22 +531,21 @@ struct AdaptedGemm {
 template <bool BF16>
 __device__ __noinline__ void add_broken(const AdaptedGemm& p, int token, int mt, int col, int q0, int q1,
                                         float (&v)[32]) {
-  const int slot = p.l.place[token], rank = p.a.rank, width = 2 * rank;
+  const int slot = p.l.place[token], rank = p.a.rank, width = (rank + 15) / 16;
   if (slot == 255) return;
   const int id = p.l.list[mt * 128 + slot];
   for (int r0 = 0; r0 < rank; r0 += 8) {
-    const int q = (slot * width + r0) / 32;  // the stage of their first terms
+    const int q = slot * width + r0 / 16;
     if (q < q0 || q >= q1) continue;
+    float z[8];
+    load_z(p.l, p.parts, p.a.tokens, token, rank, r0, z);
 #pragma unroll 1
     for (int j = 0; j < 32 && col + j < p.a.outer; ++j) {
       const uint16_t* b =
           static_cast<const uint16_t*>(p.a.b) + ((int64_t)id * p.a.outer + col + j) * rank + r0;
       if (!not_finite<BF16>(load8(b, true))) continue;
-      for (int r = 0; r < 8; ++r) {
-        float z = 0.0f;
-        for (int k = 0; k < p.parts; ++k) z += p.l.z[((int64_t)k * p.a.tokens + token) * rank + r0 + r];
-        v[j] = fmaf(z, unpack2<BF16>(b[r]).x, v[j]);
-      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v[j] = fmaf(z[r], unpack2<BF16>(b[r]).x, v[j]);
     }
   }
 }
@@ -384,7 +588,7 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
 
   const int mn_tiles = p.m_tiles * p.n_tiles;
   const int ntiles = mn_tiles * p.splits;
-  const int width = 2 * p.a.rank;  // columns that an adapter adds
+  const int width = (p.a.rank + 15) / 16;  // stages that an adapter adds
   // tile t: reduction part, M tile, N tile, k blocks [kb0, kb1)
   struct Tile {
     int part, mt, nt, kb0, kb1;
@@ -401,9 +605,9 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
   };
   // its adapters' stages [q0, q1), read behind the wait for adapter_down_kernel
   auto extra_of = [&](const Tile& tl, int& q0, int& q1) {
-    const int chunks = (uniform(p.l.count[tl.mt]) * width + 31) / 32;
-    q0 = chunks * tl.part / p.splits;
-    q1 = chunks * (tl.part + 1) / p.splits;
+    const int all = uniform(p.l.count[tl.mt]) * width;
+    q0 = all * tl.part / p.splits;
+    q1 = all * (tl.part + 1) / p.splits;
   };
   const uint32_t tmem = uniform(sm.tmem_base);
   volatile int* failed = &sm.failed;
@@ -453,10 +657,10 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
           if (!ok) break;
           fence_after_sync();
           const uint32_t base = smem_addr(sm.extra[s]);
-          const uint64_t da = smem_desc_64(base), db = smem_desc_64(base + kABM * 64);
+          const uint64_t db = smem_desc_32(base + 2 * kABM * 32);
           if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) mma_kind_f16(acc, da + 2 * k, db + 2 * k, kIdesc, 1u);
+            mma_kind_f16(acc, smem_desc_32(base), db, kIdesc, 1u);
+            mma_kind_f16(acc, smem_desc_32(base + kABM * 32), db, kIdesc, 1u);
             mma_commit(&sm.extra_empty[s]);
           }
           ++h;
@@ -533,80 +737,75 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
       if (lane == 0) mbar_arrive(&sm.acc_empty[b]);
     }
   } else {
-    // ---- the adapters' stages.  Column v of a tile's adapters belongs to adapter v / width, its first rank
-    // columns the first terms of z, the others the second.  Eight columns (16 bytes) lie in one adapter and
-    // one term; a thread writes the same eight of every 32nd row.
+    // ---- the adapters' stages: a thread has one of the tile's tokens, and a feature of every 128
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x - 192;
-    const int piece = tid & 3, row0 = tid >> 2;
     const int tokens = (int)p.a.tokens, rank = p.a.rank, outer = p.a.outer;
+    constexpr int kRows = (NT + 127) / 128;
+    struct Stage {
+      uint4 z[2][2];  // [term][half of the ranks]
+      uint4 b[kRows][2];
+    };
     uint32_t h = 0;
-    bool ok = true;
     int i = 0;
+    bool ok = true;
     for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++i) {
       const Tile tl = tile_of(t);
       int q0, q1;
       extra_of(tl, q0, q1);
-      const int columns = uniform(p.l.count[tl.mt]) * width;
+      const int token = tl.mt * kABM + tid;
+      const int place = token < tokens ? p.l.place[token] : 255;
+      auto fetch = [&](int q, Stage& e) {
+        const int slot = q / width, r0 = (q - slot * width) * 16;
+        const int id = p.l.list[tl.mt * 128 + slot];
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) {
+          const int row = tid + 128 * j, col = tl.nt * NT + row;
+          const uint16_t* b =
+              static_cast<const uint16_t*>(p.a.b) + ((int64_t)id * outer + col) * rank + r0;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            e.b[j][k] = load8(b + 8 * k, row < NT && col < outer && r0 + 8 * k < rank);
+            if (not_finite<BF16>(e.b[j][k])) {
+              e.b[j][k] = make_uint4(0, 0, 0, 0);
+              *const_cast<volatile int*>(&sm.broken[i & 1]) = t + 1;
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          e.z[0][k] = e.z[1][k] = make_uint4(0, 0, 0, 0);
+          if (place == slot && r0 + 8 * k < rank) {
+            float z[8];
+            load_z(p.l, p.parts, tokens, token, rank, r0 + 8 * k, z);
+#pragma unroll
+            for (int term = 0; term < 2; ++term) {
+              e.z[term][k] = make_uint4(pack2<BF16>(z[0], z[1]), pack2<BF16>(z[2], z[3]),
+                                        pack2<BF16>(z[4], z[5]), pack2<BF16>(z[6], z[7]));
+#pragma unroll
+              for (int r = 0; r < 8; ++r) z[r] = remainder_of<BF16>(z[r]);
+            }
+          }
+        }
+      };
+      Stage e, next;
+      if (q0 < q1) fetch(q0, next);
       for (int q = q0; q < q1; ++q, ++h) {
+        e = next;
+        if (q + 1 < q1) fetch(q + 1, next);
         const int s = h % C::kExtras;
-        const int v = q * 32 + 8 * piece;
-        const int slot = v / width, w = v - slot * width;
-        const bool in = v < columns, second = w >= rank;
-        const int r0 = second ? w - rank : w;
-        const int id = in ? p.l.list[tl.mt * 128 + slot] : 0;
-        // loaded before the stage is free
-        uint4 bv[NT / 32], av[kABM / 32];
-#pragma unroll
-        for (int j = 0; j < NT / 32; ++j) {
-          const int col = tl.nt * NT + row0 + 32 * j;
-          bv[j] = load8(static_cast<const uint16_t*>(p.a.b) + ((int64_t)id * outer + col) * rank + r0,
-                        in && col < outer);
-          if (not_finite<BF16>(bv[j])) {
-            bv[j] = make_uint4(0, 0, 0, 0);
-            *const_cast<volatile int*>(&sm.broken[i & 1]) = t + 1;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < kABM / 32; ++j) {
-          const int token = tl.mt * kABM + row0 + 32 * j;
-          av[j] = make_uint4(0, 0, 0, 0);
-          if (in && token < tokens && p.l.place[token] == slot) {
-            float z[8] = {};
-            for (int k = 0; k < p.parts; ++k) {
-              const float4* at =
-                  reinterpret_cast<const float4*>(p.l.z + ((int64_t)k * tokens + token) * rank + r0);
-              const float4 u0 = at[0], u1 = at[1];
-              z[0] += u0.x;
-              z[1] += u0.y;
-              z[2] += u0.z;
-              z[3] += u0.w;
-              z[4] += u1.x;
-              z[5] += u1.y;
-              z[6] += u1.z;
-              z[7] += u1.w;
-            }
-            if (second) {
-#pragma unroll
-              for (int k = 0; k < 8; ++k) z[k] = remainder_of<BF16>(z[k]);
-            }
-            av[j] = make_uint4(pack2<BF16>(z[0], z[1]), pack2<BF16>(z[2], z[3]),
-                               pack2<BF16>(z[4], z[5]), pack2<BF16>(z[6], z[7]));
-          }
-        }
         ok = warp_wait(&sm.extra_empty[s], ((h / C::kExtras) & 1) ^ 1, failed);
         if (!ok) break;
-        uint8_t* a = sm.extra[s];
-        uint8_t* b = a + kABM * 64;
+        uint8_t* at = sm.extra[s];
 #pragma unroll
-        for (int j = 0; j < NT / 32; ++j) {
-          const int n = row0 + 32 * j;
-          *reinterpret_cast<uint4*>(b + n * 64 + ((piece ^ (n >> 1 & 3)) << 4)) = bv[j];
-        }
+        for (int k = 0; k < 2; ++k) {
+          const int m = tid, piece = (k ^ (m >> 2 & 1)) << 4;
+          *reinterpret_cast<uint4*>(at + m * 32 + piece) = e.z[0][k];
+          *reinterpret_cast<uint4*>(at + kABM * 32 + m * 32 + piece) = e.z[1][k];
 #pragma unroll
-        for (int j = 0; j < kABM / 32; ++j) {
-          const int m = row0 + 32 * j;
-          *reinterpret_cast<uint4*>(a + m * 64 + ((piece ^ (m >> 1 & 3)) << 4)) = av[j];
+          for (int j = 0; j < kRows; ++j)
+            if (tid + 128 * j < NT)
+              *reinterpret_cast<uint4*>(at + 2 * kABM * 32 + (tid + 128 * j) * 32 + piece) = e.b[j][k];
         }
         // written by threads, read by the MMA: to the other proxy, then one arrival a warp
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -655,17 +854,17 @@ __global__ void __launch_bounds__(256)
 static int64_t ceil_of(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static int64_t up_256(int64_t b) { return (b + 255) / 256 * 256; }
 
-// z: blocks of 8 tokens up to 256 tokens, of 32 above; the reduction in parts until the card is full, at
-// least 32 columns a warp.  The GEMM: as the gated block's, tiles of 256 columns while they fill more than
-// half of the SMs, else narrower ones, and long reductions split, at least 8 stages a part.
+// z: blocks of 8 tokens up to kDownTokens, tiles of 128 above; the reduction in parts until the card is full,
+// at least 256 columns each.  The GEMM: as the gated block's, tiles of 256 columns while they
+// fill more than half of the SMs, else narrower ones, and long reductions split, at least 8 stages a part.
 static AdapterPlan plan_of(int64_t tokens, int inner, int outer) {
   const int64_t sms = sm_count() > 0 ? sm_count() : 1;
   AdapterPlan pl;
-  pl.block_tokens = tokens <= 256 ? 8 : 32;
-  const int64_t blocks = ceil_of(tokens, pl.block_tokens);
-  int64_t parts = 2 * sms / blocks;
+  const bool few = tokens <= kDownTokens;
+  const int64_t blocks = ceil_of(tokens, few ? 8 : kABM);
+  int64_t parts = (few ? 2 : 1) * sms / blocks;
   if (parts > ceil_of(inner, 256)) parts = ceil_of(inner, 256);
-  pl.parts = (int)(parts < 1 ? 1 : parts > 8 ? 8 : parts);
+  pl.parts = (int)(parts < 1 ? 1 : parts > kMostParts ? kMostParts : parts);
   pl.nt = 256;
   pl.splits = 1;
   auto tiles = [&](int nt) { return ceil_of(tokens, kABM) * ceil_of(outer, nt); };
@@ -704,24 +903,31 @@ int64_t adapters_workspace(int64_t tokens, int inner, int outer, int rank) {
   return bytes_of(tokens, outer, rank, plan_of(tokens, inner, outer)).all;
 }
 
-template <bool BF16, int MB, int NB>
+template <bool BF16, int MB>
 static cudaError_t down(const AdapterArgs& a, const AdapterLists& l, const AdapterPlan& pl,
                         int list_blocks, cudaStream_t s) {
-  auto* kern = adapter_down_kernel<BF16, MB, NB>;
-  constexpr size_t smem = 8 * 8 * NB * 16 * MB * sizeof(float);
+  const int64_t blocks = list_blocks + ceil_of(a.tokens, 8) * pl.parts;
+  return launch_pdl(adapter_down_kernel<BF16, MB>, dim3((unsigned)blocks), dim3(256), 0, s, a, l,
+                    list_blocks, pl.parts);
+}
+template <int RN, bool BF16>
+static cudaError_t down_tiles(const AdapterArgs& a, const AdapterLists& l, const AdapterPlan& pl,
+                              cudaStream_t s) {
+  constexpr auto dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  auto* kern = adapter_down_tile_kernel<RN, BF16>;
+  constexpr size_t smem = sizeof(DownSmem<RN>) + 1024;
   static std::mutex mu;
   static bool done[64] = {};
   const cudaError_t e = allow_smem(kern, smem, mu, done);
   if (e != cudaSuccess) return e;
-  const int64_t blocks = list_blocks + ceil_of(a.tokens, 8 * NB) * pl.parts;
-  return launch_pdl(kern, dim3((unsigned)blocks), dim3(256), smem, s, a, l, list_blocks, pl.parts);
-}
-template <bool BF16, int NB>
-static cudaError_t down_by_rank(const AdapterArgs& a, const AdapterLists& l, const AdapterPlan& pl,
-                                int list_blocks, cudaStream_t s) {
-  if (a.rank <= 16) return down<BF16, 1, NB>(a, l, pl, list_blocks, s);
-  if (a.rank <= 32) return down<BF16, 2, NB>(a, l, pl, list_blocks, s);
-  return down<BF16, 4, NB>(a, l, pl, list_blocks, s);
+  // (without adapters nothing of A is read, and the map only has to be one)
+  const bool any = a.adapters > 0;
+  CUtensorMap mx, ma;
+  if (!make_map(&mx, a.x, a.tokens, a.inner, kABM, dt) ||
+      !make_map(&ma, any ? a.a : a.x, any ? (uint64_t)a.adapters * a.rank : a.tokens, a.inner, RN, dt))
+    return cudaErrorInvalidValue;
+  return launch_pdl(kern, dim3((unsigned)(ceil_of(a.tokens, kABM) * pl.parts)), dim3(192), smem, s, mx,
+                    ma, a, l, pl.parts);
 }
 
 template <int NT, bool BF16>
@@ -768,9 +974,18 @@ static cudaError_t adapted(const AdapterArgs& a, uint8_t* ws, cudaStream_t s) {
   l.place = ws + by.z + by.count + by.list;
   l.part = reinterpret_cast<float*>(ws + by.z + by.count + by.list + by.place);
   const bool few = a.tokens <= kFewAdapted;
-  const int lists = few ? 0 : (int)ceil_of(a.tokens, kABM);
-  cudaError_t e = pl.block_tokens == 8 ? down_by_rank<BF16, 1>(a, l, pl, lists, s)
-                                       : down_by_rank<BF16, 4>(a, l, pl, lists, s);
+  cudaError_t e;
+  if (a.tokens <= kDownTokens) {
+    const int lists = few ? 0 : (int)ceil_of(a.tokens, kABM);
+    e = a.rank <= 16   ? down<BF16, 1>(a, l, pl, lists, s)
+        : a.rank <= 32 ? down<BF16, 2>(a, l, pl, lists, s)
+                       : down<BF16, 4>(a, l, pl, lists, s);
+  } else {
+    e = a.rank <= 16   ? down_tiles<16, BF16>(a, l, pl, s)
+        : a.rank <= 32 ? down_tiles<32, BF16>(a, l, pl, s)
+        : a.rank <= 64 ? down_tiles<64, BF16>(a, l, pl, s)
+                       : down_tiles<128, BF16>(a, l, pl, s);
+  }
   if (e != cudaSuccess) return e;
   if (few) {
     const dim3 grid((unsigned)ceil_of(a.outer, 16));

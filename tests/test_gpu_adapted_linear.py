@@ -89,7 +89,8 @@ SHAPES = [
     (100, 768, 2048, 200, 8), (127, 320, 1000, 3, 128), (128, 4096, 264, 128, 16),
     (129, 264, 136, 5, 56), (256, 1032, 520, 300, 40), (257, 2048, 768, 11, 32),
     (300, 72, 5000, 4, 64), (1000, 2056, 2056, 6, 16), (1500, 136, 4104, 9, 112),
-    (2500, 520, 4096, 12, 64), (4200, 256, 2048, 40, 8),
+    (2500, 520, 4096, 12, 64), (4200, 256, 2048, 40, 8), (300, 2048, 264, 300, 16),
+    (700, 4104, 264, 2, 128), (520, 776, 136, 3, 96), (260, 8, 8, 2, 8),
 ]
 
 
@@ -147,7 +148,8 @@ def test_which_adapter(tokens):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("tokens,inner", [(8, 264), (50, 264), (50, 4096), (300, 264)])
+@pytest.mark.parametrize("tokens,inner", [(8, 264), (50, 264), (50, 4096), (300, 264),
+                                          (300, 4096)])
 def test_one_requests_broken_adapter(tokens, inner, dtype):
     """Infinities and NaN of an adapter's B reach its own tokens' features alone."""
     x, w, a, b, _, s = inputs(tokens, inner, 136, 3, 24, dtype, tokens)
@@ -201,6 +203,9 @@ def test_shapes_strides_ids_and_empty():
     # no adapters are loaded
     none = ops.adapted_linear(x, w, a[:0], b[:0], ids)
     near(none, *formula(x, w, a[:0], b[:0], ids, None))
+    many = inputs(300, 264, 136, 1, 16, BF16, 2)
+    near(ops.adapted_linear(many[0], w, a[:0], b[:0], many[4]),
+         *formula(many[0], w, a[:0], b[:0], many[4], None))
     few = ops.adapted_linear(x[:4], w, a[:0], b[:0], ids[:4], scaling=s[:0])
     near(few, *formula(x[:4], w, a[:0], b[:0], ids[:4], None))
 
