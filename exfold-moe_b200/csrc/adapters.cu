@@ -8,7 +8,7 @@
 // z of that adapter's tokens (0 for the others) as the sum of two 16-bit terms (what one would round away is
 // in the other: 2^-16 of z in bf16), both against B.  So the adapters' part costs matrix instructions on
 // tiles that are there anyway, and y is written once, rounded once.  The GEMM starts on x and W while z is
-// still being computed.  Up to 16 tokens, where W's bytes are all that counts, a kernel of warp matrix
+// still being computed.  Up to 32 tokens, where W's bytes are all that counts, a kernel of warp matrix
 // instructions reads W by every SM and adds z B in fp32.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -25,25 +25,26 @@
 namespace exf {
 using namespace tc;
 
-constexpr int kFewAdapted = 16;       // tokens of the kernel without tiles
+constexpr int kFewAdapted = 32;       // tokens of the kernel without tiles
 constexpr int kDownTokens = 256;      // tokens of adapter_down_kernel
 constexpr int kAdaptedThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue, warps 6-9 adapters
 constexpr int kABM = 128;           // tokens of a tile
 constexpr int kABK = 64;            // columns of a stage: 128 bytes
 
 struct AdapterPlan {
-  int parts;       // z's reduction lies in this many parts, added where it is read
-  int nt, splits;  // the GEMM's tile and the parts of its reduction
+  int parts;       // blocks (a cluster) among which z's reduction is divided
+  int nt, splits;  // the GEMM's tile, and the blocks (a cluster) that share its reduction
 };
 
-// What the kernels hand on: z [parts][tokens][rank]; for each tile of 128 tokens its number of distinct
+// What the kernels hand on: z, for a few tokens fp32 [tokens][rank], else [tokens][ceil(rank / 16)][2][16], the
+// two 16-bit terms of 16 ranks (zeros past the last); for each tile of 128 tokens its number of distinct
 // adapters and their ids, and for each token its place among them (255: none).
 struct AdapterLists {
   float* z;
+  uint16_t* z16;
   int32_t* count;   // [tiles]
   int32_t* list;    // [tiles][128]
   uint8_t* place;   // [tokens]
-  float* part;      // split reductions: [splits][tokens][outer]
 };
 
 // D (16 x 8, fp32) += A (16 x 16) B (16 x 8), 16-bit operands
@@ -74,34 +75,34 @@ __device__ __forceinline__ bool not_finite(const uint4& v) {
   return not_finite2<BF16>(v.x) || not_finite2<BF16>(v.y) || not_finite2<BF16>(v.z) ||
          not_finite2<BF16>(v.w);
 }
-// 8 values of a token's z, its parts added in order; every part's load is under way at once
-constexpr int kMostParts = 8;
-__device__ __forceinline__ void load_z(const AdapterLists& l, int parts, int64_t tokens, int token,
-                                       int rank, int r0, float (&z)[8]) {
-  float4 u[kMostParts][2];
-#pragma unroll
-  for (int k = 0; k < kMostParts; ++k) {
-    if (k < parts) {
-      const float4* at = reinterpret_cast<const float4*>(l.z + (k * tokens + token) * rank + r0);
-      u[k][0] = at[0];
-      u[k][1] = at[1];
-    } else {
-      u[k][0] = u[k][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
-  }
+constexpr int kMostParts = 8;  // blocks of a cluster
+// eight sums of the cluster's blocks, added in order
+__device__ __forceinline__ void add_peers(const float* at, int parts, float (&z)[8]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) z[j] = 0.0f;
 #pragma unroll
-  for (int k = 0; k < kMostParts; ++k) {
-    z[0] += u[k][0].x;
-    z[1] += u[k][0].y;
-    z[2] += u[k][0].z;
-    z[3] += u[k][0].w;
-    z[4] += u[k][1].x;
-    z[5] += u[k][1].y;
-    z[6] += u[k][1].z;
-    z[7] += u[k][1].w;
-  }
+  for (int k = 0; k < kMostParts; ++k)
+    if (k < parts) {
+      const float4 a = load_peer4(at, k), b = load_peer4(at + 4, k);
+      z[0] += a.x;
+      z[1] += a.y;
+      z[2] += a.z;
+      z[3] += a.w;
+      z[4] += b.x;
+      z[5] += b.y;
+      z[6] += b.z;
+      z[7] += b.w;
+    }
+}
+// the two terms of ranks r0 to r0 + 7 of a token
+template <bool BF16>
+__device__ __forceinline__ void store_terms(const AdapterLists& l, int token, int rank, int r0,
+                                            float (&z)[8]) {
+  const int64_t at = ((int64_t)token * ((rank + 15) / 16) + r0 / 16) * 32 + r0 % 16;
+  store_16b<BF16>(l.z16, at, z);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) z[j] = remainder_of<BF16>(z[j]);
+  store_16b<BF16>(l.z16, at + 16, z);
 }
 // 8 columns of 16 bits, or zeros
 __device__ __forceinline__ uint4 load8(const uint16_t* p, bool there) {
@@ -162,27 +163,22 @@ __device__ __forceinline__ void write_list(const AdapterArgs& p, const AdapterLi
 // lane loads 8 columns (16 bytes) of a row, and the instruction's 16 columns are taken as words 0, 1 and then
 // 2, 3 of each: the order of a sum is free as long as both operands have the same.  (All warps on one
 // adapter after another: 64 tokens of 32 adapters, 2048 columns, rank 16: 10 us, a load's latency each.)
-// Blocks before them, one for each tile of 128 tokens that follows, list the tiles' adapters.
+// The parts are a cluster, which adds its sums.  The first block of each tile of 128 tokens lists the tile's
+// adapters for the GEMM.
 template <bool BF16, int MB>
 __global__ void __launch_bounds__(256)
-    adapter_down_kernel(const AdapterArgs p, const AdapterLists l, int list_blocks, int parts) {
+    adapter_down_kernel(const AdapterArgs p, const AdapterLists l, bool few, int parts) {
   constexpr int TB = 8, R = 16 * MB;
   __shared__ float sums[8][TB][R + 1];
+  __shared__ __align__(16) float joined[TB][R];
+  __shared__ TileAdapters tile;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // (only now: the GEMM reads x before it waits for this kernel)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tokens = (int)p.tokens;
 
-  if ((int)blockIdx.x < list_blocks) {
-    TileAdapters& sm = *reinterpret_cast<TileAdapters*>(&sums[0][0][0]);
-    const int place = list_adapters(p, blockIdx.x, sm);
-    write_list(p, l, blockIdx.x, sm, place);
-    return;
-  }
-
-  const int block = blockIdx.x - list_blocks;
-  const int part = block % parts, t0 = block / parts * TB;
+  const int part = parts > 1 ? cluster_rank() : 0, t0 = blockIdx.x / parts * TB;
   const int all = (p.inner + 31) / 32;
   const int u0 = all * part / parts, units = all * (part + 1) / parts - u0;
   int mine = lane < TB && t0 + lane < tokens ? p.ids[t0 + lane] : -1;
@@ -240,31 +236,57 @@ __global__ void __launch_bounds__(256)
     __syncthreads();
     for (int i = threadIdx.x; i < TB * R; i += 256) {
       const int t = i / R, r = i % R;
-      if (t0 + t < tokens && r0 + r < p.rank) {
-        const int id = p.ids[t0 + t];
-        if (id >= 0 && id < p.adapters) {
-          float z = 0.0f;
+      float z = 0.0f;
 #pragma unroll
-          for (int w = 0; w < 8; ++w) z += sums[w][t][r];
-          if (p.scaling) z *= p.scaling[id];
-          l.z[((int64_t)part * tokens + t0 + t) * p.rank + r0 + r] = z;
-        }
+      for (int w = 0; w < 8; ++w) z += sums[w][t][r];
+      joined[t][r] = z;
+    }
+    if (parts > 1)
+      cluster_sync();
+    else
+      __syncthreads();
+    // eight ranks a thread, dealt out to the cluster's blocks
+    for (int i = part * 256 + threadIdx.x; i < TB * R / 8; i += parts * 256) {
+      const int t = i / (R / 8), r = i % (R / 8) * 8;
+      const int id = t0 + t < tokens ? p.ids[t0 + t] : -1;
+      if (id < 0 || id >= p.adapters || r0 + r >= (p.rank + 15) / 16 * 16) continue;
+      float z[8];
+      add_peers(&joined[t][r], parts, z);
+      if (p.scaling) {
+        const float scale = p.scaling[id];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] *= scale;
+      }
+      if (!few) {
+        store_terms<BF16>(l, t0 + t, p.rank, r0 + r, z);
+      } else if (r0 + r < p.rank) {
+        float4* to = reinterpret_cast<float4*>(l.z + (int64_t)(t0 + t) * p.rank + r0 + r);
+        to[0] = make_float4(z[0], z[1], z[2], z[3]);
+        to[1] = make_float4(z[4], z[5], z[6], z[7]);
       }
     }
-    __syncthreads();
+    if (parts > 1)
+      cluster_sync();  // (nobody's sums are written over, and no block leaves, while they are read)
+    else
+      __syncthreads();
+  }
+  if (!few && part == 0 && t0 % 128 == 0) {
+    const int place = list_adapters(p, t0 / 128, tile);
+    write_list(p, l, t0 / 128, tile, place);
   }
 }
 
 // ---- z of more tokens -----------------------------------------------------------------------------------------
-// Tiles of 128 tokens on tcgen05: a block takes one part of the reduction of a tile, lists the tile's adapters
-// (for the GEMM too), and multiplies the tile by each one's rows (RN of them, from its first on; those past
+// Tiles of 128 tokens on tcgen05: a block takes one part of the reduction of a tile (the parts are a cluster,
+// which adds its sums), lists the tile's adapters (for the GEMM too), and multiplies the tile by each one's rows (RN of them, from its first on; those past
 // its rank are another's, and not used); a token's thread keeps its own adapter's.  (Warp matrix
 // instructions, 32 tokens a block: 8192 tokens, 2048 columns, rank 64: 38 us.)
 template <int RN>
 struct DownSmem {
   static constexpr int kStage = kABM * kABK * 2 + RN * kABK * 2;
-  static constexpr int kStages = 6;
+  static constexpr int kStages = RN == 128 ? 4 : 6;
   alignas(1024) uint8_t tiles[kStages][kStage];
+  alignas(16) float z[128][RN];
   alignas(8) uint64_t full[kStages];
   alignas(8) uint64_t empty[kStages];
   alignas(8) uint64_t acc_full[2];
@@ -305,7 +327,7 @@ __global__ void __launch_bounds__(192, 1)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // (only now: the GEMM reads x before it waits for this kernel)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int mt = blockIdx.x / parts, part = blockIdx.x % parts;
+  const int mt = blockIdx.x / parts, part = parts > 1 ? cluster_rank() : 0;
   const int place = list_adapters(p, mt, sm.tile);
   if (part == 0) write_list(p, l, mt, sm.tile, place);
   fence_before_sync();
@@ -370,8 +392,7 @@ __global__ void __launch_bounds__(192, 1)
     const int q = warp & 3;
     const int token = mt * kABM + q * 32 + lane;
     const int id = token < p.tokens ? sm.tile.id[q * 32 + lane] : -1;
-    const float scale = id >= 0 && p.scaling ? p.scaling[id] : 1.0f;
-    float* to = l.z + ((int64_t)part * p.tokens + token) * p.rank;
+    float* to = sm.z[q * 32 + lane];
     for (int i = 0; i < slots; ++i) {
       const int b = i & 1;
       if (!warp_wait(&sm.acc_full[b], (i >> 1) & 1, failed)) break;
@@ -387,14 +408,10 @@ __global__ void __launch_bounds__(192, 1)
           tmem_wait();
           if (mine) {
 #pragma unroll
-            for (int j = 0; j < 16; j += 8)
-              if (c + j < p.rank) {
-                float e[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) e[r] = __uint_as_float(v[j + r]) * scale;
-                *reinterpret_cast<float4*>(to + c + j) = make_float4(e[0], e[1], e[2], e[3]);
-                *reinterpret_cast<float4*>(to + c + j + 4) = make_float4(e[4], e[5], e[6], e[7]);
-              }
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<float4*>(to + c + j) =
+                  make_float4(__uint_as_float(v[j]), __uint_as_float(v[j + 1]),
+                              __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
           }
         }
       }
@@ -411,6 +428,21 @@ __global__ void __launch_bounds__(192, 1)
     tmem_free(tmem, kColumns);
   }
   if (threadIdx.x == 0 && sm.failed && p.status) atomicExch(p.status, 1);
+  if (parts > 1) cluster_sync();
+  // eight ranks a thread, the tokens dealt out to the cluster's blocks
+  const int groups = (p.rank + 15) / 16 * 2;
+  const int m0 = 128 * part / parts, m1 = 128 * (part + 1) / parts;
+  for (int i = threadIdx.x; i < (m1 - m0) * groups; i += 192) {
+    const int m = m0 + i / groups, r = i % groups * 8, id = sm.tile.id[m];
+    if (id < 0) continue;
+    float z[8];
+    add_peers(&sm.z[m][r], parts, z);
+    const float scale = p.scaling ? p.scaling[id] : 1.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) z[j] = r < p.rank ? z[j] * scale : 0.0f;
+    store_terms<BF16>(l, mt * kABM + m, p.rank, r, z);
+  }
+  if (parts > 1) cluster_sync();  // (no block leaves while its sums are read)
 }
 
 // ---- a few tokens -----------------------------------------------------------------------------------------
@@ -418,7 +450,7 @@ __global__ void __launch_bounds__(192, 1)
 // thread adds a feature's z B.  W is read ahead of the wait for z.
 template <bool BF16, int NB>
 __global__ void __launch_bounds__(256)
-    adapted_few_kernel(const AdapterArgs p, const AdapterLists l, int parts) {
+    adapted_few_kernel(const AdapterArgs p, const AdapterLists l) {
   constexpr int TB = 8 * NB;
   __shared__ float sums[8][TB][17];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -461,8 +493,9 @@ __global__ void __launch_bounds__(256)
       const uint16_t* b = static_cast<const uint16_t*>(p.b) + ((int64_t)id * p.outer + n) * p.rank;
       for (int r = 0; r < p.rank; r += 8) {
         const uint4 v = load8(b + r, true);
-        float z[8];
-        load_z(l, parts, tokens, t, p.rank, r, z);
+        const float4* at = reinterpret_cast<const float4*>(l.z + (int64_t)t * p.rank + r);
+        const float4 z0 = at[0], z1 = at[1];
+        const float z[8] = {z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w};
         const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -523,7 +556,7 @@ __device__ __forceinline__ uint64_t smem_desc_32(uint32_t addr) {
 struct AdaptedGemm {
   AdapterArgs a;
   AdapterLists l;
-  int m_tiles, n_tiles, kblocks, splits, parts;
+  int m_tiles, n_tiles, kblocks, splits;
   bool wide;  // y's rows are 32-byte aligned
 };
 
@@ -537,8 +570,11 @@ __device__ __noinline__ void add_broken(const AdaptedGemm& p, int token, int mt,
   for (int r0 = 0; r0 < rank; r0 += 8) {
     const int q = slot * width + r0 / 16;
     if (q < q0 || q >= q1) continue;
+    const uint16_t* terms = p.l.z16 + ((int64_t)token * width + r0 / 16) * 32 + r0 % 16;
     float z[8];
-    load_z(p.l, p.parts, p.a.tokens, token, rank, r0, z);
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      z[r] = unpack2<BF16>(terms[r]).x + unpack2<BF16>(terms[16 + r]).x;
 #pragma unroll 1
     for (int j = 0; j < 32 && col + j < p.a.outer; ++j) {
       const uint16_t* b =
@@ -586,8 +622,8 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
   fence_after_sync();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  const int mn_tiles = p.m_tiles * p.n_tiles;
-  const int ntiles = mn_tiles * p.splits;
+  // (with a split reduction, a tile's blocks are a cluster, and have one tile each)
+  const int ntiles = p.m_tiles * p.n_tiles * p.splits;
   const int width = (p.a.rank + 15) / 16;  // stages that an adapter adds
   // tile t: reduction part, M tile, N tile, k blocks [kb0, kb1)
   struct Tile {
@@ -595,8 +631,8 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
   };
   auto tile_of = [&](int t) {
     Tile r;
-    r.part = t / mn_tiles;
-    t -= r.part * mn_tiles;
+    r.part = t % p.splits;
+    t /= p.splits;
     r.mt = t / p.n_tiles;
     r.nt = t - r.mt * p.n_tiles;
     r.kb0 = (int)((int64_t)p.kblocks * r.part / p.splits);
@@ -719,10 +755,11 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
         if (row < p.a.tokens) {
           if (broken) add_broken<BF16>(p, row, tl.mt, col, q0, q1, v);
           if (p.splits > 1) {
-            float* at = p.l.part + ((int64_t)tl.part * p.a.tokens + row) * outer + col;
+            // (every copy into the tiles has been multiplied: they hold the sums)
+            float* at = reinterpret_cast<float*>(sm.tiles) + (q * 32 + lane) * (NT + 4) + c;
 #pragma unroll
-            for (int j = 0; j < 32; j += 8)
-              if (col + j < outer) store_sums(at + j, v + j);
+            for (int j = 0; j < 32; j += 4)
+              *reinterpret_cast<float4*>(at + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
           } else {
 #pragma unroll
             for (int j = 0; j < 32; j += 16)
@@ -737,81 +774,73 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
       if (lane == 0) mbar_arrive(&sm.acc_empty[b]);
     }
   } else {
-    // ---- the adapters' stages: a thread has one of the tile's tokens, and a feature of every 128
+    // ---- the adapters' stages: a thread copies one of the tile's tokens' z and every 128th feature's B
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x - 192;
     const int tokens = (int)p.a.tokens, rank = p.a.rank, outer = p.a.outer;
-    constexpr int kRows = (NT + 127) / 128;
-    struct Stage {
-      uint4 z[2][2];  // [term][half of the ranks]
-      uint4 b[kRows][2];
-    };
-    uint32_t h = 0;
+    constexpr int kRows = (NT + 127) / 128, kBehind = C::kExtras - 1;
+    const int piece = (tid >> 2 & 1) << 4;  // of the first half of the ranks
+    uint32_t h = 0;  // stages issued
     int i = 0;
     bool ok = true;
+    // stage j has arrived: looked over, to the other proxy (it is read by the MMA), one arrival a warp
+    auto hand_over = [&](uint32_t j, int t) {
+      uint8_t* at = sm.extra[j % C::kExtras] + 2 * kABM * 32;
+#pragma unroll
+      for (int e = 0; e < kRows; ++e)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (tid + 128 * e >= NT) continue;
+          uint4* v = reinterpret_cast<uint4*>(at + (tid + 128 * e) * 32 + (piece ^ (k << 4)));
+          if (not_finite<BF16>(*v)) {
+            *v = make_uint4(0, 0, 0, 0);
+            *const_cast<volatile int*>(&sm.broken[i & 1]) = t + 1;
+          }
+        }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.extra_full[j % C::kExtras]);
+    };
     for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++i) {
       const Tile tl = tile_of(t);
       int q0, q1;
       extra_of(tl, q0, q1);
       const int token = tl.mt * kABM + tid;
       const int place = token < tokens ? p.l.place[token] : 255;
-      auto fetch = [&](int q, Stage& e) {
-        const int slot = q / width, r0 = (q - slot * width) * 16;
-        const int id = p.l.list[tl.mt * 128 + slot];
-#pragma unroll
-        for (int j = 0; j < kRows; ++j) {
-          const int row = tid + 128 * j, col = tl.nt * NT + row;
-          const uint16_t* b =
-              static_cast<const uint16_t*>(p.a.b) + ((int64_t)id * outer + col) * rank + r0;
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            e.b[j][k] = load8(b + 8 * k, row < NT && col < outer && r0 + 8 * k < rank);
-            if (not_finite<BF16>(e.b[j][k])) {
-              e.b[j][k] = make_uint4(0, 0, 0, 0);
-              *const_cast<volatile int*>(&sm.broken[i & 1]) = t + 1;
-            }
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          e.z[0][k] = e.z[1][k] = make_uint4(0, 0, 0, 0);
-          if (place == slot && r0 + 8 * k < rank) {
-            float z[8];
-            load_z(p.l, p.parts, tokens, token, rank, r0 + 8 * k, z);
-#pragma unroll
-            for (int term = 0; term < 2; ++term) {
-              e.z[term][k] = make_uint4(pack2<BF16>(z[0], z[1]), pack2<BF16>(z[2], z[3]),
-                                        pack2<BF16>(z[4], z[5]), pack2<BF16>(z[6], z[7]));
-#pragma unroll
-              for (int r = 0; r < 8; ++r) z[r] = remainder_of<BF16>(z[r]);
-            }
-          }
-        }
-      };
-      Stage e, next;
-      if (q0 < q1) fetch(q0, next);
+      const uint16_t* z = p.l.z16 + (int64_t)(token < tokens ? token : 0) * width * 32;
       for (int q = q0; q < q1; ++q, ++h) {
-        e = next;
-        if (q + 1 < q1) fetch(q + 1, next);
         const int s = h % C::kExtras;
         ok = warp_wait(&sm.extra_empty[s], ((h / C::kExtras) & 1) ^ 1, failed);
         if (!ok) break;
+        const int slot = q / width, group = q - slot * width;
+        const int id = p.l.list[tl.mt * 128 + slot];
         uint8_t* at = sm.extra[s];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int m = tid, piece = (k ^ (m >> 2 & 1)) << 4;
-          *reinterpret_cast<uint4*>(at + m * 32 + piece) = e.z[0][k];
-          *reinterpret_cast<uint4*>(at + kABM * 32 + m * 32 + piece) = e.z[1][k];
+          const int to = piece ^ (k << 4);
+          const bool mine = place == slot;
+          copy_async16(at + tid * 32 + to, z + group * 32 + 8 * k, mine);
+          copy_async16(at + kABM * 32 + tid * 32 + to, z + group * 32 + 16 + 8 * k, mine);
 #pragma unroll
-          for (int j = 0; j < kRows; ++j)
-            if (tid + 128 * j < NT)
-              *reinterpret_cast<uint4*>(at + 2 * kABM * 32 + (tid + 128 * j) * 32 + piece) = e.b[j][k];
+          for (int e = 0; e < kRows; ++e) {
+            const int row = tid + 128 * e, col = tl.nt * NT + row, r0 = group * 16 + 8 * k;
+            const bool there = col < outer && r0 < rank;
+            if (row < NT)
+              copy_async16(at + 2 * kABM * 32 + row * 32 + to,
+                           static_cast<const uint16_t*>(p.a.b) +
+                               (there ? ((int64_t)id * outer + col) * rank + r0 : 0),
+                           there);
+          }
         }
-        // written by threads, read by the MMA: to the other proxy, then one arrival a warp
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.extra_full[s]);
+        copy_async_commit();
+        if (q - q0 >= kBehind) {
+          copy_async_wait<kBehind>();
+          hand_over(h - kBehind, t);
+        }
       }
+      copy_async_wait<0>();
+      if (!ok) break;
+      for (uint32_t j = h - (q1 - q0 < kBehind ? q1 - q0 : kBehind); j != h; ++j) hand_over(j, t);
     }
   }
   fence_before_sync();
@@ -822,32 +851,21 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
     tmem_free(tmem, C::kTmem);
   }
   if (threadIdx.x == 0 && sm.failed && p.a.status) atomicExch(p.a.status, 1);
-}
-
-// y from the parts of a split reduction, added in order; 8 columns a thread.
-template <bool BF16>
-__global__ void __launch_bounds__(256)
-    adapted_join_kernel(const float* part, int splits, int64_t count, void* y) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8; i < count;
-       i += (int64_t)gridDim.x * blockDim.x * 8) {
-    float v[8] = {};
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-      const float4* at = reinterpret_cast<const float4*>(part + s * count + i);
-      const float4 a = __ldcg(at), b = __ldcg(at + 1);
-      v[0] += a.x;
-      v[1] += a.y;
-      v[2] += a.z;
-      v[3] += a.w;
-      v[4] += b.x;
-      v[5] += b.y;
-      v[6] += b.z;
-      v[7] += b.w;
-    }
-    store_16b<BF16>(y, i, v);
+  if (p.splits == 1) return;
+  // the cluster's sums of this tile: eight features a thread, dealt out to its blocks
+  cluster_sync();
+  const Tile tl = tile_of(blockIdx.x);
+  const float* sums = reinterpret_cast<const float*>(sm.tiles);
+  const int left = (int)p.a.tokens - tl.mt * kABM, rows = left < kABM ? left : kABM;
+  for (int e = tl.part * kAdaptedThreads + threadIdx.x; e < rows * (NT / 8);
+       e += p.splits * kAdaptedThreads) {
+    const int m = e / (NT / 8), c = e % (NT / 8) * 8, col = tl.nt * NT + c;
+    if (col >= p.a.outer) continue;
+    float v[8];
+    add_peers(sums + m * (NT + 4) + c, p.splits, v);
+    store_16b<BF16>(p.a.y, (int64_t)(tl.mt * kABM + m) * p.a.outer + col, v);
   }
+  cluster_sync();  // (no block leaves while its sums are read)
 }
 
 // ---- host side ----------------------------------------------------------------------------------
@@ -876,39 +894,37 @@ static AdapterPlan plan_of(int64_t tokens, int inner, int outer) {
       pl.nt = 128;
       int64_t s = sms / tiles(128);
       if (s > kblocks / 8) s = kblocks / 8;
-      pl.splits = (int)(s > 1 ? s : 1);
+      pl.splits = (int)(s < 1 ? 1 : s > kMostParts ? kMostParts : s);
     }
   }
   return pl;
 }
 
 struct AdapterBytes {
-  int64_t z, count, list, place, part, all;
+  int64_t z, count, list, place, all;
 };
-static AdapterBytes bytes_of(int64_t tokens, int outer, int rank, const AdapterPlan& pl) {
+static AdapterBytes bytes_of(int64_t tokens, int rank) {
   AdapterBytes b;
   const int64_t tiles = ceil_of(tokens, kABM);
   const bool few = tokens <= kFewAdapted;
-  b.z = up_256(pl.parts * tokens * rank * 4);
+  b.z = up_256(few ? tokens * rank * 4 : tokens * ceil_of(rank, 16) * 64);
   b.count = few ? 0 : up_256(tiles * 4);
   b.list = few ? 0 : up_256(tiles * 128 * 4);
   b.place = few ? 0 : up_256(tokens);
-  b.part = !few && pl.splits > 1 ? pl.splits * tokens * outer * 4 : 0;
-  b.all = b.z + b.count + b.list + b.place + b.part;
+  b.all = b.z + b.count + b.list + b.place;
   return b;
 }
 
-int64_t adapters_workspace(int64_t tokens, int inner, int outer, int rank) {
-  if (tokens == 0) return 0;
-  return bytes_of(tokens, outer, rank, plan_of(tokens, inner, outer)).all;
+int64_t adapters_workspace(int64_t tokens, int rank) {
+  return tokens == 0 ? 0 : bytes_of(tokens, rank).all;
 }
 
 template <bool BF16, int MB>
-static cudaError_t down(const AdapterArgs& a, const AdapterLists& l, const AdapterPlan& pl,
-                        int list_blocks, cudaStream_t s) {
-  const int64_t blocks = list_blocks + ceil_of(a.tokens, 8) * pl.parts;
-  return launch_pdl(adapter_down_kernel<BF16, MB>, dim3((unsigned)blocks), dim3(256), 0, s, a, l,
-                    list_blocks, pl.parts);
+static cudaError_t down(const AdapterArgs& a, const AdapterLists& l, const AdapterPlan& pl, bool few,
+                        cudaStream_t s) {
+  return launch_clusters(adapter_down_kernel<BF16, MB>,
+                         dim3((unsigned)(ceil_of(a.tokens, 8) * pl.parts)), dim3(256), 0, s, pl.parts,
+                         a, l, few, pl.parts);
 }
 template <int RN, bool BF16>
 static cudaError_t down_tiles(const AdapterArgs& a, const AdapterLists& l, const AdapterPlan& pl,
@@ -926,8 +942,8 @@ static cudaError_t down_tiles(const AdapterArgs& a, const AdapterLists& l, const
   if (!make_map(&mx, a.x, a.tokens, a.inner, kABM, dt) ||
       !make_map(&ma, any ? a.a : a.x, any ? (uint64_t)a.adapters * a.rank : a.tokens, a.inner, RN, dt))
     return cudaErrorInvalidValue;
-  return launch_pdl(kern, dim3((unsigned)(ceil_of(a.tokens, kABM) * pl.parts)), dim3(192), smem, s, mx,
-                    ma, a, l, pl.parts);
+  return launch_clusters(kern, dim3((unsigned)(ceil_of(a.tokens, kABM) * pl.parts)), dim3(192), smem, s,
+                         pl.parts, mx, ma, a, l, pl.parts);
 }
 
 template <int NT, bool BF16>
@@ -950,36 +966,29 @@ static cudaError_t tiles(const AdapterArgs& a, const AdapterLists& l, const Adap
   p.n_tiles = (int)ceil_of(a.outer, NT);
   p.kblocks = (int)ceil_of(a.inner, kABK);
   p.splits = pl.splits;
-  p.parts = pl.parts;
   p.wide = a.outer % 16 == 0 && reinterpret_cast<uintptr_t>(a.y) % 32 == 0;
   const int64_t all = (int64_t)p.m_tiles * p.n_tiles * p.splits;
   const int64_t sms = sm_count() > 0 ? sm_count() : all;
-  e = launch_pdl(kern, dim3((unsigned)(all < sms ? all : sms)), dim3(kAdaptedThreads),
-                 adapted_smem_bytes<NT>(), s, mx, mw, p);
-  if (e != cudaSuccess || pl.splits == 1) return e;
-  const int64_t count = a.tokens * a.outer;
-  const int64_t blocks = ceil_of(count, 2048);
-  return launch_pdl(adapted_join_kernel<BF16>, dim3((unsigned)(blocks < 8 * sms ? blocks : 8 * sms)),
-                    dim3(256), 0, s, static_cast<const float*>(l.part), pl.splits, count, a.y);
+  return launch_clusters(kern, dim3((unsigned)(all < sms || p.splits > 1 ? all : sms)),
+                         dim3(kAdaptedThreads), adapted_smem_bytes<NT>(), s, p.splits, mx, mw, p);
 }
 
 template <bool BF16>
 static cudaError_t adapted(const AdapterArgs& a, uint8_t* ws, cudaStream_t s) {
   const AdapterPlan pl = plan_of(a.tokens, a.inner, a.outer);
-  const AdapterBytes by = bytes_of(a.tokens, a.outer, a.rank, pl);
+  const AdapterBytes by = bytes_of(a.tokens, a.rank);
   AdapterLists l;
   l.z = reinterpret_cast<float*>(ws);
+  l.z16 = reinterpret_cast<uint16_t*>(ws);
   l.count = reinterpret_cast<int32_t*>(ws + by.z);
   l.list = reinterpret_cast<int32_t*>(ws + by.z + by.count);
   l.place = ws + by.z + by.count + by.list;
-  l.part = reinterpret_cast<float*>(ws + by.z + by.count + by.list + by.place);
   const bool few = a.tokens <= kFewAdapted;
   cudaError_t e;
   if (a.tokens <= kDownTokens) {
-    const int lists = few ? 0 : (int)ceil_of(a.tokens, kABM);
-    e = a.rank <= 16   ? down<BF16, 1>(a, l, pl, lists, s)
-        : a.rank <= 32 ? down<BF16, 2>(a, l, pl, lists, s)
-                       : down<BF16, 4>(a, l, pl, lists, s);
+    e = a.rank <= 16   ? down<BF16, 1>(a, l, pl, few, s)
+        : a.rank <= 32 ? down<BF16, 2>(a, l, pl, few, s)
+                       : down<BF16, 4>(a, l, pl, few, s);
   } else {
     e = a.rank <= 16   ? down_tiles<16, BF16>(a, l, pl, s)
         : a.rank <= 32 ? down_tiles<32, BF16>(a, l, pl, s)
@@ -989,8 +998,9 @@ static cudaError_t adapted(const AdapterArgs& a, uint8_t* ws, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   if (few) {
     const dim3 grid((unsigned)ceil_of(a.outer, 16));
-    return a.tokens <= 8 ? launch_pdl(adapted_few_kernel<BF16, 1>, grid, dim3(256), 0, s, a, l, pl.parts)
-                         : launch_pdl(adapted_few_kernel<BF16, 2>, grid, dim3(256), 0, s, a, l, pl.parts);
+    return a.tokens <= 8    ? launch_pdl(adapted_few_kernel<BF16, 1>, grid, dim3(256), 0, s, a, l)
+           : a.tokens <= 16 ? launch_pdl(adapted_few_kernel<BF16, 2>, grid, dim3(256), 0, s, a, l)
+                            : launch_pdl(adapted_few_kernel<BF16, 4>, grid, dim3(256), 0, s, a, l);
   }
   switch (pl.nt) {
     case 256: return tiles<256, BF16>(a, l, pl, s);

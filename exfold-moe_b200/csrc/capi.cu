@@ -857,7 +857,7 @@ EXF_API int64_t exf_adapted_linear_workspace_bytes(int64_t tokens, int inner, in
   if (tokens < 0 || inner < 1 || outer < 1 || rank < 1 || rank > 128 ||
       adapted_too_large(tokens, inner, outer, 0))
     return -1;
-  return adapters_workspace(tokens, inner, outer, rank);
+  return adapters_workspace(tokens, rank);
 }
 
 EXF_API int exf_adapted_linear(const void* x, const void* w, const void* a, const void* b,
@@ -884,7 +884,7 @@ EXF_API int exf_adapted_linear(const void* x, const void* w, const void* a, cons
               "%s: the workspace must be 32-byte aligned", name);
   EXF_REQUIRE(reinterpret_cast<uintptr_t>(ids) % 4 == 0 && aligned_to(scaling, EXF_F32),
               "%s: a tensor is not aligned to its type", name);
-  const int64_t need = adapters_workspace(tokens, inner, outer, rank);
+  const int64_t need = adapters_workspace(tokens, rank);
   EXF_REQUIRE(workspace_bytes >= need, "%s: workspace of %lld bytes required", name,
               (long long)need);
   AdapterArgs p{x,     w,     a,     b,        ids,  scaling, dtype == EXF_BF16,

@@ -20,7 +20,7 @@ struct AdapterArgs {
   int32_t* status;
 };
 
-int64_t adapters_workspace(int64_t tokens, int inner, int outer, int rank);
+int64_t adapters_workspace(int64_t tokens, int rank);
 cudaError_t launch_adapters(const AdapterArgs& a, void* workspace, cudaStream_t s);
 
 }  // namespace exf

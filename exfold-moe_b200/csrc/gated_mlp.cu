@@ -503,10 +503,6 @@ struct PairSmem {
 };
 constexpr size_t pair_smem_bytes() { return sizeof(PairSmem) + 1024; }
 
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
-                   : "memory");
-}
 // the address of a shared object in the leader's CTA
 __device__ __forceinline__ uint32_t leader_addr(const void* p) {
   uint32_t a;
