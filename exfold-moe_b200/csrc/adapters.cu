@@ -8,8 +8,9 @@
 // z of that adapter's tokens (0 for the others) as the sum of two 16-bit terms (what one would round away is
 // in the other: 2^-16 of z in bf16), both against B.  So the adapters' part costs matrix instructions on
 // tiles that are there anyway, and y is written once, rounded once.  The GEMM starts on x and W while z is
-// still being computed.  Up to 32 tokens, where W's bytes are all that counts, a kernel of warp matrix
-// instructions reads W by every SM and adds z B in fp32.
+// still being computed.  Up to 128 tokens, where every token may have an adapter of its own, the GEMM's threads
+// add z B to its sums instead, a token's row from its own adapter, in fp32 (64 tokens of 32 adapters, rank 16:
+// as columns of the reduction 23.8 us); up to 32 tokens that follows a kernel of warp matrix instructions.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -26,7 +27,8 @@ namespace exf {
 using namespace tc;
 
 constexpr int kFewAdapted = 32;       // tokens of the kernel without tiles
-constexpr int kDownTokens = 256;      // tokens of adapter_down_kernel
+constexpr int kRowTokens = 128;       // tokens whose adapters are added row by row, z in fp32
+constexpr int kDownTokens = 1024;     // tokens of adapter_down_kernel
 constexpr int kAdaptedThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue, warps 6-9 adapters
 constexpr int kABM = 128;           // tokens of a tile
 constexpr int kABK = 64;            // columns of a stage: 128 bytes
@@ -36,7 +38,7 @@ struct AdapterPlan {
   int nt, splits;  // the GEMM's tile, and the blocks (a cluster) that share its reduction
 };
 
-// What the kernels hand on: z, for a few tokens fp32 [tokens][rank], else [tokens][ceil(rank / 16)][2][16], the
+// What the kernels hand on: z, up to kRowTokens tokens fp32 [tokens][rank], else [tokens][ceil(rank / 16)][2][16], the
 // two 16-bit terms of 16 ranks (zeros past the last); for each tile of 128 tokens its number of distinct
 // adapters and their ids, and for each token its place among them (255: none).
 struct AdapterLists {
@@ -156,7 +158,7 @@ __device__ __forceinline__ void write_list(const AdapterArgs& p, const AdapterLi
   if (threadIdx.x == 0) l.count[tile] = sm.count;
 }
 
-// ---- z of up to 256 tokens ----------------------------------------------------------------------------------
+// ---- z of up to 1024 tokens ----------------------------------------------------------------------------------
 // A block takes 8 tokens and one part of the reduction.  Its work is each distinct adapter's rows, 16 MB at a
 // time, against all 8 tokens (a token keeps its own adapter's column), in units of 32 columns, dealt out to
 // the 8 warps in equal runs: where every token has an adapter of its own, each warp streams one of them.  A
@@ -167,7 +169,7 @@ __device__ __forceinline__ void write_list(const AdapterArgs& p, const AdapterLi
 // adapters for the GEMM.
 template <bool BF16, int MB>
 __global__ void __launch_bounds__(256)
-    adapter_down_kernel(const AdapterArgs p, const AdapterLists l, bool few, int parts) {
+    adapter_down_kernel(const AdapterArgs p, const AdapterLists l, bool rows, int parts) {
   constexpr int TB = 8, R = 16 * MB;
   __shared__ float sums[8][TB][R + 1];
   __shared__ __align__(16) float joined[TB][R];
@@ -257,7 +259,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
         for (int j = 0; j < 8; ++j) z[j] *= scale;
       }
-      if (!few) {
+      if (!rows) {
         store_terms<BF16>(l, t0 + t, p.rank, r0 + r, z);
       } else if (r0 + r < p.rank) {
         float4* to = reinterpret_cast<float4*>(l.z + (int64_t)(t0 + t) * p.rank + r0 + r);
@@ -270,7 +272,7 @@ __global__ void __launch_bounds__(256)
     else
       __syncthreads();
   }
-  if (!few && part == 0 && t0 % 128 == 0) {
+  if (!rows && part == 0 && t0 % 128 == 0) {
     const int place = list_adapters(p, t0 / 128, tile);
     write_list(p, l, t0 / 128, tile, place);
   }
@@ -446,6 +448,36 @@ __global__ void __launch_bounds__(192, 1)
 }
 
 // ---- a few tokens -----------------------------------------------------------------------------------------
+// z B of a token for E features from n on, added to y
+template <bool BF16, int E>
+__device__ __forceinline__ void add_row(const AdapterArgs& p, const AdapterLists& l, int token, int n,
+                                        float (&y)[E]) {
+  const int id = p.ids[token];
+  if (id < 0 || id >= p.adapters) return;
+  const uint16_t* b = static_cast<const uint16_t*>(p.b) + ((int64_t)id * p.outer + n) * p.rank;
+  const float4* z = reinterpret_cast<const float4*>(l.z + (int64_t)token * p.rank);
+#pragma unroll 2
+  for (int r = 0; r < p.rank; r += 8) {
+    uint4 v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = load8(b + (int64_t)e * p.rank + r, true);
+    const float4 z0 = z[r / 4], z1 = z[r / 4 + 1];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float2 e0 = unpack2<BF16>(v[e].x), e1 = unpack2<BF16>(v[e].y),
+                   e2 = unpack2<BF16>(v[e].z), e3 = unpack2<BF16>(v[e].w);
+      y[e] = fmaf(z0.x, e0.x, y[e]);
+      y[e] = fmaf(z0.y, e0.y, y[e]);
+      y[e] = fmaf(z0.z, e1.x, y[e]);
+      y[e] = fmaf(z0.w, e1.y, y[e]);
+      y[e] = fmaf(z1.x, e2.x, y[e]);
+      y[e] = fmaf(z1.y, e2.y, y[e]);
+      y[e] = fmaf(z1.z, e3.x, y[e]);
+      y[e] = fmaf(z1.w, e3.y, y[e]);
+    }
+  }
+}
+
 // A block computes 16 features of up to 8 NB tokens, its 8 warps an eighth of the reduction each; then a
 // thread adds a feature's z B.  W is read ahead of the wait for z.
 template <bool BF16, int NB>
@@ -459,10 +491,11 @@ __global__ void __launch_bounds__(256)
   const uint16_t* x = static_cast<const uint16_t*>(p.x);
   const uint16_t* w = static_cast<const uint16_t*>(p.w);
   const int units = (p.inner + 31) / 32;
-  const int k0 = units * warp / 8 * 32, k1 = units * (warp + 1) / 8 * 32;
+  const int u0 = units * warp / 8, u1 = units * (warp + 1) / 8;
   float d[NB][4] = {};
 #pragma unroll 4
-  for (int k = k0 + 8 * c; k < k1 + 8 * c; k += 32) {
+  for (int u = u0; u < u1; ++u) {
+    const int k = u * 32 + 8 * c;
     const bool in = k < p.inner;
     const uint4 lo = load8(w + (int64_t)(n0 + g) * p.inner + k, in && n0 + g < p.outer);
     const uint4 hi = load8(w + (int64_t)(n0 + 8 + g) * p.inner + k, in && n0 + 8 + g < p.outer);
@@ -485,27 +518,11 @@ __global__ void __launch_bounds__(256)
   for (int i = threadIdx.x; i < TB * 16; i += 256) {
     const int t = i / 16, f = i % 16, n = n0 + f;
     if (t >= tokens || n >= p.outer) continue;
-    float y = 0.0f;
+    float y[1] = {0.0f};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) y += sums[k][t][f];
-    const int id = p.ids[t];
-    if (id >= 0 && id < p.adapters) {
-      const uint16_t* b = static_cast<const uint16_t*>(p.b) + ((int64_t)id * p.outer + n) * p.rank;
-      for (int r = 0; r < p.rank; r += 8) {
-        const uint4 v = load8(b + r, true);
-        const float4* at = reinterpret_cast<const float4*>(l.z + (int64_t)t * p.rank + r);
-        const float4 z0 = at[0], z1 = at[1];
-        const float z[8] = {z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w};
-        const uint32_t words[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 e = unpack2<BF16>(words[j]);
-          y = fmaf(z[2 * j], e.x, y);
-          y = fmaf(z[2 * j + 1], e.y, y);
-        }
-      }
-    }
-    static_cast<uint16_t*>(p.y)[(int64_t)t * p.outer + n] = (uint16_t)pack2<BF16>(y, 0.0f);
+    for (int k = 0; k < 8; ++k) y[0] += sums[k][t][f];
+    add_row<BF16, 1>(p, l, t, n, y);
+    static_cast<uint16_t*>(p.y)[(int64_t)t * p.outer + n] = (uint16_t)pack2<BF16>(y[0], 0.0f);
   }
 }
 
@@ -557,6 +574,7 @@ struct AdaptedGemm {
   AdapterArgs a;
   AdapterLists l;
   int m_tiles, n_tiles, kblocks, splits;
+  bool rows;  // the adapters are added row by row
   bool wide;  // y's rows are 32-byte aligned
 };
 
@@ -622,7 +640,7 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
   fence_after_sync();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // (with a split reduction, a tile's blocks are a cluster, and have one tile each)
+  // (with a split reduction, a tile's blocks are a cluster, and have one tile each; with rows too)
   const int ntiles = p.m_tiles * p.n_tiles * p.splits;
   const int width = (p.a.rank + 15) / 16;  // stages that an adapter adds
   // tile t: reduction part, M tile, N tile, k blocks [kb0, kb1)
@@ -641,7 +659,7 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
   };
   // its adapters' stages [q0, q1), read behind the wait for adapter_down_kernel
   auto extra_of = [&](const Tile& tl, int& q0, int& q1) {
-    const int all = uniform(p.l.count[tl.mt]) * width;
+    const int all = p.rows ? 0 : uniform(p.l.count[tl.mt]) * width;
     q0 = all * tl.part / p.splits;
     q1 = all * (tl.part + 1) / p.splits;
   };
@@ -754,7 +772,7 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
         const int col = tl.nt * NT + c;
         if (row < p.a.tokens) {
           if (broken) add_broken<BF16>(p, row, tl.mt, col, q0, q1, v);
-          if (p.splits > 1) {
+          if (p.splits > 1 || p.rows) {
             // (every copy into the tiles has been multiplied: they hold the sums)
             float* at = reinterpret_cast<float*>(sm.tiles) + (q * 32 + lane) * (NT + 4) + c;
 #pragma unroll
@@ -805,6 +823,7 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
       const Tile tl = tile_of(t);
       int q0, q1;
       extra_of(tl, q0, q1);
+      if (q0 == q1) continue;
       const int token = tl.mt * kABM + tid;
       const int place = token < tokens ? p.l.place[token] : 255;
       const uint16_t* z = p.l.z16 + (int64_t)(token < tokens ? token : 0) * width * 32;
@@ -851,9 +870,10 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
     tmem_free(tmem, C::kTmem);
   }
   if (threadIdx.x == 0 && sm.failed && p.a.status) atomicExch(p.a.status, 1);
-  if (p.splits == 1) return;
+  if (p.splits == 1 && !p.rows) return;
   // the cluster's sums of this tile: eight features a thread, dealt out to its blocks
-  cluster_sync();
+  if (p.splits > 1) cluster_sync();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const Tile tl = tile_of(blockIdx.x);
   const float* sums = reinterpret_cast<const float*>(sm.tiles);
   const int left = (int)p.a.tokens - tl.mt * kABM, rows = left < kABM ? left : kABM;
@@ -863,9 +883,10 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
     if (col >= p.a.outer) continue;
     float v[8];
     add_peers(sums + m * (NT + 4) + c, p.splits, v);
+    if (p.rows) add_row<BF16, 8>(p.a, p.l, tl.mt * kABM + m, col, v);
     store_16b<BF16>(p.a.y, (int64_t)(tl.mt * kABM + m) * p.a.outer + col, v);
   }
-  cluster_sync();  // (no block leaves while its sums are read)
+  if (p.splits > 1) cluster_sync();  // (no block leaves while its sums are read)
 }
 
 // ---- host side ----------------------------------------------------------------------------------
@@ -906,7 +927,7 @@ struct AdapterBytes {
 static AdapterBytes bytes_of(int64_t tokens, int rank) {
   AdapterBytes b;
   const int64_t tiles = ceil_of(tokens, kABM);
-  const bool few = tokens <= kFewAdapted;
+  const bool few = tokens <= kRowTokens;
   b.z = up_256(few ? tokens * rank * 4 : tokens * ceil_of(rank, 16) * 64);
   b.count = few ? 0 : up_256(tiles * 4);
   b.list = few ? 0 : up_256(tiles * 128 * 4);
@@ -920,11 +941,15 @@ int64_t adapters_workspace(int64_t tokens, int rank) {
 }
 
 template <bool BF16, int MB>
-static cudaError_t down(const AdapterArgs& a, const AdapterLists& l, const AdapterPlan& pl, bool few,
+static cudaError_t down(const AdapterArgs& a, const AdapterLists& l, const AdapterPlan& pl, bool rows,
                         cudaStream_t s) {
-  return launch_clusters(adapter_down_kernel<BF16, MB>,
-                         dim3((unsigned)(ceil_of(a.tokens, 8) * pl.parts)), dim3(256), 0, s, pl.parts,
-                         a, l, few, pl.parts);
+  auto* kern = adapter_down_kernel<BF16, MB>;
+  static std::mutex mu;
+  static bool done[64] = {};
+  const cudaError_t e = prefer_smem(kern, mu, done);
+  if (e != cudaSuccess) return e;
+  return launch_clusters(kern, dim3((unsigned)(ceil_of(a.tokens, 8) * pl.parts)), dim3(256), 0, s,
+                         pl.parts, a, l, rows, pl.parts);
 }
 template <int RN, bool BF16>
 static cudaError_t down_tiles(const AdapterArgs& a, const AdapterLists& l, const AdapterPlan& pl,
@@ -966,10 +991,11 @@ static cudaError_t tiles(const AdapterArgs& a, const AdapterLists& l, const Adap
   p.n_tiles = (int)ceil_of(a.outer, NT);
   p.kblocks = (int)ceil_of(a.inner, kABK);
   p.splits = pl.splits;
+  p.rows = a.tokens <= kRowTokens;
   p.wide = a.outer % 16 == 0 && reinterpret_cast<uintptr_t>(a.y) % 32 == 0;
   const int64_t all = (int64_t)p.m_tiles * p.n_tiles * p.splits;
   const int64_t sms = sm_count() > 0 ? sm_count() : all;
-  return launch_clusters(kern, dim3((unsigned)(all < sms || p.splits > 1 ? all : sms)),
+  return launch_clusters(kern, dim3((unsigned)(all < sms || p.splits > 1 || p.rows ? all : sms)),
                          dim3(kAdaptedThreads), adapted_smem_bytes<NT>(), s, p.splits, mx, mw, p);
 }
 
@@ -983,12 +1009,12 @@ static cudaError_t adapted(const AdapterArgs& a, uint8_t* ws, cudaStream_t s) {
   l.count = reinterpret_cast<int32_t*>(ws + by.z);
   l.list = reinterpret_cast<int32_t*>(ws + by.z + by.count);
   l.place = ws + by.z + by.count + by.list;
-  const bool few = a.tokens <= kFewAdapted;
+  const bool few = a.tokens <= kFewAdapted, rows = a.tokens <= kRowTokens;
   cudaError_t e;
   if (a.tokens <= kDownTokens) {
-    e = a.rank <= 16   ? down<BF16, 1>(a, l, pl, few, s)
-        : a.rank <= 32 ? down<BF16, 2>(a, l, pl, few, s)
-                       : down<BF16, 4>(a, l, pl, few, s);
+    e = a.rank <= 16   ? down<BF16, 1>(a, l, pl, rows, s)
+        : a.rank <= 32 ? down<BF16, 2>(a, l, pl, rows, s)
+                       : down<BF16, 4>(a, l, pl, rows, s);
   } else {
     e = a.rank <= 16   ? down_tiles<16, BF16>(a, l, pl, s)
         : a.rank <= 32 ? down_tiles<32, BF16>(a, l, pl, s)
@@ -997,10 +1023,12 @@ static cudaError_t adapted(const AdapterArgs& a, uint8_t* ws, cudaStream_t s) {
   }
   if (e != cudaSuccess) return e;
   if (few) {
-    const dim3 grid((unsigned)ceil_of(a.outer, 16));
-    return a.tokens <= 8    ? launch_pdl(adapted_few_kernel<BF16, 1>, grid, dim3(256), 0, s, a, l)
-           : a.tokens <= 16 ? launch_pdl(adapted_few_kernel<BF16, 2>, grid, dim3(256), 0, s, a, l)
-                            : launch_pdl(adapted_few_kernel<BF16, 4>, grid, dim3(256), 0, s, a, l);
+    auto go = [&](auto* kern) {
+      return launch_pdl(kern, dim3((unsigned)ceil_of(a.outer, 16)), dim3(256), 0, s, a, l);
+    };
+    return a.tokens <= 8    ? go(adapted_few_kernel<BF16, 1>)
+           : a.tokens <= 16 ? go(adapted_few_kernel<BF16, 2>)
+                            : go(adapted_few_kernel<BF16, 4>);
   }
   switch (pl.nt) {
     case 256: return tiles<256, BF16>(a, l, pl, s);

@@ -3,7 +3,7 @@
 Bounds are derived, element by element.  With u = eps / 2 of the type and t(n) = n 2^-23 (a sum of n fp32
 terms, each addition off by at most a unit in the last place, with products exact):
   |dz| <= (t(K) + 2^-23) s |x| |A|^T + (u^2 + t(8)) |z|  (the scaling's product, two terms of the type
-    above 32 tokens, parts joined), and half of fp16's smallest subnormal
+    above 128 tokens, parts joined), and half of fp16's smallest subnormal
   |dy| <= t(K + 2 rank) (|x| |W|^T + |z| |B|^T) + |dz| |B|^T + u |y|
 A result below the type's smallest normal is off by at most half its smallest subnormal.
 """
