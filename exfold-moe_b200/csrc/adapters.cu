@@ -34,6 +34,7 @@ constexpr int kABM = 128;           // tokens of a tile
 constexpr int kABK = 64;            // columns of a stage: 128 bytes
 
 struct AdapterPlan {
+  int take;        // tokens a block of adapter_down_kernel
   int parts;       // blocks (a cluster) among which z's reduction is divided
   int nt, splits;  // the GEMM's tile, and the blocks (a cluster) that share its reduction
 };
@@ -159,8 +160,8 @@ __device__ __forceinline__ void write_list(const AdapterArgs& p, const AdapterLi
 }
 
 // ---- z of up to 1024 tokens ----------------------------------------------------------------------------------
-// A block takes 8 tokens and one part of the reduction.  Its work is each distinct adapter's rows, 16 MB at a
-// time, against all 8 tokens (a token keeps its own adapter's column), in units of 32 columns, dealt out to
+// A block takes 4 or 8 tokens and one part of the reduction.  Its work is each distinct adapter's rows, 16 MB at a
+// time, against all of them (a token keeps its own adapter's column), in units of 32 columns, dealt out to
 // the 8 warps in equal runs: where every token has an adapter of its own, each warp streams one of them.  A
 // lane loads 8 columns (16 bytes) of a row, and the instruction's 16 columns are taken as words 0, 1 and then
 // 2, 3 of each: the order of a sum is free as long as both operands have the same.  (All warps on one
@@ -169,7 +170,7 @@ __device__ __forceinline__ void write_list(const AdapterArgs& p, const AdapterLi
 // adapters for the GEMM.
 template <bool BF16, int MB>
 __global__ void __launch_bounds__(256)
-    adapter_down_kernel(const AdapterArgs p, const AdapterLists l, bool rows, int parts) {
+    adapter_down_kernel(const AdapterArgs p, const AdapterLists l, bool rows, int parts, int take) {
   constexpr int TB = 8, R = 16 * MB;
   __shared__ float sums[8][TB][R + 1];
   __shared__ __align__(16) float joined[TB][R];
@@ -178,9 +179,9 @@ __global__ void __launch_bounds__(256)
   // (only now: the GEMM reads x before it waits for this kernel)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tokens = (int)p.tokens;
 
-  const int part = parts > 1 ? cluster_rank() : 0, t0 = blockIdx.x / parts * TB;
+  const int part = parts > 1 ? cluster_rank() : 0, t0 = blockIdx.x / parts * take;
+  const int tokens = (int)p.tokens < t0 + take ? (int)p.tokens : t0 + take;  // (up to here)
   const int all = (p.inner + 31) / 32;
   const int u0 = all * part / parts, units = all * (part + 1) / parts - u0;
   int mine = lane < TB && t0 + lane < tokens ? p.ids[t0 + lane] : -1;
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(256)
       const uint16_t* a = static_cast<const uint16_t*>(p.a) + ((int64_t)id * p.rank + r0) * p.inner;
       const int b0 = n == first ? i0 - n * units : 0, b1 = n == last - 1 ? i1 - n * units : units;
       float d[MB][4] = {};
-#pragma unroll(MB == 4 ? 2 : 4)
+#pragma unroll(MB == 4 ? 3 : 4)
       for (int u = b0; u < b1; ++u) {
         const int k = (u0 + u) * 32 + 8 * c;
         const bool in = k < p.inner;
@@ -448,34 +449,19 @@ __global__ void __launch_bounds__(192, 1)
 }
 
 // ---- a few tokens -----------------------------------------------------------------------------------------
-// z B of a token for E features from n on, added to y
-template <bool BF16, int E>
-__device__ __forceinline__ void add_row(const AdapterArgs& p, const AdapterLists& l, int token, int n,
-                                        float (&y)[E]) {
-  const int id = p.ids[token];
-  if (id < 0 || id >= p.adapters) return;
-  const uint16_t* b = static_cast<const uint16_t*>(p.b) + ((int64_t)id * p.outer + n) * p.rank;
-  const float4* z = reinterpret_cast<const float4*>(l.z + (int64_t)token * p.rank);
-#pragma unroll 2
-  for (int r = 0; r < p.rank; r += 8) {
-    uint4 v[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = load8(b + (int64_t)e * p.rank + r, true);
-    const float4 z0 = z[r / 4], z1 = z[r / 4 + 1];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float2 e0 = unpack2<BF16>(v[e].x), e1 = unpack2<BF16>(v[e].y),
-                   e2 = unpack2<BF16>(v[e].z), e3 = unpack2<BF16>(v[e].w);
-      y[e] = fmaf(z0.x, e0.x, y[e]);
-      y[e] = fmaf(z0.y, e0.y, y[e]);
-      y[e] = fmaf(z0.z, e1.x, y[e]);
-      y[e] = fmaf(z0.w, e1.y, y[e]);
-      y[e] = fmaf(z1.x, e2.x, y[e]);
-      y[e] = fmaf(z1.y, e2.y, y[e]);
-      y[e] = fmaf(z1.z, e3.x, y[e]);
-      y[e] = fmaf(z1.w, e3.y, y[e]);
-    }
-  }
+// z B of eight ranks
+template <bool BF16>
+__device__ __forceinline__ float dot8(const float4& z0, const float4& z1, const uint4& v, float y) {
+  const float2 e0 = unpack2<BF16>(v.x), e1 = unpack2<BF16>(v.y), e2 = unpack2<BF16>(v.z),
+               e3 = unpack2<BF16>(v.w);
+  y = fmaf(z0.x, e0.x, y);
+  y = fmaf(z0.y, e0.y, y);
+  y = fmaf(z0.z, e1.x, y);
+  y = fmaf(z0.w, e1.y, y);
+  y = fmaf(z1.x, e2.x, y);
+  y = fmaf(z1.y, e2.y, y);
+  y = fmaf(z1.z, e3.x, y);
+  return fmaf(z1.w, e3.y, y);
 }
 
 // A block computes 16 features of up to 8 NB tokens, its 8 warps an eighth of the reduction each; then a
@@ -518,11 +504,18 @@ __global__ void __launch_bounds__(256)
   for (int i = threadIdx.x; i < TB * 16; i += 256) {
     const int t = i / 16, f = i % 16, n = n0 + f;
     if (t >= tokens || n >= p.outer) continue;
-    float y[1] = {0.0f};
+    float y = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) y[0] += sums[k][t][f];
-    add_row<BF16, 1>(p, l, t, n, y);
-    static_cast<uint16_t*>(p.y)[(int64_t)t * p.outer + n] = (uint16_t)pack2<BF16>(y[0], 0.0f);
+    for (int k = 0; k < 8; ++k) y += sums[k][t][f];
+    const int id = p.ids[t];
+    if (id >= 0 && id < p.adapters) {
+      const uint16_t* b = static_cast<const uint16_t*>(p.b) + ((int64_t)id * p.outer + n) * p.rank;
+      const float4* z = reinterpret_cast<const float4*>(l.z + (int64_t)t * p.rank);
+#pragma unroll 4
+      for (int r = 0; r < p.rank; r += 8)
+        y = dot8<BF16>(z[r / 4], z[r / 4 + 1], load8(b + r, true), y);
+    }
+    static_cast<uint16_t*>(p.y)[(int64_t)t * p.outer + n] = (uint16_t)pack2<BF16>(y, 0.0f);
   }
 }
 
@@ -601,6 +594,53 @@ __device__ __noinline__ void add_broken(const AdaptedGemm& p, int token, int mt,
 #pragma unroll
       for (int r = 0; r < 8; ++r) v[j] = fmaf(z[r], unpack2<BF16>(b[r]).x, v[j]);
     }
+  }
+}
+
+// A token's NT features by a warp: the sums at `at` and z B.  The ranks of a feature lie on LANES neighbouring
+// lanes, eight each, so that a load of the warp is one stretch of B and z stays in registers; 32 features at a
+// time, whose parts are exchanged so that each lane ends with a feature of its own.  (Eight features a thread,
+// each with all of its ranks: 30 of 52 us at 128 tokens of rank 64.)
+template <int NT, bool BF16, int LANES>
+__device__ __forceinline__ void add_row(const AdaptedGemm& p, int token, int col, const float* at,
+                                        int lane) {
+  const int rank = p.a.rank, outer = p.a.outer;
+  const int piece = lane % LANES, f0 = lane / LANES;
+  constexpr int kStep = 32 / LANES;
+  const int id = p.a.ids[token];
+  const bool any = id >= 0 && id < p.a.adapters, mine = any && 8 * piece < rank;
+  float4 z0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), z1 = z0;
+  if (mine) {
+    const float4* z = reinterpret_cast<const float4*>(p.l.z + (int64_t)token * rank + 8 * piece);
+    z0 = z[0];
+    z1 = z[1];
+  }
+  const uint16_t* b = static_cast<const uint16_t*>(p.a.b) +
+                      ((int64_t)(any ? id : 0) * outer + col) * rank + 8 * piece;
+  uint16_t* y = static_cast<uint16_t*>(p.a.y) + (int64_t)token * outer + col;
+#pragma unroll 2
+  for (int g = 0; g < NT; g += 32) {
+    float e[LANES] = {};
+    if (any) {
+      uint4 v[LANES];
+#pragma unroll
+      for (int i = 0; i < LANES; ++i) {
+        const int f = g + i * kStep + f0;
+        v[i] = load8(b + (int64_t)f * rank, mine && col + f < outer);
+      }
+#pragma unroll
+      for (int i = 0; i < LANES; ++i) e[i] = dot8<BF16>(z0, z1, v[i], 0.0f);
+#pragma unroll
+      for (int d = LANES / 2; d > 0; d >>= 1)
+#pragma unroll
+        for (int i = 0; i < d; ++i) {
+          const bool upper = piece & d;
+          const float keep = upper ? e[i + d] : e[i], send = upper ? e[i] : e[i + d];
+          e[i] = keep + __shfl_xor_sync(0xffffffffu, send, d);
+        }
+    }
+    const int f = g + piece * kStep + f0;
+    if (col + f < outer) y[f] = (uint16_t)pack2<BF16>(at[f] + e[0], 0.0f);
   }
 }
 
@@ -864,29 +904,55 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
   }
   fence_before_sync();
   __syncthreads();
+  if (p.splits > 1 || p.rows) {
+    // the cluster's sums of this tile
+    if (p.splits > 1) cluster_sync();
+    const Tile tl = tile_of(blockIdx.x);
+    float* sums = reinterpret_cast<float*>(sm.tiles);
+    const int left = (int)p.a.tokens - tl.mt * kABM, rows = left < kABM ? left : kABM;
+    // eight features a thread, the tokens dealt out to the cluster's blocks; for rows into this block's memory
+    float* own = p.splits > 1 ? sums + kABM * (NT + 4) : sums;
+    if (p.splits > 1)
+      for (int e = threadIdx.x; e < (kABM + p.splits - 1) / p.splits * (NT / 8);
+           e += kAdaptedThreads) {
+        const int m = e / (NT / 8) * p.splits + tl.part, c = e % (NT / 8) * 8, col = tl.nt * NT + c;
+        if (m >= rows || col >= p.a.outer) continue;
+        float v[8];
+        add_peers(sums + m * (NT + 4) + c, p.splits, v);
+        if (p.rows) {
+          float4* to = reinterpret_cast<float4*>(own + m / p.splits * (NT + 4) + c);
+          to[0] = make_float4(v[0], v[1], v[2], v[3]);
+          to[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+          store_16b<BF16>(p.a.y, (int64_t)(tl.mt * kABM + m) * p.a.outer + col, v);
+        }
+      }
+    if (p.rows) {
+      if (p.splits > 1) __syncthreads();
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      for (int i = warp; i * p.splits + tl.part < rows; i += kAdaptedThreads / 32) {
+        const int token = tl.mt * kABM + i * p.splits + tl.part, col = tl.nt * NT;
+        const float* at = own + i * (NT + 4);
+        if (p.a.rank <= 8)
+          add_row<NT, BF16, 1>(p, token, col, at, lane);
+        else if (p.a.rank <= 16)
+          add_row<NT, BF16, 2>(p, token, col, at, lane);
+        else if (p.a.rank <= 32)
+          add_row<NT, BF16, 4>(p, token, col, at, lane);
+        else if (p.a.rank <= 64)
+          add_row<NT, BF16, 8>(p, token, col, at, lane);
+        else
+          add_row<NT, BF16, 16>(p, token, col, at, lane);
+      }
+    }
+    if (p.splits > 1) cluster_sync();  // (no block leaves while its sums are read)
+  }
   if (warp == 1) {
     __syncwarp();
     fence_after_sync();
     tmem_free(tmem, C::kTmem);
   }
   if (threadIdx.x == 0 && sm.failed && p.a.status) atomicExch(p.a.status, 1);
-  if (p.splits == 1 && !p.rows) return;
-  // the cluster's sums of this tile: eight features a thread, dealt out to its blocks
-  if (p.splits > 1) cluster_sync();
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Tile tl = tile_of(blockIdx.x);
-  const float* sums = reinterpret_cast<const float*>(sm.tiles);
-  const int left = (int)p.a.tokens - tl.mt * kABM, rows = left < kABM ? left : kABM;
-  for (int e = tl.part * kAdaptedThreads + threadIdx.x; e < rows * (NT / 8);
-       e += p.splits * kAdaptedThreads) {
-    const int m = e / (NT / 8), c = e % (NT / 8) * 8, col = tl.nt * NT + c;
-    if (col >= p.a.outer) continue;
-    float v[8];
-    add_peers(sums + m * (NT + 4) + c, p.splits, v);
-    if (p.rows) add_row<BF16, 8>(p.a, p.l, tl.mt * kABM + m, col, v);
-    store_16b<BF16>(p.a.y, (int64_t)(tl.mt * kABM + m) * p.a.outer + col, v);
-  }
-  if (p.splits > 1) cluster_sync();  // (no block leaves while its sums are read)
 }
 
 // ---- host side ----------------------------------------------------------------------------------
@@ -900,7 +966,9 @@ static AdapterPlan plan_of(int64_t tokens, int inner, int outer) {
   const int64_t sms = sm_count() > 0 ? sm_count() : 1;
   AdapterPlan pl;
   const bool few = tokens <= kDownTokens;
-  const int64_t blocks = ceil_of(tokens, few ? 8 : kABM);
+  // (4 tokens a block while two blocks of those fit an SM)
+  pl.take = tokens <= sms ? 4 : 8;
+  const int64_t blocks = ceil_of(tokens, few ? pl.take : kABM);
   int64_t parts = (few ? 2 : 1) * sms / blocks;
   if (parts > ceil_of(inner, 256)) parts = ceil_of(inner, 256);
   pl.parts = (int)(parts < 1 ? 1 : parts > kMostParts ? kMostParts : parts);
@@ -948,8 +1016,8 @@ static cudaError_t down(const AdapterArgs& a, const AdapterLists& l, const Adapt
   static bool done[64] = {};
   const cudaError_t e = prefer_smem(kern, mu, done);
   if (e != cudaSuccess) return e;
-  return launch_clusters(kern, dim3((unsigned)(ceil_of(a.tokens, 8) * pl.parts)), dim3(256), 0, s,
-                         pl.parts, a, l, rows, pl.parts);
+  return launch_clusters(kern, dim3((unsigned)(ceil_of(a.tokens, pl.take) * pl.parts)), dim3(256), 0,
+                         s, pl.parts, a, l, rows, pl.parts, pl.take);
 }
 template <int RN, bool BF16>
 static cudaError_t down_tiles(const AdapterArgs& a, const AdapterLists& l, const AdapterPlan& pl,

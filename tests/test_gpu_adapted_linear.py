@@ -91,6 +91,8 @@ SHAPES = [
     (300, 72, 5000, 4, 64), (1000, 2056, 2056, 6, 16), (1500, 136, 4104, 9, 112),
     (2500, 520, 4096, 12, 64), (4200, 256, 2048, 40, 8), (300, 2048, 264, 300, 16),
     (700, 4104, 264, 2, 128), (520, 776, 136, 3, 96), (260, 8, 8, 2, 8),
+    # reductions among 3, 5, 6 and 7 blocks
+    (128, 1544, 264, 6, 32), (127, 2568, 136, 6, 48), (256, 3112, 136, 3, 16), (128, 3592, 72, 128, 8),
 ]
 
 
