@@ -602,12 +602,11 @@ __device__ __noinline__ void add_broken(const AdaptedGemm& p, int token, int mt,
 // time, whose parts are exchanged so that each lane ends with a feature of its own.  (Eight features a thread,
 // each with all of its ranks: 30 of 52 us at 128 tokens of rank 64.)
 template <int NT, bool BF16, int LANES>
-__device__ __forceinline__ void add_row(const AdaptedGemm& p, int token, int col, const float* at,
-                                        int lane) {
+__device__ __forceinline__ void add_row(const AdaptedGemm& p, int id, int token, int col,
+                                        const float* at, int lane) {
   const int rank = p.a.rank, outer = p.a.outer;
   const int piece = lane % LANES, f0 = lane / LANES;
   constexpr int kStep = 32 / LANES;
-  const int id = p.a.ids[token];
   const bool any = id >= 0 && id < p.a.adapters, mine = any && 8 * piece < rank;
   float4 z0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), z1 = z0;
   if (mine) {
@@ -618,7 +617,7 @@ __device__ __forceinline__ void add_row(const AdaptedGemm& p, int token, int col
   const uint16_t* b = static_cast<const uint16_t*>(p.a.b) +
                       ((int64_t)(any ? id : 0) * outer + col) * rank + 8 * piece;
   uint16_t* y = static_cast<uint16_t*>(p.a.y) + (int64_t)token * outer + col;
-#pragma unroll 2
+#pragma unroll(LANES <= 4 ? 4 : 2)
   for (int g = 0; g < NT; g += 32) {
     float e[LANES] = {};
     if (any) {
@@ -777,7 +776,7 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
         }
         extras(k + 1);
       }
-      if (ok && i == 0) {
+      if (ok && i == 0 && !p.rows) {
         asm volatile("griddepcontrol.wait;" ::: "memory");
         extra_of(tl, q0, q1);
         due = 0;
@@ -789,8 +788,8 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
     if (elect_one()) mma_commit(&sm.drain);
     mbar_wait_drain(&sm.drain, 0);
   } else if (warp < 6) {
-    // ---- epilogue: one token per thread
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // ---- epilogue: one token per thread (with rows nothing before the cluster's sums waits for z)
+    if (!p.rows) asm volatile("griddepcontrol.wait;" ::: "memory");
     const int q = warp & 3;
     const int outer = p.a.outer;
     int i = 0;
@@ -831,7 +830,7 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.acc_empty[b]);
     }
-  } else {
+  } else if (!p.rows) {
     // ---- the adapters' stages: a thread copies one of the tile's tokens' z and every 128th feature's B
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x - 192;
@@ -863,7 +862,6 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
       const Tile tl = tile_of(t);
       int q0, q1;
       extra_of(tl, q0, q1);
-      if (q0 == q1) continue;
       const int token = tl.mt * kABM + tid;
       const int place = token < tokens ? p.l.place[token] : 255;
       const uint16_t* z = p.l.z16 + (int64_t)(token < tokens ? token : 0) * width * 32;
@@ -929,20 +927,25 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
       }
     if (p.rows) {
       if (p.splits > 1) __syncthreads();
+      // (z's kernel ran after whatever wrote the ids)
+      const int mine = tl.mt * kABM + (warp + kAdaptedThreads / 32 * lane) * p.splits + tl.part;
+      const int ids = mine < p.a.tokens ? p.a.ids[mine] : -1;  // lane j: of the warp's j-th token
       asm volatile("griddepcontrol.wait;" ::: "memory");
-      for (int i = warp; i * p.splits + tl.part < rows; i += kAdaptedThreads / 32) {
+      int turn = 0;
+      for (int i = warp; i * p.splits + tl.part < rows; i += kAdaptedThreads / 32, ++turn) {
         const int token = tl.mt * kABM + i * p.splits + tl.part, col = tl.nt * NT;
+        const int id = __shfl_sync(0xffffffffu, ids, turn);
         const float* at = own + i * (NT + 4);
         if (p.a.rank <= 8)
-          add_row<NT, BF16, 1>(p, token, col, at, lane);
+          add_row<NT, BF16, 1>(p, id, token, col, at, lane);
         else if (p.a.rank <= 16)
-          add_row<NT, BF16, 2>(p, token, col, at, lane);
+          add_row<NT, BF16, 2>(p, id, token, col, at, lane);
         else if (p.a.rank <= 32)
-          add_row<NT, BF16, 4>(p, token, col, at, lane);
+          add_row<NT, BF16, 4>(p, id, token, col, at, lane);
         else if (p.a.rank <= 64)
-          add_row<NT, BF16, 8>(p, token, col, at, lane);
+          add_row<NT, BF16, 8>(p, id, token, col, at, lane);
         else
-          add_row<NT, BF16, 16>(p, token, col, at, lane);
+          add_row<NT, BF16, 16>(p, id, token, col, at, lane);
       }
     }
     if (p.splits > 1) cluster_sync();  // (no block leaves while its sums are read)

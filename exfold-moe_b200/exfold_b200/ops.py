@@ -38,7 +38,7 @@ _HERE = contextlib.nullcontext()
 
 def _on(device: torch.device):
     """Makes `device` current for a launch (nothing to do, and nothing spent, where it is)."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _require_cuda(*tensors: torch.Tensor | None) -> torch.device:
