@@ -687,10 +687,10 @@ def _norm_backward(ctx, dy, ds):
     rows, weight = _rows(x, cols), weight.contiguous()
     dev, dtype, n = x.device, x.dtype, rows.shape[0]
     want_x, want_r, want_w, _ = ctx.needs_input_grad
-    dx = torch.empty(x.shape, dtype=dtype, device=dev) if want_x or want_r else None
+    dx = torch.empty(ctx.shape, dtype=dtype, device=dev) if want_x or want_r else None
     dw = torch.empty_like(weight) if want_w else None
     # (of s alone, where y was not used)
-    dy = torch.zeros(x.shape, dtype=dtype, device=dev) if dy is None else dy.contiguous()
+    dy = torch.zeros(ctx.shape, dtype=dtype, device=dev) if dy is None else dy.contiguous()
     ds = None if ds is None else ds.contiguous()
     lib = L.lib()
     with _on(dev):
@@ -716,7 +716,7 @@ class _RmsNorm(torch.autograd.Function):
         y, s, rows = _norm_forward(x, residual, weight, eps)
         copied = rows.data_ptr() != x.data_ptr()
         ctx.save_for_backward((rows if copied else x) if s is None else s, weight)
-        ctx.eps = eps
+        ctx.eps, ctx.shape = eps, x.shape
         ctx.set_materialize_grads(False)
         return y if s is None else (y, s)
 

@@ -164,6 +164,16 @@ def test_shapes_strides_and_partial_gradients():
     g, = torch.autograd.grad(y, a, dy)
     want, bound = formulas(s.detach(), w, dy, None, 1e-6)
     near(g, want[1], bound[1])
+    # memory in other orders, recorded: the gradient has the input's shape
+    a = x.view(4, 6, 256).transpose(0, 1).requires_grad_(True)
+    y = ops.rms_norm(a, w)
+    assert torch.equal(y.detach(), ops.rms_norm(x, w).view(4, 6, 256).transpose(0, 1))
+    g, gw = torch.autograd.grad(y, (a, w.requires_grad_(True)), dy.view(4, 6, 256).transpose(0, 1),
+                                allow_unused=True)
+    w = w.detach()
+    assert g.shape == a.shape and gw is None
+    want, bound = formulas(x, w, dy, None, 1e-6)
+    near(g.transpose(0, 1).reshape(24, 256), want[1], bound[1])
     # an upstream gradient that is one value for all
     a = x.clone().requires_grad_(True)
     ops.rms_norm(a, w).sum().backward()
