@@ -6,6 +6,8 @@ Each csrc/*.cu is compiled by nvcc (-gencode arch=compute_100a,code=sm_100a, -O3
 no fast-math, --fmad=false so every float operation is the one written) into
 exfold-moe_b200/_build/, then linked into exfold-moe_b200/lib/libexfold_b200.so with the CUDA
 runtime linked statically.  Objects are rebuilt only when a source or header is newer.
+binding/torch_ops.cpp (host code: autograd nodes over the C ABI) is compiled by g++ against the
+installed torch into lib/libexfold_b200_torch.so.
 """
 
 from __future__ import annotations
@@ -23,6 +25,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "lib" / "libexfold_b200.so"
+TORCH_SRC = PKG / "binding" / "torch_ops.cpp"
+TORCH_LIB = PKG / "lib" / "libexfold_b200_torch.so"
 INCLUDE = ROOT / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -49,6 +53,19 @@ def _stale(out: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def torch_command() -> list[str]:
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    libs = Path(torch.__file__).parent / "lib"
+    cuda = Path(nvcc()).resolve().parent.parent / "include"
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+            "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+            f"-I{INCLUDE}", *(arg for p in include_paths() for arg in ("-isystem", p)), "-isystem",
+            str(cuda), str(TORCH_SRC), "-o", str(TORCH_LIB), f"-L{libs}", "-ltorch_cpu",
+            "-ltorch_cuda", "-lc10", "-lc10_cuda", "-ldl", f"-Wl,-rpath,{libs}"]
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
     OBJ.mkdir(parents=True, exist_ok=True)
     LIB.parent.mkdir(parents=True, exist_ok=True)
@@ -63,21 +80,29 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
             if ptxas_info:
                 cmd += ["-Xptxas", "-v"]
             jobs.append(cmd)
+    if force or _stale(TORCH_LIB, [TORCH_SRC, *INCLUDE.glob("*.h")]):
+        jobs.append(torch_command())
 
     def run(cmd):
         if verbose:
             print(" ".join(cmd), flush=True)
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
-            raise RuntimeError(f"nvcc failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+            raise RuntimeError(f"build step failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
         if verbose or ptxas_info:
             sys.stdout.write(res.stdout + res.stderr)
         return res
 
     with ThreadPoolExecutor(max_workers=max(1, min(len(jobs), os.cpu_count() or 1))) as ex:
         list(ex.map(run, jobs))
+    # (a compiler that links its own libstdc++ into the binding would make exceptions of two kinds)
+    if "libstdc++.so" not in subprocess.run(["ldd", str(TORCH_LIB)], capture_output=True,
+                                            text=True).stdout:
+        TORCH_LIB.unlink()
+        raise RuntimeError("the torch binding was not linked against the shared libstdc++: use a g++ "
+                           "that does")
     objs = [OBJ / (s.stem + ".o") for s in sources]
-    if force or jobs or _stale(LIB, objs):
+    if force or _stale(LIB, objs):
         run([nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", str(LIB), *map(str, objs)])
     return LIB
 

@@ -120,6 +120,29 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_torch_ops = None
+
+
+def torch_ops():
+    """The operators of libexfold_b200_torch.so, beside the library (RuntimeError if it has not been
+    built)."""
+    global _torch_ops
+    if _torch_ops is None:
+        lib()
+        import torch
+
+        with _lock:
+            if _torch_ops is None:
+                path = DEFAULT_PATH.parent / "libexfold_b200_torch.so"
+                if not path.is_file():
+                    raise RuntimeError(f"ExFold B200 torch binding is missing: {path} "
+                                       "(build it with: python exfold-moe_b200/build.py)")
+                torch.ops.load_library(str(path))
+                torch.ops.exfold_b200.bind(str(library_path()))
+                _torch_ops = torch.ops.exfold_b200
+    return _torch_ops
+
+
 class ExfoldError(RuntimeError):
     """A CUDA-level failure reported by the library."""
 

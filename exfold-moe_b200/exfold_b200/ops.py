@@ -10,7 +10,6 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-import math
 
 import torch
 from torch.autograd import forward_ad
@@ -593,10 +592,11 @@ class _GatedMlp(torch.autograd.Function):
         return (_gated_backward_once if torch.is_grad_enabled() else _gated_backward)(ctx, dh)
 
 
-def _has_tangent(*tensors: torch.Tensor) -> bool:
+def _has_tangent(*tensors: torch.Tensor | None) -> bool:
     """Whether one of them is a dual tensor of forward-mode differentiation."""
     return (forward_ad._current_level >= 0
-            and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors))
+            and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                    for t in tensors))
 
 
 def gated_mlp(x: torch.Tensor, w13: torch.Tensor, activation: str = "silu",
@@ -632,100 +632,7 @@ def gated_mlp(x: torch.Tensor, w13: torch.Tensor, activation: str = "silu",
 
 
 # ---- root-mean-square norm ----------------------------------------------------------------------
-_CODE = {torch.float8_e4m3fn: L.EXF_E4M3, torch.int8: L.EXF_I8}
-
-
-def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
-    """t [..., cols] as rows [n, cols] at a constant distance, where they lie if they do."""
-    if t.dim() != 2:
-        t = t.reshape(-1, cols)
-    if (t.stride(1) == 1 or cols == 1) and (t.shape[0] <= 1 or t.stride(0) >= cols):
-        return t
-    return t.contiguous()
-
-
-def _norm_checks(name, x, weight, eps, residual):
-    _require_cuda(x, weight, residual)
-    if x.dtype not in _WDT:
-        raise TypeError(f"{name} needs a float32, bfloat16 or float16 input")
-    if weight.dtype is not x.dtype and weight.dtype is not torch.float32:
-        raise TypeError(f"{name}: the weight must be float32 or of the input's type")
-    if residual is not None and residual.dtype is not x.dtype:
-        raise TypeError(f"{name}: the residual must be of the input's type")
-    if x.dim() < 1 or weight.dim() != 1 or weight.shape[0] != x.shape[-1] or x.shape[-1] == 0:
-        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} must be [..., H] and "
-                         "[H]")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"residual {tuple(residual.shape)} must have x's shape {tuple(x.shape)}")
-    if not eps >= 0.0:
-        raise ValueError(f"eps must not be negative, got {eps}")
-
-
-def _norm_forward(x, residual, weight, eps):
-    """(y, s, x's rows); s is None without a residual."""
-    cols, dev = x.shape[-1], x.device
-    rows = _rows(x, cols)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    s, res, stride = None, None, 0
-    if residual is not None:
-        s, res = torch.empty_like(y), _rows(residual, cols)
-        stride = res.stride(0)
-    weight = weight.contiguous()
-    n = rows.shape[0]
-    if n > 0:
-        with _on(dev):
-            L.check(L.lib().exf_rms_norm(
-                rows.data_ptr(), rows.stride(0), _ptr(res), stride, weight.data_ptr(),
-                _WDT[x.dtype], _WDT[weight.dtype], n, cols, eps, _ptr(s), y.data_ptr(),
-                _stream(dev)))
-    return y, s, rows
-
-
-def _norm_backward(ctx, dy, ds):
-    x, weight = ctx.saved_tensors
-    cols = weight.shape[0]
-    rows, weight = _rows(x, cols), weight.contiguous()
-    dev, dtype, n = x.device, x.dtype, rows.shape[0]
-    want_x, want_r, want_w, _ = ctx.needs_input_grad
-    dx = torch.empty(ctx.shape, dtype=dtype, device=dev) if want_x or want_r else None
-    dw = torch.empty_like(weight) if want_w else None
-    # (of s alone, where y was not used)
-    dy = torch.zeros(ctx.shape, dtype=dtype, device=dev) if dy is None else dy.contiguous()
-    ds = None if ds is None else ds.contiguous()
-    lib = L.lib()
-    with _on(dev):
-        ws = None
-        ws_bytes = lib.exf_rms_norm_backward_workspace_bytes(n, cols) if want_w else 0
-        if ws_bytes > 0:
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        L.check(lib.exf_rms_norm_backward(
-            dy.data_ptr(), _ptr(ds), rows.data_ptr(), rows.stride(0), weight.data_ptr(),
-            _WDT[dtype], _WDT[weight.dtype], n, cols, ctx.eps, _ptr(dx), _ptr(dw), _ptr(ws),
-            ws_bytes, _stream(dev)))
-    # (the gradient of the sum is that of both of its terms)
-    return dx if want_x else None, dx if want_r else None, dw, None
-
-
-_norm_backward_once = torch.autograd.function.once_differentiable(_norm_backward)
-
-
-class _RmsNorm(torch.autograd.Function):
-    # (takes and gives the caller's shapes: a view outside would be another node of the graph)
-    @staticmethod
-    def forward(ctx, x, residual, weight, eps):
-        y, s, rows = _norm_forward(x, residual, weight, eps)
-        copied = rows.data_ptr() != x.data_ptr()
-        ctx.save_for_backward((rows if copied else x) if s is None else s, weight)
-        ctx.eps, ctx.shape = eps, x.shape
-        ctx.set_materialize_grads(False)
-        return y if s is None else (y, s)
-
-    @staticmethod
-    def backward(ctx, dy, ds=None):
-        # recorded itself (create_graph): its gradients raise when they are differentiated
-        return (_norm_backward_once if torch.is_grad_enabled() else _norm_backward)(ctx, dy, ds)
-
-
+# (these and the operators below: binding/torch_ops.cpp checks, allocates and launches)
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
              residual: torch.Tensor | None = None):
     """y = s * weight / sqrt(mean(s^2) + eps) over the last dimension, s = x, or (y, s) with s = x +
@@ -736,14 +643,10 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     x, residual and weight (once, in reverse mode; forward mode is refused); nothing is kept for the
     backward pass but s.
     """
-    _norm_checks("rms_norm", x, weight, eps, residual)
-    if _has_tangent(x, weight, *(() if residual is None else (residual,))):
+    if _has_tangent(x, weight, residual):
         raise NotImplementedError("rms_norm has no forward-mode derivative")
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                    or (residual is not None and residual.requires_grad)):
-        return _RmsNorm.apply(x, residual, weight, float(eps))
-    y, s, _ = _norm_forward(x, residual, weight, float(eps))
-    return y if s is None else (y, s)
+    out = L.torch_ops().rms_norm.default(x, weight, eps, residual)
+    return out[0] if residual is None else tuple(out)
 
 
 def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -757,110 +660,21 @@ def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     code * scale (`dequantize_8bit`).  A group with a value that is not finite reads back as NaN.  H up to
     2^17.  For inference: the result carries no gradient.
     """
-    _norm_checks("rms_norm_8bit", x, weight, eps, residual)
-    if dtype not in _CODE:
-        raise TypeError("rms_norm_8bit gives float8_e4m3fn or int8 codes")
-    if group not in (None, 32, 64, 128):
-        raise ValueError(f"group must be 32, 64, 128 or None (a row), got {group}")
-    cols, dev = x.shape[-1], x.device
-    rows, w = _rows(x, cols), weight.contiguous()
-    groups = 1 if group is None else -(-cols // group)
-    codes = torch.empty(x.shape, dtype=dtype, device=dev)
-    scales = torch.empty(*x.shape[:-1], groups, dtype=torch.float32, device=dev)
-    s, res, stride = None, None, 0
-    if residual is not None:
-        s, res = torch.empty(x.shape, dtype=x.dtype, device=dev), _rows(residual, cols)
-        stride = res.stride(0)
-    n = rows.shape[0]
-    if n > 0:
-        with _on(dev):
-            L.check(L.lib().exf_rms_norm_8bit(
-                rows.data_ptr(), rows.stride(0), _ptr(res), stride, w.data_ptr(), _WDT[x.dtype],
-                _WDT[w.dtype], n, cols, float(eps), _CODE[dtype], group or 0, _ptr(s),
-                codes.data_ptr(), scales.data_ptr(), _stream(dev)))
-    return (codes, scales) if s is None else (codes, scales, s)
+    return tuple(L.torch_ops().rms_norm_8bit.default(x, weight, eps, residual, dtype, _group(group)))
+
+
+def _group(group: int | None) -> int:
+    """A group as the binding takes it: 0 is a row (and 0 itself no group)."""
+    return 0 if group is None else group or -1
 
 
 def dequantize_8bit(codes: torch.Tensor, scales: torch.Tensor, group: int | None = 128,
                     dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values code * scale of `rms_norm_8bit`'s codes and scales, rounded to dtype."""
-    dev = _require_cuda(codes, scales)
-    if codes.dtype not in _CODE or scales.dtype != torch.float32:
-        raise TypeError("dequantize_8bit needs float8_e4m3fn or int8 codes and float32 scales")
-    if dtype not in _WDT:
-        raise TypeError("dequantize_8bit gives float32, bfloat16 or float16")
-    if group not in (None, 32, 64, 128):
-        raise ValueError(f"group must be 32, 64, 128 or None (a row), got {group}")
-    cols = codes.shape[-1] if codes.dim() else 0
-    groups = 1 if group is None else -(-cols // group)
-    if cols == 0 or scales.shape != (*codes.shape[:-1], groups):
-        raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} must be "
-                         "[..., H] and [..., groups]")
-    codes, scales = _aligned(codes), scales.contiguous()
-    out = torch.empty(codes.shape, dtype=dtype, device=dev)
-    n = out.numel()
-    if n > 0:
-        with _on(dev):
-            L.check(L.lib().exf_dequantize_8bit(codes.data_ptr(), _CODE[codes.dtype],
-                                                scales.data_ptr(), n // cols, cols, group or 0,
-                                                out.data_ptr(), _WDT[dtype], _stream(dev)))
-    return out
+    return L.torch_ops().dequantize_8bit.default(codes, scales, _group(group), dtype)
 
 
 # ---- balance loss -------------------------------------------------------------------------------
-def _balance_forward(logits, ids, mask, scoring):
-    """(loss, counts, valid) of contiguous inputs, in the logits' leading shape."""
-    *lead, tokens, experts = logits.shape
-    groups = math.prod(lead)
-    dev = logits.device
-    loss = torch.empty(lead, dtype=torch.float32, device=dev)
-    counts = torch.empty(*lead, experts, dtype=torch.int32, device=dev)
-    valid = torch.empty(lead, dtype=torch.int32, device=dev)
-    lib = L.lib()
-    with _on(dev):
-        ws_bytes = lib.exf_balance_loss_workspace_bytes(groups, tokens, experts)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
-        L.check(lib.exf_balance_loss(
-            logits.data_ptr(), _WDT[logits.dtype], ids.data_ptr(), _IDT[ids.dtype], _ptr(mask),
-            groups, tokens, experts, ids.shape[-1], scoring, loss.data_ptr(), counts.data_ptr(),
-            valid.data_ptr(), _ptr(ws), ws_bytes, _stream(dev)))
-    return loss, counts, valid
-
-
-def _balance_backward(ctx, dloss, _):
-    logits, mask, counts, valid = ctx.saved_tensors
-    *lead, tokens, experts = logits.shape
-    dev = logits.device
-    dlogits = torch.empty_like(logits)
-    dloss = dloss.contiguous()
-    with _on(dev):
-        L.check(L.lib().exf_balance_loss_backward(
-            dloss.data_ptr(), logits.data_ptr(), _WDT[logits.dtype], _ptr(mask), counts.data_ptr(),
-            valid.data_ptr(), math.prod(lead), tokens, experts, ctx.top_k, ctx.scoring,
-            dlogits.data_ptr(), _stream(dev)))
-    return dlogits, None, None, None
-
-
-_balance_backward_once = torch.autograd.function.once_differentiable(_balance_backward)
-
-
-class _BalanceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, ids, mask, scoring):
-        logits = logits.contiguous()
-        loss, counts, valid = _balance_forward(logits, ids, mask, scoring)
-        ctx.save_for_backward(logits, mask, counts, valid)
-        ctx.top_k, ctx.scoring = ids.shape[-1], scoring
-        ctx.mark_non_differentiable(counts)
-        return loss, counts
-
-    @staticmethod
-    def backward(ctx, dloss, dcounts):
-        # recorded itself (create_graph): its gradients raise when they are differentiated
-        return (_balance_backward_once if torch.is_grad_enabled()
-                else _balance_backward)(ctx, dloss, dcounts)
-
-
 def balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor, scoring: str = "softmax",
                  mask: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The balance loss of a router and the experts' counts: (loss fp32 [...], counts int32 [..., E]).
@@ -874,27 +688,11 @@ def balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor, scoring: str = "s
     [0, E) count nowhere.  Differentiable in logits (once, in reverse mode; forward mode is refused); the
     counts carry no gradient.  E up to 1024.
     """
-    _require_cuda(logits, topk_ids, mask)
-    if logits.dtype not in _WDT:
-        raise TypeError("balance_loss needs float32, bfloat16 or float16 logits")
     if scoring not in ("softmax", "sigmoid"):
         raise ValueError(f"scoring must be softmax or sigmoid, got {scoring!r}")
-    if (logits.dim() < 2 or topk_ids.shape[:-1] != logits.shape[:-1] or logits.shape[-1] == 0
-            or topk_ids.shape[-1] == 0):
-        raise ValueError(f"logits {tuple(logits.shape)} and topk_ids {tuple(topk_ids.shape)} must be "
-                         "[..., T, E] and [..., T, k]")
-    if mask is not None and (mask.dtype != torch.bool or mask.shape != logits.shape[:-1]):
-        raise ValueError(f"mask must be bool {tuple(logits.shape[:-1])}, got {mask.dtype} "
-                         f"{tuple(mask.shape)}")
     if _has_tangent(logits):
         raise NotImplementedError("balance_loss has no forward-mode derivative")
-    if topk_ids.dtype is not torch.int64:
-        topk_ids = _expert_ids(topk_ids, logits.shape[-1])
-    ids = topk_ids.contiguous()
-    m = None if mask is None else mask.contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _BalanceLoss.apply(logits, ids, m, _SCORING[scoring])
-    return _balance_forward(logits.contiguous(), ids, m, _SCORING[scoring])[:2]
+    return tuple(L.torch_ops().balance_loss.default(logits, topk_ids, _SCORING[scoring], mask))
 
 
 # ---- projection with adapters -------------------------------------------------------------------
@@ -910,35 +708,4 @@ def adapted_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
     and rank are multiples of 8, rank at most 128.  Sums are fp32; y is rounded once.  `status` as in
     `fused_experts`.  For inference: the result carries no gradient.
     """
-    dev = _require_cuda(x, w, a, b, adapter_ids, scaling, status)
-    dtype = x.dtype
-    if dtype not in (torch.bfloat16, torch.float16) or not (w.dtype is dtype and a.dtype is dtype
-                                                            and b.dtype is dtype):
-        raise TypeError("adapted_linear needs x, w, a and b all bfloat16 or all float16")
-    if (x.dim() < 1 or w.dim() != 2 or a.dim() != 3 or b.dim() != 3 or w.shape[1] != x.shape[-1]
-            or a.shape[2] != w.shape[1] or b.shape != (a.shape[0], w.shape[0], a.shape[1])
-            or w.numel() == 0 or a.shape[1] == 0):
-        raise ValueError(f"x {tuple(x.shape)}, w {tuple(w.shape)}, a {tuple(a.shape)} and b "
-                         f"{tuple(b.shape)} must be [..., K], [N, K], [R, rank, K] and [R, N, rank]")
-    if adapter_ids.shape != x.shape[:-1]:
-        raise ValueError(f"adapter_ids {tuple(adapter_ids.shape)} must have x's leading shape "
-                         f"{tuple(x.shape[:-1])}")
-    if scaling is not None and scaling.shape != a.shape[:1]:
-        raise ValueError(f"scaling {tuple(scaling.shape)} must be [{a.shape[0]}]")
-    outer, inner = w.shape
-    adapters, rank = a.shape[:2]
-    rows, w, a, b = _aligned(x), _aligned(w), _aligned(a), _aligned(b)
-    ids = _expert_ids(adapter_ids, adapters).contiguous()
-    if scaling is not None:
-        scaling = _f32c(scaling)
-    y = torch.empty(*x.shape[:-1], outer, dtype=dtype, device=dev)
-    tokens = ids.numel()
-    lib = L.lib()
-    with _on(dev):
-        ws_bytes = lib.exf_adapted_linear_workspace_bytes(tokens, inner, outer, rank)
-        ws = torch.empty(ws_bytes if ws_bytes > 32 else 32, dtype=torch.uint8, device=dev)
-        L.check(lib.exf_adapted_linear(
-            rows.data_ptr(), w.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(),
-            _ptr(scaling), _WDT[dtype], tokens, inner, outer, adapters, rank, y.data_ptr(),
-            ws.data_ptr(), ws_bytes, _status_ptr(status), _stream(dev)))
-    return y
+    return L.torch_ops().adapted_linear.default(x, w, a, b, adapter_ids, scaling, status)
