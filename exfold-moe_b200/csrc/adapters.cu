@@ -1015,10 +1015,6 @@ template <bool BF16, int MB>
 static cudaError_t down(const AdapterArgs& a, const AdapterLists& l, const AdapterPlan& pl, bool rows,
                         cudaStream_t s) {
   auto* kern = adapter_down_kernel<BF16, MB>;
-  static std::mutex mu;
-  static bool done[64] = {};
-  const cudaError_t e = prefer_smem(kern, mu, done);
-  if (e != cudaSuccess) return e;
   return launch_clusters(kern, dim3((unsigned)(ceil_of(a.tokens, pl.take) * pl.parts)), dim3(256), 0,
                          s, pl.parts, a, l, rows, pl.parts, pl.take);
 }

@@ -27,22 +27,6 @@ static cudaError_t allow_smem(K* kern, size_t bytes, std::mutex& mu, bool (&done
   return e;
 }
 
-// Gives a kernel's SMs their largest shared memory, once per device: a kernel that follows it and needs that
-// much can then start on them while it still runs (the division is an SM's, and changes only when it is idle).
-template <typename K>
-static cudaError_t prefer_smem(K* kern, std::mutex& mu, bool (&done)[64]) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  std::lock_guard<std::mutex> lock(mu);
-  if (done[dev]) return cudaSuccess;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout,
-                           cudaSharedmemCarveoutMaxShared);
-  done[dev] = e == cudaSuccess;
-  return e;
-}
-
 // Launch as a programmatic dependent of the previous kernel in the stream (the kernel calls
 // griddepcontrol.wait before reading anything that kernel wrote).
 // `cluster` neighbouring blocks form a cluster.
