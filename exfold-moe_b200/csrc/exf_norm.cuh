@@ -143,33 +143,31 @@ __device__ __forceinline__ void load_sum(const T* x, const T* r, float (&out)[V]
 // The sum over the G threads of a row (in a fixed order), for all of them.  G <= 32: lanes of a warp; else
 // the whole block, through 32 words of shared memory; the next use of the same words needs a barrier of
 // all threads in between (another row_sum over other words is one).
+__device__ __forceinline__ float plus_lane(float v, int d) { return v + __shfl_xor_sync(0xffffffffu, v, d); }
+__device__ __forceinline__ double plus_lane(double v, int d) {
+  return v + __shfl_xor_sync(0xffffffffu, v, d);
+}
+__device__ __forceinline__ float2 plus_lane(float2 v, int d) {
+  return make_float2(plus_lane(v.x, d), plus_lane(v.y, d));
+}
 template <typename A>
-__device__ __forceinline__ A row_sum(A v, int g, A* shared) {
-  const int w = g < 32 ? g : 32;
-  for (int d = w / 2; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  if (g <= 32) return v;
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-  __syncthreads();
-  const int warps = g >> 5, lane = threadIdx.x & 31;
-  v = lane < warps ? shared[lane] : A(0);
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+__device__ __forceinline__ A warp_sum(A v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v = plus_lane(v, d);
   return v;
 }
-__device__ __forceinline__ float2 row_sum2(float2 v, int g, float2* shared) {
-  auto add = [](float2 p, int d) {
-    p.x += __shfl_xor_sync(0xffffffffu, p.x, d);
-    p.y += __shfl_xor_sync(0xffffffffu, p.y, d);
-    return p;
-  };
-  const int w = g < 32 ? g : 32;
-  for (int d = w / 2; d > 0; d >>= 1) v = add(v, d);
-  if (g <= 32) return v;
+template <typename A>
+__device__ __forceinline__ A row_sum(A v, int g, A* shared) {
+  if (g < 32) {
+    for (int d = g / 2; d > 0; d >>= 1) v = plus_lane(v, d);
+    return v;
+  }
+  v = warp_sum(v);
+  if (g == 32) return v;
   if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
   __syncthreads();
-  const int warps = g >> 5, lane = threadIdx.x & 31;
-  v = lane < warps ? shared[lane] : make_float2(0.0f, 0.0f);
-  for (int d = 16; d > 0; d >>= 1) v = add(v, d);
-  return v;
+  const int lane = threadIdx.x & 31;
+  return warp_sum(lane < (g >> 5) ? shared[lane] : A{});
 }
 // Whether a sum of squares has left the range in which fp32 holds it to its last bits: it overflowed (or
 // holds an infinity or a NaN), or it is so small that its terms were cut off.  Then it is summed again in
@@ -197,13 +195,14 @@ __device__ __noinline__ double2 sums_64(const T* x, const T* r, const T* dy, con
   return d;
 }
 
-// 1 / sqrt(mean square + eps) of a row from its threads' sums q; x, r: the row.  Every thread of the block
+// 1 / sqrt(mean square + eps) of a row from its threads' sums q; mean: 1 / cols (a product, one rounding
+// of 2^-24 more than a quotient, and no division per row); x, r: the row.  Every thread of the block
 // calls it.
 template <typename T>
-__device__ __forceinline__ float inverse_norm(float q, const NormArgs& a, int g, int t, const T* x,
-                                              const T* r, float* part, double* part64) {
+__device__ __forceinline__ float inverse_norm(float q, float mean, const NormArgs& a, int g, int t,
+                                              const T* x, const T* r, float* part, double* part64) {
   q = row_sum(q, g, part);
-  float v = rsqrtf(q / (float)a.cols + a.eps);
+  float v = rsqrtf(q * mean + a.eps);
   const bool again = out_of_range(q, a.eps);
   // (the same for the block where a row is a block; else the warp's other rows go along)
   if (g > 32 ? again : __any_sync(0xffffffffu, again)) {

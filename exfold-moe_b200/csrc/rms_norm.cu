@@ -65,6 +65,7 @@ __global__ void __launch_bounds__(THREADS)
   };
   fetch(row);
   w.init(a.weight, t, g, n);
+  const float mean = 1.0f / (float)a.cols;
   // every thread of a block (G <= 32: of a warp) takes as many turns
   int b = 0;
   for (int64_t base = first; base < a.rows; base += step, row += step, b ^= 1) {
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(THREADS)
       if (extra) to[n.odd - n.shift] = from_f32<T>(s1);
     }
     const int64_t mine = live ? row : 0;
-    const float v = inverse_norm<T>(q, a, g, t, x + mine * a.x_stride,
+    const float v = inverse_norm<T>(q, mean, a, g, t, x + mine * a.x_stride,
                                     r ? r + mine * a.r_stride : nullptr, part[b], part64);
     if (live) {
       T* to = y + at + n.shift;
@@ -128,7 +129,8 @@ __global__ void __launch_bounds__(1024) rms_norm_long_kernel(const NormArgs a, T
 #pragma unroll
     for (int j = 0; j < V; ++j) q = fmaf(s[j], s[j], q);
   }
-  const float v = inverse_norm<T>(q, a, 1024, threadIdx.x, x, r, part, part64);
+  const float mean = 1.0f / (float)a.cols;
+  const float v = inverse_norm<T>(q, mean, a, 1024, threadIdx.x, x, r, part, part64);
 #pragma unroll 4
   for (int u = threadIdx.x; u < units; u += 1024) {
     float w[V];
@@ -222,7 +224,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
       c = fmaf(d1 * w.single, s1, c);
     }
     if (kAhead) fetch(row + step);
-    const float2 both = row_sum2(make_float2(q, c), g, part[b]);
+    const float2 both = row_sum(make_float2(q, c), g, part[b]);
     q = both.x;
     c = both.y;
     float v = rsqrtf(q * mean + a.eps);
@@ -320,7 +322,7 @@ __global__ void __launch_bounds__(1024)
         c = fmaf(d[j] * w[j], s[j], c);
       }
     }
-    const float2 both = row_sum2(make_float2(q, c), 1024, part);
+    const float2 both = row_sum(make_float2(q, c), 1024, part);
     q = both.x;
     c = both.y;
     float v = rsqrtf(q * mean + a.eps);

@@ -60,8 +60,9 @@ struct Top<false> {
 };
 template <bool EXACT>
 __device__ __forceinline__ typename Top<EXACT>::Key top_over(typename Top<EXACT>::Key k, int lanes) {
-  for (int d = lanes / 2; d > 0; d >>= 1)
-    k = Top<EXACT>::larger(k, __shfl_xor_sync(0xffffffffu, k, d));
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1)
+    if (2 * d <= lanes) k = Top<EXACT>::larger(k, __shfl_xor_sync(0xffffffffu, k, d));
   return k;
 }
 
@@ -210,6 +211,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
     else
       __syncwarp();
   }
+  const float mean = 1.0f / (float)a.cols;
   int b = 0, set = 0;
   for (int64_t base = first; base < a.rows; base += step, row += step, b ^= 1) {
     const bool live = row < a.rows;
@@ -271,7 +273,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
       all = top_over<EXACT>(all, 32);
       if (g > 32 && (threadIdx.x & 31) == 0) part_top[b][threadIdx.x >> 5] = all;
     }
-    const float v = inverse_norm<T>(q, a, g, t, xr, rr, part[b], part64);
+    const float v = inverse_norm<T>(q, mean, a, g, t, xr, rr, part[b], part64);
     if (group == 0 && g > 32) {
       const int lane = threadIdx.x & 31;
       all = top_over<EXACT>(lane < (g >> 5) ? part_top[b][lane] : Key(0), 32);
@@ -407,7 +409,8 @@ __global__ void __launch_bounds__(1024)
     if ((threadIdx.x & 31) == 0) atomicMax(tops, K::shared(all));
   }
   // (behind a barrier of its own: the maxima are complete)
-  const float v = inverse_norm<T>(q, a, 1024, threadIdx.x, x, r, part, part64);
+  const float mean = 1.0f / (float)a.cols;
+  const float v = inverse_norm<T>(q, mean, a, 1024, threadIdx.x, x, r, part, part64);
   for (int c = threadIdx.x; c < a.cols; c += 1024) {
     float s[1];
     load_sum<T, 1>(x + c, r ? r + c : nullptr, s);
