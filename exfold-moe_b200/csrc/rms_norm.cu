@@ -19,7 +19,7 @@
 namespace exf {
 
 // ---- forward ------------------------------------------------------------------------------------
-// Blocks that stay: G threads a row, NU units of V elements a thread (unit u = thread + G * i).  The next
+// Blocks that stay: G threads a row, NU units of V elements a thread.  The next
 // row's loads are issued before this row is reduced, so that memory stays busy through the reduction and
 // its barrier, and the weights stay in registers.  (A block a row, without either: 32768 x 4096 bf16 with a
 // residual 255 us.)  G <= 32: a block holds 128 / G rows, and nothing waits but lanes for lanes.
@@ -38,33 +38,33 @@ __global__ void __launch_bounds__(THREADS)
   const int64_t step = (int64_t)gridDim.x * per_block;
   const int64_t first = (int64_t)blockIdx.x * per_block;
   int64_t row = first + threadIdx.x / g;
-  const Units<V> n(row, a.cols);
+  const Units<V> n(row, a.cols, t, g);
   const bool extra = V == 2 && n.odd >= 0 && t == 0;
 
   Pack<T, V> nx[NU], nr[NU], s[NU];
   float nx1 = 0.0f, nr1 = 0.0f;
   Weights<W, V, NU> w;
   auto fetch = [&](int64_t at) {
-    const T* xr = x + at * a.x_stride + n.shift;
-    const T* rr = r + at * a.r_stride + n.shift;
+    const T* xr = x + at * a.x_stride + n.column(0);
+    const T* rr = r + at * a.r_stride + n.column(0);
+    const bool live = at < a.rows;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      const int u = t + g * i;
-      if (u < n.count && at < a.rows) {
-        nx[i].read(xr + u * V);
-        if (r) nr[i].read(rr + u * V);
+      if (n.has(i) && live) {
+        nx[i].read(xr + n.step(i) * V);
+        if (r) nr[i].read(rr + n.step(i) * V);
       } else {
         nx[i].clear();
         nr[i].clear();
       }
     }
-    if (extra && at < a.rows) {
-      nx1 = to_f32<T>(xr[n.odd - n.shift]);
-      if (r) nr1 = to_f32<T>(rr[n.odd - n.shift]);
+    if (extra && live) {
+      nx1 = to_f32<T>(x[at * a.x_stride + n.odd]);
+      if (r) nr1 = to_f32<T>(r[at * a.r_stride + n.odd]);
     }
   };
   fetch(row);
-  w.init(a.weight, t, g, n);
+  w.init(a.weight, t, n);
   const float mean = 1.0f / (float)a.cols;
   // every thread of a block (G <= 32: of a warp) takes as many turns
   int b = 0;
@@ -82,30 +82,29 @@ __global__ void __launch_bounds__(THREADS)
     const int64_t at = row * a.cols;
     fetch(row + step);
     if (r && live) {
-      T* to = sum + at + n.shift;
+      T* to = sum + at + n.column(0);
 #pragma unroll
       for (int i = 0; i < NU; ++i)
-        if (t + g * i < n.count) s[i].write(to + (t + g * i) * V);
-      if (extra) to[n.odd - n.shift] = from_f32<T>(s1);
+        if (n.has(i)) s[i].write(to + n.step(i) * V);
+      if (extra) sum[at + n.odd] = from_f32<T>(s1);
     }
     const int64_t mine = live ? row : 0;
     const float v = inverse_norm<T>(q, mean, a, g, t, x + mine * a.x_stride,
                                     r ? r + mine * a.r_stride : nullptr, part[b], part64);
     if (live) {
-      T* to = y + at + n.shift;
+      T* to = y + at + n.column(0);
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
-        const int u = t + g * i;
         s[i].anew();
         w.w[i].anew();
-        if (u < n.count) {
+        if (n.has(i)) {
           float e[V];
 #pragma unroll
           for (int j = 0; j < V; ++j) e[j] = s[i].get(j) * v * w.w[i].get(j);
-          store_pack<T, V>(to + u * V, e);
+          store_pack<T, V>(to + n.step(i) * V, e);
         }
       }
-      if (extra) to[n.odd - n.shift] = from_f32<T>(s1 * v * w.single);
+      if (extra) y[at + n.odd] = from_f32<T>(s1 * v * w.single);
     }
   }
 }
@@ -162,7 +161,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
   const int64_t step = (int64_t)gridDim.x * per_block;
   const int64_t first = (int64_t)blockIdx.x * per_block;
   int64_t row = first + sub;
-  const Units<V> n(row, a.cols);
+  const Units<V> n(row, a.cols, t, g);
   const bool extra = V == 2 && n.odd >= 0 && t == 0;
 
   Pack<T, V> nx[NU], ny[NU], nd[NU];
@@ -170,32 +169,32 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
   Weights<W, V, NU> w;
   float acc[NU][V], acc1 = 0.0f;
   auto fetch = [&](int64_t at) {
-    const T* xr = x + at * a.x_stride + n.shift;
-    const T* yr = dy + at * a.cols + n.shift;
-    const T* dr = ds + at * a.cols + n.shift;
+    const T* xr = x + at * a.x_stride + n.column(0);
+    const T* yr = dy + at * a.cols + n.column(0);
+    const T* dr = ds + at * a.cols + n.column(0);
+    const bool live = at < a.rows;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      const int u = t + g * i;
-      if (u < n.count && at < a.rows) {
-        nx[i].read(xr + u * V);
-        ny[i].read(yr + u * V);
-        if (ds) nd[i].read(dr + u * V);
+      if (n.has(i) && live) {
+        nx[i].read(xr + n.step(i) * V);
+        ny[i].read(yr + n.step(i) * V);
+        if (ds) nd[i].read(dr + n.step(i) * V);
       } else {
         nx[i].clear();
         ny[i].clear();
         nd[i].clear();
       }
     }
-    if (extra && at < a.rows) {
-      nx1 = to_f32<T>(xr[n.odd - n.shift]);
-      ny1 = to_f32<T>(yr[n.odd - n.shift]);
-      if (ds) nd1 = to_f32<T>(dr[n.odd - n.shift]);
+    if (extra && live) {
+      nx1 = to_f32<T>(x[at * a.x_stride + n.odd]);
+      ny1 = to_f32<T>(dy[at * a.cols + n.odd]);
+      if (ds) nd1 = to_f32<T>(ds[at * a.cols + n.odd]);
     }
   };
   // (1024 threads have no registers for the row after this one)
   constexpr bool kAhead = THREADS < 1024;
   if (kAhead) fetch(row);
-  w.init(a.weight, t, g, n);
+  w.init(a.weight, t, n);
 #pragma unroll
   for (int i = 0; i < NU; ++i)
 #pragma unroll
@@ -245,10 +244,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
       }
     }
     if (row < a.rows) {
-      T* to = dx + row * a.cols + n.shift;
+      T* to = dx + row * a.cols + n.column(0);
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
-        const int u = t + g * i;
         s[i].anew();
         d[i].anew();
         w.w[i].anew();
@@ -260,14 +258,14 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
           e[j] = v * fmaf(-hat, k, up * w.w[i].get(j));
           if (ds) e[j] += o[i].get(j);
         }
-        if (dx && u < n.count) store_pack<T, V>(to + u * V, e);
+        if (dx && n.has(i)) store_pack<T, V>(to + n.step(i) * V, e);
       }
       if (extra) {
         const float hat = s1 * v;
         acc1 = fmaf(d1, hat, acc1);
         float e = v * fmaf(-hat, k, d1 * w.single);
         if (ds) e += o1;
-        if (dx) to[n.odd - n.shift] = from_f32<T>(e);
+        if (dx) dx[row * a.cols + n.odd] = from_f32<T>(e);
       }
     }
   }
@@ -276,10 +274,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
   float* mine = per_block > 1 ? sums + sub * a.cols : to;
 #pragma unroll
   for (int i = 0; i < NU; ++i) {
-    const int u = t + g * i;
-    if (u < n.count) {
+    if (n.has(i)) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) mine[n.column(u) + j] = acc[i][j];
+      for (int j = 0; j < V; ++j) mine[n.column(i) + j] = acc[i][j];
     }
   }
   if (extra) mine[n.odd] = acc1;
@@ -396,7 +393,7 @@ static cudaError_t forward_v(const NormArgs& a, void* y, cudaStream_t s) {
     return launch_pdl(kern, dim3(grid), dim3(block), 0, s, a, g, out);
   };
   // few rows: half as many units a thread, the shorter chain
-  const int g = norm_threads(units, a.rows <= 148 ? NU / 2 : NU, 8);
+  const int g = norm_threads<V>(units, a.rows <= 148 ? NU / 2 : NU, 8);
   const int block = g <= 32 ? 128 : g;
   if (block <= 256) return go(rms_norm_kernel<T, W, V, NU, 256>, g, block);
   return go(rms_norm_kernel<T, W, V, NU, 1024>, g, block);
@@ -442,7 +439,7 @@ static cudaError_t backward_v(const NormArgs& a, const void* dy, const void* ds,
     e = launch_pdl(rms_norm_backward_long_kernel<T, V == 2 ? 1 : V>, dim3(blocks), dim3(1024), 0, s, a, up, side,
                    out, sums);
   } else {
-    const int g = norm_threads(units, NU, 8);
+    const int g = norm_threads<V>(units, NU, 8);
     const int block = g <= 32 ? 128 : g;
     const int per_block = block / g;
     const size_t smem = per_block > 1 ? (size_t)per_block * a.cols * sizeof(float) : 0;

@@ -58,10 +58,25 @@ struct Top<false> {
     return k ? (double)rounded(k) + (double)__uint_as_float(rest) : 0.0;
   }
 };
+// The largest of `lanes` neighbouring lanes (4 to 32).  A whole warp's, or a half's: the integer maximum of
+// the lanes in one instruction.
+__device__ __forceinline__ uint32_t top_bits(uint32_t k) { return __reduce_max_sync(0xffffffffu, k); }
+__device__ __forceinline__ float top_warp(float k) { return __uint_as_float(top_bits(__float_as_uint(k))); }
+__device__ __forceinline__ unsigned long long top_warp(unsigned long long k) {
+  const uint32_t hi = (uint32_t)(k >> 32), top = top_bits(hi);
+  return (unsigned long long)top << 32 | top_bits(hi == top ? (uint32_t)k : 0u);
+}
 template <bool EXACT>
 __device__ __forceinline__ typename Top<EXACT>::Key top_over(typename Top<EXACT>::Key k, int lanes) {
+  using Key = typename Top<EXACT>::Key;
+  if (lanes == 32) return top_warp(k);
+  if (lanes == 16) {
+    const bool upper = threadIdx.x & 16;
+    const Key lo = top_warp(upper ? Key(0) : k), hi = top_warp(upper ? k : Key(0));
+    return upper ? hi : lo;
+  }
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1)
+  for (int d = 4; d > 0; d >>= 1)
     if (2 * d <= lanes) k = Top<EXACT>::larger(k, __shfl_xor_sync(0xffffffffu, k, d));
   return k;
 }
@@ -173,7 +188,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
   const int64_t step = (int64_t)gridDim.x * per_block;
   const int64_t first = (int64_t)blockIdx.x * per_block;
   int64_t row = first + sub;
-  const Units<V> n(row, a.cols);
+  const Units<V> n(row, a.cols, t, g);
   const bool extra = V == 2 && n.odd >= 0 && t == 0;
   const int shift = group == 32 ? 5 : group == 64 ? 6 : 7;  // columns to groups
   const int groups = group ? (a.cols + group - 1) >> shift : 1;
@@ -184,26 +199,26 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
   float nx1 = 0.0f, nr1 = 0.0f;
   Weights<W, V, NU> w;
   auto fetch = [&](int64_t at) {
-    const T* xr = x + at * a.x_stride + n.shift;
-    const T* rr = r + at * a.r_stride + n.shift;
+    const T* xr = x + at * a.x_stride + n.column(0);
+    const T* rr = r + at * a.r_stride + n.column(0);
+    const bool live = at < a.rows;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      const int u = t + g * i;
-      if (u < n.count && at < a.rows) {
-        nx[i].read(xr + u * V);
-        if (r) nr[i].read(rr + u * V);
+      if (n.has(i) && live) {
+        nx[i].read(xr + n.step(i) * V);
+        if (r) nr[i].read(rr + n.step(i) * V);
       } else {
         nx[i].clear();
         nr[i].clear();
       }
     }
-    if (extra && at < a.rows) {
-      nx1 = to_f32<T>(xr[n.odd - n.shift]);
-      if (r) nr1 = to_f32<T>(rr[n.odd - n.shift]);
+    if (extra && live) {
+      nx1 = to_f32<T>(x[at * a.x_stride + n.odd]);
+      if (r) nr1 = to_f32<T>(r[at * a.r_stride + n.odd]);
     }
   };
   fetch(row);
-  w.init(a.weight, t, g, n);
+  w.init(a.weight, t, n);
   if (shared_tops) {
     for (int i = t; i < groups; i += g) tops[i] = 0;
     if (g > 32)
@@ -223,11 +238,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
     float q = 0.0f;
     Key top[NU], all = Key(0);
     float p[NU][V];
+    T* to = sum + at + n.column(0);
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      const int u = t + g * i;
       const Pack<T, V> s = r ? rounded_sum<T, V>(nx[i], nr[i]) : nx[i];
-      if (r && live && u < n.count) s.write(sum + at + n.column(u));
+      if (r && live && n.has(i)) s.write(to + n.step(i) * V);
       w.w[i].anew();
       Key most = Key(0), last = Key(0);
 #pragma unroll
@@ -242,8 +257,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
       }
       if (shared_tops) {
         most = top_over<EXACT>(most, kRun);
-        const int c = n.column(u);
-        if (u < n.count) {
+        const int c = n.column(i);
+        if (n.has(i)) {
           if (t % kRun == 0) atomicMax(here + (c >> shift), K::shared(most));
           if (V == 2 && n.shift && t % kRun == kRun - 1)
             atomicMax(here + ((c + 1) >> shift), K::shared(last));
@@ -283,11 +298,15 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
     uint8_t* out = codes + at;
     Quantum z = quantum_of<INT8>(K::rounded(all), v);  // (of the row; of groups below)
     if (group == 0 && live && t == 0) row_scales[0] = z.all ? top_scale(K::rounded(all), z) : z.scale;
-    uint32_t doubt = 0;  // elements (the one left over last) whose codes are taken again in 64 bits
+    // what has codes that are taken again in 64 bits: elements of vectors, small units (the element left
+    // over last)
+    uint32_t doubt = 0;
     auto word = [&](const float* e, auto count, int i) {
       constexpr int N = decltype(count)::value;
       const uint32_t low = code_word<INT8, N>(e, z.low), other = low ^ code_word<INT8, N>(e, z.high);
-      if (other || z.all) {
+      if constexpr (V <= 2) {
+        if (other || z.all) doubt |= 1u << (i / V);
+      } else if (other || z.all) {
 #pragma unroll
         for (int j = 0; j < N; ++j)
           if (z.all || (other >> (8 * j) & 255u)) doubt |= 1u << (i + j);
@@ -297,13 +316,13 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
     using std::integral_constant;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      const int u = t + g * i, c = n.column(u);
+      const int c = n.column(i);
       if constexpr (V > 2) {
         if (group != 0) {
           top[i] = top_over<EXACT>(top[i], group / V);
           z = quantum_of<INT8>(K::rounded(top[i]), v);
         }
-        if (u < n.count && live) {
+        if (n.has(i) && live) {
           if (group != 0 && (c & (group - 1)) == 0)
             row_scales[c >> shift] = z.all ? top_scale(K::rounded(top[i]), z) : z.scale;
           const integral_constant<int, 4> four;
@@ -313,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
           else
             *reinterpret_cast<uint32_t*>(out + c) = word(p[i], four, i * V);
         }
-      } else if (u < n.count && live) {
+      } else if (n.has(i) && live) {
         const integral_constant<int, 1> one;
         if (group != 0) {
           const float k = K::rounded(K::back(here[c >> shift]));
@@ -347,18 +366,24 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
       }
       out[n.odd] = (uint8_t)word(&p1, integral_constant<int, 1>(), NU * V);
     }
+    auto again = [&](int c, const Key& k) {
+      out[c] = code_64<T, W, INT8>(xr + c, rr ? rr + c : nullptr, weight + c, K::value(k));
+    };
 #pragma unroll 1
     for (; doubt; doubt &= doubt - 1) {
-      const int j = __ffs(doubt) - 1, i = j / V;
-      const int c = i < NU ? n.column(t + g * i) + j % V : n.odd;
-      Key k = all;
-      if (V > 2 && group != 0) {
+      const int j = __ffs(doubt) - 1;
+      if constexpr (V > 2) {
+        Key k = all;
+        if (group != 0) {
 #pragma unroll
-        for (int h = 0; h < NU; ++h) k = h == i ? top[h] : k;
-      } else if (V <= 2 && group != 0) {
-        k = K::back(here[c >> shift]);
+          for (int h = 0; h < NU; ++h) k = h == j / V ? top[h] : k;
+        }
+        again(n.column(j / V) + j % V, k);
+      } else {
+        const int c = j < NU ? n.column(j) : n.odd, last = j < NU ? c + V : c + 1;
+#pragma unroll 1
+        for (int h = c; h < last; ++h) again(h, group != 0 ? K::back(here[h >> shift]) : all);
       }
-      out[c] = code_64<T, W, INT8>(xr + c, rr ? rr + c : nullptr, weight + c, K::value(k));
     }
   }
 }
@@ -508,7 +533,7 @@ static cudaError_t quantize_v(const NormArgs& a, int group, uint8_t* codes, floa
   if (units > 1024 * NU)
     return launch_pdl(rms_norm_8bit_long_kernel<T, W, INT8>, dim3((unsigned)a.rows), dim3(1024),
                       groups * key, s, a, group, codes, scales);
-  const int g = norm_threads(units, a.rows <= 148 ? NU / 2 : NU, 32);
+  const int g = norm_threads<V>(units, a.rows <= 148 ? NU / 2 : NU, 32);
   const int block = g <= 32 ? 128 : g;
   const int per_block = block / g;
   const size_t smem = V <= 2 && group ? per_block * 3 * groups * key : 0;
