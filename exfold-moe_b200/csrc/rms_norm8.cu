@@ -159,24 +159,33 @@ __device__ __forceinline__ uint32_t code_word(const float* p, float m) {
   return lo;
 }
 
-// ---- the kernel -----------------------------------------------------------------------------------------
+// The codes of N products beside one another; doubt gets a bit, from the given one on, for each whose code
+// is to be taken again in 64 bits.
+template <bool INT8, int N>
+__device__ __forceinline__ uint32_t sure_word(const float* p, const Quantum& z, int bit, uint32_t& doubt) {
+  const uint32_t low = code_word<INT8, N>(p, z.low), other = low ^ code_word<INT8, N>(p, z.high);
+  if (other || z.all) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (z.all || (other >> (8 * j) & 255u)) doubt |= 1u << (bit + j);
+  }
+  return low;
+}
+
+// ---- rows of whole vectors ---------------------------------------------------------------------------------
 // Blocks that stay, as rms_norm_kernel's, with at least a warp a row.  The largest products are taken with
-// the loads' results; 32 columns lie on 32 / V neighbouring lanes.  Vectors: a group is 1 to 4 such runs, so
-// its lanes find its largest among them.  Else (V <= 2) a run's largest goes to the group's word in shared
-// memory (three sets of words: one is filled, one read, one zeroed), and where the units lie one column
-// on, the run's last element goes to its own group.  group 0: the row, reduced beside the sum of squares.
-template <typename T, typename W, int V, int NU, int THREADS, bool INT8>
+// the loads' results; a group lies on 32 / V to 128 / V neighbouring lanes, which find its largest among
+// them.  group 0: the row, reduced beside the sum of squares.
+template <typename T, typename W, int NU, int THREADS, bool INT8>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
     rms_norm_8bit_kernel(const NormArgs a, int g, int group, uint8_t* codes, float* scales) {
   constexpr bool EXACT = sizeof(T) == 2 && sizeof(W) == 2;
+  constexpr int V = 16 / sizeof(T);
   using K = Top<EXACT>;
   using Key = typename K::Key;
-  using Shared = typename K::Shared;
-  constexpr int kRun = 32 / V;
   __shared__ float part[2][32];
   __shared__ double part64[32];
   __shared__ Key part_top[2][32];
-  extern __shared__ unsigned long long words[];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int per_block = blockDim.x / g;
@@ -189,14 +198,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
   const int64_t first = (int64_t)blockIdx.x * per_block;
   int64_t row = first + sub;
   const Units<V> n(row, a.cols, t, g);
-  const bool extra = V == 2 && n.odd >= 0 && t == 0;
   const int shift = group == 32 ? 5 : group == 64 ? 6 : 7;  // columns to groups
   const int groups = group ? (a.cols + group - 1) >> shift : 1;
-  Shared* tops = reinterpret_cast<Shared*>(words) + (size_t)sub * 3 * groups;
-  const bool shared_tops = V <= 2 && group != 0;
 
   Pack<T, V> nx[NU], nr[NU];
-  float nx1 = 0.0f, nr1 = 0.0f;
   Weights<W, V, NU> w;
   auto fetch = [&](int64_t at) {
     const T* xr = x + at * a.x_stride + n.column(0);
@@ -212,29 +217,14 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
         nr[i].clear();
       }
     }
-    if (extra && live) {
-      nx1 = to_f32<T>(x[at * a.x_stride + n.odd]);
-      if (r) nr1 = to_f32<T>(r[at * a.r_stride + n.odd]);
-    }
   };
   fetch(row);
   w.init(a.weight, t, n);
-  if (shared_tops) {
-    for (int i = t; i < groups; i += g) tops[i] = 0;
-    if (g > 32)
-      __syncthreads();
-    else
-      __syncwarp();
-  }
   const float mean = 1.0f / (float)a.cols;
-  int b = 0, set = 0;
+  int b = 0;
   for (int64_t base = first; base < a.rows; base += step, row += step, b ^= 1) {
     const bool live = row < a.rows;
     const int64_t at = row * a.cols;
-    Shared* here = tops + set * groups;
-    set = set == 2 ? 0 : set + 1;
-    if (shared_tops)
-      for (int i = t; i < groups; i += g) tops[set * groups + i] = 0;
     float q = 0.0f;
     Key top[NU], all = Key(0);
     float p[NU][V];
@@ -244,40 +234,15 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
       const Pack<T, V> s = r ? rounded_sum<T, V>(nx[i], nr[i]) : nx[i];
       if (r && live && n.has(i)) s.write(to + n.step(i) * V);
       w.w[i].anew();
-      Key most = Key(0), last = Key(0);
+      top[i] = Key(0);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float e = s.get(j);
         q = fmaf(e, e, q);
         p[i][j] = e * w.w[i].get(j);
-        last = K::of(e, w.w[i].get(j), p[i][j]);
-        // (a run's last element one column on belongs to the group behind)
-        if (V == 2 && j == 1 && n.shift && t % kRun == kRun - 1) continue;
-        most = K::larger(most, last);
+        top[i] = K::larger(top[i], K::of(e, w.w[i].get(j), p[i][j]));
       }
-      if (shared_tops) {
-        most = top_over<EXACT>(most, kRun);
-        const int c = n.column(i);
-        if (n.has(i)) {
-          if (t % kRun == 0) atomicMax(here + (c >> shift), K::shared(most));
-          if (V == 2 && n.shift && t % kRun == kRun - 1)
-            atomicMax(here + ((c + 1) >> shift), K::shared(last));
-        }
-      } else if (V == 2) {
-        most = K::larger(most, last);
-      }
-      top[i] = most;
-      all = K::larger(all, most);
-    }
-    float p1 = 0.0f;
-    if (extra) {
-      const float s1 = r ? to_f32<T>(from_f32<T>(nx1 + nr1)) : nx1;
-      q = fmaf(s1, s1, q);
-      p1 = s1 * w.single;
-      const Key k = K::of(s1, w.single, p1);
-      all = K::larger(all, k);
-      if (shared_tops) atomicMax(here + (n.odd >> shift), K::shared(k));
-      if (r && live) sum[at + n.odd] = from_f32<T>(s1);
+      all = K::larger(all, top[i]);
     }
     fetch(row + step);
     const int64_t mine = live ? row : 0;
@@ -293,98 +258,198 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1)
       const int lane = threadIdx.x & 31;
       all = top_over<EXACT>(lane < (g >> 5) ? part_top[b][lane] : Key(0), 32);
     }
-    if (g <= 32 && shared_tops) __syncwarp();
     float* row_scales = scales + row * groups;
     uint8_t* out = codes + at;
     Quantum z = quantum_of<INT8>(K::rounded(all), v);  // (of the row; of groups below)
     if (group == 0 && live && t == 0) row_scales[0] = z.all ? top_scale(K::rounded(all), z) : z.scale;
-    // what has codes that are taken again in 64 bits: elements of vectors, small units (the element left
-    // over last)
     uint32_t doubt = 0;
-    auto word = [&](const float* e, auto count, int i) {
-      constexpr int N = decltype(count)::value;
-      const uint32_t low = code_word<INT8, N>(e, z.low), other = low ^ code_word<INT8, N>(e, z.high);
-      if constexpr (V <= 2) {
-        if (other || z.all) doubt |= 1u << (i / V);
-      } else if (other || z.all) {
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (z.all || (other >> (8 * j) & 255u)) doubt |= 1u << (i + j);
-      }
-      return low;
-    };
-    using std::integral_constant;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       const int c = n.column(i);
-      if constexpr (V > 2) {
-        if (group != 0) {
-          top[i] = top_over<EXACT>(top[i], group / V);
-          z = quantum_of<INT8>(K::rounded(top[i]), v);
-        }
-        if (n.has(i) && live) {
-          if (group != 0 && (c & (group - 1)) == 0)
-            row_scales[c >> shift] = z.all ? top_scale(K::rounded(top[i]), z) : z.scale;
-          const integral_constant<int, 4> four;
-          if constexpr (V == 8)
-            *reinterpret_cast<uint2*>(out + c) =
-                make_uint2(word(p[i], four, i * V), word(p[i] + (V > 4 ? 4 : 0), four, i * V + 4));
-          else
-            *reinterpret_cast<uint32_t*>(out + c) = word(p[i], four, i * V);
-        }
-      } else if (n.has(i) && live) {
-        const integral_constant<int, 1> one;
-        if (group != 0) {
-          const float k = K::rounded(K::back(here[c >> shift]));
-          z = quantum_of<INT8>(k, v);
-          if ((c & (group - 1)) == 0) row_scales[c >> shift] = z.all ? top_scale(k, z) : z.scale;
-        }
-        uint32_t code;
-        if (V == 2 && group != 0 && ((c + 1) & (group - 1)) == 0) {  // two groups
-          code = word(p[i], one, i * V);
-          const float k = K::rounded(K::back(here[(c + 1) >> shift]));
-          z = quantum_of<INT8>(k, v);
-          row_scales[(c + 1) >> shift] = z.all ? top_scale(k, z) : z.scale;
-          code |= word(p[i] + (V - 1), one, i * V + V - 1) << 8;
-        } else {
-          code = word(p[i], integral_constant<int, V>(), i * V);
-        }
-        if (V == 2 && reinterpret_cast<uintptr_t>(codes) % 2 == 0) {
-          *reinterpret_cast<uint16_t*>(out + c) = (uint16_t)code;
-        } else {
-          out[c] = (uint8_t)code;
-          if (V == 2) out[c + 1] = (uint8_t)(code >> 8);
-        }
-      }
-    }
-    if (extra && live) {
       if (group != 0) {
-        const float k = K::rounded(K::back(here[n.odd >> shift]));
-        z = quantum_of<INT8>(k, v);
-        if ((n.odd & (group - 1)) == 0)
-          row_scales[n.odd >> shift] = z.all ? top_scale(k, z) : z.scale;
+        top[i] = top_over<EXACT>(top[i], group / V);
+        z = quantum_of<INT8>(K::rounded(top[i]), v);
       }
-      out[n.odd] = (uint8_t)word(&p1, integral_constant<int, 1>(), NU * V);
+      if (n.has(i) && live) {
+        if (group != 0 && (c & (group - 1)) == 0)
+          row_scales[c >> shift] = z.all ? top_scale(K::rounded(top[i]), z) : z.scale;
+        if constexpr (V == 8)
+          *reinterpret_cast<uint2*>(out + c) =
+              make_uint2(sure_word<INT8, 4>(p[i], z, i * V, doubt),
+                         sure_word<INT8, 4>(p[i] + V / 2, z, i * V + 4, doubt));
+        else
+          *reinterpret_cast<uint32_t*>(out + c) = sure_word<INT8, 4>(p[i], z, i * V, doubt);
+      }
     }
-    auto again = [&](int c, const Key& k) {
-      out[c] = code_64<T, W, INT8>(xr + c, rr ? rr + c : nullptr, weight + c, K::value(k));
-    };
 #pragma unroll 1
     for (; doubt; doubt &= doubt - 1) {
       const int j = __ffs(doubt) - 1;
-      if constexpr (V > 2) {
-        Key k = all;
-        if (group != 0) {
+      const int c = n.column(j / V) + j % V;
+      Key k = all;
+      if (group != 0) {
 #pragma unroll
-          for (int h = 0; h < NU; ++h) k = h == j / V ? top[h] : k;
-        }
-        again(n.column(j / V) + j % V, k);
-      } else {
-        const int c = j < NU ? n.column(j) : n.odd, last = j < NU ? c + V : c + 1;
+        for (int h = 0; h < NU; ++h) k = h == j / V ? top[h] : k;
+      }
+      out[c] = code_64<T, W, INT8>(xr + c, rr ? rr + c : nullptr, weight + c, K::value(k));
+    }
+  }
+}
+
+// ---- other rows ----------------------------------------------------------------------------------------
+// Rows that begin or end inside a vector pass through shared memory: read in units of V <= 2 elements, they
+// lie there with column 0 at element 0 or, where the units are one column on, 1; then a thread takes 8
+// columns, as above, from there; its codes go back to shared memory and from there to memory in aligned
+// words.  The block's weights stay in shared memory.  g threads a row; g = 32: blockDim.x / 32 rows beside
+// one another, and nothing waits but lanes for lanes.  (Groups of units of two by atomic maxima instead:
+// 65536 x 1001 bf16 in e4m3 435 us for 142.)
+template <typename T>
+__host__ __device__ constexpr int staged_bytes(int cols) {  // of a row: elements, then codes
+  return ((cols + 7) / 8 * 8 + 8) * (int)(sizeof(T) + 1) + 15 & ~15;
+}
+template <typename T, typename W, int V, bool INT8>
+__global__ void __launch_bounds__(512, 2)
+    rms_norm_8bit_staged_kernel(const NormArgs a, int g, int group, uint8_t* codes, float* scales) {
+  constexpr bool EXACT = sizeof(T) == 2 && sizeof(W) == 2;
+  using K = Top<EXACT>;
+  using Key = typename K::Key;
+  constexpr int NU = 4;  // units of V in flight
+  __shared__ float part[32];
+  __shared__ double part64[32];
+  __shared__ Key part_top[32];
+  extern __shared__ __align__(16) unsigned char staged[];
+  const int padded = (a.cols + 7) / 8 * 8;
+  const int per_block = blockDim.x / g;
+  const int sub = threadIdx.x / g, t = threadIdx.x % g, lane = threadIdx.x & 31;
+  W* weight = reinterpret_cast<W*>(staged);
+  T* s = reinterpret_cast<T*>(staged + padded * sizeof(W) + sub * staged_bytes<T>(a.cols));
+  uint8_t* here = reinterpret_cast<uint8_t*>(s + padded + 8);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const W* given = static_cast<const W*>(a.weight);
+  for (int c = threadIdx.x; c < padded; c += blockDim.x) weight[c] = c < a.cols ? given[c] : from_f32<W>(0.0f);
+  __syncthreads();
+  auto wait = [&] {
+    if (g > 32)
+      __syncthreads();
+    else
+      __syncwarp();
+  };
+  const int shift = group == 32 ? 5 : group == 64 ? 6 : 7;  // columns to groups
+  const int groups = group ? (a.cols + group - 1) >> shift : 1;
+  const float mean = 1.0f / (float)a.cols;
+  const int64_t step = (int64_t)gridDim.x * per_block;
+  // (rows of a block end together, or a warp's alone)
+  for (int64_t row = (int64_t)blockIdx.x * per_block + sub; row < a.rows; row += step) {
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    const T* r = a.residual ? static_cast<const T*>(a.residual) + row * a.r_stride : nullptr;
+    T* sum = static_cast<T*>(a.sum) + row * a.cols;
+    const int on = V == 2 ? (int)row & a.cols & 1 : 0;
+    const int count = a.cols / V;
+    float q = 0.0f;
+    // (a warp's units behind one another: a step's accesses are one address and constants)
 #pragma unroll 1
-        for (int h = c; h < last; ++h) again(h, group != 0 ? K::back(here[h >> shift]) : all);
+    for (int u = (t >> 5) * 32 * NU + lane; u - lane < count; u += g * NU) {
+      Pack<T, V> e[NU], f[NU];
+      const int c = u * V + on;
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        e[i].clear();
+        f[i].clear();
+        if (u + 32 * i < count) {
+          e[i].read(x + c + 32 * i * V);
+          if (r) f[i].read(r + c + 32 * i * V);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        if (r) e[i] = rounded_sum<T, V>(e[i], f[i]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) q = fmaf(e[i].get(j), e[i].get(j), q);
+        if (u + 32 * i < count) {
+          e[i].write(s + c + on + 32 * i * V);
+          if (r) e[i].write(sum + c + 32 * i * V);
+        }
       }
     }
+    if (V == 2 && (a.cols & 1) && t == 0) {
+      const int c = on ? 0 : a.cols - 1;
+      float e[1];
+      load_sum<T, 1>(x + c, r ? r + c : nullptr, e);
+      q = fmaf(e[0], e[0], q);
+      store_pack<T, 1>(s + c + on, e);
+      if (r) store_pack<T, 1>(sum + c, e);
+    }
+    if (t < padded + 1 - a.cols) s[a.cols + on + t] = from_f32<T>(0.0f);  // (as far as is read)
+    // (the row is complete behind the barrier of its sum)
+    const float v = inverse_norm<T>(q, mean, a, g, t, x, r, part, part64);
+    if (g == 32) __syncwarp();
+
+    float p[8];
+    auto products = [&](int c) {  // of 8 columns; their largest
+      Pack<T, 8> e;
+      e.read(s + c);
+      if constexpr (V == 2) {
+        const uint32_t next = *reinterpret_cast<const uint32_t*>(s + c + 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e.w[i] = __funnelshift_r(e.w[i], i < 3 ? e.w[i + 1] : next, 16 * on);
+      }
+      Pack<W, 8> w;
+      w.read(weight + c);
+      Key k = Key(0);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = e.get(j) * w.get(j);
+        k = K::larger(k, K::of(e.get(j), w.get(j), p[j]));
+      }
+      return k;
+    };
+    float* row_scales = scales + row * groups;
+    Key top = Key(0);
+    Quantum z;
+    if (group == 0) {
+      for (int c = t * 8; c < padded; c += g * 8) top = K::larger(top, products(c));
+      top = top_over<EXACT>(top, 32);
+      if (g > 32) {
+        if (lane == 0) part_top[t >> 5] = top;
+        __syncthreads();
+        top = top_over<EXACT>(lane < (g >> 5) ? part_top[lane] : Key(0), 32);
+      }
+      z = quantum_of<INT8>(K::rounded(top), v);
+      if (t == 0) row_scales[0] = z.all ? top_scale(K::rounded(top), z) : z.scale;
+    }
+#pragma unroll 1
+    for (int c = t * 8; c - 8 * lane < padded; c += g * 8) {
+      const bool mine = c < padded;
+      if (group != 0) {
+        top = top_over<EXACT>(mine ? products(c) : Key(0), group / 8);
+        z = quantum_of<INT8>(K::rounded(top), v);
+        if (mine && (c & (group - 1)) == 0)
+          row_scales[c >> shift] = z.all ? top_scale(K::rounded(top), z) : z.scale;
+      } else if (mine) {
+        products(c);
+      }
+      if (mine) {
+        uint32_t doubt = 0;
+        *reinterpret_cast<uint2*>(here + c) = make_uint2(sure_word<INT8, 4>(p, z, 0, doubt),
+                                                         sure_word<INT8, 4>(p + 4, z, 4, doubt));
+#pragma unroll 1
+        for (; doubt; doubt &= doubt - 1) {
+          const int h = c + __ffs(doubt) - 1;
+          here[h] = code_64<T, W, INT8>(s + h + on, nullptr, weight + h, K::value(top));
+        }
+      }
+    }
+    wait();
+    uint8_t* out = codes + row * a.cols;
+    const int head = min((int)(-reinterpret_cast<uintptr_t>(out) & 3), a.cols);
+    const int whole = (a.cols - head) >> 2, tail = (a.cols - head) & 3;
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(here);
+    for (int i = t; i < whole; i += g)
+      *reinterpret_cast<uint32_t*>(out + head + 4 * i) =
+          __funnelshift_r(words[i], words[i + 1], 8 * head);
+    if (t < head) out[t] = here[t];
+    if (t < tail) out[a.cols - tail + t] = here[a.cols - tail + t];
+    if (g == 32) __syncwarp();
   }
 }
 
@@ -526,34 +591,49 @@ __global__ void __launch_bounds__(256)
 template <typename T, typename W, int V, bool INT8>
 static cudaError_t quantize_v(const NormArgs& a, int group, uint8_t* codes, float* scales,
                               cudaStream_t s) {
-  constexpr int NU = V > 2 ? 2 : 8;
-  const size_t key = sizeof(T) == 2 && sizeof(W) == 2 ? 4 : 8;
-  const int64_t units = a.cols / V > 0 ? a.cols / V : 1;
-  const int groups = group ? (a.cols + group - 1) / group : 1;
-  if (units > 1024 * NU)
-    return launch_pdl(rms_norm_8bit_long_kernel<T, W, INT8>, dim3((unsigned)a.rows), dim3(1024),
-                      groups * key, s, a, group, codes, scales);
-  const int g = norm_threads<V>(units, a.rows <= 148 ? NU / 2 : NU, 32);
-  const int block = g <= 32 ? 128 : g;
-  const int per_block = block / g;
-  const size_t smem = V <= 2 && group ? per_block * 3 * groups * key : 0;
-  auto go = [&](auto* kern) {
-    const int64_t need = (a.rows + per_block - 1) / per_block;
-    const unsigned grid =
-        even_grid(stay_grid(reinterpret_cast<const void*>(kern), block, smem, need), need);
+  const bool few = a.rows <= 148;
+  auto go = [&](auto* kern, int g, int block, size_t smem) {
+    const int64_t need = (a.rows + block / g - 1) / (block / g);
+    const unsigned grid = stay_grid(reinterpret_cast<const void*>(kern), block, smem, need);
     return launch_pdl(kern, dim3(grid), dim3(block), smem, s, a, g, group, codes, scales);
   };
-  if (block <= 256) return go(rms_norm_8bit_kernel<T, W, V, NU, 256, INT8>);
-  return go(rms_norm_8bit_kernel<T, W, V, NU, 1024, INT8>);
+  if constexpr (V > 2) {
+    constexpr int NU = 2;
+    const int64_t units = a.cols / V;
+    if (units > 1024 * NU)
+      return quantize_v<T, W, sizeof(T) == 2 ? 2 : 1, INT8>(a, group, codes, scales, s);
+    const int g = norm_threads<V>(units, few ? NU / 2 : NU, 32), block = g <= 32 ? 128 : g;
+    if (block <= 256) return go(rms_norm_8bit_kernel<T, W, NU, 256, INT8>, g, block, 0);
+    return go(rms_norm_8bit_kernel<T, W, NU, 1024, INT8>, g, block, 0);
+  } else {
+    const int units = (a.cols + 7) / 8;
+    int g = norm_threads<8>(units, few ? 1 : 2, 32);
+    if (g > 512) g = 512;
+    const int block = g <= 32 ? 128 : g;
+    const size_t smem = (size_t)units * 8 * sizeof(W) + (size_t)(block / g) * staged_bytes<T>(a.cols);
+    constexpr size_t kMost = 200 * 1024;
+    if (smem <= kMost) {
+      static std::mutex mu;
+      static bool done[64];
+      auto* kern = rms_norm_8bit_staged_kernel<T, W, V, INT8>;
+      if (const cudaError_t e = allow_smem(kern, kMost, mu, done); e != cudaSuccess) return e;
+      return go(kern, g, block, smem);
+    }
+    const int groups = group ? (a.cols + group - 1) / group : 1;
+    const size_t key = sizeof(T) == 2 && sizeof(W) == 2 ? 4 : 8;
+    return launch_pdl(rms_norm_8bit_long_kernel<T, W, INT8>, dim3((unsigned)a.rows), dim3(1024),
+                      groups * key, s, a, group, codes, scales);
+  }
 }
 
 template <typename T>
 static cudaError_t quantize_t(const NormArgs& a, bool int8, int group, uint8_t* codes,
                               float* scales, cudaStream_t s) {
-  // (the codes need half the vectors' alignment at most)
-  const NormUnit unit = norm_unit<T>(a);
-  const bool whole = reinterpret_cast<uintptr_t>(codes) % 8 == 0;
-  return norm_dispatch<T>(a, unit == kVector && !whole ? kSingle : unit, [&](auto w, auto v) {
+  // (vectors' codes are written 8 bytes at a time)
+  NormUnit unit = norm_unit<T>(a);
+  if (unit == kVector && reinterpret_cast<uintptr_t>(codes) % 8 != 0)
+    unit = sizeof(T) == 2 ? kPair : kSingle;
+  return norm_dispatch<T>(a, unit, [&](auto w, auto v) {
     return int8 ? quantize_v<T, decltype(w), decltype(v)::value, true>(a, group, codes, scales, s)
                 : quantize_v<T, decltype(w), decltype(v)::value, false>(a, group, codes, scales, s);
   });

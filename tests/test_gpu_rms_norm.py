@@ -19,6 +19,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from exfold_b200 import _lib as L
 from exfold_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -352,6 +353,71 @@ def test_8bit_far_values(cols, code):
     codes, scales = ops.rms_norm_8bit(tiny, torch.ones(cols, device=DEV), 0.0, dtype=code,
                                       group=None)
     assert torch.equal(codes.double(), codes64(tiny, torch.ones(cols, device=DEV), code, None, 0)[0])
+
+
+@pytest.mark.parametrize("dtype,weight", [(BF16, None), (F16, F32), (F32, None)])
+@pytest.mark.parametrize("wide,start", [(0, 0), (1, 0), (2, 1)])
+def test_8bit_rows_off_vectors(dtype, weight, wide, start):
+    """Rows that begin and end inside a vector, many a block, of one warp and of several."""
+    for rows, cols, group in ((5000, 101, 32), (20001, 9, 64), (3000, 33, 32), (1501, 255, 128),
+                              (149, 513, None), (701, 4001, 64), (151, 45001, None), (9, 7, 128)):
+        x, r, w, *_ = inputs(rows, cols + start, dtype, cols, weight, wide=wide)
+        x, r, w = x[:, start:], r[:, start:], w[start:]
+        for code in (torch.float8_e4m3fn, torch.int8):
+            codes, scales, s = ops.rms_norm_8bit(x, w, 1e-6, residual=r, dtype=code, group=group)
+            assert torch.equal(s, (x.float() + r.float()).to(dtype))
+            q, want = codes64(s, w, code, group, 1e-6)
+            assert torch.equal(codes.double(), q), (rows, cols)
+            near(scales, want, ((chain(cols) / 2 + 14) * E) * want)
+            alone = ops.rms_norm_8bit(x, w, 1e-6, dtype=code, group=group)
+            assert torch.equal(alone[0].double(), codes64(x, w, code, group, 1e-6)[0])
+
+
+@pytest.mark.parametrize("group", [None, 32])
+@pytest.mark.parametrize("code", [torch.float8_e4m3fn, torch.int8])
+def test_8bit_values_that_are_not_finite_in_odd_rows(code, group):
+    """Infinities and NaN stay in their groups, in rows that begin on even and on odd elements."""
+    rows, cols = 12, 99
+    x, _, w, *_ = inputs(rows, cols, F16, 3)
+    at = [0, 31, 32, 63, 64, 98]
+    for i in range(rows):
+        x[i, at[i // 2]] = float("inf")
+    codes, scales = ops.rms_norm_8bit(x, w, dtype=code, group=group)
+    back = ops.dequantize_8bit(codes, scales, group=group, dtype=F32)
+    for i in range(rows):  # (the inverse norm is 0)
+        mine = at[i // 2] // 32 if group else 0
+        for j in range(scales.shape[1]):
+            part = back[i, j * (group or cols):(j + 1) * (group or cols)]
+            assert bool(part.isnan().all()) if j == mine else not part.any()
+    x[3, 5] = float("nan")
+    codes, scales = ops.rms_norm_8bit(x, w, dtype=code, group=group)
+    assert bool(scales[3].isnan().all())
+    if group is None:  # products that round to 0 and to subnormals, beside one far above
+        x = torch.full((4, cols), 6e-8, device=DEV, dtype=F16)
+        x[:, 40] = 3e-5
+        codes, _ = ops.rms_norm_8bit(x, w, 0.0, dtype=code, group=group)
+        assert torch.equal(codes.double(), codes64(x, w, code, group, 0.0)[0])
+
+
+@pytest.mark.parametrize("cols", [256, 101])
+def test_8bit_codes_at_any_address(cols):
+    """Codes of vectors and of odd rows at each of eight addresses; nothing beside them is written."""
+    rows, lib = 37, L.lib()
+    for dtype, d in ((BF16, 1), (F32, 0)):
+        x, r, w, *_ = inputs(rows, cols, dtype, 8)
+        want, scales, s = ops.rms_norm_8bit(x, w, residual=r, group=64)
+        for off in range(8):
+            flat = torch.full((rows * cols + 16,), 77, dtype=torch.uint8, device=DEV)
+            got_s, got_scales = torch.zeros_like(s), torch.zeros_like(scales)
+            L.check(lib.exf_rms_norm_8bit(
+                x.data_ptr(), cols, r.data_ptr(), cols, w.data_ptr(), d, d, rows, cols, 1e-6, 0, 64,
+                got_s.data_ptr(), flat.data_ptr() + off, got_scales.data_ptr(),
+                torch.cuda.current_stream().cuda_stream))
+            codes = flat[off:off + rows * cols].view(rows, cols)
+            assert torch.equal(codes, want.view(torch.uint8))
+            assert torch.equal(got_s, s)
+            near(got_scales, scales.double(), 4 * (chain(cols) / 2 + 14) * E * scales.double())
+            assert bool((flat[:off] == 77).all()) and bool((flat[off + rows * cols:] == 77).all())
 
 
 def test_dequantize_ragged_starts():
