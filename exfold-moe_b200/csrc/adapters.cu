@@ -160,7 +160,7 @@ __device__ __forceinline__ void write_list(const AdapterArgs& p, const AdapterLi
 }
 
 // ---- z of up to 1024 tokens ----------------------------------------------------------------------------------
-// A block takes 4 or 8 tokens and one part of the reduction.  Its work is each distinct adapter's rows, 16 MB at a
+// A block takes up to 8 tokens and one part of the reduction.  Its work is each distinct adapter's rows, R at a
 // time, against all of them (a token keeps its own adapter's column), in units of 32 columns, dealt out to
 // the 8 warps in equal runs: where every token has an adapter of its own, each warp streams one of them.  A
 // lane loads 8 columns (16 bytes) of a row, and the instruction's 16 columns are taken as words 0, 1 and then
