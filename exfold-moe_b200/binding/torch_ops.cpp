@@ -1,18 +1,25 @@
 // The torch side of the norm, the balance loss and the projection with adapters: argument checks, outputs and
-// workspaces, autograd nodes, and one call of the C ABI each (registered as torch.ops.exfold_b200.*; the
+// workspaces, autograd nodes, and one call of the C ABI each.  A Python module (exfold_b200._lib loads it; the
 // documented functions are exfold_b200.ops').
 //
 // Compiled, because at small sizes these operators' time is the host's.  us a call from Python, as Python over
-// ctypes and so: norm of one token 15.5 and 7.4, 8 bits and back 31 and 16, norm of 777 x 1001 fp32 with its
-// gradients 130 and 81, balance loss of 512 x 64 with its gradient 109 and 65.  A backward pass runs in
+// ctypes and so: norm of one token 15.5 and 4.5, 8 bits and back 31 and 9.6, norm of 777 x 1001 fp32 with its
+// gradients 130 and 71, balance loss of 512 x 64 with its gradient 109 and 57.  A backward pass runs in
 // autograd's own thread, where a Python node takes the interpreter's lock and starts from cold caches.
+#include <Python.h>
+
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/library.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
+#include <pybind11/pybind11.h>
 
 #include "exfold_b200.h"
 
@@ -96,8 +103,12 @@ Tensor aligned(const Tensor& t) {
   Tensor c = t.contiguous();
   return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
+// a tensor from the caching allocator, by its function itself (through the dispatcher 0.3 us more)
+Tensor fresh(at::IntArrayRef shape, const at::TensorOptions& options) {
+  return at::detail::empty_cuda(shape, options);
+}
 Tensor bytes(int64_t n, const Tensor& like) {
-  return at::empty({n}, like.options().dtype(at::kByte));
+  return fresh({n}, like.options().dtype(at::kByte));
 }
 
 // t [..., cols] as rows at a constant distance, where they lie if they do
@@ -161,11 +172,11 @@ struct Normed {
 Normed norm_forward(const Tensor& x, const Tensor* residual, const Tensor& weight, double eps) {
   const c10::cuda::CUDAGuard guard(x.device());
   const Rows rows = rows_of(x);
-  Normed out{at::empty(x.sizes(), x.options()), Tensor(), rows.t, rows.stride};
+  Normed out{fresh(x.sizes(), x.options()), Tensor(), rows.t, rows.stride};
   Rows res{Tensor(), 0, 0};
   if (residual) {
     res = rows_of(*residual);
-    out.s = at::empty(x.sizes(), x.options());
+    out.s = fresh(x.sizes(), x.options());
   }
   const Tensor w = weight.contiguous();
   if (rows.n > 0)
@@ -202,8 +213,8 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     const Rows rows = rows_of(x);
     const int64_t cols = weight.size(0);
     Tensor dx, dw, ws;
-    if (want_x || want_r) dx = at::empty(shape, x.options());
-    if (want_w) dw = at::empty({cols}, weight.options());
+    if (want_x || want_r) dx = fresh(shape, x.options());
+    if (want_w) dw = fresh({cols}, weight.options());
     // (of s alone, where y was not used)
     const Tensor dy = grads[0].defined() ? grads[0].contiguous() : at::zeros(shape, x.options());
     const Tensor ds = residual && grads[1].defined() ? grads[1].contiguous() : Tensor();
@@ -250,12 +261,12 @@ variable_list rms_norm_8bit(const Tensor& x, const Tensor& weight, double eps,
   Tensor s;
   if (r) {
     res = rows_of(*r);
-    s = at::empty(x.sizes(), x.options());
+    s = fresh(x.sizes(), x.options());
   }
   auto shape = x.sizes().vec();
-  const Tensor codes = at::empty(shape, x.options().dtype(dtype));
+  const Tensor codes = fresh(shape, x.options().dtype(dtype));
   shape.back() = groups;
-  const Tensor scales = at::empty(shape, x.options().dtype(at::kFloat));
+  const Tensor scales = fresh(shape, x.options().dtype(at::kFloat));
   const Tensor w = weight.contiguous();
   if (rows.n > 0)
     check(api.rms_norm_8bit(rows.t.data_ptr(), rows.stride, pointer(res.t), res.stride, w.data_ptr(),
@@ -280,7 +291,7 @@ Tensor dequantize_8bit(const Tensor& codes, const Tensor& scales, int64_t group,
                     " and scales ", scales.sizes(), " must be [..., H] and [..., groups]");
   const c10::cuda::CUDAGuard guard(codes.device());
   const Tensor c = aligned(codes), s = scales.contiguous();
-  const Tensor out = at::empty(codes.sizes(), codes.options().dtype(dtype));
+  const Tensor out = fresh(codes.sizes(), codes.options().dtype(dtype));
   if (out.numel() > 0)
     check(api.dequantize_8bit(c.data_ptr(), kind, s.data_ptr<float>(), out.numel() / cols, cols,
                               static_cast<int>(group), out.data_ptr(), code_of(out), stream_of(out)));
@@ -303,10 +314,10 @@ variable_list balance_forward(const Tensor& logits, const Tensor& ids, const Ten
                               "exf_balance_loss: at most 1024 experts and 65535 groups");
   auto shape = logits.sizes().vec();
   shape.resize(shape.size() - 2);
-  const Tensor loss = at::empty(shape, logits.options().dtype(at::kFloat));
-  const Tensor valid = at::empty(shape, logits.options().dtype(at::kInt));
+  const Tensor loss = fresh(shape, logits.options().dtype(at::kFloat));
+  const Tensor valid = fresh(shape, logits.options().dtype(at::kInt));
   shape.push_back(experts);
-  const Tensor counts = at::empty(shape, logits.options().dtype(at::kInt));
+  const Tensor counts = fresh(shape, logits.options().dtype(at::kInt));
   const int64_t need =
       api.balance_workspace(static_cast<int>(groups), tokens, static_cast<int>(experts));
   Tensor ws;
@@ -340,7 +351,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &mask = saved[1];
     const c10::cuda::CUDAGuard guard(x.device());
-    const Tensor dloss = grads[0].contiguous(), out = at::empty(x.sizes(), x.options());
+    const Tensor dloss = grads[0].contiguous(), out = fresh(x.sizes(), x.options());
     check(api.balance_backward(
         dloss.data_ptr<float>(), x.data_ptr(), code_of(x),
         static_cast<const uint8_t*>(pointer(mask)), saved[2].data_ptr<int32_t>(),
@@ -417,7 +428,7 @@ Tensor adapted_linear(const Tensor& x, const Tensor& w, const Tensor& a, const T
   const Tensor factor = scale ? scale->to(at::kFloat).contiguous() : Tensor();
   auto shape = x.sizes().vec();
   shape.back() = outer;
-  const Tensor y = at::empty(shape, x.options());
+  const Tensor y = fresh(shape, x.options());
   const int64_t tokens = ids.numel();
   const int64_t need = api.adapted_workspace(tokens, static_cast<int>(inner),
                                              static_cast<int>(outer), static_cast<int>(rank));
@@ -432,19 +443,139 @@ Tensor adapted_linear(const Tensor& x, const Tensor& w, const Tensor& a, const T
 
 }  // namespace
 
-TORCH_LIBRARY(exfold_b200, m) {
-  m.def("bind(str path) -> ()", &bind);
-  m.def("rms_norm(Tensor x, Tensor weight, float eps, Tensor? residual) -> Tensor[]", &rms_norm);
-  m.def(
-      "rms_norm_8bit(Tensor x, Tensor weight, float eps, Tensor? residual, ScalarType dtype, int group)"
-      " -> Tensor[]",
-      &rms_norm_8bit);
-  m.def("dequantize_8bit(Tensor codes, Tensor scales, int group, ScalarType dtype) -> Tensor",
-        &dequantize_8bit);
-  m.def("balance_loss(Tensor logits, Tensor topk_ids, int scoring, Tensor? mask) -> Tensor[]",
-        &balance_loss);
-  m.def(
-      "adapted_linear(Tensor x, Tensor w, Tensor a, Tensor b, Tensor adapter_ids, Tensor? scaling,"
-      " Tensor? status) -> Tensor",
-      &adapted_linear);
+// ---- the Python module ---------------------------------------------------------------------------------
+// Functions of positional arguments, read here: torch's operator calls match a schema and box every argument,
+// 3 us of a call's 7.
+namespace {
+
+const Tensor& tensor_of(PyObject* o) {
+  TORCH_CHECK_TYPE(THPVariable_Check(o), "expected a tensor, got ", Py_TYPE(o)->tp_name);
+  return THPVariable_Unpack(o);
+}
+OptTensor maybe_tensor(PyObject* o) { return o == Py_None ? OptTensor() : OptTensor(tensor_of(o)); }
+double number_of(PyObject* o) {
+  const double d = PyFloat_AsDouble(o);
+  if (d == -1.0 && PyErr_Occurred()) throw python_error();
+  return d;
+}
+int64_t integer_of(PyObject* o) {
+  const int64_t i = PyLong_AsLongLong(o);
+  if (i == -1 && PyErr_Occurred()) throw python_error();
+  return i;
+}
+at::ScalarType dtype_of(PyObject* o) {
+  TORCH_CHECK_TYPE(THPDtype_Check(o), "expected a torch.dtype, got ", Py_TYPE(o)->tp_name);
+  return reinterpret_cast<THPDtype*>(o)->scalar_type;
+}
+void no_tangent(const char* name, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->_fw_grad(0).defined(), name,
+                                " has no forward-mode derivative");
+}
+
+PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }
+PyObject* wrap(const variable_list& l) {
+  THPObjectPtr tuple(PyTuple_New(static_cast<Py_ssize_t>(l.size())));
+  if (!tuple) throw python_error();
+  for (size_t i = 0; i < l.size(); ++i) {
+    PyObject* t = wrap(l[i]);
+    if (!t) throw python_error();
+    PyTuple_SET_ITEM(tuple.get(), static_cast<Py_ssize_t>(i), t);
+  }
+  return tuple.release();
+}
+
+// f(the arguments) -> a tensor or several, without the interpreter's lock where it computes
+template <Py_ssize_t N, typename F>
+PyObject* call(const char* name, Py_ssize_t n, F f) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == N, name, " takes ", N, " arguments, got ", n);
+  return wrap(f());
+  END_HANDLE_TH_ERRORS
+}
+template <typename F>
+auto unlocked(F f) {
+  pybind11::gil_scoped_release release;
+  return f();
+}
+
+PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 1 && PyUnicode_Check(a[0]), "bind takes a path");
+  const char* path = PyUnicode_AsUTF8(a[0]);
+  if (!path) throw python_error();
+  bind(path);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+// (x, weight, eps, residual or None) -> y, or (y, s)
+PyObject* py_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 4, "rms_norm takes 4 arguments, got ", n);
+  const Tensor &x = tensor_of(a[0]), &weight = tensor_of(a[1]);
+  const double eps = number_of(a[2]);
+  const OptTensor residual = maybe_tensor(a[3]);
+  no_tangent("rms_norm", {&x, &weight, get(residual)});
+  const variable_list out = unlocked([&] { return rms_norm(x, weight, eps, residual); });
+  return residual ? wrap(out) : wrap(out[0]);
+  END_HANDLE_TH_ERRORS
+}
+// (x, weight, eps, residual or None, dtype, group) -> (codes, scales), or (codes, scales, s)
+PyObject* py_rms_norm_8bit(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return call<6>("rms_norm_8bit", n, [&] {
+    const Tensor &x = tensor_of(a[0]), &weight = tensor_of(a[1]);
+    const double eps = number_of(a[2]);
+    const OptTensor residual = maybe_tensor(a[3]);
+    const at::ScalarType dtype = dtype_of(a[4]);
+    const int64_t group = integer_of(a[5]);
+    return unlocked([&] { return rms_norm_8bit(x, weight, eps, residual, dtype, group); });
+  });
+}
+// (codes, scales, group, dtype) -> values
+PyObject* py_dequantize_8bit(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return call<4>("dequantize_8bit", n, [&] {
+    const Tensor &codes = tensor_of(a[0]), &scales = tensor_of(a[1]);
+    const int64_t group = integer_of(a[2]);
+    const at::ScalarType dtype = dtype_of(a[3]);
+    return unlocked([&] { return dequantize_8bit(codes, scales, group, dtype); });
+  });
+}
+// (logits, topk_ids, scoring, mask or None) -> (loss, counts)
+PyObject* py_balance_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return call<4>("balance_loss", n, [&] {
+    const Tensor &logits = tensor_of(a[0]), &ids = tensor_of(a[1]);
+    const int64_t scoring = integer_of(a[2]);
+    const OptTensor mask = maybe_tensor(a[3]);
+    no_tangent("balance_loss", {&logits});
+    return unlocked([&] { return balance_loss(logits, ids, scoring, mask); });
+  });
+}
+// (x, w, a, b, adapter_ids, scaling or None, status or None) -> y
+PyObject* py_adapted_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return call<7>("adapted_linear", n, [&] {
+    const Tensor &x = tensor_of(a[0]), &w = tensor_of(a[1]), &down = tensor_of(a[2]),
+                 &up = tensor_of(a[3]), &ids = tensor_of(a[4]);
+    const OptTensor scaling = maybe_tensor(a[5]), status = maybe_tensor(a[6]);
+    return unlocked([&] { return adapted_linear(x, w, down, up, ids, scaling, status); });
+  });
+}
+
+PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) {
+  return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
+}
+PyMethodDef methods[] = {
+    {"bind", fast(py_bind), METH_FASTCALL, nullptr},
+    {"rms_norm", fast(py_rms_norm), METH_FASTCALL, nullptr},
+    {"rms_norm_8bit", fast(py_rms_norm_8bit), METH_FASTCALL, nullptr},
+    {"dequantize_8bit", fast(py_dequantize_8bit), METH_FASTCALL, nullptr},
+    {"balance_loss", fast(py_balance_loss), METH_FASTCALL, nullptr},
+    {"adapted_linear", fast(py_adapted_linear), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "libexfold_b200_torch", nullptr, -1, methods,
+                          nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit_libexfold_b200_torch() {
+  return PyModule_Create(&module_def);
 }

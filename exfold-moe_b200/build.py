@@ -7,7 +7,7 @@ no fast-math, --fmad=false so every float operation is the one written) into
 exfold-moe_b200/_build/, then linked into exfold-moe_b200/lib/libexfold_b200.so with the CUDA
 runtime linked statically.  Objects are rebuilt only when a source or header is newer.
 binding/torch_ops.cpp (host code: autograd nodes over the C ABI) is compiled by g++ against the
-installed torch into lib/libexfold_b200_torch.so.
+installed torch into the Python module lib/libexfold_b200_torch.so.
 """
 
 from __future__ import annotations
@@ -17,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -62,8 +63,9 @@ def torch_command() -> list[str]:
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
             "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
             f"-I{INCLUDE}", *(arg for p in include_paths() for arg in ("-isystem", p)), "-isystem",
-            str(cuda), str(TORCH_SRC), "-o", str(TORCH_LIB), f"-L{libs}", "-ltorch_cpu",
-            "-ltorch_cuda", "-lc10", "-lc10_cuda", "-ldl", f"-Wl,-rpath,{libs}"]
+            str(cuda), "-isystem", sysconfig.get_paths()["include"], str(TORCH_SRC), "-o",
+            str(TORCH_LIB), f"-L{libs}", "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10",
+            "-lc10_cuda", "-ldl", f"-Wl,-rpath,{libs}"]
 
 
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:

@@ -10,7 +10,9 @@
 // tiles that are there anyway, and y is written once, rounded once.  The GEMM starts on x and W while z is
 // still being computed.  Up to 128 tokens, where every token may have an adapter of its own, the GEMM's threads
 // add z B to its sums instead, a token's row from its own adapter, in fp32 (64 tokens of 32 adapters, rank 16:
-// as columns of the reduction 23.8 us); up to 32 tokens that follows a kernel of warp matrix instructions.
+// as columns of the reduction 23.8 us, so 17); up to 32 tokens that follows a kernel of warp matrix
+// instructions.  8192 tokens of 8 adapters, rank 64, 2048 -> 4096: 145 us, of
+// which z 22; 0.60 of a dense product's rate, the adapters' columns included.  Bound by the tensor pipe of single SMs.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -26,9 +28,15 @@
 namespace exf {
 using namespace tc;
 
-constexpr int kFewAdapted = 32;       // tokens of the kernel without tiles
-constexpr int kRowTokens = 128;       // tokens whose adapters are added row by row, z in fp32
-constexpr int kDownTokens = 1024;     // tokens of adapter_down_kernel
+// The tokens up to which a form is taken; us of this form and of the next, 2048 -> 4096 bf16.
+// The kernel without tiles (it holds no more): 16 tokens of 32 adapters, rank 16: 7.3 and 15.4; 32: 11.2, 14.7.
+constexpr int kFewAdapted = 32;
+// Adapters added row by row, z in fp32: 65 tokens of 32 adapters, rank 16: 17.5 and 22.7; 128: 25.6, 25.8, of 8
+// adapters, rank 64: 38, 32; 256: 32.5, 32.4, in 4 runs of rank 64: 39.6, 24.6.
+constexpr int kRowTokens = 128;
+// z by adapter_down_kernel: 512 tokens of 32 adapters, rank 16: 48 and 77; 1024: 73, 95, in 4 runs of rank 64: 34,
+// 32; 2048: 53.5, 49.
+constexpr int kDownTokens = 1024;
 constexpr int kAdaptedThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue, warps 6-9 adapters
 constexpr int kABM = 128;           // tokens of a tile
 constexpr int kABK = 64;            // columns of a stage: 128 bytes

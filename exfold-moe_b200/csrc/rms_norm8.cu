@@ -9,7 +9,9 @@
 // definition (products of fp32 values with fp32 weights to 2^-53).  A group with a product that is not
 // finite in fp32 gets codes 0 and a NaN scale, a group of zeros codes 0 and scale 0.
 //
-// Bound by memory: x, residual in, sum and codes out, once each.
+// Bound by memory (x, residual in, sum and codes out, once each) and, beside it, by the instructions of the
+// codes: 32768 x 4096 bf16 with a residual, a scale a row, 167 us = 0.86 of a copy's rate; e4m3 in groups of
+// 128 199 us = 0.72.
 #include <mutex>
 
 #include "exf_launch.h"
@@ -520,6 +522,7 @@ __global__ void __launch_bounds__(1024)
 // ---- reading back -------------------------------------------------------------------------------
 // out = code * scale, rounded.  A thread takes 16 values that lie together, whichever rows they belong to,
 // so every access is a whole vector whatever the row's length; most lie in one group, and need one scale.
+// 32768 x 4096 to bf16: 72 us, 0.85 of a copy's rate.
 template <typename T, bool INT8>
 __global__ void __launch_bounds__(256)
     dequantize_8bit_kernel(const uint8_t* codes, const float* scales, int64_t total, int cols,

@@ -8,6 +8,8 @@ RuntimeError at first use.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 from pathlib import Path
@@ -124,12 +126,11 @@ _torch_ops = None
 
 
 def torch_ops():
-    """The operators of libexfold_b200_torch.so, beside the library (RuntimeError if it has not been
-    built)."""
+    """The module libexfold_b200_torch.so, beside the library (RuntimeError if it has not been built)."""
     global _torch_ops
     if _torch_ops is None:
         lib()
-        import torch
+        import torch  # noqa: F401 (the module's libraries)
 
         with _lock:
             if _torch_ops is None:
@@ -137,9 +138,12 @@ def torch_ops():
                 if not path.is_file():
                     raise RuntimeError(f"ExFold B200 torch binding is missing: {path} "
                                        "(build it with: python exfold-moe_b200/build.py)")
-                torch.ops.load_library(str(path))
-                torch.ops.exfold_b200.bind(str(library_path()))
-                _torch_ops = torch.ops.exfold_b200
+                name = path.name.split(".")[0]
+                loader = importlib.machinery.ExtensionFileLoader(name, str(path))
+                module = importlib.util.module_from_spec(
+                    importlib.util.spec_from_file_location(name, path, loader=loader))
+                module.bind(str(library_path()))
+                _torch_ops = module
     return _torch_ops
 
 

@@ -643,10 +643,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     x, residual and weight (once, in reverse mode; forward mode is refused); nothing is kept for the
     backward pass but s.
     """
-    if _has_tangent(x, weight, residual):
-        raise NotImplementedError("rms_norm has no forward-mode derivative")
-    out = L.torch_ops().rms_norm.default(x, weight, eps, residual)
-    return out[0] if residual is None else tuple(out)
+    return L.torch_ops().rms_norm(x, weight, eps, residual)
 
 
 def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -660,7 +657,7 @@ def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     code * scale (`dequantize_8bit`).  A group with a value that is not finite reads back as NaN.  H up to
     2^17.  For inference: the result carries no gradient.
     """
-    return tuple(L.torch_ops().rms_norm_8bit.default(x, weight, eps, residual, dtype, _group(group)))
+    return L.torch_ops().rms_norm_8bit(x, weight, eps, residual, dtype, _group(group))
 
 
 def _group(group: int | None) -> int:
@@ -671,7 +668,7 @@ def _group(group: int | None) -> int:
 def dequantize_8bit(codes: torch.Tensor, scales: torch.Tensor, group: int | None = 128,
                     dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values code * scale of `rms_norm_8bit`'s codes and scales, rounded to dtype."""
-    return L.torch_ops().dequantize_8bit.default(codes, scales, _group(group), dtype)
+    return L.torch_ops().dequantize_8bit(codes, scales, _group(group), dtype)
 
 
 # ---- balance loss -------------------------------------------------------------------------------
@@ -690,9 +687,7 @@ def balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor, scoring: str = "s
     """
     if scoring not in ("softmax", "sigmoid"):
         raise ValueError(f"scoring must be softmax or sigmoid, got {scoring!r}")
-    if _has_tangent(logits):
-        raise NotImplementedError("balance_loss has no forward-mode derivative")
-    return tuple(L.torch_ops().balance_loss.default(logits, topk_ids, _SCORING[scoring], mask))
+    return L.torch_ops().balance_loss(logits, topk_ids, _SCORING[scoring], mask)
 
 
 # ---- projection with adapters -------------------------------------------------------------------
@@ -708,4 +703,4 @@ def adapted_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
     and rank are multiples of 8, rank at most 128.  Sums are fp32; y is rounded once.  `status` as in
     `fused_experts`.  For inference: the result carries no gradient.
     """
-    return L.torch_ops().adapted_linear.default(x, w, a, b, adapter_ids, scaling, status)
+    return L.torch_ops().adapted_linear(x, w, a, b, adapter_ids, scaling, status)
