@@ -26,45 +26,48 @@ namespace exf {
 
 constexpr int kBalanceThreads = 256;
 
-// e^x within 2^-21: 2^t of the rounded product t = x log2(e), corrected by what the rounding left.
+// e^x within 2^-21: 2^t of the rounded product t = x log2(e), corrected by what the rounding left, x - t ln 2.
 __device__ __forceinline__ float exp_near(float x) {
-  x = x < -150.0f ? -150.0f : x;  // (0 below; -inf would make a NaN of the rest; NaN stays)
+  // (0 below -150; -inf would make a NaN of the rest; NaN stays)
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(x), "f"(-150.0f));
   const float t = x * 1.44269502f;
-  const float rest = fmaf(x, 1.44269502f, -t) + x * 1.92596299e-8f;
   float e;
   asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(t));
-  return fmaf(e, rest * 0.693147182f, e);
+  return fmaf(e, fmaf(t, 1.90465432e-9f, fmaf(t, -0.693147182f, x)), e);
 }
 
-// A row's scores on `lanes` neighbouring lanes, in place of its logits; SLOPE: 1 - sigmoid in `slope`.
-// Columns past the last hold -inf.
+// A row's scores on `lanes` neighbouring lanes, in place of its logits, times the returned factor, the inverse
+// of their sum; SLOPE: 1 - sigmoid in `slope`.  Columns past the last hold -inf.
 template <int C, bool SIGMOID, bool SLOPE>
-__device__ __forceinline__ void scores(float (&x)[C], float (&slope)[SLOPE ? C : 1], int lanes) {
+__device__ __forceinline__ float scores(float (&x)[C], float (&slope)[SLOPE ? C : 1], int lanes) {
   float m = x[0];
 #pragma unroll
   for (int j = 1; j < C; ++j) m = fmaxf(m, x[j]);
   for (int d = lanes / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  // sigmoid(x) is e^x to the last bit where the row's largest is below -30: that row is a softmax too
-  const bool soft = !SIGMOID || m < -30.0f;
-  const float shift = soft && m > -__int_as_float(0x7f800000) ? m : 0.0f;
   float sum = 0.0f;
+  // sigmoid(x) is e^x to the last bit where the row's largest is below -30: that row is a softmax too
+  if (!SIGMOID || m < -30.0f) {
+    const float shift = m > -__int_as_float(0x7f800000) ? m : 0.0f;
 #pragma unroll
-  for (int j = 0; j < C; ++j) {
-    if (SIGMOID) {
-      const float e = exp_near(soft ? x[j] - shift : -fabsf(x[j]));
-      const bool high = x[j] >= 0.0f;
-      const float r = __fdividef(1.0f, 1.0f + e);
-      if (SLOPE) slope[j] = soft ? 1.0f : high ? e * r : r;
-      x[j] = soft ? e : high ? r : e * r;
-    } else {
+    for (int j = 0; j < C; ++j) {
       x[j] = exp_near(x[j] - shift);
+      if (SLOPE) slope[j] = 1.0f;
+      sum += x[j];
     }
-    sum += x[j];
-  }
-  for (int d = lanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  } else {
 #pragma unroll
-  for (int j = 0; j < C; ++j) x[j] *= inv;
+    for (int j = 0; j < C; ++j) {
+      const bool high = x[j] >= 0.0f;
+      const float e = exp_near(-fabsf(x[j]));
+      const float r = __fdividef(1.0f, 1.0f + e), low = e * r;
+      if (SLOPE) slope[j] = high ? low : r;
+      x[j] = high ? r : low;
+      sum += x[j];
+    }
+  }
+  __syncwarp();
+  for (int d = lanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  return sum == 0.0f ? 0.0f : 1.0f / sum;
 }
 
 // A lane's columns: unit u = lane + lanes * i of V columns each.
@@ -77,19 +80,24 @@ __device__ __forceinline__ void fetch_logits(const T* row, int l, int lanes, int
 }
 template <typename T, int V, int NV>
 __device__ __forceinline__ void take_logits(const Pack<T, V> (&k)[NV], int l, int lanes, int units,
-                                            bool there, float (&x)[NV * V]) {
+                                            float (&x)[NV * V]) {
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      x[i * V + j] =
-          there && l + lanes * i < units ? k[i].get(j) : -__int_as_float(0x7f800000);
+    for (int j = 0; j < V; ++j) x[i * V + j] = k[i].get(j);
+  if (lanes * NV == units) return;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (l + lanes * i >= units) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[i * V + j] = -__int_as_float(0x7f800000);
+    }
 }
 
 // Block b of a group takes tokens [T b / blocks, T (b + 1) / blocks): its sums of p, counts and number of
 // tokens.
 template <typename T, int V, int NV, bool SIGMOID>
-__global__ void __launch_bounds__(kBalanceThreads, NV * V <= 16 ? 4 : 2)
+__global__ void __launch_bounds__(kBalanceThreads, (NV * V <= 16 ? 4 : 2) / (V > 1 ? 1 : 2))
     balance_sums_kernel(const BalanceArgs a, const void* ids, bool ids64, int lanes, float* psum,
                         int32_t* pcount, int32_t* pvalid, int32_t* ticket) {
   extern __shared__ float shared[];  // [warps][experts] sums, [experts] counts
@@ -111,20 +119,50 @@ __global__ void __launch_bounds__(kBalanceThreads, NV * V <= 16 ? 4 : 2)
   float acc[NV * V] = {};
   int mine = 0;
   Pack<T, V> next[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) next[i].clear();
   const int64_t first = t0 + (threadIdx.x >> 5) * per_warp + lane / lanes, step = kWarps * per_warp;
   auto kept = [&](int64_t t) { return t < t1 && !(mask && !mask[t]); };
-  bool there = kept(first);
+  // (the mask is read a token further ahead than the logits, which wait for it)
+  bool there = kept(first), ahead = kept(first + step);
   fetch_logits<T, V, NV>(logits + first * e, l, lanes, units, there, next);
+  // the routes are counted while the first logits are on their way (a block has fewer than 2^32 of them)
+  const uint32_t routes = (uint32_t)(t1 - t0) * (uint32_t)a.top_k;
+  const int64_t at = ((int64_t)group * a.tokens + t0) * a.top_k;
+  constexpr int kRoutes = 8;
+  for (uint32_t i0 = threadIdx.x; i0 < routes; i0 += kRoutes * kBalanceThreads) {
+    int32_t id[kRoutes];
+#pragma unroll
+    for (int j = 0; j < kRoutes; ++j) {
+      const uint32_t i = i0 + j * kBalanceThreads;
+      id[j] = -1;
+      if (i < routes && !(mask && !mask[t0 + i / (uint32_t)a.top_k])) {
+        if (ids64) {
+          const int64_t wide = static_cast<const int64_t*>(ids)[at + i];
+          if (wide >= 0 && wide < e) id[j] = (int32_t)wide;
+        } else {
+          id[j] = static_cast<const int32_t*>(ids)[at + i];
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kRoutes; ++j)
+      if (id[j] >= 0 && id[j] < e) atomicAdd(count + id[j], 1);
+  }
   for (int64_t t = first; t - lane / lanes < t1; t += step) {
     float x[NV * V], none[1];
-    take_logits<T, V, NV>(next, l, lanes, units, there, x);
-    mine += there && l == 0;
+    take_logits<T, V, NV>(next, l, lanes, units, x);
+    const bool now = there;
+    mine += now && l == 0;
     // the next token's logits are on their way during this one's sums
-    there = kept(t + step);
+    there = ahead;
     fetch_logits<T, V, NV>(logits + (t + step) * e, l, lanes, units, there, next);
-    scores<NV * V, SIGMOID, false>(x, none, lanes);
+    ahead = kept(t + 2 * step);
+    const float inv = scores<NV * V, SIGMOID, false>(x, none, lanes);
+    if (now) {  // (a token left out went along with whatever was there)
 #pragma unroll
-    for (int j = 0; j < NV * V; ++j) acc[j] += x[j];
+      for (int j = 0; j < NV * V; ++j) acc[j] = fmaf(x[j], inv, acc[j]);
+    }
   }
   // the lanes of a warp that share columns, then the warps
 #pragma unroll
@@ -138,13 +176,6 @@ __global__ void __launch_bounds__(kBalanceThreads, NV * V <= 16 ? 4 : 2)
     }
   }
   if (mine) atomicAdd(&valid, mine);
-  const int64_t at = (int64_t)group * a.tokens * a.top_k;
-  for (int64_t i = t0 * a.top_k + threadIdx.x; i < t1 * a.top_k; i += kBalanceThreads) {
-    if (mask && !mask[i / a.top_k]) continue;
-    const int64_t id = ids64 ? static_cast<const int64_t*>(ids)[at + i]
-                             : static_cast<const int32_t*>(ids)[at + i];
-    if (id >= 0 && id < e) atomicAdd(count + id, 1);
-  }
   __syncthreads();
   const int64_t slot = (int64_t)group * gridDim.x + blockIdx.x;
   for (int c = threadIdx.x; c < e; c += kBalanceThreads) {
@@ -160,14 +191,16 @@ __global__ void __launch_bounds__(kBalanceThreads, NV * V <= 16 ? 4 : 2)
   }
 }
 
-// The joined sums: a block takes 8 experts of a group (a sector of each block's sums), 32 threads an expert;
+// The joined sums: a block takes 8 experts of a group (a sector of each block's sums), 64 threads an expert;
 // the last block of a group to finish adds the experts' products c_e P_e, in order.
-__global__ void __launch_bounds__(256)
+constexpr int kJoinThreads = 512;
+__global__ void __launch_bounds__(kJoinThreads)
     balance_join_kernel(const float* psum, const int32_t* pcount, const int32_t* pvalid, int blocks,
                         int experts, int top_k, double* product, int32_t* ticket, float* loss,
                         int32_t* counts, int32_t* valid) {
-  __shared__ double sums[8][8];
-  __shared__ int32_t routes[8][8];
+  constexpr int kWarps = kJoinThreads / 32;
+  __shared__ double sums[kWarps][8];
+  __shared__ int32_t routes[kWarps][8];
   __shared__ int tokens;
   __shared__ bool last;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -178,8 +211,8 @@ __global__ void __launch_bounds__(256)
   double s = 0.0;
   int32_t r = 0;
   if (c < experts) {
-#pragma unroll 8
-    for (int b = threadIdx.x >> 3; b < blocks; b += 32) {
+#pragma unroll 5
+    for (int b = threadIdx.x >> 3; b < blocks; b += kJoinThreads / 8) {
       s += (double)__ldcg(psum + (base + b) * experts + c);
       r += __ldcg(pcount + (base + b) * experts + c);
     }
@@ -196,7 +229,7 @@ __global__ void __launch_bounds__(256)
   __syncthreads();
   if (threadIdx.x < 8) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) {
+    for (int i = 1; i < kWarps; ++i) {
       s += sums[i][x];
       r += routes[i][x];
     }
@@ -214,7 +247,7 @@ __global__ void __launch_bounds__(256)
   __syncthreads();
   if (!last) return;
   int n = 0;
-  for (int b = threadIdx.x; b < blocks; b += 256) n += __ldcg(pvalid + base + b);
+  for (int b = threadIdx.x; b < blocks; b += kJoinThreads) n += __ldcg(pvalid + base + b);
   if (n) atomicAdd(&tokens, n);
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -255,25 +288,29 @@ __global__ void __launch_bounds__(kBalanceThreads)
     const bool in = t < a.tokens;
     const bool there = in && !(mask && !mask[t]);
     Pack<T, V> k[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) k[i].clear();
     float x[NV * V], slope[SIGMOID ? NV * V : 1];
     fetch_logits<T, V, NV>(logits + t * e, l, lanes, units, there, k);
-    take_logits<T, V, NV>(k, l, lanes, units, there, x);
-    scores<NV * V, SIGMOID, SIGMOID>(x, slope, lanes);
+    take_logits<T, V, NV>(k, l, lanes, units, x);
+    const float inv = scores<NV * V, SIGMOID, SIGMOID>(x, slope, lanes);
     float dot = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV * V; ++j) dot = fmaf(x[j], c[j], dot);
     for (int d = lanes / 2; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+    dot *= inv;
     if (!in) continue;  // (the loop's condition is the warp's: no lane waits for another after it)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int u = l + lanes * i;
       if (u < units) {
-        float d[V];
+        float d[V] = {};
+        if (there) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          d[j] = size * (x[i * V + j] * (c[i * V + j] - dot));
-          if (SIGMOID) d[j] *= slope[SIGMOID ? i * V + j : 0];
-          if (!there) d[j] = 0.0f;
+          for (int j = 0; j < V; ++j) {
+            d[j] = size * (x[i * V + j] * inv * (c[i * V + j] - dot));
+            if (SIGMOID) d[j] *= slope[SIGMOID ? i * V + j : 0];
+          }
         }
         store_pack<T, V>(out + t * e + u * V, d);
       }
@@ -353,7 +390,7 @@ cudaError_t launch_balance_loss(const BalanceArgs& a, const void* ids, bool ids6
             pvalid, ticket);
       });
   if (err != cudaSuccess) return err;
-  return launch_pdl(balance_join_kernel, dim3(join_blocks(a.experts), a.groups), dim3(256), 0, s,
+  return launch_pdl(balance_join_kernel, dim3(join_blocks(a.experts), a.groups), dim3(kJoinThreads), 0, s,
                     static_cast<const float*>(psum), static_cast<const int32_t*>(pcount),
                     static_cast<const int32_t*>(pvalid), (int)blocks, a.experts, a.top_k, product,
                     ticket, loss, counts, valid);
