@@ -11,7 +11,6 @@
 //
 // Bound by memory: a value is read and written once.  A row lies in the registers of its threads between
 // its reduction and its results.
-#include <mutex>
 
 #include "exf_launch.h"
 #include "exf_norm.cuh"
