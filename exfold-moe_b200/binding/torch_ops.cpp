@@ -347,7 +347,7 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    if (!grads[0].defined()) return once({Tensor(), Tensor(), Tensor(), Tensor()});
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &mask = saved[1];
     const c10::cuda::CUDAGuard guard(x.device());
