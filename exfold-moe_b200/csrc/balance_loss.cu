@@ -44,8 +44,9 @@ __device__ __forceinline__ float scores(float (&x)[C], float (&slope)[SLOPE ? C 
   for (int j = 1; j < C; ++j) m = fmaxf(m, x[j]);
   for (int d = lanes / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
   float sum = 0.0f;
-  // sigmoid(x) is e^x to the last bit where the row's largest is below -30: that row is a softmax too
-  if (!SIGMOID || m < -30.0f) {
+  // sigmoid(x) is e^x to the last bit where the row's largest is below -18 (e^-18 < 2^-25): that row is a
+  // softmax too
+  if (!SIGMOID || m < -18.0f) {
     const float shift = m > -__int_as_float(0x7f800000) ? m : 0.0f;
 #pragma unroll
     for (int j = 0; j < C; ++j) {

@@ -368,10 +368,11 @@ EXF_API int exf_rms_norm_backward(const void* dy, const void* dsum, const void* 
  * (1 when routes and scores are even; 0 for N = 0).  logits [groups][tokens][experts] EXF_F32, EXF_BF16
  * or EXF_F16; ids [groups][tokens][top_k] EXF_I32 or EXF_I64, what lies outside [0, experts) counts
  * nowhere; loss fp32 [groups], counts int32 [groups][experts], valid int32 [groups] (N).  A token whose
- * logits are all -infinity has p = 0.  exf_balance_loss_backward: dlogits of the logits' type from dloss
- * fp32 [groups] and the forward pass's counts and valid (the counts carry no gradient); left-out tokens
- * get zeros.  At most 1024 experts, 65535 groups, 2^31 - 1 routes a group.  Sums are joined in a fixed
- * order.  workspace: exf_balance_loss_workspace_bytes(), for the current device, 8-byte aligned. */
+ * logits are all -infinity has p = 0; a sigmoid, or a softmax's term over its row's largest, that is below
+ * 2^-126 counts as 0.  exf_balance_loss_backward: dlogits of the logits' type from dloss fp32 [groups] and
+ * the forward pass's counts and valid (the counts carry no gradient); left-out tokens get zeros.  At most
+ * 1024 experts, 65535 groups, 2^31 - 1 routes a group.  Sums are joined in a fixed order.  workspace:
+ * exf_balance_loss_workspace_bytes(), for the current device, 8-byte aligned. */
 EXF_API int64_t exf_balance_loss_workspace_bytes(int groups, int64_t tokens, int experts);
 EXF_API int exf_balance_loss(const void* logits, int dtype, const void* ids, int id_dtype,
                              const uint8_t* mask, int groups, int64_t tokens, int experts, int top_k,

@@ -279,3 +279,20 @@ def test_graph_streams_order_and_refusals():
         dual = torch.autograd.forward_ad.make_dual(x, x)
         with pytest.raises(NotImplementedError):
             ops.balance_loss(dual, ids)
+
+
+def test_low_sigmoid_rows():
+    """Rows whose sigmoids are all small, on both sides of where they become softmaxes."""
+    for top in (-10.0, -17.9, -18.1, -29.0, -31.0, -80.0):
+        g = torch.Generator(device=DEV).manual_seed(1)
+        x = top - 60.0 * torch.rand(1, 300, 96, generator=g, device=DEV)
+        x[:, :, 5] = top
+        ids = torch.randint(0, 96, (1, 300, 4), generator=g, device=DEV).int()
+        dloss = torch.full((1,), 300.0, device=DEV)
+        a = x.clone().requires_grad_()
+        loss, counts = ops.balance_loss(a, ids, scoring="sigmoid")
+        grad, = torch.autograd.grad(loss, a, dloss)
+        (want, c, dx), (eloss, edx) = formula(x, ids, None, dloss, "sigmoid")
+        assert torch.equal(counts, c)
+        near(loss.detach(), want, eloss)
+        near(grad, dx, edx)
