@@ -546,8 +546,14 @@ struct AdaptedCfg {
   static constexpr int kStages = (224 * 1024 - kExtras * kExtra) / kStage;
   static constexpr int kTmem = 2 * NT;  // two accumulators, a power of two
 };
+// Marks of tiles that left columns of B out, in a ring over the block's tiles that have stages of adapters at
+// all.  A stage is filled once the one kExtras before it has been multiplied, in a tile that began behind the
+// epilogue of its last but one; so at most the tiles of kExtras + 1 stages, and one before them, have marks that
+// are still to be read.
+constexpr int kMarks = 8;
 template <int NT>
 struct AdaptedSmem {
+  static_assert(AdaptedCfg<NT>::kExtras + 2 <= kMarks, "marks are read before they are written over");
   alignas(1024) uint8_t tiles[AdaptedCfg<NT>::kStages][AdaptedCfg<NT>::kStage];
   alignas(1024) uint8_t extra[AdaptedCfg<NT>::kExtras][AdaptedCfg<NT>::kExtra];
   alignas(8) uint64_t full[AdaptedCfg<NT>::kStages];
@@ -559,7 +565,7 @@ struct AdaptedSmem {
   alignas(8) uint64_t drain;
   uint32_t tmem_base;
   int failed;
-  int broken[2];  // by accumulator: 1 + the last tile that left columns of B out
+  int broken[kMarks];  // 1 + the last tile that left columns of B out
 };
 template <int NT>
 constexpr size_t adapted_smem_bytes() { return sizeof(AdaptedSmem<NT>) + 1024; }
@@ -678,7 +684,7 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
     }
     mbar_init(&sm.drain, 1);
     sm.failed = 0;
-    sm.broken[0] = sm.broken[1] = 0;
+    for (int m = 0; m < kMarks; ++m) sm.broken[m] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(&sm.tmem_base, C::kTmem);
@@ -801,6 +807,7 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
     const int q = warp & 3;
     const int outer = p.a.outer;
     int i = 0;
+    uint32_t met = 0;  // tiles with stages of adapters
     for (int t = blockIdx.x; t < ntiles; t += gridDim.x, ++i) {
       const Tile tl = tile_of(t);
       const int b = i & 1;
@@ -808,9 +815,10 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
       fence_after_sync();
       const int row = tl.mt * kABM + q * 32 + lane;
       const uint32_t taddr = tmem + static_cast<uint32_t>(b * NT) + ((uint32_t)(q * 32) << 16);
-      const bool broken = *const_cast<volatile int*>(&sm.broken[b]) == t + 1;
       int q0 = 0, q1 = 0;
       extra_of(tl, q0, q1);  // (by whole warps)
+      const bool broken =
+          q1 > q0 && *const_cast<volatile int*>(&sm.broken[met++ % kMarks]) == t + 1;
 #pragma unroll 1
       for (int c = 0; c < NT; c += 32) {
         float v[32];
@@ -845,8 +853,8 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
     const int tokens = (int)p.a.tokens, rank = p.a.rank, outer = p.a.outer;
     constexpr int kRows = (NT + 127) / 128, kBehind = C::kExtras - 1;
     const int piece = (tid >> 2 & 1) << 4;  // of the first half of the ranks
-    uint32_t h = 0;  // stages issued
-    int i = 0;
+    uint32_t h = 0;    // stages issued
+    uint32_t met = 0;  // tiles with stages, this one among them
     bool ok = true;
     // stage j has arrived: looked over, to the other proxy (it is read by the MMA), one arrival a warp
     auto hand_over = [&](uint32_t j, int t) {
@@ -859,17 +867,18 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
           uint4* v = reinterpret_cast<uint4*>(at + (tid + 128 * e) * 32 + (piece ^ (k << 4)));
           if (not_finite<BF16>(*v)) {
             *v = make_uint4(0, 0, 0, 0);
-            *const_cast<volatile int*>(&sm.broken[i & 1]) = t + 1;
+            *const_cast<volatile int*>(&sm.broken[(met - 1) % kMarks]) = t + 1;
           }
         }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.extra_full[j % C::kExtras]);
     };
-    for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++i) {
+    for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
       const Tile tl = tile_of(t);
       int q0, q1;
       extra_of(tl, q0, q1);
+      met += q1 > q0;
       const int token = tl.mt * kABM + tid;
       const int place = token < tokens ? p.l.place[token] : 255;
       const uint16_t* z = p.l.z16 + (int64_t)(token < tokens ? token : 0) * width * 32;
