@@ -4,11 +4,11 @@
 //
 // Two launches.  adapter_down_kernel computes z in fp32, each token against its own adapter, by warp matrix
 // instructions: x and the adapters in use are read once.  Then one GEMM over W whose reduction goes on over
-// z and B: a tile of 128 tokens lists its distinct adapters, and for each the reduction gains 2 rank columns,
-// z of that adapter's tokens (0 for the others) as the sum of two 16-bit terms (what one would round away is
-// in the other: 2^-16 of z in bf16), both against B.  So the adapters' part costs matrix instructions on
-// tiles that are there anyway, and y is written once, rounded once.  The GEMM starts on x and W while z is
-// still being computed.  Up to 128 tokens, where every token may have an adapter of its own, the GEMM's threads
+// z and B: a tile of 128 tokens lists its distinct adapters, and for each the reduction gains columns for z of
+// that adapter's tokens (0 for the others) as the sum of three bf16 terms, which hold an fp32 value's 24 bits and
+// its range, against B (fp16: against the two bf16 terms that hold B).  So the adapters' part costs matrix
+// instructions on tiles that are there anyway, z keeps what fp32 holds whatever the number of tokens, and y is
+// written once, rounded once.  The GEMM starts on x and W while z is still being computed.  Up to 128 tokens, where every token may have an adapter of its own, the GEMM's threads
 // add z B to its sums instead, a token's row from its own adapter, in fp32 (64 tokens of 32 adapters, rank 16:
 // as columns of the reduction 23.8 us, so 17); up to 32 tokens that follows a kernel of warp matrix
 // instructions.  8192 tokens of 8 adapters, rank 64, 2048 -> 4096: 145 us, of
@@ -47,8 +47,8 @@ struct AdapterPlan {
   int nt, splits;  // the GEMM's tile, and the blocks (a cluster) that share its reduction
 };
 
-// What the kernels hand on: z, up to kRowTokens tokens fp32 [tokens][rank], else [tokens][ceil(rank / 16)][2][16], the
-// two 16-bit terms of 16 ranks (zeros past the last); for each tile of 128 tokens its number of distinct
+// What the kernels hand on: z, up to kRowTokens tokens fp32 [tokens][rank], else [tokens][ceil(rank / 16)][3][16], the
+// three bf16 terms of 16 ranks (zeros past the last); for each tile of 128 tokens its number of distinct
 // adapters and their ids, and for each token its place among them (255: none).
 struct AdapterLists {
   float* z;
@@ -105,15 +105,28 @@ __device__ __forceinline__ void add_peers(const float* at, int parts, float (&z)
       z[7] += b.w;
     }
 }
-// the two terms of ranks r0 to r0 + 7 of a token
-template <bool BF16>
+// The three bf16 terms of ranks r0 to r0 + 7 of a token, largest first: each the nearest to what is left, and
+// the last exactly that (to 2^-133, bf16's smallest).  The first is cut off where rounding it would overflow.
+// What is not finite is the last term: of B's two terms in fp16 the second, which is 0 for most values, meets
+// only the first two.
+constexpr int kTerms = 3;
 __device__ __forceinline__ void store_terms(const AdapterLists& l, int token, int rank, int r0,
-                                            float (&z)[8]) {
-  const int64_t at = ((int64_t)token * ((rank + 15) / 16) + r0 / 16) * 32 + r0 % 16;
-  store_16b<BF16>(l.z16, at, z);
+                                            const float (&z)[8]) {
+  const float inf = __int_as_float(0x7f800000);
+  float t[kTerms][8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) z[j] = remainder_of<BF16>(z[j]);
-  store_16b<BF16>(l.z16, at + 16, z);
+  for (int j = 0; j < 8; ++j) {
+    float first = unpack2<true>(pack2<true>(z[j], 0.0f)).x;
+    if (!(fabsf(first) < inf)) first = __uint_as_float(__float_as_uint(z[j]) & 0xffff0000u);
+    if (!(fabsf(z[j]) < inf)) first = 0.0f;
+    const float rest = z[j] - first, second = unpack2<true>(pack2<true>(rest, 0.0f)).x;
+    t[0][j] = first;
+    t[1][j] = fabsf(z[j]) < inf ? second : 0.0f;
+    t[2][j] = rest - t[1][j];
+  }
+  const int64_t at = ((int64_t)token * ((rank + 15) / 16) + r0 / 16) * (16 * kTerms) + r0 % 16;
+#pragma unroll
+  for (int k = 0; k < kTerms; ++k) store_16b<true>(l.z16, at + 16 * k, t[k]);
 }
 // 8 columns of 16 bits, or zeros
 __device__ __forceinline__ uint4 load8(const uint16_t* p, bool there) {
@@ -269,7 +282,7 @@ __global__ void __launch_bounds__(256)
         for (int j = 0; j < 8; ++j) z[j] *= scale;
       }
       if (!rows) {
-        store_terms<BF16>(l, t0 + t, p.rank, r0 + r, z);
+        store_terms(l, t0 + t, p.rank, r0 + r, z);
       } else if (r0 + r < p.rank) {
         float4* to = reinterpret_cast<float4*>(l.z + (int64_t)(t0 + t) * p.rank + r0 + r);
         to[0] = make_float4(z[0], z[1], z[2], z[3]);
@@ -451,7 +464,7 @@ __global__ void __launch_bounds__(192, 1)
     const float scale = p.scaling ? p.scaling[id] : 1.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) z[j] = r < p.rank ? z[j] * scale : 0.0f;
-    store_terms<BF16>(l, mt * kABM + m, p.rank, r, z);
+    store_terms(l, mt * kABM + m, p.rank, r, z);
   }
   if (parts > 1) cluster_sync();  // (no block leaves while its sums are read)
 }
@@ -529,20 +542,23 @@ __global__ void __launch_bounds__(256)
 
 // ---- tiles ----------------------------------------------------------------------------------------------
 // Stages of 64 columns of x and W come by TMA (128-byte swizzle).  The adapters come in stages of their own,
-// 16 ranks of one adapter: z's two terms (zeros for other adapters' tokens) and B, each 16 columns (32-byte
-// swizzle), two products with one B.  Four warps write them, the next stage's loads under way while one
-// waits for its place, and they are taken in between the main stages, spread over the tile: a sum's order
-// is free.  (The first tile takes them last: z may still be on its way.)
+// 16 ranks of one adapter: z's three terms (zeros for other adapters' tokens) and B, each 16 columns (32-byte
+// swizzle), three products with one B.  fp16 B goes in as two bf16 terms (8 of its 11 bits and the rest, exact),
+// the second against z's first two: its product with the third is below 2^-26 of z B.  Four warps write the
+// stages, the next stage's loads under way while one waits for its place, and they are taken in between the main
+// stages, spread over the tile: a sum's order is free.  (The first tile takes them last: z may still be on its
+// way.)
 // A tile's tokens meet all of its adapters, all but their own times 0, and 0 times an infinity is a NaN.  So
 // eight columns of B with one that is not finite go in as zeros, and the epilogue adds them to their own
 // adapter's tokens: one request's broken adapter does not reach another's.
-template <int NT>
+template <int NT, bool BF16>
 struct AdaptedCfg {
   static constexpr int kATile = kABM * kABK * 2;
   static constexpr int kBTile = NT * kABK * 2;
   static constexpr int kStage = kATile + kBTile;
-  static constexpr int kExtra = (2 * kABM + NT) * 32;
-  static constexpr int kExtras = NT == 256 ? 2 : 4;
+  static constexpr int kZTile = kABM * 32;  // a term
+  static constexpr int kExtra = kTerms * kZTile + (BF16 ? 1 : 2) * NT * 32;
+  static constexpr int kExtras = NT == 64 ? 4 : NT == 128 || BF16 ? 3 : 2;
   static constexpr int kStages = (224 * 1024 - kExtras * kExtra) / kStage;
   static constexpr int kTmem = 2 * NT;  // two accumulators, a power of two
 };
@@ -551,15 +567,15 @@ struct AdaptedCfg {
 // epilogue of its last but one; so at most the tiles of kExtras + 1 stages, and one before them, have marks that
 // are still to be read.
 constexpr int kMarks = 8;
-template <int NT>
+template <int NT, bool BF16>
 struct AdaptedSmem {
-  static_assert(AdaptedCfg<NT>::kExtras + 2 <= kMarks, "marks are read before they are written over");
-  alignas(1024) uint8_t tiles[AdaptedCfg<NT>::kStages][AdaptedCfg<NT>::kStage];
-  alignas(1024) uint8_t extra[AdaptedCfg<NT>::kExtras][AdaptedCfg<NT>::kExtra];
-  alignas(8) uint64_t full[AdaptedCfg<NT>::kStages];
-  alignas(8) uint64_t empty[AdaptedCfg<NT>::kStages];
-  alignas(8) uint64_t extra_full[AdaptedCfg<NT>::kExtras];
-  alignas(8) uint64_t extra_empty[AdaptedCfg<NT>::kExtras];
+  static_assert(AdaptedCfg<NT, BF16>::kExtras + 2 <= kMarks, "marks are read before they are written over");
+  alignas(1024) uint8_t tiles[AdaptedCfg<NT, BF16>::kStages][AdaptedCfg<NT, BF16>::kStage];
+  alignas(1024) uint8_t extra[AdaptedCfg<NT, BF16>::kExtras][AdaptedCfg<NT, BF16>::kExtra];
+  alignas(8) uint64_t full[AdaptedCfg<NT, BF16>::kStages];
+  alignas(8) uint64_t empty[AdaptedCfg<NT, BF16>::kStages];
+  alignas(8) uint64_t extra_full[AdaptedCfg<NT, BF16>::kExtras];
+  alignas(8) uint64_t extra_empty[AdaptedCfg<NT, BF16>::kExtras];
   alignas(8) uint64_t acc_full[2];
   alignas(8) uint64_t acc_empty[2];
   alignas(8) uint64_t drain;
@@ -567,8 +583,24 @@ struct AdaptedSmem {
   int failed;
   int broken[kMarks];  // 1 + the last tile that left columns of B out
 };
-template <int NT>
-constexpr size_t adapted_smem_bytes() { return sizeof(AdaptedSmem<NT>) + 1024; }
+template <int NT, bool BF16>
+constexpr size_t adapted_smem_bytes() { return sizeof(AdaptedSmem<NT, BF16>) + 1024; }
+
+// eight fp16 values in place as bf16, and what that leaves, also bf16
+__device__ __forceinline__ void bf16_terms(uint4* at, uint4* rest) {
+  const uint4 v = *at;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t hi[4], lo[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 e = unpack2<false>(w[j]);
+    hi[j] = pack2<true>(e.x, e.y);
+    const float2 near = unpack2<true>(hi[j]);
+    lo[j] = pack2<true>(e.x - near.x, e.y - near.y);
+  }
+  *at = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+  *rest = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
 
 // Shared-memory matrix descriptor: K-major tile with 32-byte rows, 32-byte swizzle (16-byte piece j of row m
 // at piece j ^ (m / 4 % 2)); 8-row groups 256 bytes apart.
@@ -595,11 +627,11 @@ __device__ __noinline__ void add_broken(const AdaptedGemm& p, int token, int mt,
   for (int r0 = 0; r0 < rank; r0 += 8) {
     const int q = slot * width + r0 / 16;
     if (q < q0 || q >= q1) continue;
-    const uint16_t* terms = p.l.z16 + ((int64_t)token * width + r0 / 16) * 32 + r0 % 16;
+    const uint16_t* terms = p.l.z16 + ((int64_t)token * width + r0 / 16) * (16 * kTerms) + r0 % 16;
     float z[8];
 #pragma unroll
     for (int r = 0; r < 8; ++r)
-      z[r] = unpack2<BF16>(terms[r]).x + unpack2<BF16>(terms[16 + r]).x;
+      z[r] = unpack2<true>(terms[32 + r]).x + unpack2<true>(terms[16 + r]).x + unpack2<true>(terms[r]).x;
 #pragma unroll 1
     for (int j = 0; j < 32 && col + j < p.a.outer; ++j) {
       const uint16_t* b =
@@ -661,10 +693,11 @@ template <int NT, bool BF16>
 __global__ void __launch_bounds__(kAdaptedThreads, 1)
     adapted_gemm_kernel(const __grid_constant__ CUtensorMap map_x,
                         const __grid_constant__ CUtensorMap map_w, const AdaptedGemm p) {
-  using C = AdaptedCfg<NT>;
-  constexpr uint32_t kIdesc = idesc_f16(kABM, NT, BF16);
+  using C = AdaptedCfg<NT, BF16>;
+  using S = AdaptedSmem<NT, BF16>;
+  constexpr uint32_t kIdesc = idesc_f16(kABM, NT, BF16), kExtraIdesc = idesc_f16(kABM, NT, true);
   extern __shared__ uint8_t smem_raw[];
-  AdaptedSmem<NT>& sm = *reinterpret_cast<AdaptedSmem<NT>*>(
+  S& sm = *reinterpret_cast<S*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = uniform(threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -764,10 +797,17 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
           if (!ok) break;
           fence_after_sync();
           const uint32_t base = smem_addr(sm.extra[s]);
-          const uint64_t db = smem_desc_32(base + 2 * kABM * 32);
+          const uint64_t db = smem_desc_32(base + kTerms * C::kZTile);
           if (elect_one()) {
-            mma_kind_f16(acc, smem_desc_32(base), db, kIdesc, 1u);
-            mma_kind_f16(acc, smem_desc_32(base + kABM * 32), db, kIdesc, 1u);
+#pragma unroll
+            for (int k = 0; k < kTerms; ++k)
+              mma_kind_f16(acc, smem_desc_32(base + k * C::kZTile), db, kExtraIdesc, 1u);
+            if constexpr (!BF16) {
+              const uint64_t low = smem_desc_32(base + kTerms * C::kZTile + NT * 32);
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+                mma_kind_f16(acc, smem_desc_32(base + k * C::kZTile), low, kExtraIdesc, 1u);
+            }
             mma_commit(&sm.extra_empty[s]);
           }
           ++h;
@@ -858,15 +898,17 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
     bool ok = true;
     // stage j has arrived: looked over, to the other proxy (it is read by the MMA), one arrival a warp
     auto hand_over = [&](uint32_t j, int t) {
-      uint8_t* at = sm.extra[j % C::kExtras] + 2 * kABM * 32;
+      uint8_t* at = sm.extra[j % C::kExtras] + kTerms * C::kZTile;
 #pragma unroll
       for (int e = 0; e < kRows; ++e)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           if (tid + 128 * e >= NT) continue;
           uint4* v = reinterpret_cast<uint4*>(at + (tid + 128 * e) * 32 + (piece ^ (k << 4)));
-          if (not_finite<BF16>(*v)) {
-            *v = make_uint4(0, 0, 0, 0);
+          const bool broken = not_finite<BF16>(*v);
+          if (broken) *v = make_uint4(0, 0, 0, 0);
+          if constexpr (!BF16) bf16_terms(v, v + NT * 2);
+          if (broken) {
             *const_cast<volatile int*>(&sm.broken[(met - 1) % kMarks]) = t + 1;
           }
         }
@@ -881,7 +923,7 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
       met += q1 > q0;
       const int token = tl.mt * kABM + tid;
       const int place = token < tokens ? p.l.place[token] : 255;
-      const uint16_t* z = p.l.z16 + (int64_t)(token < tokens ? token : 0) * width * 32;
+      const uint16_t* z = p.l.z16 + (int64_t)(token < tokens ? token : 0) * width * (16 * kTerms);
       for (int q = q0; q < q1; ++q, ++h) {
         const int s = h % C::kExtras;
         ok = warp_wait(&sm.extra_empty[s], ((h / C::kExtras) & 1) ^ 1, failed);
@@ -893,14 +935,15 @@ __global__ void __launch_bounds__(kAdaptedThreads, 1)
         for (int k = 0; k < 2; ++k) {
           const int to = piece ^ (k << 4);
           const bool mine = place == slot;
-          copy_async16(at + tid * 32 + to, z + group * 32 + 8 * k, mine);
-          copy_async16(at + kABM * 32 + tid * 32 + to, z + group * 32 + 16 + 8 * k, mine);
+#pragma unroll
+          for (int h = 0; h < kTerms; ++h)
+            copy_async16(at + h * C::kZTile + tid * 32 + to, z + (group * kTerms + h) * 16 + 8 * k, mine);
 #pragma unroll
           for (int e = 0; e < kRows; ++e) {
             const int row = tid + 128 * e, col = tl.nt * NT + row, r0 = group * 16 + 8 * k;
             const bool there = col < outer && r0 < rank;
             if (row < NT)
-              copy_async16(at + 2 * kABM * 32 + row * 32 + to,
+              copy_async16(at + kTerms * C::kZTile + row * 32 + to,
                            static_cast<const uint16_t*>(p.a.b) +
                                (there ? ((int64_t)id * outer + col) * rank + r0 : 0),
                            there);
@@ -1016,7 +1059,7 @@ static AdapterBytes bytes_of(int64_t tokens, int rank) {
   AdapterBytes b;
   const int64_t tiles = ceil_of(tokens, kABM);
   const bool few = tokens <= kRowTokens;
-  b.z = up_256(few ? tokens * rank * 4 : tokens * ceil_of(rank, 16) * 64);
+  b.z = up_256(few ? tokens * rank * 4 : tokens * ceil_of(rank, 16) * 32 * kTerms);
   b.count = few ? 0 : up_256(tiles * 4);
   b.list = few ? 0 : up_256(tiles * 128 * 4);
   b.place = few ? 0 : up_256(tokens);
@@ -1062,7 +1105,7 @@ static cudaError_t tiles(const AdapterArgs& a, const AdapterLists& l, const Adap
   auto* kern = adapted_gemm_kernel<NT, BF16>;
   static std::mutex mu;
   static bool done[64] = {};
-  cudaError_t e = allow_smem(kern, adapted_smem_bytes<NT>(), mu, done);
+  cudaError_t e = allow_smem(kern, adapted_smem_bytes<NT, BF16>(), mu, done);
   if (e != cudaSuccess) return e;
   CUtensorMap mx, mw;
   if (!make_map(&mx, a.x, a.tokens, a.inner, kABM, dt) ||
@@ -1080,7 +1123,7 @@ static cudaError_t tiles(const AdapterArgs& a, const AdapterLists& l, const Adap
   const int64_t all = (int64_t)p.m_tiles * p.n_tiles * p.splits;
   const int64_t sms = sm_count() > 0 ? sm_count() : all;
   return launch_clusters(kern, dim3((unsigned)(all < sms || p.splits > 1 || p.rows ? all : sms)),
-                         dim3(kAdaptedThreads), adapted_smem_bytes<NT>(), s, p.splits, mx, mw, p);
+                         dim3(kAdaptedThreads), adapted_smem_bytes<NT, BF16>(), s, p.splits, mx, mw, p);
 }
 
 template <bool BF16>

@@ -387,9 +387,8 @@ EXF_API int exf_balance_loss_backward(const float* dloss, const void* logits, in
  *   y_t = x_t W^T + scaling_i (x_t A_i^T) B_i^T, i = ids[t]; tokens whose id lies outside [0, adapters)
  * have none.  x [tokens][inner], w [outer][inner], a [adapters][rank][inner], b [adapters][outer][rank]
  * and y [tokens][outer] of dtype (EXF_BF16 or EXF_F16), ids in any order, scaling fp32 [adapters] or NULL
- * (1).  Sums are fp32 and y is rounded once; above 128 tokens the sums z = scaling_i x_t A_i^T are held as
- * two terms of dtype (bf16: 2^-16 of z; fp16: 2^-22, 2^-25 at least, and z above 65504 overflows).  inner,
- * outer and rank multiples of 8, rank up to 128; tensors 16-byte aligned, the workspace
+ * (1).  Sums are fp32, z = scaling_i x_t A_i^T among them, and y is rounded once.  inner, outer and rank
+ * multiples of 8, rank up to 128; tensors 16-byte aligned, the workspace
  * (exf_adapted_linear_workspace_bytes(); -1: a shape that the call refuses) 32-byte.
  * status as in exf_fused_experts. */
 EXF_API int64_t exf_adapted_linear_workspace_bytes(int64_t tokens, int inner, int outer, int rank);
