@@ -276,8 +276,8 @@ __global__ void __launch_bounds__(256)
       if (id < 0 || id >= p.adapters || r0 + r >= (p.rank + 15) / 16 * 16) continue;
       float z[8];
       add_peers(&joined[t][r], parts, z);
-      if (p.scaling) {
-        const float scale = p.scaling[id];
+      if (p.scaling) {  // (past the rank z stays 0, whatever the factor)
+        const float scale = r0 + r < p.rank ? p.scaling[id] : 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) z[j] *= scale;
       }

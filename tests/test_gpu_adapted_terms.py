@@ -105,3 +105,21 @@ def test_one_token_far_above_the_others(tokens):
     want = torch.zeros(tokens, 40, device=DEV)
     want[:, ::2] = (x[:, :1].float() * 100.0) * 2.0 ** -10
     assert torch.equal(y, want.to(F16))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rank", [8, 16, 24, 40, 128])
+@pytest.mark.parametrize("tokens", TOKENS)
+def test_infinite_factor(tokens, rank, dtype):
+    """x, A and B above 0 and an infinite factor of one adapter: its tokens are infinite, none is a NaN."""
+    x = torch.full((tokens, 24), 0.5, dtype=dtype, device=DEV)
+    a = torch.full((2, rank, 24), 0.25, dtype=dtype, device=DEV)
+    b = torch.full((2, 136, rank), 1.5, dtype=dtype, device=DEV)
+    w = torch.ones(136, 24, dtype=dtype, device=DEV)
+    ids = (torch.arange(tokens, device=DEV) % 3 - 1).int()
+    y = ops.adapted_linear(x, w, a, b, ids,
+                           scaling=torch.tensor([float("inf"), 2.0], device=DEV)).float()
+    assert bool((y[ids == 0] == float("inf")).all())
+    assert bool((y[ids == -1] == 12.0).all())
+    want = torch.tensor(12.0 + 9.0 * rank).to(dtype).item()  # (a rank adds 2 x 24 x 0.125 x 1.5)
+    assert bool((y[ids == 1] == want).all())
