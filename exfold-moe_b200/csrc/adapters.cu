@@ -31,11 +31,12 @@ using namespace tc;
 // The tokens up to which a form is taken; us of this form and of the next, 2048 -> 4096 bf16.
 // The kernel without tiles (it holds no more): 16 tokens of 32 adapters, rank 16: 7.3 and 15.4; 32: 11.2, 14.7.
 constexpr int kFewAdapted = 32;
-// Adapters added row by row, z in fp32: 65 tokens of 32 adapters, rank 16: 17.5 and 22.7; 128: 25.6, 25.8, of 8
-// adapters, rank 64: 38, 32; 256: 32.5, 32.4, in 4 runs of rank 64: 39.6, 24.6.
+// Adapters added row by row, z in fp32: 65 tokens of 32 adapters, rank 16: 17.4 and 22.4; 128: 25.7, 25.8, of 8
+// adapters, rank 64: 38, 33, of 64: 42, 74; 256 of 32, rank 16: 32.7, 33.7, of 64, rank 64: 55, 127, in 4 runs of rank
+// 64: 41, 27.
 constexpr int kRowTokens = 128;
-// z by adapter_down_kernel: 512 tokens of 32 adapters, rank 16: 48 and 77; 1024: 73, 95, in 4 runs of rank 64: 34,
-// 32; 2048: 53.5, 49.
+// z by adapter_down_kernel: 512 tokens of 32 adapters, rank 16: 50 and 78; 1024: 73, 96, in 4 runs of rank 64: 40,
+// 39; 2048: 127, 165, in 8 runs of rank 64: 61, 59.
 constexpr int kDownTokens = 1024;
 constexpr int kAdaptedThreads = 320;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue, warps 6-9 adapters
 constexpr int kABM = 128;           // tokens of a tile
@@ -558,7 +559,9 @@ struct AdaptedCfg {
   static constexpr int kStage = kATile + kBTile;
   static constexpr int kZTile = kABM * 32;  // a term
   static constexpr int kExtra = kTerms * kZTile + (BF16 ? 1 : 2) * NT * 32;
-  static constexpr int kExtras = NT == 64 ? 4 : NT == 128 || BF16 ? 3 : 2;
+  // (three in fp16 at 128 columns would leave adapter_down_kernel's blocks no room beside this kernel's: 65 tokens
+  // 17.4 -> 21.5 us)
+  static constexpr int kExtras = NT == 64 ? 4 : BF16 ? 3 : 2;
   static constexpr int kStages = (224 * 1024 - kExtras * kExtra) / kStage;
   static constexpr int kTmem = 2 * NT;  // two accumulators, a power of two
 };
