@@ -85,11 +85,17 @@ int code_of(const Tensor& t) {
   return t.scalar_type() == at::kFloat ? EXF_F32 : t.scalar_type() == at::kBFloat16 ? EXF_BF16 : EXF_F16;
 }
 
+// (a tensor without memory, a wrapper's, would be a null pointer: an optional one that was not given)
+void require_cuda(const Tensor& t) {
+  TORCH_CHECK(t.is_cuda(), "ExFold B200 ops require CUDA tensors");
+  TORCH_CHECK_VALUE(t.numel() == 0 || t.const_data_ptr() != nullptr,
+                    "ExFold B200 ops require tensors with memory of their own");
+}
 void require_cuda(const Tensor& first, std::initializer_list<const Tensor*> others) {
-  TORCH_CHECK(first.is_cuda(), "ExFold B200 ops require CUDA tensors");
+  require_cuda(first);
   for (const Tensor* t : others)
     if (t) {
-      TORCH_CHECK(t->is_cuda(), "ExFold B200 ops require CUDA tensors");
+      require_cuda(*t);
       TORCH_CHECK(t->device() == first.device(),
                   "ExFold B200 ops require all tensors on one device");
     }
