@@ -534,6 +534,7 @@ PyObject* py_rms_norm_8bit(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const OptTensor residual = maybe_tensor(a[3]);
     const at::ScalarType dtype = dtype_of(a[4]);
     const int64_t group = integer_of(a[5]);
+    no_tangent("rms_norm_8bit", {&x, &weight, get(residual)});
     return unlocked([&] { return rms_norm_8bit(x, weight, eps, residual, dtype, group); });
   });
 }
@@ -543,6 +544,7 @@ PyObject* py_dequantize_8bit(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor &codes = tensor_of(a[0]), &scales = tensor_of(a[1]);
     const int64_t group = integer_of(a[2]);
     const at::ScalarType dtype = dtype_of(a[3]);
+    no_tangent("dequantize_8bit", {&scales});
     return unlocked([&] { return dequantize_8bit(codes, scales, group, dtype); });
   });
 }
@@ -562,6 +564,7 @@ PyObject* py_adapted_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor &x = tensor_of(a[0]), &w = tensor_of(a[1]), &down = tensor_of(a[2]),
                  &up = tensor_of(a[3]), &ids = tensor_of(a[4]);
     const OptTensor scaling = maybe_tensor(a[5]), status = maybe_tensor(a[6]);
+    no_tangent("adapted_linear", {&x, &w, &down, &up, get(scaling)});
     return unlocked([&] { return adapted_linear(x, w, down, up, ids, scaling, status); });
   });
 }

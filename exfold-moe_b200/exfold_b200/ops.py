@@ -655,7 +655,7 @@ def rms_norm_8bit(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     group of 32, 64 or 128 columns, or [..., 1] for the row (group None).  A group's largest value has
     the largest code (448, or 127); the others are rounded to the nearest, ties to even.  Values are
     code * scale (`dequantize_8bit`).  A group with a value that is not finite reads back as NaN.  H up to
-    2^17.  For inference: the result carries no gradient.
+    2^17.  For inference: the results, s among them, carry no gradient; forward mode is refused.
     """
     return L.torch_ops().rms_norm_8bit(x, weight, eps, residual, dtype, _group(group))
 
@@ -667,7 +667,8 @@ def _group(group: int | None) -> int:
 
 def dequantize_8bit(codes: torch.Tensor, scales: torch.Tensor, group: int | None = 128,
                     dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values code * scale of `rms_norm_8bit`'s codes and scales, rounded to dtype."""
+    """The values code * scale of `rms_norm_8bit`'s codes and scales, rounded to dtype.  For inference: the
+    result carries no gradient; forward mode is refused."""
     return L.torch_ops().dequantize_8bit(codes, scales, _group(group), dtype)
 
 
@@ -701,6 +702,6 @@ def adapted_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.T
     and b [R, N, rank], all bf16 or all fp16; y [..., N].  adapter_ids [...] integers of any width, in any
     order; tokens whose id lies outside [0, R) have no adapter.  scaling fp32 [R], or None for 1.  K, N
     and rank are multiples of 8, rank at most 128.  Sums are fp32; y is rounded once.  `status` as in
-    `fused_experts`.  For inference: the result carries no gradient.
+    `fused_experts`.  For inference: the result carries no gradient; forward mode is refused.
     """
     return L.torch_ops().adapted_linear(x, w, a, b, adapter_ids, scaling, status)

@@ -1,9 +1,11 @@
-"""What the norm, the balance loss and the projection with adapters refuse of a tensor: one without memory."""
+"""What the norm, the balance loss and the projection with adapters refuse of a tensor: one without memory, a dual
+tensor; and which of their results carry no gradient."""
 
 from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from exfold_b200 import ops
 
@@ -73,3 +75,26 @@ def test_subclasses_with_memory_are_taken(which):
     for i in range(len(args)):
         got = as_tuple(f(*args[:i], args[i].as_subclass(Subclass), *args[i + 1:]))
         assert len(got) == len(want) and all(torch.equal(g, v) for g, v in zip(got, want))
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_tangents_are_refused(which):
+    f, args = calls()[which]
+    real = [i for i, t in enumerate(args) if t.dtype in (BF16, torch.float32)]
+    assert real
+    with forward_ad.dual_level():
+        f(*args)
+        for i in real:
+            dual = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f(*args[:i], dual, *args[i + 1:])
+
+
+@pytest.mark.parametrize("which", [1, 2, 4])
+def test_operators_for_inference_carry_no_gradient(which):
+    f, args = calls()[which]
+    for i, t in enumerate(args):
+        if t.dtype in (BF16, torch.float32):
+            v = t.clone().requires_grad_()
+            got = f(*args[:i], v, *args[i + 1:])
+            assert not any(g.requires_grad for g in (got if isinstance(got, tuple) else (got,)))
