@@ -385,6 +385,8 @@ variable_list balance_loss(const Tensor& logits, const Tensor& topk_ids, int64_t
   TORCH_CHECK_VALUE(!m || (m->scalar_type() == at::kBool &&
                            m->sizes() == logits.sizes().slice(0, logits.dim() - 1)),
                     "mask must be bool ", logits.sizes().slice(0, logits.dim() - 1));
+  TORCH_CHECK_NOT_IMPLEMENTED(topk_ids.size(-1) < (int64_t(1) << 31),
+                              "exf_balance_loss: a group's routes must be below 2^31");
   Tensor ids = topk_ids;
   // (narrow and unsigned ids in 64 bits: what lies outside [0, E) stays outside)
   if (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) ids = ids.to(at::kLong);

@@ -1,5 +1,5 @@
 """What the norm, the balance loss and the projection with adapters refuse of a tensor: one without memory, a dual
-tensor; and which of their results carry no gradient."""
+tensor, more routes than are counted; and which of their results carry no gradient."""
 
 from __future__ import annotations
 
@@ -98,3 +98,10 @@ def test_operators_for_inference_carry_no_gradient(which):
             v = t.clone().requires_grad_()
             got = f(*args[:i], v, *args[i + 1:])
             assert not any(g.requires_grad for g in (got if isinstance(got, tuple) else (got,)))
+
+
+def test_more_routes_than_32_bits_count():
+    """2^32 + 8 routes of one token are not 8."""
+    ids = torch.zeros(1, 1, dtype=torch.int32, device=DEV).expand(1, 2 ** 32 + 8)
+    with pytest.raises(NotImplementedError, match="routes"):
+        ops.balance_loss(torch.zeros(1, 16, device=DEV), ids)
