@@ -6,7 +6,9 @@
 //   scale = top v / M, so that code scale is the norm's s_j v w_j
 //
 // v is the same for the row, so the codes do not depend on its rounding: equal inputs give the codes of the
-// definition (products of fp32 values with fp32 weights to 2^-53).  A group with a product that is not
+// definition (products of fp32 values with fp32 weights to 2^-48).  Products are held in fp32, those with fp32
+// values or weights as two fp32 terms: exact, but that what lies below fp32's smallest value, 2^-149, is rounded
+// to it, in a group's largest as in its other products.  A group with a product that is not
 // finite in fp32 gets codes 0 and a NaN scale, a group of zeros codes 0 and scale 0.
 //
 // Bound by memory (x, residual in, sum and codes out, once each) and, beside it, by the instructions of the
@@ -20,9 +22,9 @@
 namespace exf {
 
 // ---- the largest product of a group ----------------------------------------------------------------
-// Products of 16-bit values are exact in fp32 (EXACT): the value.  Others: an integer that compares as the
-// magnitudes do, the rounded product's bits and, below them, what the rounding left, its order made that of
-// unsigned integers.  Infinities and NaN come out above all.
+// Products of 16-bit values are exact in fp32 (EXACT; to 2^-149): the value.  Others: an integer that compares
+// as the magnitudes do, the rounded product's bits and, below them, what the rounding left (to 2^-149), its order
+// made that of unsigned integers.  Infinities and NaN come out above all.
 template <bool EXACT>
 struct Top;
 template <>
@@ -125,7 +127,9 @@ __device__ __noinline__ uint8_t code_64(const T* x, const T* r, const W* w, doub
   float s[1];
   load_sum<T, 1>(x, r, s);
   const float f = to_f32<W>(*w), m = INT8 ? 127.0f : 448.0f;
-  const double p = fabs((double)s[0] * (double)f) * (double)m;
+  // (as the group's largest is held, so that no product is above it)
+  using K = Top<sizeof(T) == 2 && sizeof(W) == 2>;
+  const double p = K::value(K::of(s[0], f, s[0] * f)) * (double)m;
   float c;
   if (top > 0x1p-100 && top < 0x1p100) {
     // the border beside the quotient, and the side of it on which p lies

@@ -337,7 +337,8 @@ EXF_API int exf_gated_mlp_backward(const void* dh, const float* pre, const void*
  * exf_rms_norm_8bit: the norm as 8-bit codes [rows][cols] and scales fp32 [rows][ceil(cols / group)],
  * group 32, 64 or 128 columns, or 0 for the row.  With p_j = s_j weight_j and a group's largest |p| = top,
  * a code is p_j M / top rounded to the nearest e4m3 value (EXF_E4M3, M = 448) or integer (EXF_I8, M =
- * 127), ties to even, and the scale is top / (M sqrt(mean s^2 + eps)).  A group of zeros has scale 0; one
+ * 127), ties to even, and the scale is top / (M sqrt(mean s^2 + eps)).  Products are exact but for what lies
+ * below 2^-149, fp32's smallest value.  A group of zeros has scale 0 (NaN in a row of zeros with eps 0); one
  * with a product that is not finite in fp32 has codes 0 and a NaN scale.  cols up to 2^17.
  * exf_dequantize_8bit: code * scale, rounded to dtype; codes and out 16-byte aligned.
  * exf_rms_norm_backward: from dy and dsum (the upstream gradient of s; may be NULL), both contiguous, and x
