@@ -7,12 +7,16 @@ no fast-math, --fmad=false so every float operation is the one written) into
 exfold-moe_b200/_build/, then linked into exfold-moe_b200/lib/libexfold_b200.so with the CUDA
 runtime linked statically.  Objects are rebuilt only when a source or header is newer.
 binding/torch_ops.cpp (host code: autograd nodes over the C ABI) is compiled by g++ against the
-installed torch into the Python module lib/libexfold_b200_torch.so.
+installed torch into the Python module lib/libexfold_b200_torch.so, and again when torch or Python change
+(lib/libexfold_b200_torch.txt says what it was built for).  The library needs neither torch nor g++: without
+them it is built alone.
 """
 
 from __future__ import annotations
 
 import argparse
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -28,6 +32,7 @@ OBJ = PKG / "_build"
 LIB = PKG / "lib" / "libexfold_b200.so"
 TORCH_SRC = PKG / "binding" / "torch_ops.cpp"
 TORCH_LIB = PKG / "lib" / "libexfold_b200_torch.so"
+TORCH_BUILT = TORCH_LIB.with_suffix(".txt")  # what the binding was built for
 INCLUDE = ROOT / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -68,6 +73,35 @@ def torch_command() -> list[str]:
             "-lc10_cuda", "-ldl", f"-Wl,-rpath,{libs}"]
 
 
+def torch_built() -> str | None:
+    """What a binding built here is for (exfold_b200._lib compares it); None where none can be built."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or spec.origin is None or shutil.which("g++") is None:
+        return None
+    if not (Path(spec.origin).parent / "lib" / "libtorch_cuda.so").exists():
+        return None
+    version = importlib.metadata.version("torch")
+    return f"torch {version}, Python {sys.version_info.major}.{sys.version_info.minor}"
+
+
+def build_binding(force: bool, run) -> None:
+    built = torch_built()
+    if built is None:
+        print("no torch with CUDA, or no g++: the torch binding is not built, the library is", flush=True)
+        return
+    if not (force or _stale(TORCH_LIB, [TORCH_SRC, *INCLUDE.glob("*.h")]) or
+            not TORCH_BUILT.exists() or TORCH_BUILT.read_text().strip() != built):
+        return
+    run(torch_command())
+    # (a compiler that links its own libstdc++ into the binding would make exceptions of two kinds)
+    if "libstdc++.so" not in subprocess.run(["ldd", str(TORCH_LIB)], capture_output=True,
+                                            text=True).stdout:
+        TORCH_LIB.unlink()
+        raise RuntimeError("the torch binding was not linked against the shared libstdc++: use a g++ "
+                           "that does")
+    TORCH_BUILT.write_text(built + "\n")
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
     OBJ.mkdir(parents=True, exist_ok=True)
     LIB.parent.mkdir(parents=True, exist_ok=True)
@@ -82,8 +116,6 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
             if ptxas_info:
                 cmd += ["-Xptxas", "-v"]
             jobs.append(cmd)
-    if force or _stale(TORCH_LIB, [TORCH_SRC, *INCLUDE.glob("*.h")]):
-        jobs.append(torch_command())
 
     def run(cmd):
         if verbose:
@@ -95,17 +127,13 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
             sys.stdout.write(res.stdout + res.stderr)
         return res
 
-    with ThreadPoolExecutor(max_workers=max(1, min(len(jobs), os.cpu_count() or 1))) as ex:
-        list(ex.map(run, jobs))
-    # (a compiler that links its own libstdc++ into the binding would make exceptions of two kinds)
-    if "libstdc++.so" not in subprocess.run(["ldd", str(TORCH_LIB)], capture_output=True,
-                                            text=True).stdout:
-        TORCH_LIB.unlink()
-        raise RuntimeError("the torch binding was not linked against the shared libstdc++: use a g++ "
-                           "that does")
     objs = [OBJ / (s.stem + ".o") for s in sources]
-    if force or _stale(LIB, objs):
-        run([nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", str(LIB), *map(str, objs)])
+    with ThreadPoolExecutor(max_workers=max(1, min(len(jobs) + 1, os.cpu_count() or 1))) as ex:
+        binding = ex.submit(build_binding, force, run)
+        list(ex.map(run, jobs))
+        if force or _stale(LIB, objs):
+            run([nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", str(LIB), *map(str, objs)])
+        binding.result()
     return LIB
 
 

@@ -11,6 +11,7 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import os
+import sys
 import threading
 from pathlib import Path
 
@@ -126,11 +127,12 @@ _torch_ops = None
 
 
 def torch_ops():
-    """The module libexfold_b200_torch.so, beside the library (RuntimeError if it has not been built)."""
+    """The module libexfold_b200_torch.so, beside the library (RuntimeError if it has not been built, or was built
+    for another torch or Python)."""
     global _torch_ops
     if _torch_ops is None:
         lib()
-        import torch  # noqa: F401 (the module's libraries)
+        import torch  # (the module's libraries, too)
 
         with _lock:
             if _torch_ops is None:
@@ -138,6 +140,12 @@ def torch_ops():
                 if not path.is_file():
                     raise RuntimeError(f"ExFold B200 torch binding is missing: {path} "
                                        "(build it with: python exfold-moe_b200/build.py)")
+                built = path.with_suffix(".txt")
+                here = (f"torch {torch.__version__}, Python {sys.version_info.major}."
+                        f"{sys.version_info.minor}")
+                if built.is_file() and built.read_text().strip() != here:
+                    raise RuntimeError(f"ExFold B200 torch binding was built for {built.read_text().strip()}, "
+                                       f"here is {here} (build it with: python exfold-moe_b200/build.py)")
                 name = path.name.split(".")[0]
                 loader = importlib.machinery.ExtensionFileLoader(name, str(path))
                 module = importlib.util.module_from_spec(
