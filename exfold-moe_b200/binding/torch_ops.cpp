@@ -86,10 +86,13 @@ int code_of(const Tensor& t) {
 }
 
 // (a tensor without memory, a wrapper's, would be a null pointer: an optional one that was not given)
-void require_cuda(const Tensor& t) {
-  TORCH_CHECK(t.is_cuda(), "ExFold B200 ops require CUDA tensors");
+void require_memory(const Tensor& t) {
   TORCH_CHECK_VALUE(t.numel() == 0 || t.const_data_ptr() != nullptr,
                     "ExFold B200 ops require tensors with memory of their own");
+}
+void require_cuda(const Tensor& t) {
+  TORCH_CHECK(t.is_cuda(), "ExFold B200 ops require CUDA tensors");
+  require_memory(t);
 }
 void require_cuda(const Tensor& first, std::initializer_list<const Tensor*> others) {
   require_cuda(first);
@@ -224,6 +227,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     // (of s alone, where y was not used)
     const Tensor dy = grads[0].defined() ? grads[0].contiguous() : at::zeros(shape, x.options());
     const Tensor ds = residual && grads[1].defined() ? grads[1].contiguous() : Tensor();
+    if (ds.defined()) require_memory(ds);
     const int64_t need = want_w ? api.norm_workspace(rows.n, cols) : 0;
     if (need > 0) ws = bytes(need, x);
     check(api.norm_backward(dy.data_ptr(), pointer(ds), rows.t.data_ptr(), rows.stride,

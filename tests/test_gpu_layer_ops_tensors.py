@@ -105,3 +105,13 @@ def test_more_routes_than_32_bits_count():
     ids = torch.zeros(1, 1, dtype=torch.int32, device=DEV).expand(1, 2 ** 32 + 8)
     with pytest.raises(NotImplementedError, match="routes"):
         ops.balance_loss(torch.zeros(1, 16, device=DEV), ids)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_upstream_gradients_without_memory_are_refused(which):
+    x = torch.randn(6, 64, device=DEV).to(BF16).requires_grad_()
+    y, s = ops.rms_norm(x, torch.ones(64, dtype=BF16, device=DEV), residual=torch.ones_like(x))
+    up = [torch.ones_like(y), torch.ones_like(s)]
+    up[which] = Wrapper(up[which])
+    with pytest.raises((ValueError, RuntimeError)):
+        torch.autograd.grad((y, s), x, up)
