@@ -12,8 +12,8 @@
 // over the blocks, in a fixed order.
 //
 // The logits are read once forward; backward reads them again and writes the gradient.  131072 x 128 fp32,
-// top-8: forward 26.0 us (71 MB; bound by instructions, about 30 a logit with the exponential, its correction,
-// the sums and the route counts, and by a block's start and end), backward 23.9 (134 MB, 0.86 of a copy's rate).
+// top-8: forward 26.0 us (71 MB; 29 instructions executed a logit, at 0.59 of the issue slots: a warp's few steps
+// wait for one another, and for a block's start and end), backward 23.9 (134 MB, 0.86 of a copy's rate).
 // A token lies on a few lanes of a warp (about 16 columns a lane), so that a warp takes several at a time
 // and a row's two reductions are a few shuffles; a lane keeps its columns, and adds them in registers.
 #include "exf_balance.h"

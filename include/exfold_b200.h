@@ -333,7 +333,8 @@ EXF_API int exf_gated_mlp_backward(const void* dh, const float* pre, const void*
  * x, residual: [rows][cols] of dtype (EXF_F32, EXF_BF16 or EXF_F16), rows x_stride and r_stride elements
  * apart; weight [cols] fp32 or of dtype; sum (s; required with a residual, else unused) and y contiguous,
  * neither overlapping an input.  Any number of columns and any alignment of the type (rows on 16-byte
- * boundaries are read as vectors).  Sums are fp32; a sum of squares outside fp32's range is taken in 64 bits.
+ * boundaries are read as vectors).  Sums are fp32; a sum of squares outside fp32's range is taken in 64 bits
+ * (the inverse norm is fp32: with eps 0, a row whose root mean square is below 2^-128 overflows it).
  * exf_rms_norm_8bit: the norm as 8-bit codes [rows][cols] and scales fp32 [rows][ceil(cols / group)],
  * group 32, 64 or 128 columns, or 0 for the row.  With p_j = s_j weight_j and a group's largest |p| = top,
  * a code is p_j M / top rounded to the nearest e4m3 value (EXF_E4M3, M = 448) or integer (EXF_I8, M =
