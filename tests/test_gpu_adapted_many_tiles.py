@@ -80,3 +80,56 @@ def test_wholly_broken_adapter(rank, value):
         y = ops.adapted_linear(x, w, a, broken, ids)
         assert not bool(y[own].isfinite().any())
         assert torch.equal(y[~own], ops.adapted_linear(x, w, a, b, ids)[~own])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("tokens,inner,outer,rank", [
+    (1100, 264, 520, 16), (2500, 1024, 2048, 24), (8192, 520, 2056, 64), (4200, 256, 264, 128)])
+def test_broken_rows_of_a_and_x(tokens, inner, outer, rank, dtype):
+    """A NaN or an infinity of an adapter's A reaches its own tokens alone; one of a token's x that token."""
+    x, w, a, b = inputs(tokens, inner, outer, 3, rank, dtype, tokens)
+    for pattern in ([0, 1, 2], [1, -1, 0, 2, 2]):
+        ids = adapters_of(tokens, pattern)
+        ids[7::10] = 1
+        want = ops.adapted_linear(x, w, a, b, ids)
+        for value in ("nan", "inf"):
+            broken = a.clone()
+            broken[1, rank - 1, inner - 3] = float(value)
+            broken[1, 0, 2] = float(value)
+            y = ops.adapted_linear(x, w, broken, b, ids)
+            assert not bool(y[ids == 1].isfinite().any())
+            assert torch.equal(y[ids != 1], want[ids != 1])
+            z = x.clone()
+            z[tokens // 2, 5] = float(value)
+            y = ops.adapted_linear(z, w, a, b, ids)
+            assert not bool(y[tokens // 2].isfinite().any())
+            others = torch.arange(tokens, device=DEV) != tokens // 2
+            assert torch.equal(y[others], want[others])
+
+
+@pytest.mark.parametrize("tokens", [129, 1100, 2500])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_graphs_and_streams(tokens, dtype):
+    args = [inputs(tokens, 520, 4104, 6, 40, dtype, seed) for seed in (1, 2)]
+    ids = [adapters_of(tokens, p) for p in ([0, 5, -1, 2], [3, 3, 1])]
+    want = [ops.adapted_linear(*v, i) for v, i in zip(args, ids)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(10):  # two calls at once
+        with torch.cuda.stream(side):
+            other = ops.adapted_linear(*args[1], ids[1])
+        here = ops.adapted_linear(*args[0], ids[0])
+        torch.cuda.synchronize()
+        assert torch.equal(here, want[0]) and torch.equal(other, want[1])
+    graph = torch.cuda.CUDAGraph()
+    who = ids[0].clone()
+    with torch.cuda.graph(graph):
+        y = ops.adapted_linear(*args[0], who)
+        z = ops.adapted_linear(*args[1], who)
+    for i in (ids[0], ids[1], ids[0]):
+        who.copy_(i)
+        y.zero_()
+        z.zero_()
+        graph.replay()
+        assert torch.equal(y, ops.adapted_linear(*args[0], i))
+        assert torch.equal(z, ops.adapted_linear(*args[1], i))
